@@ -256,6 +256,74 @@ int convnd_hip_timing_enable(int enable);
  * launches of kernel `kernel` since the previous read; clears that record. */
 int convnd_hip_timing_read(int kernel, double* total_ms, int64_t* launches);
 
+/* ---- Sequence operators --------------------------------------------------------------------
+ * Layer norm, linear layer and gated recurrence of token sequences around the convolution. No
+ * counterpart in the reference. Types float32, float16 and bfloat16 (anything else returns
+ * CONVND_HIP_INVALID_ARGUMENT); strides are in elements; statistics, states and sums are float32.
+ * The gradients asked for are overwritten, not added to. */
+
+/* output = (input - mean) * rstd * weight + bias for rows of `channels` contiguous elements,
+ * `input_stride` apart in the input, contiguous in the output; mean and the variance are over a
+ * row, rstd = 1 / sqrt(variance + eps). weight and bias [channels] of `param_dtype` (the input's
+ * dtype or float32), null for ones and zeros. mean, rstd [rows]: written for the backward pass,
+ * or both null. */
+int convnd_hip_layer_norm(convnd_hip_dtype dtype, convnd_hip_dtype param_dtype, const void* input,
+                          int64_t input_stride, const void* weight, const void* bias, void* output,
+                          float* mean, float* rstd, int64_t rows, int64_t channels, double eps,
+                          void* stream);
+
+/* Device scratch bytes that convnd_hip_layer_norm_backward needs for parameter gradients. */
+size_t convnd_hip_layer_norm_backward_workspace_size(convnd_hip_dtype dtype, int64_t rows,
+                                                     int64_t channels);
+
+/* Gradients of convnd_hip_layer_norm for a cotangent grad_output (rows `grad_stride` apart) from
+ * the statistics it wrote. grad_input [rows, channels], grad_weight and grad_bias [channels] of
+ * `param_dtype`; a null one is skipped. */
+int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype param_dtype,
+                                   const void* grad_output, int64_t grad_stride, const void* input,
+                                   int64_t input_stride, const void* weight, const float* mean,
+                                   const float* rstd, void* grad_input, void* grad_weight,
+                                   void* grad_bias, int64_t rows, int64_t channels,
+                                   void* workspace, size_t workspace_size, void* stream);
+
+/* Gated linear recurrence over the token axis,
+ *   h[t] = a[t] h[t-1] + (1 - a[t]) input[t],  a[t] = sigmoid(gate[t]),  h[-1] = first,
+ * for input and gate [batch, tokens, channels] with contiguous channels and the batch and token
+ * strides given. */
+typedef struct convnd_hip_recurrence_problem {
+  int64_t batch, tokens, channels;
+  int64_t input_batch, input_token; /* strides of input */
+  int64_t gate_batch, gate_token;   /* strides of gate */
+  int wide_lengths;                 /* lengths are int64 (nonzero) or int32 */
+} convnd_hip_recurrence_problem;
+
+/* Number of states per sequence that the forward saves for the backward: carries is
+ * [batch, this, channels]. */
+int64_t convnd_hip_recurrence_carries(int64_t tokens);
+
+/* Device scratch bytes of the two calls below (often 0). */
+size_t convnd_hip_recurrence_workspace_size(convnd_hip_dtype dtype,
+                                            const convnd_hip_recurrence_problem* problem, int backward);
+
+/* output [batch, tokens, channels] = h; last [batch, channels] float32 = the state after the last
+ * token. first [batch, channels] float32, null for zeros. lengths [batch], null for `tokens`:
+ * tokens at and past a sequence's length (taken as 0 below 0 and as `tokens` above) change no
+ * state and give zeros, whatever input and gate hold there. carries: saved states, or null. */
+int convnd_hip_recurrence(convnd_hip_dtype dtype, const convnd_hip_recurrence_problem* problem,
+                          const void* input, const void* gate, const float* first,
+                          const void* lengths, void* output, float* last, float* carries,
+                          void* workspace, size_t workspace_size, void* stream);
+
+/* Its gradients for the cotangents grad_output [batch, tokens, channels] (contiguous) and
+ * grad_last [batch, channels] float32 (null for zeros). grad_input and grad_gate contiguous;
+ * grad_first [batch, channels] float32, or null. */
+int convnd_hip_recurrence_backward(convnd_hip_dtype dtype, const convnd_hip_recurrence_problem* problem,
+                                   const void* grad_output, const float* grad_last,
+                                   const void* input, const void* gate, const void* lengths,
+                                   const float* carries, void* grad_input, void* grad_gate,
+                                   float* grad_first, void* workspace, size_t workspace_size,
+                                   void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

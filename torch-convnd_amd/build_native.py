@@ -36,6 +36,9 @@ HIP_SOURCES = (
     "convnd_partial.hip",
     "convnd_static.hip",
     "convnd_tiny.hip",
+    "convnd_norm.hip",
+    "convnd_recurrence.hip",
+    "convnd_sequence_capi.cpp",
     "convnd_capi.cpp",
 )
 OFFLOAD_ARCH = os.environ.get("TORCH_CONVND_OFFLOAD_ARCH", "gfx950")
@@ -124,6 +127,7 @@ def build_ops_library(verbose: bool = False) -> Path:
         f"-I{rocm_home() / 'include'}",
         f"-I{INCLUDE}",
         str(CSRC / "torch_ops.cpp"),
+        str(CSRC / "torch_sequence_ops.cpp"),
         str(CSRC / "convnd_cpu.cpp"),
         "-fopenmp",
         "-o",

@@ -30,21 +30,32 @@ namespace {
 
 thread_local std::string g_error;
 
+constexpr int64_t kI64Max = std::numeric_limits<int64_t>::max();
+constexpr int64_t kI32Safe = (int64_t{1} << 31) - 1;
+// LDS per workgroup on gfx950 is 160 KiB; keep a margin for the compiler's own use.
+constexpr int64_t kLdsBudget = 160 * 1024 - 1024;
+
+}  // namespace
+
 int fail(int status, const std::string& message) {
   g_error = message;
   return status;
 }
 
-constexpr int64_t kI64Max = std::numeric_limits<int64_t>::max();
-constexpr int64_t kI32Safe = (int64_t{1} << 31) - 1;
-// LDS per workgroup on gfx950 is 160 KiB; keep a margin for the compiler's own use.
-constexpr int64_t kLdsBudget = 160 * 1024 - 1024;
+int hip_check(hipError_t err, const char* what) {
+  if (err == hipSuccess) return CONVND_HIP_SUCCESS;
+  return fail(CONVND_HIP_LAUNCH_FAILED,
+              std::string(what) + " failed: " + hipGetErrorString(err));
+}
 
 bool mul_ok(int64_t a, int64_t b, int64_t* out) {
   if (a < 0 || b < 0 || (b != 0 && a > kI64Max / b)) return false;
   *out = a * b;
   return true;
 }
+
+namespace {
+
 bool add_ok(int64_t a, int64_t b, int64_t* out) {
   if (a < 0 || b < 0 || a > kI64Max - b) return false;
   *out = a + b;
@@ -2140,12 +2151,6 @@ std::pair<hipEvent_t, hipEvent_t> timing_begin(int kernel, hipStream_t stream) {
 
 void timing_end(const std::pair<hipEvent_t, hipEvent_t>& ev, hipStream_t stream) {
   if (ev.second != nullptr) (void)hipEventRecord(ev.second, stream);
-}
-
-int hip_check(hipError_t err, const char* what) {
-  if (err == hipSuccess) return CONVND_HIP_SUCCESS;
-  return fail(CONVND_HIP_LAUNCH_FAILED,
-              std::string(what) + " failed: " + hipGetErrorString(err));
 }
 
 int prepare(const convnd_hip_problem* problem, convnd_hip_dtype dtype, Geom* g) {

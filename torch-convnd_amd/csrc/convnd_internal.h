@@ -531,6 +531,71 @@ hipError_t launch_partial_rescale(convnd_hip_dtype dtype, const PartialRescaleAr
                                   const void* raw, const void* counts, const void* bias,
                                   void* out, hipStream_t stream);
 
+// Records a failure's message for convnd_hip_last_error and returns the status.
+int fail(int status, const std::string& message);
+int hip_check(hipError_t err, const char* what);
+// a * b into *out, or false where that is negative or passes int64.
+bool mul_ok(int64_t a, int64_t b, int64_t* out);
+
+// Layer norm (convnd_norm.hip): rows of `channels` contiguous elements; strides in elements.
+struct NormArgs {
+  const void* input;
+  const void* weight;       // or null: ones
+  const void* bias;         // or null: zeros
+  const void* grad_output;  // backward
+  void* output;             // [rows, channels]
+  void* grad_input;         // [rows, channels] or null
+  float* mean;              // [rows]; null in a forward that keeps no statistics
+  float* rstd;
+  float* partial;           // [blocks][2][channels]: sums of dw and db, or null
+  int64_t rows, channels, input_stride, grad_stride;
+  float eps;
+};
+struct NormPlan {
+  int threads_per_row;  // 0: the kernels for rows too long for registers
+  int runs;             // 16-byte runs per thread
+  int64_t blocks;
+};
+NormPlan plan_norm(int64_t rows, int64_t channels, int element_size, bool backward);
+hipError_t launch_norm(convnd_hip_dtype dtype, bool float_params, const NormArgs& a, bool backward,
+                       const NormPlan& p, hipStream_t stream);
+hipError_t launch_norm_reduce(convnd_hip_dtype param_dtype, const float* partial, int64_t rows,
+                              int64_t channels, void* dw, void* db, hipStream_t stream);
+
+// Gated linear recurrence (convnd_recurrence.hip); strides in elements, channels contiguous.
+struct RecurrenceArgs {
+  const void* input;          // [batch, tokens, channels] by batch and token strides
+  const void* gate;
+  const void* grad_output;    // backward
+  const float* first;         // [batch, channels] or null: zeros
+  const void* lengths;        // [batch] int32 or int64, or null: all `tokens`
+  const float* grad_last;     // [batch, channels] or null: zeros
+  void* output;               // [batch, tokens, channels]
+  float* last;                // [batch, channels]
+  float* carries;             // [batch, tiles, channels]: the state before each tile, or null
+  void* grad_input;           // [batch, tokens, channels]
+  void* grad_gate;
+  float* grad_first;          // [batch, channels] or null
+  float* summary;             // [batch, splits, 2, channels] where splits > 1
+  int64_t batch, tokens, channels;
+  int64_t input_batch, input_token, gate_batch, gate_token, grad_batch, grad_token;
+  int64_t split_tokens;       // tokens of one split (whole tiles)
+  int splits;
+  int wide_lengths;           // lengths are int64
+};
+struct RecurrencePlan {
+  int waves;              // of a workgroup: 1 or 8
+  int channels_per_lane;  // 1 or 2
+  int splits;
+  int64_t split_tokens;
+};
+// Tokens of one tile, the distance of the saved states: fixed, so that a backward pass may be
+// planned differently from its forward.
+constexpr int kRecurrenceTile = 128;
+RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward);
+hipError_t launch_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward,
+                             const RecurrencePlan& p, hipStream_t stream);
+
 // db[c] = sum of the nsum partial sums of channel c (fixed order).
 hipError_t launch_grad_bias_from_sums(convnd_hip_dtype dtype, const float* sums, int64_t nsum,
                                       int64_t channels, void* db, hipStream_t stream);

@@ -24,6 +24,7 @@ from .modules import (
     PartialSequential,
 )
 from .partial import PartialConvOutput, partial_conv_nd
+from .sequence import gated_recurrence, layer_norm
 
 ensure_native_definitions()
 ensure_compatible_operator()
@@ -42,6 +43,8 @@ __all__ = [
     "PartialConvOutput",
     "PartialSequential",
     "conv_nd",
+    "gated_recurrence",
+    "layer_norm",
     "partial_conv_nd",
     "load_native",
     "get_runtime_info",

@@ -200,6 +200,38 @@ def _rescale_backward(ctx, grad):
     return grad_raw, None, grad_bias, None
 
 
+def _fake_layer_norm(input, weight, bias, eps, keep_statistics):
+    rows = input.numel() // input.shape[-1] if keep_statistics else 0
+    output = torch.empty_like(input, memory_format=torch.contiguous_format)
+    return output, input.new_empty((2, rows), dtype=torch.float32)
+
+
+def _fake_layer_norm_backward(grad_output, input, weight, bias, statistics, output_mask):
+    dx = torch.empty_like(input, memory_format=torch.contiguous_format) if output_mask[0] else None
+    dw = weight.new_empty(weight.shape) if output_mask[1] and weight is not None else None
+    db = bias.new_empty(bias.shape) if output_mask[2] and bias is not None else None
+    return dx, dw, db
+
+
+def _fake_recurrence(input, gate, initial_state, lengths, keep_carries):
+    batch, tokens, channels = input.shape
+    tiles = (tokens + RECURRENCE_TILE - 1) // RECURRENCE_TILE
+    output = torch.empty_like(input, memory_format=torch.contiguous_format)
+    last = input.new_empty((batch, channels), dtype=torch.float32)
+    carries = input.new_empty((batch if keep_carries else 0, tiles, channels), dtype=torch.float32)
+    return output, last, carries
+
+
+def _fake_recurrence_backward(grad_output, grad_last, input, gate, lengths, carries, need_initial_state):
+    dx = torch.empty_like(input, memory_format=torch.contiguous_format)
+    dg = torch.empty_like(gate, memory_format=torch.contiguous_format)
+    shape = (input.shape[0], input.shape[2])
+    return dx, dg, input.new_empty(shape, dtype=torch.float32) if need_initial_state else None
+
+
+# Tokens between the states that gated_recurrence saves (convnd_hip_recurrence_carries).
+RECURRENCE_TILE = 128
+
 _PY_AUTOGRAD = None
 
 
@@ -220,6 +252,10 @@ def register_training() -> None:
     torch.library.register_fake("torch_convnd::partial_rescale")(_fake_rescale)
     torch.library.register_fake("torch_convnd::partial_count")(_fake_count)
     torch.library.register_fake("torch_convnd::conv_nd_act")(_fake_act)
+    torch.library.register_fake("torch_convnd::layer_norm")(_fake_layer_norm)
+    torch.library.register_fake("torch_convnd::layer_norm_backward")(_fake_layer_norm_backward)
+    torch.library.register_fake("torch_convnd::gated_recurrence")(_fake_recurrence)
+    torch.library.register_fake("torch_convnd::gated_recurrence_backward")(_fake_recurrence_backward)
     torch.library.register_autograd(
         "torch_convnd::partial_rescale", _rescale_backward, setup_context=_setup_rescale
     )

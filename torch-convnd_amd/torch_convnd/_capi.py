@@ -33,6 +33,13 @@ EXPORTED_SYMBOLS = (
     "convnd_hip_backward_workspace_size_layout",
     "convnd_hip_forward_layout",
     "convnd_hip_backward_layout",
+    "convnd_hip_layer_norm",
+    "convnd_hip_layer_norm_backward_workspace_size",
+    "convnd_hip_layer_norm_backward",
+    "convnd_hip_recurrence_carries",
+    "convnd_hip_recurrence_workspace_size",
+    "convnd_hip_recurrence",
+    "convnd_hip_recurrence_backward",
 )
 
 CHANNELS_FIRST, CHANNELS_LAST, CHANNELS_LAST_INPUT = 0, 1, 2
@@ -68,6 +75,15 @@ class Problem(ctypes.Structure):
             p.input[a], p.kernel[a] = x_shape[a + 2], w_shape[a + 2]
             p.stride[a], p.padding[a], p.dilation[a] = stride[a], padding[a], dilation[a]
         return p
+
+
+class RecurrenceProblem(ctypes.Structure):
+    """struct convnd_hip_recurrence_problem."""
+
+    _fields_ = [
+        (name, ctypes.c_int64)
+        for name in ("batch", "tokens", "channels", "input_batch", "input_token", "gate_batch", "gate_token")
+    ] + [("wide_lengths", ctypes.c_int)]
 
 
 def bind(library: ctypes.CDLL) -> ctypes.CDLL:
@@ -115,6 +131,27 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     library.convnd_hip_partial_rescale.restype = ctypes.c_int
     library.convnd_hip_partial_rescale.argtypes = [
         ctypes.c_int, vp, vp, vp, vp, i64, i64, i64, i64, i64, ctypes.c_double, vp
+    ]
+    R, dbl = ctypes.POINTER(RecurrenceProblem), ctypes.c_double
+    library.convnd_hip_layer_norm.restype = ctypes.c_int
+    library.convnd_hip_layer_norm.argtypes = [
+        ctypes.c_int, ctypes.c_int, vp, i64, vp, vp, vp, vp, vp, i64, i64, dbl, vp
+    ]
+    library.convnd_hip_layer_norm_backward_workspace_size.restype = sz
+    library.convnd_hip_layer_norm_backward_workspace_size.argtypes = [ctypes.c_int, i64, i64]
+    library.convnd_hip_layer_norm_backward.restype = ctypes.c_int
+    library.convnd_hip_layer_norm_backward.argtypes = [
+        ctypes.c_int, ctypes.c_int, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, vp, sz, vp
+    ]
+    library.convnd_hip_recurrence_carries.restype = i64
+    library.convnd_hip_recurrence_carries.argtypes = [i64]
+    library.convnd_hip_recurrence_workspace_size.restype = sz
+    library.convnd_hip_recurrence_workspace_size.argtypes = [ctypes.c_int, R, ctypes.c_int]
+    library.convnd_hip_recurrence.restype = ctypes.c_int
+    library.convnd_hip_recurrence.argtypes = [ctypes.c_int, R, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    library.convnd_hip_recurrence_backward.restype = ctypes.c_int
+    library.convnd_hip_recurrence_backward.argtypes = [
+        ctypes.c_int, R, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp
     ]
     return library
 

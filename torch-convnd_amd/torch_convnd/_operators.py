@@ -74,6 +74,31 @@ def _lazy_rescale(raw, counts, bias, window):
     return torch.ops.torch_convnd.partial_rescale.default(raw, counts, bias, window)
 
 
+def _lazy(name, position=0):
+    """A kernel that loads the native library and calls the operator again (its own kernels then
+    take precedence); the tensor at ``position`` says for which device."""
+
+    def load_and_call(*args):
+        _load_for(args[position])
+        return getattr(torch.ops.torch_convnd, name).default(*args)
+
+    return load_and_call
+
+
+# Sequence operators (layer norm, gated recurrence); no reference counterpart. The second
+# results of the forwards are what their backward operators read, kept only on request.
+_SEQUENCE_SCHEMAS = (
+    "layer_norm(Tensor input, Tensor? weight, Tensor? bias, float eps, bool keep_statistics) "
+    "-> (Tensor, Tensor)",
+    "layer_norm_backward(Tensor grad_output, Tensor input, Tensor? weight, Tensor? bias, "
+    "Tensor statistics, bool[3] output_mask) -> (Tensor?, Tensor?, Tensor?)",
+    "gated_recurrence(Tensor input, Tensor gate, Tensor? initial_state, Tensor? lengths, "
+    "bool keep_carries) -> (Tensor, Tensor, Tensor)",
+    "gated_recurrence_backward(Tensor grad_output, Tensor? grad_last, Tensor input, Tensor gate, "
+    "Tensor? lengths, Tensor carries, bool need_initial_state) -> (Tensor, Tensor, Tensor?)",
+)
+
+
 def ensure_native_definitions():
     """Define the schemas once per process (idempotent, thread-safe)."""
     global _LIBRARY
@@ -121,6 +146,10 @@ def ensure_native_definitions():
             "partial_count(Tensor mask, int[] kernel, int[] stride, int[] padding, "
             "int[] dilation, int count_channels) -> Tensor"
         )
+        for schema in _SEQUENCE_SCHEMAS:
+            name = schema.split("(")[0]
+            library.define(schema)
+            library.impl(name, _lazy(name), "CompositeExplicitAutograd")
         library.impl("conv_nd", _lazy_forward, "CompositeExplicitAutograd")
         library.impl("conv_nd_backward", _lazy_backward, "CompositeExplicitAutograd")
         if HAS_NATIVE_AUTOGRAD:
