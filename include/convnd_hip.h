@@ -289,7 +289,7 @@ int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype para
 /* Gated linear recurrence over the token axis,
  *   h[t] = a[t] h[t-1] + (1 - a[t]) input[t],  a[t] = sigmoid(gate[t]),  h[-1] = first,
  * for input and gate [batch, tokens, channels] with contiguous channels and the batch and token
- * strides given. */
+ * strides given (token strides of at least `channels`, below 2^21). */
 typedef struct convnd_hip_recurrence_problem {
   int64_t batch, tokens, channels;
   int64_t input_batch, input_token; /* strides of input */
@@ -303,7 +303,7 @@ int64_t convnd_hip_recurrence_carries(int64_t tokens);
 
 /* Device scratch bytes of the two calls below (often 0). */
 size_t convnd_hip_recurrence_workspace_size(convnd_hip_dtype dtype,
-                                            const convnd_hip_recurrence_problem* problem, int backward);
+                                            const convnd_hip_recurrence_problem* problem);
 
 /* output [batch, tokens, channels] = h; last [batch, channels] float32 = the state after the last
  * token. first [batch, channels] float32, null for zeros. lengths [batch], null for `tokens`:

@@ -586,13 +586,14 @@ struct RecurrenceArgs {
 struct RecurrencePlan {
   int waves;              // of a workgroup: 1 or 8
   int channels_per_lane;  // 1 or 2
+  int lanes;              // of a wave along the channels: 64, 32 or 16
   int splits;
   int64_t split_tokens;
 };
-// Tokens of one tile, the distance of the saved states: fixed, so that a backward pass may be
-// planned differently from its forward.
-constexpr int kRecurrenceTile = 128;
-RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward);
+// Distance of the saved states in tokens: every plan's tiles start at whole multiples of it (or
+// are a single one).
+constexpr int kRecurrenceTile = 64;
+RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a);
 hipError_t launch_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward,
                              const RecurrencePlan& p, hipStream_t stream);
 

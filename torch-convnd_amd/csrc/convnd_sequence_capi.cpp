@@ -41,6 +41,8 @@ int64_t norm_partials(int64_t rows, int64_t channels, convnd_hip_dtype dtype) {
   return plan_norm(rows, channels, size_of(dtype), true).blocks * 2 * channels;
 }
 
+constexpr int64_t kMaxTokenStride = int64_t{1} << 21;
+
 int check_recurrence(convnd_hip_dtype dtype, const convnd_hip_recurrence_problem* r) {
   if (size_of(dtype) == 0)
     return fail(CONVND_HIP_INVALID_ARGUMENT, std::string("gated_recurrence ") + kTypes);
@@ -53,9 +55,16 @@ int check_recurrence(convnd_hip_dtype dtype, const convnd_hip_recurrence_problem
     if (step < 0 || !mul_ok(step, std::max(r->batch, r->tokens), &extent))
       return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence strides overflow int64");
   if (!mul_ok(r->batch, r->tokens, &rows) || !mul_ok(rows, r->channels, &total) ||
-      !mul_ok(r->batch, r->channels, &total) || total >= (int64_t{1} << 37) ||
-      r->channels >= (int64_t{1} << 30))
-    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence sizes are too large");
+      !mul_ok(r->batch, r->channels, &total))
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence sizes overflow int64");
+  // A lane's place in a tile of up to 256 tokens is a 32-bit byte offset.
+  if (r->input_token < r->channels || r->gate_token < r->channels)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_recurrence needs tokens at least their channels apart");
+  if (r->channels >= kMaxTokenStride || r->input_token >= kMaxTokenStride ||
+      r->gate_token >= kMaxTokenStride)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_recurrence needs channels and token strides below 2^21 elements");
   return CONVND_HIP_SUCCESS;
 }
 
@@ -79,9 +88,9 @@ int64_t summary_floats(const RecurrenceArgs& a, const RecurrencePlan& p) {
 }
 
 // Plans the call into `a` and checks the workspace and the size of the grid.
-int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, bool backward, void* workspace,
-              size_t workspace_size, RecurrencePlan* p) {
-  *p = plan_recurrence(dtype, *a, backward);
+int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, void* workspace, size_t workspace_size,
+              RecurrencePlan* p) {
+  *p = plan_recurrence(dtype, *a);
   a->splits = p->splits;
   a->split_tokens = p->split_tokens;
   const int64_t floats = summary_floats(*a, *p);
@@ -90,7 +99,7 @@ int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, bool backward, void* wo
                 "gated_recurrence needs a workspace of " + std::to_string(floats * sizeof(float)) +
                     " bytes");
   a->summary = static_cast<float*>(workspace);
-  const int64_t strips = (a->channels + 63) / 64;
+  const int64_t strips = (a->channels + 15) / 16;
   if (strips * p->splits * a->batch > std::numeric_limits<int32_t>::max())
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence sizes are too large");
   return CONVND_HIP_SUCCESS;
@@ -187,10 +196,10 @@ int64_t convnd_hip_recurrence_carries(int64_t tokens) {
 }
 
 size_t convnd_hip_recurrence_workspace_size(convnd_hip_dtype dtype,
-                                            const convnd_hip_recurrence_problem* problem, int backward) {
+                                            const convnd_hip_recurrence_problem* problem) {
   if (check_recurrence(dtype, problem) != CONVND_HIP_SUCCESS) return 0;
   const RecurrenceArgs a = to_args(*problem);
-  return static_cast<size_t>(summary_floats(a, plan_recurrence(dtype, a, backward != 0))) *
+  return static_cast<size_t>(summary_floats(a, plan_recurrence(dtype, a))) *
          sizeof(float);
 }
 
@@ -213,7 +222,7 @@ int convnd_hip_recurrence(convnd_hip_dtype dtype, const convnd_hip_recurrence_pr
   a.last = last;
   a.carries = carries;
   RecurrencePlan p;
-  st = plan_call(dtype, &a, false, workspace, workspace_size, &p);
+  st = plan_call(dtype, &a, workspace, workspace_size, &p);
   if (st != CONVND_HIP_SUCCESS) return st;
   return hip_check(launch_recurrence(dtype, a, false, p, static_cast<hipStream_t>(stream)),
                    "gated recurrence launch");
@@ -243,7 +252,7 @@ int convnd_hip_recurrence_backward(convnd_hip_dtype dtype, const convnd_hip_recu
   a.grad_gate = grad_gate;
   a.grad_first = grad_first;
   RecurrencePlan p;
-  st = plan_call(dtype, &a, true, workspace, workspace_size, &p);
+  st = plan_call(dtype, &a, workspace, workspace_size, &p);
   if (st != CONVND_HIP_SUCCESS) return st;
   return hip_check(launch_recurrence(dtype, a, true, p, static_cast<hipStream_t>(stream)),
                    "gated recurrence backward launch");

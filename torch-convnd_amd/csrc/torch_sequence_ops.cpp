@@ -187,6 +187,7 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
     ctx->save_for_backward({input, weight.value_or(at::Tensor()), bias.value_or(at::Tensor()),
                             statistics});
     ctx->mark_non_differentiable({statistics});
+    ctx->set_materialize_grads(false);
     return {output, statistics};
   }
 
@@ -197,6 +198,8 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
       return t.defined() ? OptionalTensor(t) : std::nullopt;
     };
     if (!grads[0].defined()) return variable_list(4);
+    // Refused above where it would be differentiated, so no autograd kernel is needed below.
+    at::AutoDispatchBelowADInplaceOrView below;
     // Needed edges are counted over the tensors that were given.
     int edge = 0;
     std::array<bool, 3> mask{};
@@ -248,8 +251,14 @@ void check_state(const OptionalTensor& state, const at::Tensor& input, const cha
               "gated_recurrence ", name, " must be float32 of [batch, channels] on the input's device");
 }
 
+// The tensor itself where its channels are contiguous and its tokens neither overlap nor lie too
+// far apart for the kernels' offsets, else a contiguous copy.
 at::Tensor token_rows(const at::Tensor& t) {
-  return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous();
+  const bool direct = (t.stride(2) == 1 || t.size(2) == 1) && t.stride(1) >= t.size(2) &&
+                      t.stride(1) < (int64_t{1} << 21);
+  if (direct) return t;
+  // A single token's stride may be anything, a copy's too.
+  return t.size(1) == 1 ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
 }
 
 convnd_hip_recurrence_problem recurrence_problem(const at::Tensor& x, const at::Tensor& g,
@@ -266,9 +275,8 @@ convnd_hip_recurrence_problem recurrence_problem(const at::Tensor& x, const at::
   return p;
 }
 
-at::Tensor recurrence_workspace(const convnd_hip_recurrence_problem& p, const at::Tensor& input,
-                                bool backward) {
-  const size_t bytes = convnd_hip_recurrence_workspace_size(sequence_dtype(input), &p, backward);
+at::Tensor recurrence_workspace(const convnd_hip_recurrence_problem& p, const at::Tensor& input) {
+  const size_t bytes = convnd_hip_recurrence_workspace_size(sequence_dtype(input), &p);
   if (bytes == 0) return at::Tensor();
   return at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte));
 }
@@ -287,7 +295,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_recurrence_device(
   auto last = at::empty({p.batch, p.channels}, single);
   auto carries = at::empty(
       {keep_carries ? p.batch : 0, convnd_hip_recurrence_carries(p.tokens), p.channels}, single);
-  auto workspace = recurrence_workspace(p, input, false);
+  auto workspace = recurrence_workspace(p, input);
   check_status(convnd_hip_recurrence(
       sequence_dtype(input), &p, x.const_data_ptr(), g.const_data_ptr(),
       f.has_value() ? f->const_data_ptr<float>() : nullptr, data_or_null(n),
@@ -321,7 +329,7 @@ std::tuple<at::Tensor, at::Tensor, OptionalTensor> gated_recurrence_backward_dev
   auto dg = at::empty(input.sizes(), input.options());
   OptionalTensor df;
   if (need_first) df = at::empty({p.batch, p.channels}, input.options().dtype(at::kFloat));
-  auto workspace = recurrence_workspace(p, input, true);
+  auto workspace = recurrence_workspace(p, input);
   check_status(convnd_hip_recurrence_backward(
       sequence_dtype(input), &p, dy.const_data_ptr(),
       dl.has_value() ? dl->const_data_ptr<float>() : nullptr, x.const_data_ptr(),
@@ -362,6 +370,7 @@ class RecurrenceFunction : public torch::autograd::Function<RecurrenceFunction> 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_once("gated_recurrence");
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
+    at::AutoDispatchBelowADInplaceOrView below;
     const auto saved = ctx->get_saved_variables();
     const auto optional = [](const at::Tensor& t) {
       return t.defined() ? OptionalTensor(t) : std::nullopt;

@@ -230,7 +230,7 @@ def _fake_recurrence_backward(grad_output, grad_last, input, gate, lengths, carr
 
 
 # Tokens between the states that gated_recurrence saves (convnd_hip_recurrence_carries).
-RECURRENCE_TILE = 128
+RECURRENCE_TILE = 64
 
 _PY_AUTOGRAD = None
 

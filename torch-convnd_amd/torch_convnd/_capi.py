@@ -146,7 +146,7 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     library.convnd_hip_recurrence_carries.restype = i64
     library.convnd_hip_recurrence_carries.argtypes = [i64]
     library.convnd_hip_recurrence_workspace_size.restype = sz
-    library.convnd_hip_recurrence_workspace_size.argtypes = [ctypes.c_int, R, ctypes.c_int]
+    library.convnd_hip_recurrence_workspace_size.argtypes = [ctypes.c_int, R]
     library.convnd_hip_recurrence.restype = ctypes.c_int
     library.convnd_hip_recurrence.argtypes = [ctypes.c_int, R, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     library.convnd_hip_recurrence_backward.restype = ctypes.c_int

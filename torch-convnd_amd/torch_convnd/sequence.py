@@ -22,6 +22,15 @@ _NATIVE_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 def _use_native(input, backend, name):
     """Whether a call runs on the gfx950 kernels; loads them, or raises where they cannot."""
+    if (
+        _build._LOADED
+        and input.is_cuda
+        and input.dtype in _NATIVE_DTYPES
+        and (backend == "auto" or backend == "native")
+        and not transforms_active()
+        and torch._C._get_tracing_state() is None
+    ):
+        return True
     device = input.device
     if backend not in BACKENDS:
         raise ValueError(f"Invalid backend {backend!r}; expected 'auto', 'native' or 'torch'")
