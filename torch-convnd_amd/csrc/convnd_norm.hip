@@ -13,14 +13,17 @@
 // workgroups' sums go to a [workgroups, channels] buffer that a second launch adds in a fixed order.
 // Rows of more channels than 1024 threads hold run on kernels that read the row three times.
 
+#include <algorithm>
+
 #include "convnd_internal.h"
 #include "convnd_sequence.h"
 
 namespace convnd {
 namespace {
 
+// Threads of a workgroup: one row above a wave's width, else four waves of rows.
 template <int TPR>
-constexpr int norm_threads = TPR > 256 ? TPR : 256;
+constexpr int norm_threads = TPR > 64 ? TPR : 256;
 
 // Sum over the TPR threads of a row; `slot` alternates between calls so that one barrier each is
 // enough (a slot is written again only after the barrier of the call between).
@@ -398,13 +401,11 @@ hipError_t launch_norm_typed(const NormArgs& a, bool backward, const NormPlan& p
     case 16 * 16 + 1: return launch_rows<T, W, 16, 1>(a, backward, p.blocks, stream);
     case 32 * 16 + 1: return launch_rows<T, W, 32, 1>(a, backward, p.blocks, stream);
     case 64 * 16 + 1: return launch_rows<T, W, 64, 1>(a, backward, p.blocks, stream);
-    case 64 * 16 + 2: return launch_rows<T, W, 64, 2>(a, backward, p.blocks, stream);
-    case 64 * 16 + 4: return launch_rows<T, W, 64, 4>(a, backward, p.blocks, stream);
+    case 128 * 16 + 1: return launch_rows<T, W, 128, 1>(a, backward, p.blocks, stream);
     case 256 * 16 + 1: return launch_rows<T, W, 256, 1>(a, backward, p.blocks, stream);
-    case 256 * 16 + 2: return launch_rows<T, W, 256, 2>(a, backward, p.blocks, stream);
-    case 256 * 16 + 4: return launch_rows<T, W, 256, 4>(a, backward, p.blocks, stream);
+    case 512 * 16 + 1: return launch_rows<T, W, 512, 1>(a, backward, p.blocks, stream);
+    case 1024 * 16 + 1: return launch_rows<T, W, 1024, 1>(a, backward, p.blocks, stream);
     case 1024 * 16 + 2: return launch_rows<T, W, 1024, 2>(a, backward, p.blocks, stream);
-    case 1024 * 16 + 4: return launch_rows<T, W, 1024, 4>(a, backward, p.blocks, stream);
     default: return hipErrorInvalidValue;
   }
 }
@@ -414,31 +415,27 @@ hipError_t launch_norm_typed(const NormArgs& a, bool backward, const NormPlan& p
 NormPlan plan_norm(int64_t rows, int64_t channels, int element_size, bool backward) {
   const int64_t runs = (channels + 16 / element_size - 1) / (16 / element_size);
   NormPlan p{};
-  if (runs <= 8) {
+  // One run a thread: the backward's sums and next row are many registers, and a row over more
+  // waves beats more runs a thread (65536 x 2048 fp16: forward 133 / backward 379 us with 64
+  // threads of four runs, 110 / 227 with 128 of two, 99 / 179 with 256 of one).
+  if (runs <= 1024) {
     p.threads_per_row = 8, p.runs = 1;
-  } else if (runs <= 16) {
-    p.threads_per_row = 16, p.runs = 1;
-  } else if (runs <= 32) {
-    p.threads_per_row = 32, p.runs = 1;
-  } else if (runs <= 64) {
-    p.threads_per_row = 64, p.runs = 1;
-  } else if (rows <= 1024 && runs <= 1024) {
-    // Few rows: four waves to a row rather than four rows to a workgroup.
-    p.threads_per_row = 256, p.runs = runs <= 256 ? 1 : (runs <= 512 ? 2 : 4);
-  } else if (runs <= 256) {
-    p.threads_per_row = 64, p.runs = runs <= 128 ? 2 : 4;
-  } else if (runs <= 1024) {
-    p.threads_per_row = 256, p.runs = runs <= 512 ? 2 : 4;
-  } else if (runs <= 4096) {
-    p.threads_per_row = 1024, p.runs = runs <= 2048 ? 2 : 4;
+    while (p.threads_per_row < runs) p.threads_per_row *= 2;
+  } else if (runs <= 2048) {
+    p.threads_per_row = 1024, p.runs = 2;
   }
-  const int threads = p.threads_per_row == 0 || p.threads_per_row > 256 ? 1024 : 256;
-  const int per_block = p.threads_per_row == 0 ? 1 : threads / p.threads_per_row;
-  // The forward's rows are independent: enough workgroups to fill the chip, each keeping its
-  // parameters for several rows. The backward's workgroups each leave a row of sums.
-  const int64_t most = threads == 1024 ? 512 : (backward ? 1024 : 2048);
+  const int threads = p.threads_per_row == 0 ? 1024 : (p.threads_per_row > 64 ? p.threads_per_row : 256);
+  const int per_block = p.threads_per_row == 0 ? 1 : threads / std::min(threads, p.threads_per_row);
   const int64_t needed = (rows + per_block - 1) / per_block;
-  p.blocks = needed < most ? needed : most;
+  // The forward fills the chip with rows in flight (32 waves a compute unit: 99 us above, 131 with
+  // 16). Every workgroup of the backward leaves a row of sums to be added up: 16 waves a compute unit
+  // (179 us; 191 with 32), and several rows each (5003 x 769 fp32: 512 workgroups 16 us, 2048 19).
+  if (backward) {
+    const int64_t most = std::min<int64_t>(262144 / threads, std::max<int64_t>(256, rows / 8));
+    p.blocks = std::min(needed, most);
+  } else {
+    p.blocks = std::min<int64_t>(needed, 524288 / threads);
+  }
   return p;
 }
 
