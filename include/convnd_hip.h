@@ -286,6 +286,47 @@ int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype para
                                    void* grad_bias, int64_t rows, int64_t channels,
                                    void* workspace, size_t workspace_size, void* stream);
 
+/* Linear layer over rows of features, output = act(input weight^T + bias) + residual. */
+typedef struct convnd_hip_linear_problem {
+  int64_t rows, inputs, outputs; /* inputs, outputs below 2^21, rows below 2^31 */
+  int64_t input_stride;          /* of the rows of input, at least `inputs`, below 2^21 */
+  int64_t residual_stride;       /* of residual */
+  int64_t grad_stride;           /* of grad_output (backward), at least `outputs` */
+  int activation;                /* convnd_hip_activation */
+} convnd_hip_linear_problem;
+
+/* Device scratch bytes of convnd_hip_linear; of the pointers only the alignment is looked at (rows
+ * that do not start on 16 bytes are copied). */
+size_t convnd_hip_linear_workspace_size(convnd_hip_dtype dtype,
+                                        const convnd_hip_linear_problem* problem,
+                                        const void* input, const void* weight);
+
+/* input [rows, inputs] by its stride, weight [outputs, inputs], bias [outputs] or null, residual
+ * [rows, outputs] by its stride or null, output [rows, outputs]. Products are summed in float32;
+ * bias, activation and residual are applied in float32 before the one rounding. pre [rows, outputs],
+ * or null: the sum before the activation, for the backward. */
+int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                      const void* input, const void* weight, const void* bias,
+                      const void* residual, void* output, void* pre, void* workspace,
+                      size_t workspace_size, void* stream);
+
+size_t convnd_hip_linear_backward_workspace_size(convnd_hip_dtype dtype,
+                                                 const convnd_hip_linear_problem* problem,
+                                                 const void* grad_output, const void* input,
+                                                 const void* weight, int need_grad_input,
+                                                 int need_grad_weight, int need_grad_bias);
+
+/* Gradients for the cotangent grad_output [rows, outputs] by its stride; pre is what the forward
+ * left (not read without an activation). A null grad_input [rows, inputs], grad_weight [outputs,
+ * inputs] or grad_bias [outputs] is skipped; the residual's gradient is grad_output itself. The
+ * cotangent before the activation, grad_output * act'(pre), is rounded to the element type, which
+ * the matrix cores multiply. */
+int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                               const void* grad_output, const void* input, const void* weight,
+                               const void* pre, void* grad_input, void* grad_weight,
+                               void* grad_bias, void* workspace, size_t workspace_size,
+                               void* stream);
+
 /* Gated linear recurrence over the token axis,
  *   h[t] = a[t] h[t-1] + (1 - a[t]) input[t],  a[t] = sigmoid(gate[t]),  h[-1] = first,
  * for input and gate [batch, tokens, channels] with contiguous channels and the batch and token

@@ -112,3 +112,63 @@ def recurrence_reference(x, gate, first=None, lengths=None, dy=None, dlast=None)
         out[name] = tuple(torch.where(live, stack([p[i] for p in parts]), 0) for i in range(2))
     out["dfirst"] = (back, noise)
     return out
+
+
+def activation_reference(z, kind):
+    """act(z) and act'(z) in float64."""
+    if kind is None:
+        return z, torch.ones_like(z)
+    if kind == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if kind == "gelu":
+        phi = 0.5 * (1 + torch.erf(z / 2**0.5))
+        return z * phi, phi + z * torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5
+    c = (2 / torch.pi) ** 0.5
+    t = torch.tanh(c * (z + 0.044715 * z**3))
+    return 0.5 * z * (1 + t), 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+
+
+def linear_reference(x, w, b, residual, kind, dy=None):
+    """{name: (value, noise)} of y and, with dy, dx, dw, db in float64 (on the CPU).
+
+    Sums of n products in any order: n roundings of the magnitudes' sum. The activations and their
+    slopes vary by at most 1.13 of their argument's error (1.2 for a slope); their own evaluation
+    adds 16 roundings of |z| + 1. The backward's z and dz are rounded to the element type, and relu's
+    slope may be either side of the step where z is within its error of zero.
+    """
+    dtype = x.dtype
+    f = lambda t: None if t is None else t.detach().double().cpu()  # noqa: E731
+    x, w, b, r = f(x).reshape(-1, x.shape[-1]), f(w), f(b), f(residual)
+    z = x @ w.T
+    size = x.abs() @ w.abs().T
+    if b is not None:
+        z, size = z + b, size + b.abs()
+    z_noise = EPS32 * (x.shape[1] + 8) * size
+    y, slope = activation_reference(z, kind)
+    y_noise = z_noise
+    if kind is not None:
+        y_noise = 1.13 * z_noise + 16 * EPS32 * (z.abs() + 1)
+    if r is not None:
+        r = r.reshape(y.shape)
+        y_noise = y_noise + 2 * EPS32 * (y.abs() + r.abs())
+        y = y + r
+    out = {"y": (y, y_noise)}
+    if dy is None:
+        return out
+    g = f(dy).reshape(y.shape)
+    dz = g * slope
+    if kind is None:
+        dz_noise = torch.zeros_like(dz)
+    else:
+        z_error = z_noise + ROUND[dtype] * (z.abs() + z_noise) + TINY[dtype]
+        slope_noise = 1.2 * z_error + 16 * EPS32 * (z.abs() + 1)
+        if kind == "relu":
+            slope_noise = (z.abs() <= z_error).double()
+        dz_noise = g.abs() * slope_noise
+        dz_noise = dz_noise + ROUND[dtype] * (dz.abs() + dz_noise) + TINY[dtype]
+    dz_size = dz.abs() + dz_noise
+    rows, outputs = dz.shape
+    out["dx"] = (dz @ w, dz_noise @ w.abs() + EPS32 * (outputs + 8) * (dz_size @ w.abs()))
+    out["dw"] = (dz.T @ x, dz_noise.T @ x.abs() + EPS32 * (rows + 8) * (dz_size.T @ x.abs()))
+    out["db"] = (dz.sum(0), dz_noise.sum(0) + EPS32 * (rows + 8) * dz_size.sum(0))
+    return out

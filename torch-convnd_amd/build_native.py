@@ -37,6 +37,7 @@ HIP_SOURCES = (
     "convnd_static.hip",
     "convnd_tiny.hip",
     "convnd_norm.hip",
+    "convnd_linear.hip",
     "convnd_recurrence.hip",
     "convnd_sequence_capi.cpp",
     "convnd_capi.cpp",

@@ -559,8 +559,51 @@ struct NormPlan {
 NormPlan plan_norm(int64_t rows, int64_t channels, int element_size, bool backward);
 hipError_t launch_norm(convnd_hip_dtype dtype, bool float_params, const NormArgs& a, bool backward,
                        const NormPlan& p, hipStream_t stream);
-hipError_t launch_norm_reduce(convnd_hip_dtype param_dtype, const float* partial, int64_t rows,
-                              int64_t channels, void* dw, void* db, hipStream_t stream);
+// dw[c] (and with pitch > channels db[c], its sums `channels` floats on) = the sum over `rows` rows of
+// sums, `pitch` floats apart; a null result is skipped.
+hipError_t launch_sum_rows(convnd_hip_dtype param_dtype, const float* partial, int64_t rows,
+                           int64_t pitch, int64_t channels, void* dw, void* db, hipStream_t stream);
+
+// Linear layer (convnd_linear.hip): C[m][n] = sum_k A[m][k] B[n][k], strides in elements. Rows of A
+// and B start on 16 bytes and their lengths are whole 16 bytes (few_rows: any).
+struct LinearArgs {
+  const void* a;
+  const void* b;
+  int64_t lda, ldb, m, n, k;
+  int64_t split_k;            // K values of a split (whole stages)
+  unsigned tiles_m, tiles_n;
+  const void* bias;           // [n] or null
+  const void* residual;       // [m, n] or null
+  int64_t residual_stride;
+  void* output;               // [m, n]
+  void* pre;                  // [m, n]: the sum before the activation, or null
+  float* partial;             // [splits, m, n] where K is split, else null
+  int activation;
+};
+enum class LinearProduct { kForward, kGradInput, kGradWeight };
+struct LinearPlan {
+  bool few_rows;
+  int tile;         // 128 or 256
+  int splits;
+  int64_t split_k;
+};
+LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n, int64_t k);
+hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, LinearProduct which,
+                                 const LinearPlan& p, float* partial, hipStream_t stream);
+hipError_t launch_linear_pad(convnd_hip_dtype dtype, const void* src, int64_t stride, int64_t rows,
+                             int64_t columns, void* dst, hipStream_t stream);
+// The activation's gradient and the bias's.
+struct LinearGradArgs {
+  const void* grad_output;  // [rows, columns] by grad_stride
+  const void* pre;          // [rows, columns], null without an activation
+  void* grad_pre;           // [rows, columns] by pitch, or null
+  float* partial;           // [parts, columns], or null
+  int64_t rows, columns, grad_stride, pitch;
+  int activation;
+};
+int64_t linear_grad_parts(int64_t rows, int64_t columns);
+hipError_t launch_linear_grad(convnd_hip_dtype dtype, const LinearGradArgs& a, int64_t parts,
+                              hipStream_t stream);
 
 // Gated linear recurrence (convnd_recurrence.hip); strides in elements, channels contiguous.
 struct RecurrenceArgs {

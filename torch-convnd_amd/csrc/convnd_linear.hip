@@ -1,0 +1,769 @@
+// Linear layer, y = act(x W^T + b) + r, and its backward pass: products on the matrix cores.
+//
+//   z = x W^T + b, y = act(z) + r
+//   dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum_rows dz (dr = dy needs no work)
+//
+// A product C[m][n] = sum_k A[m][k] B[n][k] takes each operand as it lies in memory: with K
+// contiguous ("inner": x and W in the forward, dz for dx) or with K as the row index ("outer": W for
+// dx, dz and x for dW). 16-bit types multiply on the 16x16x32 MFMA, float on the 16x16x4 one, both
+// from 16-byte fragments and with float sums.
+//   * Many rows: workgroups of 4 waves take tiles of 128 x 128 or 256 x 256. Stages of 128 bytes of K
+//     go straight from memory to LDS, a whole stage ahead; their 16-byte chunks are permuted so that
+//     fragment reads meet no bank twice. An outer operand is read with the transposing LDS read. The
+//     barrier of a stage falls between its two halves, whose fragments are then in registers.
+//   * Few tiles and a long K: K is split over workgroups, their float sums go to the workspace and
+//     are added in order by a second launch with the epilogue.
+//   * Up to 64 rows (decoding): bound by reading W once. A workgroup takes 16 rows of W, its waves
+//     take parts of K and read fragments from memory into registers, all in flight at once.
+// The bounds of a tile are those of the buffers it reads through; rows that do not start on 16 bytes
+// are first copied to the workspace with padding.
+
+#include <algorithm>
+#include <atomic>
+
+#include "convnd_internal.h"
+#include "convnd_sequence.h"
+
+namespace convnd {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr unsigned kNowhere = 0x80000000u;  // past every buffer (below 2^31 bytes)
+
+// 16 bytes of a fragment: for 16-bit types 8 values of K for one MFMA, for float 4 for four.
+template <typename T>
+struct Fragment {
+  static constexpr int kSteps = 1;
+  using type = typename Mfma16<T>::frag;
+  __device__ __forceinline__ static f32x4 mma(type a, type b, f32x4 c) {
+    return Mfma16<T>::run(a, b, c);
+  }
+};
+template <>
+struct Fragment<float> {
+  using type = f32x4;
+  __device__ __forceinline__ static f32x4 mma(type a, type b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned char* dst,
+                                           unsigned offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst), 16,
+                                           offset, 0, 0, 0);
+}
+
+// One operand of the product: `extent` rows (its side of the result) by K. Inner: row-major with K
+// contiguous; outer: K rows of `extent` contiguous values. Staged in LDS as it lies in memory, 128 bytes
+// of K (inner) or rows of EXT values (outer), its 16-byte chunks permuted within a row. Rows are whole
+// chunks (the last one padded with zeros), and so are the bounds: a value cut off from its 4 bytes
+// would read as zero.
+template <typename T, bool OUTER, int EXT, int W>
+struct Operand {
+  static constexpr int kK = 128 / sizeof(T);             // K values of a stage
+  static constexpr int kBytes = EXT * 128;               // of a stage
+  static constexpr int kLoads = kBytes / 1024 / W;       // loads of a wave (1 KB each)
+  static constexpr int kPitch = OUTER ? EXT * int(sizeof(T)) : 128;
+  static constexpr int kChunks = kPitch / 16;            // of a row
+  static constexpr int kVec = 16 / sizeof(T);
+  const char* base;      // of the workgroup's rows or columns, at the first K value of the next stage
+  int64_t ld;            // bytes of a row
+  int64_t rows_left;     // outer: K rows from base on
+  unsigned records;      // inner: bytes of the workgroup's rows; outer: bytes of a row from base on
+  unsigned offset[kLoads];
+  int chunk;             // inner: K chunk of the lane's loads
+
+  __device__ __forceinline__ static int swizzle(int row) {
+    if constexpr (!OUTER) return (row >> 1) & 7;
+    if constexpr (sizeof(T) == 2) return ((row & 3) | ((row >> 1) & 4)) << 1;
+    return 0;
+  }
+
+  __device__ __forceinline__ void init(const void* p, int64_t ld_elements, int64_t extent,
+                                       int64_t at, int64_t k0, int64_t k_end) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    ld = ld_elements * sizeof(T);
+    if constexpr (OUTER) {
+      base = static_cast<const char*>(p) + k0 * ld + at * sizeof(T);
+      rows_left = k_end - k0;
+      records = static_cast<unsigned>((extent - at + kVec - 1) / kVec * 16);
+    } else {
+      base = static_cast<const char*>(p) + at * ld + k0 * sizeof(T);
+      const int64_t rows = extent - at < EXT ? extent - at : EXT;
+      records = static_cast<unsigned>((rows - 1) * ld);
+      rows_left = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at_chunk = (i * W + wave) * 64 + lane;  // in the stage
+      const int row = at_chunk / kChunks;
+      const int c = (at_chunk % kChunks) ^ swizzle(row);
+      if (!OUTER) chunk = c;
+      offset[i] = static_cast<unsigned>(row * static_cast<unsigned>(ld) + c * 16);
+    }
+  }
+
+  // Loads the next stage into LDS at `dst`; k_left values of K remain.
+  __device__ __forceinline__ void load(unsigned char* dst, int64_t k_left) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned bytes;
+    bool inside = true;
+    if constexpr (OUTER) {
+      const int64_t rows = k_left < kK ? k_left : kK;
+      bytes = rows > 0 ? static_cast<unsigned>((rows - 1) * ld) + records : 0u;
+    } else {
+      // Chunks past K lie in the next row.
+      const int64_t k = k_left < kK ? k_left : kK;
+      bytes = k > 0 ? records + static_cast<unsigned>((k + kVec - 1) / kVec * 16) : 0u;
+      inside = chunk * kVec < k;
+    }
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(base), 0, static_cast<int>(bytes), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      load_lds16(r, dst + (i * W + wave) * 1024, inside ? offset[i] : kNowhere);
+    base += OUTER ? kK * ld : 128;
+  }
+};
+
+// Fragment reads of a wave: COUNT fragments of 16 rows (or columns) from `first` on.
+template <typename T, bool OUTER, int EXT, int COUNT>
+struct Reader {
+  using frag = typename Fragment<T>::type;
+  unsigned at[OUTER ? COUNT : 2];
+  __device__ __forceinline__ void init(int first) {
+    const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+    if constexpr (!OUTER) {
+      // Row first + l (+ 16 per fragment: the swizzle repeats every 16 rows).
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        at[ks] = (first + l) * 128 + (((ks * 4 + g) ^ ((l >> 1) & 7)) << 4);
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int n = 0; n < COUNT; ++n) {
+        const int pair = (first / 16 + n) ^ ((l >> 2) | ((g & 1) << 2));
+        at[n] = (8 * g + (l >> 2)) * (EXT * 2) + pair * 32 + (l & 3) * 8;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < COUNT; ++n) at[n] = 4 * g * (EXT * 4) + (first + n * 16 + l) * 4;
+    }
+  }
+  __device__ __forceinline__ void read(frag (&f)[COUNT], const unsigned char* lds, int ks) const {
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n) {
+      if constexpr (!OUTER) {
+        f[n] = *reinterpret_cast<const frag*>(lds + at[ks] + n * 2048);
+      } else if constexpr (sizeof(T) == 2) {
+        // Transposing reads: each gives the lane 4 K values of its column.
+        using lds_vec = __attribute__((address_space(3))) s16x4*;
+        const unsigned char* p = lds + at[n] + ks * 32 * (EXT * 2);
+        union {
+          s16x4 part[2];
+          frag whole;
+        } u;
+        u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(p));
+        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(p + 4 * (EXT * 2)));
+        f[n] = u.whole;
+      } else {
+        const unsigned char* p = lds + at[n] + ks * 16 * (EXT * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[n][i] = *reinterpret_cast<const float*>(p + i * (EXT * 4));
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void activate_all(float (&v)[8], int act) {
+  if (act == CONVND_HIP_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // NaN stays
+  } else if (act == CONVND_HIP_ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.5f * v[e] * (1.f + erff(v[e] * 0.70710678118654752f));
+  } else if (act == CONVND_HIP_ACT_GELU_TANH) {
+    // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float u = 0.79788456080286536f * v[e] * fmaf(0.044715f * v[e], v[e], 1.f);
+      v[e] = v[e] / (1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
+    }
+  }
+}
+
+// Up to 8 neighbouring sums of row m from column n on: the partial sums of a split as they are, else
+// bias, activation and residual in float and one rounding (one more of the sum before the
+// activation, where the backward pass is to have it).
+template <typename T>
+__device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const float (&bias)[8],
+                                       int64_t split, int64_t m, int64_t n, int count) {
+  const int64_t at = m * a.n + n;
+  if (a.partial != nullptr) {
+    float* p = a.partial + split * a.m * a.n + at;
+    if (count == 8) {
+      Run<float, 4> r[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e / 4].v[e % 4] = v[e];
+      store_run<4>(p, r[0]);
+      store_run<4>(p + 4, r[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) p[e] = v[e];
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
+  T* out = static_cast<T*>(a.output) + at;
+  Run<T, 8> y;
+  if (a.pre != nullptr) {
+    T* pre = static_cast<T*>(a.pre) + at;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.v[e] = static_cast<T>(v[e]);
+    if (count == 8) {
+      store_run<8>(pre, y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) pre[e] = y.v[e];
+    }
+  }
+  activate_all(v, a.activation);
+  if (a.residual != nullptr) {
+    const T* residual = static_cast<const T*>(a.residual) + m * a.residual_stride + n;
+    if (count == 8) {
+      const Run<T, 8> r = load_run<8>(residual);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += static_cast<float>(r.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) v[e] += static_cast<float>(residual[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y.v[e] = static_cast<T>(v[e]);
+  if (count == 8) {
+    store_run<8>(out, y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) out[e] = y.v[e];
+  }
+}
+
+// C[m][n] = sum over K of A's row m and B's row n; a workgroup's tile is BM x BN, its 4 waves 2 x 2
+// quarters of MB x NB fragments.
+template <typename T, bool AOUT, bool BOUT, int MB, int NB>
+__global__ __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) void linear_kernel(LinearArgs a) {
+  constexpr int BM = 2 * MB * 16, BN = 2 * NB * 16;
+  using OpA = Operand<T, AOUT, BM, 4>;
+  using OpB = Operand<T, BOUT, BN, 4>;
+  using frag = typename Fragment<T>::type;
+  constexpr int kStage = OpA::kBytes + OpB::kBytes;
+  constexpr int kK = OpA::kK;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+
+  // Workgroup ids go round the eight XCDs: each takes a run of tiles, in bands of 8 tile rows, so
+  // that what its workgroups read at a time stays in its L2.
+  unsigned id = blockIdx.x;
+  {
+    const unsigned n = gridDim.x, per = n >> 3, rest = n & 7, x = id & 7;
+    id = x * per + (x < rest ? x : rest) + (id >> 3);
+  }
+  const unsigned tiles = a.tiles_m * a.tiles_n;
+  const unsigned split = id / tiles;
+  id -= split * tiles;
+  constexpr unsigned kBand = 8;
+  const unsigned band = id / (kBand * a.tiles_n), in_band = id - band * kBand * a.tiles_n;
+  const unsigned height = a.tiles_m - band * kBand < kBand ? a.tiles_m - band * kBand : kBand;
+  const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % height) * BM;
+  const int64_t n0 = static_cast<int64_t>(in_band / height) * BN;
+
+  const int64_t k0 = split * a.split_k;
+  const int64_t k_end = k0 + a.split_k < a.k ? k0 + a.split_k : a.k;
+  OpA opa;
+  OpB opb;
+  opa.init(a.a, a.lda, a.m, m0, k0, k_end);
+  opb.init(a.b, a.ldb, a.n, n0, k0, k_end);
+  Reader<T, AOUT, BM, MB> ra;
+  Reader<T, BOUT, BN, NB> rb;
+  ra.init(wm * MB * 16);
+  rb.init(wn * NB * 16);
+
+  f32x4 acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto wait_loads = []() __attribute__((always_inline)) { __builtin_amdgcn_s_waitcnt(0x0f70); };
+  int64_t k_left = k_end - k0;
+  const int stages = static_cast<int>((k_left + kK - 1) / kK);
+  auto load = [&](int s) __attribute__((always_inline)) {
+    unsigned char* dst = lds + (s & 1) * kStage;
+    opa.load(dst, k_left);
+    opb.load(dst + OpA::kBytes, k_left);
+    k_left -= kK;
+  };
+  frag fa[2][MB], fb[2][NB];
+  auto read = [&](int s, int ks) __attribute__((always_inline)) {
+    const unsigned char* src = lds + (s & 1) * kStage;
+    ra.read(fa[ks], src, ks);
+    rb.read(fb[ks], src + OpA::kBytes, ks);
+  };
+  auto multiply = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = Fragment<T>::mma(fb[ks][j], fa[ks][i], acc[i][j]);
+  };
+  load(0);
+  wait_loads();
+  __syncthreads();
+  read(0, 0);
+  if (stages > 1) load(1);
+  for (int s = 0; s < stages; ++s) {
+    read(s, 1);
+    multiply(0);
+    if (s + 1 < stages) {
+      wait_loads();
+      __syncthreads();  // stage s is in registers everywhere, stage s + 1 in LDS
+      read(s + 1, 0);
+      if (s + 2 < stages) load(s + 2);
+    }
+    multiply(1);
+  }
+
+  // Each wave turns its sums through its own part of LDS, two fragment rows at a time, so that a
+  // lane finishes 8 columns of a row and a store covers whole segments of rows.
+  __syncthreads();
+  constexpr int kPitch = NB * 16 + 4;  // floats; 4 more keep the 16 rows off each other's banks
+  constexpr int kLanes = NB * 2;       // lanes of a row
+  float* turn = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
+  const int l = lane & 15, g = lane >> 4;
+  const int64_t n = n0 + wn * NB * 16 + lane % kLanes * 8;
+  const int count = n >= a.n ? 0 : (a.n - n < 8 ? static_cast<int>(a.n - n) : 8);
+  float bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    bias[e] = a.bias != nullptr && e < count ? static_cast<float>(static_cast<const T*>(a.bias)[n + e])
+                                             : 0.f;
+#pragma unroll
+  for (int i = 0; i < MB; i += 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        *reinterpret_cast<f32x4*>(turn + (h * 16 + l) * kPitch + j * 16 + g * 4) = acc[i + h][j];
+    const int64_t m_first = m0 + (wm * MB + i) * 16;
+#pragma unroll 1
+    for (int r = lane / kLanes; r < 32; r += 64 / kLanes) {
+      const int64_t m = m_first + r;
+      if (m >= a.m || count == 0) continue;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(turn + r * kPitch + lane % kLanes * 8 + q * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q * 4 + e] = t[e];
+      }
+      finish<T>(a, v, bias, split, m, n, count);
+    }
+  }
+}
+
+// ---- few rows --------------------------------------------------------------------------------
+
+// Rows m < 16 MF of x times 16 rows of W a workgroup; W waves share K. Fragment reads straight
+// from memory, of any alignment; past K's end zeros.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::type load_fragment(const T* row, int64_t k,
+                                                                    int64_t k_end) {
+  constexpr int kVec = 16 / sizeof(T);
+  using frag = typename Fragment<T>::type;
+  if (k + kVec <= k_end) return __builtin_bit_cast(frag, load_run<kVec>(row + k));
+  Run<T, kVec> r;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) r.v[i] = k + i < k_end ? row[k + i] : static_cast<T>(0.f);
+  return __builtin_bit_cast(frag, r);
+}
+
+constexpr int kFewWaves = 8;
+template <typename T, int MF>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_rows(LinearArgs a) {
+  constexpr int kStep = 64 / sizeof(T);  // K values of a fragment over its four lane groups
+  constexpr int kUnroll = MF == 4 ? 2 : 4;
+  using frag = typename Fragment<T>::type;
+  __shared__ float sums[kFewWaves][16][MF * 16 + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const T* x = static_cast<const T*>(a.a);
+  const T* w = static_cast<const T*>(a.b);
+  // Rows past the end read the last one; their sums are not used.
+  const T* w_row = w + std::min<int64_t>(n0 + l, a.n - 1) * a.ldb;
+  const T* x_row[MF];
+#pragma unroll
+  for (int f = 0; f < MF; ++f) x_row[f] = x + std::min<int64_t>(f * 16 + l, a.m - 1) * a.lda;
+  f32x4 acc[MF];
+#pragma unroll
+  for (int f = 0; f < MF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // Every wave a run of K: whole steps, the last wave the rest.
+  const int64_t steps = (a.k + kStep - 1) / kStep;
+  const int64_t first = steps * wave / kFewWaves, last = steps * (wave + 1) / kFewWaves;
+  int64_t s = first;
+  for (; s + kUnroll <= last && (s + kUnroll) * kStep <= a.k; s += kUnroll) {
+    frag fw[kUnroll], fx[kUnroll][MF];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t k = (s + u) * kStep + g * (16 / sizeof(T));
+      fw[u] = __builtin_bit_cast(frag, load_run<16 / sizeof(T)>(w_row + k));
+#pragma unroll
+      for (int f = 0; f < MF; ++f)
+        fx[u][f] = __builtin_bit_cast(frag, load_run<16 / sizeof(T)>(x_row[f] + k));
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int f = 0; f < MF; ++f) acc[f] = Fragment<T>::mma(fw[u], fx[u][f], acc[f]);
+  }
+  for (; s < last; ++s) {
+    const int64_t k = s * kStep + g * (16 / sizeof(T));
+    const frag fw = load_fragment(w_row, k, a.k);
+#pragma unroll
+    for (int f = 0; f < MF; ++f) acc[f] = Fragment<T>::mma(fw, load_fragment(x_row[f], k, a.k), acc[f]);
+  }
+  // acc[f][e]: column n0 + 4 g + e of row f * 16 + l.
+#pragma unroll
+  for (int f = 0; f < MF; ++f)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[wave][g * 4 + e][f * 16 + l] = acc[f][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MF * 16 * 2; i += 64 * kFewWaves) {
+    const int m = i / 2, c = i % 2 * 8;
+    const int64_t n = n0 + c;
+    if (m >= a.m || n >= a.n) continue;
+    const int count = a.n - n < 8 ? static_cast<int>(a.n - n) : 8;
+    float v[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < kFewWaves; ++q) v[e] += sums[q][c + e][m];
+      bias[e] = a.bias != nullptr && e < count
+                    ? static_cast<float>(static_cast<const T*>(a.bias)[n + e])
+                    : 0.f;
+    }
+    finish<T>(a, v, bias, 0, m, n, count);
+  }
+}
+
+// ---- sums of a split K, padding, the activation's gradient -----------------------------------------
+
+// Adds the splits' sums in order and finishes 8 columns of a row a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join(LinearArgs a, const float* __restrict__ partial,
+                                                   int64_t splits) {
+  const int64_t parts = (a.n + 7) / 8, total = a.m * parts, step = a.m * a.n;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t m = id / parts, n = id % parts * 8;
+    const int count = a.n - n < 8 ? static_cast<int>(a.n - n) : 8;
+    float v[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = 0.f;
+      bias[e] = a.bias != nullptr && e < count
+                    ? static_cast<float>(static_cast<const T*>(a.bias)[n + e])
+                    : 0.f;
+    }
+    const float* p = partial + m * a.n + n;
+#pragma unroll 4
+    for (int64_t s = 0; s < splits; ++s, p += step) {
+      if (count == 8) {
+        const Run<float, 4> lo = load_run<4>(p), hi = load_run<4>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] += lo.v[e];
+          v[e + 4] += hi.v[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < count) v[e] += p[e];
+      }
+    }
+    finish<T>(a, v, bias, 0, m, n, count);
+  }
+}
+
+// Rows copied with a pitch of whole 16 bytes, zeros past their end.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pad(const T* __restrict__ src, int64_t stride,
+                                                  int64_t rows, int64_t columns, T* __restrict__ dst) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int64_t parts = (columns + kVec - 1) / kVec, total = rows * parts;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = id / parts, c = id % parts * kVec;
+    const T* p = src + r * stride + c;
+    Run<T, kVec> v;
+    if (c + kVec <= columns) {
+      v = load_run<kVec>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v.v[i] = c + i < columns ? p[i] : static_cast<T>(0.f);
+    }
+    store_run<kVec>(dst + id * kVec, v);
+  }
+}
+
+__device__ __forceinline__ float slope(float z, int act) {
+  if (act == CONVND_HIP_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (act == CONVND_HIP_ACT_GELU)
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
+           z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+  // s = sigmoid(2 u): d/dz (z s) = s + 2 z s (1 - s) du/dz
+  const float u = 0.79788456080286536f * z * fmaf(0.044715f * z, z, 1.f);
+  const float s = 1.f / (1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
+  const float du = 0.79788456080286536f * fmaf(3.f * 0.044715f * z, z, 1.f);
+  return s + 2.f * z * s * (1.f - s) * du;
+}
+
+// dz = dy act'(z) (with a pitch of whole 16 bytes, zeros past a row's end) and the sums of dz over
+// each workgroup's rows. 64 threads a row, 8 columns a thread; 4 rows at a time.
+constexpr int kGradColumns = 512, kGradRows = 4;
+template <typename T>
+__global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
+  __shared__ float sums[kGradRows][kGradColumns];
+  const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kGradColumns + lane * 8;
+  const int count = n >= a.columns ? 0 : (a.columns - n < 8 ? static_cast<int>(a.columns - n) : 8);
+  const T* dy = static_cast<const T*>(a.grad_output);
+  const T* pre = static_cast<const T*>(a.pre);
+  T* dz = static_cast<T*>(a.grad_pre);
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (count > 0) {
+    const int64_t step = static_cast<int64_t>(gridDim.y) * kGradRows;
+#pragma unroll 2
+    for (int64_t m = static_cast<int64_t>(blockIdx.y) * kGradRows + group; m < a.rows; m += step) {
+      const T* p = dy + m * a.grad_stride + n;
+      const T* q = pre + m * a.columns + n;
+      Run<T, 8> d, z;
+      if (count == 8) {
+        d = load_run<8>(p);
+        if (pre != nullptr) z = load_run<8>(q);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d.v[e] = e < count ? p[e] : static_cast<T>(0.f);
+          z.v[e] = pre != nullptr && e < count ? q[e] : static_cast<T>(0.f);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (pre != nullptr)
+          d.v[e] = static_cast<T>(static_cast<float>(d.v[e]) *
+                                  slope(static_cast<float>(z.v[e]), a.activation));
+        // The sums are of dz as the products take it.
+        sum[e] += static_cast<float>(d.v[e]);
+      }
+      if (dz != nullptr) {
+        T* o = dz + m * a.pitch + n;
+        if (n + 8 <= a.pitch) {
+          store_run<8>(o, d);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < a.pitch) o[e] = d.v[e];
+        }
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[group][lane * 8 + e] = sum[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < kGradColumns; c += 256) {
+    const int64_t column = static_cast<int64_t>(blockIdx.x) * kGradColumns + c;
+    if (column >= a.columns) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < kGradRows; ++r) s += sums[r][c];
+    a.partial[blockIdx.y * a.columns + column] = s;
+  }
+}
+
+template <typename T, bool AOUT, bool BOUT, int B>
+hipError_t launch_tiles(const LinearArgs& a, int64_t splits, hipStream_t stream) {
+  constexpr int kBytes = 2 * 2 * (2 * B * 16) * 128;
+  const auto kernel = linear_kernel<T, AOUT, BOUT, B, B>;
+  // More than 64 KB of LDS has to be asked for, once per device and kernel.
+  static std::atomic<uint64_t> asked{0};
+  int device = 0;
+  hipError_t err = hipGetDevice(&device);
+  if (err != hipSuccess) return err;
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (kBytes > 65536 && (asked.load(std::memory_order_relaxed) & bit) == 0) {
+    err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (err != hipSuccess) return err;
+    asked.fetch_or(bit, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * splits)), dim3(256),
+                     kBytes, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, bool AOUT, bool BOUT>
+hipError_t launch_product_typed(LinearArgs a, const LinearPlan& p, float* partial,
+                                hipStream_t stream) {
+  if constexpr (!AOUT && !BOUT) {
+    if (p.few_rows) {
+      const dim3 grid(static_cast<unsigned>((a.n + 15) / 16)), block(64 * kFewWaves);
+      if (a.m <= 16)
+        hipLaunchKernelGGL((linear_few_rows<T, 1>), grid, block, 0, stream, a);
+      else if (a.m <= 32)
+        hipLaunchKernelGGL((linear_few_rows<T, 2>), grid, block, 0, stream, a);
+      else
+        hipLaunchKernelGGL((linear_few_rows<T, 4>), grid, block, 0, stream, a);
+      return hipGetLastError();
+    }
+  }
+  LinearArgs t = a;
+  t.split_k = p.split_k;
+  t.tiles_m = static_cast<unsigned>((a.m + p.tile - 1) / p.tile);
+  t.tiles_n = static_cast<unsigned>((a.n + p.tile - 1) / p.tile);
+  if (p.splits > 1) t.partial = partial;
+  hipError_t err;
+  if constexpr (sizeof(T) == 2)
+    err = p.tile == 256 ? launch_tiles<T, AOUT, BOUT, 8>(t, p.splits, stream)
+                        : launch_tiles<T, AOUT, BOUT, 4>(t, p.splits, stream);
+  else
+    err = launch_tiles<T, AOUT, BOUT, 4>(t, p.splits, stream);
+  if (err != hipSuccess || p.splits <= 1) return err;
+  const int64_t work = a.m * ((a.n + 7) / 8);
+  hipLaunchKernelGGL(linear_join<T>,
+                     dim3(static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 8192))),
+                     dim3(256), 0, stream, a, partial, static_cast<int64_t>(p.splits));
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_product(const LinearArgs& a, LinearProduct which, const LinearPlan& p,
+                          float* partial, hipStream_t stream) {
+  switch (which) {
+    case LinearProduct::kForward:
+      return launch_product_typed<T, false, false>(a, p, partial, stream);
+    case LinearProduct::kGradInput:
+      return launch_product_typed<T, false, true>(a, p, partial, stream);
+    default:
+      return launch_product_typed<T, true, true>(a, p, partial, stream);
+  }
+}
+
+}  // namespace
+
+LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n,
+                        int64_t k) {
+  LinearPlan p{};
+  p.splits = 1;
+  p.split_k = k;
+  if (which == LinearProduct::kForward && m <= 64) {
+    p.few_rows = true;
+    return p;
+  }
+  const int64_t stage = dtype == CONVND_HIP_FLOAT32 ? 32 : 64;
+  const double speed = dtype == CONVND_HIP_FLOAT32 ? 8.0 : 1.0;
+  double best = 0;
+  for (int tile : {128, 256}) {
+    if (tile == 256 && dtype == CONVND_HIP_FLOAT32) continue;
+    const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
+    for (int64_t splits = 1; splits <= 32; ++splits) {
+      const int64_t split_k = ((k + splits - 1) / splits + stage - 1) / stage * stage;
+      const int64_t real = (k + split_k - 1) / split_k;
+      if (real != splits || (splits > 1 && split_k < 4 * stage)) continue;
+      const int64_t groups = tiles * splits;
+      double us;
+      if (tile == 256) {
+        us = ((groups + 255) / 256) * (speed * split_k * 0.029 + 6.0);
+      } else {
+        const int64_t rest = groups % 512;
+        us = (groups / 512) * (speed * split_k * 0.016 + 3.0) +
+             (rest == 0 ? 0.0 : (speed * split_k * (rest > 256 ? 0.016 : 0.014) + 3.0));
+      }
+      if (splits > 1) us += 4.0 + 8e-6 * static_cast<double>(m) * n * splits / 4.0;
+      if (best == 0 || us < best) {
+        best = us;
+        p.tile = tile;
+        p.splits = static_cast<int>(splits);
+        p.split_k = split_k;
+      }
+    }
+  }
+  return p;
+}
+
+hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, LinearProduct which,
+                                 const LinearPlan& p, float* partial, hipStream_t stream) {
+  switch (dtype) {
+    case CONVND_HIP_FLOAT32:
+      return launch_product<float>(a, which, p, partial, stream);
+    case CONVND_HIP_FLOAT16:
+      return launch_product<_Float16>(a, which, p, partial, stream);
+    case CONVND_HIP_BFLOAT16:
+      return launch_product<__bf16>(a, which, p, partial, stream);
+    default:
+      return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_linear_pad(convnd_hip_dtype dtype, const void* src, int64_t stride, int64_t rows,
+                             int64_t columns, void* dst, hipStream_t stream) {
+  const int vec = dtype == CONVND_HIP_FLOAT32 ? 4 : 8;
+  const int64_t work = rows * ((columns + vec - 1) / vec);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 8192))), block(256);
+  if (dtype == CONVND_HIP_FLOAT32)
+    hipLaunchKernelGGL(linear_pad<float>, grid, block, 0, stream, static_cast<const float*>(src),
+                       stride, rows, columns, static_cast<float*>(dst));
+  else  // either 16-bit type: only zeros are made, the rest is moved
+    hipLaunchKernelGGL(linear_pad<_Float16>, grid, block, 0, stream,
+                       static_cast<const _Float16*>(src), stride, rows, columns,
+                       static_cast<_Float16*>(dst));
+  return hipGetLastError();
+}
+
+int64_t linear_grad_parts(int64_t rows, int64_t columns) {
+  const int64_t wide = (columns + kGradColumns - 1) / kGradColumns;
+  const int64_t needed = (rows + kGradRows - 1) / kGradRows;
+  return std::max<int64_t>(1, std::min<int64_t>(needed, std::max<int64_t>(1, 1024 / wide)));
+}
+
+hipError_t launch_linear_grad(convnd_hip_dtype dtype, const LinearGradArgs& a, int64_t parts,
+                              hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((a.columns + kGradColumns - 1) / kGradColumns),
+                  static_cast<unsigned>(parts));
+  switch (dtype) {
+    case CONVND_HIP_FLOAT32:
+      hipLaunchKernelGGL(linear_grad<float>, grid, dim3(256), 0, stream, a);
+      break;
+    case CONVND_HIP_FLOAT16:
+      hipLaunchKernelGGL(linear_grad<_Float16>, grid, dim3(256), 0, stream, a);
+      break;
+    case CONVND_HIP_BFLOAT16:
+      hipLaunchKernelGGL(linear_grad<__bf16>, grid, dim3(256), 0, stream, a);
+      break;
+    default:
+      return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace convnd

@@ -348,12 +348,12 @@ __global__ __launch_bounds__(1024) void norm_backward_long(NormArgs a) {
   }
 }
 
-// dw and db from the workgroups' sums: 32 channels a workgroup, its 32 groups of 32 lanes add
-// every 32nd row of `partial`, then the groups' sums are added in order.
+// Up to two results (dw and db) from the workgroups' sums, rows of `pitch` floats: 32 channels a
+// workgroup, its 32 groups of 32 lanes add every 32nd row, then the groups' sums are added in order.
 constexpr int kReduceChannels = 32, kReduceGroups = 32;
 template <typename W>
-__global__ __launch_bounds__(kReduceChannels* kReduceGroups) void norm_reduce(
-    const float* __restrict__ partial, int64_t rows, int64_t channels, W* dw, W* db) {
+__global__ __launch_bounds__(kReduceChannels* kReduceGroups) void sum_rows(
+    const float* __restrict__ partial, int64_t rows, int64_t pitch, int64_t channels, W* dw, W* db) {
   __shared__ float sums[kReduceGroups][kReduceChannels + 1];
   const int lane = threadIdx.x % kReduceChannels, group = threadIdx.x / kReduceChannels;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kReduceChannels + lane;
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(kReduceChannels* kReduceGroups) void norm_reduce(
   if (c < channels) {
     const float* p = partial + blockIdx.y * channels + c;
 #pragma unroll 8
-    for (int64_t r = group; r < rows; r += kReduceGroups) s += p[r * 2 * channels];
+    for (int64_t r = group; r < rows; r += kReduceGroups) s += p[r * pitch];
   }
   sums[group][lane] = s;
   __syncthreads();
@@ -455,21 +455,22 @@ hipError_t launch_norm(convnd_hip_dtype dtype, bool float_params, const NormArgs
   }
 }
 
-hipError_t launch_norm_reduce(convnd_hip_dtype param_dtype, const float* partial, int64_t rows,
-                              int64_t channels, void* dw, void* db, hipStream_t stream) {
-  const dim3 grid((channels + kReduceChannels - 1) / kReduceChannels, 2);
+hipError_t launch_sum_rows(convnd_hip_dtype param_dtype, const float* partial, int64_t rows,
+                           int64_t pitch, int64_t channels, void* dw, void* db,
+                           hipStream_t stream) {
+  const dim3 grid((channels + kReduceChannels - 1) / kReduceChannels, pitch > channels ? 2 : 1);
   const dim3 block(kReduceChannels * kReduceGroups);
   switch (param_dtype) {
     case CONVND_HIP_FLOAT32:
-      hipLaunchKernelGGL(norm_reduce<float>, grid, block, 0, stream, partial, rows, channels,
+      hipLaunchKernelGGL(sum_rows<float>, grid, block, 0, stream, partial, rows, pitch, channels,
                          static_cast<float*>(dw), static_cast<float*>(db));
       break;
     case CONVND_HIP_FLOAT16:
-      hipLaunchKernelGGL(norm_reduce<_Float16>, grid, block, 0, stream, partial, rows, channels,
+      hipLaunchKernelGGL(sum_rows<_Float16>, grid, block, 0, stream, partial, rows, pitch, channels,
                          static_cast<_Float16*>(dw), static_cast<_Float16*>(db));
       break;
     case CONVND_HIP_BFLOAT16:
-      hipLaunchKernelGGL(norm_reduce<__bf16>, grid, block, 0, stream, partial, rows, channels,
+      hipLaunchKernelGGL(sum_rows<__bf16>, grid, block, 0, stream, partial, rows, pitch, channels,
                          static_cast<__bf16*>(dw), static_cast<__bf16*>(db));
       break;
     default:

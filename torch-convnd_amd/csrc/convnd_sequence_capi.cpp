@@ -1,4 +1,4 @@
-// C ABI of the sequence operators (layer norm, gated recurrence): argument checks and launches.
+// C ABI of the sequence operators (layer norm, linear layer, gated recurrence): argument checks and launches.
 #include <algorithm>
 #include <limits>
 
@@ -105,6 +105,151 @@ int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, void* workspace, size_t
   return CONVND_HIP_SUCCESS;
 }
 
+// ---- linear --------------------------------------------------------------------------------------
+
+// A tile's 256 rows of an operand are addressed with 31-bit byte offsets.
+constexpr int64_t kMaxLinear = int64_t{1} << 21;
+
+int check_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* p) {
+  if (size_of(dtype) == 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, std::string("linear_act ") + kTypes);
+  if (p == nullptr || p->rows < 0 || p->inputs <= 0 || p->outputs <= 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "linear_act needs nonnegative rows and positive inputs and outputs");
+  if (p->activation < CONVND_HIP_ACT_NONE || p->activation > CONVND_HIP_ACT_GELU_TANH)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "activation must be 'none', 'relu', 'gelu' or 'gelu_tanh'");
+  if (p->inputs >= kMaxLinear || p->outputs >= kMaxLinear || p->input_stride >= kMaxLinear ||
+      p->grad_stride >= kMaxLinear || p->residual_stride >= kMaxLinear)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "linear_act needs inputs, outputs and strides below 2^21 elements");
+  if (p->rows >= int64_t{1} << 31)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs fewer than 2^31 rows");
+  const auto tiles = [](int64_t n) { return (n + 127) / 128; };
+  const int64_t widest = std::max(tiles(p->inputs), tiles(p->outputs));
+  if (tiles(p->rows) * widest >= (int64_t{1} << 26) ||
+      tiles(p->inputs) * tiles(p->outputs) >= (int64_t{1} << 26))
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act sizes are too large");
+  if (p->input_stride < p->inputs)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs rows at least their length apart");
+  return CONVND_HIP_SUCCESS;
+}
+
+// A workspace handed out in parts of whole 256 bytes; sizes only where there is none.
+struct Parts {
+  char* base;
+  size_t used = 0;
+  void* take(int64_t bytes) {
+    void* p = base == nullptr ? nullptr : base + used;
+    used += (static_cast<size_t>(bytes) + 255) & ~size_t{255};
+    return p;
+  }
+};
+
+// One operand as the product kernels want it: itself, or a padded copy in the workspace.
+struct Padded {
+  const void* data;
+  int64_t stride;
+  bool copy;
+};
+bool whole(const void* data, int64_t stride, int64_t columns, int size) {
+  return (reinterpret_cast<uintptr_t>(data) | static_cast<uintptr_t>(stride * size) |
+          static_cast<uintptr_t>(columns * size)) % 16 == 0;
+}
+int64_t padded_columns(int64_t columns, int size) {
+  const int64_t vec = 16 / size;
+  return (columns + vec - 1) / vec * vec;
+}
+Padded padded(const void* data, int64_t stride, int64_t rows, int64_t columns, int size, Parts* ws) {
+  if (whole(data, stride, columns, size)) return {data, stride, false};
+  const int64_t pitch = padded_columns(columns, size);
+  return {ws->take(rows * pitch * size), pitch, true};
+}
+int fill_padded(convnd_hip_dtype dtype, const Padded& p, const void* data, int64_t stride,
+                int64_t rows, int64_t columns, hipStream_t stream) {
+  if (!p.copy) return CONVND_HIP_SUCCESS;
+  return hip_check(launch_linear_pad(dtype, data, stride, rows, columns,
+                                     const_cast<void*>(p.data), stream),
+                   "linear operand copy");
+}
+
+float* partial_sums(const LinearPlan& p, int64_t m, int64_t n, Parts* ws) {
+  return p.splits > 1 ? static_cast<float*>(ws->take(p.splits * m * n * sizeof(float))) : nullptr;
+}
+
+int check_parts(const Parts& ws, size_t size, const char* what) {
+  if (ws.used == 0 || (ws.base != nullptr && size >= ws.used)) return CONVND_HIP_SUCCESS;
+  return fail(CONVND_HIP_WORKSPACE_TOO_SMALL,
+              std::string(what) + " needs a workspace of " + std::to_string(ws.used) + " bytes");
+}
+
+struct LinearForward {
+  LinearPlan plan;
+  Padded x, w;
+  float* partial;
+};
+LinearForward lay_out(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p, const void* input,
+                      const void* weight, Parts* ws) {
+  const int size = size_of(dtype);
+  LinearForward f{};
+  f.plan = plan_product(dtype, LinearProduct::kForward, p.rows, p.outputs, p.inputs);
+  f.x = {input, p.input_stride, false};
+  f.w = {weight, p.inputs, false};
+  if (!f.plan.few_rows) {
+    f.x = padded(input, p.input_stride, p.rows, p.inputs, size, ws);
+    f.w = padded(weight, p.inputs, p.outputs, p.inputs, size, ws);
+  }
+  f.partial = partial_sums(f.plan, p.rows, p.outputs, ws);
+  return f;
+}
+
+struct LinearBackward {
+  LinearPlan input_plan, weight_plan;
+  Padded dz, x, w;
+  bool make_dz;     // dz = dy act'(z), or a padded copy of dy
+  int64_t parts;    // rows of the bias gradient's sums
+  float* sums;
+  float* partial;   // of either product: one runs after the other
+};
+LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p,
+                                const void* grad_output, const void* input, const void* weight,
+                                bool need_input, bool need_weight, bool need_bias, Parts* ws) {
+  const int size = size_of(dtype);
+  LinearBackward b{};
+  b.dz = {grad_output, p.grad_stride, false};
+  const bool products = need_input || need_weight;
+  if (products) {
+    if (p.activation != CONVND_HIP_ACT_NONE) {
+      const int64_t pitch = padded_columns(p.outputs, size);
+      b.dz = {ws->take(p.rows * pitch * size), pitch, true};
+    } else {
+      b.dz = padded(grad_output, p.grad_stride, p.rows, p.outputs, size, ws);
+    }
+  }
+  b.make_dz = b.dz.copy;
+  if (need_weight) b.x = padded(input, p.input_stride, p.rows, p.inputs, size, ws);
+  if (need_input) b.w = padded(weight, p.inputs, p.outputs, p.inputs, size, ws);
+  b.parts = linear_grad_parts(p.rows, p.outputs);
+  if (need_bias) b.sums = static_cast<float*>(ws->take(b.parts * p.outputs * sizeof(float)));
+  // The two products' sums take the same place.
+  const size_t before = ws->used;
+  size_t most = before;
+  if (need_input) {
+    b.input_plan = plan_product(dtype, LinearProduct::kGradInput, p.rows, p.inputs, p.outputs);
+    b.partial = partial_sums(b.input_plan, p.rows, p.inputs, ws);
+    most = std::max(most, ws->used);
+  }
+  if (need_weight) {
+    ws->used = before;
+    b.weight_plan = plan_product(dtype, LinearProduct::kGradWeight, p.outputs, p.inputs, p.rows);
+    float* sums = partial_sums(b.weight_plan, p.outputs, p.inputs, ws);
+    if (sums != nullptr) b.partial = sums;
+    most = std::max(most, ws->used);
+  }
+  ws->used = most;
+  return b;
+}
+
 }  // namespace
 }  // namespace convnd
 
@@ -186,8 +331,8 @@ int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype para
     if (st != CONVND_HIP_SUCCESS) return st;
   }
   if (!params) return CONVND_HIP_SUCCESS;
-  return hip_check(launch_norm_reduce(param_dtype, partial, p.blocks, channels, grad_weight,
-                                      grad_bias, static_cast<hipStream_t>(stream)),
+  return hip_check(launch_sum_rows(param_dtype, partial, p.blocks, 2 * channels, channels,
+                                   grad_weight, grad_bias, static_cast<hipStream_t>(stream)),
                    "layer norm reduction launch");
 }
 
@@ -256,6 +401,148 @@ int convnd_hip_recurrence_backward(convnd_hip_dtype dtype, const convnd_hip_recu
   if (st != CONVND_HIP_SUCCESS) return st;
   return hip_check(launch_recurrence(dtype, a, true, p, static_cast<hipStream_t>(stream)),
                    "gated recurrence backward launch");
+}
+
+size_t convnd_hip_linear_workspace_size(convnd_hip_dtype dtype,
+                                        const convnd_hip_linear_problem* problem,
+                                        const void* input, const void* weight) {
+  if (check_linear(dtype, problem) != CONVND_HIP_SUCCESS || problem->rows == 0) return 0;
+  Parts ws{nullptr};
+  lay_out(dtype, *problem, input, weight, &ws);
+  return ws.used;
+}
+
+int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                      const void* input, const void* weight, const void* bias,
+                      const void* residual, void* output, void* pre, void* workspace,
+                      size_t workspace_size, void* stream) {
+  int st = check_linear(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const convnd_hip_linear_problem& p = *problem;
+  if (p.rows == 0) return CONVND_HIP_SUCCESS;
+  if (input == nullptr || weight == nullptr || output == nullptr)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "input, weight and output must not be null");
+  Parts ws{static_cast<char*>(workspace)};
+  const LinearForward f = lay_out(dtype, p, input, weight, &ws);
+  st = check_parts(ws, workspace_size, "linear_act");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const auto on = static_cast<hipStream_t>(stream);
+  st = fill_padded(dtype, f.x, input, p.input_stride, p.rows, p.inputs, on);
+  if (st == CONVND_HIP_SUCCESS)
+    st = fill_padded(dtype, f.w, weight, p.inputs, p.outputs, p.inputs, on);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  LinearArgs a{};
+  a.a = f.x.data;
+  a.b = f.w.data;
+  a.lda = f.x.stride;
+  a.ldb = f.w.stride;
+  a.m = p.rows;
+  a.n = p.outputs;
+  a.k = p.inputs;
+  a.bias = bias;
+  a.residual = residual;
+  a.residual_stride = p.residual_stride;
+  a.output = output;
+  a.pre = pre;
+  a.activation = p.activation;
+  return hip_check(launch_linear_product(dtype, a, LinearProduct::kForward, f.plan, f.partial, on),
+                   "linear launch");
+}
+
+size_t convnd_hip_linear_backward_workspace_size(convnd_hip_dtype dtype,
+                                                 const convnd_hip_linear_problem* problem,
+                                                 const void* grad_output, const void* input,
+                                                 const void* weight, int need_grad_input,
+                                                 int need_grad_weight, int need_grad_bias) {
+  if (check_linear(dtype, problem) != CONVND_HIP_SUCCESS || problem->rows == 0) return 0;
+  Parts ws{nullptr};
+  lay_out_backward(dtype, *problem, grad_output, input, weight, need_grad_input != 0,
+                   need_grad_weight != 0, need_grad_bias != 0, &ws);
+  return ws.used;
+}
+
+int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                               const void* grad_output, const void* input, const void* weight,
+                               const void* pre, void* grad_input, void* grad_weight,
+                               void* grad_bias, void* workspace, size_t workspace_size,
+                               void* stream) {
+  int st = check_linear(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const convnd_hip_linear_problem& p = *problem;
+  const auto on = static_cast<hipStream_t>(stream);
+  if (p.rows == 0) {
+    if (grad_weight != nullptr)
+      st = hip_check(launch_fill_zero(grad_weight, p.outputs * p.inputs * size_of(dtype), on),
+                     "linear backward launch");
+    if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr)
+      st = hip_check(launch_fill_zero(grad_bias, p.outputs * size_of(dtype), on),
+                     "linear backward launch");
+    return st;
+  }
+  const bool activated = p.activation != CONVND_HIP_ACT_NONE;
+  if (p.grad_stride < p.outputs)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs rows at least their length apart");
+  if (grad_output == nullptr || (activated && pre == nullptr) ||
+      (grad_input != nullptr && weight == nullptr) || (grad_weight != nullptr && input == nullptr))
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "grad_output, input, weight and (with an activation) pre must not be null");
+  Parts ws{static_cast<char*>(workspace)};
+  const LinearBackward b =
+      lay_out_backward(dtype, p, grad_output, input, weight, grad_input != nullptr,
+                       grad_weight != nullptr, grad_bias != nullptr, &ws);
+  st = check_parts(ws, workspace_size, "linear_act backward");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  if (b.make_dz || grad_bias != nullptr) {
+    LinearGradArgs g{};
+    g.grad_output = grad_output;
+    g.pre = activated ? pre : nullptr;
+    g.grad_pre = b.make_dz ? const_cast<void*>(b.dz.data) : nullptr;
+    g.partial = b.sums;
+    g.rows = p.rows;
+    g.columns = p.outputs;
+    g.grad_stride = p.grad_stride;
+    g.pitch = b.dz.stride;
+    g.activation = p.activation;
+    st = hip_check(launch_linear_grad(dtype, g, b.parts, on), "linear gradient launch");
+    if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr)
+      st = hip_check(launch_sum_rows(dtype, b.sums, b.parts, p.outputs, p.outputs, grad_bias,
+                                     nullptr, on),
+                     "linear bias gradient launch");
+    if (st != CONVND_HIP_SUCCESS) return st;
+  }
+  LinearArgs a{};
+  if (grad_input != nullptr) {
+    st = fill_padded(dtype, b.w, weight, p.inputs, p.outputs, p.inputs, on);
+    if (st != CONVND_HIP_SUCCESS) return st;
+    a.a = b.dz.data;
+    a.lda = b.dz.stride;
+    a.b = b.w.data;
+    a.ldb = b.w.stride;
+    a.m = p.rows;
+    a.n = p.inputs;
+    a.k = p.outputs;
+    a.output = grad_input;
+    st = hip_check(launch_linear_product(dtype, a, LinearProduct::kGradInput, b.input_plan,
+                                         b.partial, on),
+                   "linear input gradient launch");
+    if (st != CONVND_HIP_SUCCESS) return st;
+  }
+  if (grad_weight != nullptr) {
+    st = fill_padded(dtype, b.x, input, p.input_stride, p.rows, p.inputs, on);
+    if (st != CONVND_HIP_SUCCESS) return st;
+    a.a = b.dz.data;
+    a.lda = b.dz.stride;
+    a.b = b.x.data;
+    a.ldb = b.x.stride;
+    a.m = p.outputs;
+    a.n = p.inputs;
+    a.k = p.rows;
+    a.output = grad_weight;
+    st = hip_check(launch_linear_product(dtype, a, LinearProduct::kGradWeight, b.weight_plan,
+                                         b.partial, on),
+                   "linear weight gradient launch");
+  }
+  return st;
 }
 
 }  // extern "C"

@@ -1,5 +1,5 @@
-// PyTorch dispatcher kernels of the sequence operators: torch_convnd::layer_norm and
-// torch_convnd::gated_recurrence with their backward operators, a thin layer over the C ABI. The
+// PyTorch dispatcher kernels of the sequence operators: torch_convnd::layer_norm, linear_act and
+// gated_recurrence with their backward operators, a thin layer over the C ABI. The
 // schemas are defined from Python (torch_convnd/_operators.py); no counterpart in the reference.
 
 #include <ATen/ATen.h>
@@ -8,8 +8,11 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <array>
 #include <optional>
+#include <string>
 #include <tuple>
+#include <vector>
 
 #include "convnd_hip.h"
 
@@ -225,6 +228,196 @@ std::tuple<at::Tensor, at::Tensor> layer_norm_autograd(const at::Tensor& input,
   return {out[0], out[1]};
 }
 
+// ---- linear --------------------------------------------------------------------------------
+
+int linear_activation(c10::string_view activation) {
+  if (activation == "none") return CONVND_HIP_ACT_NONE;
+  if (activation == "relu") return CONVND_HIP_ACT_RELU;
+  if (activation == "gelu") return CONVND_HIP_ACT_GELU;
+  if (activation == "gelu_tanh") return CONVND_HIP_ACT_GELU_TANH;
+  TORCH_CHECK(false, "activation must be 'none', 'relu', 'gelu' or 'gelu_tanh'");
+}
+
+std::vector<int64_t> linear_shape(const at::Tensor& input, const at::Tensor& weight) {
+  auto shape = input.sizes().vec();
+  shape.back() = weight.size(0);
+  return shape;
+}
+
+void check_linear_input(const at::Tensor& input, const at::Tensor& weight) {
+  TORCH_CHECK(native_type(input.scalar_type()),
+              "native linear_act supports float16, bfloat16 and float32");
+  TORCH_CHECK(weight.dim() == 2 && input.dim() >= 1 && weight.size(0) > 0 && weight.size(1) > 0 &&
+                  input.size(-1) == weight.size(1),
+              "linear_act expects an input of [..., inputs] and a weight of [outputs, inputs]");
+  TORCH_CHECK(weight.device() == input.device() && weight.scalar_type() == input.scalar_type(),
+              "input and weight must have the same device and dtype");
+}
+
+// Rows no closer than their length, as the kernels take them.
+Rows as_apart_rows(const at::Tensor& t) {
+  auto r = as_rows(t);
+  if (r.stride >= t.size(-1) && r.stride < (int64_t{1} << 21)) return r;
+  return {t.contiguous(), t.size(-1)};
+}
+
+convnd_hip_linear_problem linear_problem(const at::Tensor& input, const at::Tensor& weight,
+                                         const Rows& x, int activation) {
+  convnd_hip_linear_problem p{};
+  p.rows = input.numel() / weight.size(1);
+  p.inputs = weight.size(1);
+  p.outputs = weight.size(0);
+  p.input_stride = x.stride;
+  p.residual_stride = p.grad_stride = p.outputs;
+  p.activation = activation;
+  return p;
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_act_device(const at::Tensor& input,
+                                                     const at::Tensor& weight,
+                                                     const OptionalTensor& bias,
+                                                     const OptionalTensor& residual,
+                                                     c10::string_view activation, bool keep_pre) {
+  const int act = linear_activation(activation);
+  check_linear_input(input, weight);
+  if (bias.has_value())
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0) &&
+                    bias->device() == input.device() && bias->scalar_type() == input.scalar_type(),
+                "bias must match the outputs, device and dtype");
+  const auto shape = linear_shape(input, weight);
+  if (residual.has_value())
+    TORCH_CHECK(residual->sizes() == at::IntArrayRef(shape) &&
+                    residual->device() == input.device() &&
+                    residual->scalar_type() == input.scalar_type(),
+                "residual must match the output's shape, device and dtype");
+  const c10::OptionalDeviceGuard guard(input.device());
+  const auto x = as_apart_rows(input);
+  const auto w = weight.contiguous();
+  const auto b = contiguous(bias);
+  auto p = linear_problem(input, weight, x, act);
+  Rows r;
+  if (residual.has_value()) {
+    r = as_apart_rows(*residual);
+    p.residual_stride = r.stride;
+  }
+  const auto dtype = sequence_dtype(input);
+  auto output = at::empty(shape, input.options());
+  const bool keep = keep_pre && act != CONVND_HIP_ACT_NONE;
+  auto pre = keep ? at::empty(shape, input.options()) : at::empty({0}, input.options());
+  const size_t bytes =
+      convnd_hip_linear_workspace_size(dtype, &p, x.tensor.const_data_ptr(), w.const_data_ptr());
+  at::Tensor workspace;
+  if (bytes > 0)
+    workspace = at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte));
+  check_status(convnd_hip_linear(
+      dtype, &p, x.tensor.const_data_ptr(), w.const_data_ptr(), data_or_null(b),
+      residual.has_value() ? r.tensor.const_data_ptr() : nullptr, output.mutable_data_ptr(),
+      keep ? pre.mutable_data_ptr() : nullptr, bytes > 0 ? workspace.mutable_data_ptr() : nullptr,
+      bytes, stream_of(input)));
+  return {output, pre};
+}
+
+std::tuple<OptionalTensor, OptionalTensor, OptionalTensor> linear_act_backward_device(
+    const at::Tensor& grad_output, const at::Tensor& input, const at::Tensor& weight,
+    const at::Tensor& pre, c10::string_view activation, std::array<bool, 3> output_mask) {
+  const int act = linear_activation(activation);
+  check_linear_input(input, weight);
+  const auto shape = linear_shape(input, weight);
+  TORCH_CHECK(grad_output.sizes() == at::IntArrayRef(shape) &&
+                  grad_output.device() == input.device() &&
+                  grad_output.scalar_type() == input.scalar_type(),
+              "linear_act grad_output must match the output's shape, device and dtype");
+  TORCH_CHECK(act == CONVND_HIP_ACT_NONE ||
+                  (pre.sizes() == at::IntArrayRef(shape) && pre.is_contiguous() &&
+                   pre.device() == input.device() && pre.scalar_type() == input.scalar_type()),
+              "linear_act pre must be what its forward kept");
+  OptionalTensor dx, dw, db;
+  if (!output_mask[0] && !output_mask[1] && !output_mask[2]) return {dx, dw, db};
+  const c10::OptionalDeviceGuard guard(input.device());
+  const auto x = as_apart_rows(input), dy = as_apart_rows(grad_output);
+  const auto w = weight.contiguous();
+  auto p = linear_problem(input, weight, x, act);
+  p.grad_stride = dy.stride;
+  if (output_mask[0]) dx = at::empty(input.sizes(), input.options());
+  if (output_mask[1]) dw = at::empty(weight.sizes(), weight.options());
+  if (output_mask[2]) db = at::empty({p.outputs}, weight.options());
+  const auto dtype = sequence_dtype(input);
+  const size_t bytes = convnd_hip_linear_backward_workspace_size(
+      dtype, &p, dy.tensor.const_data_ptr(), x.tensor.const_data_ptr(), w.const_data_ptr(),
+      output_mask[0], output_mask[1], output_mask[2]);
+  at::Tensor workspace;
+  if (bytes > 0)
+    workspace = at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte));
+  check_status(convnd_hip_linear_backward(
+      dtype, &p, dy.tensor.const_data_ptr(), x.tensor.const_data_ptr(), w.const_data_ptr(),
+      act != CONVND_HIP_ACT_NONE ? pre.const_data_ptr() : nullptr,
+      dx.has_value() ? dx->mutable_data_ptr() : nullptr,
+      dw.has_value() ? dw->mutable_data_ptr() : nullptr,
+      db.has_value() ? db->mutable_data_ptr() : nullptr,
+      bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, stream_of(input)));
+  return {dx, dw, db};
+}
+
+const auto& linear_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("torch_convnd::linear_act", "")
+                             .typed<decltype(linear_act_device)>();
+  return op;
+}
+const auto& linear_backward_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("torch_convnd::linear_act_backward", "")
+                             .typed<decltype(linear_act_backward_device)>();
+  return op;
+}
+
+class LinearActFunction : public torch::autograd::Function<LinearActFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& input,
+                               const at::Tensor& weight, const OptionalTensor& bias,
+                               const OptionalTensor& residual, const std::string& activation) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [output, pre] = linear_op().call(input, weight, bias, residual, activation, true);
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->save_for_backward({input, weight, pre});
+    ctx->mark_non_differentiable({pre});
+    ctx->set_materialize_grads(false);
+    return {output, pre};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("linear_act");
+    if (!grads[0].defined()) return variable_list(5);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto saved = ctx->get_saved_variables();
+    const bool bias = ctx->saved_data["bias"].toBool();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const std::array<bool, 3> mask = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                      bias && ctx->needs_input_grad(2)};
+    auto [dx, dw, db] =
+        linear_backward_op().call(grads[0], saved[0], saved[1], saved[2],
+                                  ctx->saved_data["activation"].toStringRef(), mask);
+    return {dx.value_or(at::Tensor()), dw.value_or(at::Tensor()), db.value_or(at::Tensor()),
+            residual ? grads[0] : at::Tensor(), at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> linear_act_autograd(const at::Tensor& input,
+                                                       const at::Tensor& weight,
+                                                       const OptionalTensor& bias,
+                                                       const OptionalTensor& residual,
+                                                       c10::string_view activation, bool keep_pre) {
+  if (!at::GradMode::is_enabled() || !(wants_grad(input) || wants_grad(weight) ||
+                                       wants_grad(bias) || wants_grad(residual))) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear_op().call(input, weight, bias, residual, activation, keep_pre);
+  }
+  auto out = LinearActFunction::apply(input, weight, bias, residual, std::string(activation));
+  return {out[0], out[1]};
+}
+
 // ---- gated recurrence ------------------------------------------------------------------------
 
 void check_recurrence_input(const at::Tensor& input, const at::Tensor& gate,
@@ -401,12 +594,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_recurrence_autograd(
 
 TORCH_LIBRARY_IMPL(torch_convnd, Autograd, library) {
   library.impl("layer_norm", &torch_convnd_hip::layer_norm_autograd);
+  library.impl("linear_act", &torch_convnd_hip::linear_act_autograd);
   library.impl("gated_recurrence", &torch_convnd_hip::gated_recurrence_autograd);
 }
 
 TORCH_LIBRARY_IMPL(torch_convnd, CUDA, library) {
   library.impl("layer_norm", &torch_convnd_hip::layer_norm_device);
   library.impl("layer_norm_backward", &torch_convnd_hip::layer_norm_backward_device);
+  library.impl("linear_act", &torch_convnd_hip::linear_act_device);
+  library.impl("linear_act_backward", &torch_convnd_hip::linear_act_backward_device);
   library.impl("gated_recurrence", &torch_convnd_hip::gated_recurrence_device);
   library.impl("gated_recurrence_backward", &torch_convnd_hip::gated_recurrence_backward_device);
 }

@@ -24,7 +24,7 @@ from .modules import (
     PartialSequential,
 )
 from .partial import PartialConvOutput, partial_conv_nd
-from .sequence import gated_recurrence, layer_norm
+from .sequence import gated_recurrence, layer_norm, linear_act
 
 ensure_native_definitions()
 ensure_compatible_operator()
@@ -45,6 +45,7 @@ __all__ = [
     "conv_nd",
     "gated_recurrence",
     "layer_norm",
+    "linear_act",
     "partial_conv_nd",
     "load_native",
     "get_runtime_info",

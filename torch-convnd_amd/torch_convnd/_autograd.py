@@ -213,6 +213,18 @@ def _fake_layer_norm_backward(grad_output, input, weight, bias, statistics, outp
     return dx, dw, db
 
 
+def _fake_linear_act(input, weight, bias, residual, activation, keep_pre):
+    shape = (*input.shape[:-1], weight.shape[0])
+    return input.new_empty(shape), input.new_empty(shape if keep_pre and activation != "none" else (0,))
+
+
+def _fake_linear_act_backward(grad_output, input, weight, pre, activation, output_mask):
+    contiguous = torch.contiguous_format
+    dx = torch.empty_like(input, memory_format=contiguous) if output_mask[0] else None
+    dw = torch.empty_like(weight, memory_format=contiguous) if output_mask[1] else None
+    return dx, dw, weight.new_empty(weight.shape[0]) if output_mask[2] else None
+
+
 def _fake_recurrence(input, gate, initial_state, lengths, keep_carries):
     batch, tokens, channels = input.shape
     tiles = (tokens + RECURRENCE_TILE - 1) // RECURRENCE_TILE
@@ -254,6 +266,8 @@ def register_training() -> None:
     torch.library.register_fake("torch_convnd::conv_nd_act")(_fake_act)
     torch.library.register_fake("torch_convnd::layer_norm")(_fake_layer_norm)
     torch.library.register_fake("torch_convnd::layer_norm_backward")(_fake_layer_norm_backward)
+    torch.library.register_fake("torch_convnd::linear_act")(_fake_linear_act)
+    torch.library.register_fake("torch_convnd::linear_act_backward")(_fake_linear_act_backward)
     torch.library.register_fake("torch_convnd::gated_recurrence")(_fake_recurrence)
     torch.library.register_fake("torch_convnd::gated_recurrence_backward")(_fake_recurrence_backward)
     torch.library.register_autograd(

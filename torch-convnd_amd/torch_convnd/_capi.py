@@ -36,6 +36,10 @@ EXPORTED_SYMBOLS = (
     "convnd_hip_layer_norm",
     "convnd_hip_layer_norm_backward_workspace_size",
     "convnd_hip_layer_norm_backward",
+    "convnd_hip_linear_workspace_size",
+    "convnd_hip_linear",
+    "convnd_hip_linear_backward_workspace_size",
+    "convnd_hip_linear_backward",
     "convnd_hip_recurrence_carries",
     "convnd_hip_recurrence_workspace_size",
     "convnd_hip_recurrence",
@@ -75,6 +79,15 @@ class Problem(ctypes.Structure):
             p.input[a], p.kernel[a] = x_shape[a + 2], w_shape[a + 2]
             p.stride[a], p.padding[a], p.dilation[a] = stride[a], padding[a], dilation[a]
         return p
+
+
+class LinearProblem(ctypes.Structure):
+    """struct convnd_hip_linear_problem."""
+
+    _fields_ = [
+        (name, ctypes.c_int64)
+        for name in ("rows", "inputs", "outputs", "input_stride", "residual_stride", "grad_stride")
+    ] + [("activation", ctypes.c_int)]
 
 
 class RecurrenceProblem(ctypes.Structure):
@@ -142,6 +155,19 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     library.convnd_hip_layer_norm_backward.restype = ctypes.c_int
     library.convnd_hip_layer_norm_backward.argtypes = [
         ctypes.c_int, ctypes.c_int, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, vp, sz, vp
+    ]
+    L = ctypes.POINTER(LinearProblem)
+    library.convnd_hip_linear_workspace_size.restype = sz
+    library.convnd_hip_linear_workspace_size.argtypes = [ctypes.c_int, L, vp, vp]
+    library.convnd_hip_linear.restype = ctypes.c_int
+    library.convnd_hip_linear.argtypes = [ctypes.c_int, L, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    library.convnd_hip_linear_backward_workspace_size.restype = sz
+    library.convnd_hip_linear_backward_workspace_size.argtypes = [
+        ctypes.c_int, L, vp, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_int
+    ]
+    library.convnd_hip_linear_backward.restype = ctypes.c_int
+    library.convnd_hip_linear_backward.argtypes = [
+        ctypes.c_int, L, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp
     ]
     library.convnd_hip_recurrence_carries.restype = i64
     library.convnd_hip_recurrence_carries.argtypes = [i64]

@@ -85,13 +85,17 @@ def _lazy(name, position=0):
     return load_and_call
 
 
-# Sequence operators (layer norm, gated recurrence); no reference counterpart. The second
+# Sequence operators (layer norm, linear layer, gated recurrence); no reference counterpart. The second
 # results of the forwards are what their backward operators read, kept only on request.
 _SEQUENCE_SCHEMAS = (
     "layer_norm(Tensor input, Tensor? weight, Tensor? bias, float eps, bool keep_statistics) "
     "-> (Tensor, Tensor)",
     "layer_norm_backward(Tensor grad_output, Tensor input, Tensor? weight, Tensor? bias, "
     "Tensor statistics, bool[3] output_mask) -> (Tensor?, Tensor?, Tensor?)",
+    "linear_act(Tensor input, Tensor weight, Tensor? bias, Tensor? residual, str activation, "
+    "bool keep_pre) -> (Tensor, Tensor)",
+    "linear_act_backward(Tensor grad_output, Tensor input, Tensor weight, Tensor pre, "
+    "str activation, bool[3] output_mask) -> (Tensor?, Tensor?, Tensor?)",
     "gated_recurrence(Tensor input, Tensor gate, Tensor? initial_state, Tensor? lengths, "
     "bool keep_carries) -> (Tensor, Tensor, Tensor)",
     "gated_recurrence_backward(Tensor grad_output, Tensor? grad_last, Tensor input, Tensor gate, "

@@ -1,5 +1,6 @@
-"""Operators of token sequences around the convolution: layer norm and the gated linear
-recurrence over activations of [..., channels]. No counterpart in the reference.
+"""Operators of token sequences around the convolution: layer norm, the linear layer with its
+activation and residual, and the gated linear recurrence, over activations of [..., channels]. No
+counterpart in the reference.
 
 ``backend`` as for ``conv_nd``: ``auto`` runs the gfx950 kernels for ROCm GPU tensors (float16,
 bfloat16, float32; other types are refused there) and PyTorch operations for other devices and
@@ -13,9 +14,17 @@ from torch import Tensor
 from torch.nn import functional as F
 
 from . import _build
-from ._compat import is_autocast_enabled, autocast_dtype, is_compiling, is_onnx_exporting, transforms_active
+from ._compat import (
+    autocast_disabled,
+    autocast_dtype,
+    is_autocast_enabled,
+    is_compiling,
+    is_onnx_exporting,
+    transforms_active,
+)
 from ._dispatch import BACKENDS
 from ._toolchain import native_unavailable_reason
+from .functional import _ACTIVATIONS, _apply_activation
 
 _NATIVE_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -89,6 +98,60 @@ def layer_norm(
     wide = torch.float64 if input.dtype == torch.float64 else torch.float32
     cast = lambda t: None if t is None else t.to(wide)  # noqa: E731
     return F.layer_norm(cast(input), input.shape[-1:], cast(weight), cast(bias), eps).to(input.dtype)
+
+
+def linear_act(
+    input: Tensor,
+    weight: Tensor,
+    bias: Tensor | None = None,
+    residual: Tensor | None = None,
+    *,
+    activation: str | None = None,
+    backend: str = "auto",
+) -> Tensor:
+    """``act(input @ weight.T + bias) + residual`` over the last dimension of ``input`` [..., inputs].
+
+    ``weight`` is [outputs, inputs], ``bias`` [outputs], ``residual`` of the output's shape
+    [..., outputs]; all in the input's dtype. ``activation`` as for ``conv_nd``: "relu", "gelu",
+    "gelu_tanh" or None. On the gfx950 path all of it is one rounding of the float32 sums (a training
+    step also keeps the sums before the activation, in the input's dtype). ``input`` and ``residual``
+    may be slices of wider rows. Under autocast the operands are cast to its dtype.
+    """
+    if activation is not None and activation not in _ACTIVATIONS:
+        raise ValueError(f"Invalid activation {activation!r}; expected 'relu', 'gelu' or 'gelu_tanh'")
+    if is_autocast_enabled(input.device.type):
+        dtype = autocast_dtype(input.device.type)
+        cast = lambda t: t.to(dtype) if t is not None and t.dtype in _NATIVE_DTYPES else t  # noqa: E731
+        input, weight, bias, residual = cast(input), cast(weight), cast(bias), cast(residual)
+    if _use_native(input, backend, "linear_act"):
+        keep = _recording(input, weight, bias, residual)
+        return torch.ops.torch_convnd.linear_act.default(
+            input, weight, bias, residual, activation or "none", keep
+        )[0]
+    return _portable_linear(input, weight, bias, residual, activation)
+
+
+def _portable_linear(input, weight, bias, residual, activation):
+    if weight.dim() != 2 or input.dim() == 0 or input.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise RuntimeError("linear_act expects an input of [..., inputs] and a weight of [outputs, inputs]")
+    if weight.device != input.device or weight.dtype != input.dtype:
+        raise RuntimeError("input and weight must have the same device and dtype")
+    if bias is not None and (
+        bias.shape != weight.shape[:1] or bias.device != input.device or bias.dtype != input.dtype
+    ):
+        raise RuntimeError("bias must match the outputs, device and dtype")
+    shape = (*input.shape[:-1], weight.shape[0])
+    if residual is not None and (
+        residual.shape != shape or residual.device != input.device or residual.dtype != input.dtype
+    ):
+        raise RuntimeError("residual must match the output's shape, device and dtype")
+    wide = torch.float64 if input.dtype == torch.float64 else torch.float32
+    with autocast_disabled(input.device.type):
+        output = F.linear(input.to(wide), weight.to(wide), None if bias is None else bias.to(wide))
+        output = _apply_activation(output, activation)
+        if residual is not None:
+            output = output + residual.to(wide)
+    return output.to(input.dtype)
 
 
 def gated_recurrence(
