@@ -296,7 +296,7 @@ typedef struct convnd_hip_linear_problem {
 } convnd_hip_linear_problem;
 
 /* Device scratch bytes of convnd_hip_linear; of the pointers only the alignment is looked at (rows
- * that do not start on 16 bytes are copied). */
+ * that do not start on 4 bytes are copied). */
 size_t convnd_hip_linear_workspace_size(convnd_hip_dtype dtype,
                                         const convnd_hip_linear_problem* problem,
                                         const void* input, const void* weight);

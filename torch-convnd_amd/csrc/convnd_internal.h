@@ -565,7 +565,7 @@ hipError_t launch_sum_rows(convnd_hip_dtype param_dtype, const float* partial, i
                            int64_t pitch, int64_t channels, void* dw, void* db, hipStream_t stream);
 
 // Linear layer (convnd_linear.hip): C[m][n] = sum_k A[m][k] B[n][k], strides in elements. Rows of A
-// and B start on 16 bytes and their lengths are whole 16 bytes (few_rows: any).
+// and B start on 4 bytes and their lengths are whole 4 bytes (few_rows: any).
 struct LinearArgs {
   const void* a;
   const void* b;
@@ -583,7 +583,7 @@ struct LinearArgs {
 enum class LinearProduct { kForward, kGradInput, kGradWeight };
 struct LinearPlan {
   bool few_rows;
-  int tile;         // 128 or 256
+  int tile;         // 64, 128 or 256
   int splits;
   int64_t split_k;
 };

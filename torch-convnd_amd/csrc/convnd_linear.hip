@@ -7,19 +7,22 @@
 // contiguous ("inner": x and W in the forward, dz for dx) or with K as the row index ("outer": W for
 // dx, dz and x for dW). 16-bit types multiply on the 16x16x32 MFMA, float on the 16x16x4 one, both
 // from 16-byte fragments and with float sums.
-//   * Many rows: workgroups of 4 waves take tiles of 128 x 128 or 256 x 256. Stages of 128 bytes of K
-//     go straight from memory to LDS, a whole stage ahead; their 16-byte chunks are permuted so that
-//     fragment reads meet no bank twice. An outer operand is read with the transposing LDS read. The
-//     barrier of a stage falls between its two halves, whose fragments are then in registers.
+//   * Many rows: workgroups take tiles of 256 x 256 (8 waves of 128 x 64: half the LDS reads a
+//     product of 64 x 64), 128 x 128 or 64 x 64 (4 waves) as plan_product weighs them. Stages of 128
+//     bytes of K go straight from memory to LDS, a whole stage ahead; their 16-byte chunks are
+//     permuted so that fragment reads meet no bank twice. An outer operand is read with the
+//     transposing LDS read. The barrier of a stage falls between its two halves, whose fragments are
+//     then in registers.
 //   * Few tiles and a long K: K is split over workgroups, their float sums go to the workspace and
 //     are added in order by a second launch with the epilogue.
 //   * Up to 64 rows (decoding): bound by reading W once. A workgroup takes 16 rows of W, its waves
 //     take parts of K and read fragments from memory into registers, all in flight at once.
-// The bounds of a tile are those of the buffers it reads through; rows that do not start on 16 bytes
+// The bounds of a tile are those of the buffers it reads through; 16-bit rows of odd length or stride
 // are first copied to the workspace with padding.
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "convnd_internal.h"
 #include "convnd_sequence.h"
@@ -56,11 +59,17 @@ __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned ch
                                            offset, 0, 0, 0);
 }
 
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned char* dst,
+                                          unsigned offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst), 4,
+                                           offset, 0, 0, 0);
+}
+
 // One operand of the product: `extent` rows (its side of the result) by K. Inner: row-major with K
 // contiguous; outer: K rows of `extent` contiguous values. Staged in LDS as it lies in memory, 128 bytes
-// of K (inner) or rows of EXT values (outer), its 16-byte chunks permuted within a row. Rows are whole
-// chunks (the last one padded with zeros), and so are the bounds: a value cut off from its 4 bytes
-// would read as zero.
+// of K (inner) or rows of EXT values (outer), its 16-byte chunks permuted within a row. Rows start
+// on 4 bytes, and one whose length is no whole 4 bytes is padded with a zero: the buffer's bounds are
+// checked by 4 bytes.
 template <typename T, bool OUTER, int EXT, int W>
 struct Operand {
   static constexpr int kK = 128 / sizeof(T);             // K values of a stage
@@ -69,63 +78,85 @@ struct Operand {
   static constexpr int kPitch = OUTER ? EXT * int(sizeof(T)) : 128;
   static constexpr int kChunks = kPitch / 16;            // of a row
   static constexpr int kVec = 16 / sizeof(T);
+  static_assert(kLoads >= 1, "at least one load a wave");
   const char* base;      // of the workgroup's rows or columns, at the first K value of the next stage
   int64_t ld;            // bytes of a row
-  int64_t rows_left;     // outer: K rows from base on
-  unsigned records;      // inner: bytes of the workgroup's rows; outer: bytes of a row from base on
+  unsigned before_last;  // inner: bytes of the workgroup's rows but the last
+  unsigned row_bytes;    // outer: bytes of a row from base on
   unsigned offset[kLoads];
-  int chunk;             // inner: K chunk of the lane's loads
 
   __device__ __forceinline__ static int swizzle(int row) {
     if constexpr (!OUTER) return (row >> 1) & 7;
-    if constexpr (sizeof(T) == 2) return ((row & 3) | ((row >> 1) & 4)) << 1;
+    // A transposing read takes 32 bytes of rows r .. r + 3 and r + 8 .. r + 11 at a time.
+    if constexpr (sizeof(T) == 2 && EXT >= 128) return ((row & 3) | ((row >> 1) & 4)) << 1;
+    if constexpr (sizeof(T) == 2) return (((row >> 1) & 1) | ((row >> 2) & 2)) << 1;
     return 0;
   }
 
+  __device__ __forceinline__ static unsigned whole_words(unsigned bytes) {
+    return (bytes + 3) & ~3u;
+  }
+
   __device__ __forceinline__ void init(const void* p, int64_t ld_elements, int64_t extent,
-                                       int64_t at, int64_t k0, int64_t k_end) {
+                                       int64_t at, int64_t k0) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     ld = ld_elements * sizeof(T);
-    if constexpr (OUTER) {
-      base = static_cast<const char*>(p) + k0 * ld + at * sizeof(T);
-      rows_left = k_end - k0;
-      records = static_cast<unsigned>((extent - at + kVec - 1) / kVec * 16);
-    } else {
-      base = static_cast<const char*>(p) + at * ld + k0 * sizeof(T);
-      const int64_t rows = extent - at < EXT ? extent - at : EXT;
-      records = static_cast<unsigned>((rows - 1) * ld);
-      rows_left = 0;
-    }
+    base = static_cast<const char*>(p) + (OUTER ? k0 * ld + at * int64_t{sizeof(T)}
+                                                : at * ld + k0 * int64_t{sizeof(T)});
+    const int64_t rows = extent - at < EXT ? extent - at : EXT;
+    before_last = static_cast<unsigned>((rows - 1) * ld);
+    row_bytes = whole_words(static_cast<unsigned>((extent - at) * sizeof(T)));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int at_chunk = (i * W + wave) * 64 + lane;  // in the stage
-      const int row = at_chunk / kChunks;
-      const int c = (at_chunk % kChunks) ^ swizzle(row);
-      if (!OUTER) chunk = c;
-      offset[i] = static_cast<unsigned>(row * static_cast<unsigned>(ld) + c * 16);
+      const int chunk = (i * W + wave) * 64 + lane;  // in the stage
+      const int row = chunk / kChunks;
+      offset[i] = static_cast<unsigned>(row) * static_cast<unsigned>(ld) +
+                  ((chunk % kChunks) ^ swizzle(row)) * 16;
     }
   }
 
-  // Loads the next stage into LDS at `dst`; k_left values of K remain.
-  __device__ __forceinline__ void load(unsigned char* dst, int64_t k_left) {
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(int k) const {
+    const unsigned bytes = OUTER ? static_cast<unsigned>((k - 1) * ld) + row_bytes
+                                 : before_last + whole_words(static_cast<unsigned>(k) * unsigned{sizeof(T)});
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(bytes),
+                                             0x00020000);
+  }
+
+  // Loads a whole stage into LDS at `dst`.
+  __device__ __forceinline__ void load(unsigned char* dst) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned bytes;
-    bool inside = true;
-    if constexpr (OUTER) {
-      const int64_t rows = k_left < kK ? k_left : kK;
-      bytes = rows > 0 ? static_cast<unsigned>((rows - 1) * ld) + records : 0u;
-    } else {
-      // Chunks past K lie in the next row.
-      const int64_t k = k_left < kK ? k_left : kK;
-      bytes = k > 0 ? records + static_cast<unsigned>((k + kVec - 1) / kVec * 16) : 0u;
-      inside = chunk * kVec < k;
-    }
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(base), 0, static_cast<int>(bytes), 0x00020000);
+    const __amdgpu_buffer_rsrc_t r = rows(kK);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      load_lds16(r, dst + (i * W + wave) * 1024, inside ? offset[i] : kNowhere);
+    for (int i = 0; i < kLoads; ++i) load_lds16(r, dst + (i * W + wave) * 1024, offset[i]);
     base += OUTER ? kK * ld : 128;
+  }
+
+  // Loads the last stage, of k <= kK values of K; zeros follow them. An inner row goes on in the next
+  // one there: whole chunks past k are sent nowhere, and where k ends inside a chunk the loads are of
+  // 4 bytes.
+  __device__ __forceinline__ void load_last(unsigned char* dst, int k) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const __amdgpu_buffer_rsrc_t r = rows(k);
+    if (OUTER || k % kVec == 0) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int chunk = (i * W + wave) * 64 + lane;
+        const bool inside =
+            OUTER || (((chunk % kChunks) ^ swizzle(chunk / kChunks)) * kVec) < k;
+        load_lds16(r, dst + (i * W + wave) * 1024, inside ? offset[i] : kNowhere);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kLoads * 4; ++i) {
+        const int part = (i / 4 * W + wave) * 4 + i % 4;  // of 256 bytes
+        const int word = part * 64 + lane;
+        const int row = word / 32;
+        const int column = ((word % 32 / 4) ^ swizzle(row)) * 16 + word % 4 * 4;
+        const unsigned at = static_cast<unsigned>(row) * static_cast<unsigned>(ld) + column;
+        load_lds4(r, dst + part * 256, column < k * int{sizeof(T)} ? at : kNowhere);
+      }
+    }
   }
 };
 
@@ -133,6 +164,7 @@ struct Operand {
 template <typename T, bool OUTER, int EXT, int COUNT>
 struct Reader {
   using frag = typename Fragment<T>::type;
+  static constexpr int kReads = COUNT * (!OUTER ? 1 : (sizeof(T) == 2 ? 2 : 4));
   unsigned at[OUTER ? COUNT : 2];
   __device__ __forceinline__ void init(int first) {
     const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
@@ -144,7 +176,8 @@ struct Reader {
     } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int n = 0; n < COUNT; ++n) {
-        const int pair = (first / 16 + n) ^ ((l >> 2) | ((g & 1) << 2));
+        const int swizzle = EXT >= 128 ? (l >> 2) | ((g & 1) << 2) : (l >> 3) | ((g & 1) << 1);
+        const int pair = (first / 16 + n) ^ swizzle;
         at[n] = (8 * g + (l >> 2)) * (EXT * 2) + pair * 32 + (l & 3) * 8;
       }
     } else {
@@ -189,7 +222,7 @@ __device__ __forceinline__ void activate_all(float (&v)[8], int act) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float u = 0.79788456080286536f * v[e] * fmaf(0.044715f * v[e], v[e], 1.f);
-      v[e] = v[e] / (1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
+      v[e] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
     }
   }
 }
@@ -256,20 +289,36 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
   }
 }
 
-// C[m][n] = sum over K of A's row m and B's row n; a workgroup's tile is BM x BN, its 4 waves 2 x 2
-// quarters of MB x NB fragments.
-template <typename T, bool AOUT, bool BOUT, int MB, int NB>
-__global__ __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) void linear_kernel(LinearArgs a) {
-  constexpr int BM = 2 * MB * 16, BN = 2 * NB * 16;
-  using OpA = Operand<T, AOUT, BM, 4>;
-  using OpB = Operand<T, BOUT, BN, 4>;
+// Spreads READS LDS reads, then LOADS loads to LDS, evenly between the MFMAS of a scheduling region.
+template <int READS, int LOADS, int MFMAS>
+__device__ __forceinline__ void interleave() {
+  constexpr int kPer = MFMAS / (READS + LOADS) > 0 ? MFMAS / (READS + LOADS) : 1;
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+    __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
+    __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
+  }
+}
+
+// C[m][n] = sum over K of A's row m and B's row n; a workgroup's tile is BM x BN, its WM x WN
+// waves take MB x NB fragments each.
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinearArgs a) {
+  constexpr int BM = WM * MB * 16, BN = WN * NB * 16;
+  using OpA = Operand<T, AOUT, BM, WM * WN>;
+  using OpB = Operand<T, BOUT, BN, WM * WN>;
   using frag = typename Fragment<T>::type;
   constexpr int kStage = OpA::kBytes + OpB::kBytes;
   constexpr int kK = OpA::kK;
   extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave % WM, wn = wave / WM;
 
   // Workgroup ids go round the eight XCDs: each takes a run of tiles, in bands of 8 tile rows, so
   // that what its workgroups read at a time stays in its L2.
@@ -288,11 +337,13 @@ __global__ __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) void linear_kernel(Line
   const int64_t n0 = static_cast<int64_t>(in_band / height) * BN;
 
   const int64_t k0 = split * a.split_k;
-  const int64_t k_end = k0 + a.split_k < a.k ? k0 + a.split_k : a.k;
+  const int64_t k_count = k0 + a.split_k < a.k ? a.split_k : a.k - k0;
+  const int stages = static_cast<int>((k_count + kK - 1) / kK);
+  const int k_last = static_cast<int>(k_count - int64_t{stages - 1} * kK);
   OpA opa;
   OpB opb;
-  opa.init(a.a, a.lda, a.m, m0, k0, k_end);
-  opb.init(a.b, a.ldb, a.n, n0, k0, k_end);
+  opa.init(a.a, a.lda, a.m, m0, k0);
+  opb.init(a.b, a.ldb, a.n, n0, k0);
   Reader<T, AOUT, BM, MB> ra;
   Reader<T, BOUT, BN, NB> rb;
   ra.init(wm * MB * 16);
@@ -305,13 +356,15 @@ __global__ __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) void linear_kernel(Line
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   auto wait_loads = []() __attribute__((always_inline)) { __builtin_amdgcn_s_waitcnt(0x0f70); };
-  int64_t k_left = k_end - k0;
-  const int stages = static_cast<int>((k_left + kK - 1) / kK);
   auto load = [&](int s) __attribute__((always_inline)) {
     unsigned char* dst = lds + (s & 1) * kStage;
-    opa.load(dst, k_left);
-    opb.load(dst + OpA::kBytes, k_left);
-    k_left -= kK;
+    opa.load(dst);
+    opb.load(dst + OpA::kBytes);
+  };
+  auto load_last = [&](int s) __attribute__((always_inline)) {
+    unsigned char* dst = lds + (s & 1) * kStage;
+    opa.load_last(dst, k_last);
+    opb.load_last(dst + OpA::kBytes, k_last);
   };
   frag fa[2][MB], fb[2][NB];
   auto read = [&](int s, int ks) __attribute__((always_inline)) {
@@ -325,22 +378,51 @@ __global__ __launch_bounds__(256, MB * NB >= 64 ? 1 : 2) void linear_kernel(Line
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = Fragment<T>::mma(fb[ks][j], fa[ks][i], acc[i][j]);
   };
-  load(0);
+  // A stage: the products of its first half while its second half is read, a barrier (then the
+  // stage is in registers everywhere, and the next in LDS), the products of the second half while
+  // the next stage's first half is read and the loads of the one after go out. Reads and loads are
+  // spread between the MFMAs: a wave issues in order, and many in a row wait for their queues.
+  constexpr int kMfma = MB * NB * (sizeof(T) == 4 ? 4 : 1);
+  constexpr int kReads = Reader<T, AOUT, BM, MB>::kReads + Reader<T, BOUT, BN, NB>::kReads;
+  constexpr int kLoads = OpA::kLoads + OpB::kLoads;
+  // Two workgroups a compute unit fill each other's gaps by themselves (128 x 128 in this order:
+  // dx 934, dW 893 TFLOP/s; left to the compiler 998 and 992).
+  constexpr bool kSpread = MB * NB >= 32;
+  auto stage = [&](int s, auto next, auto after) __attribute__((always_inline)) {
+    read(s, 1);
+    multiply(0);
+    if constexpr (kSpread) {
+      interleave<kReads, 0, kMfma>();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (decltype(next)::value) {
+      wait_loads();
+      __syncthreads();
+      if constexpr (kSpread) __builtin_amdgcn_sched_barrier(0);
+      read(s + 1, 0);
+    }
+    if constexpr (decltype(after)::value) load(s + 2);
+    if constexpr (decltype(next)::value && !decltype(after)::value) {
+      if (s + 2 < stages) load_last(s + 2);
+    }
+    multiply(1);
+    if constexpr (kSpread) {
+      if constexpr (decltype(next)::value)
+        interleave<kReads, decltype(after)::value ? kLoads : 0, kMfma>();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (stages > 1) load(0); else load_last(0);
   wait_loads();
   __syncthreads();
   read(0, 0);
-  if (stages > 1) load(1);
-  for (int s = 0; s < stages; ++s) {
-    read(s, 1);
-    multiply(0);
-    if (s + 1 < stages) {
-      wait_loads();
-      __syncthreads();  // stage s is in registers everywhere, stage s + 1 in LDS
-      read(s + 1, 0);
-      if (s + 2 < stages) load(s + 2);
-    }
-    multiply(1);
-  }
+  if (stages > 2) load(1); else if (stages > 1) load_last(1);
+  if constexpr (kSpread) __builtin_amdgcn_sched_barrier(0);
+  int s = 0;
+  for (; s + 3 < stages; ++s) stage(s, std::true_type{}, std::true_type{});
+#pragma unroll 1
+  for (; s + 1 < stages; ++s) stage(s, std::true_type{}, std::false_type{});
+  stage(s, std::false_type{}, std::false_type{});
 
   // Each wave turns its sums through its own part of LDS, two fragment rows at a time, so that a
   // lane finishes 8 columns of a row and a store covers whole segments of rows.
@@ -532,7 +614,7 @@ __device__ __forceinline__ float slope(float z, int act) {
            z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
   // s = sigmoid(2 u): d/dz (z s) = s + 2 z s (1 - s) du/dz
   const float u = 0.79788456080286536f * z * fmaf(0.044715f * z, z, 1.f);
-  const float s = 1.f / (1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
+  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
   const float du = 0.79788456080286536f * fmaf(3.f * 0.044715f * z, z, 1.f);
   return s + 2.f * z * s * (1.f - s) * du;
 }
@@ -601,10 +683,10 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
   }
 }
 
-template <typename T, bool AOUT, bool BOUT, int B>
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
 hipError_t launch_tiles(const LinearArgs& a, int64_t splits, hipStream_t stream) {
-  constexpr int kBytes = 2 * 2 * (2 * B * 16) * 128;
-  const auto kernel = linear_kernel<T, AOUT, BOUT, B, B>;
+  constexpr int kBytes = 2 * (WM * MB + WN * NB) * 16 * 128;
+  const auto kernel = linear_kernel<T, AOUT, BOUT, MB, NB, WM, WN>;
   // More than 64 KB of LDS has to be asked for, once per device and kernel.
   static std::atomic<uint64_t> asked{0};
   int device = 0;
@@ -617,8 +699,8 @@ hipError_t launch_tiles(const LinearArgs& a, int64_t splits, hipStream_t stream)
     if (err != hipSuccess) return err;
     asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * splits)), dim3(256),
-                     kBytes, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * splits)),
+                     dim3(64 * WM * WN), kBytes, stream, a);
   return hipGetLastError();
 }
 
@@ -644,10 +726,12 @@ hipError_t launch_product_typed(LinearArgs a, const LinearPlan& p, float* partia
   if (p.splits > 1) t.partial = partial;
   hipError_t err;
   if constexpr (sizeof(T) == 2)
-    err = p.tile == 256 ? launch_tiles<T, AOUT, BOUT, 8>(t, p.splits, stream)
-                        : launch_tiles<T, AOUT, BOUT, 4>(t, p.splits, stream);
+    err = p.tile == 256 ? launch_tiles<T, AOUT, BOUT, 8, 4, 2, 4>(t, p.splits, stream)
+          : p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2>(t, p.splits, stream)
+                          : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2>(t, p.splits, stream);
   else
-    err = launch_tiles<T, AOUT, BOUT, 4>(t, p.splits, stream);
+    err = p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2>(t, p.splits, stream)
+                        : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2>(t, p.splits, stream);
   if (err != hipSuccess || p.splits <= 1) return err;
   const int64_t work = a.m * ((a.n + 7) / 8);
   hipLaunchKernelGGL(linear_join<T>,
@@ -671,6 +755,31 @@ hipError_t launch_product(const LinearArgs& a, LinearProduct which, const Linear
 
 }  // namespace
 
+namespace {
+
+// Time (us) of `groups` workgroups of a tile over k values of K, from measurements: `wide` of them run
+// side by side, whole turns of the chip take set-up and epilogue plus a time per K value, and a
+// last turn that does not fill every compute unit's places takes less per K value.
+// 16-bit: 256 x 256 alone on a compute unit 26.5 ns a K value (1270 TFLOP/s at 8192^3); 128 x 128
+// two to a compute unit 14.2 (1125), alone 11.9; 64 x 64 five 14.0 (700). float is bound by its MFMA
+// rate at any tile (130 TFLOP/s).
+double tile_time(bool single, int tile, int64_t groups, double k) {
+  const double per_cu = static_cast<double>((groups + 255) / 256);
+  if (single) return 4.0 + per_cu * k * (tile == 64 ? 0.0162 : 0.0640);
+  if (tile == 256) return per_cu * (6.0 + 0.0265 * k);
+  const int64_t wide = tile == 128 ? 512 : 1280;
+  const double set_up = tile == 128 ? 6.0 : 3.0;
+  const int64_t rest = groups % wide;
+  double us = static_cast<double>(groups / wide) * (set_up + (tile == 128 ? 0.0142 : 0.0140) * k);
+  if (rest > 0) {
+    const int64_t side = (rest + 255) / 256;
+    us += set_up + (tile == 128 ? (side == 1 ? 0.0119 : 0.0142) : 0.004 + 0.002 * side) * k;
+  }
+  return us;
+}
+
+}  // namespace
+
 LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n,
                         int64_t k) {
   LinearPlan p{};
@@ -680,26 +789,18 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
     p.few_rows = true;
     return p;
   }
-  const int64_t stage = dtype == CONVND_HIP_FLOAT32 ? 32 : 64;
-  const double speed = dtype == CONVND_HIP_FLOAT32 ? 8.0 : 1.0;
+  const bool single = dtype == CONVND_HIP_FLOAT32;
+  const int64_t stage = single ? 32 : 64;
   double best = 0;
-  for (int tile : {128, 256}) {
-    if (tile == 256 && dtype == CONVND_HIP_FLOAT32) continue;
+  for (int tile : {64, 128, 256}) {
+    if (tile == 256 && single) continue;
     const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
     for (int64_t splits = 1; splits <= 32; ++splits) {
       const int64_t split_k = ((k + splits - 1) / splits + stage - 1) / stage * stage;
-      const int64_t real = (k + split_k - 1) / split_k;
-      if (real != splits || (splits > 1 && split_k < 4 * stage)) continue;
-      const int64_t groups = tiles * splits;
-      double us;
-      if (tile == 256) {
-        us = ((groups + 255) / 256) * (speed * split_k * 0.029 + 6.0);
-      } else {
-        const int64_t rest = groups % 512;
-        us = (groups / 512) * (speed * split_k * 0.016 + 3.0) +
-             (rest == 0 ? 0.0 : (speed * split_k * (rest > 256 ? 0.016 : 0.014) + 3.0));
-      }
-      if (splits > 1) us += 4.0 + 8e-6 * static_cast<double>(m) * n * splits / 4.0;
+      if ((k + split_k - 1) / split_k != splits || (splits > 1 && split_k < 4 * stage)) continue;
+      double us = tile_time(single, tile, tiles * splits, static_cast<double>(std::min(split_k, k)));
+      // The splits' sums are written, read and joined (through the last cache level at 7 TB/s).
+      if (splits > 1) us += 3.0 + static_cast<double>(m) * n * (4.0 * splits + 2.0) / 7e6;
       if (best == 0 || us < best) {
         best = us;
         p.tile = tile;

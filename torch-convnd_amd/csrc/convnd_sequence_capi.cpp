@@ -154,7 +154,7 @@ struct Padded {
 };
 bool whole(const void* data, int64_t stride, int64_t columns, int size) {
   return (reinterpret_cast<uintptr_t>(data) | static_cast<uintptr_t>(stride * size) |
-          static_cast<uintptr_t>(columns * size)) % 16 == 0;
+          static_cast<uintptr_t>(columns * size)) % 4 == 0;
 }
 int64_t padded_columns(int64_t columns, int size) {
   const int64_t vec = 16 / size;
