@@ -53,17 +53,19 @@ struct Fragment<float> {
   }
 };
 
-__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned char* dst,
-                                           unsigned offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst), 16,
-                                           offset, 0, 0, 0);
+// 16 or 4 bytes per lane from the buffer straight into LDS: lane l writes dst + 16 l (4 l), dst the
+// same for the whole wave. Inline assembly, so that the compiler does not take the LDS reads that
+// follow, of other stages, to depend on them: whoever reads what they bring waits with wait_loads.
+__device__ __forceinline__ void load_lds16(u32x4 rows, unsigned dst, unsigned offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst),
+      "v"(offset), "s"(rows));
 }
-
-__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned char* dst,
-                                          unsigned offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst), 4,
-                                           offset, 0, 0, 0);
+__device__ __forceinline__ void load_lds4(u32x4 rows, unsigned dst, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(dst),
+               "v"(offset), "s"(rows));
 }
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // One operand of the product: `extent` rows (its side of the result) by K. Inner: row-major with K
 // contiguous; outer: K rows of `extent` contiguous values. Staged in LDS as it lies in memory, 128 bytes
@@ -115,29 +117,31 @@ struct Operand {
     }
   }
 
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(int k) const {
+  // The stage's rows up to K value k as a buffer.
+  __device__ __forceinline__ u32x4 rows(int k) const {
     const unsigned bytes = OUTER ? static_cast<unsigned>((k - 1) * ld) + row_bytes
                                  : before_last + whole_words(static_cast<unsigned>(k) * unsigned{sizeof(T)});
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(bytes),
-                                             0x00020000);
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(at));
+    r[1] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(at >> 32) & 0xffffu);
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[3] = 0x00020000u;
+    return r;
   }
+  __device__ __forceinline__ void advance() { base += OUTER ? kK * ld : 128; }
 
-  // Loads a whole stage into LDS at `dst`.
-  __device__ __forceinline__ void load(unsigned char* dst) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const __amdgpu_buffer_rsrc_t r = rows(kK);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_lds16(r, dst + (i * W + wave) * 1024, offset[i]);
-    base += OUTER ? kK * ld : 128;
+  // Load i (of kLoads) of a whole stage into LDS at `dst`.
+  __device__ __forceinline__ void load(u32x4 r, unsigned dst, int wave, int i) const {
+    load_lds16(r, dst + (i * W + wave) * 1024, offset[i]);
   }
 
   // Loads the last stage, of k <= kK values of K; zeros follow them. An inner row goes on in the next
   // one there: whole chunks past k are sent nowhere, and where k ends inside a chunk the loads are of
   // 4 bytes.
-  __device__ __forceinline__ void load_last(unsigned char* dst, int k) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __device__ __forceinline__ void load_last(unsigned dst, int wave, int k) const {
     const int lane = threadIdx.x & 63;
-    const __amdgpu_buffer_rsrc_t r = rows(k);
+    const u32x4 r = rows(k);
     if (OUTER || k % kVec == 0) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
@@ -164,7 +168,6 @@ struct Operand {
 template <typename T, bool OUTER, int EXT, int COUNT>
 struct Reader {
   using frag = typename Fragment<T>::type;
-  static constexpr int kReads = COUNT * (!OUTER ? 1 : (sizeof(T) == 2 ? 2 : 4));
   unsigned at[OUTER ? COUNT : 2];
   __device__ __forceinline__ void init(int first) {
     const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
@@ -185,28 +188,28 @@ struct Reader {
       for (int n = 0; n < COUNT; ++n) at[n] = 4 * g * (EXT * 4) + (first + n * 16 + l) * 4;
     }
   }
-  __device__ __forceinline__ void read(frag (&f)[COUNT], const unsigned char* lds, int ks) const {
+  // Fragment n of half ks of the stage at `lds`.
+  __device__ __forceinline__ frag read(const unsigned char* lds, int ks, int n) const {
+    frag f;
+    if constexpr (!OUTER) {
+      f = *reinterpret_cast<const frag*>(lds + at[ks] + n * 2048);
+    } else if constexpr (sizeof(T) == 2) {
+      // Transposing reads: each gives the lane 4 K values of its column.
+      using lds_vec = __attribute__((address_space(3))) s16x4*;
+      const unsigned char* p = lds + at[n] + ks * 32 * (EXT * 2);
+      union {
+        s16x4 part[2];
+        frag whole;
+      } u;
+      u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(p));
+      u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(p + 4 * (EXT * 2)));
+      f = u.whole;
+    } else {
+      const unsigned char* p = lds + at[n] + ks * 16 * (EXT * 4);
 #pragma unroll
-    for (int n = 0; n < COUNT; ++n) {
-      if constexpr (!OUTER) {
-        f[n] = *reinterpret_cast<const frag*>(lds + at[ks] + n * 2048);
-      } else if constexpr (sizeof(T) == 2) {
-        // Transposing reads: each gives the lane 4 K values of its column.
-        using lds_vec = __attribute__((address_space(3))) s16x4*;
-        const unsigned char* p = lds + at[n] + ks * 32 * (EXT * 2);
-        union {
-          s16x4 part[2];
-          frag whole;
-        } u;
-        u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(p));
-        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec)(p + 4 * (EXT * 2)));
-        f[n] = u.whole;
-      } else {
-        const unsigned char* p = lds + at[n] + ks * 16 * (EXT * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[n][i] = *reinterpret_cast<const float*>(p + i * (EXT * 4));
-      }
+      for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const float*>(p + i * (EXT * 4));
     }
+    return f;
   }
 };
 
@@ -289,22 +292,6 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
   }
 }
 
-// Spreads READS LDS reads, then LOADS loads to LDS, evenly between the MFMAS of a scheduling region.
-template <int READS, int LOADS, int MFMAS>
-__device__ __forceinline__ void interleave() {
-  constexpr int kPer = MFMAS / (READS + LOADS) > 0 ? MFMAS / (READS + LOADS) : 1;
-#pragma unroll
-  for (int i = 0; i < READS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-    __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
-  }
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
-    __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
-  }
-}
-
 // C[m][n] = sum over K of A's row m and B's row n; a workgroup's tile is BM x BN, its WM x WN
 // waves take MB x NB fragments each.
 template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
@@ -355,69 +342,90 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinearArgs a) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto wait_loads = []() __attribute__((always_inline)) { __builtin_amdgcn_s_waitcnt(0x0f70); };
-  auto load = [&](int s) __attribute__((always_inline)) {
-    unsigned char* dst = lds + (s & 1) * kStage;
-    opa.load(dst);
-    opb.load(dst + OpA::kBytes);
-  };
-  auto load_last = [&](int s) __attribute__((always_inline)) {
-    unsigned char* dst = lds + (s & 1) * kStage;
-    opa.load_last(dst, k_last);
-    opb.load_last(dst + OpA::kBytes, k_last);
-  };
   frag fa[2][MB], fb[2][NB];
-  auto read = [&](int s, int ks) __attribute__((always_inline)) {
+  const unsigned lds_at = static_cast<unsigned>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(lds)));
+  auto load = [&](int s) __attribute__((always_inline)) {
+    const unsigned dst = lds_at + (s & 1) * kStage;
+    if (s + 1 < stages) {
+      const u32x4 a_rows = opa.rows(kK), b_rows = opb.rows(kK);
+#pragma unroll
+      for (int i = 0; i < OpA::kLoads; ++i) opa.load(a_rows, dst, wave, i);
+#pragma unroll
+      for (int i = 0; i < OpB::kLoads; ++i) opb.load(b_rows, dst + OpA::kBytes, wave, i);
+    } else {
+      opa.load_last(dst, wave, k_last);
+      opb.load_last(dst + OpA::kBytes, wave, k_last);
+    }
+    opa.advance();
+    opb.advance();
+  };
+  // Fragments i of A and B (where there is one) of half ks.
+  auto read = [&](int s, int ks, int i) __attribute__((always_inline)) {
     const unsigned char* src = lds + (s & 1) * kStage;
-    ra.read(fa[ks], src, ks);
-    rb.read(fb[ks], src + OpA::kBytes, ks);
+    if (i < MB) fa[ks][i] = ra.read(src, ks, i);
+    if (i < NB) fb[ks][i] = rb.read(src + OpA::kBytes, ks, i);
   };
-  auto multiply = [&](int ks) __attribute__((always_inline)) {
+  auto multiply = [&](int ks, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int j = 0; j < NB; ++j) acc[i][j] = Fragment<T>::mma(fb[ks][j], fa[ks][i], acc[i][j]);
+    for (int j = 0; j < NB; ++j) acc[i][j] = Fragment<T>::mma(fb[ks][j], fa[ks][i], acc[i][j]);
   };
+  static_assert(NB <= MB, "the steps of a stage are fragment rows of A");
   // A stage: the products of its first half while its second half is read, a barrier (then the
   // stage is in registers everywhere, and the next in LDS), the products of the second half while
-  // the next stage's first half is read and the loads of the one after go out. Reads and loads are
-  // spread between the MFMAs: a wave issues in order, and many in a row wait for their queues.
-  constexpr int kMfma = MB * NB * (sizeof(T) == 4 ? 4 : 1);
-  constexpr int kReads = Reader<T, AOUT, BM, MB>::kReads + Reader<T, BOUT, BN, NB>::kReads;
-  constexpr int kLoads = OpA::kLoads + OpB::kLoads;
-  // Two workgroups a compute unit fill each other's gaps by themselves (128 x 128 in this order:
-  // dx 934, dW 893 TFLOP/s; left to the compiler 998 and 992).
-  constexpr bool kSpread = MB * NB >= 32;
+  // the loads of the stage after next go out and the next stage's first half is read. A wave issues
+  // in order and many reads or loads in a row wait for their queues: they are spread over the rows of
+  // products, in this order.
   auto stage = [&](int s, auto next, auto after) __attribute__((always_inline)) {
-    read(s, 1);
-    multiply(0);
-    if constexpr (kSpread) {
-      interleave<kReads, 0, kMfma>();
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      multiply(0, i);
+      // The first products wait for the fragments read before, not for these too.
+      if (i == 0) __builtin_amdgcn_sched_barrier(0);
+      read(s, 1, i);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    u32x4 a_rows, b_rows;
+    if constexpr (decltype(after)::value) {
+      a_rows = opa.rows(kK);
+      b_rows = opb.rows(kK);
     }
     if constexpr (decltype(next)::value) {
       wait_loads();
       __syncthreads();
-      if constexpr (kSpread) __builtin_amdgcn_sched_barrier(0);
-      read(s + 1, 0);
+      if constexpr (!decltype(after)::value) {
+        if (s + 2 < stages) load(s + 2);
+      }
     }
-    if constexpr (decltype(after)::value) load(s + 2);
-    if constexpr (decltype(next)::value && !decltype(after)::value) {
-      if (s + 2 < stages) load_last(s + 2);
-    }
-    multiply(1);
-    if constexpr (kSpread) {
-      if constexpr (decltype(next)::value)
-        interleave<kReads, decltype(after)::value ? kLoads : 0, kMfma>();
+    const unsigned dst = lds_at + (s & 1) * kStage;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      if constexpr (decltype(after)::value) {
+        constexpr int kPer = (OpA::kLoads + MB - 1) / MB;
+        constexpr int kPerB = (OpB::kLoads + MB - 1) / MB;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+          if (i * kPer + q < OpA::kLoads) opa.load(a_rows, dst, wave, i * kPer + q);
+#pragma unroll
+        for (int q = 0; q < kPerB; ++q)
+          if (i * kPerB + q < OpB::kLoads)
+            opb.load(b_rows, dst + OpA::kBytes, wave, i * kPerB + q);
+      }
+      multiply(1, i);
+      if constexpr (decltype(next)::value) read(s + 1, 0, i);
       __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (decltype(after)::value) {
+      opa.advance();
+      opb.advance();
+    }
   };
-  if (stages > 1) load(0); else load_last(0);
+  load(0);
   wait_loads();
   __syncthreads();
-  read(0, 0);
-  if (stages > 2) load(1); else if (stages > 1) load_last(1);
-  if constexpr (kSpread) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < MB; ++i) read(0, 0, i);
+  if (stages > 1) load(1);
   int s = 0;
   for (; s + 3 < stages; ++s) stage(s, std::true_type{}, std::true_type{});
 #pragma unroll 1
@@ -620,65 +628,76 @@ __device__ __forceinline__ float slope(float z, int act) {
 }
 
 // dz = dy act'(z) (with a pitch of whole 16 bytes, zeros past a row's end) and the sums of dz over
-// each workgroup's rows. 64 threads a row, 8 columns a thread; 4 rows at a time.
-constexpr int kGradColumns = 512, kGradRows = 4;
-template <typename T>
+// each workgroup's rows, which follow each other. TPR threads a row, 8 columns a thread.
+template <typename T, int TPR>
 __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
-  __shared__ float sums[kGradRows][kGradColumns];
-  const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * kGradColumns + lane * 8;
+  constexpr int kColumns = TPR * 8, kRows = 256 / TPR;
+  __shared__ float sums[kRows][kColumns];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kColumns + lane * 8;
   const int count = n >= a.columns ? 0 : (a.columns - n < 8 ? static_cast<int>(a.columns - n) : 8);
   const T* dy = static_cast<const T*>(a.grad_output);
   const T* pre = static_cast<const T*>(a.pre);
   T* dz = static_cast<T*>(a.grad_pre);
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (count > 0) {
-    const int64_t step = static_cast<int64_t>(gridDim.y) * kGradRows;
-#pragma unroll 2
-    for (int64_t m = static_cast<int64_t>(blockIdx.y) * kGradRows + group; m < a.rows; m += step) {
-      const T* p = dy + m * a.grad_stride + n;
-      const T* q = pre + m * a.columns + n;
-      Run<T, 8> d, z;
-      if (count == 8) {
-        d = load_run<8>(p);
-        if (pre != nullptr) z = load_run<8>(q);
-      } else {
+  auto finish_row = [&](int64_t m, Run<T, 8> d, const Run<T, 8>& z) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d.v[e] = e < count ? p[e] : static_cast<T>(0.f);
-          z.v[e] = pre != nullptr && e < count ? q[e] : static_cast<T>(0.f);
-        }
+    for (int e = 0; e < 8; ++e) {
+      if (pre != nullptr)
+        d.v[e] = static_cast<T>(static_cast<float>(d.v[e]) *
+                                slope(static_cast<float>(z.v[e]), a.activation));
+      // The sums are of dz as the products take it.
+      sum[e] += static_cast<float>(d.v[e]);
+    }
+    if (dz == nullptr) return;
+    T* o = dz + m * a.pitch + n;
+    if (n + 8 <= a.pitch) {
+      store_run<8>(o, d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < a.pitch) o[e] = d.v[e];
+    }
+  };
+  const int64_t first = a.rows * blockIdx.y / gridDim.y, last = a.rows * (blockIdx.y + 1) / gridDim.y;
+  if (count == 8) {
+    // Four rows' loads at a time.
+    int64_t m = first + group;
+    for (; m + 3 * kRows < last; m += 4 * kRows) {
+      Run<T, 8> d[4], z[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        d[u] = load_run<8>(dy + (m + u * kRows) * a.grad_stride + n);
+        if (pre != nullptr) z[u] = load_run<8>(pre + (m + u * kRows) * a.columns + n);
       }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) finish_row(m + u * kRows, d[u], z[u]);
+    }
+    for (; m < last; m += kRows) {
+      const Run<T, 8> d = load_run<8>(dy + m * a.grad_stride + n);
+      finish_row(m, d, pre != nullptr ? load_run<8>(pre + m * a.columns + n) : d);
+    }
+  } else if (count > 0) {
+    for (int64_t m = first + group; m < last; m += kRows) {
+      Run<T, 8> d, z;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (pre != nullptr)
-          d.v[e] = static_cast<T>(static_cast<float>(d.v[e]) *
-                                  slope(static_cast<float>(z.v[e]), a.activation));
-        // The sums are of dz as the products take it.
-        sum[e] += static_cast<float>(d.v[e]);
+        d.v[e] = e < count ? dy[m * a.grad_stride + n + e] : static_cast<T>(0.f);
+        z.v[e] = pre != nullptr && e < count ? pre[m * a.columns + n + e] : static_cast<T>(0.f);
       }
-      if (dz != nullptr) {
-        T* o = dz + m * a.pitch + n;
-        if (n + 8 <= a.pitch) {
-          store_run<8>(o, d);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < a.pitch) o[e] = d.v[e];
-        }
-      }
+      finish_row(m, d, z);
     }
   }
   if (a.partial == nullptr) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) sums[group][lane * 8 + e] = sum[e];
   __syncthreads();
-  for (int c = threadIdx.x; c < kGradColumns; c += 256) {
-    const int64_t column = static_cast<int64_t>(blockIdx.x) * kGradColumns + c;
-    if (column >= a.columns) continue;
+  for (int c = threadIdx.x; c < kColumns; c += 256) {
+    const int64_t column = static_cast<int64_t>(blockIdx.x) * kColumns + c;
+    if (column >= a.columns) break;
     float s = 0.f;
 #pragma unroll
-    for (int r = 0; r < kGradRows; ++r) s += sums[r][c];
+    for (int r = 0; r < kRows; ++r) s += sums[r][c];
     a.partial[blockIdx.y * a.columns + column] = s;
   }
 }
@@ -760,20 +779,20 @@ namespace {
 // Time (us) of `groups` workgroups of a tile over k values of K, from measurements: `wide` of them run
 // side by side, whole turns of the chip take set-up and epilogue plus a time per K value, and a
 // last turn that does not fill every compute unit's places takes less per K value.
-// 16-bit: 256 x 256 alone on a compute unit 26.5 ns a K value (1270 TFLOP/s at 8192^3); 128 x 128
-// two to a compute unit 14.2 (1125), alone 11.9; 64 x 64 five 14.0 (700). float is bound by its MFMA
+// 16-bit: 256 x 256 alone on a compute unit 26 ns a K value (1305 TFLOP/s at 8192^3); 128 x 128
+// two to a compute unit 14.0 (1170), alone 9.8; 64 x 64 five 14.0 (700). float is bound by its MFMA
 // rate at any tile (130 TFLOP/s).
 double tile_time(bool single, int tile, int64_t groups, double k) {
   const double per_cu = static_cast<double>((groups + 255) / 256);
   if (single) return 4.0 + per_cu * k * (tile == 64 ? 0.0162 : 0.0640);
-  if (tile == 256) return per_cu * (6.0 + 0.0265 * k);
+  if (tile == 256) return per_cu * (7.0 + 0.026 * k);
   const int64_t wide = tile == 128 ? 512 : 1280;
   const double set_up = tile == 128 ? 6.0 : 3.0;
   const int64_t rest = groups % wide;
-  double us = static_cast<double>(groups / wide) * (set_up + (tile == 128 ? 0.0142 : 0.0140) * k);
+  double us = static_cast<double>(groups / wide) * (set_up + 0.0140 * k);
   if (rest > 0) {
     const int64_t side = (rest + 255) / 256;
-    us += set_up + (tile == 128 ? (side == 1 ? 0.0119 : 0.0142) : 0.004 + 0.002 * side) * k;
+    us += set_up + (tile == 128 ? (side == 1 ? 0.0098 : 0.0140) : 0.004 + 0.002 * side) * k;
   }
   return us;
 }
@@ -841,25 +860,41 @@ hipError_t launch_linear_pad(convnd_hip_dtype dtype, const void* src, int64_t st
   return hipGetLastError();
 }
 
+namespace {
+
+int grad_threads(int64_t columns) { return columns <= 1024 ? 64 : 256; }
+
+template <typename T>
+void launch_grad(const LinearGradArgs& a, int64_t parts, hipStream_t stream) {
+  const int threads = grad_threads(a.columns);
+  const dim3 grid(static_cast<unsigned>((a.columns + threads * 8 - 1) / (threads * 8)),
+                  static_cast<unsigned>(parts));
+  if (threads == 64)
+    hipLaunchKernelGGL((linear_grad<T, 64>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((linear_grad<T, 256>), grid, dim3(256), 0, stream, a);
+}
+
+}  // namespace
+
 int64_t linear_grad_parts(int64_t rows, int64_t columns) {
-  const int64_t wide = (columns + kGradColumns - 1) / kGradColumns;
-  const int64_t needed = (rows + kGradRows - 1) / kGradRows;
+  const int threads = grad_threads(columns);
+  const int64_t wide = (columns + threads * 8 - 1) / (threads * 8), at_a_time = 256 / threads;
+  const int64_t needed = (rows + at_a_time - 1) / at_a_time;
   return std::max<int64_t>(1, std::min<int64_t>(needed, std::max<int64_t>(1, 1024 / wide)));
 }
 
 hipError_t launch_linear_grad(convnd_hip_dtype dtype, const LinearGradArgs& a, int64_t parts,
                               hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((a.columns + kGradColumns - 1) / kGradColumns),
-                  static_cast<unsigned>(parts));
   switch (dtype) {
     case CONVND_HIP_FLOAT32:
-      hipLaunchKernelGGL(linear_grad<float>, grid, dim3(256), 0, stream, a);
+      launch_grad<float>(a, parts, stream);
       break;
     case CONVND_HIP_FLOAT16:
-      hipLaunchKernelGGL(linear_grad<_Float16>, grid, dim3(256), 0, stream, a);
+      launch_grad<_Float16>(a, parts, stream);
       break;
     case CONVND_HIP_BFLOAT16:
-      hipLaunchKernelGGL(linear_grad<__bf16>, grid, dim3(256), 0, stream, a);
+      launch_grad<__bf16>(a, parts, stream);
       break;
     default:
       return hipErrorInvalidValue;
