@@ -213,13 +213,42 @@ struct Reader {
   }
 };
 
+// 0.5 erfc(|z| / sqrt 2) and exp(-z^2 / 2) for 16-bit results: Abramowitz and Stegun's formula
+// 7.1.26, off by at most 0.75e-7, at a third of erff's instructions (8192 x 1024 -> 4096 with exact
+// GELU 92 -> 79 us). float results take erff.
+struct Normal {
+  float tail, gauss;
+};
+__device__ __forceinline__ Normal gauss_tail(float z) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, fabsf(z), 1.f));
+  const float gauss = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+  float p = fmaf(0.5307027145f, t, -0.7265760135f);
+  p = fmaf(p, t, 0.7107068705f);
+  p = fmaf(p, t, -0.142248368f);
+  p = fmaf(p, t, 0.127414796f);
+  return {p * t * gauss, gauss};
+}
+
+// The normal distribution's Phi(z) (as `tail`: the part below z), and exp(-z^2 / 2).
+template <typename T>
+__device__ __forceinline__ Normal normal(float z) {
+  if constexpr (sizeof(T) == 2) {
+    const Normal q = gauss_tail(z);
+    return {z < 0.f ? q.tail : 1.f - q.tail, q.gauss};
+  } else {
+    return {0.5f * (1.f + erff(z * 0.70710678118654752f)),
+            __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z)};
+  }
+}
+
+template <typename T>
 __device__ __forceinline__ void activate_all(float (&v)[8], int act) {
   if (act == CONVND_HIP_ACT_RELU) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // NaN stays
   } else if (act == CONVND_HIP_ACT_GELU) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.5f * v[e] * (1.f + erff(v[e] * 0.70710678118654752f));
+    for (int e = 0; e < 8; ++e) v[e] *= normal<T>(v[e]).tail;
   } else if (act == CONVND_HIP_ACT_GELU_TANH) {
     // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
 #pragma unroll
@@ -268,7 +297,7 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
         if (e < count) pre[e] = y.v[e];
     }
   }
-  activate_all(v, a.activation);
+  activate_all<T>(v, a.activation);
   if (a.residual != nullptr) {
     const T* residual = static_cast<const T*>(a.residual) + m * a.residual_stride + n;
     if (count == 8) {
@@ -615,11 +644,13 @@ __global__ __launch_bounds__(256) void linear_pad(const T* __restrict__ src, int
   }
 }
 
+template <typename T>
 __device__ __forceinline__ float slope(float z, int act) {
   if (act == CONVND_HIP_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == CONVND_HIP_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
-           z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+  if (act == CONVND_HIP_ACT_GELU) {
+    const auto [phi, gauss] = normal<T>(z);
+    return fmaf(z * 0.39894228040143268f, gauss, phi);
+  }
   // s = sigmoid(2 u): d/dz (z s) = s + 2 z s (1 - s) du/dz
   const float u = 0.79788456080286536f * z * fmaf(0.044715f * z, z, 1.f);
   const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
@@ -645,7 +676,7 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
     for (int e = 0; e < 8; ++e) {
       if (pre != nullptr)
         d.v[e] = static_cast<T>(static_cast<float>(d.v[e]) *
-                                slope(static_cast<float>(z.v[e]), a.activation));
+                                slope<T>(static_cast<float>(z.v[e]), a.activation));
       // The sums are of dz as the products take it.
       sum[e] += static_cast<float>(d.v[e]);
     }

@@ -428,11 +428,13 @@ NormPlan plan_norm(int64_t rows, int64_t channels, int element_size, bool backwa
   const int per_block = p.threads_per_row == 0 ? 1 : threads / std::min(threads, p.threads_per_row);
   const int64_t needed = (rows + per_block - 1) / per_block;
   // The forward fills the chip with rows in flight (32 waves a compute unit: 99 us above, 131 with
-  // 16). Every workgroup of the backward leaves a row of sums to be added up: 16 waves a compute unit
-  // (179 us; 191 with 32), and several rows each (5003 x 769 fp32: 512 workgroups 16 us, 2048 19).
+  // 16). Every workgroup of the backward leaves a row of sums to be added up, so there are as many as
+  // run side by side (20 waves a compute unit by their registers, 16 in workgroups of 8 or 16 waves;
+  // 65536 x 2048 fp16: 162 us with these 1280, 179 with 1024, 188 with 2048; 16384 x 4096 bf16: 95
+  // with these 512, 118 with 768), and several rows each (5003 x 769 fp32: 17 us with 768, 23 with 2560).
   if (backward) {
-    const int64_t most = std::min<int64_t>(262144 / threads, std::max<int64_t>(256, rows / 8));
-    p.blocks = std::min(needed, most);
+    const int64_t resident = 256 * (threads > 256 ? 16 : 20) * 64 / threads;
+    p.blocks = std::min(needed, std::min(resident, std::max<int64_t>(256, rows / 8)));
   } else {
     p.blocks = std::min<int64_t>(needed, 524288 / threads);
   }
