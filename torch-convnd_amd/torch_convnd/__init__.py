@@ -25,6 +25,7 @@ from .modules import (
 )
 from .partial import PartialConvOutput, partial_conv_nd
 from .sequence import gated_recurrence, layer_norm, linear_act
+from .sequence_modules import GatedConvBlock, LayerNorm, LinearAct
 
 ensure_native_definitions()
 ensure_compatible_operator()
@@ -35,6 +36,9 @@ __all__ = [
     "Conv3d",
     "Conv4d",
     "ConvNd",
+    "GatedConvBlock",
+    "LayerNorm",
+    "LinearAct",
     "PartialConv1d",
     "PartialConv2d",
     "PartialConv3d",
