@@ -840,25 +840,28 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
     return p;
   }
   const bool single = dtype == CONVND_HIP_FLOAT32;
-  const int64_t stage = single ? 32 : 64;
+  const int64_t stage = single ? 32 : 64, stages = (k + stage - 1) / stage;
   double best = 0;
+  // A few splits only: this runs on every call.
+  constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
   for (int tile : {64, 128, 256}) {
     if (tile == 256 && single) continue;
     const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-    for (int64_t splits = 1; splits <= 32; ++splits) {
-      const int64_t split_k = ((k + splits - 1) / splits + stage - 1) / stage * stage;
-      if ((k + split_k - 1) / split_k != splits || (splits > 1 && split_k < 4 * stage)) continue;
-      double us = tile_time(single, tile, tiles * splits, static_cast<double>(std::min(split_k, k)));
+    for (int splits : kSplits) {
+      const int64_t each = (stages + splits - 1) / splits;
+      if (splits > 1 && (each < 4 || each * (splits - 1) >= stages)) break;
+      double us = tile_time(single, tile, tiles * splits, static_cast<double>(each * stage));
       // The splits' sums are written, read and joined (through the last cache level at 7 TB/s).
       if (splits > 1) us += 3.0 + static_cast<double>(m) * n * (4.0 * splits + 2.0) / 7e6;
       if (best == 0 || us < best) {
         best = us;
         p.tile = tile;
-        p.splits = static_cast<int>(splits);
-        p.split_k = split_k;
+        p.splits = splits;
+        p.split_k = each * stage;
       }
     }
   }
+  if (p.splits == 1) p.split_k = k;
   return p;
 }
 
