@@ -342,7 +342,7 @@ typedef struct convnd_hip_recurrence_problem {
  * [batch, this, channels]. */
 int64_t convnd_hip_recurrence_carries(int64_t tokens);
 
-/* Device scratch bytes of the two calls below (often 0). */
+/* Device scratch bytes of the two calls below (often 0), aligned to 8 bytes. */
 size_t convnd_hip_recurrence_workspace_size(convnd_hip_dtype dtype,
                                             const convnd_hip_recurrence_problem* problem);
 

@@ -45,10 +45,38 @@ def test_sizes(batch, tokens, c, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize(("batch", "tokens", "c"), [(1, 2500, 70), (2, 1025, 64), (1, 5000, 3)])
-def test_split_token_axis(batch, tokens, c, dtype):
-    """Few channels and many tokens: the token axis is split over workgroups."""
+@pytest.mark.parametrize(("batch", "tokens", "c"), [(1, 2500, 70), (2, 1025, 64), (1, 5000, 3), (3, 9000, 131)])
+def test_chunks_of_the_token_axis(batch, tokens, c, dtype):
+    """Few channels and many tokens: workgroups take chunks of the token axis, several groups of them."""
     check(*make(batch, tokens, c, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_chunks_with_lengths_and_closed_gates(dtype):
+    """Lengths around the chunks' edges, documents that start there, and the same bits every time."""
+    x, gate, first, dy, dlast = make(6, 4200, 33, dtype)
+    lengths = torch.tensor([4200, 0, 256, 2049, 4097, 63], device="cuda")
+    for t in (0, 63, 64, 255, 256, 2048, 4096):
+        gate[:, t, ::2] = -float("inf")
+    h, last, grads = check(x, gate, first, dy, dlast, lengths)
+    for _ in range(3):
+        again = check(x, gate, first, dy, dlast, lengths)
+        for got, want in zip((again[0], again[1], *again[2]), (h, last, *grads)):
+            assert torch.equal(got, want)
+
+
+def test_chunks_of_infinities():
+    """A non-finite state goes on to the tokens after it, of its channel only."""
+    x, gate, first, dy, dlast = make(1, 3000, 64, torch.float32)
+    clean, _ = gated_recurrence(x, gate, first)
+    x[0, 1500, 7] = float("inf")
+    x[0, 10, 9] = float("nan")
+    h, last = gated_recurrence(x, gate, first)
+    others = [c for c in range(64) if c not in (7, 9)]
+    assert torch.equal(h[..., others], clean[..., others])
+    assert torch.equal(h[:, :1500, 7], clean[:, :1500, 7]) and not torch.isfinite(h[:, 1500:, 7]).any()
+    assert torch.equal(h[:, :10, 9], clean[:, :10, 9]) and h[:, 10:, 9].isnan().all()
+    assert torch.isfinite(last[:, others]).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -619,24 +619,24 @@ struct RecurrenceArgs {
   void* grad_input;           // [batch, tokens, channels]
   void* grad_gate;
   float* grad_first;          // [batch, channels] or null
-  float* summary;             // [batch, splits, 2, channels] where splits > 1
+  void* words;                // workspace of the chunks, word_count 8-byte words
+  int64_t word_count;
   int64_t batch, tokens, channels;
   int64_t input_batch, input_token, gate_batch, gate_token, grad_batch, grad_token;
-  int64_t split_tokens;       // tokens of one split (whole tiles)
-  int splits;
   int wide_lengths;           // lengths are int64
 };
 struct RecurrencePlan {
   int waves;              // of a workgroup: 1 or 8
   int channels_per_lane;  // 1 or 2
   int lanes;              // of a wave along the channels: 64, 32 or 16
-  int splits;
-  int64_t split_tokens;
+  bool chain;             // chunks of the token axis instead
+  int64_t word_count;     // their workspace in 8-byte words
+  int64_t workgroups;
 };
-// Distance of the saved states in tokens: every plan's tiles start at whole multiples of it (or
-// are a single one).
+// Distance of the saved states in tokens: every plan's tiles and chunks start at whole multiples of
+// it (or are a single one).
 constexpr int kRecurrenceTile = 64;
-RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a);
+RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward);
 hipError_t launch_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward,
                              const RecurrencePlan& p, hipStream_t stream);
 

@@ -19,10 +19,8 @@
 //     meanwhile. Fewer channels make more workgroups of the same problem.
 //   * Rows are addressed as buffers with a 32-bit lane offset, the tile's end being the buffer's:
 //     64-bit row addresses cost more than the arithmetic (8 x 2048 x 1024 bf16 backward 51 -> 44 us).
-//   * Where there are still few, the token axis is split over workgroups: a first launch leaves
-//     every split's map, the second composes the maps before its split and goes on as above (it
-//     reads the inputs again; the first walks each split from the end the second comes to last, so
-//     that what is read again first is what was read last).
+//   * With few sequences and channels and many tokens, workgroups take chunks of the token axis
+//     instead and hand the state on (below).
 // Every sum is in fp32 and in a fixed order; 1 - a is computed as sigmoid(-gate), which keeps its
 // relative precision where a is near 1.
 
@@ -35,7 +33,8 @@
 namespace convnd {
 namespace {
 
-constexpr int kRun = 8;  // tokens of a run
+constexpr int kRun = 8;    // tokens of a run
+constexpr int kWaves = 8;  // of a workgroup
 
 struct Gate {
   float keep, take;  // sigmoid(g), sigmoid(-g)
@@ -98,19 +97,17 @@ __device__ __forceinline__ void scan_runs(Map<CPL>& m, Map<CPL>& before) {
 // The place of this workgroup and lane in the problem.
 template <int CPL, int LANES>
 struct Place {
-  int64_t batch, length, begin, end;  // tokens [begin, end) of the split
-  int split, channel;  // the lane's first channel, or the last whole one past the edge
+  int64_t batch, length;
+  int channel;  // the lane's first, or the last whole one past the edge
   bool valid;
   __device__ __forceinline__ explicit Place(const RecurrenceArgs& a) {
     const int strips = static_cast<int>((a.channels + LANES * CPL - 1) / (LANES * CPL));
     // Workgroup ids go round the eight XCDs: neighbouring strips, whose row segments may share a
     // cache line, are given to the same one.
     const unsigned per = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
-    unsigned id = xcd * per + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+    const unsigned id = xcd * per + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
     const int strip = static_cast<int>(id % strips);
-    id /= strips;
-    split = static_cast<int>(id % a.splits);
-    batch = id / a.splits;
+    batch = id / strips;
     const int C = static_cast<int>(a.channels);
     const int own = (strip * LANES + static_cast<int>(threadIdx.x) % LANES) * CPL;
     valid = own < C;
@@ -121,15 +118,14 @@ struct Place {
                                        : static_cast<const int32_t*>(a.lengths)[batch];
       length = n < 0 ? 0 : (n < a.tokens ? n : a.tokens);
     }
-    begin = split * a.split_tokens;
-    end = begin + a.split_tokens < a.tokens ? begin + a.split_tokens : a.tokens;
   }
 };
 
-// The lane's tokens of a tile before `stop`, 0 to kRun, given the tile's first token.
+// The lane's tokens of a tile before `stop`, 0 to N, given the tile's first token.
+template <int N = kRun>
 __device__ __forceinline__ int tokens_before(int64_t tile, int run_token, int64_t stop) {
   const int64_t n = stop - tile - run_token;
-  return n <= 0 ? 0 : (n < kRun ? static_cast<int>(n) : kRun);
+  return n <= 0 ? 0 : (n < N ? static_cast<int>(n) : N);
 }
 
 // The rows of a tile before token `stop` as a buffer: reads past it give zeros, writes are dropped.
@@ -143,14 +139,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const T* base, int64
                                            static_cast<int>(bytes), 0x00020000);
 }
 
-// kRun tokens of the lane's channels, `step` bytes apart.
-template <typename T, int CPL>
-__device__ __forceinline__ void load_tokens(Run<T, CPL> (&r)[kRun], __amdgpu_buffer_rsrc_t rows,
+// N tokens of the lane's channels, `step` bytes apart.
+template <typename T, int CPL, int N>
+__device__ __forceinline__ void load_tokens(Run<T, CPL> (&r)[N], __amdgpu_buffer_rsrc_t rows,
                                             unsigned offset, unsigned step) {
-  // Hidden, so that the kRun offsets are added up here and not kept over the loop of tiles.
+  // Hidden, so that the N offsets are added up here and not kept over the loop of tiles.
   asm volatile("" : "+v"(offset));
 #pragma unroll
-  for (int i = 0; i < kRun; ++i, offset += step) {
+  for (int i = 0; i < N; ++i, offset += step) {
     if constexpr (sizeof(T) * CPL == 4)
       r[i] = __builtin_bit_cast(Run<T, CPL>,
                                 __builtin_amdgcn_raw_buffer_load_b32(rows, offset, 0, 0));
@@ -160,12 +156,12 @@ __device__ __forceinline__ void load_tokens(Run<T, CPL> (&r)[kRun], __amdgpu_buf
   }
 }
 
-template <typename T, int CPL>
+template <typename T, int CPL, int N>
 __device__ __forceinline__ void store_tokens(__amdgpu_buffer_rsrc_t rows, unsigned offset,
-                                             unsigned step, const float (&v)[kRun][CPL]) {
+                                             unsigned step, const float (&v)[N][CPL]) {
   asm volatile("" : "+v"(offset));
 #pragma unroll
-  for (int i = 0; i < kRun; ++i, offset += step) {
+  for (int i = 0; i < N; ++i, offset += step) {
     Run<T, CPL> r;
 #pragma unroll
     for (int j = 0; j < CPL; ++j) r.v[j] = static_cast<T>(v[i][j]);
@@ -178,17 +174,17 @@ __device__ __forceinline__ void store_tokens(__amdgpu_buffer_rsrc_t rows, unsign
 }
 
 // From token `live` on, `fill`.
-template <typename T, int CPL>
-__device__ __forceinline__ void fill_tokens(Run<T, CPL> (&r)[kRun], int live, float fill) {
+template <typename T, int CPL, int N>
+__device__ __forceinline__ void fill_tokens(Run<T, CPL> (&r)[N], int live, float fill) {
 #pragma unroll
-  for (int i = 0; i < kRun; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < CPL; ++j) r[i].v[j] = i < live ? r[i].v[j] : static_cast<T>(fill);
 }
-template <int CPL>
-__device__ __forceinline__ void clear_tokens(float (&v)[kRun][CPL], int live) {
+template <int CPL, int N>
+__device__ __forceinline__ void clear_tokens(float (&v)[N][CPL], int live) {
 #pragma unroll
-  for (int i = 0; i < kRun; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < CPL; ++j) v[i][j] = i < live ? v[i][j] : 0.f;
 }
@@ -213,11 +209,10 @@ __device__ __forceinline__ void hold(Run<T, 2>& r) {
 template <typename T>
 __device__ __forceinline__ void hold(Run<T, 1>&) {}
 
-// kSummary: only the split's map is left, in a.summary.
-template <typename T, int CPL, int LANES, int NW, bool kSummary>
-__global__ __launch_bounds__(64 * NW) void recurrence_forward(RecurrenceArgs a) {
-  constexpr int kTile = NW * (64 / LANES) * kRun;
-  __shared__ float maps[2][NW][2][LANES * CPL];
+template <typename T, int CPL, int LANES>
+__global__ __launch_bounds__(64 * kWaves) void recurrence_forward(RecurrenceArgs a) {
+  constexpr int kTile = kWaves * (64 / LANES) * kRun;
+  __shared__ float maps[2][kWaves][2][LANES * CPL];
   const Place<CPL, LANES> at(a);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -231,36 +226,19 @@ __global__ __launch_bounds__(64 * NW) void recurrence_forward(RecurrenceArgs a) 
   const unsigned g_lane = lane_offset<T>(run_token, a.gate_token, at.channel);
   const unsigned y_lane = at.valid ? lane_offset<T>(run_token, C, at.channel) : kNowhere;
   float carry[CPL];  // the state before the tile
-  Map<CPL> total;    // the split's map (kSummary)
-  total.clear();
 #pragma unroll
-  for (int j = 0; j < CPL; ++j) carry[j] = 0.f;
-  if constexpr (!kSummary) {
-    if (a.first != nullptr) {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) carry[j] = a.first[at.batch * C + at.channel + j];
-    }
-    const float* sum = a.summary + at.batch * a.splits * 2 * C + at.channel;
-#pragma unroll 8
-    for (int s = 0; s < at.split; ++s, sum += 2 * C) {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) carry[j] = fmaf(sum[j], carry[j], sum[C + j]);
-    }
-  }
+  for (int j = 0; j < CPL; ++j)
+    carry[j] = a.first != nullptr ? a.first[at.batch * C + at.channel + j] : 0.f;
   Run<T, CPL> nx[kRun], ng[kRun];
   auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
-    load_tokens<T, CPL>(ng, tile_rows<kTile>(g, tile, at.length, a.gate_token, C), g_lane,
-                        static_cast<unsigned>(a.gate_token) * sizeof(T));
-    load_tokens<T, CPL>(nx, tile_rows<kTile>(x, tile, at.length, a.input_token, C), x_lane,
-                        static_cast<unsigned>(a.input_token) * sizeof(T));
+    load_tokens(ng, tile_rows<kTile>(g, tile, at.length, a.gate_token, C), g_lane,
+                static_cast<unsigned>(a.gate_token) * sizeof(T));
+    load_tokens(nx, tile_rows<kTile>(x, tile, at.length, a.input_token, C), x_lane,
+                static_cast<unsigned>(a.input_token) * sizeof(T));
   };
-  const int64_t count = at.end > at.begin ? (at.end - at.begin + kTile - 1) / kTile : 0;
-  // The summary goes from the last tile to the first.
-  int64_t tile = kSummary ? at.begin + (count - 1) * kTile : at.begin;
-  constexpr int64_t kNext = kSummary ? -kTile : kTile;
-  if (count > 0) fetch(tile);
+  fetch(0);
   int buffer = 0;
-  for (int64_t n = 0; n < count; ++n, tile += kNext, buffer ^= 1) {
+  for (int64_t tile = 0; tile < a.tokens; tile += kTile, buffer ^= 1) {
     float keep[kRun][CPL], add[kRun][CPL];
     Map<CPL> map, before;
     map.clear();
@@ -278,83 +256,56 @@ __global__ __launch_bounds__(64 * NW) void recurrence_forward(RecurrenceArgs a) 
         map.a[j] *= q.keep;
         map.b[j] = fmaf(q.keep, map.b[j], add[i][j]);
       }
-    if (n + 1 < count) fetch(tile + kNext);
+    if (tile + kTile < a.tokens) fetch(tile + kTile);
     scan_runs<CPL, LANES, true>(map, before);
     float h[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; ++j) h[j] = carry[j];
-    if constexpr (NW > 1) {
-      if (lane >= 64 - LANES) {
+    if (lane >= 64 - LANES) {
 #pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-          maps[buffer][wave][0][slot + j] = map.a[j];
-          maps[buffer][wave][1][slot + j] = map.b[j];
-        }
+      for (int j = 0; j < CPL; ++j) {
+        maps[buffer][wave][0][slot + j] = map.a[j];
+        maps[buffer][wave][1][slot + j] = map.b[j];
       }
-      __syncthreads();
-      Map<CPL> whole;
-      whole.clear();
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-          const float aw = maps[buffer][w][0][slot + j], bw = maps[buffer][w][1][slot + j];
-          if constexpr (kSummary) {
-            whole.b[j] = fmaf(aw, whole.b[j], bw);
-            whole.a[j] *= aw;
-          } else {
-            if (w == wave) h[j] = carry[j];
-            carry[j] = fmaf(aw, carry[j], bw);
-          }
-        }
-      }
-      if constexpr (kSummary) total.after(whole);  // the tiles before this one came later
-    } else {
-      static_assert(NW > 1 || (LANES == 64 && !kSummary), "one wave takes one run, without splits");
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) carry[j] = fmaf(map.a[j], carry[j], map.b[j]);
     }
-    if constexpr (!kSummary) {
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < CPL; ++j) h[j] = fmaf(before.a[j], h[j], before.b[j]);
-      const int64_t first = tile + run_token;
-      if (a.carries != nullptr && at.valid && first % kRecurrenceTile == 0 && first < at.end) {
-        const int64_t tiles = (a.tokens + kRecurrenceTile - 1) / kRecurrenceTile;
-        float* c = a.carries + (at.batch * tiles + first / kRecurrenceTile) * C + at.channel;
+    for (int w = 0; w < kWaves; ++w)
 #pragma unroll
-        for (int j = 0; j < CPL; ++j) c[j] = h[j];
+      for (int j = 0; j < CPL; ++j) {
+        if (w == wave) h[j] = carry[j];
+        carry[j] = fmaf(maps[buffer][w][0][slot + j], carry[j], maps[buffer][w][1][slot + j]);
       }
 #pragma unroll
-      for (int i = 0; i < kRun; ++i)
+    for (int j = 0; j < CPL; ++j) h[j] = fmaf(before.a[j], h[j], before.b[j]);
+    const int64_t first = tile + run_token;
+    if (a.carries != nullptr && at.valid && first % kRecurrenceTile == 0 && first < a.tokens) {
+      const int64_t tiles = (a.tokens + kRecurrenceTile - 1) / kRecurrenceTile;
+      float* c = a.carries + (at.batch * tiles + first / kRecurrenceTile) * C + at.channel;
 #pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-          h[j] = fmaf(keep[i][j], h[j], add[i][j]);
-          keep[i][j] = h[j];
-        }
-      if (cut) clear_tokens(keep, live);
-      store_tokens<T, CPL>(tile_rows<kTile>(y, tile, at.end, C, C), y_lane,
-                           static_cast<unsigned>(C) * sizeof(T), keep);
+      for (int j = 0; j < CPL; ++j) c[j] = h[j];
     }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        h[j] = fmaf(keep[i][j], h[j], add[i][j]);
+        keep[i][j] = h[j];
+      }
+    if (cut) clear_tokens(keep, live);
+    store_tokens<T, CPL>(tile_rows<kTile>(y, tile, a.tokens, C, C), y_lane,
+                         static_cast<unsigned>(C) * sizeof(T), keep);
   }
   if (threadIdx.x >= LANES || !at.valid) return;
-  if constexpr (kSummary) {
-    float* sum = a.summary + (at.batch * a.splits + at.split) * 2 * C + at.channel;
 #pragma unroll
-    for (int j = 0; j < CPL; ++j) {
-      sum[j] = total.a[j];
-      sum[C + j] = total.b[j];
-    }
-  } else if (at.split == a.splits - 1) {
-#pragma unroll
-    for (int j = 0; j < CPL; ++j) a.last[at.batch * C + at.channel + j] = carry[j];
-  }
+  for (int j = 0; j < CPL; ++j) a.last[at.batch * C + at.channel + j] = carry[j];
 }
 
-// The backward walks the tiles from the last. kSummary: only the split's map of E is left.
-template <typename T, int CPL, int LANES, int NW, bool kSummary>
+// The backward walks the tiles from the last.
+template <typename T, int CPL, int LANES, int NW>
 __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a) {
   constexpr int kTile = NW * (64 / LANES) * kRun;
-  __shared__ float maps[2][NW][kSummary ? 2 : 3][LANES * CPL];
+  __shared__ float maps[2][NW][3][LANES * CPL];
   const Place<CPL, LANES> at(a);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -372,44 +323,26 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
   const unsigned out_lane = at.valid ? lane_offset<T>(run_token, C, at.channel) : kNowhere;
   const int64_t tiles = (a.tokens + kRecurrenceTile - 1) / kRecurrenceTile;
   float carry[CPL];  // E after the tile
-  Map<CPL> total;    // the split's map (kSummary)
-  total.clear();
 #pragma unroll
-  for (int j = 0; j < CPL; ++j) carry[j] = 0.f;
-  if constexpr (!kSummary) {
-    if (a.grad_last != nullptr) {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) carry[j] = a.grad_last[at.batch * C + at.channel + j];
-    }
-    const float* sum = a.summary + ((at.batch + 1) * a.splits - 1) * 2 * C + at.channel;
-#pragma unroll 8
-    for (int s = a.splits - 1; s > at.split; --s, sum -= 2 * C) {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) carry[j] = fmaf(sum[j], carry[j], sum[C + j]);
-    }
-  }
+  for (int j = 0; j < CPL; ++j)
+    carry[j] = a.grad_last != nullptr ? a.grad_last[at.batch * C + at.channel + j] : 0.f;
   Run<T, CPL> nx[kRun], ng[kRun], nd[kRun];
   float nh[CPL];  // the state before the tile
   auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
-    load_tokens<T, CPL>(ng, tile_rows<kTile>(g, tile, at.length, a.gate_token, C), g_lane,
-                        static_cast<unsigned>(a.gate_token) * sizeof(T));
-    load_tokens<T, CPL>(nd, tile_rows<kTile>(dy, tile, at.length, a.grad_token, C), d_lane,
-                        static_cast<unsigned>(a.grad_token) * sizeof(T));
-    if constexpr (!kSummary) {
-      load_tokens<T, CPL>(nx, tile_rows<kTile>(x, tile, at.length, a.input_token, C), x_lane,
-                          static_cast<unsigned>(a.input_token) * sizeof(T));
-      const float* c = a.carries + (at.batch * tiles + tile / kRecurrenceTile) * C + at.channel;
+    load_tokens(ng, tile_rows<kTile>(g, tile, at.length, a.gate_token, C), g_lane,
+                static_cast<unsigned>(a.gate_token) * sizeof(T));
+    load_tokens(nd, tile_rows<kTile>(dy, tile, at.length, a.grad_token, C), d_lane,
+                static_cast<unsigned>(a.grad_token) * sizeof(T));
+    load_tokens(nx, tile_rows<kTile>(x, tile, at.length, a.input_token, C), x_lane,
+                static_cast<unsigned>(a.input_token) * sizeof(T));
+    const float* c = a.carries + (at.batch * tiles + tile / kRecurrenceTile) * C + at.channel;
 #pragma unroll
-      for (int j = 0; j < CPL; ++j) nh[j] = c[j];
-    }
+    for (int j = 0; j < CPL; ++j) nh[j] = c[j];
   };
-  const int64_t count = at.end > at.begin ? (at.end - at.begin + kTile - 1) / kTile : 0;
-  // The summary goes from the first tile to the last.
-  int64_t tile = kSummary ? at.begin : at.begin + (count - 1) * kTile;
-  constexpr int64_t kNext = kSummary ? kTile : -kTile;
-  if (count > 0) fetch(tile);
+  int64_t tile = (a.tokens - 1) / kTile * kTile;
+  if (a.tokens > 0) fetch(tile);
   int buffer = 0;
-  for (int64_t n = 0; n < count; ++n, tile += kNext, buffer ^= 1) {
+  for (; a.tokens > 0 && tile >= 0; tile -= kTile, buffer ^= 1) {
     float keep[kRun][CPL], take[kRun][CPL];
     Run<T, CPL> cx[kRun], cd[kRun];  // this tile's x and dy, as loaded
     Map<CPL> states, states_before, grads, grads_before;
@@ -420,7 +353,7 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
     const int live = tokens_before(tile, run_token, at.length);
     if (cut) fill_tokens(ng, live, __builtin_inff());
 #pragma unroll
-    for (int j = 0; j < CPL; ++j) h[j] = kSummary ? 0.f : nh[j];
+    for (int j = 0; j < CPL; ++j) h[j] = nh[j];
 #pragma unroll
     for (int i = 0; i < kRun; ++i)
 #pragma unroll
@@ -428,10 +361,8 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
         const Gate q = open_gate(static_cast<float>(ng[i].v[j]));
         keep[i][j] = q.keep;
         states.a[j] *= q.keep;
-        if constexpr (!kSummary) {
-          take[i][j] = q.take;
-          states.b[j] = fmaf(q.keep, states.b[j], q.take * static_cast<float>(nx[i].v[j]));
-        }
+        take[i][j] = q.take;
+        states.b[j] = fmaf(q.keep, states.b[j], q.take * static_cast<float>(nx[i].v[j]));
       }
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i)
@@ -440,13 +371,13 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       cd[i] = nd[i];
-      if constexpr (!kSummary) cx[i] = nx[i];
+      cx[i] = nx[i];
     }
 #pragma unroll
     for (int j = 0; j < CPL; ++j) grads.a[j] = states.a[j];
-    if (n + 1 < count) fetch(tile + kNext);
+    if (tile > 0) fetch(tile - kTile);
     scan_runs<CPL, LANES, false>(grads, grads_before);
-    if constexpr (!kSummary) scan_runs<CPL, LANES, true>(states, states_before);
+    scan_runs<CPL, LANES, true>(states, states_before);
 #pragma unroll
     for (int j = 0; j < CPL; ++j) e[j] = carry[j];
     if constexpr (NW > 1) {
@@ -458,93 +389,492 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
           maps[buffer][wave][1][slot + j] = grads.b[j];
         }
       }
-      if constexpr (!kSummary) {
-        if (lane >= 64 - LANES) {
+      if (lane >= 64 - LANES) {
 #pragma unroll
-          for (int j = 0; j < CPL; ++j) maps[buffer][wave][2][slot + j] = states.b[j];
-        }
+        for (int j = 0; j < CPL; ++j) maps[buffer][wave][2][slot + j] = states.b[j];
       }
       __syncthreads();
-      Map<CPL> whole;
-      whole.clear();
 #pragma unroll
       for (int w = NW - 1; w >= 0; --w)
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-          const float aw = maps[buffer][w][0][slot + j], bw = maps[buffer][w][1][slot + j];
-          if constexpr (kSummary) {
-            whole.b[j] = fmaf(aw, whole.b[j], bw);
-            whole.a[j] *= aw;
-          } else {
-            if (w == wave) e[j] = carry[j];
-            carry[j] = fmaf(aw, carry[j], bw);
-          }
+          if (w == wave) e[j] = carry[j];
+          carry[j] = fmaf(maps[buffer][w][0][slot + j], carry[j], maps[buffer][w][1][slot + j]);
         }
-      if constexpr (kSummary) {
-        total.after(whole);
-      } else {
 #pragma unroll
-        for (int w = 0; w < NW - 1; ++w)
+      for (int w = 0; w < NW - 1; ++w)
 #pragma unroll
-          for (int j = 0; j < CPL; ++j)
-            if (w < wave)
-              h[j] = fmaf(maps[buffer][w][0][slot + j], h[j], maps[buffer][w][2][slot + j]);
-      }
+        for (int j = 0; j < CPL; ++j)
+          if (w < wave)
+            h[j] = fmaf(maps[buffer][w][0][slot + j], h[j], maps[buffer][w][2][slot + j]);
     } else {
-      static_assert(NW > 1 || (LANES == 64 && !kSummary), "one wave takes one run, without splits");
+      static_assert(NW > 1 || LANES == 64, "a single wave takes one run");
 #pragma unroll
       for (int j = 0; j < CPL; ++j) carry[j] = fmaf(grads.a[j], carry[j], grads.b[j]);
     }
-    if constexpr (!kSummary) {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) {
-        h[j] = fmaf(states_before.a[j], h[j], states_before.b[j]);
-        e[j] = fmaf(grads_before.a[j], e[j], grads_before.b[j]);
-      }
-      // slope is (h_before - x) a (1 - a), then dgate; take becomes dx.
-      float slope[kRun][CPL];
-#pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        hold(cx[i]);
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-          const float xi = static_cast<float>(cx[i].v[j]);
-          slope[i][j] = (h[j] - xi) * (keep[i][j] * take[i][j]);
-          h[j] = fmaf(keep[i][j], h[j], take[i][j] * xi);
-        }
-      }
-#pragma unroll
-      for (int i = kRun - 1; i >= 0; --i) {
-        hold(cd[i]);
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-          const float d = static_cast<float>(cd[i].v[j]) + e[j];
-          e[j] = keep[i][j] * d;
-          take[i][j] *= d;
-          slope[i][j] *= d;
-        }
-      }
-      if (cut) {
-        clear_tokens(take, live);
-        clear_tokens(slope, live);
-      }
-      const unsigned step = static_cast<unsigned>(C) * sizeof(T);
-      store_tokens<T, CPL>(tile_rows<kTile>(dx, tile, at.end, C, C), out_lane, step, take);
-      store_tokens<T, CPL>(tile_rows<kTile>(dg, tile, at.end, C, C), out_lane, step, slope);
-    }
-  }
-  if (threadIdx.x >= LANES || !at.valid) return;
-  if constexpr (kSummary) {
-    float* sum = a.summary + (at.batch * a.splits + at.split) * 2 * C + at.channel;
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
-      sum[j] = total.a[j];
-      sum[C + j] = total.b[j];
+      h[j] = fmaf(states_before.a[j], h[j], states_before.b[j]);
+      e[j] = fmaf(grads_before.a[j], e[j], grads_before.b[j]);
     }
-  } else if (at.split == 0 && a.grad_first != nullptr) {
+    // slope is (h_before - x) a (1 - a), then dgate; take becomes dx.
+    float slope[kRun][CPL];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      hold(cx[i]);
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        const float xi = static_cast<float>(cx[i].v[j]);
+        slope[i][j] = (h[j] - xi) * (keep[i][j] * take[i][j]);
+        h[j] = fmaf(keep[i][j], h[j], take[i][j] * xi);
+      }
+    }
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {
+      hold(cd[i]);
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        const float d = static_cast<float>(cd[i].v[j]) + e[j];
+        e[j] = keep[i][j] * d;
+        take[i][j] *= d;
+        slope[i][j] *= d;
+      }
+    }
+    if (cut) {
+      clear_tokens(take, live);
+      clear_tokens(slope, live);
+    }
+    const unsigned step = static_cast<unsigned>(C) * sizeof(T);
+    store_tokens<T, CPL>(tile_rows<kTile>(dx, tile, a.tokens, C, C), out_lane, step, take);
+    store_tokens<T, CPL>(tile_rows<kTile>(dg, tile, a.tokens, C, C), out_lane, step, slope);
+  }
+  if (threadIdx.x >= LANES || !at.valid) return;
+  if (a.grad_first != nullptr) {
 #pragma unroll
     for (int j = 0; j < CPL; ++j) a.grad_first[at.batch * C + at.channel + j] = carry[j];
   }
+}
+
+// ---- few sequences and channels: chunks of the token axis in one pass ------------------------------
+//
+// A workgroup takes a chunk of a strip's tokens, holds it in registers, leaves the chunk's map (A, B) in
+// the workspace, composes the maps of the chunks before it in its group of kGroup with the state at
+// the group's start, and finishes its tokens. The group's last chunk leaves the next group's state.
+// So the inputs are read once, and what runs along the token axis is one hand-over a group, while
+// many groups' chunks load and store. The maps are always composed in token order: the result does
+// not depend on who came first.
+//
+// Every wait ends: a workgroup takes its chunk from a counter when it starts, chunks of earlier
+// tokens first, so all that it waits for belongs to workgroups that have started, and those wait only
+// for earlier ones still (a map is left before any wait). Should a word not come all the same, a
+// wait gives up after kPatience looks and the state becomes NaN.
+//
+// A map or state is one 8-byte word, written and read whole by relaxed device-scope atomics, which
+// pass the caches of the eight XCDs; it needs no order to anything else. Words are complemented:
+// zero, to which a small kernel sets the workspace, is "not there yet", and the one value that would
+// come out as zero (two NaNs of all ones) is replaced by another pair of NaNs.
+
+constexpr int kGroup = 32;       // chunks of a group
+constexpr int kPatience = 1 << 20;
+// Tokens of a wave's run, times the channels of a lane.
+constexpr int kForwardRun = 32, kBackwardRun = 16;
+
+using Word = unsigned long long;
+
+__device__ __forceinline__ void leave_word(Word* at, float a, float b) {
+  Word w = (static_cast<Word>(__builtin_bit_cast(unsigned, b)) << 32) | __builtin_bit_cast(unsigned, a);
+  w = w == ~Word{0} ? ~Word{1} : w;
+  __hip_atomic_store(at, ~w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// CPL words of a lane, once all lanes of the wave have theirs.
+template <int CPL>
+__device__ __forceinline__ void await_words(const Word* at, float (&a)[CPL], float (&b)[CPL]) {
+  Word w[CPL];
+  for (int look = 0;; ++look) {
+    bool there = true;
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      w[j] = __hip_atomic_load(at + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      there = there && w[j] != 0;
+    }
+    if (__all(there) || look == kPatience) break;
+    __builtin_amdgcn_s_sleep(2);
+  }
+#pragma unroll
+  for (int j = 0; j < CPL; ++j) {
+    const Word v = ~w[j];  // of a word that never came: NaN, NaN
+    a[j] = __builtin_bit_cast(float, static_cast<unsigned>(v));
+    b[j] = __builtin_bit_cast(float, static_cast<unsigned>(v >> 32));
+  }
+}
+
+// Words of the workspace: the counter (the first of kChainHead), the groups' first states
+// [rows][groups][64 CPL], the chunks' maps [rows][chunks][64 CPL]; a row is a strip of a sequence.
+constexpr int64_t kChainHead = 8;
+
+// What a ticket stands for: chunk `chunk` (counted in the direction of the walk) of a strip of a
+// sequence.
+template <int CPL, int kChunk>
+struct ChainPlace {
+  unsigned rows, chunks, groups, chunk, row, group, place;
+  int64_t batch, length;
+  int channel;  // the lane's first, or the last whole one past the edge
+  bool valid;
+  __device__ __forceinline__ ChainPlace(const RecurrenceArgs& a, unsigned ticket) {
+    constexpr int kWide = 64 * CPL;
+    const int C = static_cast<int>(a.channels);
+    const unsigned strips = static_cast<unsigned>((C + kWide - 1) / kWide);
+    rows = strips * static_cast<unsigned>(a.batch);
+    chunks = static_cast<unsigned>((a.tokens + kChunk - 1) / kChunk);
+    groups = (chunks + kGroup - 1) / kGroup;
+    chunk = ticket / rows;
+    row = ticket - chunk * rows;
+    group = chunk / kGroup;
+    place = chunk - group * kGroup;
+    batch = row / strips;
+    const int own = static_cast<int>(row % strips) * kWide + static_cast<int>(threadIdx.x & 63) * CPL;
+    valid = own < C;
+    channel = valid ? own : C - CPL;
+    length = a.tokens;
+    if (a.lengths != nullptr) {
+      const int64_t n = a.wide_lengths ? static_cast<const int64_t*>(a.lengths)[batch]
+                                       : static_cast<const int32_t*>(a.lengths)[batch];
+      length = n < 0 ? 0 : (n < a.tokens ? n : a.tokens);
+    }
+  }
+  __device__ __forceinline__ Word* states(Word* words) const {
+    return words + kChainHead + static_cast<int64_t>(row) * groups * (64 * CPL);
+  }
+  __device__ __forceinline__ Word* left(Word* words) const {
+    return words + kChainHead +
+           (static_cast<int64_t>(rows) * groups + static_cast<int64_t>(row) * chunks) * (64 * CPL);
+  }
+};
+
+template <typename T, int CPL, int N>
+__global__ __launch_bounds__(64 * kWaves, 4) void recurrence_chain(RecurrenceArgs a) {
+  constexpr int kChunk = kWaves * N, kWide = 64 * CPL;
+  __shared__ float maps[kWaves][2][kWide];  // of the chunk's waves
+  __shared__ float earlier[kGroup - 1][2][kWide];
+  __shared__ float start[kWide];
+  __shared__ unsigned taken;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slot = lane * CPL;
+  const int64_t C = a.channels;
+  Word* words = reinterpret_cast<Word*>(a.words);
+  if (threadIdx.x == 0) taken = atomicAdd(reinterpret_cast<unsigned*>(words), 1u);
+  __syncthreads();
+  const ChainPlace<CPL, kChunk> at(a, __builtin_amdgcn_readfirstlane(taken));
+  Word* states = at.states(words) + slot;
+  Word* left = at.left(words) + slot;
+  const int64_t tile = static_cast<int64_t>(at.chunk) * kChunk;
+  const int run_token = wave * N;
+  const T* x = static_cast<const T*>(a.input) + at.batch * a.input_batch;
+  const T* g = static_cast<const T*>(a.gate) + at.batch * a.gate_batch;
+  T* y = static_cast<T*>(a.output) + at.batch * a.tokens * C;
+  Run<T, CPL> nx[N], ng[N];
+  load_tokens(ng, tile_rows<kChunk>(g, tile, at.length, a.gate_token, C),
+              lane_offset<T>(run_token, a.gate_token, at.channel),
+              static_cast<unsigned>(a.gate_token) * sizeof(T));
+  load_tokens(nx, tile_rows<kChunk>(x, tile, at.length, a.input_token, C),
+              lane_offset<T>(run_token, a.input_token, at.channel),
+              static_cast<unsigned>(a.input_token) * sizeof(T));
+  const bool cut = tile + kChunk > at.length;
+  const int live = tokens_before<N>(tile, run_token, at.length);
+  if (cut) fill_tokens(ng, live, __builtin_inff());
+  float keep[N][CPL], add[N][CPL];
+  Map<CPL> map;
+  map.clear();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const Gate q = open_gate(static_cast<float>(ng[i].v[j]));
+      keep[i][j] = q.keep;
+      add[i][j] = q.take * static_cast<float>(nx[i].v[j]);
+      map.a[j] *= q.keep;
+      map.b[j] = fmaf(q.keep, map.b[j], add[i][j]);
+    }
+#pragma unroll
+  for (int j = 0; j < CPL; ++j) {
+    maps[wave][0][slot + j] = map.a[j];
+    maps[wave][1][slot + j] = map.b[j];
+  }
+  __syncthreads();
+  const bool last_of_group = at.place == kGroup - 1 || at.chunk + 1 == at.chunks;
+  if (wave == 0 && !last_of_group) {
+    Map<CPL> whole;
+    whole.clear();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        const float aw = maps[w][0][slot + j];
+        whole.b[j] = fmaf(aw, whole.b[j], maps[w][1][slot + j]);
+        whole.a[j] *= aw;
+      }
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      leave_word(left + static_cast<int64_t>(at.chunk) * kWide + j, whole.a[j], whole.b[j]);
+  }
+  for (unsigned e = wave; e < at.place; e += kWaves) {
+    float wa[CPL], wb[CPL];
+    await_words<CPL>(left + static_cast<int64_t>(at.group * kGroup + e) * kWide, wa, wb);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      earlier[e][0][slot + j] = wa[j];
+      earlier[e][1][slot + j] = wb[j];
+    }
+  }
+  if (wave == kWaves - 1) {
+    float unused[CPL], h0[CPL];
+    if (at.group == 0) {
+#pragma unroll
+      for (int j = 0; j < CPL; ++j)
+        h0[j] = a.first != nullptr ? a.first[at.batch * C + at.channel + j] : 0.f;
+    } else {
+      await_words<CPL>(states + static_cast<int64_t>(at.group) * kWide, unused, h0);
+    }
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) start[slot + j] = h0[j];
+  }
+  __syncthreads();
+  float h[CPL];
+#pragma unroll
+  for (int j = 0; j < CPL; ++j) h[j] = start[slot + j];
+  for (unsigned e = 0; e < at.place; ++e)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      h[j] = fmaf(earlier[e][0][slot + j], h[j], earlier[e][1][slot + j]);
+#pragma unroll
+  for (int w = 0; w < kWaves - 1; ++w)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      if (w < wave) h[j] = fmaf(maps[w][0][slot + j], h[j], maps[w][1][slot + j]);
+  if (wave == kWaves - 1 && last_of_group) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const float after = fmaf(map.a[j], h[j], map.b[j]);
+      if (at.chunk + 1 < at.chunks)
+        leave_word(states + static_cast<int64_t>(at.group + 1) * kWide + j, 0.f, after);
+      else if (at.valid)
+        a.last[at.batch * C + at.channel + j] = after;
+    }
+  }
+  const int64_t first = tile + run_token;
+  if (a.carries != nullptr && at.valid && first % kRecurrenceTile == 0 && first < a.tokens) {
+    const int64_t tiles = (a.tokens + kRecurrenceTile - 1) / kRecurrenceTile;
+    float* c = a.carries + (at.batch * tiles + first / kRecurrenceTile) * C + at.channel;
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) c[j] = h[j];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      h[j] = fmaf(keep[i][j], h[j], add[i][j]);
+      keep[i][j] = h[j];
+    }
+  if (cut) clear_tokens(keep, live);
+  store_tokens<T, CPL>(tile_rows<kChunk>(y, tile, a.tokens, C, C),
+               at.valid ? lane_offset<T>(run_token, C, at.channel) : kNowhere,
+               static_cast<unsigned>(C) * sizeof(T), keep);
+}
+
+// The backward's chunks, from the last token to the first: maps and words are those of E.
+template <typename T, int CPL, int N>
+__global__ __launch_bounds__(64 * kWaves) void recurrence_chain_backward(RecurrenceArgs a) {
+  constexpr int kChunk = kWaves * N, kWide = 64 * CPL;
+  __shared__ float maps[kWaves][3][kWide];  // A, R (of E) and F (of the state) of the waves
+  __shared__ float later[kGroup - 1][2][kWide];
+  __shared__ float start[kWide];
+  __shared__ unsigned taken;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t C = a.channels;
+  Word* words = reinterpret_cast<Word*>(a.words);
+  if (threadIdx.x == 0) taken = atomicAdd(reinterpret_cast<unsigned*>(words), 1u);
+  __syncthreads();
+  const ChainPlace<CPL, kChunk> at(a, __builtin_amdgcn_readfirstlane(taken));
+  const int slot = lane * CPL;
+  Word* states = at.states(words) + slot;
+  Word* left = at.left(words) + slot;
+  const int64_t tile = static_cast<int64_t>(at.chunks - 1 - at.chunk) * kChunk;
+  const int run_token = wave * N;
+  const T* x = static_cast<const T*>(a.input) + at.batch * a.input_batch;
+  const T* g = static_cast<const T*>(a.gate) + at.batch * a.gate_batch;
+  const T* dy = static_cast<const T*>(a.grad_output) + at.batch * a.grad_batch;
+  Run<T, CPL> nx[N], ng[N], nd[N];
+  load_tokens(ng, tile_rows<kChunk>(g, tile, at.length, a.gate_token, C),
+              lane_offset<T>(run_token, a.gate_token, at.channel),
+              static_cast<unsigned>(a.gate_token) * sizeof(T));
+  load_tokens(nd, tile_rows<kChunk>(dy, tile, at.length, a.grad_token, C),
+              lane_offset<T>(run_token, a.grad_token, at.channel),
+              static_cast<unsigned>(a.grad_token) * sizeof(T));
+  load_tokens(nx, tile_rows<kChunk>(x, tile, at.length, a.input_token, C),
+              lane_offset<T>(run_token, a.input_token, at.channel),
+              static_cast<unsigned>(a.input_token) * sizeof(T));
+  const int64_t tiles = (a.tokens + kRecurrenceTile - 1) / kRecurrenceTile;
+  float h[CPL], e[CPL];
+#pragma unroll
+  for (int j = 0; j < CPL; ++j)
+    h[j] = a.carries[(at.batch * tiles + tile / kRecurrenceTile) * C + at.channel + j];
+  const bool cut = tile + kChunk > at.length;
+  const int live = tokens_before<N>(tile, run_token, at.length);
+  if (cut) fill_tokens(ng, live, __builtin_inff());
+  Map<CPL> map;
+  float state[CPL];
+  map.clear();
+#pragma unroll
+  for (int j = 0; j < CPL; ++j) state[j] = 0.f;
+  float keep[N][CPL], take[N][CPL];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const Gate q = open_gate(static_cast<float>(ng[i].v[j]));
+      keep[i][j] = q.keep;
+      take[i][j] = q.take;
+      map.a[j] *= q.keep;
+      state[j] = fmaf(q.keep, state[j], q.take * static_cast<float>(nx[i].v[j]));
+    }
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      map.b[j] = keep[i][j] * (static_cast<float>(nd[i].v[j]) + map.b[j]);
+#pragma unroll
+  for (int j = 0; j < CPL; ++j) {
+    maps[wave][0][slot + j] = map.a[j];
+    maps[wave][1][slot + j] = map.b[j];
+    maps[wave][2][slot + j] = state[j];
+  }
+  __syncthreads();
+  const bool last_of_group = at.place == kGroup - 1 || at.chunk + 1 == at.chunks;
+  if (wave == 0 && !last_of_group) {
+    Map<CPL> whole;
+    whole.clear();
+#pragma unroll
+    for (int w = kWaves - 1; w >= 0; --w)
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        const float aw = maps[w][0][slot + j];
+        whole.b[j] = fmaf(aw, whole.b[j], maps[w][1][slot + j]);
+        whole.a[j] *= aw;
+      }
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      leave_word(left + static_cast<int64_t>(at.chunk) * kWide + j, whole.a[j], whole.b[j]);
+  }
+  for (unsigned c = wave; c < at.place; c += kWaves) {
+    float wa[CPL], wb[CPL];
+    await_words<CPL>(left + static_cast<int64_t>(at.group * kGroup + c) * kWide, wa, wb);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      later[c][0][slot + j] = wa[j];
+      later[c][1][slot + j] = wb[j];
+    }
+  }
+  if (wave == kWaves - 1) {
+    float unused[CPL], e0[CPL];
+    if (at.group == 0) {
+#pragma unroll
+      for (int j = 0; j < CPL; ++j)
+        e0[j] = a.grad_last != nullptr ? a.grad_last[at.batch * C + at.channel + j] : 0.f;
+    } else {
+      await_words<CPL>(states + static_cast<int64_t>(at.group) * kWide, unused, e0);
+    }
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) start[slot + j] = e0[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < CPL; ++j) e[j] = start[slot + j];
+  for (unsigned c = 0; c < at.place; ++c)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) e[j] = fmaf(later[c][0][slot + j], e[j], later[c][1][slot + j]);
+#pragma unroll
+  for (int w = kWaves - 1; w > 0; --w)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      if (w > wave) e[j] = fmaf(maps[w][0][slot + j], e[j], maps[w][1][slot + j]);
+#pragma unroll
+  for (int w = 0; w < kWaves - 1; ++w)
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      if (w < wave) h[j] = fmaf(maps[w][0][slot + j], h[j], maps[w][2][slot + j]);
+  if (wave == 0 && last_of_group) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const float before = fmaf(map.a[j], e[j], map.b[j]);
+      if (at.chunk + 1 < at.chunks)
+        leave_word(states + static_cast<int64_t>(at.group + 1) * kWide + j, 0.f, before);
+      else if (at.valid && a.grad_first != nullptr)
+        a.grad_first[at.batch * C + at.channel + j] = before;
+    }
+  }
+  // slope is (h_before - x) a (1 - a), then dgate; take becomes dx.
+  float slope[N][CPL];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    hold(nx[i]);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const float xi = static_cast<float>(nx[i].v[j]);
+      slope[i][j] = (h[j] - xi) * (keep[i][j] * take[i][j]);
+      h[j] = fmaf(keep[i][j], h[j], take[i][j] * xi);
+    }
+  }
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i) {
+    hold(nd[i]);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const float d = static_cast<float>(nd[i].v[j]) + e[j];
+      e[j] = keep[i][j] * d;
+      take[i][j] *= d;
+      slope[i][j] *= d;
+    }
+  }
+  if (cut) {
+    clear_tokens(take, live);
+    clear_tokens(slope, live);
+  }
+  const unsigned step = static_cast<unsigned>(C) * sizeof(T);
+  const unsigned out = at.valid ? lane_offset<T>(run_token, C, at.channel) : kNowhere;
+  T* dx = static_cast<T*>(a.grad_input) + at.batch * a.tokens * C;
+  T* dg = static_cast<T*>(a.grad_gate) + at.batch * a.tokens * C;
+  store_tokens<T, CPL>(tile_rows<kChunk>(dx, tile, a.tokens, C, C), out, step, take);
+  store_tokens<T, CPL>(tile_rows<kChunk>(dg, tile, a.tokens, C, C), out, step, slope);
+}
+
+__global__ __launch_bounds__(256) void clear_words(Word* words, int64_t count) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count;
+       i += static_cast<int64_t>(gridDim.x) * 256)
+    words[i] = 0;
+}
+
+template <typename T, int CPL>
+hipError_t launch_chain(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
+  constexpr int kForward = kForwardRun / CPL, kBackward = kBackwardRun / CPL;
+  const int64_t rows = (a.channels + 64 * CPL - 1) / (64 * CPL) * a.batch;
+  const int64_t chunk = kWaves * (backward ? kBackward : kForward);
+  const dim3 grid(static_cast<unsigned>(rows * ((a.tokens + chunk - 1) / chunk)));
+  const int64_t count = a.word_count;
+  hipLaunchKernelGGL(clear_words,
+                     dim3(static_cast<unsigned>(std::min<int64_t>((count + 255) / 256, 2048))),
+                     dim3(256), 0, stream, reinterpret_cast<Word*>(a.words), count);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  if (backward)
+    hipLaunchKernelGGL((recurrence_chain_backward<T, CPL, kBackward>), grid,
+                       dim3(64 * kWaves), 0, stream, a);
+  else
+    hipLaunchKernelGGL((recurrence_chain<T, CPL, kForward>), grid, dim3(64 * kWaves), 0,
+                       stream, a);
+  return hipGetLastError();
 }
 
 // Up to kRun tokens, as in decoding: a thread walks its channels' tokens from the state.
@@ -592,43 +922,37 @@ __global__ __launch_bounds__(kStepThreads) void recurrence_step(RecurrenceArgs a
   for (int j = 0; j < CPL; ++j) a.last[state + j] = h[j];
 }
 
-template <typename T, int CPL, int LANES, int NW>
-hipError_t launch_shape(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
+template <typename T, int CPL, int LANES>
+void launch_whole(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
   const int64_t strips = (a.channels + LANES * CPL - 1) / (LANES * CPL);
-  const dim3 grid(static_cast<unsigned>(strips * a.splits * a.batch)), block(64 * NW);
-  if constexpr (LANES == 64 && NW > 1) {
-    if (a.splits > 1) {
-      if (backward)
-        hipLaunchKernelGGL((recurrence_backward<T, CPL, LANES, NW, true>), grid, block, 0, stream,
-                           a);
-      else
-        hipLaunchKernelGGL((recurrence_forward<T, CPL, LANES, NW, true>), grid, block, 0, stream,
-                           a);
-      const hipError_t err = hipGetLastError();
-      if (err != hipSuccess) return err;
-    }
-  }
+  const dim3 grid(static_cast<unsigned>(strips * a.batch)), block(64 * kWaves);
   if (backward)
-    hipLaunchKernelGGL((recurrence_backward<T, CPL, LANES, NW, false>), grid, block, 0, stream, a);
-  else if constexpr (NW > 1)
-    hipLaunchKernelGGL((recurrence_forward<T, CPL, LANES, NW, false>), grid, block, 0, stream, a);
-  return hipGetLastError();
+    hipLaunchKernelGGL((recurrence_backward<T, CPL, LANES, kWaves>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((recurrence_forward<T, CPL, LANES>), grid, block, 0, stream, a);
 }
 
 template <typename T, int CPL>
 hipError_t launch_channels(const RecurrenceArgs& a, bool backward, const RecurrencePlan& p,
                            hipStream_t stream) {
-  if (p.waves == 1) {
-    if (backward) return launch_shape<T, CPL, 64, 1>(a, true, stream);
+  if (p.chain) return launch_chain<T, CPL>(a, backward, stream);
+  if (p.waves == 1 && backward) {
+    const int64_t strips = (a.channels + 64 * CPL - 1) / (64 * CPL);
+    hipLaunchKernelGGL((recurrence_backward<T, CPL, 64, 1>),
+                       dim3(static_cast<unsigned>(strips * a.batch)), dim3(64), 0, stream, a);
+  } else if (p.waves == 1) {
     const int64_t threads = (a.channels + CPL - 1) / CPL * a.batch;
     hipLaunchKernelGGL((recurrence_step<T, CPL>),
                        dim3(static_cast<unsigned>((threads + kStepThreads - 1) / kStepThreads)),
                        dim3(kStepThreads), 0, stream, a);
-    return hipGetLastError();
+  } else if (p.lanes == 64) {
+    launch_whole<T, CPL, 64>(a, backward, stream);
+  } else if (p.lanes == 32) {
+    launch_whole<T, CPL, 32>(a, backward, stream);
+  } else {
+    launch_whole<T, CPL, 16>(a, backward, stream);
   }
-  if (p.lanes == 64) return launch_shape<T, CPL, 64, 8>(a, backward, stream);
-  if (p.lanes == 32) return launch_shape<T, CPL, 32, 8>(a, backward, stream);
-  return launch_shape<T, CPL, 16, 8>(a, backward, stream);
+  return hipGetLastError();
 }
 
 template <typename T>
@@ -642,37 +966,37 @@ hipError_t launch_recurrence_typed(const RecurrenceArgs& a, bool backward, const
 
 }  // namespace
 
-RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a) {
+RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward) {
   RecurrencePlan p{};
   p.waves = a.tokens <= kRun ? 1 : 8;
   p.channels_per_lane = dtype != CONVND_HIP_FLOAT32 && a.channels % 2 == 0 ? 2 : 1;
   p.lanes = 64;
-  p.splits = 1;
-  const int64_t batch = std::max<int64_t>(1, a.batch);
   const auto groups = [&](int lanes) {
     const int64_t wide = lanes * p.channels_per_lane;
-    return batch * ((a.channels + wide - 1) / wide);
+    return std::max<int64_t>(1, a.batch) * ((a.channels + wide - 1) / wide);
   };
-  const auto tile = [&](int lanes) { return int64_t{8} * (64 / lanes) * kRun; };
-  // The widest lanes that give every compute unit a workgroup: forward / backward of
-  // 8 x 4096 x 4096 fp16 (256 workgroups at 64 lanes) 163 / 315 us at 64, 189 / 340 at 32;
-  // 4 x 4096 x 2048 fp32 102 / 151 at 64 (128 workgroups), 93 / 150 at 32;
-  // 8 x 2048 x 1024 bf16 25 / 44 at 16 (128 workgroups), 39 / 52 at 64 in four splits;
-  // 13 x 777 x 300 fp16 12 / 20 at 16 (130), 22 / 34 at 64 in four splits.
-  while (p.waves > 1 && p.lanes > 16 && a.tokens > tile(p.lanes) && groups(p.lanes) < 256)
-    p.lanes /= 2;
-  p.split_tokens = std::max<int64_t>(a.tokens, 1);
-  // Few workgroups and a long token axis: splits of at least 512 tokens at 64 lanes, one
-  // workgroup for every compute unit (1 x 65536 x 512 fp32: 174 us forward at 128 workgroups, 118 at
-  // 256, 117 at 512, 128 at 1024).
-  if (groups(16) < 128 && a.tokens >= 2048) {
-    p.lanes = 64;
-    const int64_t tiles = (a.tokens + tile(64) - 1) / tile(64);
-    const int64_t wanted = std::min<int64_t>((256 + groups(64) - 1) / groups(64), tiles / 8);
-    const int64_t per = (tiles + wanted - 1) / wanted;
-    p.splits = static_cast<int>((tiles + per - 1) / per);
-    p.split_tokens = per * tile(64);
+  // Whole sequences a workgroup where those fill the chip (8 x 4096 x 4096 fp16, 256 workgroups:
+  // forward 163 us, in chunks 176) or are short (600 tokens of 256 channels, fp32: 7 us against 11);
+  // else chunks of the token axis (forward / backward of 1 x 65536 x 512 fp32: 85 / 143 us, in
+  // splits with a second reading of the inputs 130 / 180; 4 x 16384 x 1024 bf16: 97 / 174, whole
+  // sequences 202 / 404; 8 x 2048 x 1024 bf16: 33 / 51 and 32 / 57).
+  if (a.tokens >= 1024 && groups(64) < 256) {
+    p.chain = true;
+    const int64_t wide = 64 * p.channels_per_lane;
+    const int64_t chunk = kWaves * (backward ? kBackwardRun : kForwardRun) / p.channels_per_lane;
+    const int64_t chunks = (a.tokens + chunk - 1) / chunk;
+    p.word_count = kChainHead + groups(64) * wide * (chunks + (chunks + kGroup - 1) / kGroup);
+    p.workgroups = groups(64) * chunks;
+    return p;
   }
+  // The widest lanes that give every compute unit a workgroup, of those that one tile needs
+  // (forward / backward of 4 x 4096 x 2048 fp32 at 32 lanes, 256 workgroups, 93 / 150 us, at 64
+  // 102 / 151; 8 x 2048 x 1024 bf16 at 16 lanes 25 / 44; 13 x 777 x 300 fp16 at 16 12 / 20, at 64
+  // 31 / 67).
+  while (p.waves > 1 && p.lanes > 16 && a.tokens > int64_t{8} * (64 / p.lanes) * kRun &&
+         groups(p.lanes) < 256)
+    p.lanes /= 2;
+  p.workgroups = groups(p.lanes);
   return p;
 }
 

@@ -83,24 +83,19 @@ RecurrenceArgs to_args(const convnd_hip_recurrence_problem& r) {
   return a;
 }
 
-int64_t summary_floats(const RecurrenceArgs& a, const RecurrencePlan& p) {
-  return p.splits > 1 ? a.batch * p.splits * 2 * a.channels : 0;
-}
-
 // Plans the call into `a` and checks the workspace and the size of the grid.
-int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, void* workspace, size_t workspace_size,
-              RecurrencePlan* p) {
-  *p = plan_recurrence(dtype, *a);
-  a->splits = p->splits;
-  a->split_tokens = p->split_tokens;
-  const int64_t floats = summary_floats(*a, *p);
-  if (floats > 0 && (workspace == nullptr || workspace_size < floats * sizeof(float)))
-    return fail(CONVND_HIP_WORKSPACE_TOO_SMALL,
-                "gated_recurrence needs a workspace of " + std::to_string(floats * sizeof(float)) +
-                    " bytes");
-  a->summary = static_cast<float*>(workspace);
-  const int64_t strips = (a->channels + 15) / 16;
-  if (strips * p->splits * a->batch > std::numeric_limits<int32_t>::max())
+int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, bool backward, void* workspace,
+              size_t workspace_size, RecurrencePlan* p) {
+  *p = plan_recurrence(dtype, *a, backward);
+  const size_t bytes = static_cast<size_t>(p->word_count) * 8;
+  if (bytes > 0 && (workspace == nullptr || workspace_size < bytes))
+    return fail(CONVND_HIP_WORKSPACE_TOO_SMALL, "gated_recurrence needs a workspace of " +
+                                                    std::to_string(bytes) + " bytes");
+  if (bytes > 0 && reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence needs a workspace aligned to 8 bytes");
+  a->words = workspace;
+  a->word_count = p->word_count;
+  if (p->workgroups > std::numeric_limits<int32_t>::max())
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence sizes are too large");
   return CONVND_HIP_SUCCESS;
 }
@@ -344,8 +339,9 @@ size_t convnd_hip_recurrence_workspace_size(convnd_hip_dtype dtype,
                                             const convnd_hip_recurrence_problem* problem) {
   if (check_recurrence(dtype, problem) != CONVND_HIP_SUCCESS) return 0;
   const RecurrenceArgs a = to_args(*problem);
-  return static_cast<size_t>(summary_floats(a, plan_recurrence(dtype, a))) *
-         sizeof(float);
+  return static_cast<size_t>(std::max(plan_recurrence(dtype, a, false).word_count,
+                                      plan_recurrence(dtype, a, true).word_count)) *
+         8;
 }
 
 int convnd_hip_recurrence(convnd_hip_dtype dtype, const convnd_hip_recurrence_problem* problem,
@@ -367,7 +363,7 @@ int convnd_hip_recurrence(convnd_hip_dtype dtype, const convnd_hip_recurrence_pr
   a.last = last;
   a.carries = carries;
   RecurrencePlan p;
-  st = plan_call(dtype, &a, workspace, workspace_size, &p);
+  st = plan_call(dtype, &a, false, workspace, workspace_size, &p);
   if (st != CONVND_HIP_SUCCESS) return st;
   return hip_check(launch_recurrence(dtype, a, false, p, static_cast<hipStream_t>(stream)),
                    "gated recurrence launch");
@@ -397,7 +393,7 @@ int convnd_hip_recurrence_backward(convnd_hip_dtype dtype, const convnd_hip_recu
   a.grad_gate = grad_gate;
   a.grad_first = grad_first;
   RecurrencePlan p;
-  st = plan_call(dtype, &a, workspace, workspace_size, &p);
+  st = plan_call(dtype, &a, true, workspace, workspace_size, &p);
   if (st != CONVND_HIP_SUCCESS) return st;
   return hip_check(launch_recurrence(dtype, a, true, p, static_cast<hipStream_t>(stream)),
                    "gated recurrence backward launch");
