@@ -303,11 +303,12 @@ size_t convnd_hip_linear_workspace_size(convnd_hip_dtype dtype,
 
 /* input [rows, inputs] by its stride, weight [outputs, inputs], bias [outputs] or null, residual
  * [rows, outputs] by its stride or null, output [rows, outputs]. Products are summed in float32;
- * bias, activation and residual are applied in float32 before the one rounding. pre [rows, outputs],
- * or null: the sum before the activation, for the backward. */
+ * bias, activation and residual are applied in float32 before the one rounding. slope [rows, outputs],
+ * or null: the activation's slope for the backward, float32 beside float32, else int16 in steps of
+ * 1 / 28672 with -32768 for NaN (not written without an activation). */
 int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
                       const void* input, const void* weight, const void* bias,
-                      const void* residual, void* output, void* pre, void* workspace,
+                      const void* residual, void* output, void* slope, void* workspace,
                       size_t workspace_size, void* stream);
 
 size_t convnd_hip_linear_backward_workspace_size(convnd_hip_dtype dtype,
@@ -316,14 +317,14 @@ size_t convnd_hip_linear_backward_workspace_size(convnd_hip_dtype dtype,
                                                  const void* weight, int need_grad_input,
                                                  int need_grad_weight, int need_grad_bias);
 
-/* Gradients for the cotangent grad_output [rows, outputs] by its stride; pre is what the forward
+/* Gradients for the cotangent grad_output [rows, outputs] by its stride; slope is what the forward
  * left (not read without an activation). A null grad_input [rows, inputs], grad_weight [outputs,
  * inputs] or grad_bias [outputs] is skipped; the residual's gradient is grad_output itself. The
- * cotangent before the activation, grad_output * act'(pre), is rounded to the element type, which
+ * cotangent before the activation, grad_output * slope, is rounded to the element type, which
  * the matrix cores multiply. */
 int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
                                const void* grad_output, const void* input, const void* weight,
-                               const void* pre, void* grad_input, void* grad_weight,
+                               const void* slope, void* grad_input, void* grad_weight,
                                void* grad_bias, void* workspace, size_t workspace_size,
                                void* stream);
 

@@ -133,8 +133,9 @@ def linear_reference(x, w, b, residual, kind, dy=None):
 
     Sums of n products in any order: n roundings of the magnitudes' sum. The activations and their
     slopes vary by at most 1.13 of their argument's error (1.2 for a slope); their own evaluation
-    adds 16 roundings of |z| + 1. The backward's z and dz are rounded to the element type, and relu's
-    slope may be either side of the step where z is within its error of zero.
+    adds 16 roundings of |z| + 1. Beside 16-bit values the slope is kept in steps of 1 / 28672, dz is
+    rounded to the element type, and relu's slope may be either side of the step where z is within its
+    error of zero.
     """
     dtype = x.dtype
     f = lambda t: None if t is None else t.detach().double().cpu()  # noqa: E731
@@ -160,10 +161,11 @@ def linear_reference(x, w, b, residual, kind, dy=None):
     if kind is None:
         dz_noise = torch.zeros_like(dz)
     else:
-        z_error = z_noise + ROUND[dtype] * (z.abs() + z_noise) + TINY[dtype]
-        slope_noise = 1.2 * z_error + 16 * EPS32 * (z.abs() + 1)
+        slope_noise = 1.2 * z_noise + 16 * EPS32 * (z.abs() + 1)
         if kind == "relu":
-            slope_noise = (z.abs() <= z_error).double()
+            slope_noise = (z.abs() <= z_noise).double()
+        elif dtype != torch.float32:
+            slope_noise = slope_noise + 0.5 / 28672
         dz_noise = g.abs() * slope_noise
         dz_noise = dz_noise + ROUND[dtype] * (dz.abs() + dz_noise) + TINY[dtype]
     dz_size = dz.abs() + dz_noise

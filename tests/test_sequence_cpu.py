@@ -120,9 +120,9 @@ def test_fake_kernels():
         assert y.shape == x.shape and statistics.shape == (2, 210) and statistics.dtype == torch.float32
         dx, dw, db = ops.layer_norm_backward(y, x, w, None, statistics, [True, True, True])
         assert dx.shape == x.shape and dw.shape == (16,) and db is None
-        y, pre = ops.linear_act(x, m, None, None, "gelu", True)
-        assert y.shape == pre.shape == (3, 70, 24)
-        dx, dw, db = ops.linear_act_backward(y, x, m, pre, "gelu", [True, False, True])
+        y, slope = ops.linear_act(x, m, None, None, "gelu", True)
+        assert y.shape == slope.shape == (3, 70, 24) and slope.dtype == torch.int16
+        dx, dw, db = ops.linear_act_backward(y, x, m, slope, "gelu", [True, False, True])
         assert dx.shape == x.shape and dw is None and db.shape == (24,)
         h, last, carries = ops.gated_recurrence(x, x, None, None, True)
         assert h.shape == x.shape and last.shape == (3, 16) and last.dtype == torch.float32
@@ -193,7 +193,7 @@ def test_c_abi_checks(lib):
                                                size - 1, None), small, str(size))
     p.activation = 2
     expect(lib, lib.convnd_hip_linear_backward(bf16, ctypes.byref(p), one, one, one, None, one, one, one, one, size,
-                                               None), bad, "pre must not be null")
+                                               None), bad, "slope must not be null")
 
     def recurrence(dtype=bf16, x=one, size=0, **fields):
         p = _capi.RecurrenceProblem(batch=1, tokens=5000, channels=8, input_batch=40000, input_token=8,

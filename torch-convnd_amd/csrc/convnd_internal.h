@@ -576,7 +576,7 @@ struct LinearArgs {
   const void* residual;       // [m, n] or null
   int64_t residual_stride;
   void* output;               // [m, n]
-  void* pre;                  // [m, n]: the sum before the activation, or null
+  void* slope;                // [m, n]: the activation's slope (float, or 16 bits), or null
   float* partial;             // [splits, m, n] where K is split, else null
   int activation;
 };
@@ -595,11 +595,10 @@ hipError_t launch_linear_pad(convnd_hip_dtype dtype, const void* src, int64_t st
 // The activation's gradient and the bias's.
 struct LinearGradArgs {
   const void* grad_output;  // [rows, columns] by grad_stride
-  const void* pre;          // [rows, columns], null without an activation
+  const void* slope;        // [rows, columns] as the forward left it, null without an activation
   void* grad_pre;           // [rows, columns] by pitch, or null
   float* partial;           // [parts, columns], or null
   int64_t rows, columns, grad_stride, pitch;
-  int activation;
 };
 int64_t linear_grad_parts(int64_t rows, int64_t columns);
 hipError_t launch_linear_grad(convnd_hip_dtype dtype, const LinearGradArgs& a, int64_t parts,

@@ -214,8 +214,8 @@ struct Reader {
 };
 
 // 0.5 erfc(|z| / sqrt 2) and exp(-z^2 / 2) for 16-bit results: Abramowitz and Stegun's formula
-// 7.1.26, off by at most 0.75e-7, at a third of erff's instructions (8192 x 1024 -> 4096 with exact
-// GELU 92 -> 79 us). float results take erff.
+// 7.1.26, off by at most 0.75e-7, at a third of erff's instructions (13 us of 8192 x 1024 -> 4096).
+// float results take erff.
 struct Normal {
   float tail, gauss;
 };
@@ -241,27 +241,91 @@ __device__ __forceinline__ Normal normal(float z) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void activate_all(float (&v)[8], int act) {
+// Activates v; with SLOPE, d is the activation's slope at v (of an infinite v NaN, as the formulas).
+// An epilogue of this size is bound by its instructions: each one an element less is 0.9 us of
+// 8192 x 1024 -> 4096.
+template <typename T, bool SLOPE>
+__device__ __forceinline__ void activate_all(float (&v)[8], float (&d)[8], int act) {
   if (act == CONVND_HIP_ACT_RELU) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // NaN stays
+    for (int e = 0; e < 8; ++e) {
+      d[e] = v[e] > 0.f ? 1.f : 0.f;
+      v[e] = v[e] < 0.f ? 0.f : v[e];  // NaN stays
+    }
   } else if (act == CONVND_HIP_ACT_GELU) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= normal<T>(v[e]).tail;
+    for (int e = 0; e < 8; ++e) {
+      const auto [phi, gauss] = normal<T>(v[e]);
+      if constexpr (SLOPE) d[e] = fmaf(v[e] * 0.39894228040143268f, gauss, phi);
+      v[e] *= phi;
+    }
   } else if (act == CONVND_HIP_ACT_GELU_TANH) {
-    // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
+    // 0.5 z (1 + tanh u) = z s, s = 1 / (1 + exp(-2 u)), u = c z (1 + q z^2) with c = sqrt(2 / pi)
+    // and q = 0.044715; its slope s + 2 z s (1 - s) c (1 + 3 q z^2). The bound on z^2 keeps its
+    // products with a vanished s (1 - s) finite.
+    constexpr float c = 0.79788456080286536f, q = 0.044715f, to_base_2 = -2.88539008177792681f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float u = 0.79788456080286536f * v[e] * fmaf(0.044715f * v[e], v[e], 1.f);
-      v[e] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
+      const float z2 = fminf(v[e] * v[e], 1e30f);
+      const float u = v[e] * fmaf(to_base_2 * c * q, z2, to_base_2 * c);
+      const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u));
+      if constexpr (SLOPE) d[e] = fmaf(v[e] * fmaf(-s, s, s), fmaf(6.f * c * q, z2, 2.f * c), s);
+      v[e] *= s;
     }
   }
 }
 
+// What the backward pass needs of the activation is its slope, within -0.13 and 1.13. Beside 16-bit
+// values it is kept in 16 bits of fixed point, 1 / 28672 a step (1 is on the grid; the lowest code
+// is NaN): at most 1.8e-5 off, where the sum before the activation in bfloat16 moved gradients by
+// half of their own rounding, and read by one multiplication (8192 x 4096 with GELU 40 -> 27 us).
+template <typename T>
+using Slope = std::conditional_t<sizeof(T) == 2, int16_t, float>;
+template <typename T>
+__device__ __forceinline__ Run<Slope<T>, 8> keep_slopes(const float (&d)[8]) {
+  Run<Slope<T>, 8> r;
+  if constexpr (sizeof(T) == 2) {
+    typedef short Pair __attribute__((ext_vector_type(2)));
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      // Rounded products with 32767.
+      constexpr float step = 28672.f / 32767.f;
+      const Pair q = __builtin_bit_cast(
+          Pair, __builtin_amdgcn_cvt_pknorm_i16(d[e] * step, d[e + 1] * step));
+      r.v[e] = q[0];
+      r.v[e + 1] = q[1];
+      nan |= __builtin_isunordered(d[e], d[e + 1]);
+    }
+    if (nan)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d[e] != d[e]) r.v[e] = -32768;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = d[e];
+  }
+  return r;
+}
+__device__ __forceinline__ float slope_of(int16_t q) {
+  return q == -32768 ? __builtin_nanf("") : static_cast<float>(q) * (1.f / 28672.f);
+}
+__device__ __forceinline__ float slope_of(float d) { return d; }
+
+// The slopes are read long after they are written: in 16 bits they are stored past the caches' order
+// of use, so that they do not push out what the next operator reads (layer norm and two layers
+// 16384 x 1024 -> 4096 -> 1024 in bfloat16, slopes kept: 329 -> 291 us).
+__device__ __forceinline__ void store_slopes(int16_t* p, const Run<int16_t, 8>& r) {
+  typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(__builtin_bit_cast(Words, r), reinterpret_cast<Words*>(p));
+}
+__device__ __forceinline__ void store_slopes(float* p, const Run<float, 8>& r) {
+  store_run<8>(p, r);
+}
+
 // Up to 8 neighbouring sums of row m from column n on: the partial sums of a split as they are, else
-// bias, activation and residual in float and one rounding (one more of the sum before the
-// activation, where the backward pass is to have it).
+// bias, activation and residual in float and one rounding (and the activation's slope, where the
+// backward pass is to have it).
 template <typename T>
 __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const float (&bias)[8],
                                        int64_t split, int64_t m, int64_t n, int count) {
@@ -278,26 +342,29 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (e < count) p[e] = v[e];
+      end_of_part();
     }
     return;
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
   T* out = static_cast<T*>(a.output) + at;
-  Run<T, 8> y;
-  if (a.pre != nullptr) {
-    T* pre = static_cast<T*>(a.pre) + at;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y.v[e] = static_cast<T>(v[e]);
+  float d[8];
+  if (a.slope != nullptr) {
+    activate_all<T, true>(v, d, a.activation);
+    const Run<Slope<T>, 8> kept = keep_slopes<T>(d);
+    Slope<T>* slope = static_cast<Slope<T>*>(a.slope) + at;
     if (count == 8) {
-      store_run<8>(pre, y);
+      store_slopes(slope, kept);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (e < count) pre[e] = y.v[e];
+        if (e < count) slope[e] = kept.v[e];
+      end_of_part();
     }
+  } else {
+    activate_all<T, false>(v, d, a.activation);
   }
-  activate_all<T>(v, a.activation);
   if (a.residual != nullptr) {
     const T* residual = static_cast<const T*>(a.residual) + m * a.residual_stride + n;
     if (count == 8) {
@@ -308,8 +375,10 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (e < count) v[e] += static_cast<float>(residual[e]);
+      end_of_part();
     }
   }
+  Run<T, 8> y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y.v[e] = static_cast<T>(v[e]);
   if (count == 8) {
@@ -318,6 +387,7 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < count) out[e] = y.v[e];
+    end_of_part();
   }
 }
 
@@ -617,6 +687,7 @@ __global__ __launch_bounds__(256) void linear_join(LinearArgs a, const float* __
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (e < count) v[e] += p[e];
+        end_of_part();
       }
     }
     finish<T>(a, v, bias, 0, m, n, count);
@@ -644,20 +715,6 @@ __global__ __launch_bounds__(256) void linear_pad(const T* __restrict__ src, int
   }
 }
 
-template <typename T>
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act == CONVND_HIP_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == CONVND_HIP_ACT_GELU) {
-    const auto [phi, gauss] = normal<T>(z);
-    return fmaf(z * 0.39894228040143268f, gauss, phi);
-  }
-  // s = sigmoid(2 u): d/dz (z s) = s + 2 z s (1 - s) du/dz
-  const float u = 0.79788456080286536f * z * fmaf(0.044715f * z, z, 1.f);
-  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.88539008177792681f * u));
-  const float du = 0.79788456080286536f * fmaf(3.f * 0.044715f * z, z, 1.f);
-  return s + 2.f * z * s * (1.f - s) * du;
-}
-
 // dz = dy act'(z) (with a pitch of whole 16 bytes, zeros past a row's end) and the sums of dz over
 // each workgroup's rows, which follow each other. TPR threads a row, 8 columns a thread.
 template <typename T, int TPR>
@@ -668,17 +725,17 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
   const int64_t n = static_cast<int64_t>(blockIdx.x) * kColumns + lane * 8;
   const int count = n >= a.columns ? 0 : (a.columns - n < 8 ? static_cast<int>(a.columns - n) : 8);
   const T* dy = static_cast<const T*>(a.grad_output);
-  const T* pre = static_cast<const T*>(a.pre);
+  const Slope<T>* slope = static_cast<const Slope<T>*>(a.slope);
   T* dz = static_cast<T*>(a.grad_pre);
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto finish_row = [&](int64_t m, Run<T, 8> d, const Run<T, 8>& z) __attribute__((always_inline)) {
+  auto finish_row = [&](int64_t m, Run<T, 8> d, const Run<Slope<T>, 8>& z)
+                        __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (pre != nullptr)
-        d.v[e] = static_cast<T>(static_cast<float>(d.v[e]) *
-                                slope<T>(static_cast<float>(z.v[e]), a.activation));
-      // The sums are of dz as the products take it.
-      sum[e] += static_cast<float>(d.v[e]);
+      float g = static_cast<float>(d.v[e]);
+      if (slope != nullptr) g *= slope_of(z.v[e]);
+      d.v[e] = static_cast<T>(g);
+      sum[e] += g;
     }
     if (dz == nullptr) return;
     T* o = dz + m * a.pitch + n;
@@ -688,6 +745,7 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (n + e < a.pitch) o[e] = d.v[e];
+      end_of_part();
     }
   };
   const int64_t first = a.rows * blockIdx.y / gridDim.y, last = a.rows * (blockIdx.y + 1) / gridDim.y;
@@ -695,26 +753,29 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
     // Four rows' loads at a time.
     int64_t m = first + group;
     for (; m + 3 * kRows < last; m += 4 * kRows) {
-      Run<T, 8> d[4], z[4];
+      Run<T, 8> d[4];
+      Run<Slope<T>, 8> z[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         d[u] = load_run<8>(dy + (m + u * kRows) * a.grad_stride + n);
-        if (pre != nullptr) z[u] = load_run<8>(pre + (m + u * kRows) * a.columns + n);
+        if (slope != nullptr) z[u] = load_run<8>(slope + (m + u * kRows) * a.columns + n);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) finish_row(m + u * kRows, d[u], z[u]);
     }
     for (; m < last; m += kRows) {
       const Run<T, 8> d = load_run<8>(dy + m * a.grad_stride + n);
-      finish_row(m, d, pre != nullptr ? load_run<8>(pre + m * a.columns + n) : d);
+      finish_row(m, d, slope != nullptr ? load_run<8>(slope + m * a.columns + n)
+                                        : Run<Slope<T>, 8>{});
     }
   } else if (count > 0) {
     for (int64_t m = first + group; m < last; m += kRows) {
-      Run<T, 8> d, z;
+      Run<T, 8> d;
+      Run<Slope<T>, 8> z;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         d.v[e] = e < count ? dy[m * a.grad_stride + n + e] : static_cast<T>(0.f);
-        z.v[e] = pre != nullptr && e < count ? pre[m * a.columns + n + e] : static_cast<T>(0.f);
+        z.v[e] = slope != nullptr && e < count ? slope[m * a.columns + n + e] : Slope<T>(0);
       }
       finish_row(m, d, z);
     }

@@ -410,7 +410,7 @@ size_t convnd_hip_linear_workspace_size(convnd_hip_dtype dtype,
 
 int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
                       const void* input, const void* weight, const void* bias,
-                      const void* residual, void* output, void* pre, void* workspace,
+                      const void* residual, void* output, void* slope, void* workspace,
                       size_t workspace_size, void* stream) {
   int st = check_linear(dtype, problem);
   if (st != CONVND_HIP_SUCCESS) return st;
@@ -439,7 +439,7 @@ int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* p
   a.residual = residual;
   a.residual_stride = p.residual_stride;
   a.output = output;
-  a.pre = pre;
+  a.slope = p.activation != CONVND_HIP_ACT_NONE ? slope : nullptr;
   a.activation = p.activation;
   return hip_check(launch_linear_product(dtype, a, LinearProduct::kForward, f.plan, f.partial, on),
                    "linear launch");
@@ -459,7 +459,7 @@ size_t convnd_hip_linear_backward_workspace_size(convnd_hip_dtype dtype,
 
 int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
                                const void* grad_output, const void* input, const void* weight,
-                               const void* pre, void* grad_input, void* grad_weight,
+                               const void* slope, void* grad_input, void* grad_weight,
                                void* grad_bias, void* workspace, size_t workspace_size,
                                void* stream) {
   int st = check_linear(dtype, problem);
@@ -478,10 +478,10 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
   const bool activated = p.activation != CONVND_HIP_ACT_NONE;
   if (p.grad_stride < p.outputs)
     return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs rows at least their length apart");
-  if (grad_output == nullptr || (activated && pre == nullptr) ||
+  if (grad_output == nullptr || (activated && slope == nullptr) ||
       (grad_input != nullptr && weight == nullptr) || (grad_weight != nullptr && input == nullptr))
     return fail(CONVND_HIP_INVALID_ARGUMENT,
-                "grad_output, input, weight and (with an activation) pre must not be null");
+                "grad_output, input, weight and (with an activation) slope must not be null");
   Parts ws{static_cast<char*>(workspace)};
   const LinearBackward b =
       lay_out_backward(dtype, p, grad_output, input, weight, grad_input != nullptr,
@@ -491,14 +491,13 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
   if (b.make_dz || grad_bias != nullptr) {
     LinearGradArgs g{};
     g.grad_output = grad_output;
-    g.pre = activated ? pre : nullptr;
+    g.slope = activated ? slope : nullptr;
     g.grad_pre = b.make_dz ? const_cast<void*>(b.dz.data) : nullptr;
     g.partial = b.sums;
     g.rows = p.rows;
     g.columns = p.outputs;
     g.grad_stride = p.grad_stride;
     g.pitch = b.dz.stride;
-    g.activation = p.activation;
     st = hip_check(launch_linear_grad(dtype, g, b.parts, on), "linear gradient launch");
     if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr)
       st = hip_check(launch_sum_rows(dtype, b.sums, b.parts, p.outputs, p.outputs, grad_bias,

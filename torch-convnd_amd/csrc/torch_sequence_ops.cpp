@@ -273,11 +273,16 @@ convnd_hip_linear_problem linear_problem(const at::Tensor& input, const at::Tens
   return p;
 }
 
+// The element type of the kept slopes.
+at::ScalarType slope_type(const at::Tensor& input) {
+  return input.scalar_type() == at::kFloat ? at::kFloat : at::kShort;
+}
+
 std::tuple<at::Tensor, at::Tensor> linear_act_device(const at::Tensor& input,
                                                      const at::Tensor& weight,
                                                      const OptionalTensor& bias,
                                                      const OptionalTensor& residual,
-                                                     c10::string_view activation, bool keep_pre) {
+                                                     c10::string_view activation, bool keep_slope) {
   const int act = linear_activation(activation);
   check_linear_input(input, weight);
   if (bias.has_value())
@@ -302,8 +307,9 @@ std::tuple<at::Tensor, at::Tensor> linear_act_device(const at::Tensor& input,
   }
   const auto dtype = sequence_dtype(input);
   auto output = at::empty(shape, input.options());
-  const bool keep = keep_pre && act != CONVND_HIP_ACT_NONE;
-  auto pre = keep ? at::empty(shape, input.options()) : at::empty({0}, input.options());
+  const bool keep = keep_slope && act != CONVND_HIP_ACT_NONE;
+  const auto kept = input.options().dtype(slope_type(input));
+  auto slope = keep ? at::empty(shape, kept) : at::empty({0}, kept);
   const size_t bytes =
       convnd_hip_linear_workspace_size(dtype, &p, x.tensor.const_data_ptr(), w.const_data_ptr());
   at::Tensor workspace;
@@ -312,14 +318,14 @@ std::tuple<at::Tensor, at::Tensor> linear_act_device(const at::Tensor& input,
   check_status(convnd_hip_linear(
       dtype, &p, x.tensor.const_data_ptr(), w.const_data_ptr(), data_or_null(b),
       residual.has_value() ? r.tensor.const_data_ptr() : nullptr, output.mutable_data_ptr(),
-      keep ? pre.mutable_data_ptr() : nullptr, bytes > 0 ? workspace.mutable_data_ptr() : nullptr,
+      keep ? slope.mutable_data_ptr() : nullptr, bytes > 0 ? workspace.mutable_data_ptr() : nullptr,
       bytes, stream_of(input)));
-  return {output, pre};
+  return {output, slope};
 }
 
 std::tuple<OptionalTensor, OptionalTensor, OptionalTensor> linear_act_backward_device(
     const at::Tensor& grad_output, const at::Tensor& input, const at::Tensor& weight,
-    const at::Tensor& pre, c10::string_view activation, std::array<bool, 3> output_mask) {
+    const at::Tensor& slope, c10::string_view activation, std::array<bool, 3> output_mask) {
   const int act = linear_activation(activation);
   check_linear_input(input, weight);
   const auto shape = linear_shape(input, weight);
@@ -328,9 +334,9 @@ std::tuple<OptionalTensor, OptionalTensor, OptionalTensor> linear_act_backward_d
                   grad_output.scalar_type() == input.scalar_type(),
               "linear_act grad_output must match the output's shape, device and dtype");
   TORCH_CHECK(act == CONVND_HIP_ACT_NONE ||
-                  (pre.sizes() == at::IntArrayRef(shape) && pre.is_contiguous() &&
-                   pre.device() == input.device() && pre.scalar_type() == input.scalar_type()),
-              "linear_act pre must be what its forward kept");
+                  (slope.sizes() == at::IntArrayRef(shape) && slope.is_contiguous() &&
+                   slope.device() == input.device() && slope.scalar_type() == slope_type(input)),
+              "linear_act slope must be what its forward kept");
   OptionalTensor dx, dw, db;
   if (!output_mask[0] && !output_mask[1] && !output_mask[2]) return {dx, dw, db};
   const c10::OptionalDeviceGuard guard(input.device());
@@ -350,7 +356,7 @@ std::tuple<OptionalTensor, OptionalTensor, OptionalTensor> linear_act_backward_d
     workspace = at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte));
   check_status(convnd_hip_linear_backward(
       dtype, &p, dy.tensor.const_data_ptr(), x.tensor.const_data_ptr(), w.const_data_ptr(),
-      act != CONVND_HIP_ACT_NONE ? pre.const_data_ptr() : nullptr,
+      act != CONVND_HIP_ACT_NONE ? slope.const_data_ptr() : nullptr,
       dx.has_value() ? dx->mutable_data_ptr() : nullptr,
       dw.has_value() ? dw->mutable_data_ptr() : nullptr,
       db.has_value() ? db->mutable_data_ptr() : nullptr,
@@ -377,14 +383,14 @@ class LinearActFunction : public torch::autograd::Function<LinearActFunction> {
                                const at::Tensor& weight, const OptionalTensor& bias,
                                const OptionalTensor& residual, const std::string& activation) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [output, pre] = linear_op().call(input, weight, bias, residual, activation, true);
+    auto [output, slope] = linear_op().call(input, weight, bias, residual, activation, true);
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
-    ctx->save_for_backward({input, weight, pre});
-    ctx->mark_non_differentiable({pre});
+    ctx->save_for_backward({input, weight, slope});
+    ctx->mark_non_differentiable({slope});
     ctx->set_materialize_grads(false);
-    return {output, pre};
+    return {output, slope};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -408,11 +414,11 @@ std::tuple<at::Tensor, at::Tensor> linear_act_autograd(const at::Tensor& input,
                                                        const at::Tensor& weight,
                                                        const OptionalTensor& bias,
                                                        const OptionalTensor& residual,
-                                                       c10::string_view activation, bool keep_pre) {
+                                                       c10::string_view activation, bool keep_slope) {
   if (!at::GradMode::is_enabled() || !(wants_grad(input) || wants_grad(weight) ||
                                        wants_grad(bias) || wants_grad(residual))) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return linear_op().call(input, weight, bias, residual, activation, keep_pre);
+    return linear_op().call(input, weight, bias, residual, activation, keep_slope);
   }
   auto out = LinearActFunction::apply(input, weight, bias, residual, std::string(activation));
   return {out[0], out[1]};

@@ -213,12 +213,14 @@ def _fake_layer_norm_backward(grad_output, input, weight, bias, statistics, outp
     return dx, dw, db
 
 
-def _fake_linear_act(input, weight, bias, residual, activation, keep_pre):
+def _fake_linear_act(input, weight, bias, residual, activation, keep_slope):
     shape = (*input.shape[:-1], weight.shape[0])
-    return input.new_empty(shape), input.new_empty(shape if keep_pre and activation != "none" else (0,))
+    kept = shape if keep_slope and activation != "none" else (0,)
+    kind = torch.int16 if input.element_size() == 2 else torch.float32
+    return input.new_empty(shape), input.new_empty(kept, dtype=kind)
 
 
-def _fake_linear_act_backward(grad_output, input, weight, pre, activation, output_mask):
+def _fake_linear_act_backward(grad_output, input, weight, slope, activation, output_mask):
     contiguous = torch.contiguous_format
     dx = torch.empty_like(input, memory_format=contiguous) if output_mask[0] else None
     dw = torch.empty_like(weight, memory_format=contiguous) if output_mask[1] else None

@@ -93,8 +93,8 @@ _SEQUENCE_SCHEMAS = (
     "layer_norm_backward(Tensor grad_output, Tensor input, Tensor? weight, Tensor? bias, "
     "Tensor statistics, bool[3] output_mask) -> (Tensor?, Tensor?, Tensor?)",
     "linear_act(Tensor input, Tensor weight, Tensor? bias, Tensor? residual, str activation, "
-    "bool keep_pre) -> (Tensor, Tensor)",
-    "linear_act_backward(Tensor grad_output, Tensor input, Tensor weight, Tensor pre, "
+    "bool keep_slope) -> (Tensor, Tensor)",
+    "linear_act_backward(Tensor grad_output, Tensor input, Tensor weight, Tensor slope, "
     "str activation, bool[3] output_mask) -> (Tensor?, Tensor?, Tensor?)",
     "gated_recurrence(Tensor input, Tensor gate, Tensor? initial_state, Tensor? lengths, "
     "bool keep_carries) -> (Tensor, Tensor, Tensor)",
