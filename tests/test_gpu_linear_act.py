@@ -4,7 +4,7 @@ with ragged and unaligned operands, split K, activations, residuals, refusals, s
 import pytest
 import torch
 
-from sequence_helpers import assert_within, linear_reference
+from sequence_helpers import EPS32, activation_reference, assert_within, linear_reference
 from torch_convnd import linear_act
 
 pytestmark = pytest.mark.gpu
@@ -206,3 +206,37 @@ def test_refusals():
     y = linear_act(x.requires_grad_(), w)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(y.float().sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh"])
+@pytest.mark.parametrize("m", [7, 90, 600])
+def test_nan_stays_in_its_row(m, kind, dtype):
+    """A NaN's slope reaches the gradients of its row and of the weight, and no other row."""
+    x, w, b, r, dy = make(m, 40, 72, dtype)
+    bad = m // 2
+    clean = linear_reference(x, w, b, r, kind, dy)
+    x[bad, 3] = float("nan")
+    leaves = [t.requires_grad_() for t in (x, w)]
+    y = linear_act(*leaves, b, r, activation=kind, backend="native")
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    assert y[bad].isnan().all() and dx[bad].isnan().all() and dw.isnan().all()
+    rest = torch.arange(m) != bad
+    assert_within(y[rest.cuda()], *(t[rest] for t in clean["y"]), "y")
+    assert_within(dx[rest.cuda()], *(t[rest] for t in clean["dx"]), "dx")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["relu", "gelu", "gelu_tanh"])
+def test_kept_slopes(kind, dtype):
+    """What the forward keeps in 16 bits: every slope to half a step of 1 / 28672, 0 and 1 exactly."""
+    z = torch.cat([torch.linspace(-12, 12, 4001), torch.tensor([-3e4, -60.0, 0.0, 60.0, 3e4])]).to(dtype).cuda()
+    w = torch.ones(1, 1, device="cuda", dtype=dtype)
+    _, kept = torch.ops.torch_convnd.linear_act(z[:, None], w, None, None, kind, True)
+    assert kept.dtype == torch.int16
+    z64 = z.double().cpu()
+    _, slope = activation_reference(z64, kind)
+    error = (kept.cpu().double().squeeze(1) / 28672 - slope).abs()
+    # The evaluation adds 16 roundings of |z| + 1 where the slope changes, none where it is flat.
+    assert (error <= 0.5 / 28672 + 16 * EPS32 * (z64.abs().clamp(max=16) + 1)).all(), error.max()
+    assert (kept[z >= 12] == 28672).all() and (kept[z <= -12] == 0).all()
