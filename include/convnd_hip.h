@@ -260,7 +260,7 @@ int convnd_hip_timing_read(int kernel, double* total_ms, int64_t* launches);
  * Layer norm, linear layer and gated recurrence of token sequences around the convolution. No
  * counterpart in the reference. Types float32, float16 and bfloat16 (anything else returns
  * CONVND_HIP_INVALID_ARGUMENT); strides are in elements; statistics, states and sums are float32.
- * The gradients asked for are overwritten, not added to. */
+ * The gradients asked for are overwritten, not added to. A workspace is aligned to 16 bytes. */
 
 /* output = (input - mean) * rstd * weight + bias for rows of `channels` contiguous elements,
  * `input_stride` apart in the input, contiguous in the output; mean and the variance are over a
@@ -343,7 +343,7 @@ typedef struct convnd_hip_recurrence_problem {
  * [batch, this, channels]. */
 int64_t convnd_hip_recurrence_carries(int64_t tokens);
 
-/* Device scratch bytes of the two calls below (often 0), aligned to 8 bytes. */
+/* Device scratch bytes of the two calls below (often 0). */
 size_t convnd_hip_recurrence_workspace_size(convnd_hip_dtype dtype,
                                             const convnd_hip_recurrence_problem* problem);
 

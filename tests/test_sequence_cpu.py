@@ -265,3 +265,19 @@ def test_example_learns():
     assert result.returncode == 0, result.stderr
     losses = [float(line.split()[-1]) for line in result.stdout.splitlines() if line.startswith("step")]
     assert losses[-1] < losses[0] - 1, result.stdout
+
+
+def test_c_abi_refuses_unaligned_workspaces(lib):
+    bf16, bad = _capi.BFLOAT16, _capi.INVALID_ARGUMENT
+    one, odd = ctypes.c_void_p(16), ctypes.c_void_p(20)
+    size = lib.convnd_hip_layer_norm_backward_workspace_size(bf16, 100, 8)
+    expect(lib, lib.convnd_hip_layer_norm_backward(bf16, bf16, one, 8, one, 8, None, one, one, one, one, None, 100, 8,
+                                                   odd, size, None), bad, "aligned to 16 bytes")
+    p = _capi.LinearProblem(rows=100, inputs=63, outputs=32, input_stride=63, residual_stride=32, grad_stride=32)
+    at = ctypes.byref(p)
+    size = lib.convnd_hip_linear_workspace_size(bf16, at, one, one)
+    expect(lib, lib.convnd_hip_linear(bf16, at, one, one, None, None, one, None, odd, size, None), bad,
+           "aligned to 16 bytes")
+    size = lib.convnd_hip_linear_backward_workspace_size(bf16, at, one, one, one, 1, 1, 1)
+    expect(lib, lib.convnd_hip_linear_backward(bf16, at, one, one, one, None, one, one, one, odd, size, None), bad,
+           "aligned to 16 bytes")

@@ -83,16 +83,26 @@ RecurrenceArgs to_args(const convnd_hip_recurrence_problem& r) {
   return a;
 }
 
+// A workspace of `needed` bytes, on a whole multiple of `align`.
+int check_workspace(const void* workspace, size_t size, size_t needed, size_t align,
+                    const char* what) {
+  if (needed == 0) return CONVND_HIP_SUCCESS;
+  if (workspace == nullptr || size < needed)
+    return fail(CONVND_HIP_WORKSPACE_TOO_SMALL, std::string(what) + " needs a workspace of " +
+                                                    std::to_string(needed) + " bytes");
+  if (reinterpret_cast<uintptr_t>(workspace) % align != 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, std::string(what) + " needs a workspace aligned to " +
+                                                 std::to_string(align) + " bytes");
+  return CONVND_HIP_SUCCESS;
+}
+
 // Plans the call into `a` and checks the workspace and the size of the grid.
 int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, bool backward, void* workspace,
               size_t workspace_size, RecurrencePlan* p) {
   *p = plan_recurrence(dtype, *a, backward);
   const size_t bytes = static_cast<size_t>(p->word_count) * 8;
-  if (bytes > 0 && (workspace == nullptr || workspace_size < bytes))
-    return fail(CONVND_HIP_WORKSPACE_TOO_SMALL, "gated_recurrence needs a workspace of " +
-                                                    std::to_string(bytes) + " bytes");
-  if (bytes > 0 && reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
-    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence needs a workspace aligned to 8 bytes");
+  const int st = check_workspace(workspace, workspace_size, bytes, 8, "gated_recurrence");
+  if (st != CONVND_HIP_SUCCESS) return st;
   a->words = workspace;
   a->word_count = p->word_count;
   if (p->workgroups > std::numeric_limits<int32_t>::max())
@@ -173,9 +183,7 @@ float* partial_sums(const LinearPlan& p, int64_t m, int64_t n, Parts* ws) {
 }
 
 int check_parts(const Parts& ws, size_t size, const char* what) {
-  if (ws.used == 0 || (ws.base != nullptr && size >= ws.used)) return CONVND_HIP_SUCCESS;
-  return fail(CONVND_HIP_WORKSPACE_TOO_SMALL,
-              std::string(what) + " needs a workspace of " + std::to_string(ws.used) + " bytes");
+  return check_workspace(ws.base, size, ws.used, 16, what);
 }
 
 struct LinearForward {
@@ -301,10 +309,11 @@ int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype para
     return fail(CONVND_HIP_INVALID_ARGUMENT,
                 "grad_output, input and the statistics must not be null");
   const int64_t floats = norm_partials(rows, channels, dtype);
-  if (params && floats > 0 && (workspace == nullptr || workspace_size < floats * sizeof(float)))
-    return fail(CONVND_HIP_WORKSPACE_TOO_SMALL,
-                "layer_norm backward needs a workspace of " +
-                    std::to_string(floats * sizeof(float)) + " bytes");
+  if (params) {
+    st = check_workspace(workspace, workspace_size, floats * sizeof(float), 16,
+                         "layer_norm backward");
+    if (st != CONVND_HIP_SUCCESS) return st;
+  }
   const NormPlan p = plan_norm(rows, channels, size_of(dtype), true);
   float* partial = params ? static_cast<float*>(workspace) : nullptr;
   if (rows > 0) {
