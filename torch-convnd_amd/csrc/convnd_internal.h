@@ -590,6 +590,19 @@ struct LinearPlan {
 LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n, int64_t k);
 hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, LinearProduct which,
                                  const LinearPlan& p, float* partial, hipStream_t stream);
+// The input's and the weight's gradient in one launch, and with them the bias's: `output` [columns] is
+// the sum of `parts` rows (null: none).
+struct LinearSums {
+  const float* partial;
+  int64_t parts, columns;
+  void* output;
+};
+void plan_gradients(convnd_hip_dtype dtype, int64_t rows, int64_t inputs, int64_t outputs,
+                    LinearPlan* x, LinearPlan* w);
+hipError_t launch_linear_gradients(convnd_hip_dtype dtype, const LinearArgs& x,
+                                   const LinearPlan& xp, float* x_partial, const LinearArgs& w,
+                                   const LinearPlan& wp, float* w_partial, const LinearSums& sums,
+                                   hipStream_t stream);
 hipError_t launch_linear_pad(convnd_hip_dtype dtype, const void* src, int64_t stride, int64_t rows,
                              int64_t columns, void* dst, hipStream_t stream);
 // The activation's gradient and the bias's.

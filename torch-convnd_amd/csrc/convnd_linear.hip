@@ -392,25 +392,24 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
 }
 
 // C[m][n] = sum over K of A's row m and B's row n; a workgroup's tile is BM x BN, its WM x WN
-// waves take MB x NB fragments each.
+// waves take MB x NB fragments each. This is workgroup `id` of `workgroups`.
 template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinearArgs a) {
+__device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, unsigned workgroups,
+                                            unsigned char* lds) {
   constexpr int BM = WM * MB * 16, BN = WN * NB * 16;
   using OpA = Operand<T, AOUT, BM, WM * WN>;
   using OpB = Operand<T, BOUT, BN, WM * WN>;
   using frag = typename Fragment<T>::type;
   constexpr int kStage = OpA::kBytes + OpB::kBytes;
   constexpr int kK = OpA::kK;
-  extern __shared__ __align__(1024) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
   // Workgroup ids go round the eight XCDs: each takes a run of tiles, in bands of 8 tile rows, so
   // that what its workgroups read at a time stays in its L2.
-  unsigned id = blockIdx.x;
   {
-    const unsigned n = gridDim.x, per = n >> 3, rest = n & 7, x = id & 7;
+    const unsigned per = workgroups >> 3, rest = workgroups & 7, x = id & 7;
     id = x * per + (x < rest ? x : rest) + (id >> 3);
   }
   const unsigned tiles = a.tiles_m * a.tiles_n;
@@ -569,6 +568,57 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinearArgs a) {
   }
 }
 
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinearArgs a) {
+  extern __shared__ __align__(1024) unsigned char lds[];
+  linear_tile<T, AOUT, BOUT, MB, NB, WM, WN>(a, blockIdx.x, gridDim.x, lds);
+}
+
+// 32 columns' sums of a bias gradient from their partial sums, in a fixed order.
+template <typename T, int THREADS>
+__device__ __forceinline__ void add_sums(const LinearSums& a, unsigned id, float* scratch) {
+  constexpr int kGroups = THREADS / 32;
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const int64_t c = int64_t{id} * 32 + lane;
+  float s = 0.f;
+  if (c < a.columns) {
+    const float* p = a.partial + c;
+#pragma unroll 8
+    for (int64_t r = group; r < a.parts; r += kGroups) s += p[r * a.columns];
+  }
+  scratch[group * 33 + lane] = s;
+  __syncthreads();
+  if (group != 0 || c >= a.columns) return;
+  float total = 0.f;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) total += scratch[g * 33 + lane];
+  static_cast<T*>(a.output)[c] = static_cast<T>(total);
+}
+
+// Both gradients' products and the bias's sums in one launch: `first` workgroups of the product with
+// more K values a tile, then the other's up to `products`. Workgroups of one fill the places that
+// the other leaves free, and one plan weighs both (8192 x 1024 -> 4096 in bfloat16 142 -> 124 us, 1001
+// x 333 -> 517 in float 31 -> 22; a launch each with plans of their own before).
+template <typename T, int MB, int NB, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_gradients(LinearArgs x, LinearArgs w,
+                                                                   LinearSums sums,
+                                                                   unsigned first,
+                                                                   unsigned products,
+                                                                   bool weight_first) {
+  extern __shared__ __align__(1024) unsigned char lds[];
+  if (blockIdx.x >= products) {
+    add_sums<T, 64 * WM * WN>(sums, blockIdx.x - products, reinterpret_cast<float*>(lds));
+    return;
+  }
+  const bool in_first = blockIdx.x < first;
+  const unsigned id = in_first ? blockIdx.x : blockIdx.x - first;
+  const unsigned workgroups = in_first ? first : products - first;
+  if (in_first == weight_first)
+    linear_tile<T, true, true, MB, NB, WM, WN>(w, id, workgroups, lds);
+  else
+    linear_tile<T, false, true, MB, NB, WM, WN>(x, id, workgroups, lds);
+}
+
 // ---- few rows --------------------------------------------------------------------------------
 
 // Rows m < 16 MF of x times 16 rows of W a workgroup; W waves share K. Fragment reads straight
@@ -656,13 +706,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_rows(LinearArgs a) 
 
 // ---- sums of a split K, padding, the activation's gradient -----------------------------------------
 
-// Adds the splits' sums in order and finishes 8 columns of a row a thread.
+// Adds the splits' sums of one or two products in order and finishes 8 columns of a row a thread.
+struct LinearJoin {
+  LinearArgs a;
+  const float* partial;
+  int64_t splits;
+  unsigned workgroups;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void linear_join(LinearArgs a, const float* __restrict__ partial,
-                                                   int64_t splits) {
+__global__ __launch_bounds__(256) void linear_join(LinearJoin one, LinearJoin two) {
+  const bool second = blockIdx.x >= one.workgroups;
+  const LinearArgs& a = second ? two.a : one.a;
+  const int64_t splits = second ? two.splits : one.splits;
+  const int64_t workgroups = second ? two.workgroups : one.workgroups;
   const int64_t parts = (a.n + 7) / 8, total = a.m * parts, step = a.m * a.n;
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
-       id += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t id = static_cast<int64_t>(blockIdx.x - (second ? one.workgroups : 0)) * 256 +
+                    threadIdx.x;
+       id < total; id += workgroups * 256) {
     const int64_t m = id / parts, n = id % parts * 8;
     const int count = a.n - n < 8 ? static_cast<int>(a.n - n) : 8;
     float v[8], bias[8];
@@ -673,7 +733,7 @@ __global__ __launch_bounds__(256) void linear_join(LinearArgs a, const float* __
                     ? static_cast<float>(static_cast<const T*>(a.bias)[n + e])
                     : 0.f;
     }
-    const float* p = partial + m * a.n + n;
+    const float* p = (second ? two.partial : one.partial) + m * a.n + n;
 #pragma unroll 4
     for (int64_t s = 0; s < splits; ++s, p += step) {
       if (count == 8) {
@@ -794,29 +854,85 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
   }
 }
 
-template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
-hipError_t launch_tiles(const LinearArgs& a, int64_t splits, hipStream_t stream) {
-  constexpr int kBytes = 2 * (WM * MB + WN * NB) * 16 * 128;
-  const auto kernel = linear_kernel<T, AOUT, BOUT, MB, NB, WM, WN>;
-  // More than 64 KB of LDS has to be asked for, once per device and kernel.
-  static std::atomic<uint64_t> asked{0};
+// More than 64 KB of LDS has to be asked for, once per device and kernel (`asked` is the kernel's).
+template <typename Kernel>
+hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+  if (bytes <= 65536) return hipSuccess;
   int device = 0;
   hipError_t err = hipGetDevice(&device);
   if (err != hipSuccess) return err;
   const uint64_t bit = uint64_t{1} << (device & 63);
-  if (kBytes > 65536 && (asked.load(std::memory_order_relaxed) & bit) == 0) {
-    err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-    if (err != hipSuccess) return err;
-    asked.fetch_or(bit, std::memory_order_relaxed);
-  }
+  if ((asked.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
+  err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return err;
+}
+
+template <int MB, int NB, int WM, int WN>
+constexpr int kTileBytes = 2 * (WM * MB + WN * NB) * 16 * 128;
+
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
+hipError_t launch_tiles(const LinearArgs& a, int64_t splits, hipStream_t stream) {
+  constexpr int kBytes = kTileBytes<MB, NB, WM, WN>;
+  const auto kernel = linear_kernel<T, AOUT, BOUT, MB, NB, WM, WN>;
+  static std::atomic<uint64_t> asked{0};
+  const hipError_t err = ask_lds(kernel, kBytes, asked);
+  if (err != hipSuccess) return err;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.tiles_m * a.tiles_n * splits)),
                      dim3(64 * WM * WN), kBytes, stream, a);
   return hipGetLastError();
 }
 
+template <typename T, int MB, int NB, int WM, int WN>
+hipError_t launch_gradients(const LinearArgs& x, unsigned x_groups, const LinearArgs& w,
+                            unsigned w_groups, const LinearSums& sums, hipStream_t stream) {
+  constexpr int kBytes = kTileBytes<MB, NB, WM, WN>;
+  const auto kernel = linear_gradients<T, MB, NB, WM, WN>;
+  static std::atomic<uint64_t> asked{0};
+  const hipError_t err = ask_lds(kernel, kBytes, asked);
+  if (err != hipSuccess) return err;
+  const bool weight_first = w.split_k >= x.split_k;
+  const unsigned products = x_groups + w_groups;
+  const unsigned extra =
+      sums.output != nullptr ? static_cast<unsigned>((sums.columns + 31) / 32) : 0;
+  hipLaunchKernelGGL(kernel, dim3(products + extra), dim3(64 * WM * WN), kBytes, stream, x, w, sums,
+                     weight_first ? w_groups : x_groups, products, weight_first);
+  return hipGetLastError();
+}
+
+// The product's arguments with its tiles and, where K is split, the place of its sums.
+LinearArgs planned(LinearArgs a, const LinearPlan& p, float* partial) {
+  a.split_k = p.split_k;
+  a.tiles_m = static_cast<unsigned>((a.m + p.tile - 1) / p.tile);
+  a.tiles_n = static_cast<unsigned>((a.n + p.tile - 1) / p.tile);
+  if (p.splits > 1) a.partial = partial;
+  return a;
+}
+
+LinearJoin join_of(const LinearArgs& a, const LinearPlan& p, const float* partial) {
+  const int64_t work = a.m * ((a.n + 7) / 8);
+  return {a, partial, p.splits,
+          p.splits > 1 ? static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 8192)) : 0};
+}
+template <typename T>
+hipError_t launch_join(const LinearJoin& one, const LinearJoin& two, hipStream_t stream) {
+  if (one.workgroups + two.workgroups == 0) return hipSuccess;
+  hipLaunchKernelGGL(linear_join<T>, dim3(one.workgroups + two.workgroups), dim3(256), 0, stream,
+                     one, two);
+  return hipGetLastError();
+}
+
 template <typename T, bool AOUT, bool BOUT>
-hipError_t launch_product_typed(LinearArgs a, const LinearPlan& p, float* partial,
+hipError_t launch_tiles_of(const LinearArgs& t, const LinearPlan& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (p.tile == 256) return launch_tiles<T, AOUT, BOUT, 8, 4, 2, 4>(t, p.splits, stream);
+  return p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2>(t, p.splits, stream)
+                       : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2>(t, p.splits, stream);
+}
+
+template <typename T, bool AOUT, bool BOUT>
+hipError_t launch_product_typed(const LinearArgs& a, const LinearPlan& p, float* partial,
                                 hipStream_t stream) {
   if constexpr (!AOUT && !BOUT) {
     if (p.few_rows) {
@@ -830,25 +946,9 @@ hipError_t launch_product_typed(LinearArgs a, const LinearPlan& p, float* partia
       return hipGetLastError();
     }
   }
-  LinearArgs t = a;
-  t.split_k = p.split_k;
-  t.tiles_m = static_cast<unsigned>((a.m + p.tile - 1) / p.tile);
-  t.tiles_n = static_cast<unsigned>((a.n + p.tile - 1) / p.tile);
-  if (p.splits > 1) t.partial = partial;
-  hipError_t err;
-  if constexpr (sizeof(T) == 2)
-    err = p.tile == 256 ? launch_tiles<T, AOUT, BOUT, 8, 4, 2, 4>(t, p.splits, stream)
-          : p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2>(t, p.splits, stream)
-                          : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2>(t, p.splits, stream);
-  else
-    err = p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2>(t, p.splits, stream)
-                        : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2>(t, p.splits, stream);
-  if (err != hipSuccess || p.splits <= 1) return err;
-  const int64_t work = a.m * ((a.n + 7) / 8);
-  hipLaunchKernelGGL(linear_join<T>,
-                     dim3(static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 8192))),
-                     dim3(256), 0, stream, a, partial, static_cast<int64_t>(p.splits));
-  return hipGetLastError();
+  const hipError_t err = launch_tiles_of<T, AOUT, BOUT>(planned(a, p, partial), p, stream);
+  if (err != hipSuccess) return err;
+  return launch_join<T>(join_of(a, p, partial), LinearJoin{}, stream);
 }
 
 template <typename T>
@@ -862,6 +962,24 @@ hipError_t launch_product(const LinearArgs& a, LinearProduct which, const Linear
     default:
       return launch_product_typed<T, true, true>(a, p, partial, stream);
   }
+}
+
+template <typename T>
+hipError_t launch_both(const LinearArgs& x, const LinearPlan& xp, float* x_partial,
+                       const LinearArgs& w, const LinearPlan& wp, float* w_partial,
+                       const LinearSums& sums, hipStream_t stream) {
+  const LinearArgs tx = planned(x, xp, x_partial), tw = planned(w, wp, w_partial);
+  const auto gx = static_cast<unsigned>(tx.tiles_m * tx.tiles_n * xp.splits);
+  const auto gw = static_cast<unsigned>(tw.tiles_m * tw.tiles_n * wp.splits);
+  hipError_t err = hipErrorInvalidValue;
+  if (xp.tile == 64)
+    err = launch_gradients<T, 2, 2, 2, 2>(tx, gx, tw, gw, sums, stream);
+  else if (xp.tile == 128)
+    err = launch_gradients<T, 4, 4, 2, 2>(tx, gx, tw, gw, sums, stream);
+  else if constexpr (sizeof(T) == 2)
+    err = launch_gradients<T, 8, 4, 2, 4>(tx, gx, tw, gw, sums, stream);
+  if (err != hipSuccess) return err;
+  return launch_join<T>(join_of(x, xp, x_partial), join_of(w, wp, w_partial), stream);
 }
 
 }  // namespace
@@ -891,6 +1009,15 @@ double tile_time(bool single, int tile, int64_t groups, double k) {
 
 }  // namespace
 
+// Time (us) to write, read and join the sums of a product's splits (through the last cache level at
+// 7 TB/s), without the launch.
+namespace {
+constexpr double kJoinLaunch = 3.0;
+double join_time(int64_t m, int64_t n, int64_t splits) {
+  return splits > 1 ? static_cast<double>(m) * n * (4.0 * splits + 2.0) / 7e6 : 0.0;
+}
+}  // namespace
+
 LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n,
                         int64_t k) {
   LinearPlan p{};
@@ -912,8 +1039,7 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
       const int64_t each = (stages + splits - 1) / splits;
       if (splits > 1 && (each < 4 || each * (splits - 1) >= stages)) break;
       double us = tile_time(single, tile, tiles * splits, static_cast<double>(each * stage));
-      // The splits' sums are written, read and joined (through the last cache level at 7 TB/s).
-      if (splits > 1) us += 3.0 + static_cast<double>(m) * n * (4.0 * splits + 2.0) / 7e6;
+      if (splits > 1) us += kJoinLaunch + join_time(m, n, splits);
       if (best == 0 || us < best) {
         best = us;
         p.tile = tile;
@@ -926,6 +1052,47 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
   return p;
 }
 
+// Both gradients' products in one launch, so of one tile: workgroups of both run side by side and take
+// about as long each where K is cut into parts of about one length.
+void plan_gradients(convnd_hip_dtype dtype, int64_t rows, int64_t inputs, int64_t outputs,
+                    LinearPlan* x, LinearPlan* w) {
+  const bool single = dtype == CONVND_HIP_FLOAT32;
+  const int64_t stage = single ? 32 : 64;
+  const int64_t x_stages = (outputs + stage - 1) / stage, w_stages = (rows + stage - 1) / stage;
+  *x = LinearPlan{};
+  *w = LinearPlan{};
+  double best = 0;
+  constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  for (int tile : {64, 128, 256}) {
+    if (tile == 256 && single) continue;
+    const int64_t across = (inputs + tile - 1) / tile;
+    const int64_t x_tiles = (rows + tile - 1) / tile * across;
+    const int64_t w_tiles = (outputs + tile - 1) / tile * across;
+    for (int parts : kParts) {
+      const int64_t each = (std::max(x_stages, w_stages) + parts - 1) / parts;
+      if (parts > 1 && each < 4) break;
+      // Parts of at most `each` stages, as even as they come.
+      const int64_t x_splits = (x_stages + each - 1) / each, w_splits = (w_stages + each - 1) / each;
+      const int64_t x_each = (x_stages + x_splits - 1) / x_splits;
+      const int64_t w_each = (w_stages + w_splits - 1) / w_splits;
+      const int64_t groups = x_tiles * x_splits + w_tiles * w_splits;
+      const double work = static_cast<double>(x_tiles * x_stages + w_tiles * w_stages) * stage;
+      double us = std::max(tile_time(single, tile, groups, work / static_cast<double>(groups)),
+                           tile_time(single, tile, 1, static_cast<double>(std::max(x_each, w_each) * stage)));
+      if (x_splits > 1 || w_splits > 1)
+        us += kJoinLaunch + join_time(rows, inputs, x_splits) + join_time(outputs, inputs, w_splits);
+      if (best == 0 || us < best) {
+        best = us;
+        x->tile = w->tile = tile;
+        x->splits = static_cast<int>((x_stages + x_each - 1) / x_each);
+        w->splits = static_cast<int>((w_stages + w_each - 1) / w_each);
+        x->split_k = x->splits > 1 ? x_each * stage : outputs;
+        w->split_k = w->splits > 1 ? w_each * stage : rows;
+      }
+    }
+  }
+}
+
 hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, LinearProduct which,
                                  const LinearPlan& p, float* partial, hipStream_t stream) {
   switch (dtype) {
@@ -935,6 +1102,22 @@ hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, Li
       return launch_product<_Float16>(a, which, p, partial, stream);
     case CONVND_HIP_BFLOAT16:
       return launch_product<__bf16>(a, which, p, partial, stream);
+    default:
+      return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_linear_gradients(convnd_hip_dtype dtype, const LinearArgs& x,
+                                   const LinearPlan& xp, float* x_partial, const LinearArgs& w,
+                                   const LinearPlan& wp, float* w_partial, const LinearSums& sums,
+                                   hipStream_t stream) {
+  switch (dtype) {
+    case CONVND_HIP_FLOAT32:
+      return launch_both<float>(x, xp, x_partial, w, wp, w_partial, sums, stream);
+    case CONVND_HIP_FLOAT16:
+      return launch_both<_Float16>(x, xp, x_partial, w, wp, w_partial, sums, stream);
+    case CONVND_HIP_BFLOAT16:
+      return launch_both<__bf16>(x, xp, x_partial, w, wp, w_partial, sums, stream);
     default:
       return hipErrorInvalidValue;
   }

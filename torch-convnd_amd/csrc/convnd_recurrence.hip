@@ -18,7 +18,7 @@
 //     buffers), and the carried state goes on to the next tile, whose loads are in flight
 //     meanwhile. Fewer channels make more workgroups of the same problem.
 //   * Rows are addressed as buffers with a 32-bit lane offset, the tile's end being the buffer's:
-//     64-bit row addresses cost more than the arithmetic (8 x 2048 x 1024 bf16 backward 51 -> 44 us).
+//     64-bit row addresses cost more than the arithmetic (a seventh of a bf16 backward's time).
 //   * With few sequences and channels and many tokens, workgroups take chunks of the token axis
 //     instead and hand the state on (below).
 // Every sum is in fp32 and in a fixed order; 1 - a is computed as sigmoid(-gate), which keeps its

@@ -212,7 +212,8 @@ struct LinearBackward {
   bool make_dz;     // dz = dy act'(z), or a padded copy of dy
   int64_t parts;    // rows of the bias gradient's sums
   float* sums;
-  float* partial;   // of either product: one runs after the other
+  float* input_partial;   // of the products' splits, or null
+  float* weight_partial;
 };
 LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p,
                                 const void* grad_output, const void* input, const void* weight,
@@ -234,22 +235,14 @@ LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_
   if (need_input) b.w = padded(weight, p.inputs, p.outputs, p.inputs, size, ws);
   b.parts = linear_grad_parts(p.rows, p.outputs);
   if (need_bias) b.sums = static_cast<float*>(ws->take(b.parts * p.outputs * sizeof(float)));
-  // The two products' sums take the same place.
-  const size_t before = ws->used;
-  size_t most = before;
-  if (need_input) {
+  if (need_input && need_weight)
+    plan_gradients(dtype, p.rows, p.inputs, p.outputs, &b.input_plan, &b.weight_plan);
+  else if (need_input)
     b.input_plan = plan_product(dtype, LinearProduct::kGradInput, p.rows, p.inputs, p.outputs);
-    b.partial = partial_sums(b.input_plan, p.rows, p.inputs, ws);
-    most = std::max(most, ws->used);
-  }
-  if (need_weight) {
-    ws->used = before;
+  else if (need_weight)
     b.weight_plan = plan_product(dtype, LinearProduct::kGradWeight, p.outputs, p.inputs, p.rows);
-    float* sums = partial_sums(b.weight_plan, p.outputs, p.inputs, ws);
-    if (sums != nullptr) b.partial = sums;
-    most = std::max(most, ws->used);
-  }
-  ws->used = most;
+  if (need_input) b.input_partial = partial_sums(b.input_plan, p.rows, p.inputs, ws);
+  if (need_weight) b.weight_partial = partial_sums(b.weight_plan, p.outputs, p.inputs, ws);
   return b;
 }
 
@@ -497,6 +490,7 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
                        grad_weight != nullptr, grad_bias != nullptr, &ws);
   st = check_parts(ws, workspace_size, "linear_act backward");
   if (st != CONVND_HIP_SUCCESS) return st;
+  const bool both = grad_input != nullptr && grad_weight != nullptr;
   if (b.make_dz || grad_bias != nullptr) {
     LinearGradArgs g{};
     g.grad_output = grad_output;
@@ -508,44 +502,50 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
     g.grad_stride = p.grad_stride;
     g.pitch = b.dz.stride;
     st = hip_check(launch_linear_grad(dtype, g, b.parts, on), "linear gradient launch");
-    if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr)
+    if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr && !both)
       st = hip_check(launch_sum_rows(dtype, b.sums, b.parts, p.outputs, p.outputs, grad_bias,
                                      nullptr, on),
                      "linear bias gradient launch");
     if (st != CONVND_HIP_SUCCESS) return st;
   }
-  LinearArgs a{};
+  LinearArgs x{}, w{};
   if (grad_input != nullptr) {
     st = fill_padded(dtype, b.w, weight, p.inputs, p.outputs, p.inputs, on);
     if (st != CONVND_HIP_SUCCESS) return st;
-    a.a = b.dz.data;
-    a.lda = b.dz.stride;
-    a.b = b.w.data;
-    a.ldb = b.w.stride;
-    a.m = p.rows;
-    a.n = p.inputs;
-    a.k = p.outputs;
-    a.output = grad_input;
-    st = hip_check(launch_linear_product(dtype, a, LinearProduct::kGradInput, b.input_plan,
-                                         b.partial, on),
-                   "linear input gradient launch");
-    if (st != CONVND_HIP_SUCCESS) return st;
+    x.a = b.dz.data;
+    x.lda = b.dz.stride;
+    x.b = b.w.data;
+    x.ldb = b.w.stride;
+    x.m = p.rows;
+    x.n = p.inputs;
+    x.k = p.outputs;
+    x.output = grad_input;
   }
   if (grad_weight != nullptr) {
     st = fill_padded(dtype, b.x, input, p.input_stride, p.rows, p.inputs, on);
     if (st != CONVND_HIP_SUCCESS) return st;
-    a.a = b.dz.data;
-    a.lda = b.dz.stride;
-    a.b = b.x.data;
-    a.ldb = b.x.stride;
-    a.m = p.outputs;
-    a.n = p.inputs;
-    a.k = p.rows;
-    a.output = grad_weight;
-    st = hip_check(launch_linear_product(dtype, a, LinearProduct::kGradWeight, b.weight_plan,
-                                         b.partial, on),
-                   "linear weight gradient launch");
+    w.a = b.dz.data;
+    w.lda = b.dz.stride;
+    w.b = b.x.data;
+    w.ldb = b.x.stride;
+    w.m = p.outputs;
+    w.n = p.inputs;
+    w.k = p.rows;
+    w.output = grad_weight;
   }
+  if (both)
+    return hip_check(launch_linear_gradients(dtype, x, b.input_plan, b.input_partial, w,
+                                             b.weight_plan, b.weight_partial,
+                                             {b.sums, b.parts, p.outputs, grad_bias}, on),
+                     "linear gradients launch");
+  if (grad_input != nullptr)
+    return hip_check(launch_linear_product(dtype, x, LinearProduct::kGradInput, b.input_plan,
+                                           b.input_partial, on),
+                     "linear input gradient launch");
+  if (grad_weight != nullptr)
+    return hip_check(launch_linear_product(dtype, w, LinearProduct::kGradWeight, b.weight_plan,
+                                           b.weight_partial, on),
+                     "linear weight gradient launch");
   return st;
 }
 
