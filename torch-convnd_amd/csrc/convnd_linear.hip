@@ -982,40 +982,68 @@ hipError_t launch_both(const LinearArgs& x, const LinearPlan& xp, float* x_parti
   return launch_join<T>(join_of(x, xp, x_partial), join_of(w, wp, w_partial), stream);
 }
 
-}  // namespace
+// What a launch of a tile's workgroups takes (us), fitted to 1200 timings of 47 problems each way: `slots`
+// run side by side on the chip; a turn of them takes `turn` and `full` a K value, a workgroup alone
+// `alone` a K value. (16-bit at 8192^3: 256 x 256 1370 TFLOP/s, 128 x 128 1160; float is bound by its
+// MFMA rate at either tile, 130.)
+struct TileCost {
+  int tile, slots;
+  float set_up, alone, turn, full;
+};
+constexpr TileCost kTiles16[] = {{64, 1280, 4.0f, 0.0046f, 2.7f, 0.0150f},
+                                 {128, 512, 5.0f, 0.0102f, 4.0f, 0.0140f},
+                                 {256, 256, 4.5f, 0.0210f, 6.0f, 0.0238f}};
+constexpr TileCost kTiles32[] = {{64, 1280, 3.9f, 0.0206f, 4.8f, 0.0772f},
+                                 {128, 512, 5.7f, 0.0656f, 7.9f, 0.1122f}};
 
-namespace {
+// `groups` workgroups of `k` K values on the average, at most `most`: bound by the longest, or by what the
+// busiest compute unit is given.
+float tiles_time(const TileCost& c, uint32_t groups, float k, float most) {
+  const float turns = static_cast<float>((groups + 255) / 256 * 256) / static_cast<float>(c.slots);
+  return c.set_up + std::max(c.alone * most, turns * (c.turn + c.full * k));
+}
 
-// Time (us) of `groups` workgroups of a tile over k values of K, from measurements: `wide` of them run
-// side by side, whole turns of the chip take set-up and epilogue plus a time per K value, and a
-// last turn that does not fill every compute unit's places takes less per K value.
-// 16-bit: 256 x 256 alone on a compute unit 26 ns a K value (1305 TFLOP/s at 8192^3); 128 x 128
-// two to a compute unit 14.0 (1170), alone 9.8; 64 x 64 five 14.0 (700). float is bound by its MFMA
-// rate at any tile (130 TFLOP/s).
-double tile_time(bool single, int tile, int64_t groups, double k) {
-  const double per_cu = static_cast<double>((groups + 255) / 256);
-  if (single) return 4.0 + per_cu * k * (tile == 64 ? 0.0162 : 0.0640);
-  if (tile == 256) return per_cu * (7.0 + 0.026 * k);
-  const int64_t wide = tile == 128 ? 512 : 1280;
-  const double set_up = tile == 128 ? 6.0 : 3.0;
-  const int64_t rest = groups % wide;
-  double us = static_cast<double>(groups / wide) * (set_up + 0.0140 * k);
-  if (rest > 0) {
-    const int64_t side = (rest + 255) / 256;
-    us += set_up + (tile == 128 ? (side == 1 ? 0.0098 : 0.0140) : 0.004 + 0.002 * side) * k;
+// Writing, reading and joining splits' sums: `bytes`, at most `splits` of them in a row of loads.
+float join_time(bool single, float bytes, uint32_t splits) {
+  return 2.0f + (single ? 0.5f : 0.3f) * static_cast<float>(splits) +
+         bytes / (single ? 8.5e6f : 4.6e6f);
+}
+float split_bytes(uint32_t m, uint32_t n, uint32_t splits) {
+  return splits > 1 ? static_cast<float>(m) * static_cast<float>(n) *
+                          static_cast<float>(4 * splits + 2)
+                    : 0.f;
+}
+
+// A few parts only: this runs on every call.
+constexpr uint32_t kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+
+// K's stages in parts of at most `each`, as even as they come.
+struct Split {
+  uint32_t count, stages;
+  Split(uint32_t all, uint32_t each) {
+    stages = (all + (all + each - 1) / each - 1) / ((all + each - 1) / each);
+    count = (all + stages - 1) / stages;
   }
-  return us;
+};
+
+LinearPlan plan_of(int tile, const Split& split, uint32_t stage, int64_t k) {
+  LinearPlan p{};
+  p.tile = tile;
+  p.splits = static_cast<int>(split.count);
+  p.split_k = split.count > 1 ? int64_t{split.stages} * stage : k;
+  return p;
 }
 
-}  // namespace
-
-// Time (us) to write, read and join the sums of a product's splits (through the last cache level at
-// 7 TB/s), without the launch.
-namespace {
-constexpr double kJoinLaunch = 3.0;
-double join_time(int64_t m, int64_t n, int64_t splits) {
-  return splits > 1 ? static_cast<double>(m) * n * (4.0 * splits + 2.0) / 7e6 : 0.0;
+template <typename Visit>
+void each_tile(bool single, Visit visit) {
+  if (single)
+    for (const TileCost& c : kTiles32) visit(c);
+  else
+    for (const TileCost& c : kTiles16) visit(c);
 }
+
+uint32_t over(int64_t n, int64_t by) { return static_cast<uint32_t>((n + by - 1) / by); }
+
 }  // namespace
 
 LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n,
@@ -1028,27 +1056,24 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
     return p;
   }
   const bool single = dtype == CONVND_HIP_FLOAT32;
-  const int64_t stage = single ? 32 : 64, stages = (k + stage - 1) / stage;
-  double best = 0;
-  // A few splits only: this runs on every call.
-  constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-  for (int tile : {64, 128, 256}) {
-    if (tile == 256 && single) continue;
-    const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-    for (int splits : kSplits) {
-      const int64_t each = (stages + splits - 1) / splits;
-      if (splits > 1 && (each < 4 || each * (splits - 1) >= stages)) break;
-      double us = tile_time(single, tile, tiles * splits, static_cast<double>(each * stage));
-      if (splits > 1) us += kJoinLaunch + join_time(m, n, splits);
+  const uint32_t stage = single ? 32 : 64, stages = over(k, stage);
+  float best = 0;
+  each_tile(single, [&](const TileCost& c) {
+    const uint32_t tiles = over(m, c.tile) * over(n, c.tile);
+    for (const uint32_t parts : kParts) {
+      const Split split(stages, (stages + parts - 1) / parts);
+      if (parts > 1 && split.stages < 4) break;
+      const float length = static_cast<float>(split.stages * stage);
+      float us = tiles_time(c, tiles * split.count,
+                            static_cast<float>(k) / static_cast<float>(split.count), length);
+      if (split.count > 1)
+        us += join_time(single, split_bytes(m, n, split.count), split.count);
       if (best == 0 || us < best) {
         best = us;
-        p.tile = tile;
-        p.splits = splits;
-        p.split_k = each * stage;
+        p = plan_of(c.tile, split, stage, k);
       }
     }
-  }
-  if (p.splits == 1) p.split_k = k;
+  });
   return p;
 }
 
@@ -1057,40 +1082,34 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
 void plan_gradients(convnd_hip_dtype dtype, int64_t rows, int64_t inputs, int64_t outputs,
                     LinearPlan* x, LinearPlan* w) {
   const bool single = dtype == CONVND_HIP_FLOAT32;
-  const int64_t stage = single ? 32 : 64;
-  const int64_t x_stages = (outputs + stage - 1) / stage, w_stages = (rows + stage - 1) / stage;
-  *x = LinearPlan{};
-  *w = LinearPlan{};
-  double best = 0;
-  constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-  for (int tile : {64, 128, 256}) {
-    if (tile == 256 && single) continue;
-    const int64_t across = (inputs + tile - 1) / tile;
-    const int64_t x_tiles = (rows + tile - 1) / tile * across;
-    const int64_t w_tiles = (outputs + tile - 1) / tile * across;
-    for (int parts : kParts) {
-      const int64_t each = (std::max(x_stages, w_stages) + parts - 1) / parts;
+  const uint32_t stage = single ? 32 : 64;
+  const uint32_t x_stages = over(outputs, stage), w_stages = over(rows, stage);
+  const uint32_t longest = std::max(x_stages, w_stages);
+  float best = 0;
+  each_tile(single, [&](const TileCost& c) {
+    const uint32_t across = over(inputs, c.tile);
+    const uint32_t x_tiles = over(rows, c.tile) * across, w_tiles = over(outputs, c.tile) * across;
+    const float work = (static_cast<float>(x_tiles) * static_cast<float>(x_stages) +
+                        static_cast<float>(w_tiles) * static_cast<float>(w_stages)) *
+                       static_cast<float>(stage);
+    for (const uint32_t parts : kParts) {
+      const uint32_t each = (longest + parts - 1) / parts;
       if (parts > 1 && each < 4) break;
-      // Parts of at most `each` stages, as even as they come.
-      const int64_t x_splits = (x_stages + each - 1) / each, w_splits = (w_stages + each - 1) / each;
-      const int64_t x_each = (x_stages + x_splits - 1) / x_splits;
-      const int64_t w_each = (w_stages + w_splits - 1) / w_splits;
-      const int64_t groups = x_tiles * x_splits + w_tiles * w_splits;
-      const double work = static_cast<double>(x_tiles * x_stages + w_tiles * w_stages) * stage;
-      double us = std::max(tile_time(single, tile, groups, work / static_cast<double>(groups)),
-                           tile_time(single, tile, 1, static_cast<double>(std::max(x_each, w_each) * stage)));
-      if (x_splits > 1 || w_splits > 1)
-        us += kJoinLaunch + join_time(rows, inputs, x_splits) + join_time(outputs, inputs, w_splits);
+      const Split xs(x_stages, each), ws(w_stages, each);
+      const uint32_t groups = x_tiles * xs.count + w_tiles * ws.count;
+      float us = tiles_time(c, groups, work / static_cast<float>(groups),
+                            static_cast<float>(std::max(xs.stages, ws.stages) * stage));
+      if (xs.count > 1 || ws.count > 1)
+        us += join_time(single,
+                        split_bytes(rows, inputs, xs.count) + split_bytes(outputs, inputs, ws.count),
+                        std::max(xs.count, ws.count));
       if (best == 0 || us < best) {
         best = us;
-        x->tile = w->tile = tile;
-        x->splits = static_cast<int>((x_stages + x_each - 1) / x_each);
-        w->splits = static_cast<int>((w_stages + w_each - 1) / w_each);
-        x->split_k = x->splits > 1 ? x_each * stage : outputs;
-        w->split_k = w->splits > 1 ? w_each * stage : rows;
+        *x = plan_of(c.tile, xs, stage, outputs);
+        *w = plan_of(c.tile, ws, stage, rows);
       }
     }
-  }
+  });
 }
 
 hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, LinearProduct which,
