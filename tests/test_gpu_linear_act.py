@@ -240,3 +240,17 @@ def test_kept_slopes(kind, dtype):
     # The evaluation adds 16 roundings of |z| + 1 where the slope changes, none where it is flat.
     assert (error <= 0.5 / 28672 + 16 * EPS32 * (z64.abs().clamp(max=16) + 1)).all(), error.max()
     assert (kept[z >= 12] == 28672).all() and (kept[z <= -12] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1024, 1003])
+def test_outputs_beyond_the_caches(n, dtype):
+    """Outputs of over 96 MB are stored past the caches: rows all over them, and the row ends."""
+    m = 52001
+    x, w, b, r, _ = make(m, 24, n, dtype)
+    rows = torch.cat([torch.arange(0, m, 1999), torch.arange(m - 70, m)]).cuda()
+    with torch.no_grad():
+        y = linear_act(x, w, b, r, activation="gelu")
+        again = linear_act(x, w, b, r, activation="gelu")
+    assert torch.equal(y, again)
+    assert_within(y[rows], *linear_reference(x[rows], w, b, r[rows], "gelu")["y"], "y")

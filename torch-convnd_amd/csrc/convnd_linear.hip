@@ -312,16 +312,19 @@ __device__ __forceinline__ float slope_of(int16_t q) {
 }
 __device__ __forceinline__ float slope_of(float d) { return d; }
 
-// The slopes are read long after they are written: in 16 bits they are stored past the caches' order
-// of use, so that they do not push out what the next operator reads (layer norm and two layers
-// 16384 x 1024 -> 4096 -> 1024 in bfloat16, slopes kept: 329 -> 291 us).
-__device__ __forceinline__ void store_slopes(int16_t* p, const Run<int16_t, 8>& r) {
+// 16 bytes stored past the caches' order of use, for what is not read before much else is.
+template <typename T>
+__device__ __forceinline__ void stream_run(T* p, const Run<T, 8>& r) {
+  static_assert(sizeof(T) == 2, "8 values of 16 bits");
   typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2)));
   __builtin_nontemporal_store(__builtin_bit_cast(Words, r), reinterpret_cast<Words*>(p));
 }
-__device__ __forceinline__ void store_slopes(float* p, const Run<float, 8>& r) {
-  store_run<8>(p, r);
-}
+
+// Outputs of this size and more are streamed past the caches: their reader finds little of them there
+// either way. Training steps of three blocks (layer norm and two layers) in bfloat16 with outputs of
+// 32 MB (4096 x 1024 -> 4096 -> 1024) 926 us plain and 980 streamed, of 64 MB (8192 rows) 1539 and
+// 1567, (16384 x 2048 -> 2048) 2810 and 2762, of 128 MB (16384 x 1024 -> 4096) 2884 and 2799.
+constexpr int64_t kStreamBytes = int64_t{96} << 20;
 
 // Up to 8 neighbouring sums of row m from column n on: the partial sums of a split as they are, else
 // bias, activation and residual in float and one rounding (and the activation's slope, where the
@@ -355,7 +358,11 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
     const Run<Slope<T>, 8> kept = keep_slopes<T>(d);
     Slope<T>* slope = static_cast<Slope<T>*>(a.slope) + at;
     if (count == 8) {
-      store_slopes(slope, kept);
+      // Read by the backward pass, long after.
+      if constexpr (sizeof(T) == 2)
+        stream_run(slope, kept);
+      else
+        store_run<8>(slope, kept);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -382,7 +389,17 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
 #pragma unroll
   for (int e = 0; e < 8; ++e) y.v[e] = static_cast<T>(v[e]);
   if (count == 8) {
-    store_run<8>(out, y);
+    if constexpr (sizeof(T) == 2) {
+      if (a.m * a.n * int64_t{sizeof(T)} >= kStreamBytes) {
+        end_of_part();  // around it, else the two stores become one
+        stream_run(out, y);
+        end_of_part();
+      } else {
+        store_run<8>(out, y);
+      }
+    } else {
+      store_run<8>(out, y);
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -982,7 +999,8 @@ hipError_t launch_both(const LinearArgs& x, const LinearPlan& xp, float* x_parti
   return launch_join<T>(join_of(x, xp, x_partial), join_of(w, wp, w_partial), stream);
 }
 
-// What a launch of a tile's workgroups takes (us), fitted to 1200 timings of 47 problems each way: `slots`
+// What a launch of a tile's workgroups takes (us), fitted to over a thousand timings (25 problems,
+// forward and backward, 16-bit and float, every tile and number of parts): `slots`
 // run side by side on the chip; a turn of them takes `turn` and `full` a K value, a workgroup alone
 // `alone` a K value. (16-bit at 8192^3: 256 x 256 1370 TFLOP/s, 128 x 128 1160; float is bound by its
 // MFMA rate at either tile, 130.)
