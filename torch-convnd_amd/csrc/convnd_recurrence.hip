@@ -10,7 +10,7 @@
 // Bound by HBM: two elements read and one written per token and channel in the forward, three and
 // two in the backward, which makes its states again from one saved state per 64 tokens instead of
 // reading h. A run of tokens acts on the state as h -> A h + B, and such maps compose:
-//   * A lane owns a channel (two of a 16-bit type) and walks 8 consecutive tokens of it in
+//   * A lane owns a channel (or two of a 16-bit type) and walks 8 consecutive tokens of it in
 //     registers, once for the run's map and, when the state before the run is known, again.
 //   * The 64 lanes of a wave are one run, or two or four that follow each other, of as many times
 //     fewer channels; the 8 waves of a workgroup take the next runs. The maps are scanned over the
@@ -304,9 +304,12 @@ __global__ __launch_bounds__(64 * kWaves) void recurrence_forward(RecurrenceArgs
   for (int j = 0; j < CPL; ++j) a.last[at.batch * C + at.channel + j] = carry[j];
 }
 
-// The backward walks the tiles from the last.
-template <typename T, int CPL, int LANES, int NW>
+// The backward walks the tiles from the last. One channel a lane in 16 bits too: two take 200 registers,
+// which leaves two waves a SIMD (8 x 4096 x 4096 fp16 320 us with two, 285 with one; 64 x 512 x 4096 bf16
+// 322 and 278; 13 x 777 x 300 fp16 23 and 17).
+template <typename T, int LANES, int NW>
 __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a) {
+  constexpr int CPL = 1;
   constexpr int kTile = NW * (64 / LANES) * kRun;
   __shared__ float maps[2][NW][3][LANES * CPL];
   const Place<CPL, LANES> at(a);
@@ -424,7 +427,6 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
     float slope[kRun][CPL];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      hold(cx[i]);
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
         const float xi = static_cast<float>(cx[i].v[j]);
@@ -434,7 +436,6 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
     }
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
-      hold(cd[i]);
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
         const float d = static_cast<float>(cd[i].v[j]) + e[j];
@@ -929,19 +930,23 @@ template <typename T, int CPL, int LANES>
 void launch_whole(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
   const int64_t strips = (a.channels + LANES * CPL - 1) / (LANES * CPL);
   const dim3 grid(static_cast<unsigned>(strips * a.batch)), block(64 * kWaves);
-  if (backward)
-    hipLaunchKernelGGL((recurrence_backward<T, CPL, LANES, kWaves>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((recurrence_forward<T, CPL, LANES>), grid, block, 0, stream, a);
+  if constexpr (CPL == 1) {
+    if (backward) {
+      hipLaunchKernelGGL((recurrence_backward<T, LANES, kWaves>), grid, block, 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((recurrence_forward<T, CPL, LANES>), grid, block, 0, stream, a);
 }
 
 template <typename T, int CPL>
 hipError_t launch_channels(const RecurrenceArgs& a, bool backward, const RecurrencePlan& p,
                            hipStream_t stream) {
   if (p.chain) return launch_chain<T, CPL>(a, backward, stream);
+  if (backward && CPL != 1) return hipErrorInvalidValue;  // no plan has it
   if (p.waves == 1 && backward) {
-    const int64_t strips = (a.channels + 64 * CPL - 1) / (64 * CPL);
-    hipLaunchKernelGGL((recurrence_backward<T, CPL, 64, 1>),
+    const int64_t strips = (a.channels + 63) / 64;
+    hipLaunchKernelGGL((recurrence_backward<T, 64, 1>),
                        dim3(static_cast<unsigned>(strips * a.batch)), dim3(64), 0, stream, a);
   } else if (p.waves == 1) {
     const int64_t threads = (a.channels + CPL - 1) / CPL * a.batch;
@@ -992,10 +997,15 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
     p.workgroups = groups(64) * chunks;
     return p;
   }
+  // The forward takes one channel a lane in 16 bits too where that makes workgroups for idle compute
+  // units (13 x 777 x 300 fp16 14.3 us with two channels, 11.8 with one; 8 x 4096 x 4096, 256
+  // workgroups of two, 164 and 154). Else two are loaded at half the cost (64 x 512 x 4096 bf16 154
+  // and 173; 16 x 512 x 1024, 128 workgroups, 15 and 18).
+  if (backward || groups(16) < 256 || (groups(64) >= 256 && groups(64) <= 512))
+    p.channels_per_lane = 1;
   // The widest lanes that give every compute unit a workgroup, of those that one tile needs
   // (forward / backward of 4 x 4096 x 2048 fp32 at 32 lanes, 256 workgroups, 93 / 150 us, at 64
-  // 102 / 151; 8 x 2048 x 1024 bf16 at 16 lanes 25 / 44; 13 x 777 x 300 fp16 at 16 12 / 20, at 64
-  // 31 / 67).
+  // 102 / 151; 13 x 777 x 300 fp16 at 16 12 / 17, at 64 31 / 67).
   while (p.waves > 1 && p.lanes > 16 && a.tokens > int64_t{8} * (64 / p.lanes) * kRun &&
          groups(p.lanes) < 256)
     p.lanes /= 2;
