@@ -977,18 +977,24 @@ hipError_t launch_recurrence_typed(const RecurrenceArgs& a, bool backward, const
 RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward) {
   RecurrencePlan p{};
   p.waves = a.tokens <= kRun ? 1 : 8;
-  p.channels_per_lane = dtype != CONVND_HIP_FLOAT32 && a.channels % 2 == 0 ? 2 : 1;
+  // Two 16-bit channels a lane, where they fill more than half of a wave's lanes.
+  p.channels_per_lane =
+      dtype != CONVND_HIP_FLOAT32 && a.channels % 2 == 0 && a.channels > 64 ? 2 : 1;
   p.lanes = 64;
   const auto groups = [&](int lanes) {
     const int64_t wide = lanes * p.channels_per_lane;
     return std::max<int64_t>(1, a.batch) * ((a.channels + wide - 1) / wide);
   };
   // Whole sequences a workgroup where those fill the chip (8 x 4096 x 4096 fp16, 256 workgroups:
-  // forward 163 us, in chunks 176) or are short (600 tokens of 256 channels, fp32: 7 us against 11);
-  // else chunks of the token axis (forward / backward of 1 x 65536 x 512 fp32: 85 / 143 us, in
-  // splits with a second reading of the inputs 130 / 180; 4 x 16384 x 1024 bf16: 97 / 174, whole
-  // sequences 202 / 404; 8 x 2048 x 1024 bf16: 33 / 51 and 32 / 57).
-  if (a.tokens >= 1024 && groups(64) < 256) {
+  // forward 163 us, in chunks 176) or are short (600 tokens of 256 channels, fp32: 7 us against 11), up to
+  // 2048 tokens also where fewer lanes make just one for each compute unit of the forward (8 x 1024 x
+  // 1024 bf16 16 and 21, 16 x 2048 x 1024 48 and 52; 7 x 2000 x 1024, 224 of them, 41 and 31, 8 x 16384
+  // x 1024 216 and 176; backward 8 x 2048 x 1024 77 and 51); else chunks of the token axis (forward /
+  // backward of 1 x 65536 x 512 fp32: 85 / 143 us, in splits with a second reading of the inputs 130 /
+  // 180; 4 x 16384 x 1024 bf16: 97 / 174, whole sequences 202 / 404).
+  const bool whole = !backward && a.tokens <= 2048 &&
+                     (groups(64) == 256 || groups(32) == 256 || groups(16) == 256);
+  if (a.tokens >= 1024 && groups(64) < 256 && !whole) {
     p.chain = true;
     const int64_t wide = 64 * p.channels_per_lane;
     const int64_t chunk = kWaves * (backward ? kBackwardRun : kForwardRun) / p.channels_per_lane;
