@@ -15,7 +15,7 @@
 //     then in registers.
 //   * Few tiles and a long K: K is split over workgroups, their float sums go to the workspace and
 //     are added in order by a second launch with the epilogue.
-//   * Up to 64 rows (decoding): bound by reading W once. A workgroup takes 16 rows of W, its waves
+//   * Up to 32 or 64 rows (decoding): bound by reading W once. A workgroup takes 16 rows of W, its waves
 //     take parts of K and read fragments from memory into registers, all in flight at once.
 // The bounds of a tile are those of the buffers it reads through; 16-bit rows of odd length or stride
 // are first copied to the workspace with padding.
@@ -1069,11 +1069,16 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
   LinearPlan p{};
   p.splits = 1;
   p.split_k = k;
-  if (which == LinearProduct::kForward && m <= 64) {
+  const bool single = dtype == CONVND_HIP_FLOAT32;
+  // Over 32 rows of 8 KB and more are better off in tiles with K in parts, which read the input less often
+  // (us of a few rows' kernel and of tiles with cold weights: 64 x 4096 -> 4096 bf16 25 and 21, fp32 45
+  // and 31, 48 x 4096 -> 1024 20 and 15.5, 40 and 20.5; 64 x 1024 -> 4096 9 and 15, 15 and 17; 32 x 4096
+  // -> 4096 17 and 21, 29 and 30).
+  if (which == LinearProduct::kForward &&
+      (m <= 32 || (m <= 64 && k * (single ? 4 : 2) < 8192))) {
     p.few_rows = true;
     return p;
   }
-  const bool single = dtype == CONVND_HIP_FLOAT32;
   const uint32_t stage = single ? 32 : 64, stages = over(k, stage);
   float best = 0;
   each_tile(single, [&](const TileCost& c) {
