@@ -254,3 +254,10 @@ def test_outputs_beyond_the_caches(n, dtype):
         again = linear_act(x, w, b, r, activation="gelu")
     assert torch.equal(y, again)
     assert_within(y[rows], *linear_reference(x[rows], w, b, r[rows], "gelu")["y"], "y")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize(("m", "k", "n"), [(5, 16385, 40), (16, 8200, 33), (20, 8192, 72), (31, 4097, 17), (33, 4099, 50)])
+def test_few_long_rows(m, k, n, dtype):
+    """A few rows, on either side of the lengths from which tiles take them with K in parts."""
+    check(*make(m, k, n, dtype), "gelu_tanh")

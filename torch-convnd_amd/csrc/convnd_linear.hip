@@ -15,7 +15,7 @@
 //     then in registers.
 //   * Few tiles and a long K: K is split over workgroups, their float sums go to the workspace and
 //     are added in order by a second launch with the epilogue.
-//   * Up to 32 or 64 rows (decoding): bound by reading W once. A workgroup takes 16 rows of W, its waves
+//   * Up to 64 rows (decoding), not too long: bound by reading W once. A workgroup takes 16 rows of W, its waves
 //     take parts of K and read fragments from memory into registers, all in flight at once.
 // The bounds of a tile are those of the buffers it reads through; 16-bit rows of odd length or stride
 // are first copied to the workspace with padding.
@@ -1070,12 +1070,15 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
   p.splits = 1;
   p.split_k = k;
   const bool single = dtype == CONVND_HIP_FLOAT32;
-  // Over 32 rows of 8 KB and more are better off in tiles with K in parts, which read the input less often
-  // (us of a few rows' kernel and of tiles with cold weights: 64 x 4096 -> 4096 bf16 25 and 21, fp32 45
-  // and 31, 48 x 4096 -> 1024 20 and 15.5, 40 and 20.5; 64 x 1024 -> 4096 9 and 15, 15 and 17; 32 x 4096
-  // -> 4096 17 and 21, 29 and 30).
-  if (which == LinearProduct::kForward &&
-      (m <= 32 || (m <= 64 && k * (single ? 4 : 2) < 8192))) {
+  // The few rows' kernel reads W once but its input once per 16 columns, and 16 rows of W through one
+  // compute unit; from some length of K on tiles with K in parts are better off, sooner the more rows
+  // there are, and with up to 16 only where columns are few (us of the few rows' kernel and of tiles
+  // with cold weights: 64 x 4096 -> 4096 bf16 25 and 21, 64 x 1024 -> 4096 9 and 15; 32 x 8192 -> 4096
+  // 29 and 25, 20 x 4096 -> 1024 13.6 and 15.4; 8 x 16384 -> 1024 33 and 25, 4 x 8192 -> 1024 17.2 and
+  // 17.7, 2 x 16384 -> 4096 38 and 44).
+  const int64_t row_bytes = k * (single ? 4 : 2);
+  if (which == LinearProduct::kForward && m <= 64 &&
+      (row_bytes < (m > 32 ? 8192 : m > 16 ? 16384 : 32768) || (m <= 16 && n >= 4096))) {
     p.few_rows = true;
     return p;
   }
