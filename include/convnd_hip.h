@@ -290,7 +290,7 @@ int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype para
 typedef struct convnd_hip_linear_problem {
   int64_t rows, inputs, outputs; /* inputs, outputs below 2^21, rows below 2^31 */
   int64_t input_stride;          /* of the rows of input, at least `inputs`, below 2^21 */
-  int64_t residual_stride;       /* of residual */
+  int64_t residual_stride;       /* of residual, where there is one: at least `outputs` */
   int64_t grad_stride;           /* of grad_output (backward), at least `outputs` */
   int activation;                /* convnd_hip_activation */
 } convnd_hip_linear_problem;

@@ -281,3 +281,11 @@ def test_c_abi_refuses_unaligned_workspaces(lib):
     size = lib.convnd_hip_linear_backward_workspace_size(bf16, at, one, one, one, 1, 1, 1)
     expect(lib, lib.convnd_hip_linear_backward(bf16, at, one, one, one, None, one, one, one, odd, size, None), bad,
            "aligned to 16 bytes")
+
+
+def test_c_abi_refuses_overlapping_residual_rows(lib):
+    one = ctypes.c_void_p(16)
+    for stride in (31, 0, -32):
+        p = _capi.LinearProblem(rows=4, inputs=64, outputs=32, input_stride=64, residual_stride=stride, grad_stride=32)
+        expect(lib, lib.convnd_hip_linear(_capi.BFLOAT16, ctypes.byref(p), one, one, None, one, one, None, None, 0, None),
+               _capi.INVALID_ARGUMENT, "apart")

@@ -420,6 +420,8 @@ int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* p
   if (p.rows == 0) return CONVND_HIP_SUCCESS;
   if (input == nullptr || weight == nullptr || output == nullptr)
     return fail(CONVND_HIP_INVALID_ARGUMENT, "input, weight and output must not be null");
+  if (residual != nullptr && p.residual_stride < p.outputs)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs rows at least their length apart");
   Parts ws{static_cast<char*>(workspace)};
   const LinearForward f = lay_out(dtype, p, input, weight, &ws);
   st = check_parts(ws, workspace_size, "linear_act");
