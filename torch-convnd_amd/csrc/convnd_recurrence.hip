@@ -992,8 +992,7 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
   // x 1024 216 and 176; backward 8 x 2048 x 1024 77 and 51); else chunks of the token axis (forward /
   // backward of 1 x 65536 x 512 fp32: 85 / 143 us, in splits with a second reading of the inputs 130 /
   // 180; 4 x 16384 x 1024 bf16: 97 / 174, whole sequences 202 / 404).
-  const bool whole = !backward && a.tokens <= 2048 &&
-                     (groups(64) == 256 || groups(32) == 256 || groups(16) == 256);
+  const bool whole = !backward && a.tokens <= 2048 && (groups(32) == 256 || groups(16) == 256);
   if (a.tokens >= 1024 && groups(64) < 256 && !whole) {
     p.chain = true;
     const int64_t wide = 64 * p.channels_per_lane;
