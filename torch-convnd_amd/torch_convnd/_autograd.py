@@ -246,12 +246,99 @@ def _fake_recurrence_backward(grad_output, grad_last, input, gate, lengths, carr
 # Tokens between the states that gated_recurrence saves (convnd_hip_recurrence_carries).
 RECURRENCE_TILE = 64
 
+
+# Derivatives of the sequence operators while the native library is not loaded (a graph compiled as
+# the first use, a direct call of the operator), as its C++ autograd kernels have them: what the
+# backward reads is no differentiable result, and they are differentiable once. A forward called
+# without keeping it is run again, keeping it.
+
+
+def _keep_apart(ctx, *results):
+    ctx.mark_non_differentiable(*results)
+    ctx.set_materialize_grads(False)
+
+
+def _check_once(name):
+    if torch.is_grad_enabled():
+        raise RuntimeError(
+            f"{name} is differentiable once on the gfx950 kernels; use backend='torch' for create_graph=True"
+        )
+
+
+def _setup_layer_norm(ctx, inputs, output):
+    input, weight, bias, ctx.eps, ctx.kept = inputs
+    ctx.save_for_backward(input, weight, bias, output[1])
+    _keep_apart(ctx, output[1])
+
+
+def _layer_norm_backward(ctx, grad_output, _):
+    _check_once("layer_norm")
+    if grad_output is None:
+        return (None,) * 5
+    input, weight, bias, statistics = ctx.saved_tensors
+    ops = torch.ops.torch_convnd
+    if not ctx.kept:
+        statistics = ops.layer_norm.default(input, weight, bias, ctx.eps, True)[1]
+    mask = list(ctx.needs_input_grad[:3])
+    return (*ops.layer_norm_backward.default(grad_output, input, weight, bias, statistics, mask), None, None)
+
+
+def _setup_linear_act(ctx, inputs, output):
+    input, weight, bias, residual, ctx.activation, ctx.kept = inputs
+    ctx.residual = residual is not None
+    ctx.bias = bias is not None
+    ctx.save_for_backward(input, weight, output[1], None if ctx.kept else bias)
+    _keep_apart(ctx, output[1])
+
+
+def _linear_act_backward(ctx, grad_output, _):
+    _check_once("linear_act")
+    if grad_output is None:
+        return (None,) * 6
+    input, weight, slope, bias = ctx.saved_tensors
+    ops = torch.ops.torch_convnd
+    if not ctx.kept:
+        slope = ops.linear_act.default(input, weight, bias, None, ctx.activation, True)[1]
+    mask = [*ctx.needs_input_grad[:2], ctx.bias and ctx.needs_input_grad[2]]
+    grads = ops.linear_act_backward.default(grad_output, input, weight, slope, ctx.activation, mask)
+    return (*grads, grad_output if ctx.residual else None, None, None)
+
+
+def _setup_recurrence(ctx, inputs, output):
+    input, gate, initial_state, lengths, ctx.kept = inputs
+    ctx.first = initial_state is not None
+    ctx.save_for_backward(input, gate, lengths, output[2], None if ctx.kept else initial_state)
+    _keep_apart(ctx, output[2])
+
+
+def _recurrence_backward(ctx, grad_output, grad_last, _):
+    _check_once("gated_recurrence")
+    if grad_output is None and grad_last is None:
+        return (None,) * 5
+    input, gate, lengths, carries, initial_state = ctx.saved_tensors
+    ops = torch.ops.torch_convnd
+    if not ctx.kept:
+        carries = ops.gated_recurrence.default(input, gate, initial_state, lengths, True)[2]
+    if grad_output is None:
+        grad_output = torch.zeros_like(input)
+    grads = ops.gated_recurrence_backward.default(
+        grad_output, grad_last, input, gate, lengths, carries, ctx.first and ctx.needs_input_grad[2]
+    )
+    return (*grads, None, None)
+
+
+_SEQUENCE_DERIVATIVES = {
+    "layer_norm": (_layer_norm_backward, _setup_layer_norm),
+    "linear_act": (_linear_act_backward, _setup_linear_act),
+    "gated_recurrence": (_recurrence_backward, _setup_recurrence),
+}
+
 _PY_AUTOGRAD = None
 
 
 def release_python_autograd() -> None:
-    """Drop the Python autograd registrations of conv_nd / conv_nd_backward (called right
-    before the native library, whose C++ autograd kernels replace them, is loaded)."""
+    """Drop the Python autograd registrations of the convolution and sequence operators (called
+    right before the native library, whose C++ autograd kernels replace them, is loaded)."""
     global _PY_AUTOGRAD
     if _PY_AUTOGRAD is not None:
         _PY_AUTOGRAD._destroy()
@@ -275,10 +362,11 @@ def register_training() -> None:
     torch.library.register_autograd(
         "torch_convnd::partial_rescale", _rescale_backward, setup_context=_setup_rescale
     )
-    # The convolution operators' derivatives are registered here for use before the native
-    # library loads; that library carries the same contract as C++ autograd kernels
-    # (torch_ops.cpp), and release_python_autograd() drops these registrations just before it
-    # loads, so a training step does not pay the Python autograd machinery per call.
+    # The convolution and sequence operators' derivatives are registered here for use before the
+    # native library loads; that library carries the same contract as C++ autograd kernels
+    # (torch_ops.cpp, torch_sequence_ops.cpp), and release_python_autograd() drops these
+    # registrations just before it loads, so a training step does not pay the Python autograd
+    # machinery per call.
     global _PY_AUTOGRAD
     _PY_AUTOGRAD = torch.library.Library("torch_convnd", "FRAGMENT")
     torch.library.register_autograd(
@@ -290,5 +378,9 @@ def register_training() -> None:
         setup_context=_setup_backward_context,
         lib=_PY_AUTOGRAD,
     )
+    for name, (backward, setup) in _SEQUENCE_DERIVATIVES.items():
+        torch.library.register_autograd(
+            f"torch_convnd::{name}", backward, setup_context=setup, lib=_PY_AUTOGRAD
+        )
     if HAS_NATIVE_VMAP:
         torch.library.register_vmap("torch_convnd::conv_nd", _vmap_forward)
