@@ -49,6 +49,17 @@ __device__ __forceinline__ Gate open_gate(float g) {
   return g >= 0.f ? Gate{r, s} : Gate{s, r};
 }
 
+// A product of gates, the smallest of them `least`. It stays above zero where none is zero, at the
+// smallest value there is, so that an infinite state stays infinite over tokens whose gates' product
+// passes below the type's range, as it does token by token (zero times infinity is NaN). To a finite
+// state that adds less than 5e-7.
+__device__ __forceinline__ float bound_gates(float product, float least) {
+  return fmaxf(product, fminf(least, 1.401298464e-45f));
+}
+__device__ __forceinline__ float join_gates(float a, float b) {
+  return bound_gates(a * b, fminf(a, b));
+}
+
 // The maps v -> a v + b of one lane's channels.
 template <int CPL>
 struct Map {
@@ -58,7 +69,7 @@ struct Map {
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
       b[j] = fmaf(a[j], before.b[j], b[j]);
-      a[j] *= before.a[j];
+      a[j] = join_gates(a[j], before.a[j]);
     }
   }
   __device__ __forceinline__ void clear() {
@@ -66,6 +77,18 @@ struct Map {
     for (int j = 0; j < CPL; ++j) {
       a[j] = 1.f;
       b[j] = 0.f;
+    }
+  }
+  // Bounds `a`, the product of these gates. Apart from the product, whose multiplications wait for
+  // each other (4 x 16384 x 1024 bf16 took 111 us with a bound at each of them, 99 so).
+  template <int N>
+  __device__ __forceinline__ void bound(const float (&gates)[N][CPL]) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      float least = gates[0][j];
+#pragma unroll
+      for (int i = 1; i < N; ++i) least = fminf(least, gates[i][j]);
+      a[j] = bound_gates(a[j], least);
     }
   }
 };
@@ -259,6 +282,7 @@ __global__ __launch_bounds__(64 * kWaves) void recurrence_forward(RecurrenceArgs
         map.a[j] *= q.keep;
         map.b[j] = fmaf(q.keep, map.b[j], add[i][j]);
       }
+    map.bound(keep);
     if (tile + kTile < a.tokens) fetch(tile + kTile);
     scan_runs<CPL, LANES, true>(map, before);
     float h[CPL];
@@ -370,6 +394,7 @@ __global__ __launch_bounds__(64 * NW) void recurrence_backward(RecurrenceArgs a)
         take[i][j] = q.take;
         states.b[j] = fmaf(q.keep, states.b[j], q.take * static_cast<float>(nx[i].v[j]));
       }
+    states.bound(keep);
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i)
 #pragma unroll
@@ -601,6 +626,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_chain(RecurrenceArg
       map.a[j] *= q.keep;
       map.b[j] = fmaf(q.keep, map.b[j], add[i][j]);
     }
+  // Else the two are interleaved, which takes 128 registers and spills (108 without; 4 x 16384 x 1024
+  // bf16 129 us).
+  __builtin_amdgcn_sched_barrier(0);
+  map.bound(keep);
 #pragma unroll
   for (int j = 0; j < CPL; ++j) {
     maps[wave][0][slot + j] = map.a[j];
@@ -617,7 +646,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_chain(RecurrenceArg
       for (int j = 0; j < CPL; ++j) {
         const float aw = maps[w][0][slot + j];
         whole.b[j] = fmaf(aw, whole.b[j], maps[w][1][slot + j]);
-        whole.a[j] *= aw;
+        whole.a[j] = join_gates(whole.a[j], aw);
       }
 #pragma unroll
     for (int j = 0; j < CPL; ++j)
@@ -744,6 +773,7 @@ __global__ __launch_bounds__(64 * kWaves) void recurrence_chain_backward(Recurre
       map.a[j] *= q.keep;
       state[j] = fmaf(q.keep, state[j], q.take * static_cast<float>(nx[i].v[j]));
     }
+  map.bound(keep);
 #pragma unroll
   for (int i = N - 1; i >= 0; --i)
 #pragma unroll
@@ -766,7 +796,7 @@ __global__ __launch_bounds__(64 * kWaves) void recurrence_chain_backward(Recurre
       for (int j = 0; j < CPL; ++j) {
         const float aw = maps[w][0][slot + j];
         whole.b[j] = fmaf(aw, whole.b[j], maps[w][1][slot + j]);
-        whole.a[j] *= aw;
+        whole.a[j] = join_gates(whole.a[j], aw);
       }
 #pragma unroll
     for (int j = 0; j < CPL; ++j)
