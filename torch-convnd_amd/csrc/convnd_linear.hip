@@ -59,11 +59,13 @@ struct Fragment<float> {
 __device__ __forceinline__ void load_lds16(u32x4 rows, unsigned dst, unsigned offset) {
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst),
-      "v"(offset), "s"(rows));
+      "v"(offset), "s"(rows)
+      : "m0");
 }
 __device__ __forceinline__ void load_lds4(u32x4 rows, unsigned dst, unsigned offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(dst),
-               "v"(offset), "s"(rows));
+               "v"(offset), "s"(rows)
+               : "m0");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
