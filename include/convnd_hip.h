@@ -260,7 +260,9 @@ int convnd_hip_timing_read(int kernel, double* total_ms, int64_t* launches);
  * Layer norm, linear layer and gated recurrence of token sequences around the convolution. No
  * counterpart in the reference. Types float32, float16 and bfloat16 (anything else returns
  * CONVND_HIP_INVALID_ARGUMENT); strides are in elements; statistics, states and sums are float32.
- * The gradients asked for are overwritten, not added to. A workspace is aligned to 16 bytes. */
+ * The gradients asked for are overwritten, not added to. A workspace is aligned to 16 bytes. Sizes
+ * that would take 2^32 threads or more in one launch (2^23 sequences of 9 tokens and up to 64 channels,
+ * 2^31 rows of 16 outputs, parameter gradients of 2^27 channels) return CONVND_HIP_INVALID_ARGUMENT. */
 
 /* output = (input - mean) * rstd * weight + bias for rows of `channels` contiguous elements,
  * `input_stride` apart in the input, contiguous in the output; mean and the variance are over a

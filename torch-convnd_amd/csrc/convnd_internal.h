@@ -536,6 +536,10 @@ int fail(int status, const std::string& message);
 int hip_check(hipError_t err, const char* what);
 // a * b into *out, or false where that is negative or passes int64.
 bool mul_ok(int64_t a, int64_t b, int64_t* out);
+// What one launch may have: fewer than 2^32 threads along an axis of the grid.
+inline bool launch_fits(int64_t workgroups, int64_t threads) {
+  return workgroups <= ((int64_t{1} << 32) - 1) / threads;
+}
 
 // Layer norm (convnd_norm.hip): rows of `channels` contiguous elements; strides in elements.
 struct NormArgs {
@@ -583,7 +587,7 @@ struct LinearArgs {
 enum class LinearProduct { kForward, kGradInput, kGradWeight };
 struct LinearPlan {
   bool few_rows;
-  int tile;         // 64, 128 or 256
+  int tile;         // 64, 128 or 256; 0 without few_rows: too many tiles of any size for a launch
   int splits;
   int64_t split_k;
 };
@@ -643,7 +647,8 @@ struct RecurrencePlan {
   int lanes;              // of a wave along the channels: 64, 32 or 16
   bool chain;             // chunks of the token axis instead
   int64_t word_count;     // their workspace in 8-byte words
-  int64_t workgroups;
+  int64_t workgroups;     // of the launch, and the threads of each
+  int threads;
 };
 // Distance of the saved states in tokens: every plan's tiles and chunks start at whole multiples of
 // it (or are a single one).

@@ -1007,14 +1007,14 @@ hipError_t launch_both(const LinearArgs& x, const LinearPlan& xp, float* x_parti
 // `alone` a K value. (16-bit at 8192^3: 256 x 256 1370 TFLOP/s, 128 x 128 1160; float is bound by its
 // MFMA rate at either tile, 130.)
 struct TileCost {
-  int tile, slots;
+  int tile, threads, slots;
   float set_up, alone, turn, full;
 };
-constexpr TileCost kTiles16[] = {{64, 1280, 4.0f, 0.0046f, 2.7f, 0.0150f},
-                                 {128, 512, 5.0f, 0.0102f, 4.0f, 0.0140f},
-                                 {256, 256, 4.5f, 0.0210f, 6.0f, 0.0238f}};
-constexpr TileCost kTiles32[] = {{64, 1280, 3.9f, 0.0206f, 4.8f, 0.0772f},
-                                 {128, 512, 5.7f, 0.0656f, 7.9f, 0.1122f}};
+constexpr TileCost kTiles16[] = {{64, 256, 1280, 4.0f, 0.0046f, 2.7f, 0.0150f},
+                                 {128, 256, 512, 5.0f, 0.0102f, 4.0f, 0.0140f},
+                                 {256, 512, 256, 4.5f, 0.0210f, 6.0f, 0.0238f}};
+constexpr TileCost kTiles32[] = {{64, 256, 1280, 3.9f, 0.0206f, 4.8f, 0.0772f},
+                                 {128, 256, 512, 5.7f, 0.0656f, 7.9f, 0.1122f}};
 
 // `groups` workgroups of `k` K values on the average, at most `most`: bound by the longest, or by what the
 // busiest compute unit is given.
@@ -1087,12 +1087,13 @@ LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, 
   const uint32_t stage = single ? 32 : 64, stages = over(k, stage);
   float best = 0;
   each_tile(single, [&](const TileCost& c) {
-    const uint32_t tiles = over(m, c.tile) * over(n, c.tile);
+    const int64_t tiles = int64_t{over(m, c.tile)} * over(n, c.tile);
     for (const uint32_t parts : kParts) {
       const Split split(stages, (stages + parts - 1) / parts);
       if (parts > 1 && split.stages < 4) break;
+      if (!launch_fits(tiles * split.count, c.threads)) break;
       const float length = static_cast<float>(split.stages * stage);
-      float us = tiles_time(c, tiles * split.count,
+      float us = tiles_time(c, static_cast<uint32_t>(tiles * split.count),
                             static_cast<float>(k) / static_cast<float>(split.count), length);
       if (split.count > 1)
         us += join_time(single, split_bytes(m, n, split.count), split.count);
@@ -1116,7 +1117,8 @@ void plan_gradients(convnd_hip_dtype dtype, int64_t rows, int64_t inputs, int64_
   float best = 0;
   each_tile(single, [&](const TileCost& c) {
     const uint32_t across = over(inputs, c.tile);
-    const uint32_t x_tiles = over(rows, c.tile) * across, w_tiles = over(outputs, c.tile) * across;
+    const int64_t x_tiles = int64_t{over(rows, c.tile)} * across;
+    const int64_t w_tiles = int64_t{over(outputs, c.tile)} * across;
     const float work = (static_cast<float>(x_tiles) * static_cast<float>(x_stages) +
                         static_cast<float>(w_tiles) * static_cast<float>(w_stages)) *
                        static_cast<float>(stage);
@@ -1124,8 +1126,10 @@ void plan_gradients(convnd_hip_dtype dtype, int64_t rows, int64_t inputs, int64_
       const uint32_t each = (longest + parts - 1) / parts;
       if (parts > 1 && each < 4) break;
       const Split xs(x_stages, each), ws(w_stages, each);
-      const uint32_t groups = x_tiles * xs.count + w_tiles * ws.count;
-      float us = tiles_time(c, groups, work / static_cast<float>(groups),
+      const int64_t groups = x_tiles * xs.count + w_tiles * ws.count;
+      // With the bias's sums in the same launch.
+      if (!launch_fits(groups + over(outputs, 32), c.threads)) break;
+      float us = tiles_time(c, static_cast<uint32_t>(groups), work / static_cast<float>(groups),
                             static_cast<float>(std::max(xs.stages, ws.stages) * stage));
       if (xs.count > 1 || ws.count > 1)
         us += join_time(single,

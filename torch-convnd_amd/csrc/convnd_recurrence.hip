@@ -891,11 +891,10 @@ __global__ __launch_bounds__(256) void clear_words(Word* words, int64_t count) {
 }
 
 template <typename T, int CPL>
-hipError_t launch_chain(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
+hipError_t launch_chain(const RecurrenceArgs& a, bool backward, const RecurrencePlan& p,
+                        hipStream_t stream) {
   constexpr int kForward = kForwardRun / CPL, kBackward = kBackwardRun / CPL;
-  const int64_t rows = (a.channels + 64 * CPL - 1) / (64 * CPL) * a.batch;
-  const int64_t chunk = kWaves * (backward ? kBackward : kForward);
-  const dim3 grid(static_cast<unsigned>(rows * ((a.tokens + chunk - 1) / chunk)));
+  const dim3 grid(static_cast<unsigned>(p.workgroups)), block(static_cast<unsigned>(p.threads));
   const int64_t count = a.word_count;
   hipLaunchKernelGGL(clear_words,
                      dim3(static_cast<unsigned>(std::min<int64_t>((count + 255) / 256, 2048))),
@@ -903,11 +902,9 @@ hipError_t launch_chain(const RecurrenceArgs& a, bool backward, hipStream_t stre
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   if (backward)
-    hipLaunchKernelGGL((recurrence_chain_backward<T, CPL, kBackward>), grid,
-                       dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((recurrence_chain_backward<T, CPL, kBackward>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((recurrence_chain<T, CPL, kForward>), grid, dim3(64 * kWaves), 0,
-                       stream, a);
+    hipLaunchKernelGGL((recurrence_chain<T, CPL, kForward>), grid, block, 0, stream, a);
   return hipGetLastError();
 }
 
@@ -957,9 +954,9 @@ __global__ __launch_bounds__(kStepThreads) void recurrence_step(RecurrenceArgs a
 }
 
 template <typename T, int CPL, int LANES>
-void launch_whole(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
-  const int64_t strips = (a.channels + LANES * CPL - 1) / (LANES * CPL);
-  const dim3 grid(static_cast<unsigned>(strips * a.batch)), block(64 * kWaves);
+void launch_whole(const RecurrenceArgs& a, bool backward, const RecurrencePlan& p,
+                  hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.workgroups)), block(static_cast<unsigned>(p.threads));
   if constexpr (CPL == 1) {
     if (backward) {
       hipLaunchKernelGGL((recurrence_backward<T, LANES, kWaves>), grid, block, 0, stream, a);
@@ -972,24 +969,19 @@ void launch_whole(const RecurrenceArgs& a, bool backward, hipStream_t stream) {
 template <typename T, int CPL>
 hipError_t launch_channels(const RecurrenceArgs& a, bool backward, const RecurrencePlan& p,
                            hipStream_t stream) {
-  if (p.chain) return launch_chain<T, CPL>(a, backward, stream);
+  if (p.chain) return launch_chain<T, CPL>(a, backward, p, stream);
   if (backward && CPL != 1) return hipErrorInvalidValue;  // no plan has it
-  if (p.waves == 1 && backward) {
-    const int64_t strips = (a.channels + 63) / 64;
-    hipLaunchKernelGGL((recurrence_backward<T, 64, 1>),
-                       dim3(static_cast<unsigned>(strips * a.batch)), dim3(64), 0, stream, a);
-  } else if (p.waves == 1) {
-    const int64_t threads = (a.channels + CPL - 1) / CPL * a.batch;
-    hipLaunchKernelGGL((recurrence_step<T, CPL>),
-                       dim3(static_cast<unsigned>((threads + kStepThreads - 1) / kStepThreads)),
-                       dim3(kStepThreads), 0, stream, a);
-  } else if (p.lanes == 64) {
-    launch_whole<T, CPL, 64>(a, backward, stream);
-  } else if (p.lanes == 32) {
-    launch_whole<T, CPL, 32>(a, backward, stream);
-  } else {
-    launch_whole<T, CPL, 16>(a, backward, stream);
-  }
+  const dim3 grid(static_cast<unsigned>(p.workgroups)), block(static_cast<unsigned>(p.threads));
+  if (p.waves == 1 && backward)
+    hipLaunchKernelGGL((recurrence_backward<T, 64, 1>), grid, block, 0, stream, a);
+  else if (p.waves == 1)
+    hipLaunchKernelGGL((recurrence_step<T, CPL>), grid, block, 0, stream, a);
+  else if (p.lanes == 64)
+    launch_whole<T, CPL, 64>(a, backward, p, stream);
+  else if (p.lanes == 32)
+    launch_whole<T, CPL, 32>(a, backward, p, stream);
+  else
+    launch_whole<T, CPL, 16>(a, backward, p, stream);
   return hipGetLastError();
 }
 
@@ -1030,6 +1022,7 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
     const int64_t chunks = (a.tokens + chunk - 1) / chunk;
     p.word_count = kChainHead + groups(64) * wide * (chunks + (chunks + kGroup - 1) / kGroup);
     p.workgroups = groups(64) * chunks;
+    p.threads = 64 * kWaves;
     return p;
   }
   // The forward takes one channel a lane in 16 bits too where that makes workgroups for idle compute
@@ -1045,6 +1038,12 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
          groups(p.lanes) < 256)
     p.lanes /= 2;
   p.workgroups = groups(p.lanes);
+  p.threads = 64 * p.waves;
+  if (p.waves == 1 && !backward) {  // the step kernel
+    const int64_t each = (a.channels + p.channels_per_lane - 1) / p.channels_per_lane;
+    p.workgroups = (each * a.batch + kStepThreads - 1) / kStepThreads;
+    p.threads = kStepThreads;
+  }
   return p;
 }
 

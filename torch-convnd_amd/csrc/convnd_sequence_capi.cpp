@@ -1,6 +1,5 @@
 // C ABI of the sequence operators (layer norm, linear layer, gated recurrence): argument checks and launches.
 #include <algorithm>
-#include <limits>
 
 #include "convnd_internal.h"
 
@@ -105,8 +104,9 @@ int plan_call(convnd_hip_dtype dtype, RecurrenceArgs* a, bool backward, void* wo
   if (st != CONVND_HIP_SUCCESS) return st;
   a->words = workspace;
   a->word_count = p->word_count;
-  if (p->workgroups > std::numeric_limits<int32_t>::max())
-    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_recurrence sizes are too large");
+  if (!launch_fits(p->workgroups, p->threads))
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_recurrence sizes are too large: more than 2^32 threads");
   return CONVND_HIP_SUCCESS;
 }
 
@@ -180,6 +180,13 @@ int fill_padded(convnd_hip_dtype dtype, const Padded& p, const void* data, int64
 
 float* partial_sums(const LinearPlan& p, int64_t m, int64_t n, Parts* ws) {
   return p.splits > 1 ? static_cast<float*>(ws->take(p.splits * m * n * sizeof(float))) : nullptr;
+}
+
+// Whether the sizes leave a plan that one launch can hold.
+int check_plan(const LinearPlan& p) {
+  if (p.few_rows || p.tile != 0) return CONVND_HIP_SUCCESS;
+  return fail(CONVND_HIP_INVALID_ARGUMENT,
+              "linear_act sizes are too large: more than 2^32 threads");
 }
 
 int check_parts(const Parts& ws, size_t size, const char* what) {
@@ -297,6 +304,9 @@ int convnd_hip_layer_norm_backward(convnd_hip_dtype dtype, convnd_hip_dtype para
   if (st == CONVND_HIP_SUCCESS) st = check_norm(dtype, param_dtype, rows, channels, grad_stride);
   if (st != CONVND_HIP_SUCCESS) return st;
   const bool params = grad_weight != nullptr || grad_bias != nullptr;
+  if (params && channels >= int64_t{1} << 27)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "layer_norm parameter gradients need fewer than 2^27 channels");
   if (!params && (grad_input == nullptr || rows == 0)) return CONVND_HIP_SUCCESS;
   if (rows > 0 && (grad_output == nullptr || input == nullptr || mean == nullptr || rstd == nullptr))
     return fail(CONVND_HIP_INVALID_ARGUMENT,
@@ -424,7 +434,8 @@ int convnd_hip_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* p
     return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs rows at least their length apart");
   Parts ws{static_cast<char*>(workspace)};
   const LinearForward f = lay_out(dtype, p, input, weight, &ws);
-  st = check_parts(ws, workspace_size, "linear_act");
+  st = check_plan(f.plan);
+  if (st == CONVND_HIP_SUCCESS) st = check_parts(ws, workspace_size, "linear_act");
   if (st != CONVND_HIP_SUCCESS) return st;
   const auto on = static_cast<hipStream_t>(stream);
   st = fill_padded(dtype, f.x, input, p.input_stride, p.rows, p.inputs, on);
@@ -490,7 +501,9 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
   const LinearBackward b =
       lay_out_backward(dtype, p, grad_output, input, weight, grad_input != nullptr,
                        grad_weight != nullptr, grad_bias != nullptr, &ws);
-  st = check_parts(ws, workspace_size, "linear_act backward");
+  if (grad_input != nullptr) st = check_plan(b.input_plan);
+  if (st == CONVND_HIP_SUCCESS && grad_weight != nullptr) st = check_plan(b.weight_plan);
+  if (st == CONVND_HIP_SUCCESS) st = check_parts(ws, workspace_size, "linear_act backward");
   if (st != CONVND_HIP_SUCCESS) return st;
   const bool both = grad_input != nullptr && grad_weight != nullptr;
   if (b.make_dz || grad_bias != nullptr) {
