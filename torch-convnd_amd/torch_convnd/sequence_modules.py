@@ -143,6 +143,8 @@ class GatedConvBlock(nn.Module):
         kept = self.kernel_size - 1
         if lengths is None:
             window = tokens[:, tokens.shape[1] - kept :]
+            if input.shape[1] > kept:  # a view would hold the whole prompt as long as the state lives
+                window = window.clone(memory_format=torch.contiguous_format)
         else:  # the last tokens before each sequence's end
             first = lengths.clamp(0, input.shape[1]).long()[:, None, None]
             index = first + torch.arange(kept, device=input.device)[None, :, None]
