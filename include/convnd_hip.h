@@ -330,6 +330,13 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
                                void* grad_bias, void* workspace, size_t workspace_size,
                                void* stream);
 
+/* JSON description of a linear layer's launch plan (kernel, tile, parts of K, workgroups) written to
+ * `buffer` (NUL-terminated, truncated to `length`). `which`: 0 forward, 1 the input's gradient alone,
+ * 2 the weight's alone, 3 both. Diagnostic only; touches no device. */
+int convnd_hip_linear_plan_describe(convnd_hip_dtype dtype,
+                                    const convnd_hip_linear_problem* problem, int which,
+                                    char* buffer, size_t length);
+
 /* Gated linear recurrence over the token axis,
  *   h[t] = a[t] h[t-1] + (1 - a[t]) input[t],  a[t] = sigmoid(gate[t]),  h[-1] = first,
  * for input and gate [batch, tokens, channels] with contiguous channels and the batch and token
@@ -367,6 +374,12 @@ int convnd_hip_recurrence_backward(convnd_hip_dtype dtype, const convnd_hip_recu
                                    const float* carries, void* grad_input, void* grad_gate,
                                    float* grad_first, void* workspace, size_t workspace_size,
                                    void* stream);
+
+/* JSON description of a recurrence's launch plan (kernel, channels a lane, lanes, tokens of a tile or
+ * chunk, workgroups), as above; `backward` 0 or 1. */
+int convnd_hip_recurrence_plan_describe(convnd_hip_dtype dtype,
+                                        const convnd_hip_recurrence_problem* problem, int backward,
+                                        char* buffer, size_t length);
 
 #ifdef __cplusplus
 } /* extern "C" */

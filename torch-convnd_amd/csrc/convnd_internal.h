@@ -646,6 +646,7 @@ struct RecurrencePlan {
   int channels_per_lane;  // 1 or 2
   int lanes;              // of a wave along the channels: 64, 32 or 16
   bool chain;             // chunks of the token axis instead
+  int tile;               // tokens of a workgroup's tile or chunk
   int64_t word_count;     // their workspace in 8-byte words
   int64_t workgroups;     // of the launch, and the threads of each
   int threads;

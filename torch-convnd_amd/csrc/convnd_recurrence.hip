@@ -1018,8 +1018,8 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
   if (a.tokens >= 1024 && groups(64) < 256 && !whole) {
     p.chain = true;
     const int64_t wide = 64 * p.channels_per_lane;
-    const int64_t chunk = kWaves * (backward ? kBackwardRun : kForwardRun) / p.channels_per_lane;
-    const int64_t chunks = (a.tokens + chunk - 1) / chunk;
+    p.tile = kWaves * (backward ? kBackwardRun : kForwardRun) / p.channels_per_lane;
+    const int64_t chunks = (a.tokens + p.tile - 1) / p.tile;
     p.word_count = kChainHead + groups(64) * wide * (chunks + (chunks + kGroup - 1) / kGroup);
     p.workgroups = groups(64) * chunks;
     p.threads = 64 * kWaves;
@@ -1039,6 +1039,7 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
     p.lanes /= 2;
   p.workgroups = groups(p.lanes);
   p.threads = 64 * p.waves;
+  p.tile = p.waves * (64 / p.lanes) * kRun;
   if (p.waves == 1 && !backward) {  // the step kernel
     const int64_t each = (a.channels + p.channels_per_lane - 1) / p.channels_per_lane;
     p.workgroups = (each * a.batch + kStepThreads - 1) / kStepThreads;

@@ -1,5 +1,7 @@
 // C ABI of the sequence operators (layer norm, linear layer, gated recurrence): argument checks and launches.
 #include <algorithm>
+#include <cstring>
+#include <string>
 
 #include "convnd_internal.h"
 
@@ -251,6 +253,28 @@ LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_
   if (need_input) b.input_partial = partial_sums(b.input_plan, p.rows, p.inputs, ws);
   if (need_weight) b.weight_partial = partial_sums(b.weight_plan, p.outputs, p.inputs, ws);
   return b;
+}
+
+// A plan's description as JSON; numbers only beside the kernel's name.
+struct Description {
+  std::string text;
+  explicit Description(const char* kernel) : text(std::string("{\"kernel\":\"") + kernel + "\"") {}
+  Description& add(const char* name, int64_t value) {
+    text += std::string(",\"") + name + "\":" + std::to_string(value);
+    return *this;
+  }
+  int write(char* buffer, size_t length) const {
+    if (buffer == nullptr || length == 0) return CONVND_HIP_SUCCESS;
+    const std::string whole = text + "}";
+    const size_t n = std::min(length - 1, whole.size());
+    std::memcpy(buffer, whole.data(), n);
+    buffer[n] = '\0';
+    return CONVND_HIP_SUCCESS;
+  }
+};
+
+int64_t tiles_of(const LinearPlan& p, int64_t m, int64_t n) {
+  return ((m + p.tile - 1) / p.tile) * ((n + p.tile - 1) / p.tile) * p.splits;
 }
 
 }  // namespace
@@ -562,6 +586,58 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
                                            b.weight_partial, on),
                      "linear weight gradient launch");
   return st;
+}
+
+int convnd_hip_linear_plan_describe(convnd_hip_dtype dtype,
+                                    const convnd_hip_linear_problem* problem, int which,
+                                    char* buffer, size_t length) {
+  int st = check_linear(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const convnd_hip_linear_problem& p = *problem;
+  if (which < 0 || which > 3 || p.rows == 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "which must be 0 to 3, and rows positive");
+  LinearPlan x{}, w{};
+  if (which == 0)
+    x = plan_product(dtype, LinearProduct::kForward, p.rows, p.outputs, p.inputs);
+  else if (which == 1)
+    x = plan_product(dtype, LinearProduct::kGradInput, p.rows, p.inputs, p.outputs);
+  else if (which == 2)
+    x = plan_product(dtype, LinearProduct::kGradWeight, p.outputs, p.inputs, p.rows);
+  else
+    plan_gradients(dtype, p.rows, p.inputs, p.outputs, &x, &w);
+  st = check_plan(x);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  if (x.few_rows)
+    return Description("few_rows").add("workgroups", (p.outputs + 15) / 16).write(buffer, length);
+  if (which == 3)
+    return Description("both_gradients")
+        .add("tile", x.tile)
+        .add("input_splits", x.splits)
+        .add("weight_splits", w.splits)
+        .add("workgroups", tiles_of(x, p.rows, p.inputs) + tiles_of(w, p.outputs, p.inputs))
+        .write(buffer, length);
+  const int64_t m = which == 2 ? p.outputs : p.rows, n = which == 0 ? p.outputs : p.inputs;
+  return Description("tiles")
+      .add("tile", x.tile)
+      .add("splits", x.splits)
+      .add("workgroups", tiles_of(x, m, n))
+      .write(buffer, length);
+}
+
+int convnd_hip_recurrence_plan_describe(convnd_hip_dtype dtype,
+                                        const convnd_hip_recurrence_problem* problem, int backward,
+                                        char* buffer, size_t length) {
+  const int st = check_recurrence(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const RecurrencePlan p = plan_recurrence(dtype, to_args(*problem), backward != 0);
+  const bool step = p.waves == 1 && backward == 0;
+  return Description(p.chain ? "chain" : step ? "step" : "whole")
+      .add("channels_per_lane", p.channels_per_lane)
+      .add("lanes", p.lanes)
+      .add("waves", p.waves)
+      .add("tile", p.tile)
+      .add("workgroups", p.workgroups)
+      .write(buffer, length);
 }
 
 }  // extern "C"

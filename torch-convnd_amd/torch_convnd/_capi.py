@@ -40,10 +40,12 @@ EXPORTED_SYMBOLS = (
     "convnd_hip_linear",
     "convnd_hip_linear_backward_workspace_size",
     "convnd_hip_linear_backward",
+    "convnd_hip_linear_plan_describe",
     "convnd_hip_recurrence_carries",
     "convnd_hip_recurrence_workspace_size",
     "convnd_hip_recurrence",
     "convnd_hip_recurrence_backward",
+    "convnd_hip_recurrence_plan_describe",
 )
 
 CHANNELS_FIRST, CHANNELS_LAST, CHANNELS_LAST_INPUT = 0, 1, 2
@@ -179,6 +181,10 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     library.convnd_hip_recurrence_backward.argtypes = [
         ctypes.c_int, R, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp
     ]
+    library.convnd_hip_linear_plan_describe.restype = ctypes.c_int
+    library.convnd_hip_linear_plan_describe.argtypes = [ctypes.c_int, L, ctypes.c_int, ctypes.c_char_p, sz]
+    library.convnd_hip_recurrence_plan_describe.restype = ctypes.c_int
+    library.convnd_hip_recurrence_plan_describe.argtypes = [ctypes.c_int, R, ctypes.c_int, ctypes.c_char_p, sz]
     return library
 
 
@@ -223,3 +229,28 @@ def plan_details(library, x_shape, w_shape, stride, padding, dilation, groups, d
             raise RuntimeError(library.convnd_hip_last_error().decode())
         out.append(json.loads(buffer.value.decode()))
     return tuple(out)
+
+
+def _described(library, describe, *args):
+    import json
+
+    buffer = ctypes.create_string_buffer(1024)
+    if describe(*args, buffer, len(buffer)) != SUCCESS:
+        raise RuntimeError(library.convnd_hip_last_error().decode())
+    return json.loads(buffer.value.decode())
+
+
+def linear_plan(library, rows, inputs, outputs, dtype, which=0):
+    """Launch plan of a linear layer (0 forward, 1 and 2 one gradient, 3 both) as a dict."""
+    p = LinearProblem(rows=rows, inputs=inputs, outputs=outputs, input_stride=inputs, grad_stride=outputs)
+    return _described(library, library.convnd_hip_linear_plan_describe, dtype_code(dtype), ctypes.byref(p), which)
+
+
+def recurrence_plan(library, batch, tokens, channels, dtype, backward=False):
+    """Launch plan of a gated recurrence as a dict."""
+    p = RecurrenceProblem(
+        batch=batch, tokens=tokens, channels=channels, input_batch=tokens * channels, input_token=channels,
+        gate_batch=tokens * channels, gate_token=channels,
+    )
+    describe = library.convnd_hip_recurrence_plan_describe
+    return _described(library, describe, dtype_code(dtype), ctypes.byref(p), int(backward))
