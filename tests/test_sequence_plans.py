@@ -41,3 +41,33 @@ def test_refusals(lib):
     p = _capi.LinearProblem(rows=4, inputs=16, outputs=16, input_stride=16)
     assert lib.convnd_hip_linear_plan_describe(_capi.FLOAT32, ctypes.byref(p), 0, buffer, 8) == _capi.SUCCESS
     assert len(buffer.value) == 7  # truncated, with its end
+
+
+# Batch and tokens of 1024 channels where one of the two forward kernels was at least 8 % faster.
+FASTER = {
+    ("whole", torch.bfloat16): [(6, 1024), (7, 1024), (8, 1024), (12, 1024), (16, 1024), (6, 1536), (7, 1536), (8, 1536)],
+    ("whole", torch.float32): [(3, 1024), (4, 1024), (6, 1024), (8, 1024), (12, 1024), (15, 1024), (4, 2048), (6, 2048)],
+    ("chain", torch.bfloat16): [(2, 1536), (2, 2048), (4, 2560), (6, 2560), (9, 1536), (10, 2048), (4, 4096), (7, 4096)],
+    ("chain", torch.float32): [(2, 2048), (2, 4096), (3, 4096), (5, 4096)],
+}
+
+
+@pytest.mark.parametrize(("kernel", "dtype", "sizes"), [(*k, v) for k, v in FASTER.items()])
+def test_forward_takes_the_faster_kernel(lib, kernel, dtype, sizes):
+    for batch, tokens in sizes:
+        assert _capi.recurrence_plan(lib, batch, tokens, 1024, dtype)["kernel"] == kernel, (batch, tokens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_neighbouring_sizes_take_one_kernel(lib, dtype):
+    """No single count of workgroups, tokens or channels has a rule of its own."""
+    for batch, tokens in ((7, 1200), (8, 2048), (15, 1100), (4, 6000)):
+        kernels = {
+            _capi.recurrence_plan(lib, batch, t, c, dtype)["kernel"]
+            for t in range(tokens - 3, tokens + 4)
+            for c in (992, 1008, 1024)
+        }
+        assert len(kernels) == 1, (batch, tokens, kernels)
+    for batch in range(1, 16):
+        kernels = [_capi.recurrence_plan(lib, batch, t, 1024, dtype)["kernel"] for t in range(1024, 9000, 97)]
+        assert kernels == sorted(kernels, reverse=True), batch  # whole sequences, from some length on chunks

@@ -996,6 +996,33 @@ hipError_t launch_recurrence_typed(const RecurrenceArgs& a, bool backward, const
 
 }  // namespace
 
+namespace {
+
+// What a forward of 1024 tokens and more takes (us), in whole sequences at one workgroup or less a
+// compute unit and in chunks of the token axis: a share of each 1024 tokens, which follow each other
+// on 16, 32 or 64 lanes, and of each MB moved. Fitted to 87 sizes of 1024 to 4096 tokens and 32 to 256
+// workgroups. What it takes is at most 8 % slower than the other there (7 x 1024 x 1024 bf16 whole 14.4 us, in
+// chunks 19.4; 7 x 2048 x 1024 30.4 and 31.8; 7 x 4096 x 1024 58 and 51), at most 6 % in 44 sizes besides.
+struct ForwardCost {
+  float whole, tokens[3], bytes;
+  float chain, chain_tokens, chain_bytes;
+};
+constexpr ForwardCost kOneChannel = {-0.9f, {6.4f, 7.1f, 12.0f}, 0.148f, 5.7f, 0.4f, 0.204f};
+constexpr ForwardCost kTwoChannels = {1.0f, {9.6f, 15.8f, 26.6f}, 0.094f, 8.3f, 1.1f, 0.218f};
+
+bool weigh_whole(convnd_hip_dtype dtype, const RecurrenceArgs& a, int channels_per_lane, int lanes) {
+  const ForwardCost& c = channels_per_lane == 2 ? kTwoChannels : kOneChannel;
+  const float thousands = static_cast<float>(a.tokens) / 1024.f;
+  const float mb = static_cast<float>(a.batch) * static_cast<float>(a.tokens) *
+                   static_cast<float>(a.channels) *
+                   (dtype == CONVND_HIP_FLOAT32 ? 12e-6f : 6e-6f);
+  const float turn = c.tokens[lanes == 16 ? 0 : lanes == 32 ? 1 : 2];
+  return c.whole + turn * thousands + c.bytes * mb <
+         c.chain + c.chain_tokens * thousands + c.chain_bytes * mb;
+}
+
+}  // namespace
+
 RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward) {
   RecurrencePlan p{};
   p.waves = a.tokens <= kRun ? 1 : 8;
@@ -1008,14 +1035,21 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
     return std::max<int64_t>(1, a.batch) * ((a.channels + wide - 1) / wide);
   };
   // Whole sequences a workgroup where those fill the chip (8 x 4096 x 4096 fp16, 256 workgroups:
-  // forward 163 us, in chunks 176) or are short (600 tokens of 256 channels, fp32: 7 us against 11), up to
-  // 2048 tokens also where fewer lanes make just one for each compute unit of the forward (8 x 1024 x
-  // 1024 bf16 16 and 21, 16 x 2048 x 1024 48 and 52; 7 x 2000 x 1024, 224 of them, 41 and 31, 8 x 16384
-  // x 1024 216 and 176; backward 8 x 2048 x 1024 77 and 51); else chunks of the token axis (forward /
-  // backward of 1 x 65536 x 512 fp32: 85 / 143 us, in splits with a second reading of the inputs 130 /
-  // 180; 4 x 16384 x 1024 bf16: 97 / 174, whole sequences 202 / 404).
-  const bool whole = !backward && a.tokens <= 2048 && (groups(32) == 256 || groups(16) == 256);
-  if (a.tokens >= 1024 && groups(64) < 256 && !whole) {
+  // forward 163 us, in chunks 176) or are short (600 tokens of 256 channels, fp32: 7 us against 11); else
+  // chunks of the token axis (forward / backward of 1 x 65536 x 512 fp32: 85 / 143 us, in splits with a
+  // second reading of the inputs 130 / 180; 4 x 16384 x 1024 bf16: 97 / 174, whole sequences 202 / 404;
+  // backward 8 x 2048 x 1024 51 and 77). The forward weighs the two: whole sequences on as few lanes as
+  // leave a workgroup for each compute unit at most.
+  if (a.tokens >= 1024 && groups(64) < 256) {
+    int lanes = 16;
+    while (lanes < 64 && groups(lanes) > 256) lanes *= 2;
+    if (!backward && weigh_whole(dtype, a, p.channels_per_lane, lanes)) {
+      p.lanes = lanes;
+      p.tile = kWaves * (64 / lanes) * kRun;
+      p.workgroups = groups(lanes);
+      p.threads = 64 * kWaves;
+      return p;
+    }
     p.chain = true;
     const int64_t wide = 64 * p.channels_per_lane;
     p.tile = kWaves * (backward ? kBackwardRun : kForwardRun) / p.channels_per_lane;
