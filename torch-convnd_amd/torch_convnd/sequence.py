@@ -114,8 +114,10 @@ def linear_act(
     ``weight`` is [outputs, inputs], ``bias`` [outputs], ``residual`` of the output's shape
     [..., outputs]; all in the input's dtype. ``activation`` as for ``conv_nd``: "relu", "gelu",
     "gelu_tanh" or None. On the gfx950 path all of it is one rounding of the float32 sums (a training
-    step also keeps the activation's slope, in 16 bits beside 16-bit types, else float32). ``input``
-    and ``residual`` may be slices of wider rows. Under autocast the operands are cast to its dtype.
+    step also keeps the activation's slope, in 16 bits beside 16-bit types, else float32, and its
+    backward rounds the gradient before the activation to the element type). ``input`` and
+    ``residual`` may be slices of wider rows. Under autocast the operands are cast to its dtype, the
+    residual too: a residual stream in float32 is added outside (``x + linear_act(...)``).
     """
     if activation is not None and activation not in _ACTIVATIONS:
         raise ValueError(f"Invalid activation {activation!r}; expected 'relu', 'gelu' or 'gelu_tanh'")

@@ -87,6 +87,8 @@ class GatedConvBlock(nn.Module):
     ``forward(x, state, lengths)`` returns ``(x, state)``; the state (the last ``kernel_size - 1``
     normalised tokens and the recurrence's state) starts the next call, so a prompt is followed by
     calls of one token. ``lengths`` [batch]: tokens at and past a sequence's length are padding.
+    ``backend`` is that of every part; "auto" leaves the convolution, which has one axis, to PyTorch,
+    as it does for ``Conv1d``, and "native" runs it on the gfx950 kernels too.
     """
 
     def __init__(
