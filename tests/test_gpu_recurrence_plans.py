@@ -37,12 +37,80 @@ CASES = [
     [(dtype, *rest) for types, *rest in CASES for dtype in types],
 )
 def test_forms(dtype, batch, tokens, c, forward, backward):
+    for plan in planned(dtype, batch, tokens, c, forward, backward):
+        # More than one tile, or group of 32 chunks, in the kernels that have them.
+        assert tokens > plan["tile"] * {"whole": 1, "chain": 32}.get(plan["kernel"], 0) or tokens <= 8, plan
+    check(dtype, batch, tokens, c)
+
+
+# A forward of whole sequences leaves the states that a backward of chunks starts from.
+MIXED = [
+    (HALF, 6, 1100, 1022, ("whole", 2, 16), ("chain", 2, 64)),
+    (HALF, 12, 1100, 1022, ("whole", 2, 32), ("chain", 2, 64)),
+    (HALF, 30, 1030, 1022, ("whole", 2, 64), ("chain", 2, 64)),
+    (ALL, 3, 1100, 999, ("whole", 1, 16), ("chain", 1, 64)),
+    (SINGLE, 7, 1100, 1000, ("whole", 1, 32), ("chain", 1, 64)),
+    (SINGLE, 12, 1100, 1000, ("whole", 1, 64), ("chain", 1, 64)),
+]
+
+
+@pytest.mark.parametrize(
+    ("dtype", "batch", "tokens", "c", "forward", "backward"),
+    [(dtype, *rest) for types, *rest in MIXED for dtype in types],
+)
+def test_whole_forward_with_chunks_behind(dtype, batch, tokens, c, forward, backward):
+    planned(dtype, batch, tokens, c, forward, backward)
+    check(dtype, batch, tokens, c)
+
+
+@pytest.mark.parametrize(("dtype", "c"), [(torch.bfloat16, 130), (torch.float32, 65)])
+def test_graph_replays_of_chunks(dtype, c):
+    """The words that chunks hand on are cleared in every replay."""
+    per_lane = 2 if c == 130 else 1
+    planned(dtype, 2, 9000, c, ("chain", per_lane, 64), ("chain", per_lane, 64))
+
+    def make(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        randn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+        return [randn(2, 9000, c).to(dtype), (randn(2, 9000, c) + 3).to(dtype), randn(2, c), randn(2, 9000, c).to(dtype), randn(2, c)]
+
+    inputs = make(0)
+    leaves = [v.requires_grad_() for v in inputs[:3]]
+
+    def step():
+        h, last = gated_recurrence(*leaves)
+        return (h, last, *torch.autograd.grad((h, last), leaves, tuple(inputs[3:])))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (1, 2, 3):
+        with torch.no_grad():
+            for held, fresh in zip(inputs, make(seed)):
+                held.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(captured, step()):
+            assert torch.equal(got, want)
+
+
+def planned(dtype, batch, tokens, c, forward, backward):
+    """The forward's and the backward's plan, which have to be the expected ones."""
     load_native()
+    plans = []
     for expected, back in ((forward, False), (backward, True)):
         plan = _capi.recurrence_plan(_build.hip_library(), batch, tokens, c, dtype, back)
         assert (plan["kernel"], plan["channels_per_lane"], plan["lanes"]) == expected, plan
-        # More than one tile, or group of 32 chunks, in the kernels that have them.
-        assert tokens > plan["tile"] * {"whole": 1, "chain": 32}.get(plan["kernel"], 0) or tokens <= 8, plan
+        plans.append(plan)
+    return plans
+
+
+def check(dtype, batch, tokens, c):
     g = torch.Generator().manual_seed(tokens)
     both = torch.randn(batch, tokens, 2 * c + 1, generator=g)
     both[..., c + 1 :] += torch.linspace(-1, 8, c)
