@@ -381,6 +381,67 @@ int convnd_hip_recurrence_plan_describe(convnd_hip_dtype dtype,
                                         const convnd_hip_recurrence_problem* problem, int backward,
                                         char* buffer, size_t length);
 
+/* Gated delta rule: a state S [key_size, value_size] a head,
+ *   S_t = a_t S_(t-1) + k_t u_t^T,  u_t = beta_t (v_t - a_t S_(t-1)^T k_t),  a_t = exp(decay_t),
+ *   o_t = scale S_t^T q_t,  S_0 = first,
+ * with q and k divided by sqrt(|.|^2 + 1e-6) where `normalize` says so. query and key are [batch, tokens,
+ * key_heads, key_size], value [batch, tokens, heads, value_size], each by its strides with a contiguous
+ * last axis; heads is a multiple of key_heads, and value heads h key_group .. h key_group + key_group - 1
+ * share key head h. decay and beta [batch, tokens, heads] are of `gate_dtype`, the element type or float32.
+ * A decay below -104, -inf among them, closes the gate (a = 0, as its exp in float32). */
+typedef struct convnd_hip_delta_problem {
+  int64_t batch, tokens, key_heads, heads;
+  int64_t key_size, value_size; /* 1 to 128; 1 to 65535 */
+  int64_t query_batch, query_token, query_head; /* strides; of tokens below 2^21 */
+  int64_t key_batch, key_token, key_head;
+  int64_t value_batch, value_token, value_head;
+  int64_t decay_batch, decay_token, decay_head;
+  int64_t beta_batch, beta_token, beta_head;
+  int64_t grad_batch, grad_token, grad_head; /* of grad_output (backward) */
+  double scale;
+  int normalize;
+  int gate_dtype;   /* convnd_hip_dtype of decay and beta */
+  int wide_lengths; /* lengths are int64 (nonzero) or int32 */
+} convnd_hip_delta_problem;
+
+/* Elements (of the element type) that the forward saves for the backward: for each chunk of 64 tokens (32
+ * of float32) the state before it and what its tokens add. */
+int64_t convnd_hip_delta_saved(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem);
+
+/* Device scratch bytes of convnd_hip_delta; of the pointers only the alignment is looked at (rows that
+ * do not start on 4 bytes or are no whole 16 bytes long are copied). saving: whether `saved` is given. */
+size_t convnd_hip_delta_workspace_size(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
+                                       const void* query, const void* key, const void* value, int saving);
+
+/* output [batch, tokens, heads, value_size] contiguous; last [batch, heads, key_size, value_size] float32, the
+ * state after the last token; first of the same shape, null for zeros. lengths [batch], null for
+ * `tokens`: tokens at and past a sequence's length (taken as 0 below 0 and as `tokens` above) change no
+ * state and give zeros, whatever the inputs hold there. saved: for the backward, or null. A few tokens
+ * without `saved` run token by token in float32; else tokens of a chunk are taken together, and a NaN
+ * reaches the outputs of its whole chunk. Beside float16 states, and what tokens add to them, have to be
+ * within its range. */
+int convnd_hip_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem, const void* query,
+                     const void* key, const void* value, const void* decay, const void* beta,
+                     const float* first, const void* lengths, void* output, float* last, void* saved,
+                     void* workspace, size_t workspace_size, void* stream);
+
+size_t convnd_hip_delta_backward_workspace_size(convnd_hip_dtype dtype,
+                                                const convnd_hip_delta_problem* problem,
+                                                const void* grad_output, const void* query,
+                                                const void* key, const void* value);
+
+/* Its gradients for the cotangents grad_output [batch, tokens, heads, value_size] by its strides and
+ * grad_last [batch, heads, key_size, value_size] float32 (null for zeros), all contiguous: grad_query and
+ * grad_key [batch, tokens, key_heads, key_size] (sums over the value heads that share them), grad_value,
+ * grad_decay and grad_beta [batch, tokens, heads] of `gate_dtype`, and grad_first float32 or null. Zeros past a
+ * sequence's length, and for a closed gate's decay. */
+int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
+                              const void* grad_output, const float* grad_last, const void* query,
+                              const void* key, const void* value, const void* decay, const void* beta,
+                              const void* lengths, const void* saved, void* grad_query, void* grad_key,
+                              void* grad_value, void* grad_decay, void* grad_beta, float* grad_first,
+                              void* workspace, size_t workspace_size, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

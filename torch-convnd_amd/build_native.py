@@ -39,6 +39,7 @@ HIP_SOURCES = (
     "convnd_norm.hip",
     "convnd_linear.hip",
     "convnd_recurrence.hip",
+    "convnd_delta.hip",
     "convnd_sequence_capi.cpp",
     "convnd_capi.cpp",
 )
@@ -129,6 +130,7 @@ def build_ops_library(verbose: bool = False) -> Path:
         f"-I{INCLUDE}",
         str(CSRC / "torch_ops.cpp"),
         str(CSRC / "torch_sequence_ops.cpp"),
+        str(CSRC / "torch_delta_ops.cpp"),
         str(CSRC / "convnd_cpu.cpp"),
         "-fopenmp",
         "-o",

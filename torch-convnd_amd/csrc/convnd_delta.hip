@@ -1,0 +1,1597 @@
+// Gated delta rule: a matrix state S [key_size, value_size] a head, corrected towards each token's value,
+//
+//   S_t = a_t S_(t-1) + k_t u_t^T,  u_t = beta_t (v_t - a_t S_(t-1)^T k_t),  a_t = exp(decay_t)
+//   o_t = S_t^T q_t
+//
+// with q scaled (and q, k of unit length where asked for). Over a chunk of C tokens with the state S
+// before it, the products G_ij = a_(j+1) .. a_i and their ends c_i = a_1 .. a_i, e_j = G_Cj,
+//
+//   A_ij = beta_i G_ij k_i.k_j (i > j),  T = (I + A)^-1,  U = T diag(beta) (V - diag(c) K S)
+//   O = diag(c) Q S + P U,  P_ij = G_ij q_i.k_j (i >= j),  S' = c_C S + K^T diag(e) U
+//
+// T and P do not need the state: delta_prepare makes them for all chunks side by side, then
+// delta_forward walks each head's chunks with S in registers. Of a step's few tokens delta_step
+// computes the definition itself.
+//
+// Products run on the matrix cores: in 16 bits on chunks of 64 tokens, in float of 32 (128 bytes a row
+// of T either way, the row of every panel in LDS). Decays' sums are kept in 64 bits and differences of
+// them taken before exp, so that long chunks of strong decays lose nothing; a decay whose exp is zero
+// in float (-inf, a packed document's start) is left out of the sums and its pairs masked. Unit lengths
+// are factors of rows (rk, rq), never rounded into the operands.
+//
+// What is not an input is split into two 16-bit terms before a product (S, U, T, P and what they are
+// made of), which doubles matrix instructions but not LDS reads of the shared operand, by which the
+// walk is bound: the state stays within 1e-5 of the 64-bit one over thousands of tokens (one term:
+// 3e-3) and outputs within their own rounding (1.65e-3 in bfloat16; one term 3.6e-3).
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "convnd_internal.h"
+#include "convnd_sequence.h"
+
+namespace convnd {
+namespace {
+
+constexpr float kNormEps = 1e-6f;
+
+template <typename T>
+struct Chunk {
+  using frag = typename Fragment<T>::type;
+  static constexpr int kTokens = delta_chunk(sizeof(T));
+  static constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int kTiles = kTokens / 16;    // of 16 rows
+  static constexpr int kStep = 64 / sizeof(T);   // contraction values of a fragment
+  static constexpr int kPer = kStep / 16;        // tiles a fragment is made of
+  static constexpr int kPanel = kTokens * 128;   // bytes of kTokens rows of 128
+};
+
+template <typename T>
+using Four = T __attribute__((ext_vector_type(4)));
+
+// Panels: rows of 128 bytes whose 16-byte pieces are permuted by the row, so that reads of 16 rows at a
+// piece, in order or as 8 (i / 4) + i % 4, and transposing reads meet no bank twice.
+__device__ __forceinline__ int swizzle(int row) {
+  return ((row >> 1) & 1) << 2 | ((row >> 3) & 1) << 1 | (((row >> 4) ^ (row >> 2)) & 1);
+}
+
+// Lane's place among 16 columns (or rows) and its group of contraction values.
+struct Lane {
+  int l, g;
+  __device__ __forceinline__ Lane() : l(threadIdx.x & 15), g((threadIdx.x >> 4) & 3) {}
+};
+
+// The row that lane l of tile m reads as operand, so that results' registers are contraction values in
+// order: register e of lane group g in tile m holds row first_row(m, g) + e, and the kPer tiles of a
+// fragment together its 16 bytes.
+template <typename T>
+__device__ __forceinline__ int operand_row(int m, int l) {
+  if constexpr (sizeof(T) == 2) return m / 2 * 32 + (l >> 2) * 8 + m % 2 * 4 + (l & 3);
+  return m * 16 + l;
+}
+template <typename T>
+__device__ __forceinline__ int first_row(int m, int g) {
+  if constexpr (sizeof(T) == 2) return m / 2 * 32 + g * 8 + m % 2 * 4;
+  return m * 16 + g * 4;
+}
+
+// Fragment of step ks (two a panel) of the lane's row.
+template <typename T>
+__device__ __forceinline__ typename Chunk<T>::frag read_row(const unsigned char* panels, int row, int ks,
+                                                            const Lane& lane) {
+  return *reinterpret_cast<const typename Chunk<T>::frag*>(
+      panels + ks / 2 * Chunk<T>::kPanel + row * 128 + (((ks % 2 * 4 + lane.g) ^ swizzle(row)) << 4));
+}
+
+// Four values down a column: rows `row` to row + 3 of a panel (row a whole four) at column `column` of
+// each lane. The 16 lanes of a group read 4 rows of 4 pieces of 8 bytes; lane l gets value l % 4 of
+// piece l / 4. `piece` is the byte offset, within the rows, of the 8 bytes that this lane fetches.
+template <typename T>
+__device__ __forceinline__ s16x4 read_down(const unsigned char* panel, int row, int piece, const Lane& lane) {
+  using lds_vec = __attribute__((address_space(3))) s16x4*;
+  const int r = row + (lane.l >> 2);
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_vec)(panel + r * 128 + (((piece >> 4) ^ swizzle(r)) << 4) + (piece & 8)));
+}
+
+// Fragment of the transposed panels: contraction values are rows kt * kStep .., the lane's row of the
+// operand is column operand_row(m) (ORDERED: m * 16 + l) of the panels.
+template <typename T, bool ORDERED = false>
+__device__ __forceinline__ typename Chunk<T>::frag read_column(const unsigned char* panels, int m, int kt,
+                                                               const Lane& lane) {
+  if constexpr (sizeof(T) == 2) {
+    const unsigned char* panel = panels + m / 4 * Chunk<T>::kPanel;
+    const int piece = ORDERED ? m % 4 * 32 + (lane.l & 3) * 8
+                              : m / 2 % 2 * 64 + (lane.l & 3) * 16 + m % 2 * 8;
+    union {
+      s16x4 part[2];
+      typename Chunk<T>::frag whole;
+    } u;
+    u.part[0] = read_down<T>(panel, kt * 32 + lane.g * 8, piece, lane);
+    u.part[1] = read_down<T>(panel, kt * 32 + lane.g * 8 + 4, piece, lane);
+    return u.whole;
+  } else {
+    const unsigned char* panel = panels + m / 2 * Chunk<T>::kPanel;
+    f32x4 f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = kt * 16 + lane.g * 4 + i;
+      f[i] = *reinterpret_cast<const float*>(panel + r * 128 +
+                                             (((m % 2 * 4 + (lane.l >> 2)) ^ swizzle(r)) << 4) +
+                                             (lane.l & 3) * 4);
+    }
+    return f;
+  }
+}
+
+// Column 16 tile + l of the panels at the rows of result tile m.
+template <typename T>
+__device__ __forceinline__ f32x4 read_values(const unsigned char* panels, int tile, int m, const Lane& lane) {
+  f32x4 v;
+  if constexpr (sizeof(T) == 2) {
+    const Four<T> s = __builtin_bit_cast(
+        Four<T>, read_down<T>(panels + tile / 4 * Chunk<T>::kPanel, first_row<T>(m, lane.g),
+                           tile % 4 * 32 + (lane.l & 3) * 8, lane));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(s[e]);
+  } else {
+    v = read_column<T>(panels, tile, m, lane);
+  }
+  return v;
+}
+
+// The second terms of float16 values are kept 2^11 times as large, in sums of their own: as they are, those of
+// values below 0.1 would end in the type's fixed-point range (states 1.4e-5 off where bfloat16's are 4e-6).
+template <typename T>
+constexpr float kRestScale = std::is_same_v<T, _Float16> ? 2048.f : 1.f;
+
+// A sum of products, and that of their second terms.
+template <typename T>
+struct Sum {
+  f32x4 whole;
+  f32x4 rest = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ explicit Sum(f32x4 from = {0.f, 0.f, 0.f, 0.f}) : whole(from) {}
+  __device__ __forceinline__ void add(typename Chunk<T>::frag a, typename Chunk<T>::frag b, bool second) {
+    if (second && kRestScale<T> != 1.f)
+      rest = Fragment<T>::mma(a, b, rest);
+    else
+      whole = Fragment<T>::mma(a, b, whole);
+  }
+  __device__ __forceinline__ f32x4 value() const {
+    return kRestScale<T> != 1.f ? whole + rest * (1.f / kRestScale<T>) : whole;
+  }
+};
+
+// Four values rounded. They are rounded once for every use: the compiler would otherwise take float16 values
+// for the product from one instruction and for the difference from another (a fused multiply-add that rounds
+// once where the first rounds twice), and a last place between the two would be lost.
+template <typename T>
+__device__ __forceinline__ Four<T> nearest(const f32x4& v) {
+  Four<T> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = static_cast<T>(v[i]);
+  if constexpr (sizeof(T) == 2) {
+    typedef unsigned Words __attribute__((ext_vector_type(2)));
+    Words w = __builtin_bit_cast(Words, r);
+    asm("" : "+v"(w));
+    r = __builtin_bit_cast(Four<T>, w);
+  }
+  return r;
+}
+// What rounding left, as the second terms have it.
+template <typename T>
+__device__ __forceinline__ f32x4 rest_of(const f32x4& v, const Four<T>& rounded) {
+  f32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (v[i] - static_cast<float>(rounded[i])) * kRestScale<T>;
+  return r;
+}
+
+// kPer result tiles as a fragment: the nearest values, and (16 bits) what they leave.
+template <typename T, int TERMS>
+__device__ __forceinline__ void split(const f32x4* tiles, typename Chunk<T>::frag (&out)[TERMS]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Four<T> hi = nearest<T>(tiles[i]);
+      Four<T> lo;
+      if constexpr (TERMS > 1) lo = nearest<T>(rest_of<T>(tiles[i], hi));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        out[0][i * 4 + e] = hi[e];
+        if constexpr (TERMS > 1) out[1][i * 4 + e] = lo[e];
+      }
+    }
+  } else {
+    out[0] = tiles[0];
+  }
+}
+
+__device__ __forceinline__ u32x4 buffer_at(const void* p) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  u32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(at));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(at >> 32) & 0xffffu);
+  r[2] = kNowhere;
+  r[3] = 0x00020000u;
+  return r;
+}
+
+// Loads panels of kTokens rows into LDS: `count` panels of 128 bytes from `column` on of rows `stride`
+// bytes apart; zeros past `rows` rows and `bytes` bytes of a row. Waves take turns from wave `turn` on.
+template <typename T>
+__device__ __forceinline__ void load_panels(u32x4 buffer, unsigned dst, int count, unsigned column,
+                                            unsigned stride, int rows, unsigned bytes, int wave, int waves) {
+  constexpr int kLoads = Chunk<T>::kTokens / 8;
+  const int lane = threadIdx.x & 63;
+  for (int i = wave; i < count * kLoads; i += waves) {
+    const int panel = i / kLoads, row = i % kLoads * 8 + lane / 8;
+    const unsigned at = column + panel * 128 + (((lane % 8) ^ swizzle(row)) << 4);
+    load_lds16(buffer, dst + i * 1024,
+               row < rows && at < bytes ? static_cast<unsigned>(row) * stride + at : kNowhere);
+  }
+}
+// Panels that lie in memory one after another as they are.
+template <typename T>
+__device__ __forceinline__ void load_whole(u32x4 buffer, unsigned dst, int count, int wave, int waves) {
+  constexpr int kLoads = Chunk<T>::kTokens / 8;
+  const int lane = threadIdx.x & 63;
+  for (int i = wave; i < count * kLoads; i += waves) {
+    const int row = i % kLoads * 8 + lane / 8;
+    load_lds16(buffer, dst + i * 1024,
+               static_cast<unsigned>(i * 1024 + lane / 8 * 128 + (((lane % 8) ^ swizzle(row)) << 4)));
+  }
+}
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
+}
+
+// A wave's own exchange through LDS: what its lanes wrote is there for the others.
+__device__ __forceinline__ void wait_own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+constexpr int kTurnPitch = 20;  // elements of a row of 16 columns
+
+// Tokens of sequence b that count.
+__device__ __forceinline__ int length_of(const DeltaArgs& a, int b) {
+  if (a.lengths == nullptr) return static_cast<int>(a.tokens);
+  const int64_t n = a.wide_lengths ? static_cast<const int64_t*>(a.lengths)[b]
+                                   : static_cast<const int32_t*>(a.lengths)[b];
+  return static_cast<int>(n < 0 ? 0 : n > a.tokens ? a.tokens : n);
+}
+
+// Up to four neighbouring values.
+template <typename T>
+__device__ __forceinline__ void store_four(T* p, const f32x4& v, int count) {
+  Run<T, 4> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r.v[e] = static_cast<T>(v[e]);
+  if (count >= 4) {
+    store_run<4>(p, r);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < count) p[e] = r.v[e];
+    end_of_part();
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ const T* at_token(const void* p, const DeltaStrides& s, int64_t batch, int64_t token,
+                                             int64_t head) {
+  return static_cast<const T*>(p) + batch * s.batch + token * s.token + head * s.head;
+}
+
+// A chunk's record beside its panels: factors of rows in float (one value a token each), the sums of
+// decays in 64 bits, and a bit for each closed token.
+template <typename T>
+struct Record {
+  static constexpr int kTokens = Chunk<T>::kTokens;
+  float state_to_value[kTokens];  // beta c rk: what a row of K S takes from its value
+  float beta[kTokens];
+  float value_to_state[kTokens];  // e rk
+  float state_to_output[kTokens];  // c rq
+  float rk[kTokens];
+  float rq[kTokens];
+  float norm[kTokens];            // rq without the scale
+  double sum[kTokens];
+  uint64_t closed;
+  float whole;  // c of the last token
+  float unused;
+};
+
+// ---- T, P and the factors of every chunk ----------------------------------------------------------
+
+// exp of the decays between tokens j and i > j, none of them closed.
+__device__ __forceinline__ bool open_between(uint64_t closed, int j, int i) {
+  // Bits j + 1 .. i.
+  return ((closed >> 1 >> j) & ((uint64_t{1} << (i - j)) - 1)) == 0;
+}
+__device__ __forceinline__ float decay_between(double later, double earlier) {
+  return __builtin_amdgcn_exp2f(static_cast<float>(later - earlier) * 1.44269504088896341f);
+}
+
+// A workgroup takes a chunk of a key head and its value heads one after another; wave w makes rows 16 w
+// to 16 w + 15. k.k and q.k are in registers for all heads. T: each wave inverts its 16 x 16 block of I
+// + A by substitution, then makes its row of blocks from the right, T_ij = -(sum_k T_ik A_kj) T_jj, on
+// the float matrix instructions, transposed so that a result is the next product's operand and a lane's
+// four values neighbours in a row.
+template <typename T, int DK>
+__global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs a) {
+  using C = Chunk<T>;
+  using frag = typename C::frag;
+  constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kPanels = DK / kTokens;
+  constexpr int kSteps = DK / C::kStep;
+  constexpr int kPitch = kTokens + 4, kBlockPitch = 20;
+  __shared__ __align__(1024) union {
+    unsigned char operands[2][kPanels * C::kPanel];
+    struct {
+      float rest[kTokens][kPitch];                // A transposed
+      float block[kTiles][16][kBlockPitch];       // the diagonal blocks' inverses, transposed
+    } solve;
+  } lds;
+  __shared__ float rk[kTokens], rq[kTokens], norm[kTokens], beta[kTokens];
+  __shared__ double sum[kTokens];
+  const Lane lane;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = static_cast<int>(blockIdx.x % a.chunks);
+  const int64_t row = blockIdx.x / a.chunks;
+  const int kh = static_cast<int>(row % a.key_heads), b = static_cast<int>(row / a.key_heads);
+  const int length = length_of(a, b), t0 = chunk * kTokens;
+  if (t0 >= length) return;
+  const int rows = length - t0 < kTokens ? length - t0 : kTokens;
+  {
+    const unsigned bytes = static_cast<unsigned>(a.key_size * sizeof(T));
+    const u32x4 k = buffer_at(at_token<T>(a.key, a.key_strides, b, t0, kh));
+    const u32x4 q = buffer_at(at_token<T>(a.query, a.query_strides, b, t0, kh));
+    load_panels<T>(k, lds_address(lds.operands[0]), kPanels, 0,
+                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kTiles);
+    load_panels<T>(q, lds_address(lds.operands[1]), kPanels, 0,
+                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kTiles);
+    wait_loads();
+    __syncthreads();
+  }
+  {
+    // Four threads a row.
+    float ss[2] = {1.f, 1.f};
+    const int r = threadIdx.x / 4;
+    if (a.normalize) {
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        float s = 0.f;
+        for (int c = threadIdx.x % 4; c < kPanels * 8; c += 4) {
+          const frag f = *reinterpret_cast<const frag*>(lds.operands[o] + c / 8 * C::kPanel + r * 128 + c % 8 * 16);
+#pragma unroll
+          for (int i = 0; i < 16 / int(sizeof(T)); ++i) {
+            const float v = static_cast<float>(f[i]);
+            s = fmaf(v, v, s);
+          }
+        }
+        s += dpp_read<0xb1>(s);
+        s += dpp_read<0x4e>(s);
+        ss[o] = 1.f / sqrtf(s + kNormEps);
+      }
+    }
+    if (threadIdx.x % 4 == 0) {
+      rk[r] = ss[0];
+      rq[r] = ss[1] * a.scale;
+      norm[r] = ss[1];
+    }
+  }
+  f32x4 kk[kTiles], qk[kTiles];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) kk[j] = qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < kSteps; ++ks) {
+    const frag own_k = read_row<T>(lds.operands[0], wave * 16 + lane.l, ks, lane);
+    const frag own_q = read_row<T>(lds.operands[1], wave * 16 + lane.l, ks, lane);
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      if (j > wave) continue;
+      const frag k = read_row<T>(lds.operands[0], j * 16 + lane.l, ks, lane);
+      kk[j] = Fragment<T>::mma(own_k, k, kk[j]);  // registers rows of this wave, lanes columns
+      qk[j] = Fragment<T>::mma(k, own_q, qk[j]);  // registers columns, lanes rows of this wave
+    }
+  }
+  const int groups = static_cast<int>(a.heads / a.key_heads);
+  for (int group = 0; group < groups; ++group) {
+    const int h = kh * groups + group;
+    const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
+    // Every wave adds the decays up; the first one keeps them for the rows' use.
+    const int token = threadIdx.x & 63;
+    float decay = 0.f, factor = 0.f;
+    if (token < rows) {
+      const int64_t d = b * a.decay_strides.batch + (t0 + token) * a.decay_strides.token + h * a.decay_strides.head;
+      const int64_t f = b * a.beta_strides.batch + (t0 + token) * a.beta_strides.token + h * a.beta_strides.head;
+      if (a.float_gates) {
+        decay = static_cast<const float*>(a.decay)[d];
+        factor = static_cast<const float*>(a.beta)[f];
+      } else {
+        decay = static_cast<float>(static_cast<const T*>(a.decay)[d]);
+        factor = static_cast<float>(static_cast<const T*>(a.beta)[f]);
+      }
+    }
+    const bool shut = decay < kDeltaClosed;
+    const uint64_t closed = __ballot(shut);
+    double total = shut ? 0. : static_cast<double>(decay);
+#pragma unroll
+    for (int step = 1; step < kTokens; step *= 2) {
+      const double before = __shfl_up(total, step);
+      if (token >= step) total += before;
+    }
+    const double last = __shfl(total, kTokens - 1);
+    __syncthreads();  // rk and rq are there; the head before has read what follows
+    if (wave == 0 && token < kTokens) {
+      sum[token] = total;
+      beta[token] = factor;
+      Record<T>* r = reinterpret_cast<Record<T>*>(a.records) + at;
+      const float c = (closed & (~uint64_t{0} >> (63 - token))) == 0 ? decay_between(total, 0.) : 0.f;
+      const float e = open_between(closed, token, kTokens - 1) ? decay_between(last, total) : 0.f;
+      r->state_to_value[token] = factor * c * rk[token];
+      r->beta[token] = factor;
+      r->value_to_state[token] = e * rk[token];
+      r->state_to_output[token] = c * rq[token];
+      r->rk[token] = rk[token];
+      r->rq[token] = rq[token];
+      r->norm[token] = norm[token];
+      r->sum[token] = total;
+      if (token == kTokens - 1) {
+        r->closed = closed;
+        r->whole = c;
+      }
+    }
+    __syncthreads();
+    T* panels = reinterpret_cast<T*>(a.panels + at * (2 * C::kTerms * C::kPanel));
+    {
+      // A, transposed: lane's column j, four rows of this wave.
+      double later[4];
+      float up[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = wave * 16 + lane.g * 4 + e;
+        later[e] = sum[i];
+        up[e] = beta[i] * rk[i];
+      }
+#pragma unroll
+      for (int jb = 0; jb < kTiles; ++jb) {
+        if (jb > wave) continue;
+        const int j = jb * 16 + lane.l;
+        const double earlier = sum[j];
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = wave * 16 + lane.g * 4 + e;
+          v[e] = i > j && open_between(closed, j, i) ? up[e] * rk[j] * decay_between(later[e], earlier) * kk[jb][e]
+                                                     : 0.f;
+        }
+        *reinterpret_cast<f32x4*>(&lds.solve.rest[j][wave * 16 + lane.g * 4]) = v;
+      }
+    }
+    {
+      // P: lane's row i, four columns; blocks past the diagonal as far as a fragment reaches.
+      const int i = wave * 16 + lane.l;
+      const double later = sum[i];
+      T* p = panels + C::kTerms * kTokens * kTokens + i * kTokens + lane.g * 4;
+#pragma unroll
+      for (int jb = 0; jb < kTiles; ++jb) {
+        if (jb / C::kPer > wave / C::kPer) continue;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = jb * 16 + lane.g * 4 + e;
+          v[e] = i >= j && open_between(closed, j, i) ? rq[i] * rk[j] * decay_between(later, sum[j]) * qk[jb][e]
+                                                      : 0.f;
+        }
+#pragma unroll
+        for (int term = 0; term < C::kTerms; ++term) {
+          const Four<T> hi = nearest<T>(v);
+          *reinterpret_cast<Four<T>*>(p + term * kTokens * kTokens + jb * 16) = hi;
+          v = rest_of<T>(v, hi);
+        }
+      }
+    }
+    __syncthreads();
+    {
+      // Column l of the inverse of this wave's diagonal block, x = e_l - (A - its diagonal) x.
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = i == lane.l ? 1.f : 0.f;
+#pragma unroll
+      for (int k = 0; k < 15; ++k) {
+        const float* column = &lds.solve.rest[wave * 16 + k][wave * 16];
+#pragma unroll
+        for (int i = k + 1; i < 16; ++i) x[i] = fmaf(-column[i], x[k], x[i]);
+      }
+      if (lane.g == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<f32x4*>(&lds.solve.block[wave][lane.l][i]) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+      }
+    }
+    __syncthreads();
+    {
+      f32x4 t[kTiles];  // T_ij transposed: registers columns, lanes rows
+#pragma unroll
+      for (int j = kTiles - 1; j >= 0; --j) {
+        if (j > wave) {
+          t[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else if (j == wave) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[j][e] = lds.solve.block[wave][lane.g * 4 + e][lane.l];
+        } else {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = j + 1; k < kTiles; ++k) {
+            if (k > wave) continue;
+            const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.solve.rest[j * 16 + lane.l][k * 16 + lane.g * 4]);
+            acc = Fragment<float>::mma(f, t[k], acc);
+          }
+          const f32x4 d = *reinterpret_cast<const f32x4*>(&lds.solve.block[j][lane.l][lane.g * 4]);
+          t[j] = Fragment<float>::mma(-d, acc, f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+      }
+      T* p = panels + (wave * 16 + lane.l) * kTokens + lane.g * 4;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        if (j / C::kPer > wave / C::kPer) continue;
+#pragma unroll
+        for (int term = 0; term < C::kTerms; ++term) {
+          const Four<T> hi = nearest<T>(t[j]);
+          *reinterpret_cast<Four<T>*>(p + term * kTokens * kTokens + j * 16) = hi;
+          t[j] = rest_of<T>(t[j], hi);
+        }
+      }
+    }
+  }
+}
+
+// ---- the walk over the chunks ------------------------------------------------------------------------
+
+// LDS of a chunk: K, Q, T, P (each in its terms), V or dO, the factors.
+template <typename T, int DK, int W>
+struct Stage {
+  using C = Chunk<T>;
+  static constexpr int kKeys = DK / C::kTokens * C::kPanel;
+  static constexpr int kQuery = kKeys;
+  static constexpr int kSolve = 2 * kKeys;
+  static constexpr int kPairs = kSolve + C::kTerms * C::kPanel;
+  static constexpr int kValues = kPairs + C::kTerms * C::kPanel;
+  static constexpr int kValuePanels = W * 16 / C::kTokens;
+  static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
+  static constexpr int kBytes = kFactors + 1024;
+  static_assert(W * 16 % C::kTokens == 0, "whole panels of values");
+};
+
+// A wave keeps 16 columns of S in registers, as results [key, column] of the products that update it, and
+// walks through all of them by itself: K S, T R, P U and K^T U take its columns' values as one
+// operand straight from the results before (operand_row puts them in order) and the shared panels as the
+// other, from LDS, so waves meet only where panels change hands, once a chunk. The next chunk's panels
+// load meanwhile.
+template <typename T, int DK, int W, bool KEEP>
+__global__ __launch_bounds__(64 * W) void delta_forward(DeltaArgs a) {
+  using C = Chunk<T>;
+  using frag = typename C::frag;
+  using S = Stage<T, DK, W>;
+  constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kTerms = C::kTerms, kPer = C::kPer;
+  constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  const Lane lane;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups of a head's columns are a whole number of heads apart: where that is a multiple of eight
+  // they run on one XCD and share its L2.
+  const int64_t heads = a.batch * a.heads;
+  const int64_t bh = blockIdx.x % heads;
+  const int b = static_cast<int>(bh / a.heads), h = static_cast<int>(bh % a.heads);
+  const int kh = h / static_cast<int>(a.heads / a.key_heads);
+  const int v0 = static_cast<int>(blockIdx.x / heads) * W * 16;
+  const int column = v0 + wave * 16;  // of the wave
+  const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
+  const bool active = column < value_size;
+  const int mine = column + lane.l;
+  const int length = length_of(a, b);
+  const int chunks = (length + kTokens - 1) / kTokens;
+  const int64_t first_chunk = bh * a.chunks;
+
+  f32x4 state[kStateTiles];
+#pragma unroll
+  for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = first_row<T>(m, lane.g) + e;
+      state[m][e] = a.first != nullptr && d < key_size && mine < value_size
+                        ? a.first[(bh * key_size + d) * value_size + mine]
+                        : 0.f;
+    }
+
+  const unsigned lds_at = lds_address(lds);
+  const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
+  const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
+  const T* v_at = at_token<T>(a.value, a.value_strides, b, 0, h);
+  auto load = [&](int c) __attribute__((always_inline)) {
+    const unsigned dst = lds_at + (c & 1) * S::kBytes;
+    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
+    const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
+    const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
+    load_panels<T>(buffer_at(k_at + t0 * a.key_strides.token), dst, DK / kTokens, 0,
+                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, key_bytes, wave, W);
+    load_whole<T>(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, 2 * kTerms,
+                  wave, W);
+    load_panels<T>(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, S::kValuePanels,
+                   static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
+                   rows, static_cast<unsigned>(value_size * sizeof(T)), wave, W);
+    load_panels<T>(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, DK / kTokens, 0,
+                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, key_bytes, wave, W);
+    if (wave == W - 1) {
+      const unsigned at = (threadIdx.x & 63) * 16;
+      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c), dst + S::kFactors,
+                 at < 16 * kTokens ? at : kNowhere);
+    }
+  };
+
+  T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
+  const int64_t out_token = a.heads * value_size;
+  const int store_at = column + lane.g * 4, store_count = value_size - store_at;
+  if (chunks > 0) load(0);
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    wait_loads();
+    __syncthreads();
+    if (c + 1 < chunks) load(c + 1);
+    if (!active) continue;
+    const unsigned char* at = lds + (c & 1) * S::kBytes;
+    const float* factors = reinterpret_cast<const float*>(at + S::kFactors);
+    const float whole = reinterpret_cast<const Record<T>*>(a.records)[first_chunk + c].whole;
+    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
+
+    frag s[kSteps][kTerms];
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
+    if constexpr (KEEP) {
+      T* keep = static_cast<T*>(a.states) + ((first_chunk + c) * a.value_pad + mine) * DK + lane.g * (16 / sizeof(T));
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + ks * C::kStep) = s[ks][0];
+    }
+
+    // R = beta V - (beta c rk) K S.
+    f32x4 r[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      Sum<T> sum;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const frag k = read_row<T>(at, operand_row<T>(m, lane.l), ks, lane);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) sum.add(k, s[ks][term], term > 0);
+      }
+      const f32x4 acc = sum.value();
+      const f32x4 v = read_values<T>(at + S::kValues, wave, m, lane);
+      const int row = first_row<T>(m, lane.g);
+      const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[e], -take[e] * acc[e]);
+    }
+    frag rf[2][kTerms], uf[2][kTerms], df[2][kTerms];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&r[kt * kPer], rf[kt]);
+    // U = T R.
+    f32x4 u[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      Sum<T> sum;
+#pragma unroll
+      for (int kt = 0; kt <= m / kPer; ++kt) {
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          const frag t = read_row<T>(at + S::kSolve + term * C::kPanel, operand_row<T>(m, lane.l), kt, lane);
+#pragma unroll
+          for (int other = 0; other < kTerms - term; ++other) sum.add(t, rf[kt][other], term + other > 0);
+        }
+      }
+      u[m] = sum.value();
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
+    if constexpr (KEEP) {
+      T* keep = static_cast<T*>(a.updates) + ((first_chunk + c) * a.value_pad + mine) * kTokens +
+                lane.g * (16 / sizeof(T));
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + kt * C::kStep) = uf[kt][0];
+    }
+    // O, its lanes tokens and its registers columns.
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      Sum<T> sum;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const frag q = read_row<T>(at + S::kQuery, n * 16 + lane.l, ks, lane);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) sum.add(s[ks][term], q, term > 0);
+      }
+      const float factor = factors[3 * kTokens + n * 16 + lane.l];
+      sum.whole *= factor;
+      sum.rest *= factor;
+#pragma unroll
+      for (int kt = 0; kt <= n / kPer; ++kt) {
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          const frag p = read_row<T>(at + S::kPairs + term * C::kPanel, n * 16 + lane.l, kt, lane);
+#pragma unroll
+          for (int other = 0; other < kTerms - term; ++other) sum.add(uf[kt][other], p, term + other > 0);
+        }
+      }
+      const f32x4 o = sum.value();
+      const int64_t t = t0 + n * 16 + lane.l;
+      if (t < a.tokens && store_count > 0) store_four(out + t * out_token + store_at, o, store_count);
+    }
+    // S = c S + K^T (e rk U).
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], df[kt]);
+#pragma unroll
+    for (int m = 0; m < kStateTiles; ++m) {
+      Sum<T> sum(state[m] * whole);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const frag k = read_column<T>(at, m, kt, lane);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) sum.add(k, df[kt][term], term > 0);
+      }
+      state[m] = sum.value();
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = first_row<T>(m, lane.g) + e;
+      if (d < key_size && mine < value_size) a.last[(bh * key_size + d) * value_size + mine] = state[m][e];
+    }
+  // Tokens past the last chunk give zeros.
+  for (int64_t t = static_cast<int64_t>(chunks) * kTokens + lane.l; t < a.tokens; t += 16)
+    if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
+}
+
+// ---- the walk back ----------------------------------------------------------------------------------------
+
+// With D the gradient of the state after a chunk and Y = T^T dU,
+//
+//   dU = P^T dO + diag(e rk) K D,  dV = diag(beta) Y
+//   D' = c_C D + Q^T diag(c rq) dO - K^T diag(beta c rk) Y
+//
+// in the forward walk's form: a wave has 16 columns of D in registers. D and Y of every chunk are kept for
+// delta_gradients.
+template <typename T, int DK, int W>
+__global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
+  using C = Chunk<T>;
+  using frag = typename C::frag;
+  using S = Stage<T, DK, W>;
+  constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kTerms = C::kTerms, kPer = C::kPer;
+  constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  const Lane lane;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t heads = a.batch * a.heads;
+  const int64_t bh = blockIdx.x % heads;
+  const int b = static_cast<int>(bh / a.heads), h = static_cast<int>(bh % a.heads);
+  const int kh = h / static_cast<int>(a.heads / a.key_heads);
+  const int v0 = static_cast<int>(blockIdx.x / heads) * W * 16;
+  const int column = v0 + wave * 16;
+  const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
+  const bool active = column < value_size;
+  const int mine = column + lane.l;
+  const int length = length_of(a, b);
+  const int chunks = (length + kTokens - 1) / kTokens;
+  const int64_t first_chunk = bh * a.chunks;
+  T* turn = reinterpret_cast<T*>(lds + 2 * S::kBytes) + wave * kTokens * kTurnPitch;
+
+  f32x4 state[kStateTiles];
+#pragma unroll
+  for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = first_row<T>(m, lane.g) + e;
+      state[m][e] = a.grad_last != nullptr && d < key_size && mine < value_size
+                        ? a.grad_last[(bh * key_size + d) * value_size + mine]
+                        : 0.f;
+    }
+
+  const unsigned lds_at = lds_address(lds);
+  const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
+  const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
+  const T* g_at = at_token<T>(a.grad_output, a.grad_strides, b, 0, h);
+  auto load = [&](int c) __attribute__((always_inline)) {
+    const unsigned dst = lds_at + (c & 1) * S::kBytes;
+    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
+    const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
+    const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
+    load_panels<T>(buffer_at(k_at + t0 * a.key_strides.token), dst, DK / kTokens, 0,
+                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, key_bytes, wave, W);
+    load_whole<T>(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, 2 * kTerms,
+                  wave, W);
+    load_panels<T>(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, S::kValuePanels,
+                   static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
+                   rows, static_cast<unsigned>(value_size * sizeof(T)), wave, W);
+    load_panels<T>(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, DK / kTokens, 0,
+                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, key_bytes, wave, W);
+    if (wave == W - 1) {
+      const unsigned at = (threadIdx.x & 63) * 16;
+      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c), dst + S::kFactors,
+                 at < 16 * kTokens ? at : kNowhere);
+    }
+  };
+
+  T* out = static_cast<T*>(a.grad_value) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
+  const int64_t out_token = a.heads * value_size;
+  const int store_at = column + lane.g * 4, store_count = value_size - store_at;
+  if (chunks > 0) load(chunks - 1);
+#pragma unroll 1
+  for (int c = chunks - 1; c >= 0; --c) {
+    wait_loads();
+    __syncthreads();
+    if (c > 0) load(c - 1);
+    if (!active) continue;
+    const unsigned char* at = lds + (c & 1) * S::kBytes;
+    const float* factors = reinterpret_cast<const float*>(at + S::kFactors);
+    const float whole = reinterpret_cast<const Record<T>*>(a.records)[first_chunk + c].whole;
+    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
+
+    frag s[kSteps][kTerms];
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
+    {
+      T* keep = static_cast<T*>(a.grad_states) + ((first_chunk + c) * a.value_pad + mine) * DK +
+                lane.g * (16 / sizeof(T));
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + ks * C::kStep) = s[ks][0];
+    }
+    frag g[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) g[kt] = read_column<T, true>(at + S::kValues, wave, kt, lane);
+
+    f32x4 u[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      Sum<T> sum;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const frag k = read_row<T>(at, operand_row<T>(m, lane.l), ks, lane);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) sum.add(k, s[ks][term], term > 0);
+      }
+      const f32x4 factor = *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
+      sum.whole *= factor;
+      sum.rest *= factor;
+#pragma unroll
+      for (int kt = m / kPer; kt < 2; ++kt)
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+          sum.add(read_column<T>(at + S::kPairs + term * C::kPanel, m, kt, lane), g[kt], term > 0);
+      u[m] = sum.value();
+    }
+    frag uf[2][kTerms];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
+    f32x4 y[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      Sum<T> sum;
+#pragma unroll
+      for (int kt = m / kPer; kt < 2; ++kt)
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          const frag t = read_column<T>(at + S::kSolve + term * C::kPanel, m, kt, lane);
+#pragma unroll
+          for (int other = 0; other < kTerms - term; ++other) sum.add(t, uf[kt][other], term + other > 0);
+        }
+      y[m] = sum.value();
+    }
+    {
+      T* keep = static_cast<T*>(a.grad_updates) + ((first_chunk + c) * a.value_pad + mine) * kTokens +
+                lane.g * (16 / sizeof(T));
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        frag hi[1];
+        split<T>(&y[kt * kPer], hi);
+        *reinterpret_cast<frag*>(keep + kt * C::kStep) = hi[0];
+      }
+    }
+    // dV, through this wave's part of LDS: lanes tokens, four columns each.
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      const int row = first_row<T>(m, lane.g);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) turn[(row + e) * kTurnPitch + lane.l] = static_cast<T>(beta[e] * y[m][e]);
+    }
+    wait_own_lds();
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const int64_t t = t0 + n * 16 + lane.l;
+      const Run<T, 4> v = load_run<4>(turn + (n * 16 + lane.l) * kTurnPitch + lane.g * 4);
+      if (t < a.tokens && store_count > 0) {
+        T* p = out + t * out_token + store_at;
+        if (store_count >= 4) {
+          store_run<4>(p, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 3; ++e)
+            if (e < store_count) p[e] = v.v[e];
+          end_of_part();
+        }
+      }
+    }
+    wait_own_lds();
+    // D.
+    frag gf[2][kTerms], yf[2][kTerms];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x4 v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int row = first_row<T>(kt * kPer + i, lane.g);
+        const f32x4 f = *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + row);
+        const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[i][e] = f[e] * static_cast<float>(g[kt][i * 4 + e]);
+          y[kt * kPer + i][e] *= -take[e];
+        }
+      }
+      split<T>(v, gf[kt]);
+      split<T>(&y[kt * kPer], yf[kt]);
+    }
+#pragma unroll
+    for (int m = 0; m < kStateTiles; ++m) {
+      Sum<T> sum(state[m] * whole);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const frag q = read_column<T>(at + S::kQuery, m, kt, lane);
+        const frag k = read_column<T>(at, m, kt, lane);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          sum.add(q, gf[kt][term], term > 0);
+          sum.add(k, yf[kt][term], term > 0);
+        }
+      }
+      state[m] = sum.value();
+    }
+  }
+  if (!active) return;
+  if (a.grad_first != nullptr) {
+#pragma unroll
+    for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = first_row<T>(m, lane.g) + e;
+        if (d < key_size && mine < value_size) a.grad_first[(bh * key_size + d) * value_size + mine] = state[m][e];
+      }
+  }
+  for (int64_t t = static_cast<int64_t>(chunks) * kTokens + lane.l; t < a.tokens; t += 16)
+    if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
+}
+
+// ---- gradients within every chunk --------------------------------------------------------------------------
+
+// With dP = dO U^T and dA = -Y U^T (i > j), N = G dA,
+//
+//   dq' = diag(c) dO S^T + (G dP rk) K                                   (q' the scaled and normalised q)
+//   dk' = -diag(beta c) Y S^T + diag(e) U D^T + (G dP)^T q' + (beta N) k' + (beta N)^T k'
+//   dbeta_i = Y_i.V_i - c_i k'_i.(Y S^T)_i + sum_j N_ij k'_i.k'_j
+//
+// and a decay's gradient is the sum over the pairs, and the states, that its token lies between: with the
+// gradients of the sums of decays, their total from the token on. A workgroup takes a chunk of a key head and
+// adds up its value heads. Wave w has the tokens 16 w to 16 w + 15 as lanes throughout: as rows i, for which
+// pairs are made with registers j, and again as columns j with registers i, so that either is the operand of
+// the next product from registers.
+template <typename T, int DK, bool GROUPED>
+__global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_gradients(DeltaArgs a) {
+  using C = Chunk<T>;
+  using frag = typename C::frag;
+  constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kPer = C::kPer, kThreads = kTokens * 4;
+  constexpr int kPanels = DK / kTokens, kSteps = DK / C::kStep, kKeyTiles = DK / 16;
+  constexpr int kVec = 16 / sizeof(T);
+  // States and their gradients, then keys and queries.
+  __shared__ __align__(1024) unsigned char wide[2][kPanels * C::kPanel];
+  __shared__ __align__(1024) unsigned char narrow[3][C::kPanel];  // U and Y transposed, dO
+  __shared__ double sum[kTokens];
+  __shared__ float beta[kTokens], rk[kTokens], rq[kTokens], slope[kTokens], kept[kTokens], inner[kTiles];
+  const Lane lane;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = static_cast<int>(blockIdx.x % a.chunks);
+  const int64_t row = blockIdx.x / a.chunks;
+  const int kh = static_cast<int>(row % a.key_heads), b = static_cast<int>(row / a.key_heads);
+  const int length = length_of(a, b), t0 = chunk * kTokens;
+  const int groups = static_cast<int>(a.heads / a.key_heads);
+  const int own = wave * 16 + lane.l;  // this lane's token in the chunk
+  const int64_t token = static_cast<int64_t>(b) * a.tokens + t0 + own;
+  const bool in_range = t0 + own < a.tokens;
+  const int key_size = static_cast<int>(a.key_size), value_size = static_cast<int>(a.value_size);
+  T* dq_out = static_cast<T*>(a.grad_query) + (token * a.key_heads + kh) * key_size;
+  T* dk_out = static_cast<T*>(a.grad_key) + (token * a.key_heads + kh) * key_size;
+  const auto store_gate = [&](void* p, int64_t at, float v) __attribute__((always_inline)) {
+    if (a.float_gates)
+      static_cast<float*>(p)[at] = v;
+    else
+      static_cast<T*>(p)[at] = static_cast<T>(v);
+  };
+  if (t0 >= length) {
+    if (!in_range) return;
+#pragma unroll
+    for (int m = 0; m < kKeyTiles; ++m) {
+      const int d = m * 16 + lane.g * 4;
+      if (d >= key_size) continue;
+      store_four(dq_out + d, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
+      store_four(dk_out + d, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
+    }
+    if (lane.g == 0)
+      for (int group = 0; group < groups; ++group) {
+        store_gate(a.grad_decay, token * a.heads + kh * groups + group, 0.f);
+        store_gate(a.grad_beta, token * a.heads + kh * groups + group, 0.f);
+      }
+    return;
+  }
+  const int rows = length - t0 < kTokens ? length - t0 : kTokens;
+  f32x4 dq_all[GROUPED ? kKeyTiles : 1], dk_all[GROUPED ? kKeyTiles : 1];
+  if constexpr (GROUPED) {
+#pragma unroll
+    for (int m = 0; m < kKeyTiles; ++m) dq_all[m] = dk_all[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // Four neighbouring values of this lane's row of a panel set, from column 16 m + 4 g on.
+  const auto own_values = [&](const unsigned char* panels, int m) __attribute__((always_inline)) {
+    const int at = (m * 16 + lane.g * 4) * sizeof(T);
+    const Run<T, 4> v = *reinterpret_cast<const Run<T, 4>*>(
+        panels + at / 128 * C::kPanel + own * 128 + (((at % 128 >> 4) ^ swizzle(own)) << 4) + at % 16);
+    return f32x4{static_cast<float>(v.v[0]), static_cast<float>(v.v[1]), static_cast<float>(v.v[2]),
+                 static_cast<float>(v.v[3])};
+  };
+  const auto over_groups = [](float v) __attribute__((always_inline)) {
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    return v;
+  };
+  float norm = 1.f;
+
+#pragma unroll 1
+  for (int group = 0; group < groups; ++group) {
+    const int h = kh * groups + group;
+    const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
+    const Record<T>* record = reinterpret_cast<const Record<T>*>(a.records) + at;
+    f32x4 dq[kKeyTiles], dk[kKeyTiles], back[kKeyTiles];  // dO S^T, Y S^T, U D^T
+#pragma unroll
+    for (int m = 0; m < kKeyTiles; ++m) dq[m] = dk[m] = back[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // dP and Y U^T: of rows (registers columns j) and of columns (registers rows i).
+    f32x4 row_p[kTiles], row_a[kTiles], column_p[kTiles], column_a[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) row_p[m] = row_a[m] = column_p[m] = column_a[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float dbeta = 0.f, product = 0.f;
+    const T* value = at_token<T>(a.value, a.value_strides, b, t0 + own, h);
+#pragma unroll 1
+    for (int v0 = 0; v0 < a.value_pad; v0 += kTokens) {
+      __syncthreads();
+      {
+        const int left = static_cast<int>(a.value_pad) - v0, v_rows = left < kTokens ? left : kTokens;
+        const int64_t v_at = at * a.value_pad + v0;
+        const T* panels[] = {static_cast<const T*>(a.states) + v_at * DK,
+                             static_cast<const T*>(a.grad_states) + v_at * DK,
+                             static_cast<const T*>(a.updates) + v_at * kTokens,
+                             static_cast<const T*>(a.grad_updates) + v_at * kTokens};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          load_panels<T>(buffer_at(panels[i]), lds_address(wide[i]), kPanels, 0, DK * sizeof(T), v_rows,
+                         DK * sizeof(T), wave, kTiles);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          load_panels<T>(buffer_at(panels[2 + i]), lds_address(narrow[i]), 1, 0, 128, v_rows, 128, wave, kTiles);
+        load_panels<T>(buffer_at(at_token<T>(a.grad_output, a.grad_strides, b, t0, h)), lds_address(narrow[2]), 1,
+                       static_cast<unsigned>(v0 * sizeof(T)),
+                       static_cast<unsigned>(a.grad_strides.token * sizeof(T)), rows,
+                       static_cast<unsigned>(value_size * sizeof(T)), wave, kTiles);
+      }
+      wait_loads();
+      __syncthreads();
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const frag g = read_row<T>(narrow[2], own, kt, lane);
+        const frag u = read_column<T, true>(narrow[0], wave, kt, lane);
+        const frag y = read_column<T, true>(narrow[1], wave, kt, lane);
+#pragma unroll
+        for (int m = 0; m < kKeyTiles; ++m) {
+          const frag s = read_column<T, true>(wide[0], m, kt, lane);
+          dq[m] = Fragment<T>::mma(s, g, dq[m]);
+          dk[m] = Fragment<T>::mma(s, y, dk[m]);
+          back[m] = Fragment<T>::mma(read_column<T, true>(wide[1], m, kt, lane), u, back[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) {
+          if (m / kPer <= wave / kPer) {
+            const frag other = read_column<T>(narrow[0], m, kt, lane);
+            row_p[m] = Fragment<T>::mma(other, g, row_p[m]);
+            row_a[m] = Fragment<T>::mma(other, y, row_a[m]);
+          }
+          if (m / kPer >= wave / kPer) {
+            column_p[m] = Fragment<T>::mma(read_row<T>(narrow[2], operand_row<T>(m, lane.l), kt, lane), u, column_p[m]);
+            column_a[m] = Fragment<T>::mma(read_column<T>(narrow[1], m, kt, lane), u, column_a[m]);
+          }
+        }
+        const int v = v0 + kt * C::kStep + lane.g * kVec;
+        if (own < rows && v < value_size) {
+          const frag f = __builtin_bit_cast(frag, load_run<kVec>(value + v));
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) dbeta = fmaf(static_cast<float>(f[i]), static_cast<float>(y[i]), dbeta);
+        }
+      }
+      // The state's product with its gradient.
+      for (int i = threadIdx.x; i < kPanels * C::kPanel / 16; i += kThreads) {
+        const frag s = *reinterpret_cast<const frag*>(wide[0] + i * 16);
+        const frag d = *reinterpret_cast<const frag*>(wide[1] + i * 16);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) product = fmaf(static_cast<float>(s[e]), static_cast<float>(d[e]), product);
+      }
+    }
+    __syncthreads();
+    {
+      const unsigned bytes = static_cast<unsigned>(key_size * sizeof(T));
+      load_panels<T>(buffer_at(at_token<T>(a.key, a.key_strides, b, t0, kh)), lds_address(wide[0]), kPanels, 0,
+                     static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kTiles);
+      load_panels<T>(buffer_at(at_token<T>(a.query, a.query_strides, b, t0, kh)), lds_address(wide[1]), kPanels, 0,
+                     static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kTiles);
+      if (threadIdx.x < kTokens) {
+        sum[threadIdx.x] = record->sum[threadIdx.x];
+        beta[threadIdx.x] = record->beta[threadIdx.x];
+        rk[threadIdx.x] = record->rk[threadIdx.x];
+        rq[threadIdx.x] = record->rq[threadIdx.x];
+      }
+      product = lanes_sum<64>(product);
+      if ((threadIdx.x & 63) == 0) inner[wave] = product;
+    }
+    norm = record->norm[own];
+    const uint64_t closed = record->closed;
+    wait_loads();
+    __syncthreads();
+    const unsigned char *keys = wide[0], *queries = wide[1];
+    const double own_sum = sum[own];
+    const float own_beta = beta[own], own_rk = rk[own], own_rq = rq[own];
+    const float c = (closed & (~uint64_t{0} >> (63 - own))) == 0 ? decay_between(own_sum, 0.) : 0.f;
+    const float e_own = open_between(closed, own, kTokens - 1) ? decay_between(sum[kTokens - 1], own_sum) : 0.f;
+
+    float dsum = 0.f;
+    dbeta = over_groups(dbeta);
+    {
+      // What comes through the states.
+      float q_dot = 0.f, k_dot = 0.f, b_dot = 0.f;
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        const f32x4 q = own_values(queries, m), k = own_values(keys, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          q_dot = fmaf(q[e], dq[m][e], q_dot);
+          k_dot = fmaf(k[e], dk[m][e], k_dot);
+          b_dot = fmaf(k[e], back[m][e], b_dot);
+          dq[m][e] *= c;
+          dk[m][e] = fmaf(e_own, back[m][e], -own_beta * c * dk[m][e]);
+        }
+      }
+      q_dot = over_groups(q_dot) * c * own_rq;
+      k_dot = over_groups(k_dot) * c * own_rk;
+      b_dot = over_groups(b_dot) * e_own * own_rk;
+      dbeta -= k_dot;
+      dsum = q_dot - own_beta * k_dot - b_dot;
+      if (lane.g == 0) kept[own] = b_dot;
+    }
+    // Pairs: this lane's token as the row.
+    f32x4 kk[kTiles], qk[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) kk[m] = qk[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      const frag q = read_row<T>(queries, own, ks, lane), k = read_row<T>(keys, own, ks, lane);
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) {
+        if (m / kPer > wave / kPer) continue;
+        const frag other = read_row<T>(keys, operand_row<T>(m, lane.l), ks, lane);
+        qk[m] = Fragment<T>::mma(other, q, qk[m]);
+        kk[m] = Fragment<T>::mma(other, k, kk[m]);
+      }
+    }
+    float pairs = 0.f, steps = 0.f;
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      if (m / kPer > wave / kPer) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = first_row<T>(m, lane.g) + e;
+        const bool open = j <= own && open_between(closed, j < own ? j : own, own);
+        const float ratio = open ? decay_between(own_sum, sum[j]) * rk[j] : 0.f;
+        const float p = open ? ratio * row_p[m][e] : 0.f;
+        const float n = open && j < own ? -ratio * row_a[m][e] : 0.f;
+        pairs = fmaf(p * own_rq, qk[m][e], pairs);
+        steps = fmaf(n * own_rk, kk[m][e], steps);
+        row_p[m][e] = p;
+        row_a[m][e] = own_beta * n;
+      }
+    }
+    steps = over_groups(steps);
+    dbeta += steps;
+    dsum += over_groups(pairs) + own_beta * steps;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      if (kt > wave / kPer) continue;
+      frag p[1], n[1];
+      split<T>(&row_p[kt * kPer], p);
+      split<T>(&row_a[kt * kPer], n);
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        const frag k = read_column<T, true>(keys, m, kt, lane);
+        dq[m] = Fragment<T>::mma(k, p[0], dq[m]);
+        dk[m] = Fragment<T>::mma(k, n[0], dk[m]);
+      }
+    }
+    // And as the column.
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) kk[m] = qk[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      const frag k = read_row<T>(keys, own, ks, lane);
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) {
+        if (m / kPer < wave / kPer) continue;
+        qk[m] = Fragment<T>::mma(read_row<T>(queries, operand_row<T>(m, lane.l), ks, lane), k, qk[m]);
+        kk[m] = Fragment<T>::mma(read_row<T>(keys, operand_row<T>(m, lane.l), ks, lane), k, kk[m]);
+      }
+    }
+    pairs = 0.f;
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      if (m / kPer < wave / kPer) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = first_row<T>(m, lane.g) + e;
+        const bool open = i >= own && open_between(closed, own, i > own ? i : own);
+        const float ratio = open ? decay_between(sum[i], own_sum) : 0.f;
+        const float p = open ? ratio * rq[i] * column_p[m][e] : 0.f;
+        const float n = open && i > own ? -beta[i] * rk[i] * ratio * column_a[m][e] : 0.f;
+        pairs = fmaf(p, qk[m][e], pairs);
+        pairs = fmaf(n, kk[m][e], pairs);
+        column_p[m][e] = p;
+        column_a[m][e] = n;
+      }
+    }
+    dsum -= over_groups(pairs) * own_rk;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      if (kt < wave / kPer) continue;
+      frag p[1], n[1];
+      split<T>(&column_p[kt * kPer], p);
+      split<T>(&column_a[kt * kPer], n);
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        dk[m] = Fragment<T>::mma(read_column<T, true>(queries, m, kt, lane), p[0], dk[m]);
+        dk[m] = Fragment<T>::mma(read_column<T, true>(keys, m, kt, lane), n[0], dk[m]);
+      }
+    }
+    if (lane.g == 0) {
+      slope[own] = dsum;
+      if (in_range) store_gate(a.grad_beta, token * a.heads + h, own < rows ? dbeta : 0.f);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // A token's decay: the gradients of the sums from it on, the last of which has the states' too.
+      const int t = threadIdx.x & 63;
+      float v = t < kTokens ? slope[t] : 0.f, k = t < kTokens ? kept[t] : 0.f;
+      k = lanes_sum<64>(k);
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTiles; ++w) s += inner[w];
+      if (t == kTokens - 1) v += k + record->whole * s;
+#pragma unroll
+      for (int step = 1; step < kTokens; step *= 2) {
+        const float after = __shfl_down(v, step);
+        if (t + step < kTokens) v += after;
+      }
+      if (t < kTokens && t0 + t < a.tokens)
+        store_gate(a.grad_decay, (static_cast<int64_t>(b) * a.tokens + t0 + t) * a.heads + h,
+                   t < rows && (closed >> t & 1) == 0 ? v : 0.f);
+    }
+    if constexpr (GROUPED) {
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        dq_all[m] += dq[m];
+        dk_all[m] += dk[m];
+      }
+    }
+    if (GROUPED && group + 1 < groups) continue;
+    // q = q' / rq and k = k' / rk, with their lengths.
+    const f32x4* dqs = GROUPED ? dq_all : dq;
+    const f32x4* dks = GROUPED ? dk_all : dk;
+    float q_dot = 0.f, k_dot = 0.f;
+    if (a.normalize) {
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        const f32x4 q = own_values(queries, m), k = own_values(keys, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          q_dot = fmaf(q[e], dqs[m][e], q_dot);
+          k_dot = fmaf(k[e], dks[m][e], k_dot);
+        }
+      }
+      q_dot = over_groups(q_dot) * norm * norm;
+      k_dot = over_groups(k_dot) * own_rk * own_rk;
+    }
+    if (in_range) {
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        const int d = m * 16 + lane.g * 4;
+        if (d >= key_size) continue;
+        const f32x4 q = own_values(queries, m), k = own_values(keys, m);
+        store_four(dq_out + d, own_rq * (dqs[m] - q_dot * q), key_size - d);
+        store_four(dk_out + d, own_rk * (dks[m] - k_dot * k), key_size - d);
+      }
+    }
+  }
+}
+
+// ---- few tokens ----------------------------------------------------------------------------------------
+
+// The definition, token by token: a workgroup keeps kDeltaStepColumns columns of a head's state, a
+// thread four of them at DK / 16 keys. One pass over the state gives S^T k and S^T q together, since
+// o = a S^T q + (k.q) u; a token costs one barrier. Bound by reading and writing the state.
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_step(DeltaArgs a) {
+  constexpr int kRows = DK / 16, kQuads = kDeltaStepColumns / 4;
+  __shared__ float sums[2][4][kQuads][12];
+  const int quad = threadIdx.x % kQuads, part = threadIdx.x / kQuads, wave = threadIdx.x >> 6;
+  const int64_t heads = a.batch * a.heads;
+  const int64_t bh = blockIdx.x % heads;
+  const int b = static_cast<int>(bh / a.heads), h = static_cast<int>(bh % a.heads);
+  const int kh = h / static_cast<int>(a.heads / a.key_heads);
+  const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
+  const int v0 = static_cast<int>(blockIdx.x / heads) * kDeltaStepColumns + quad * 4;
+  const int count = value_size - v0;  // columns of this thread, of four
+  const int length = length_of(a, b);
+  f32x4 state[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int d = part + i * 16;
+    state[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (a.first == nullptr || d >= key_size || count <= 0) continue;
+    const float* p = a.first + (bh * key_size + d) * value_size + v0;
+    if (count >= 4) {
+      state[i] = __builtin_bit_cast(f32x4, load_run<4>(p));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < count) state[i][e] = p[e];
+      end_of_part();
+    }
+  }
+  T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size + v0;
+#pragma unroll 1
+  for (int t = 0; t < length; ++t) {
+    const T* kp = at_token<T>(a.key, a.key_strides, b, t, kh);
+    const T* qp = at_token<T>(a.query, a.query_strides, b, t, kh);
+    float k[kRows], q[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int d = part + i * 16;
+      k[i] = d < key_size ? static_cast<float>(kp[d]) : 0.f;
+      q[i] = d < key_size ? static_cast<float>(qp[d]) : 0.f;
+    }
+    const T* vp = at_token<T>(a.value, a.value_strides, b, t, h) + v0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < count) v[e] = static_cast<float>(vp[e]);
+    const int64_t d_at = b * a.decay_strides.batch + t * a.decay_strides.token + h * a.decay_strides.head;
+    const int64_t f_at = b * a.beta_strides.batch + t * a.beta_strides.token + h * a.beta_strides.head;
+    const float decay = a.float_gates ? static_cast<const float*>(a.decay)[d_at]
+                                      : static_cast<float>(static_cast<const T*>(a.decay)[d_at]);
+    const float beta = a.float_gates ? static_cast<const float*>(a.beta)[f_at]
+                                     : static_cast<float>(static_cast<const T*>(a.beta)[f_at]);
+    // S^T k, S^T q, then k.k, q.q, k.q.
+    float s[11] = {};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e] = fmaf(state[i][e], k[i], s[e]);
+        s[4 + e] = fmaf(state[i][e], q[i], s[4 + e]);
+      }
+      s[8] = fmaf(k[i], k[i], s[8]);
+      s[9] = fmaf(q[i], q[i], s[9]);
+      s[10] = fmaf(k[i], q[i], s[10]);
+    }
+#pragma unroll
+    for (int j = 0; j < 11; ++j) {
+      s[j] += __shfl_xor(s[j], 16);
+      s[j] += __shfl_xor(s[j], 32);
+    }
+    if ((threadIdx.x & 63) < kQuads) {
+#pragma unroll
+      for (int j = 0; j < 11; ++j) sums[t & 1][wave][quad][j] = s[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 11; ++j) {
+      s[j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) s[j] += sums[t & 1][w][quad][j];
+    }
+    const float rk = a.normalize ? 1.f / sqrtf(s[8] + kNormEps) : 1.f;
+    const float rq = a.scale * (a.normalize ? 1.f / sqrtf(s[9] + kNormEps) : 1.f);
+    const float keep = decay < kDeltaClosed ? 0.f : expf(decay);
+    f32x4 o;
+    float u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      u[e] = beta * fmaf(-keep * rk, s[e], v[e]) * rk;
+      o[e] = rq * fmaf(keep, s[4 + e], s[10] * u[e]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[i][e] = fmaf(k[i], u[e], keep * state[i][e]);
+    if (part == 0 && count > 0) store_four(out + static_cast<int64_t>(t) * a.heads * value_size, o, count);
+  }
+  if (count <= 0) return;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int d = part + i * 16;
+    if (d < key_size) store_four(a.last + (bh * key_size + d) * value_size + v0, state[i], count);
+  }
+  for (int t = length + part; t < a.tokens; t += 16)
+    store_four(out + static_cast<int64_t>(t) * a.heads * value_size, f32x4{0.f, 0.f, 0.f, 0.f}, count);
+}
+
+// ---- launches --------------------------------------------------------------------------------------------
+
+// Rows [batch, tokens, heads, size] copied with a pitch of whole 16 bytes, zeros past their end.
+template <typename T>
+__global__ __launch_bounds__(256) void delta_copy(DeltaCopy c) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int64_t parts = c.pitch / kVec, total = c.batch * c.tokens * c.heads * parts;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t at = id % parts * kVec, row = id / parts;
+    const int64_t h = row % c.heads, t = row / c.heads % c.tokens, b = row / c.heads / c.tokens;
+    const T* p = at_token<T>(c.from, c.strides, b, t, h) + at;
+    Run<T, kVec> v;
+    if (at + kVec <= c.size) {
+      v = load_run<kVec>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v.v[i] = at + i < c.size ? p[i] : static_cast<T>(0.f);
+    }
+    store_run<kVec>(static_cast<T*>(c.to) + id * kVec, v);
+  }
+}
+
+// More than 64 KB of LDS has to be asked for, once per device and kernel (`asked` is the kernel's).
+template <typename Kernel>
+hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+  if (bytes <= 65536) return hipSuccess;
+  int device = 0;
+  hipError_t err = hipGetDevice(&device);
+  if (err != hipSuccess) return err;
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if ((asked.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
+  err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return err;
+}
+
+template <typename T, int DK>
+hipError_t launch_prepare(const DeltaArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((delta_prepare<T, DK>), dim3(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)),
+                     dim3(Chunk<T>::kTokens * 4), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, int DK, int W, bool KEEP>
+hipError_t launch_walk(const DeltaArgs& a, hipStream_t stream) {
+  constexpr int kBytes = 2 * Stage<T, DK, W>::kBytes;
+  const auto kernel = delta_forward<T, DK, W, KEEP>;
+  static std::atomic<uint64_t> asked{0};
+  const hipError_t err = ask_lds(kernel, kBytes, asked);
+  if (err != hipSuccess) return err;
+  const int64_t tiles = (a.value_size + W * 16 - 1) / (W * 16);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(64 * W), kBytes, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, int DK>
+hipError_t launch_forward(const DeltaArgs& a, const DeltaPlan& p, hipStream_t stream) {
+  if (p.step) {
+    const int64_t tiles = (a.value_size + kDeltaStepColumns - 1) / kDeltaStepColumns;
+    hipLaunchKernelGGL((delta_step<T, DK>), dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(256), 0,
+                       stream, a);
+    return hipGetLastError();
+  }
+  if (a.chunks > 0) {
+    const hipError_t err = launch_prepare<T, DK>(a, stream);
+    if (err != hipSuccess) return err;
+  }
+  return a.states != nullptr ? launch_walk<T, DK, 4, true>(a, stream) : launch_walk<T, DK, 4, false>(a, stream);
+}
+
+template <typename T, int DK>
+hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
+  constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
+  const auto kernel = delta_backward<T, DK, W>;
+  static std::atomic<uint64_t> asked{0};
+  hipError_t err = ask_lds(kernel, kBytes, asked);
+  if (err == hipSuccess && a.chunks > 0) err = launch_prepare<T, DK>(a, stream);
+  if (err != hipSuccess) return err;
+  const int64_t tiles = (a.value_size + W * 16 - 1) / (W * 16);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(64 * W), kBytes, stream, a);
+  err = hipGetLastError();
+  if (err != hipSuccess || a.chunks == 0) return err;
+  const dim3 grid(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)), block(Chunk<T>::kTokens * 4);
+  if (a.heads == a.key_heads)
+    hipLaunchKernelGGL((delta_gradients<T, DK, false>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((delta_gradients<T, DK, true>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t backward_of(const DeltaArgs& a, hipStream_t stream) {
+  return a.key_size <= 64 ? launch_backward<T, 64>(a, stream) : launch_backward<T, 128>(a, stream);
+}
+
+template <typename T>
+hipError_t forward_of(const DeltaArgs& a, const DeltaPlan& p, hipStream_t stream) {
+  return a.key_size <= 64 ? launch_forward<T, 64>(a, p, stream) : launch_forward<T, 128>(a, p, stream);
+}
+
+}  // namespace
+
+int64_t delta_panel_bytes(int element_size) {
+  const int64_t terms = element_size == 2 ? 2 : 1;
+  return 2 * terms * delta_chunk(element_size) * 128;
+}
+int64_t delta_record_bytes(int element_size) {
+  return element_size == 2 ? sizeof(Record<__bf16>) : sizeof(Record<float>);
+}
+
+hipError_t launch_delta_copy(convnd_hip_dtype dtype, const DeltaCopy& c, hipStream_t stream) {
+  const int vec = dtype == CONVND_HIP_FLOAT32 ? 4 : 8;
+  const int64_t work = c.batch * c.tokens * c.heads * (c.pitch / vec);
+  if (work == 0) return hipSuccess;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 8192))), block(256);
+  if (dtype == CONVND_HIP_FLOAT32)
+    hipLaunchKernelGGL(delta_copy<float>, grid, block, 0, stream, c);
+  else  // either 16-bit type: only zeros are made, the rest is moved
+    hipLaunchKernelGGL(delta_copy<_Float16>, grid, block, 0, stream, c);
+  return hipGetLastError();
+}
+
+hipError_t launch_delta(convnd_hip_dtype dtype, const DeltaArgs& a, const DeltaPlan& p, hipStream_t stream) {
+  switch (dtype) {
+    case CONVND_HIP_FLOAT32:
+      return forward_of<float>(a, p, stream);
+    case CONVND_HIP_FLOAT16:
+      return forward_of<_Float16>(a, p, stream);
+    case CONVND_HIP_BFLOAT16:
+      return forward_of<__bf16>(a, p, stream);
+    default:
+      return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_delta_backward(convnd_hip_dtype dtype, const DeltaArgs& a, hipStream_t stream) {
+  switch (dtype) {
+    case CONVND_HIP_FLOAT32:
+      return backward_of<float>(a, stream);
+    case CONVND_HIP_FLOAT16:
+      return backward_of<_Float16>(a, stream);
+    case CONVND_HIP_BFLOAT16:
+      return backward_of<__bf16>(a, stream);
+    default:
+      return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace convnd

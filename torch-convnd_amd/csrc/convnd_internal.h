@@ -658,6 +658,66 @@ RecurrencePlan plan_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, 
 hipError_t launch_recurrence(convnd_hip_dtype dtype, const RecurrenceArgs& a, bool backward,
                              const RecurrencePlan& p, hipStream_t stream);
 
+// Gated delta rule (convnd_delta.hip). Strides in elements of [batch, tokens, heads, size], the last axis
+// contiguous; rows of query, key, value and grad_output start on 4 bytes and are whole 16 bytes long.
+struct DeltaStrides {
+  int64_t batch, token, head;
+};
+struct DeltaArgs {
+  const void* query;          // [batch, tokens, key_heads, key_size]
+  const void* key;
+  const void* value;          // [batch, tokens, heads, value_size]
+  const void* decay;          // [batch, tokens, heads]
+  const void* beta;
+  const void* grad_output;    // [batch, tokens, heads, value_size], backward
+  const float* first;         // [batch, heads, key_size, value_size] or null: zeros
+  const float* grad_last;     // or null: zeros
+  const void* lengths;        // [batch] int32 or int64, or null: all `tokens`
+  void* output;               // [batch, tokens, heads, value_size]
+  float* last;                // [batch, heads, key_size, value_size]
+  char* panels;               // [batch, heads, chunks] of delta_panel_bytes: T and P
+  char* records;              // [batch, heads, chunks] of delta_record_bytes
+  void* states;               // [batch, heads, chunks, value_pad, padded key size]: before each chunk; or null
+  void* updates;              // [batch, heads, chunks, value_pad, chunk]: U transposed
+  void* grad_states;          // as states: the gradient of the state after each chunk
+  void* grad_updates;         // as updates: Y
+  void* grad_query;           // gradients, contiguous
+  void* grad_key;
+  void* grad_value;
+  void* grad_decay;
+  void* grad_beta;
+  float* grad_first;          // or null
+  int64_t batch, tokens, key_heads, heads, key_size, value_size;
+  int64_t chunks;             // of `tokens`
+  int64_t value_pad;          // value_size in whole 16
+  DeltaStrides query_strides, key_strides, value_strides, decay_strides, beta_strides, grad_strides;
+  float scale;
+  int normalize;
+  int float_gates;            // decay and beta are float, else of the element type
+  int wide_lengths;           // lengths are int64
+};
+struct DeltaPlan {
+  bool step;                  // token by token, without workspace
+  int64_t workgroups;         // of the largest launch, and the threads of each
+  int threads;
+};
+// A chunk's tokens for an element size; columns of a step's workgroup; a decay below this closes the
+// token's gate (its exp is zero in float).
+constexpr int delta_chunk(int element_size) { return 128 / element_size; }
+constexpr int kDeltaStepColumns = 64;
+constexpr float kDeltaClosed = -104.f;
+int64_t delta_panel_bytes(int element_size);
+int64_t delta_record_bytes(int element_size);
+struct DeltaCopy {
+  const void* from;           // [batch, tokens, heads, size] by strides
+  void* to;                   // [batch, tokens, heads, pitch]
+  DeltaStrides strides;
+  int64_t batch, tokens, heads, size, pitch;
+};
+hipError_t launch_delta_copy(convnd_hip_dtype dtype, const DeltaCopy& c, hipStream_t stream);
+hipError_t launch_delta(convnd_hip_dtype dtype, const DeltaArgs& a, const DeltaPlan& p, hipStream_t stream);
+hipError_t launch_delta_backward(convnd_hip_dtype dtype, const DeltaArgs& a, hipStream_t stream);
+
 // db[c] = sum of the nsum partial sums of channel c (fixed order).
 hipError_t launch_grad_bias_from_sums(convnd_hip_dtype dtype, const float* sums, int64_t nsum,
                                       int64_t channels, void* db, hipStream_t stream);

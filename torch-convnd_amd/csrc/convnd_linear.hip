@@ -30,45 +30,6 @@
 namespace convnd {
 namespace {
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-constexpr unsigned kNowhere = 0x80000000u;  // past every buffer (below 2^31 bytes)
-
-// 16 bytes of a fragment: for 16-bit types 8 values of K for one MFMA, for float 4 for four.
-template <typename T>
-struct Fragment {
-  static constexpr int kSteps = 1;
-  using type = typename Mfma16<T>::frag;
-  __device__ __forceinline__ static f32x4 mma(type a, type b, f32x4 c) {
-    return Mfma16<T>::run(a, b, c);
-  }
-};
-template <>
-struct Fragment<float> {
-  using type = f32x4;
-  __device__ __forceinline__ static f32x4 mma(type a, type b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-  }
-};
-
-// 16 or 4 bytes per lane from the buffer straight into LDS: lane l writes dst + 16 l (4 l), dst the
-// same for the whole wave. Inline assembly, so that the compiler does not take the LDS reads that
-// follow, of other stages, to depend on them: whoever reads what they bring waits with wait_loads.
-__device__ __forceinline__ void load_lds16(u32x4 rows, unsigned dst, unsigned offset) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst),
-      "v"(offset), "s"(rows)
-      : "m0");
-}
-__device__ __forceinline__ void load_lds4(u32x4 rows, unsigned dst, unsigned offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(dst),
-               "v"(offset), "s"(rows)
-               : "m0");
-}
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // One operand of the product: `extent` rows (its side of the result) by K. Inner: row-major with K
 // contiguous; outer: K rows of `extent` contiguous values. Staged in LDS as it lies in memory, 128 bytes
 // of K (inner) or rows of EXT values (outer), its 16-byte chunks permuted within a row. Rows start

@@ -1,5 +1,6 @@
-// Shared by the sequence kernels (layer norm, linear, gated recurrence): vector accesses of any
-// alignment and reductions over the lanes of a wave.
+// Shared by the sequence kernels (layer norm, linear, gated recurrence, delta rule): vector accesses of
+// any alignment, reductions over the lanes of a wave, fragments of the matrix instructions and loads
+// from memory straight into LDS.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -50,5 +51,44 @@ __device__ __forceinline__ float lanes_sum(float v) {
   if constexpr (N >= 64) v += __shfl_xor(v, 32);
   return v;
 }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr unsigned kNowhere = 0x80000000u;  // past every buffer (below 2^31 bytes)
+
+// 16 bytes of a fragment: for 16-bit types 8 values of K for one MFMA, for float 4 for four.
+template <typename T>
+struct Fragment {
+  static constexpr int kSteps = 1;
+  using type = typename Mfma16<T>::frag;
+  __device__ __forceinline__ static f32x4 mma(type a, type b, f32x4 c) {
+    return Mfma16<T>::run(a, b, c);
+  }
+};
+template <>
+struct Fragment<float> {
+  using type = f32x4;
+  __device__ __forceinline__ static f32x4 mma(type a, type b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// 16 or 4 bytes per lane from the buffer straight into LDS: lane l writes dst + 16 l (4 l), dst the
+// same for the whole wave. Inline assembly, so that the compiler does not take the LDS reads that
+// follow, of other stages, to depend on them: whoever reads what they bring waits with wait_loads.
+__device__ __forceinline__ void load_lds16(u32x4 rows, unsigned dst, unsigned offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst),
+      "v"(offset), "s"(rows)
+      : "m0");
+}
+__device__ __forceinline__ void load_lds4(u32x4 rows, unsigned dst, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(dst),
+               "v"(offset), "s"(rows)
+               : "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 }  // namespace convnd

@@ -1,4 +1,5 @@
-// C ABI of the sequence operators (layer norm, linear layer, gated recurrence): argument checks and launches.
+// C ABI of the sequence operators (layer norm, linear layer, gated recurrence, delta rule): argument checks
+// and launches.
 #include <algorithm>
 #include <cstring>
 #include <string>
@@ -253,6 +254,153 @@ LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_
   if (need_input) b.input_partial = partial_sums(b.input_plan, p.rows, p.inputs, ws);
   if (need_weight) b.weight_partial = partial_sums(b.weight_plan, p.outputs, p.inputs, ws);
   return b;
+}
+
+// ---- delta rule ----------------------------------------------------------------------------------
+
+// Up to so many tokens run one by one.
+constexpr int64_t kDeltaStepTokens = 8;
+
+int check_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* p) {
+  if (size_of(dtype) == 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, std::string("gated_delta_rule ") + kTypes);
+  if (p == nullptr || p->batch < 0 || p->tokens < 0 || p->key_heads <= 0 || p->heads <= 0 ||
+      p->heads % p->key_heads != 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_delta_rule needs nonnegative batch and tokens, and heads that are a multiple of "
+                "the key heads");
+  if (p->key_size <= 0 || p->key_size > 128 || p->value_size <= 0 || p->value_size > 65535)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_delta_rule needs key sizes of 1 to 128 and value sizes of 1 to 65535");
+  if (p->gate_dtype != dtype && p->gate_dtype != CONVND_HIP_FLOAT32)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_delta_rule decay and beta must have the inputs' dtype or float32");
+  if (p->tokens >= (int64_t{1} << 31) - 64 || p->batch >= int64_t{1} << 31 || p->heads >= int64_t{1} << 31)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule needs fewer than 2^31 tokens, sequences and heads");
+  int64_t rows = 0, total = 0, extent = 0;
+  const int64_t steps[] = {p->query_batch, p->query_token, p->query_head, p->key_batch,   p->key_token,
+                           p->key_head,    p->value_batch, p->value_token, p->value_head, p->decay_batch,
+                           p->decay_token, p->decay_head,  p->beta_batch,  p->beta_token, p->beta_head,
+                           p->grad_batch,  p->grad_token,  p->grad_head};
+  const int64_t most = std::max({p->batch, p->tokens, p->heads});
+  for (int64_t step : steps)
+    if (step < 0 || !mul_ok(step, most, &extent))
+      return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule strides overflow int64");
+  if (!mul_ok(p->batch, p->heads, &rows) || !mul_ok(rows, p->tokens + 64, &total) ||
+      !mul_ok(total, (p->value_size + 127) * 128, &total))
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes overflow int64");
+  // A row's place in a chunk is a 32-bit byte offset.
+  if (p->query_token >= kMaxTokenStride || p->key_token >= kMaxTokenStride ||
+      p->value_token >= kMaxTokenStride || p->grad_token >= kMaxTokenStride)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule needs token strides below 2^21 elements");
+  return CONVND_HIP_SUCCESS;
+}
+
+DeltaArgs to_args(convnd_hip_dtype dtype, const convnd_hip_delta_problem& p) {
+  DeltaArgs a{};
+  a.batch = p.batch;
+  a.tokens = p.tokens;
+  a.key_heads = p.key_heads;
+  a.heads = p.heads;
+  a.key_size = p.key_size;
+  a.value_size = p.value_size;
+  const int64_t chunk = delta_chunk(size_of(dtype));
+  a.chunks = (p.tokens + chunk - 1) / chunk;
+  a.value_pad = (p.value_size + 15) / 16 * 16;
+  a.query_strides = {p.query_batch, p.query_token, p.query_head};
+  a.key_strides = {p.key_batch, p.key_token, p.key_head};
+  a.value_strides = {p.value_batch, p.value_token, p.value_head};
+  a.decay_strides = {p.decay_batch, p.decay_token, p.decay_head};
+  a.beta_strides = {p.beta_batch, p.beta_token, p.beta_head};
+  a.grad_strides = {p.grad_batch, p.grad_token, p.grad_head};
+  a.scale = static_cast<float>(p.scale);
+  a.normalize = p.normalize;
+  a.float_gates = p.gate_dtype == CONVND_HIP_FLOAT32;
+  a.wide_lengths = p.wide_lengths;
+  return a;
+}
+
+// Rows as the kernels take them: themselves, or a padded copy in the workspace.
+bool delta_copied(const void* data, const DeltaStrides& s, int64_t columns, int size) {
+  return (reinterpret_cast<uintptr_t>(data) |
+          static_cast<uintptr_t>((s.batch | s.token | s.head) * size)) % 4 != 0 ||
+         columns * size % 16 != 0;
+}
+struct DeltaRows {
+  const void* data;
+  DeltaStrides strides;
+  DeltaCopy copy;
+  bool copied;
+};
+DeltaRows delta_rows(const void* data, const DeltaStrides& s, const DeltaArgs& a, int64_t heads,
+                     int64_t columns, int size, Parts* ws) {
+  DeltaRows r{data, s, {}, delta_copied(data, s, columns, size)};
+  if (!r.copied) return r;
+  const int64_t pitch = padded_columns(columns, size);
+  r.copy = {data, ws->take(a.batch * a.tokens * heads * pitch * size), s, a.batch, a.tokens, heads, columns, pitch};
+  r.data = r.copy.to;
+  r.strides = {a.tokens * heads * pitch, heads * pitch, pitch};
+  return r;
+}
+int fill_rows(convnd_hip_dtype dtype, const DeltaRows& r, hipStream_t stream) {
+  if (!r.copied) return CONVND_HIP_SUCCESS;
+  return hip_check(launch_delta_copy(dtype, r.copy, stream), "delta rule operand copy");
+}
+
+DeltaPlan plan_delta(const DeltaArgs& a, bool saving) {
+  DeltaPlan p{};
+  p.step = !saving && a.tokens <= kDeltaStepTokens;
+  const int64_t columns = kDeltaStepColumns;  // of a walk's four waves too
+  p.workgroups = a.batch * a.heads * ((a.value_size + columns - 1) / columns);
+  p.threads = 256;
+  if (!p.step) p.workgroups = std::max(p.workgroups, a.batch * a.key_heads * a.chunks);
+  return p;
+}
+
+// The workspace of a forward, with the arguments that point into it.
+struct DeltaLayout {
+  DeltaRows query, key, value, grad;
+};
+DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, const void* query, const void* key,
+                          const void* value, Parts* ws) {
+  DeltaLayout l{};
+  l.query = {query, a->query_strides, {}, false};
+  l.key = {key, a->key_strides, {}, false};
+  l.value = {value, a->value_strides, {}, false};
+  if (!p.step) {
+    l.query = delta_rows(query, a->query_strides, *a, a->key_heads, a->key_size, size, ws);
+    l.key = delta_rows(key, a->key_strides, *a, a->key_heads, a->key_size, size, ws);
+    l.value = delta_rows(value, a->value_strides, *a, a->heads, a->value_size, size, ws);
+    const int64_t records = a->batch * a->heads * a->chunks;
+    a->panels = static_cast<char*>(ws->take(records * delta_panel_bytes(size)));
+    a->records = static_cast<char*>(ws->take(records * delta_record_bytes(size)));
+  }
+  a->query = l.query.data;
+  a->key = l.key.data;
+  a->value = l.value.data;
+  a->query_strides = l.query.strides;
+  a->key_strides = l.key.strides;
+  a->value_strides = l.value.strides;
+  return l;
+}
+
+// Elements of the saved states and of the saved updates.
+int64_t saved_states(const DeltaArgs& a) {
+  return a.batch * a.heads * a.chunks * a.value_pad * (a.key_size <= 64 ? 64 : 128);
+}
+int64_t saved_updates(const DeltaArgs& a, int size) {
+  return a.batch * a.heads * a.chunks * a.value_pad * delta_chunk(size);
+}
+
+DeltaLayout lay_out_delta_backward(DeltaArgs* a, int size, const void* grad_output, const void* query,
+                                   const void* key, const void* value, Parts* ws) {
+  DeltaLayout l = lay_out_delta(a, size, plan_delta(*a, true), query, key, value, ws);
+  l.grad = delta_rows(grad_output, a->grad_strides, *a, a->heads, a->value_size, size, ws);
+  a->grad_output = l.grad.data;
+  a->grad_strides = l.grad.strides;
+  a->grad_states = ws->take(saved_states(*a) * size);
+  a->grad_updates = ws->take(saved_updates(*a, size) * size);
+  return l;
 }
 
 // A plan's description as JSON; numbers only beside the kernel's name.
@@ -586,6 +734,114 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
                                            b.weight_partial, on),
                      "linear weight gradient launch");
   return st;
+}
+
+int64_t convnd_hip_delta_saved(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem) {
+  if (check_delta(dtype, problem) != CONVND_HIP_SUCCESS) return 0;
+  const DeltaArgs a = to_args(dtype, *problem);
+  return saved_states(a) + saved_updates(a, size_of(dtype));
+}
+
+size_t convnd_hip_delta_workspace_size(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
+                                       const void* query, const void* key, const void* value, int saving) {
+  if (check_delta(dtype, problem) != CONVND_HIP_SUCCESS || problem->batch == 0) return 0;
+  DeltaArgs a = to_args(dtype, *problem);
+  Parts ws{nullptr};
+  lay_out_delta(&a, size_of(dtype), plan_delta(a, saving != 0), query, key, value, &ws);
+  return ws.used;
+}
+
+int convnd_hip_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem, const void* query,
+                     const void* key, const void* value, const void* decay, const void* beta,
+                     const float* first, const void* lengths, void* output, float* last, void* saved,
+                     void* workspace, size_t workspace_size, void* stream) {
+  int st = check_delta(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  if (problem->batch == 0) return CONVND_HIP_SUCCESS;
+  if (last == nullptr || (problem->tokens > 0 && (query == nullptr || key == nullptr || value == nullptr ||
+                                                  decay == nullptr || beta == nullptr || output == nullptr)))
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "query, key, value, decay, beta, output and last must not be null");
+  DeltaArgs a = to_args(dtype, *problem);
+  const int size = size_of(dtype);
+  const DeltaPlan p = plan_delta(a, saved != nullptr);
+  Parts ws{static_cast<char*>(workspace)};
+  const DeltaLayout l = lay_out_delta(&a, size, p, query, key, value, &ws);
+  if (!launch_fits(p.workgroups, p.threads))
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes are too large: more than 2^32 threads");
+  st = check_parts(ws, workspace_size, "gated_delta_rule");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  a.decay = decay;
+  a.beta = beta;
+  a.first = first;
+  a.lengths = lengths;
+  a.output = output;
+  a.last = last;
+  if (saved != nullptr) {
+    a.states = saved;
+    a.updates = static_cast<char*>(saved) + saved_states(a) * size;
+  }
+  const auto on = static_cast<hipStream_t>(stream);
+  for (const DeltaRows* r : {&l.query, &l.key, &l.value}) {
+    st = fill_rows(dtype, *r, on);
+    if (st != CONVND_HIP_SUCCESS) return st;
+  }
+  return hip_check(launch_delta(dtype, a, p, on), "delta rule launch");
+}
+
+size_t convnd_hip_delta_backward_workspace_size(convnd_hip_dtype dtype,
+                                                const convnd_hip_delta_problem* problem,
+                                                const void* grad_output, const void* query,
+                                                const void* key, const void* value) {
+  if (check_delta(dtype, problem) != CONVND_HIP_SUCCESS || problem->batch == 0) return 0;
+  DeltaArgs a = to_args(dtype, *problem);
+  Parts ws{nullptr};
+  lay_out_delta_backward(&a, size_of(dtype), grad_output, query, key, value, &ws);
+  return ws.used;
+}
+
+int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
+                              const void* grad_output, const float* grad_last, const void* query,
+                              const void* key, const void* value, const void* decay, const void* beta,
+                              const void* lengths, const void* saved, void* grad_query, void* grad_key,
+                              void* grad_value, void* grad_decay, void* grad_beta, float* grad_first,
+                              void* workspace, size_t workspace_size, void* stream) {
+  int st = check_delta(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  if (problem->batch == 0) return CONVND_HIP_SUCCESS;
+  if (problem->tokens > 0 &&
+      (grad_output == nullptr || query == nullptr || key == nullptr || value == nullptr || decay == nullptr ||
+       beta == nullptr || saved == nullptr || grad_query == nullptr || grad_key == nullptr ||
+       grad_value == nullptr || grad_decay == nullptr || grad_beta == nullptr))
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "grad_output, query, key, value, decay, beta, saved and their gradients must not be null");
+  DeltaArgs a = to_args(dtype, *problem);
+  const int size = size_of(dtype);
+  Parts ws{static_cast<char*>(workspace)};
+  const DeltaLayout l = lay_out_delta_backward(&a, size, grad_output, query, key, value, &ws);
+  const DeltaPlan p = plan_delta(a, true);
+  if (!launch_fits(p.workgroups, p.threads))
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes are too large: more than 2^32 threads");
+  st = check_parts(ws, workspace_size, "gated_delta_rule backward");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  a.decay = decay;
+  a.beta = beta;
+  a.lengths = lengths;
+  a.grad_last = grad_last;
+  a.states = const_cast<void*>(saved);
+  a.updates = const_cast<char*>(static_cast<const char*>(saved)) + saved_states(a) * size;
+  a.grad_query = grad_query;
+  a.grad_key = grad_key;
+  a.grad_value = grad_value;
+  a.grad_decay = grad_decay;
+  a.grad_beta = grad_beta;
+  a.grad_first = grad_first;
+  const auto on = static_cast<hipStream_t>(stream);
+  for (const DeltaRows* r : {&l.query, &l.key, &l.value, &l.grad}) {
+    st = fill_rows(dtype, *r, on);
+    if (st != CONVND_HIP_SUCCESS) return st;
+  }
+  return hip_check(launch_delta_backward(dtype, a, on), "delta rule backward launch");
 }
 
 int convnd_hip_linear_plan_describe(convnd_hip_dtype dtype,

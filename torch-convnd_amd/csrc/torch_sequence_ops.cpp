@@ -2,83 +2,10 @@
 // gated_recurrence with their backward operators, a thin layer over the C ABI. The
 // schemas are defined from Python (torch_convnd/_operators.py); no counterpart in the reference.
 
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
-
-#include <array>
-#include <optional>
-#include <string>
-#include <tuple>
-#include <vector>
-
-#include "convnd_hip.h"
+#include "torch_sequence.h"
 
 namespace torch_convnd_hip {
 namespace {
-
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-using OptionalTensor = std::optional<at::Tensor>;
-
-bool native_type(at::ScalarType type) {
-  return type == at::kFloat || type == at::kHalf || type == at::kBFloat16;
-}
-
-convnd_hip_dtype sequence_dtype(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat:
-      return CONVND_HIP_FLOAT32;
-    case at::kHalf:
-      return CONVND_HIP_FLOAT16;
-    default:
-      return CONVND_HIP_BFLOAT16;
-  }
-}
-
-void check_status(int status) {
-  TORCH_CHECK(status == CONVND_HIP_SUCCESS, convnd_hip_last_error());
-}
-
-void* stream_of(const at::Tensor& t) {
-  return static_cast<void*>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
-}
-
-const void* data_or_null(const OptionalTensor& t) {
-  return t.has_value() ? t->const_data_ptr() : nullptr;
-}
-
-bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
-bool wants_grad(const OptionalTensor& t) { return t.has_value() && wants_grad(*t); }
-
-void check_once(const char* name) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), name,
-              " is differentiable once on the gfx950 kernels; use backend='torch' for "
-              "create_graph=True");
-}
-
-// Rows of contiguous channels a fixed stride apart: the tensor itself where its layout allows,
-// else a contiguous copy.
-struct Rows {
-  at::Tensor tensor;
-  int64_t stride;
-};
-Rows as_rows(const at::Tensor& t) {
-  const int64_t last = t.dim() - 1, channels = t.size(last);
-  if (t.is_contiguous()) return {t, channels};
-  bool regular = t.stride(last) == 1 || channels == 1;
-  int64_t stride = -1, span = 1;
-  for (int64_t a = last - 1; a >= 0 && regular; --a) {
-    if (t.size(a) == 1) continue;
-    if (stride < 0) stride = t.stride(a);
-    regular = t.stride(a) == stride * span;
-    span *= t.size(a);
-  }
-  if (!regular || t.numel() == 0) return {t.contiguous(), channels};
-  return {t, stride < 0 ? channels : stride};
-}
 
 // ---- layer norm ----------------------------------------------------------------------------
 
@@ -107,11 +34,6 @@ convnd_hip_dtype parameter_dtype(const at::Tensor& input, const OptionalTensor& 
                                  const OptionalTensor& bias) {
   if (weight.has_value()) return sequence_dtype(*weight);
   return bias.has_value() ? sequence_dtype(*bias) : sequence_dtype(input);
-}
-
-OptionalTensor contiguous(const OptionalTensor& t) {
-  if (!t.has_value()) return std::nullopt;
-  return t->contiguous();
 }
 
 std::tuple<at::Tensor, at::Tensor> layer_norm_device(const at::Tensor& input,
@@ -252,13 +174,6 @@ void check_linear_input(const at::Tensor& input, const at::Tensor& weight) {
               "linear_act expects an input of [..., inputs] and a weight of [outputs, inputs]");
   TORCH_CHECK(weight.device() == input.device() && weight.scalar_type() == input.scalar_type(),
               "input and weight must have the same device and dtype");
-}
-
-// Rows no closer than their length, as the kernels take them.
-Rows as_apart_rows(const at::Tensor& t) {
-  auto r = as_rows(t);
-  if (r.stride >= t.size(-1) && r.stride < (int64_t{1} << 21)) return r;
-  return {t.contiguous(), t.size(-1)};
 }
 
 convnd_hip_linear_problem linear_problem(const at::Tensor& input, const at::Tensor& weight,

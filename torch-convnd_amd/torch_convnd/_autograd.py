@@ -247,6 +247,30 @@ def _fake_recurrence_backward(grad_output, grad_last, input, gate, lengths, carr
 RECURRENCE_TILE = 64
 
 
+def delta_saved(query, value):
+    """Elements that gated_delta_rule saves: a state and its tokens' updates a chunk
+    (convnd_hip_delta_saved)."""
+    batch, tokens, _, key_size = query.shape
+    chunk = 128 // query.element_size()
+    rows = batch * value.shape[2] * ((tokens + chunk - 1) // chunk) * ((value.shape[3] + 15) // 16 * 16)
+    return rows * ((64 if key_size <= 64 else 128) + chunk)
+
+
+def _fake_delta(query, key, value, decay, beta, initial_state, lengths, scale, normalize, keep):
+    contiguous = torch.contiguous_format
+    shape = (query.shape[0], value.shape[2], query.shape[3], value.shape[3])
+    saved = query.new_empty((delta_saved(query, value) if keep else 0,))
+    return torch.empty_like(value, memory_format=contiguous), query.new_empty(shape, dtype=torch.float32), saved
+
+
+def _fake_delta_backward(
+    grad_output, grad_last, query, key, value, decay, beta, lengths, saved, scale, normalize, need_initial_state
+):
+    grads = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (query, key, value, decay, beta)]
+    shape = (query.shape[0], value.shape[2], query.shape[3], value.shape[3])
+    return (*grads, query.new_empty(shape, dtype=torch.float32) if need_initial_state else None)
+
+
 # Derivatives of the sequence operators while the native library is not loaded (a graph compiled as
 # the first use, a direct call of the operator), as its C++ autograd kernels have them: what the
 # backward reads is no differentiable result, and they are differentiable once. A forward called
@@ -327,10 +351,35 @@ def _recurrence_backward(ctx, grad_output, grad_last, _):
     return (*grads, None, None)
 
 
+def _setup_delta(ctx, inputs, output):
+    *tensors, initial_state, lengths, ctx.scale, ctx.normalize, ctx.kept = inputs
+    ctx.first = initial_state is not None
+    ctx.save_for_backward(*tensors, lengths, output[2], None if ctx.kept else initial_state)
+    _keep_apart(ctx, output[2])
+
+
+def _delta_backward(ctx, grad_output, grad_last, _):
+    _check_once("gated_delta_rule")
+    if grad_output is None and grad_last is None:
+        return (None,) * 10
+    *tensors, lengths, saved, initial_state = ctx.saved_tensors
+    ops = torch.ops.torch_convnd
+    if not ctx.kept:
+        saved = ops.gated_delta_rule.default(*tensors, initial_state, lengths, ctx.scale, ctx.normalize, True)[2]
+    if grad_output is None:
+        grad_output = torch.zeros_like(tensors[2])
+    need = ctx.first and ctx.needs_input_grad[5]
+    grads = ops.gated_delta_rule_backward.default(
+        grad_output, grad_last, *tensors, lengths, saved, ctx.scale, ctx.normalize, need
+    )
+    return (*grads, None, None, None, None)
+
+
 _SEQUENCE_DERIVATIVES = {
     "layer_norm": (_layer_norm_backward, _setup_layer_norm),
     "linear_act": (_linear_act_backward, _setup_linear_act),
     "gated_recurrence": (_recurrence_backward, _setup_recurrence),
+    "gated_delta_rule": (_delta_backward, _setup_delta),
 }
 
 _PY_AUTOGRAD = None
@@ -359,6 +408,8 @@ def register_training() -> None:
     torch.library.register_fake("torch_convnd::linear_act_backward")(_fake_linear_act_backward)
     torch.library.register_fake("torch_convnd::gated_recurrence")(_fake_recurrence)
     torch.library.register_fake("torch_convnd::gated_recurrence_backward")(_fake_recurrence_backward)
+    torch.library.register_fake("torch_convnd::gated_delta_rule")(_fake_delta)
+    torch.library.register_fake("torch_convnd::gated_delta_rule_backward")(_fake_delta_backward)
     torch.library.register_autograd(
         "torch_convnd::partial_rescale", _rescale_backward, setup_context=_setup_rescale
     )

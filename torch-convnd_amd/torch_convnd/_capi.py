@@ -46,6 +46,11 @@ EXPORTED_SYMBOLS = (
     "convnd_hip_recurrence",
     "convnd_hip_recurrence_backward",
     "convnd_hip_recurrence_plan_describe",
+    "convnd_hip_delta_saved",
+    "convnd_hip_delta_workspace_size",
+    "convnd_hip_delta",
+    "convnd_hip_delta_backward_workspace_size",
+    "convnd_hip_delta_backward",
 )
 
 CHANNELS_FIRST, CHANNELS_LAST, CHANNELS_LAST_INPUT = 0, 1, 2
@@ -99,6 +104,23 @@ class RecurrenceProblem(ctypes.Structure):
         (name, ctypes.c_int64)
         for name in ("batch", "tokens", "channels", "input_batch", "input_token", "gate_batch", "gate_token")
     ] + [("wide_lengths", ctypes.c_int)]
+
+
+class DeltaProblem(ctypes.Structure):
+    """struct convnd_hip_delta_problem."""
+
+    _fields_ = [
+        (name, ctypes.c_int64) for name in ("batch", "tokens", "key_heads", "heads", "key_size", "value_size")
+    ] + [
+        (f"{tensor}_{axis}", ctypes.c_int64)
+        for tensor in ("query", "key", "value", "decay", "beta", "grad")
+        for axis in ("batch", "token", "head")
+    ] + [
+        ("scale", ctypes.c_double),
+        ("normalize", ctypes.c_int),
+        ("gate_dtype", ctypes.c_int),
+        ("wide_lengths", ctypes.c_int),
+    ]
 
 
 def bind(library: ctypes.CDLL) -> ctypes.CDLL:
@@ -181,6 +203,17 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     library.convnd_hip_recurrence_backward.argtypes = [
         ctypes.c_int, R, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp
     ]
+    D = ctypes.POINTER(DeltaProblem)
+    library.convnd_hip_delta_saved.restype = i64
+    library.convnd_hip_delta_saved.argtypes = [ctypes.c_int, D]
+    library.convnd_hip_delta_workspace_size.restype = sz
+    library.convnd_hip_delta_workspace_size.argtypes = [ctypes.c_int, D, vp, vp, vp, ctypes.c_int]
+    library.convnd_hip_delta.restype = ctypes.c_int
+    library.convnd_hip_delta.argtypes = [ctypes.c_int, D, *[vp] * 11, sz, vp]
+    library.convnd_hip_delta_backward_workspace_size.restype = sz
+    library.convnd_hip_delta_backward_workspace_size.argtypes = [ctypes.c_int, D, vp, vp, vp, vp]
+    library.convnd_hip_delta_backward.restype = ctypes.c_int
+    library.convnd_hip_delta_backward.argtypes = [ctypes.c_int, D, *[vp] * 16, sz, vp]
     library.convnd_hip_linear_plan_describe.restype = ctypes.c_int
     library.convnd_hip_linear_plan_describe.argtypes = [ctypes.c_int, L, ctypes.c_int, ctypes.c_char_p, sz]
     library.convnd_hip_recurrence_plan_describe.restype = ctypes.c_int

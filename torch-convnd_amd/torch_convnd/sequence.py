@@ -1,6 +1,6 @@
 """Operators of token sequences around the convolution: layer norm, the linear layer with its
-activation and residual, and the gated linear recurrence, over activations of [..., channels]. No
-counterpart in the reference.
+activation and residual, the gated linear recurrence and the gated delta rule, over activations of
+[..., channels]. No counterpart in the reference.
 
 ``backend`` as for ``conv_nd``: ``auto`` runs the gfx950 kernels for ROCm GPU tensors (float16,
 bfloat16, float32; other types are refused there) and PyTorch operations for other devices and
@@ -225,3 +225,123 @@ def _portable_recurrence(input, gate, initial_state, lengths):
     if lengths is not None:
         output = torch.where(live, output, 0)
     return output.to(input.dtype), h
+
+
+def gated_delta_rule(
+    query: Tensor,
+    key: Tensor,
+    value: Tensor,
+    decay: Tensor,
+    beta: Tensor,
+    initial_state: Tensor | None = None,
+    *,
+    lengths: Tensor | None = None,
+    scale: float | None = None,
+    normalize: bool = False,
+    backend: str = "auto",
+) -> tuple[Tensor, Tensor]:
+    """A matrix state a head, corrected towards each token's value; returns ``(output, last_state)``:
+
+        S[t] = a[t] * S[t-1] + k[t] u[t]^T,  u[t] = beta[t] * (v[t] - a[t] * S[t-1]^T k[t])
+        output[t] = scale * S[t]^T q[t],  a = exp(decay)
+
+    ``query`` and ``key`` are [batch, tokens, key_heads, key_size], ``value`` [batch, tokens, heads,
+    value_size] with ``heads`` a multiple of ``key_heads`` (value heads share the query and key head of
+    their group, in order). ``decay`` (the logarithm of what a token keeps of the state) and ``beta``
+    are [batch, tokens, heads], both in the inputs' dtype or float32. ``scale`` is ``key_size ** -0.5`` if
+    None; ``normalize`` divides q and k by ``sqrt(|.|^2 + 1e-6)``, without which keys have to be of
+    about unit length (a beta of more than 2 / |k|^2 makes the state grow without end).
+
+    ``initial_state`` and ``last_state`` are float32 [batch, heads, key_size, value_size] (zeros if None), so
+    that a prompt's last state starts the next call, of one token when decoding. ``lengths`` as for
+    ``gated_recurrence``. A decay of -inf (below -104, where its exp in float32 is zero) forgets all before
+    it: where a packed document starts. The gfx950 kernels take key sizes up to 128. They read slices of
+    wider rows in place, keep states in float32 and products within the last bits of the result's dtype, and
+    take more than a few tokens in chunks: there a NaN reaches its whole chunk of 64 tokens, and beside
+    float16 what is added to states has to be within its range.
+    """
+    if is_autocast_enabled(query.device.type):
+        dtype = autocast_dtype(query.device.type)
+        cast = lambda t: t.to(dtype) if t.dtype in _NATIVE_DTYPES else t  # noqa: E731
+        query, key, value = cast(query), cast(key), cast(value)
+        if decay.dtype != beta.dtype or decay.dtype != torch.float32:
+            decay, beta = cast(decay), cast(beta)
+    if scale is None:
+        scale = query.shape[-1] ** -0.5 if query.dim() > 0 and query.shape[-1] > 0 else 1.0
+    if _use_native(query, backend, "gated_delta_rule"):
+        keep = _recording(query, key, value, decay, beta, initial_state)
+        output, last, _ = torch.ops.torch_convnd.gated_delta_rule.default(
+            query, key, value, decay, beta, initial_state, lengths, scale, normalize, keep
+        )
+        return output, last
+    return _portable_delta(query, key, value, decay, beta, initial_state, lengths, scale, normalize)
+
+
+def _portable_delta(query, key, value, decay, beta, initial_state, lengths, scale, normalize):
+    """Token by token in float32 (float64 for float64 inputs)."""
+    if query.dim() != 4 or key.shape != query.shape or query.shape[2] == 0 or query.shape[3] == 0:
+        raise RuntimeError("gated_delta_rule expects query and key of [batch, tokens, key_heads, key_size]")
+    batch, tokens, key_heads, key_size = query.shape
+    if (
+        value.dim() != 4
+        or value.shape[:2] != query.shape[:2]
+        or value.shape[2] == 0
+        or value.shape[3] == 0
+        or value.shape[2] % key_heads
+    ):
+        raise RuntimeError(
+            "gated_delta_rule expects a value of [batch, tokens, heads, value_size], heads a multiple of key_heads"
+        )
+    heads, value_size = value.shape[2:]
+    if decay.shape != value.shape[:3] or beta.shape != value.shape[:3]:
+        raise RuntimeError("gated_delta_rule expects decay and beta of [batch, tokens, heads]")
+    if any(t.device != query.device or t.dtype != query.dtype for t in (key, value)):
+        raise RuntimeError("gated_delta_rule query, key and value must have the same device and dtype")
+    if (
+        decay.device != query.device
+        or beta.device != query.device
+        or beta.dtype != decay.dtype
+        or decay.dtype not in (query.dtype, torch.float32)
+    ):
+        raise RuntimeError(
+            "gated_delta_rule decay and beta must be on the inputs' device, both of their dtype or float32"
+        )
+    wide = torch.float64 if query.dtype == torch.float64 else torch.float32
+    shape = (batch, heads, key_size, value_size)
+    if initial_state is not None and (
+        initial_state.shape != shape
+        or initial_state.device != query.device
+        or initial_state.dtype not in (torch.float32, wide)
+    ):
+        raise RuntimeError(
+            "gated_delta_rule initial_state must be float32 of [batch, heads, key_size, value_size] on the "
+            "inputs' device"
+        )
+    if lengths is not None and (
+        lengths.shape != (batch,)
+        or lengths.device != query.device
+        or lengths.dtype not in (torch.int32, torch.int64)
+    ):
+        raise RuntimeError("gated_delta_rule lengths must be int32 or int64 of [batch] on the inputs' device")
+    state = query.new_zeros(shape, dtype=wide) if initial_state is None else initial_state.to(wide)
+    q, k, v, g, b = (t.to(wide) for t in (query, key, value, decay, beta))
+    if lengths is not None:
+        # Tokens that do nothing, before any arithmetic, so that nothing held past a length reaches a
+        # state or a gradient.
+        live = torch.arange(tokens, device=query.device) < lengths[:, None]
+        q, k, v = (torch.where(live[..., None, None], t, 0) for t in (q, k, v))
+        g, b = (torch.where(live[..., None], t, 0) for t in (g, b))
+    if normalize:
+        q = q / (q.square().sum(dim=-1, keepdim=True) + 1e-6).sqrt()
+        k = k / (k.square().sum(dim=-1, keepdim=True) + 1e-6).sqrt()
+    q = (q * scale).repeat_interleave(heads // key_heads, dim=2)
+    k = k.repeat_interleave(heads // key_heads, dim=2)
+    keep = torch.where(g < -104, 0, torch.exp(g))
+    outputs = []
+    for t in range(tokens):
+        state = keep[:, t, :, None, None] * state
+        update = b[:, t, :, None] * (v[:, t] - (k[:, t, :, :, None] * state).sum(dim=2))
+        state = state + k[:, t, :, :, None] * update[:, :, None, :]
+        outputs.append((q[:, t, :, :, None] * state).sum(dim=2))
+    output = torch.stack(outputs, dim=1) if outputs else v
+    return output.to(value.dtype), state
