@@ -43,7 +43,8 @@ typedef enum convnd_hip_activation {
   CONVND_HIP_ACT_NONE = 0,
   CONVND_HIP_ACT_RELU = 1,
   CONVND_HIP_ACT_GELU = 2,
-  CONVND_HIP_ACT_GELU_TANH = 3
+  CONVND_HIP_ACT_GELU_TANH = 3,
+  CONVND_HIP_ACT_SILU = 4 /* of the gated linear layer */
 } convnd_hip_activation;
 
 /* Memory layout of the activation tensors of a call (input, output, grad_output and
@@ -336,6 +337,39 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
 int convnd_hip_linear_plan_describe(convnd_hip_dtype dtype,
                                     const convnd_hip_linear_problem* problem, int which,
                                     char* buffer, size_t length);
+
+/* Gated linear layer over rows of features: with weight = [Wg; Wu] of [2 outputs, inputs] and bias =
+ * [bg; bu] of [2 outputs] or null,
+ *   output = act(input Wg^T + bg) * (input Wu^T + bu)
+ * by a linear problem whose `outputs` are those of the layer (2 outputs below 2^21), without a residual.
+ * activation: relu, gelu, gelu_tanh or silu. */
+size_t convnd_hip_gated_linear_workspace_size(convnd_hip_dtype dtype,
+                                              const convnd_hip_linear_problem* problem,
+                                              const void* input, const void* weight);
+
+/* Bytes of what the forward keeps for the backward: two factors an output, of 4 bytes beside float32, else
+ * of 3. */
+size_t convnd_hip_gated_linear_kept_size(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem);
+
+/* Products are summed in float32; biases, activation and product are applied in float32 before the one
+ * rounding. kept: for the backward, or null. */
+int convnd_hip_gated_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                            const void* input, const void* weight, const void* bias, void* output,
+                            void* kept, void* workspace, size_t workspace_size, void* stream);
+
+size_t convnd_hip_gated_linear_backward_workspace_size(convnd_hip_dtype dtype,
+                                                       const convnd_hip_linear_problem* problem,
+                                                       const void* input, const void* weight,
+                                                       int need_grad_input, int need_grad_weight,
+                                                       int need_grad_bias);
+
+/* Gradients for the cotangent grad_output [rows, outputs] by its stride, as of the linear layer: a null
+ * grad_input [rows, inputs], grad_weight [2 outputs, inputs] or grad_bias [2 outputs] is skipped. */
+int convnd_hip_gated_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                                     const void* grad_output, const void* input, const void* weight,
+                                     const void* kept, void* grad_input, void* grad_weight,
+                                     void* grad_bias, void* workspace, size_t workspace_size,
+                                     void* stream);
 
 /* Gated linear recurrence over the token axis,
  *   h[t] = a[t] h[t-1] + (1 - a[t]) input[t],  a[t] = sigmoid(gate[t]),  h[-1] = first,

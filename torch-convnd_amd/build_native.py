@@ -131,6 +131,7 @@ def build_ops_library(verbose: bool = False) -> Path:
         str(CSRC / "torch_ops.cpp"),
         str(CSRC / "torch_sequence_ops.cpp"),
         str(CSRC / "torch_delta_ops.cpp"),
+        str(CSRC / "torch_gated_linear_ops.cpp"),
         str(CSRC / "convnd_cpu.cpp"),
         "-fopenmp",
         "-o",

@@ -580,7 +580,8 @@ struct LinearArgs {
   const void* residual;       // [m, n] or null
   int64_t residual_stride;
   void* output;               // [m, n]
-  void* slope;                // [m, n]: the activation's slope (float, or 16 bits), or null
+  void* slope;                // [m, n]: the activation's slope (float, or 16 bits), or null; of the gated
+                              // layer, whose n is that of its outputs, [m, 2 n] factors
   float* partial;             // [splits, m, n] where K is split, else null
   int activation;
 };
@@ -594,6 +595,9 @@ struct LinearPlan {
 LinearPlan plan_product(convnd_hip_dtype dtype, LinearProduct which, int64_t m, int64_t n, int64_t k);
 hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, LinearProduct which,
                                  const LinearPlan& p, float* partial, hipStream_t stream);
+// The gated layer's forward: b is [2 n, k], the plan that of a product of 2 n columns.
+hipError_t launch_gated_product(convnd_hip_dtype dtype, const LinearArgs& a, const LinearPlan& p, float* partial,
+                                hipStream_t stream);
 // The input's and the weight's gradient in one launch, and with them the bias's: `output` [columns] is
 // the sum of `parts` rows (null: none).
 struct LinearSums {
@@ -616,6 +620,7 @@ struct LinearGradArgs {
   void* grad_pre;           // [rows, columns] by pitch, or null
   float* partial;           // [parts, columns], or null
   int64_t rows, columns, grad_stride, pitch;
+  bool gated;               // slope is [rows, 2 columns] of factors, grad_pre and partial of 2 columns
 };
 int64_t linear_grad_parts(int64_t rows, int64_t columns);
 hipError_t launch_linear_grad(convnd_hip_dtype dtype, const LinearGradArgs& a, int64_t parts,

@@ -17,6 +17,11 @@
 //     are added in order by a second launch with the epilogue.
 //   * Up to 64 rows (decoding), not too long: bound by reading W once. A workgroup takes 16 rows of W, its waves
 //     take parts of K and read fragments from memory into registers, all in flight at once.
+//
+// The gated layer, y = act(x Wg^T + bg) (x Wu^T + bu) with W = [Wg; Wu], takes the same product with the
+// columns of a tile half Wg's rows and half the matching ones of Wu, a wave's both, so that its epilogue has
+// both sums of an output. Its backward is dz = [dy u act'(g), dy act(g)] in one pass and the linear layer's
+// products of twice the outputs.
 // The bounds of a tile are those of the buffers it reads through; 16-bit rows of odd length or stride
 // are first copied to the workspace with padding.
 
@@ -127,6 +132,69 @@ struct Operand {
   }
 };
 
+// The gated layer's W as such an operand: of every 16 NB rows of the stage (a wave's columns) the first half
+// are Wg's from `at` on, the second half the same ones of Wu, `extent` rows further.
+template <typename T, int EXT, int W, int NB>
+struct GatedOperand {
+  using Half = Operand<T, false, EXT, W>;
+  static constexpr int kK = Half::kK, kBytes = Half::kBytes, kLoads = Half::kLoads;
+  struct Buffers {
+    u32x4 half[2];
+  };
+  Half gate, up;
+
+  // Whether load i is of Wu's rows (8 rows a load).
+  __device__ __forceinline__ static bool second(int wave, int i) { return (i * W + wave) * 8 / 16 % NB >= NB / 2; }
+  __device__ __forceinline__ void init(const void* p, int64_t ld_elements, int64_t extent, int64_t at, int64_t k0) {
+    gate.init(p, ld_elements, extent, at, k0);
+    const int64_t rows = extent - at < EXT / 2 ? extent - at : EXT / 2;
+    gate.before_last = static_cast<unsigned>((rows - 1) * gate.ld);
+    up = gate;
+    up.base += extent * gate.ld;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = ((i * W + wave) * 64 + lane) / 8;  // of the stage, to that of its half
+      const int local = row / (16 * NB) * (8 * NB) + row % (8 * NB);
+      gate.offset[i] += static_cast<unsigned>(local - row) * static_cast<unsigned>(gate.ld);
+    }
+  }
+  __device__ __forceinline__ Buffers rows(int k) const { return {{gate.rows(k), up.rows(k)}}; }
+  __device__ __forceinline__ void advance() {
+    gate.advance();
+    up.advance();
+  }
+  __device__ __forceinline__ void load(const Buffers& b, unsigned dst, int wave, int i) const {
+    gate.load(second(wave, i) ? b.half[1] : b.half[0], dst, wave, i);
+  }
+  __device__ __forceinline__ void load_last(unsigned dst, int wave, int k) const {
+    const Buffers b = rows(k);
+    const int lane = threadIdx.x & 63;
+    if (k % Half::kVec == 0) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int chunk = (i * W + wave) * 64 + lane;
+        const bool inside = ((chunk % 8) ^ Half::swizzle(chunk / 8)) * Half::kVec < k;
+        load_lds16(second(wave, i) ? b.half[1] : b.half[0], dst + (i * W + wave) * 1024,
+                   inside ? gate.offset[i] : kNowhere);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const u32x4 r = second(wave, i) ? b.half[1] : b.half[0];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int word = ((i * W + wave) * 4 + q) * 64 + lane, row = word / 32;
+          const int local = row / (16 * NB) * (8 * NB) + row % (8 * NB);
+          const int column = ((word % 32 / 4) ^ Half::swizzle(row)) * 16 + word % 4 * 4;
+          const unsigned at = static_cast<unsigned>(local) * static_cast<unsigned>(gate.ld) + column;
+          load_lds4(r, dst + ((i * W + wave) * 4 + q) * 256, column < k * int{sizeof(T)} ? at : kNowhere);
+        }
+      }
+    }
+  }
+};
+
 // Fragment reads of a wave: COUNT fragments of 16 rows (or columns) from `first` on.
 template <typename T, bool OUTER, int EXT, int COUNT>
 struct Reader {
@@ -221,6 +289,14 @@ __device__ __forceinline__ void activate_all(float (&v)[8], float (&d)[8], int a
       const auto [phi, gauss] = normal<T>(v[e]);
       if constexpr (SLOPE) d[e] = fmaf(v[e] * 0.39894228040143268f, gauss, phi);
       v[e] *= phi;
+    }
+  } else if (act == CONVND_HIP_ACT_SILU) {
+    // z s, s = 1 / (1 + exp(-z)); its slope s + z s (1 - s).
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * v[e]));
+      if constexpr (SLOPE) d[e] = fmaf(v[e], fmaf(-s, s, s), s);
+      v[e] *= s;
     }
   } else if (act == CONVND_HIP_ACT_GELU_TANH) {
     // 0.5 z (1 + tanh u) = z s, s = 1 / (1 + exp(-2 u)), u = c z (1 + q z^2) with c = sqrt(2 / pi)
@@ -373,14 +449,102 @@ __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[8], const
   }
 }
 
+// What the gated layer keeps for its backward: [u act'(g), act(g)], by which dy is multiplied. Beside
+// 16-bit types 24 bits of each float, the upper 16 and the next 8 in arrays of their own: rounded to the
+// element type they would add two roundings to dz's own one (gradients 1.73 of their rounding off where this
+// makes 1.41), and as floats a third more bytes.
+template <typename T>
+__device__ __forceinline__ void keep_factors(const LinearArgs& a, const float (&v)[8], int64_t at, int count) {
+  if constexpr (sizeof(T) == 2) {
+    Run<uint16_t, 8> high;
+    Run<uint8_t, 8> low;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned bits = __builtin_bit_cast(unsigned, v[e]) + 0x80u;
+      high.v[e] = static_cast<uint16_t>(bits >> 16);
+      low.v[e] = static_cast<uint8_t>(bits >> 8);
+    }
+    uint16_t* h = static_cast<uint16_t*>(a.slope) + at;
+    uint8_t* l = static_cast<uint8_t*>(a.slope) + a.m * a.n * 4 + at;
+    if (count == 8) {
+      stream_run(h, high);  // read by the backward pass, long after
+      store_run<8>(l, low);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) {
+          h[e] = high.v[e];
+          l[e] = low.v[e];
+        }
+      end_of_part();
+    }
+  } else {
+    float* p = static_cast<float*>(a.slope) + at;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) p[e] = v[e];
+  }
+}
+__device__ __forceinline__ float factor_of(uint16_t high, uint8_t low) {
+  return __builtin_bit_cast(float, static_cast<unsigned>(high) << 16 | static_cast<unsigned>(low) << 8);
+}
+
+// Up to 8 neighbouring outputs of row m from column n on, of the gate's sums and the others'.
+template <typename T>
+__device__ __forceinline__ void finish_gated(const LinearArgs& a, float (&g)[8], float (&u)[8], int64_t split,
+                                             int64_t m, int64_t n, int count) {
+  if (a.partial != nullptr) {
+    float* p = a.partial + (split * a.m + m) * 2 * a.n + n;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) {
+        p[e] = g[e];
+        p[a.n + e] = u[e];
+      }
+    end_of_part();
+    return;
+  }
+  if (a.bias != nullptr) {
+    const T* bias = static_cast<const T*>(a.bias) + n;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) {
+        g[e] += static_cast<float>(bias[e]);
+        u[e] += static_cast<float>(bias[a.n + e]);
+      }
+  }
+  float d[8];
+  if (a.slope != nullptr) {
+    activate_all<T, true>(g, d, a.activation);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] *= u[e];
+    keep_factors<T>(a, d, m * 2 * a.n + n, count);
+    keep_factors<T>(a, g, m * 2 * a.n + a.n + n, count);
+  } else {
+    activate_all<T, false>(g, d, a.activation);
+  }
+  T* out = static_cast<T*>(a.output) + m * a.n + n;
+  Run<T, 8> y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y.v[e] = static_cast<T>(g[e] * u[e]);
+  if (count == 8) {
+    store_run<8>(out, y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) out[e] = y.v[e];
+    end_of_part();
+  }
+}
+
 // C[m][n] = sum over K of A's row m and B's row n; a workgroup's tile is BM x BN, its WM x WN
 // waves take MB x NB fragments each. This is workgroup `id` of `workgroups`.
-template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN, bool GATED = false>
 __device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, unsigned workgroups,
                                             unsigned char* lds) {
   constexpr int BM = WM * MB * 16, BN = WN * NB * 16;
   using OpA = Operand<T, AOUT, BM, WM * WN>;
-  using OpB = Operand<T, BOUT, BN, WM * WN>;
+  using OpB = std::conditional_t<GATED, GatedOperand<T, BN, WM * WN, NB>, Operand<T, BOUT, BN, WM * WN>>;
   using frag = typename Fragment<T>::type;
   constexpr int kStage = OpA::kBytes + OpB::kBytes;
   constexpr int kK = OpA::kK;
@@ -401,7 +565,7 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, un
   const unsigned band = id / (kBand * a.tiles_n), in_band = id - band * kBand * a.tiles_n;
   const unsigned height = a.tiles_m - band * kBand < kBand ? a.tiles_m - band * kBand : kBand;
   const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % height) * BM;
-  const int64_t n0 = static_cast<int64_t>(in_band / height) * BN;
+  const int64_t n0 = static_cast<int64_t>(in_band / height) * (GATED ? BN / 2 : BN);
 
   const int64_t k0 = split * a.split_k;
   const int64_t k_count = k0 + a.split_k < a.k ? a.split_k : a.k - k0;
@@ -428,7 +592,8 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, un
   auto load = [&](int s) __attribute__((always_inline)) {
     const unsigned dst = lds_at + (s & 1) * kStage;
     if (s + 1 < stages) {
-      const u32x4 a_rows = opa.rows(kK), b_rows = opb.rows(kK);
+      const auto a_rows = opa.rows(kK);
+      const auto b_rows = opb.rows(kK);
 #pragma unroll
       for (int i = 0; i < OpA::kLoads; ++i) opa.load(a_rows, dst, wave, i);
 #pragma unroll
@@ -465,7 +630,8 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, un
       read(s, 1, i);
       __builtin_amdgcn_sched_barrier(0);
     }
-    u32x4 a_rows, b_rows;
+    u32x4 a_rows;
+    decltype(opb.rows(0)) b_rows;
     if constexpr (decltype(after)::value) {
       a_rows = opa.rows(kK);
       b_rows = opb.rows(kK);
@@ -516,16 +682,17 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, un
   // lane finishes 8 columns of a row and a store covers whole segments of rows.
   __syncthreads();
   constexpr int kPitch = NB * 16 + 4;  // floats; 4 more keep the 16 rows off each other's banks
-  constexpr int kLanes = NB * 2;       // lanes of a row
+  constexpr int kLanes = GATED ? NB : NB * 2;  // lanes of a row
   float* turn = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
   const int l = lane & 15, g = lane >> 4;
-  const int64_t n = n0 + wn * NB * 16 + lane % kLanes * 8;
+  const int64_t n = n0 + wn * kLanes * 8 + lane % kLanes * 8;
   const int count = n >= a.n ? 0 : (a.n - n < 8 ? static_cast<int>(a.n - n) : 8);
   float bias[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    bias[e] = a.bias != nullptr && e < count ? static_cast<float>(static_cast<const T*>(a.bias)[n + e])
-                                             : 0.f;
+    bias[e] = !GATED && a.bias != nullptr && e < count
+                  ? static_cast<float>(static_cast<const T*>(a.bias)[n + e])
+                  : 0.f;
 #pragma unroll
   for (int i = 0; i < MB; i += 2) {
 #pragma unroll
@@ -545,15 +712,26 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, unsigned id, un
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[q * 4 + e] = t[e];
       }
-      finish<T>(a, v, bias, split, m, n, count);
+      if constexpr (GATED) {
+        float u[8];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const f32x4 t = *reinterpret_cast<const f32x4*>(turn + r * kPitch + NB * 8 + lane % kLanes * 8 + q * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[q * 4 + e] = t[e];
+        }
+        finish_gated<T>(a, v, u, split, m, n, count);
+      } else {
+        finish<T>(a, v, bias, split, m, n, count);
+      }
     }
   }
 }
 
-template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinearArgs a) {
   extern __shared__ __align__(1024) unsigned char lds[];
-  linear_tile<T, AOUT, BOUT, MB, NB, WM, WN>(a, blockIdx.x, gridDim.x, lds);
+  linear_tile<T, AOUT, BOUT, MB, NB, WM, WN, GATED>(a, blockIdx.x, gridDim.x, lds);
 }
 
 // 32 columns' sums of a bias gradient from their partial sums, in a fixed order.
@@ -617,19 +795,22 @@ __device__ __forceinline__ typename Fragment<T>::type load_fragment(const T* row
   return __builtin_bit_cast(frag, r);
 }
 
+// Gated: 8 rows of Wg and the matching 8 of Wu.
 constexpr int kFewWaves = 8;
-template <typename T, int MF>
+template <typename T, int MF, bool GATED>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_few_rows(LinearArgs a) {
   constexpr int kStep = 64 / sizeof(T);  // K values of a fragment over its four lane groups
   constexpr int kUnroll = MF == 4 ? 2 : 4;
   using frag = typename Fragment<T>::type;
   __shared__ float sums[kFewWaves][16][MF * 16 + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (GATED ? 8 : 16);
   const T* x = static_cast<const T*>(a.a);
   const T* w = static_cast<const T*>(a.b);
   // Rows past the end read the last one; their sums are not used.
-  const T* w_row = w + std::min<int64_t>(n0 + l, a.n - 1) * a.ldb;
+  const T* w_row = w + (GATED ? std::min<int64_t>(n0 + l % 8, a.n - 1) + (l < 8 ? 0 : a.n)
+                              : std::min<int64_t>(n0 + l, a.n - 1)) *
+                           a.ldb;
   const T* x_row[MF];
 #pragma unroll
   for (int f = 0; f < MF; ++f) x_row[f] = x + std::min<int64_t>(f * 16 + l, a.m - 1) * a.lda;
@@ -667,6 +848,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_rows(LinearArgs a) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) sums[wave][g * 4 + e][f * 16 + l] = acc[f][e];
   __syncthreads();
+  if constexpr (GATED) {
+    const int m = threadIdx.x;
+    if (m >= MF * 16 || m >= a.m) return;
+    const int count = a.n - n0 < 8 ? static_cast<int>(a.n - n0) : 8;
+    float v[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = u[e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < kFewWaves; ++q) {
+        v[e] += sums[q][e][m];
+        u[e] += sums[q][8 + e][m];
+      }
+    }
+    finish_gated<T>(a, v, u, 0, m, n0, count);
+    return;
+  }
   for (int i = threadIdx.x; i < MF * 16 * 2; i += 64 * kFewWaves) {
     const int m = i / 2, c = i % 2 * 8;
     const int64_t n = n0 + c;
@@ -733,6 +931,39 @@ __global__ __launch_bounds__(256) void linear_join(LinearJoin one, LinearJoin tw
       }
     }
     finish<T>(a, v, bias, 0, m, n, count);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gated_join(LinearArgs a, const float* partial, int64_t splits) {
+  const int64_t parts = (a.n + 7) / 8, total = a.m * parts, step = a.m * 2 * a.n;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t m = id / parts, n = id % parts * 8;
+    const int count = a.n - n < 8 ? static_cast<int>(a.n - n) : 8;
+    float v[2][8] = {};
+    const float* p = partial + m * 2 * a.n + n;
+#pragma unroll 2
+    for (int64_t s = 0; s < splits; ++s, p += step) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float* q = p + half * a.n;
+        if (count == 8) {
+          const Run<float, 4> lo = load_run<4>(q), hi = load_run<4>(q + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[half][e] += lo.v[e];
+            v[half][e + 4] += hi.v[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < count) v[half][e] += q[e];
+          end_of_part();
+        }
+      }
+    }
+    finish_gated<T>(a, v[0], v[1], 0, m, n, count);
   }
 }
 
@@ -840,6 +1071,102 @@ __global__ __launch_bounds__(256) void linear_grad(LinearGradArgs a) {
   }
 }
 
+// The gated layer's dz = [dy u act'(g), dy act(g)] from the kept factors, and both halves' column sums over
+// each workgroup's rows; otherwise as linear_grad, 8 columns of dy a thread. Rounded to the element type for
+// the products, as there.
+template <typename T, int TPR>
+__global__ __launch_bounds__(256) void gated_grad(LinearGradArgs a) {
+  constexpr int kColumns = TPR * 8, kRows = 256 / TPR;
+  __shared__ float sums[kRows][kColumns];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kColumns + lane * 8;
+  const int count = n >= a.columns ? 0 : (a.columns - n < 8 ? static_cast<int>(a.columns - n) : 8);
+  const T* dy = static_cast<const T*>(a.grad_output);
+  T* dz = static_cast<T*>(a.grad_pre);
+  const int64_t both = 2 * a.columns, tail = a.pitch - both;  // zeros follow a row
+  float sum[2][8] = {};
+  const int64_t first = a.rows * blockIdx.y / gridDim.y, last = a.rows * (blockIdx.y + 1) / gridDim.y;
+  if (count > 0) {
+#pragma unroll 2
+    for (int64_t m = first + group; m < last; m += kRows) {
+      Run<T, 8> d;
+      float f[2][8];
+      const T* from = dy + m * a.grad_stride + n;
+      if (count == 8) {
+        d = load_run<8>(from);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int64_t at = m * both + half * a.columns + n;
+          if constexpr (sizeof(T) == 2) {
+            const auto high = load_run<8>(static_cast<const uint16_t*>(a.slope) + at);
+            const auto low = load_run<8>(static_cast<const uint8_t*>(a.slope) + a.rows * both * 2 + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[half][e] = factor_of(high.v[e], low.v[e]);
+          } else {
+            const auto whole = load_run<8>(static_cast<const float*>(a.slope) + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[half][e] = whole.v[e];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d.v[e] = e < count ? from[e] : static_cast<T>(0.f);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int64_t at = m * both + half * a.columns + n + e;
+            f[half][e] = 0.f;
+            if (e >= count) continue;
+            if constexpr (sizeof(T) == 2)
+              f[half][e] = factor_of(static_cast<const uint16_t*>(a.slope)[at],
+                                     (static_cast<const uint8_t*>(a.slope) + a.rows * both * 2)[at]);
+            else
+              f[half][e] = static_cast<const float*>(a.slope)[at];
+          }
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        Run<T, 8> z;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = static_cast<float>(d.v[e]) * f[half][e];
+          z.v[e] = static_cast<T>(v);
+          sum[half][e] += v;
+        }
+        if (dz == nullptr) continue;
+        T* o = dz + m * a.pitch + half * a.columns + n;
+        if (count == 8) {
+          store_run<8>(o, z);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < count) o[e] = z.v[e];
+          end_of_part();
+        }
+      }
+      if (dz != nullptr && n + 8 >= a.columns)
+        for (int64_t e = 0; e < tail; ++e) dz[m * a.pitch + both + e] = static_cast<T>(0.f);
+    }
+  }
+  if (a.partial == nullptr) return;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[group][lane * 8 + e] = sum[half][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < kColumns; c += 256) {
+      const int64_t column = static_cast<int64_t>(blockIdx.x) * kColumns + c;
+      if (column >= a.columns) break;
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) s += sums[r][c];
+      a.partial[blockIdx.y * both + half * a.columns + column] = s;
+    }
+  }
+}
+
 // More than 64 KB of LDS has to be asked for, once per device and kernel (`asked` is the kernel's).
 template <typename Kernel>
 hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
@@ -858,10 +1185,10 @@ hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
 template <int MB, int NB, int WM, int WN>
 constexpr int kTileBytes = 2 * (WM * MB + WN * NB) * 16 * 128;
 
-template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN>
+template <typename T, bool AOUT, bool BOUT, int MB, int NB, int WM, int WN, bool GATED>
 hipError_t launch_tiles(const LinearArgs& a, int64_t splits, hipStream_t stream) {
   constexpr int kBytes = kTileBytes<MB, NB, WM, WN>;
-  const auto kernel = linear_kernel<T, AOUT, BOUT, MB, NB, WM, WN>;
+  const auto kernel = linear_kernel<T, AOUT, BOUT, MB, NB, WM, WN, GATED>;
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
   if (err != hipSuccess) return err;
@@ -909,12 +1236,37 @@ hipError_t launch_join(const LinearJoin& one, const LinearJoin& two, hipStream_t
   return hipGetLastError();
 }
 
-template <typename T, bool AOUT, bool BOUT>
+template <typename T, bool AOUT, bool BOUT, bool GATED = false>
 hipError_t launch_tiles_of(const LinearArgs& t, const LinearPlan& p, hipStream_t stream) {
   if constexpr (sizeof(T) == 2)
-    if (p.tile == 256) return launch_tiles<T, AOUT, BOUT, 8, 4, 2, 4>(t, p.splits, stream);
-  return p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2>(t, p.splits, stream)
-                       : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2>(t, p.splits, stream);
+    if (p.tile == 256) return launch_tiles<T, AOUT, BOUT, 8, 4, 2, 4, GATED>(t, p.splits, stream);
+  return p.tile == 128 ? launch_tiles<T, AOUT, BOUT, 4, 4, 2, 2, GATED>(t, p.splits, stream)
+                       : launch_tiles<T, AOUT, BOUT, 2, 2, 2, 2, GATED>(t, p.splits, stream);
+}
+
+template <typename T, bool GATED>
+hipError_t launch_few_rows(const LinearArgs& a, unsigned workgroups, hipStream_t stream) {
+  const dim3 grid(workgroups), block(64 * kFewWaves);
+  if (a.m <= 16)
+    hipLaunchKernelGGL((linear_few_rows<T, 1, GATED>), grid, block, 0, stream, a);
+  else if (a.m <= 32)
+    hipLaunchKernelGGL((linear_few_rows<T, 2, GATED>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((linear_few_rows<T, 4, GATED>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_gated_typed(const LinearArgs& a, const LinearPlan& p, float* partial, hipStream_t stream) {
+  if (p.few_rows) return launch_few_rows<T, true>(a, static_cast<unsigned>((a.n + 7) / 8), stream);
+  LinearArgs t = planned(a, p, partial);
+  t.tiles_n = static_cast<unsigned>((a.n + p.tile / 2 - 1) / (p.tile / 2));
+  const hipError_t err = launch_tiles_of<T, false, false, true>(t, p, stream);
+  if (err != hipSuccess || p.splits == 1) return err;
+  const int64_t work = a.m * ((a.n + 7) / 8);
+  hipLaunchKernelGGL(gated_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>((work + 255) / 256, 8192))),
+                     dim3(256), 0, stream, a, partial, p.splits);
+  return hipGetLastError();
 }
 
 template <typename T, bool AOUT, bool BOUT>
@@ -922,14 +1274,7 @@ hipError_t launch_product_typed(const LinearArgs& a, const LinearPlan& p, float*
                                 hipStream_t stream) {
   if constexpr (!AOUT && !BOUT) {
     if (p.few_rows) {
-      const dim3 grid(static_cast<unsigned>((a.n + 15) / 16)), block(64 * kFewWaves);
-      if (a.m <= 16)
-        hipLaunchKernelGGL((linear_few_rows<T, 1>), grid, block, 0, stream, a);
-      else if (a.m <= 32)
-        hipLaunchKernelGGL((linear_few_rows<T, 2>), grid, block, 0, stream, a);
-      else
-        hipLaunchKernelGGL((linear_few_rows<T, 4>), grid, block, 0, stream, a);
-      return hipGetLastError();
+      return launch_few_rows<T, false>(a, static_cast<unsigned>((a.n + 15) / 16), stream);
     }
   }
   const hipError_t err = launch_tiles_of<T, AOUT, BOUT>(planned(a, p, partial), p, stream);
@@ -1125,6 +1470,20 @@ hipError_t launch_linear_product(convnd_hip_dtype dtype, const LinearArgs& a, Li
   }
 }
 
+hipError_t launch_gated_product(convnd_hip_dtype dtype, const LinearArgs& a, const LinearPlan& p, float* partial,
+                                hipStream_t stream) {
+  switch (dtype) {
+    case CONVND_HIP_FLOAT32:
+      return launch_gated_typed<float>(a, p, partial, stream);
+    case CONVND_HIP_FLOAT16:
+      return launch_gated_typed<_Float16>(a, p, partial, stream);
+    case CONVND_HIP_BFLOAT16:
+      return launch_gated_typed<__bf16>(a, p, partial, stream);
+    default:
+      return hipErrorInvalidValue;
+  }
+}
+
 hipError_t launch_linear_gradients(convnd_hip_dtype dtype, const LinearArgs& x,
                                    const LinearPlan& xp, float* x_partial, const LinearArgs& w,
                                    const LinearPlan& wp, float* w_partial, const LinearSums& sums,
@@ -1165,6 +1524,13 @@ void launch_grad(const LinearGradArgs& a, int64_t parts, hipStream_t stream) {
   const int threads = grad_threads(a.columns);
   const dim3 grid(static_cast<unsigned>((a.columns + threads * 8 - 1) / (threads * 8)),
                   static_cast<unsigned>(parts));
+  if (a.gated) {
+    if (threads == 64)
+      hipLaunchKernelGGL((gated_grad<T, 64>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((gated_grad<T, 256>), grid, dim3(256), 0, stream, a);
+    return;
+  }
   if (threads == 64)
     hipLaunchKernelGGL((linear_grad<T, 64>), grid, dim3(256), 0, stream, a);
   else

@@ -202,7 +202,7 @@ struct LinearForward {
   float* partial;
 };
 LinearForward lay_out(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p, const void* input,
-                      const void* weight, Parts* ws) {
+                      const void* weight, Parts* ws) {  // gated: of 2 outputs
   const int size = size_of(dtype);
   LinearForward f{};
   f.plan = plan_product(dtype, LinearProduct::kForward, p.rows, p.outputs, p.inputs);
@@ -227,13 +227,14 @@ struct LinearBackward {
 };
 LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p,
                                 const void* grad_output, const void* input, const void* weight,
-                                bool need_input, bool need_weight, bool need_bias, Parts* ws) {
+                                bool need_input, bool need_weight, bool need_bias, Parts* ws,
+                                bool gated = false) {  // gated: of 2 outputs
   const int size = size_of(dtype);
   LinearBackward b{};
   b.dz = {grad_output, p.grad_stride, false};
   const bool products = need_input || need_weight;
   if (products) {
-    if (p.activation != CONVND_HIP_ACT_NONE) {
+    if (gated || p.activation != CONVND_HIP_ACT_NONE) {
       const int64_t pitch = padded_columns(p.outputs, size);
       b.dz = {ws->take(p.rows * pitch * size), pitch, true};
     } else {
@@ -243,7 +244,7 @@ LinearBackward lay_out_backward(convnd_hip_dtype dtype, const convnd_hip_linear_
   b.make_dz = b.dz.copy;
   if (need_weight) b.x = padded(input, p.input_stride, p.rows, p.inputs, size, ws);
   if (need_input) b.w = padded(weight, p.inputs, p.outputs, p.inputs, size, ws);
-  b.parts = linear_grad_parts(p.rows, p.outputs);
+  b.parts = linear_grad_parts(p.rows, gated ? p.outputs / 2 : p.outputs);
   if (need_bias) b.sums = static_cast<float*>(ws->take(b.parts * p.outputs * sizeof(float)));
   if (need_input && need_weight)
     plan_gradients(dtype, p.rows, p.inputs, p.outputs, &b.input_plan, &b.weight_plan);
@@ -401,6 +402,82 @@ DeltaLayout lay_out_delta_backward(DeltaArgs* a, int size, const void* grad_outp
   a->grad_states = ws->take(saved_states(*a) * size);
   a->grad_updates = ws->take(saved_updates(*a, size) * size);
   return l;
+}
+
+// The products of a backward from its dz.
+int run_gradients(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p, const LinearBackward& b,
+                  const void* input, const void* weight, void* grad_input, void* grad_weight,
+                  void* grad_bias, hipStream_t on) {
+  int st = CONVND_HIP_SUCCESS;
+  const bool both = grad_input != nullptr && grad_weight != nullptr;
+  LinearArgs x{}, w{};
+  if (grad_input != nullptr) {
+    st = fill_padded(dtype, b.w, weight, p.inputs, p.outputs, p.inputs, on);
+    if (st != CONVND_HIP_SUCCESS) return st;
+    x.a = b.dz.data;
+    x.lda = b.dz.stride;
+    x.b = b.w.data;
+    x.ldb = b.w.stride;
+    x.m = p.rows;
+    x.n = p.inputs;
+    x.k = p.outputs;
+    x.output = grad_input;
+  }
+  if (grad_weight != nullptr) {
+    st = fill_padded(dtype, b.x, input, p.input_stride, p.rows, p.inputs, on);
+    if (st != CONVND_HIP_SUCCESS) return st;
+    w.a = b.dz.data;
+    w.lda = b.dz.stride;
+    w.b = b.x.data;
+    w.ldb = b.x.stride;
+    w.m = p.outputs;
+    w.n = p.inputs;
+    w.k = p.rows;
+    w.output = grad_weight;
+  }
+  if (both)
+    return hip_check(launch_linear_gradients(dtype, x, b.input_plan, b.input_partial, w,
+                                             b.weight_plan, b.weight_partial,
+                                             {b.sums, b.parts, p.outputs, grad_bias}, on),
+                     "linear gradients launch");
+  if (grad_input != nullptr)
+    return hip_check(launch_linear_product(dtype, x, LinearProduct::kGradInput, b.input_plan,
+                                           b.input_partial, on),
+                     "linear input gradient launch");
+  if (grad_weight != nullptr)
+    return hip_check(launch_linear_product(dtype, w, LinearProduct::kGradWeight, b.weight_plan,
+                                           b.weight_partial, on),
+                     "linear weight gradient launch");
+  return st;
+}
+
+// Zeros where there are no rows.
+int fill_no_rows(convnd_hip_dtype dtype, const convnd_hip_linear_problem& p, void* grad_weight,
+                 void* grad_bias, hipStream_t on) {
+  int st = CONVND_HIP_SUCCESS;
+  if (grad_weight != nullptr)
+    st = hip_check(launch_fill_zero(grad_weight, p.outputs * p.inputs * size_of(dtype), on),
+                   "linear backward launch");
+  if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr)
+    st = hip_check(launch_fill_zero(grad_bias, p.outputs * size_of(dtype), on),
+                   "linear backward launch");
+  return st;
+}
+
+// The gated layer as a linear one of both halves' outputs.
+int check_gated(convnd_hip_dtype dtype, const convnd_hip_linear_problem* p, convnd_hip_linear_problem* both) {
+  if (size_of(dtype) == 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, std::string("gated_linear ") + kTypes);
+  if (p == nullptr || p->outputs <= 0 || p->outputs >= kMaxLinear / 2)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_linear needs 1 to 2^20 - 1 outputs");
+  if (p->activation < CONVND_HIP_ACT_RELU || p->activation > CONVND_HIP_ACT_SILU)
+    return fail(CONVND_HIP_INVALID_ARGUMENT,
+                "gated_linear activation must be 'silu', 'relu', 'gelu' or 'gelu_tanh'");
+  *both = *p;
+  both->outputs = 2 * p->outputs;
+  both->residual_stride = 0;
+  both->activation = CONVND_HIP_ACT_NONE;
+  return check_linear(dtype, both);
 }
 
 // A plan's description as JSON; numbers only beside the kernel's name.
@@ -653,15 +730,7 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
   if (st != CONVND_HIP_SUCCESS) return st;
   const convnd_hip_linear_problem& p = *problem;
   const auto on = static_cast<hipStream_t>(stream);
-  if (p.rows == 0) {
-    if (grad_weight != nullptr)
-      st = hip_check(launch_fill_zero(grad_weight, p.outputs * p.inputs * size_of(dtype), on),
-                     "linear backward launch");
-    if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr)
-      st = hip_check(launch_fill_zero(grad_bias, p.outputs * size_of(dtype), on),
-                     "linear backward launch");
-    return st;
-  }
+  if (p.rows == 0) return fill_no_rows(dtype, p, grad_weight, grad_bias, on);
   const bool activated = p.activation != CONVND_HIP_ACT_NONE;
   if (p.grad_stride < p.outputs)
     return fail(CONVND_HIP_INVALID_ARGUMENT, "linear_act needs rows at least their length apart");
@@ -695,45 +764,7 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
                      "linear bias gradient launch");
     if (st != CONVND_HIP_SUCCESS) return st;
   }
-  LinearArgs x{}, w{};
-  if (grad_input != nullptr) {
-    st = fill_padded(dtype, b.w, weight, p.inputs, p.outputs, p.inputs, on);
-    if (st != CONVND_HIP_SUCCESS) return st;
-    x.a = b.dz.data;
-    x.lda = b.dz.stride;
-    x.b = b.w.data;
-    x.ldb = b.w.stride;
-    x.m = p.rows;
-    x.n = p.inputs;
-    x.k = p.outputs;
-    x.output = grad_input;
-  }
-  if (grad_weight != nullptr) {
-    st = fill_padded(dtype, b.x, input, p.input_stride, p.rows, p.inputs, on);
-    if (st != CONVND_HIP_SUCCESS) return st;
-    w.a = b.dz.data;
-    w.lda = b.dz.stride;
-    w.b = b.x.data;
-    w.ldb = b.x.stride;
-    w.m = p.outputs;
-    w.n = p.inputs;
-    w.k = p.rows;
-    w.output = grad_weight;
-  }
-  if (both)
-    return hip_check(launch_linear_gradients(dtype, x, b.input_plan, b.input_partial, w,
-                                             b.weight_plan, b.weight_partial,
-                                             {b.sums, b.parts, p.outputs, grad_bias}, on),
-                     "linear gradients launch");
-  if (grad_input != nullptr)
-    return hip_check(launch_linear_product(dtype, x, LinearProduct::kGradInput, b.input_plan,
-                                           b.input_partial, on),
-                     "linear input gradient launch");
-  if (grad_weight != nullptr)
-    return hip_check(launch_linear_product(dtype, w, LinearProduct::kGradWeight, b.weight_plan,
-                                           b.weight_partial, on),
-                     "linear weight gradient launch");
-  return st;
+  return run_gradients(dtype, p, b, input, weight, grad_input, grad_weight, grad_bias, on);
 }
 
 int64_t convnd_hip_delta_saved(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem) {
@@ -842,6 +873,112 @@ int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_pro
     if (st != CONVND_HIP_SUCCESS) return st;
   }
   return hip_check(launch_delta_backward(dtype, a, on), "delta rule backward launch");
+}
+
+size_t convnd_hip_gated_linear_workspace_size(convnd_hip_dtype dtype,
+                                              const convnd_hip_linear_problem* problem,
+                                              const void* input, const void* weight) {
+  convnd_hip_linear_problem both;
+  if (check_gated(dtype, problem, &both) != CONVND_HIP_SUCCESS || both.rows == 0) return 0;
+  Parts ws{nullptr};
+  lay_out(dtype, both, input, weight, &ws);
+  return ws.used;
+}
+
+size_t convnd_hip_gated_linear_kept_size(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem) {
+  convnd_hip_linear_problem both;
+  if (check_gated(dtype, problem, &both) != CONVND_HIP_SUCCESS) return 0;
+  return static_cast<size_t>(both.rows) * both.outputs * (size_of(dtype) == 4 ? 4 : 3);
+}
+
+int convnd_hip_gated_linear(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                            const void* input, const void* weight, const void* bias, void* output,
+                            void* kept, void* workspace, size_t workspace_size, void* stream) {
+  convnd_hip_linear_problem both;
+  int st = check_gated(dtype, problem, &both);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const convnd_hip_linear_problem& p = *problem;
+  if (p.rows == 0) return CONVND_HIP_SUCCESS;
+  if (input == nullptr || weight == nullptr || output == nullptr)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "input, weight and output must not be null");
+  Parts ws{static_cast<char*>(workspace)};
+  const LinearForward f = lay_out(dtype, both, input, weight, &ws);
+  st = check_plan(f.plan);
+  if (st == CONVND_HIP_SUCCESS) st = check_parts(ws, workspace_size, "gated_linear");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const auto on = static_cast<hipStream_t>(stream);
+  st = fill_padded(dtype, f.x, input, p.input_stride, p.rows, p.inputs, on);
+  if (st == CONVND_HIP_SUCCESS)
+    st = fill_padded(dtype, f.w, weight, p.inputs, both.outputs, p.inputs, on);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  LinearArgs a{};
+  a.a = f.x.data;
+  a.b = f.w.data;
+  a.lda = f.x.stride;
+  a.ldb = f.w.stride;
+  a.m = p.rows;
+  a.n = p.outputs;
+  a.k = p.inputs;
+  a.bias = bias;
+  a.output = output;
+  a.slope = kept;
+  a.activation = p.activation;
+  return hip_check(launch_gated_product(dtype, a, f.plan, f.partial, on), "gated linear launch");
+}
+
+size_t convnd_hip_gated_linear_backward_workspace_size(convnd_hip_dtype dtype,
+                                                       const convnd_hip_linear_problem* problem,
+                                                       const void* input, const void* weight,
+                                                       int need_grad_input, int need_grad_weight,
+                                                       int need_grad_bias) {
+  convnd_hip_linear_problem both;
+  if (check_gated(dtype, problem, &both) != CONVND_HIP_SUCCESS || both.rows == 0) return 0;
+  Parts ws{nullptr};
+  lay_out_backward(dtype, both, nullptr, input, weight, need_grad_input != 0, need_grad_weight != 0,
+                   need_grad_bias != 0, &ws, true);
+  return ws.used;
+}
+
+int convnd_hip_gated_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_problem* problem,
+                                     const void* grad_output, const void* input, const void* weight,
+                                     const void* kept, void* grad_input, void* grad_weight,
+                                     void* grad_bias, void* workspace, size_t workspace_size,
+                                     void* stream) {
+  convnd_hip_linear_problem both;
+  int st = check_gated(dtype, problem, &both);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const auto on = static_cast<hipStream_t>(stream);
+  if (both.rows == 0) return fill_no_rows(dtype, both, grad_weight, grad_bias, on);
+  if (problem->grad_stride < problem->outputs)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_linear needs rows at least their length apart");
+  if (grad_input == nullptr && grad_weight == nullptr && grad_bias == nullptr) return CONVND_HIP_SUCCESS;
+  if (grad_output == nullptr || kept == nullptr || (grad_input != nullptr && weight == nullptr) ||
+      (grad_weight != nullptr && input == nullptr))
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "grad_output, input, weight and kept must not be null");
+  Parts ws{static_cast<char*>(workspace)};
+  const LinearBackward b =
+      lay_out_backward(dtype, both, nullptr, input, weight, grad_input != nullptr, grad_weight != nullptr,
+                       grad_bias != nullptr, &ws, true);
+  if (grad_input != nullptr) st = check_plan(b.input_plan);
+  if (st == CONVND_HIP_SUCCESS && grad_weight != nullptr) st = check_plan(b.weight_plan);
+  if (st == CONVND_HIP_SUCCESS) st = check_parts(ws, workspace_size, "gated_linear backward");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  LinearGradArgs g{};
+  g.grad_output = grad_output;
+  g.slope = kept;
+  g.grad_pre = b.make_dz ? const_cast<void*>(b.dz.data) : nullptr;
+  g.partial = b.sums;
+  g.rows = both.rows;
+  g.columns = problem->outputs;
+  g.grad_stride = problem->grad_stride;
+  g.pitch = b.make_dz ? b.dz.stride : both.outputs;
+  g.gated = true;
+  st = hip_check(launch_linear_grad(dtype, g, b.parts, on), "gated linear gradient launch");
+  if (st == CONVND_HIP_SUCCESS && grad_bias != nullptr && (grad_input == nullptr || grad_weight == nullptr))
+    st = hip_check(launch_sum_rows(dtype, b.sums, b.parts, both.outputs, both.outputs, grad_bias, nullptr, on),
+                   "gated linear bias gradient launch");
+  if (st != CONVND_HIP_SUCCESS) return st;
+  return run_gradients(dtype, both, b, input, weight, grad_input, grad_weight, grad_bias, on);
 }
 
 int convnd_hip_linear_plan_describe(convnd_hip_dtype dtype,

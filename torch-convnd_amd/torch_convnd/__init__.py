@@ -24,7 +24,7 @@ from .modules import (
     PartialSequential,
 )
 from .partial import PartialConvOutput, partial_conv_nd
-from .sequence import gated_delta_rule, gated_recurrence, layer_norm, linear_act
+from .sequence import gated_delta_rule, gated_linear, gated_recurrence, layer_norm, linear_act
 from .sequence_modules import GatedConvBlock, LayerNorm, LinearAct
 
 ensure_native_definitions()
@@ -48,6 +48,7 @@ __all__ = [
     "PartialSequential",
     "conv_nd",
     "gated_delta_rule",
+    "gated_linear",
     "gated_recurrence",
     "layer_norm",
     "linear_act",

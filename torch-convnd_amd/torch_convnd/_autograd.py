@@ -227,6 +227,18 @@ def _fake_linear_act_backward(grad_output, input, weight, slope, activation, out
     return dx, dw, weight.new_empty(weight.shape[0]) if output_mask[2] else None
 
 
+def _fake_gated_linear(input, weight, bias, activation, keep):
+    outputs = weight.shape[0] // 2
+    output = input.new_empty((*input.shape[:-1], outputs))
+    # convnd_hip_gated_linear_kept_size
+    kept = 2 * output.numel() * (4 if input.element_size() == 4 else 3) if keep else 0
+    return output, input.new_empty((kept,), dtype=torch.uint8)
+
+
+def _fake_gated_linear_backward(grad_output, input, weight, kept, activation, output_mask):
+    return _fake_linear_act_backward(grad_output, input, weight, kept, activation, output_mask)
+
+
 def _fake_recurrence(input, gate, initial_state, lengths, keep_carries):
     batch, tokens, channels = input.shape
     tiles = (tokens + RECURRENCE_TILE - 1) // RECURRENCE_TILE
@@ -328,6 +340,26 @@ def _linear_act_backward(ctx, grad_output, _):
     return (*grads, grad_output if ctx.residual else None, None, None)
 
 
+def _setup_gated_linear(ctx, inputs, output):
+    input, weight, bias, ctx.activation, ctx.kept = inputs
+    ctx.bias = bias is not None
+    ctx.save_for_backward(input, weight, output[1], None if ctx.kept else bias)
+    _keep_apart(ctx, output[1])
+
+
+def _gated_linear_backward(ctx, grad_output, _):
+    _check_once("gated_linear")
+    if grad_output is None:
+        return (None,) * 5
+    input, weight, kept, bias = ctx.saved_tensors
+    ops = torch.ops.torch_convnd
+    if not ctx.kept:
+        kept = ops.gated_linear.default(input, weight, bias, ctx.activation, True)[1]
+    mask = [*ctx.needs_input_grad[:2], ctx.bias and ctx.needs_input_grad[2]]
+    grads = ops.gated_linear_backward.default(grad_output, input, weight, kept, ctx.activation, mask)
+    return (*grads, None, None)
+
+
 def _setup_recurrence(ctx, inputs, output):
     input, gate, initial_state, lengths, ctx.kept = inputs
     ctx.first = initial_state is not None
@@ -379,6 +411,7 @@ _SEQUENCE_DERIVATIVES = {
     "layer_norm": (_layer_norm_backward, _setup_layer_norm),
     "linear_act": (_linear_act_backward, _setup_linear_act),
     "gated_recurrence": (_recurrence_backward, _setup_recurrence),
+    "gated_linear": (_gated_linear_backward, _setup_gated_linear),
     "gated_delta_rule": (_delta_backward, _setup_delta),
 }
 
@@ -408,6 +441,8 @@ def register_training() -> None:
     torch.library.register_fake("torch_convnd::linear_act_backward")(_fake_linear_act_backward)
     torch.library.register_fake("torch_convnd::gated_recurrence")(_fake_recurrence)
     torch.library.register_fake("torch_convnd::gated_recurrence_backward")(_fake_recurrence_backward)
+    torch.library.register_fake("torch_convnd::gated_linear")(_fake_gated_linear)
+    torch.library.register_fake("torch_convnd::gated_linear_backward")(_fake_gated_linear_backward)
     torch.library.register_fake("torch_convnd::gated_delta_rule")(_fake_delta)
     torch.library.register_fake("torch_convnd::gated_delta_rule_backward")(_fake_delta_backward)
     torch.library.register_autograd(

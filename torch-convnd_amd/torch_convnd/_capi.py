@@ -46,6 +46,11 @@ EXPORTED_SYMBOLS = (
     "convnd_hip_recurrence",
     "convnd_hip_recurrence_backward",
     "convnd_hip_recurrence_plan_describe",
+    "convnd_hip_gated_linear_workspace_size",
+    "convnd_hip_gated_linear_kept_size",
+    "convnd_hip_gated_linear",
+    "convnd_hip_gated_linear_backward_workspace_size",
+    "convnd_hip_gated_linear_backward",
     "convnd_hip_delta_saved",
     "convnd_hip_delta_workspace_size",
     "convnd_hip_delta",
@@ -191,6 +196,20 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     ]
     library.convnd_hip_linear_backward.restype = ctypes.c_int
     library.convnd_hip_linear_backward.argtypes = [
+        ctypes.c_int, L, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp
+    ]
+    library.convnd_hip_gated_linear_workspace_size.restype = sz
+    library.convnd_hip_gated_linear_workspace_size.argtypes = [ctypes.c_int, L, vp, vp]
+    library.convnd_hip_gated_linear_kept_size.restype = sz
+    library.convnd_hip_gated_linear_kept_size.argtypes = [ctypes.c_int, L]
+    library.convnd_hip_gated_linear.restype = ctypes.c_int
+    library.convnd_hip_gated_linear.argtypes = [ctypes.c_int, L, vp, vp, vp, vp, vp, vp, sz, vp]
+    library.convnd_hip_gated_linear_backward_workspace_size.restype = sz
+    library.convnd_hip_gated_linear_backward_workspace_size.argtypes = [
+        ctypes.c_int, L, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_int
+    ]
+    library.convnd_hip_gated_linear_backward.restype = ctypes.c_int
+    library.convnd_hip_gated_linear_backward.argtypes = [
         ctypes.c_int, L, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp
     ]
     library.convnd_hip_recurrence_carries.restype = i64

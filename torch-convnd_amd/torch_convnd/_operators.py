@@ -85,7 +85,7 @@ def _lazy(name, position=0):
     return load_and_call
 
 
-# Sequence operators (layer norm, linear layer, gated recurrence, delta rule); no reference counterpart. The second
+# Sequence operators (layer norm, linear layers, gated recurrence, delta rule); no reference counterpart. The second
 # results of the forwards are what their backward operators read, kept only on request.
 _SEQUENCE_SCHEMAS = (
     "layer_norm(Tensor input, Tensor? weight, Tensor? bias, float eps, bool keep_statistics) "
@@ -100,6 +100,9 @@ _SEQUENCE_SCHEMAS = (
     "bool keep_carries) -> (Tensor, Tensor, Tensor)",
     "gated_recurrence_backward(Tensor grad_output, Tensor? grad_last, Tensor input, Tensor gate, "
     "Tensor? lengths, Tensor carries, bool need_initial_state) -> (Tensor, Tensor, Tensor?)",
+    "gated_linear(Tensor input, Tensor weight, Tensor? bias, str activation, bool keep) -> (Tensor, Tensor)",
+    "gated_linear_backward(Tensor grad_output, Tensor input, Tensor weight, Tensor kept, str activation, "
+    "bool[3] output_mask) -> (Tensor?, Tensor?, Tensor?)",
     "gated_delta_rule(Tensor query, Tensor key, Tensor value, Tensor decay, Tensor beta, "
     "Tensor? initial_state, Tensor? lengths, float scale, bool normalize, bool keep) "
     "-> (Tensor, Tensor, Tensor)",

@@ -1,5 +1,5 @@
 """Operators of token sequences around the convolution: layer norm, the linear layer with its
-activation and residual, the gated linear recurrence and the gated delta rule, over activations of
+activation and residual, the gated linear layer, the gated linear recurrence and the gated delta rule, over activations of
 [..., channels]. No counterpart in the reference.
 
 ``backend`` as for ``conv_nd``: ``auto`` runs the gfx950 kernels for ROCm GPU tensors (float16,
@@ -154,6 +154,57 @@ def _portable_linear(input, weight, bias, residual, activation):
         if residual is not None:
             output = output + residual.to(wide)
     return output.to(input.dtype)
+
+
+_GATED_ACTIVATIONS = ("silu", "relu", "gelu", "gelu_tanh")
+
+
+def gated_linear(
+    input: Tensor,
+    weight: Tensor,
+    bias: Tensor | None = None,
+    *,
+    activation: str = "silu",
+    backend: str = "auto",
+) -> Tensor:
+    """``act(input @ Wg.T + bg) * (input @ Wu.T + bu)`` over the last dimension of ``input`` [..., inputs]:
+    the two projections of a gated feed-forward block, its activation and the product.
+
+    ``weight`` [2 * outputs, inputs] is Wg above Wu, ``bias`` [2 * outputs] bg before bu, in the input's
+    dtype; ``activation`` is "silu", "relu", "gelu" or "gelu_tanh". On the gfx950 path all of it is one
+    rounding of the float32 sums; a training step also keeps two factors an output (in 24 bits beside
+    16-bit types, else float32), and its backward rounds the gradients before the product to the element
+    type. ``input`` may be a slice of wider rows. Under autocast the operands are cast to its dtype.
+    """
+    if activation not in _GATED_ACTIVATIONS:
+        raise ValueError(f"Invalid activation {activation!r}; expected 'silu', 'relu', 'gelu' or 'gelu_tanh'")
+    if is_autocast_enabled(input.device.type):
+        dtype = autocast_dtype(input.device.type)
+        cast = lambda t: t.to(dtype) if t is not None and t.dtype in _NATIVE_DTYPES else t  # noqa: E731
+        input, weight, bias = cast(input), cast(weight), cast(bias)
+    if _use_native(input, backend, "gated_linear"):
+        keep = _recording(input, weight, bias)
+        return torch.ops.torch_convnd.gated_linear.default(input, weight, bias, activation, keep)[0]
+    if (
+        weight.dim() != 2
+        or input.dim() == 0
+        or input.shape[-1] != weight.shape[1]
+        or weight.numel() == 0
+        or weight.shape[0] % 2
+    ):
+        raise RuntimeError("gated_linear expects an input of [..., inputs] and a weight of [2 * outputs, inputs]")
+    if weight.device != input.device or weight.dtype != input.dtype:
+        raise RuntimeError("input and weight must have the same device and dtype")
+    if bias is not None and (
+        bias.shape != weight.shape[:1] or bias.device != input.device or bias.dtype != input.dtype
+    ):
+        raise RuntimeError("bias must match the weight's rows, device and dtype")
+    wide = torch.float64 if input.dtype == torch.float64 else torch.float32
+    with autocast_disabled(input.device.type):
+        both = F.linear(input.to(wide), weight.to(wide), None if bias is None else bias.to(wide))
+        gate, up = both.chunk(2, dim=-1)
+        gate = F.silu(gate) if activation == "silu" else _apply_activation(gate, activation)
+        return (gate * up).to(input.dtype)
 
 
 def gated_recurrence(
