@@ -232,17 +232,40 @@ __device__ __forceinline__ void load_panels(u32x4 buffer, unsigned dst, int coun
                row < rows && at < bytes ? static_cast<unsigned>(row) * stride + at : kNowhere);
   }
 }
-// Panels that lie in memory one after another as they are.
-template <typename T>
-__device__ __forceinline__ void load_whole(u32x4 buffer, unsigned dst, int count, int wave, int waves) {
-  constexpr int kLoads = Chunk<T>::kTokens / 8;
-  const int lane = threadIdx.x & 63;
-  for (int i = wave; i < count * kLoads; i += waves) {
-    const int row = i % kLoads * 8 + lane / 8;
-    load_lds16(buffer, dst + i * 1024,
-               static_cast<unsigned>(i * 1024 + lane / 8 * 128 + (((lane % 8) ^ swizzle(row)) << 4)));
+// The same with the lane's places made once, for a walk over chunks: COUNT panels by W waves.
+template <typename T, int COUNT, int W>
+struct PanelLoads {
+  static constexpr int kLoads = Chunk<T>::kTokens / 8, kMine = COUNT * kLoads / W;
+  static_assert(COUNT * kLoads % W == 0, "as many loads a wave");
+  unsigned offset[kMine];
+  __device__ __forceinline__ static int row(int j, int wave) {
+    return (j * W + wave) % kLoads * 8 + static_cast<int>(threadIdx.x & 63) / 8;
   }
-}
+  __device__ __forceinline__ PanelLoads(unsigned column, unsigned stride, unsigned bytes, int wave) {
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int r = row(j, wave);
+      const unsigned at = column + (j * W + wave) / kLoads * 128 + (((threadIdx.x % 8) ^ swizzle(r)) << 4);
+      offset[j] = at < bytes ? static_cast<unsigned>(r) * stride + at : kNowhere;
+    }
+  }
+  // Panels that lie in memory one after another as they are.
+  __device__ __forceinline__ explicit PanelLoads(int wave) {
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      offset[j] = (j * W + wave) * 1024 + (threadIdx.x & 63) / 8 * 128 + (((threadIdx.x % 8) ^ swizzle(row(j, wave))) << 4);
+  }
+  __device__ __forceinline__ void load(u32x4 buffer, unsigned dst, int wave, int rows) const {
+    if (rows == Chunk<T>::kTokens) {
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) load_lds16(buffer, dst + (j * W + wave) * 1024, offset[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kMine; ++j)
+        load_lds16(buffer, dst + (j * W + wave) * 1024, row(j, wave) < rows ? offset[j] : kNowhere);
+    }
+  }
+};
 
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
@@ -291,13 +314,14 @@ struct Record {
   float beta[kTokens];
   float value_to_state[kTokens];  // e rk
   float state_to_output[kTokens];  // c rq
+  float whole;                     // c of the last token
+  float unused[3];
   float rk[kTokens];
   float rq[kTokens];
   float norm[kTokens];            // rq without the scale
   double sum[kTokens];
   uint64_t closed;
-  float whole;  // c of the last token
-  float unused;
+  uint64_t filler;
 };
 
 // ---- T, P and the factors of every chunk ----------------------------------------------------------
@@ -558,9 +582,22 @@ struct Stage {
   static constexpr int kValues = kPairs + C::kTerms * C::kPanel;
   static constexpr int kValuePanels = W * 16 / C::kTokens;
   static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
-  static constexpr int kBytes = kFactors + 1024;
+  static constexpr int kBytes = kFactors + 2048;
   static_assert(W * 16 % C::kTokens == 0, "whole panels of values");
 };
+
+// Block i of a lower triangle of tiles by steps of a fragment, its first steps before its second ones.
+template <typename T>
+struct Triangle {
+  static constexpr int kTiles = Chunk<T>::kTiles, kPer = Chunk<T>::kPer, kBlocks = 2 * kTiles - kPer;
+  int tile, step;
+  __device__ __forceinline__ explicit Triangle(int i)
+      : tile(i < kTiles ? i : i - kTiles + kPer), step(i < kTiles ? 0 : 1) {}
+};
+// Reads of LDS and matrix instructions stay in the order written; arithmetic and stores may move. Left to
+// itself the compiler reads each fragment right before its product (a chunk 8 us, where this takes XX).
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x40); }
+constexpr int kAhead = 10;  // of the 15 that may be under way
 
 // A wave keeps 16 columns of S in registers, as results [key, column] of the products that update it, and
 // walks through all of them by itself: K S, T R, P U and K^T U take its columns' values as one
@@ -568,7 +605,7 @@ struct Stage {
 // other, from LDS, so waves meet only where panels change hands, once a chunk. The next chunk's panels
 // load meanwhile.
 template <typename T, int DK, int W, bool KEEP>
-__global__ __launch_bounds__(64 * W) void delta_forward(DeltaArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_forward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
   using S = Stage<T, DK, W>;
@@ -607,30 +644,49 @@ __global__ __launch_bounds__(64 * W) void delta_forward(DeltaArgs a) {
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
   const T* v_at = at_token<T>(a.value, a.value_strides, b, 0, h);
+  const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
+  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, S::kValuePanels, W> value_loads(
+      static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
+      static_cast<unsigned>(value_size * sizeof(T)), wave);
+  const PanelLoads<T, 2 * kTerms, W> pair_loads(wave);
   auto load = [&](int c) __attribute__((always_inline)) {
     const unsigned dst = lds_at + (c & 1) * S::kBytes;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
-    const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
-    load_panels<T>(buffer_at(k_at + t0 * a.key_strides.token), dst, DK / kTokens, 0,
-                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, key_bytes, wave, W);
-    load_whole<T>(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, 2 * kTerms,
-                  wave, W);
-    load_panels<T>(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, S::kValuePanels,
-                   static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
-                   rows, static_cast<unsigned>(value_size * sizeof(T)), wave, W);
-    load_panels<T>(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, DK / kTokens, 0,
-                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, key_bytes, wave, W);
-    if (wave == W - 1) {
-      const unsigned at = (threadIdx.x & 63) * 16;
-      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c), dst + S::kFactors,
-                 at < 16 * kTokens ? at : kNowhere);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst, wave, rows);
+    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, wave, rows);
+    query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
+    if (wave < 2) {  // the factors, and after them `whole`
+      const unsigned at = wave * 16 * kTokens + (threadIdx.x & 63) * 16;
+      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
+                 dst + S::kFactors + wave * 1024, at < (wave == 0 ? 16 : 17) * kTokens ? at : kNowhere);
     }
   };
 
   T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
   const int64_t out_token = a.heads * value_size;
   const int store_at = column + lane.g * 4, store_count = value_size - store_at;
+  // A chunk's results are stored while the next one is worked on: the wait for loads is for stores too.
+  f32x4 held_output[kTiles];
+  frag held_update[2];
+  int held = -1;
+  const auto store_held = [&]() __attribute__((always_inline)) {
+    if (held < 0) return;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const int64_t t = static_cast<int64_t>(held) * kTokens + n * 16 + lane.l;
+      if (t < a.tokens && store_count > 0) store_four(out + t * out_token + store_at, held_output[n], store_count);
+    }
+    if constexpr (KEEP) {
+      T* keep = static_cast<T*>(a.updates) + ((first_chunk + held) * a.value_pad + mine) * kTokens +
+                lane.g * (16 / sizeof(T));
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + kt * C::kStep) = held_update[kt];
+    }
+  };
   if (chunks > 0) load(0);
 #pragma unroll 1
   for (int c = 0; c < chunks; ++c) {
@@ -638,10 +694,10 @@ __global__ __launch_bounds__(64 * W) void delta_forward(DeltaArgs a) {
     __syncthreads();
     if (c + 1 < chunks) load(c + 1);
     if (!active) continue;
+    store_held();
     const unsigned char* at = lds + (c & 1) * S::kBytes;
     const float* factors = reinterpret_cast<const float*>(at + S::kFactors);
-    const float whole = reinterpret_cast<const Record<T>*>(a.records)[first_chunk + c].whole;
-    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
+    const float whole = factors[256];
 
     frag s[kSteps][kTerms];
 #pragma unroll
@@ -652,95 +708,141 @@ __global__ __launch_bounds__(64 * W) void delta_forward(DeltaArgs a) {
       for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + ks * C::kStep) = s[ks][0];
     }
 
+    // The chunk's fragments in the order of their products, read kAhead of them before: K, Q, T, K^T, P.
+    // Neighbouring products are of different sums, since one waits for the last of its own sum.
+    constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
+    frag kf[kRows], qf[kRows], tf[kTerms * kBlocks], pf[kTerms * kBlocks], cf[kColumns];
+    const auto fetch = [&](int i) __attribute__((always_inline)) {
+      if (i < kRows) {
+        kf[i] = read_row<T>(at, operand_row<T>(i % kTiles, lane.l), i / kTiles, lane);
+      } else if ((i -= kRows) < kRows) {
+        qf[i] = read_row<T>(at + S::kQuery, i % kTiles * 16 + lane.l, i / kTiles, lane);
+      } else if ((i -= kRows) < kTerms * kBlocks) {
+        const Triangle<T> b(i % kBlocks);
+        tf[i] = read_row<T>(at + S::kSolve + i / kBlocks * C::kPanel, operand_row<T>(b.tile, lane.l), b.step, lane);
+      } else if ((i -= kTerms * kBlocks) < kColumns) {
+        cf[i] = read_column<T>(at, i / 8 * 4 + i % 4, i / 4 % 2, lane);
+      } else if ((i -= kColumns) < kTerms * kBlocks) {
+        const Triangle<T> b(i % kBlocks);
+        pf[i] = read_row<T>(at + S::kPairs + i / kBlocks * C::kPanel, b.tile * 16 + lane.l, b.step, lane);
+      }
+    };
+    constexpr int kFirstQ = kRows, kFirstT = 2 * kRows, kFirstC = kFirstT + kTerms * kBlocks,
+                  kFirstP = kFirstC + kColumns;
+    f32x4 v[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) v[m] = read_values<T>(at + S::kValues, wave, m, lane);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(i);
+
     // R = beta V - (beta c rk) K S.
+    Sum<T> sums[kTiles];
+#pragma unroll
+    for (int i = 0; i < kRows; i += kTiles) {
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) fetch(i + m + kAhead);
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) sums[m].add(kf[i + m], s[i / kTiles][term], term > 0);
+      keep_order();
+    }
     f32x4 r[kTiles];
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
-      Sum<T> sum;
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-        const frag k = read_row<T>(at, operand_row<T>(m, lane.l), ks, lane);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) sum.add(k, s[ks][term], term > 0);
-      }
-      const f32x4 acc = sum.value();
-      const f32x4 v = read_values<T>(at + S::kValues, wave, m, lane);
+      const f32x4 acc = sums[m].value();
       const int row = first_row<T>(m, lane.g);
       const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
       const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[e], -take[e] * acc[e]);
+      for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[m][e], -take[e] * acc[e]);
+      sums[m] = Sum<T>();
     }
+    // Q S: O's lanes are tokens and its registers columns.
+    Sum<T> o[kTiles];
     frag rf[2][kTerms], uf[2][kTerms], df[2][kTerms];
+#pragma unroll
+    for (int i = 0; i < kRows; i += kTiles) {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) fetch(kFirstQ + i + n + kAhead);
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) o[n].add(s[i / kTiles][term], qf[i + n], term > 0);
+      keep_order();
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const float factor = factors[3 * kTokens + n * 16 + lane.l];
+      o[n].whole *= factor;
+      o[n].rest *= factor;
+    }
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) split<T>(&r[kt * kPer], rf[kt]);
     // U = T R.
+#pragma unroll
+    for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) fetch(kFirstT + term * kBlocks + i + kAhead);
+#pragma unroll
+      for (int other = 0; other < kTerms - term; ++other)
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const Triangle<T> b(i);
+          sums[b.tile].add(tf[term * kBlocks + i], rf[b.step][other], term + other > 0);
+        }
+      keep_order();
+    }
     f32x4 u[kTiles];
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      Sum<T> sum;
-#pragma unroll
-      for (int kt = 0; kt <= m / kPer; ++kt) {
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          const frag t = read_row<T>(at + S::kSolve + term * C::kPanel, operand_row<T>(m, lane.l), kt, lane);
-#pragma unroll
-          for (int other = 0; other < kTerms - term; ++other) sum.add(t, rf[kt][other], term + other > 0);
-        }
-      }
-      u[m] = sum.value();
-    }
+    for (int m = 0; m < kTiles; ++m) u[m] = sums[m].value();
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
-    if constexpr (KEEP) {
-      T* keep = static_cast<T*>(a.updates) + ((first_chunk + c) * a.value_pad + mine) * kTokens +
-                lane.g * (16 / sizeof(T));
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + kt * C::kStep) = uf[kt][0];
-    }
-    // O, its lanes tokens and its registers columns.
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      Sum<T> sum;
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-        const frag q = read_row<T>(at + S::kQuery, n * 16 + lane.l, ks, lane);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) sum.add(s[ks][term], q, term > 0);
-      }
-      const float factor = factors[3 * kTokens + n * 16 + lane.l];
-      sum.whole *= factor;
-      sum.rest *= factor;
-#pragma unroll
-      for (int kt = 0; kt <= n / kPer; ++kt) {
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          const frag p = read_row<T>(at + S::kPairs + term * C::kPanel, n * 16 + lane.l, kt, lane);
-#pragma unroll
-          for (int other = 0; other < kTerms - term; ++other) sum.add(uf[kt][other], p, term + other > 0);
-        }
-      }
-      const f32x4 o = sum.value();
-      const int64_t t = t0 + n * 16 + lane.l;
-      if (t < a.tokens && store_count > 0) store_four(out + t * out_token + store_at, o, store_count);
-    }
     // S = c S + K^T (e rk U).
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], df[kt]);
 #pragma unroll
-    for (int m = 0; m < kStateTiles; ++m) {
-      Sum<T> sum(state[m] * whole);
+    for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
+      Sum<T> part[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) part[m].whole = state[m0 + m] * whole;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const frag k = read_column<T>(at, m, kt, lane);
 #pragma unroll
-        for (int term = 0; term < kTerms; ++term) sum.add(k, df[kt][term], term > 0);
+        for (int m = 0; m < 4; ++m) fetch(kFirstC + m0 * 2 + kt * 4 + m + kAhead);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) part[m].add(cf[m0 * 2 + kt * 4 + m], df[kt][term], term > 0);
+        keep_order();
       }
-      state[m] = sum.value();
+#pragma unroll
+      for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
     }
+    // O = c rq Q S + P U.
+#pragma unroll
+    for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+      for (int other = 0; other < kTerms - term; ++other)
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const Triangle<T> b(i);
+          if (other == 0) fetch(kFirstP + term * kBlocks + i + kAhead);
+          o[b.tile].add(uf[b.step][other], pf[term * kBlocks + i], term + other > 0);
+        }
+      keep_order();
+    }
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) held_output[n] = o[n].value();
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) held_update[kt] = uf[kt][0];
+    }
+    held = c;
   }
+  store_held();
   if (!active) return;
 #pragma unroll
   for (int m = 0; m < kStateTiles; ++m)
@@ -802,24 +904,25 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
   const T* g_at = at_token<T>(a.grad_output, a.grad_strides, b, 0, h);
+  const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
+  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, S::kValuePanels, W> value_loads(
+      static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
+      static_cast<unsigned>(value_size * sizeof(T)), wave);
+  const PanelLoads<T, 2 * kTerms, W> pair_loads(wave);
   auto load = [&](int c) __attribute__((always_inline)) {
     const unsigned dst = lds_at + (c & 1) * S::kBytes;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
-    const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
-    load_panels<T>(buffer_at(k_at + t0 * a.key_strides.token), dst, DK / kTokens, 0,
-                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, key_bytes, wave, W);
-    load_whole<T>(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, 2 * kTerms,
-                  wave, W);
-    load_panels<T>(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, S::kValuePanels,
-                   static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
-                   rows, static_cast<unsigned>(value_size * sizeof(T)), wave, W);
-    load_panels<T>(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, DK / kTokens, 0,
-                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, key_bytes, wave, W);
-    if (wave == W - 1) {
-      const unsigned at = (threadIdx.x & 63) * 16;
-      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c), dst + S::kFactors,
-                 at < 16 * kTokens ? at : kNowhere);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst, wave, rows);
+    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, wave, rows);
+    query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
+    if (wave < 2) {  // the factors, and after them `whole`
+      const unsigned at = wave * 16 * kTokens + (threadIdx.x & 63) * 16;
+      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
+                 dst + S::kFactors + wave * 1024, at < (wave == 0 ? 16 : 17) * kTokens ? at : kNowhere);
     }
   };
 
@@ -835,7 +938,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
     if (!active) continue;
     const unsigned char* at = lds + (c & 1) * S::kBytes;
     const float* factors = reinterpret_cast<const float*>(at + S::kFactors);
-    const float whole = reinterpret_cast<const Record<T>*>(a.records)[first_chunk + c].whole;
+    const float whole = factors[256];
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
 
     frag s[kSteps][kTerms];
