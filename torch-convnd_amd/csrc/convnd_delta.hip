@@ -76,70 +76,160 @@ __device__ __forceinline__ int first_row(int m, int g) {
   return m * 16 + g * 4;
 }
 
-// Fragment of step ks (two a panel) of the lane's row.
-template <typename T>
-__device__ __forceinline__ typename Chunk<T>::frag read_row(const unsigned char* panels, int row, int ks,
-                                                            const Lane& lane) {
-  return *reinterpret_cast<const typename Chunk<T>::frag*>(
-      panels + ks / 2 * Chunk<T>::kPanel + row * 128 + (((ks % 2 * 4 + lane.g) ^ swizzle(row)) << 4));
+template <typename V>
+__device__ __forceinline__ V lds_read(unsigned at) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const V*>(static_cast<uintptr_t>(at));
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
 }
 
-// Four values down a column: rows `row` to row + 3 of a panel (row a whole four) at column `column` of
-// each lane. The 16 lanes of a group read 4 rows of 4 pieces of 8 bytes; lane l gets value l % 4 of
-// piece l / 4. `piece` is the byte offset, within the rows, of the 8 bytes that this lane fetches.
+// Reads of panels by their LDS address. The swizzle of a place is the exclusive or of a part of the lane and
+// one of the place, so a lane holds one address for each value of the latter and every read is one of them
+// and a constant; computed place by place, the compiler kept hundreds of addresses (and spilled).
 template <typename T>
-__device__ __forceinline__ s16x4 read_down(const unsigned char* panel, int row, int piece, const Lane& lane) {
-  using lds_vec = __attribute__((address_space(3))) s16x4*;
-  const int r = row + (lane.l >> 2);
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds_vec)(panel + r * 128 + (((piece >> 4) ^ swizzle(r)) << 4) + (piece & 8)));
-}
+struct Reader {
+  using frag = typename Chunk<T>::frag;
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kPanel = Chunk<T>::kPanel;
+  unsigned rows[4], operands[kHalf ? 4 : 1], columns[4], ordered[kHalf ? 8 : 1];
 
-// Fragment of the transposed panels: contraction values are rows kt * kStep .., the lane's row of the
-// operand is column operand_row(m) (ORDERED: m * 16 + l) of the panels.
-template <typename T, bool ORDERED = false>
-__device__ __forceinline__ typename Chunk<T>::frag read_column(const unsigned char* panels, int m, int kt,
-                                                               const Lane& lane) {
-  if constexpr (sizeof(T) == 2) {
-    const unsigned char* panel = panels + m / 4 * Chunk<T>::kPanel;
-    const int piece = ORDERED ? m % 4 * 32 + (lane.l & 3) * 8
-                              : m / 2 % 2 * 64 + (lane.l & 3) * 16 + m % 2 * 8;
+  // `flip` goes into the places of ordered columns (64: two tiles further in a panel).
+  __device__ __forceinline__ explicit Reader(unsigned flip = 0) {
+    const unsigned l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const auto bit = [](unsigned v, int i) { return v >> i & 1; };
+#pragma unroll
+    for (unsigned x = 0; x < 4; ++x)  // halves of a panel's rows, odd tiles
+      rows[x] = l * 128 + (((g ^ (bit(l, 1) << 2 | bit(l, 3) << 1 | bit(l, 2))) << 4) ^ (x >> 1 << 6) ^ ((x & 1) << 4));
+    if constexpr (kHalf) {
+#pragma unroll
+      for (unsigned x = 0; x < 4; ++x) {
+        operands[x] = (l >> 2) * 1024 + (l & 3) * 128 +
+                      (((g ^ (bit(l, 1) << 2 | bit(l, 2) << 1 | bit(l, 3))) << 4) ^ (x >> 1 << 6) ^ ((x & 1) << 4));
+        const unsigned row = bit(l, 3) << 2 | bit(g, 0) << 1 | bit(g, 1);  // odd pairs of tiles, second rows
+        columns[x] = g * 1024 + (l >> 2) * 128 + ((((l & 3) ^ row) << 4) ^ (x >> 1 << 6) ^ ((x & 1) << 4));
+      }
+#pragma unroll
+      for (unsigned x = 0; x < 8; ++x)  // tiles of a panel, second rows
+        ordered[x] = g * 1024 + (l >> 2) * 128 + (l & 1) * 8 +
+                     (flip ^ ((bit(l, 1) ^ (bit(l, 3) << 2 | bit(g, 0) << 1 | bit(g, 1))) << 4) ^ (x >> 1 << 5) ^ ((x & 1) << 4));
+    } else {
+#pragma unroll
+      for (unsigned x = 0; x < 4; ++x)  // odd tiles and second rows, odd steps
+        columns[x] = g * 512 + (l & 3) * 4 +
+                     ((((l >> 2) ^ (bit(g, 1) << 1 | bit(g, 0))) << 4) ^ (x >> 1 << 6) ^ ((x & 1) << 4));
+    }
+  }
+
+  // Fragment of step ks (two a panel) of row 16 n + l.
+  __device__ __forceinline__ frag row(unsigned panels, int n, int ks) const {
+    return lds_read<frag>(panels + rows[ks % 2 * 2 + n % 2] + ks / 2 * kPanel + n * 2048);
+  }
+  // Of row operand_row(m, l).
+  __device__ __forceinline__ frag operand(unsigned panels, int m, int ks) const {
+    if constexpr (kHalf)
+      return lds_read<frag>(panels + operands[ks % 2 * 2 + m % 2] + ks / 2 * kPanel + m / 2 * 4096 + m % 2 * 512);
+    else
+      return row(panels, m, ks);
+  }
+  // Fragments of the transposed panels: contraction values are rows kt * kStep .., the lane's row of the
+  // operand is column operand_row(m, l).
+  __device__ __forceinline__ frag column(unsigned panels, int m, int kt) const {
+    if constexpr (kHalf) {
+      const unsigned at = panels + m / 4 * kPanel + kt * 4096 + m % 2 * 8;
+      return join(down(at + columns[m / 2 % 2 * 2]), down(at + columns[m / 2 % 2 * 2 + 1] + 512));
+    } else {
+      f32x4 f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        f[i] = lds_read<float>(panels + columns[(m % 2 ^ i / 2) * 2 + kt % 2] + m / 2 * kPanel + kt * 2048 + i * 128);
+      return f;
+    }
+  }
+  // Column 16 m + l.
+  __device__ __forceinline__ frag ordered_column(unsigned panels, int m, int kt) const {
+    if constexpr (kHalf) {
+      const unsigned at = panels + m / 4 * kPanel + kt * 4096;
+      return join(down(at + ordered[m % 4 * 2]), down(at + ordered[m % 4 * 2 + 1] + 512));
+    } else {
+      return column(panels, m, kt);
+    }
+  }
+  // Four values down a column. The 16 lanes of a group read 4 rows of 4 pieces of 8 bytes; lane l gets value
+  // l % 4 of piece l / 4 of each.
+  __device__ __forceinline__ static s16x4 down(unsigned at) {
+    using lds_vec = __attribute__((address_space(3))) s16x4*;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_vec>(static_cast<uintptr_t>(at)));
+  }
+  __device__ __forceinline__ static frag join(s16x4 a, s16x4 b) {
     union {
       s16x4 part[2];
-      typename Chunk<T>::frag whole;
+      frag whole;
     } u;
-    u.part[0] = read_down<T>(panel, kt * 32 + lane.g * 8, piece, lane);
-    u.part[1] = read_down<T>(panel, kt * 32 + lane.g * 8 + 4, piece, lane);
+    u.part[0] = a;
+    u.part[1] = b;
     return u.whole;
-  } else {
-    const unsigned char* panel = panels + m / 2 * Chunk<T>::kPanel;
-    f32x4 f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = kt * 16 + lane.g * 4 + i;
-      f[i] = *reinterpret_cast<const float*>(panel + r * 128 +
-                                             (((m % 2 * 4 + (lane.l >> 2)) ^ swizzle(r)) << 4) +
-                                             (lane.l & 3) * 4);
-    }
-    return f;
   }
-}
+};
 
-// Column 16 tile + l of the panels at the rows of result tile m.
+// The same for one tile that the wave has as its own (rows 16 tile + l, columns 16 tile + l of the panels).
 template <typename T>
-__device__ __forceinline__ f32x4 read_values(const unsigned char* panels, int tile, int m, const Lane& lane) {
-  f32x4 v;
-  if constexpr (sizeof(T) == 2) {
-    const Four<T> s = __builtin_bit_cast(
-        Four<T>, read_down<T>(panels + tile / 4 * Chunk<T>::kPanel, first_row<T>(m, lane.g),
-                           tile % 4 * 32 + (lane.l & 3) * 8, lane));
+struct Own {
+  using frag = typename Chunk<T>::frag;
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int kPanel = Chunk<T>::kPanel;
+  unsigned rows[2], columns[kHalf ? 2 : 4], place;
+
+  __device__ __forceinline__ explicit Own(int tile) {
+    const int l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, r = tile * 16 + l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(s[e]);
-  } else {
-    v = read_column<T>(panels, tile, m, lane);
+    for (int x = 0; x < 2; ++x) rows[x] = r * 128 + (((x * 4 + g) ^ swizzle(r)) << 4);
+    // Of the first four values of a lane's (tile 0 of 16, four a lane group).
+    const int at = g * 4 * sizeof(T);
+    place = r * 128 + (((at >> 4) ^ swizzle(r)) << 4) + at % 16;
+    if constexpr (kHalf) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int row = g * 8 + x * 4 + (l >> 2);
+        columns[x] = tile / 4 * kPanel + row * 128 + (((tile % 4 * 2 + (l >> 1 & 1)) ^ swizzle(row)) << 4) + (l & 1) * 8;
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {  // second rows, odd steps
+        const int row = x % 2 * 16 + g * 4 + x / 2 * 2;
+        columns[x] = tile / 2 * kPanel + g * 512 + (((tile % 2 * 4 + (l >> 2)) ^ swizzle(row)) << 4) + (l & 3) * 4;
+      }
+    }
   }
-  return v;
-}
+  __device__ __forceinline__ frag row(unsigned panels, int ks) const {
+    return lds_read<frag>(panels + rows[ks % 2] + ks / 2 * kPanel);
+  }
+  // Values 16 m + 4 g to 16 m + 4 g + 3 of the lane's row.
+  __device__ __forceinline__ f32x4 four(unsigned panels, int m) const {
+    constexpr int kTilePieces = sizeof(T);  // 16-byte pieces of 16 values
+    const Four<T> v = lds_read<Four<T>>(panels + (place ^ (m * kTilePieces % 8 << 4)) + m * kTilePieces / 8 * kPanel);
+    return f32x4{static_cast<float>(v[0]), static_cast<float>(v[1]), static_cast<float>(v[2]), static_cast<float>(v[3])};
+  }
+  __device__ __forceinline__ frag column(unsigned panels, int kt) const {
+    if constexpr (kHalf) {
+      return Reader<T>::join(Reader<T>::down(panels + columns[0] + kt * 4096), Reader<T>::down(panels + columns[1] + kt * 4096));
+    } else {
+      f32x4 f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = lds_read<float>(panels + columns[i / 2 * 2 + kt % 2] + kt * 2048 + i * 128);
+      return f;
+    }
+  }
+  // The column at the rows of result tile m.
+  __device__ __forceinline__ f32x4 values(unsigned panels, int m) const {
+    if constexpr (kHalf) {
+      const Four<T> s = __builtin_bit_cast(Four<T>, Reader<T>::down(panels + columns[m % 2] + m / 2 * 4096));
+      return f32x4{static_cast<float>(s[0]), static_cast<float>(s[1]), static_cast<float>(s[2]), static_cast<float>(s[3])};
+    } else {
+      return column(panels, m);
+    }
+  }
+};
 
 // The second terms of float16 values are kept 2^11 times as large, in sums of their own: as they are, those of
 // values below 0.1 would end in the type's fixed-point range (states 1.4e-5 off where bfloat16's are 4e-6).
@@ -266,10 +356,6 @@ struct PanelLoads {
     }
   }
 };
-
-__device__ __forceinline__ unsigned lds_address(const void* p) {
-  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
-}
 
 // A wave's own exchange through LDS: what its lanes wrote is there for the others.
 __device__ __forceinline__ void wait_own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -402,17 +488,19 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs
       norm[r] = ss[1];
     }
   }
+  const Reader<T> read;
+  const Own<T> own(wave);
+  const unsigned keys = lds_address(lds.operands[0]), queries = lds_address(lds.operands[1]);
   f32x4 kk[kTiles], qk[kTiles];
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) kk[j] = qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int ks = 0; ks < kSteps; ++ks) {
-    const frag own_k = read_row<T>(lds.operands[0], wave * 16 + lane.l, ks, lane);
-    const frag own_q = read_row<T>(lds.operands[1], wave * 16 + lane.l, ks, lane);
+    const frag own_k = own.row(keys, ks), own_q = own.row(queries, ks);
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
       if (j > wave) continue;
-      const frag k = read_row<T>(lds.operands[0], j * 16 + lane.l, ks, lane);
+      const frag k = read.row(keys, j, ks);
       kk[j] = Fragment<T>::mma(own_k, k, kk[j]);  // registers rows of this wave, lanes columns
       qk[j] = Fragment<T>::mma(k, own_q, qk[j]);  // registers columns, lanes rows of this wave
     }
@@ -613,6 +701,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
+  const Reader<T> read;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups of a head's columns are a whole number of heads apart: where that is a multiple of eight
   // they run on one XCD and share its L2.
@@ -640,6 +729,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
                         : 0.f;
     }
 
+  const Own<T> own(wave);
   const unsigned lds_at = lds_address(lds);
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
@@ -695,8 +785,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     if (c + 1 < chunks) load(c + 1);
     if (!active) continue;
     store_held();
-    const unsigned char* at = lds + (c & 1) * S::kBytes;
-    const float* factors = reinterpret_cast<const float*>(at + S::kFactors);
+    const unsigned at = lds_at + (c & 1) * S::kBytes;
+    const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
     const float whole = factors[256];
 
     frag s[kSteps][kTerms];
@@ -714,24 +804,24 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     frag kf[kRows], qf[kRows], tf[kTerms * kBlocks], pf[kTerms * kBlocks], cf[kColumns];
     const auto fetch = [&](int i) __attribute__((always_inline)) {
       if (i < kRows) {
-        kf[i] = read_row<T>(at, operand_row<T>(i % kTiles, lane.l), i / kTiles, lane);
+        kf[i] = read.operand(at, i % kTiles, i / kTiles);
       } else if ((i -= kRows) < kRows) {
-        qf[i] = read_row<T>(at + S::kQuery, i % kTiles * 16 + lane.l, i / kTiles, lane);
+        qf[i] = read.row(at + S::kQuery, i % kTiles, i / kTiles);
       } else if ((i -= kRows) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
-        tf[i] = read_row<T>(at + S::kSolve + i / kBlocks * C::kPanel, operand_row<T>(b.tile, lane.l), b.step, lane);
+        tf[i] = read.operand(at + S::kSolve + i / kBlocks * C::kPanel, b.tile, b.step);
       } else if ((i -= kTerms * kBlocks) < kColumns) {
-        cf[i] = read_column<T>(at, i / 8 * 4 + i % 4, i / 4 % 2, lane);
+        cf[i] = read.column(at, i / 8 * 4 + i % 4, i / 4 % 2);
       } else if ((i -= kColumns) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
-        pf[i] = read_row<T>(at + S::kPairs + i / kBlocks * C::kPanel, b.tile * 16 + lane.l, b.step, lane);
+        pf[i] = read.row(at + S::kPairs + i / kBlocks * C::kPanel, b.tile, b.step);
       }
     };
     constexpr int kFirstQ = kRows, kFirstT = 2 * kRows, kFirstC = kFirstT + kTerms * kBlocks,
                   kFirstP = kFirstC + kColumns;
     f32x4 v[kTiles];
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) v[m] = read_values<T>(at + S::kValues, wave, m, lane);
+    for (int m = 0; m < kTiles; ++m) v[m] = own.values(at + S::kValues, m);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch(i);
 
@@ -874,6 +964,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
   constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
+  const Reader<T> read;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t heads = a.batch * a.heads;
   const int64_t bh = blockIdx.x % heads;
@@ -900,6 +991,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
                         : 0.f;
     }
 
+  const Own<T> own(wave);
   const unsigned lds_at = lds_address(lds);
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
@@ -936,8 +1028,8 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
     __syncthreads();
     if (c > 0) load(c - 1);
     if (!active) continue;
-    const unsigned char* at = lds + (c & 1) * S::kBytes;
-    const float* factors = reinterpret_cast<const float*>(at + S::kFactors);
+    const unsigned at = lds_at + (c & 1) * S::kBytes;
+    const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
     const float whole = factors[256];
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
 
@@ -952,7 +1044,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
     }
     frag g[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) g[kt] = read_column<T, true>(at + S::kValues, wave, kt, lane);
+    for (int kt = 0; kt < 2; ++kt) g[kt] = own.column(at + S::kValues, kt);
 
     f32x4 u[kTiles];
 #pragma unroll
@@ -960,7 +1052,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
       Sum<T> sum;
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) {
-        const frag k = read_row<T>(at, operand_row<T>(m, lane.l), ks, lane);
+        const frag k = read.operand(at, m, ks);
 #pragma unroll
         for (int term = 0; term < kTerms; ++term) sum.add(k, s[ks][term], term > 0);
       }
@@ -971,7 +1063,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
       for (int kt = m / kPer; kt < 2; ++kt)
 #pragma unroll
         for (int term = 0; term < kTerms; ++term)
-          sum.add(read_column<T>(at + S::kPairs + term * C::kPanel, m, kt, lane), g[kt], term > 0);
+          sum.add(read.column(at + S::kPairs + term * C::kPanel, m, kt), g[kt], term > 0);
       u[m] = sum.value();
     }
     frag uf[2][kTerms];
@@ -985,7 +1077,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
       for (int kt = m / kPer; kt < 2; ++kt)
 #pragma unroll
         for (int term = 0; term < kTerms; ++term) {
-          const frag t = read_column<T>(at + S::kSolve + term * C::kPanel, m, kt, lane);
+          const frag t = read.column(at + S::kSolve + term * C::kPanel, m, kt);
 #pragma unroll
           for (int other = 0; other < kTerms - term; ++other) sum.add(t, uf[kt][other], term + other > 0);
         }
@@ -1051,8 +1143,8 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
       Sum<T> sum(state[m] * whole);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const frag q = read_column<T>(at + S::kQuery, m, kt, lane);
-        const frag k = read_column<T>(at, m, kt, lane);
+        const frag q = read.column(at + S::kQuery, m, kt);
+        const frag k = read.column(at, m, kt);
 #pragma unroll
         for (int term = 0; term < kTerms; ++term) {
           sum.add(q, gf[kt][term], term > 0);
@@ -1086,32 +1178,51 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
 //
 // and a decay's gradient is the sum over the pairs, and the states, that its token lies between: with the
 // gradients of the sums of decays, their total from the token on. A workgroup takes a chunk of a key head and
-// adds up its value heads. Wave w has the tokens 16 w to 16 w + 15 as lanes throughout: as rows i, for which
-// pairs are made with registers j, and again as columns j with registers i, so that either is the operand of
-// the next product from registers.
-template <typename T, int DK, bool GROUPED>
-__global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_gradients(DeltaArgs a) {
+// adds up its value heads. Two waves share 16 tokens, which are their lanes throughout: each makes half of the
+// keys' gradients, and one makes the pairs with its token as the row i (registers j), the other those with it
+// as the column j (registers i), so that either is the operand of the next products, which they exchange.
+template <typename T, int DK>
+struct GradientsLds {
+  using C = Chunk<T>;
+  static constexpr int kWide = DK / C::kTokens * C::kPanel;
+  unsigned char wide[2][kWide];         // states and their gradients, then keys and queries
+  unsigned char narrow[3][C::kPanel];   // U and Y transposed, dO; then the pairs as fragments
+  double sum[C::kTokens];
+  float beta[C::kTokens], rk[C::kTokens], rq[C::kTokens], inner[2 * C::kTiles];
+  float slope[2][C::kTokens], kept[2][C::kTokens], step[2][C::kTokens];
+};
+
+// What a wave does that makes the pairs with its tokens as rows (HALF 0) or columns (1), of the first (SIDE 0) or
+// the second fragment of the chunk's tokens: all of it is known to the compiler but the tokens.
+template <typename T, int DK, bool GROUPED, int HALF, int SIDE>
+__device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T, DK>& lds) {
   using C = Chunk<T>;
   using frag = typename C::frag;
-  constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kPer = C::kPer, kThreads = kTokens * 4;
-  constexpr int kPanels = DK / kTokens, kSteps = DK / C::kStep, kKeyTiles = DK / 16;
+  constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kPer = C::kPer, kWaves = 2 * kTiles;
+  constexpr int kPanels = DK / kTokens, kSteps = DK / C::kStep, kKeyTiles = DK / 32;  // of a wave
   constexpr int kVec = 16 / sizeof(T);
-  // States and their gradients, then keys and queries.
-  __shared__ __align__(1024) unsigned char wide[2][kPanels * C::kPanel];
-  __shared__ __align__(1024) unsigned char narrow[3][C::kPanel];  // U and Y transposed, dO
-  __shared__ double sum[kTokens];
-  __shared__ float beta[kTokens], rk[kTokens], rq[kTokens], slope[kTokens], kept[kTokens], inner[kTiles];
+  auto& [wide, narrow, sum, beta, rk, rq, inner, slope, kept, step] = lds;
   const Lane lane;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int half = HALF;
+  const int block = wave % kTiles;
+  // The wave's keys: from a panel of its half on, or (64 keys of 16 bits) from the middle of the only one.
+  constexpr bool kFlip = DK / 2 * sizeof(T) < 128;
+  const Reader<T> read(kFlip ? half * 64 : 0);
+  const Own<T> mine(block);
+  const unsigned wide_at = lds_address(wide[0]), narrow_at = lds_address(narrow[0]);
+  constexpr unsigned kWide = kPanels * C::kPanel;
+  const unsigned states = wide_at + (kFlip ? 0 : half * (kWide / 2)), grads = states + kWide;
   const int chunk = static_cast<int>(blockIdx.x % a.chunks);
   const int64_t row = blockIdx.x / a.chunks;
   const int kh = static_cast<int>(row % a.key_heads), b = static_cast<int>(row / a.key_heads);
   const int length = length_of(a, b), t0 = chunk * kTokens;
-  const int groups = static_cast<int>(a.heads / a.key_heads);
-  const int own = wave * 16 + lane.l;  // this lane's token in the chunk
-  const int64_t token = static_cast<int64_t>(b) * a.tokens + t0 + own;
-  const bool in_range = t0 + own < a.tokens;
+  const int groups = GROUPED ? static_cast<int>(a.heads / a.key_heads) : 1;
+  const int own_token = block * 16 + lane.l;  // this lane's in the chunk
+  const int64_t token = static_cast<int64_t>(b) * a.tokens + t0 + own_token;
+  const bool in_range = t0 + own_token < a.tokens;
   const int key_size = static_cast<int>(a.key_size), value_size = static_cast<int>(a.value_size);
+  const int first_key = half * (DK / 2) + lane.g * 4;  // of the lane's four in the wave's first tile
   T* dq_out = static_cast<T*>(a.grad_query) + (token * a.key_heads + kh) * key_size;
   T* dk_out = static_cast<T*>(a.grad_key) + (token * a.key_heads + kh) * key_size;
   const auto store_gate = [&](void* p, int64_t at, float v) __attribute__((always_inline)) {
@@ -1124,12 +1235,12 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
     if (!in_range) return;
 #pragma unroll
     for (int m = 0; m < kKeyTiles; ++m) {
-      const int d = m * 16 + lane.g * 4;
+      const int d = first_key + m * 16;
       if (d >= key_size) continue;
       store_four(dq_out + d, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
       store_four(dk_out + d, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
     }
-    if (lane.g == 0)
+    if (lane.g == 0 && half == 0)
       for (int group = 0; group < groups; ++group) {
         store_gate(a.grad_decay, token * a.heads + kh * groups + group, 0.f);
         store_gate(a.grad_beta, token * a.heads + kh * groups + group, 0.f);
@@ -1142,33 +1253,36 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
 #pragma unroll
     for (int m = 0; m < kKeyTiles; ++m) dq_all[m] = dk_all[m] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // Four neighbouring values of this lane's row of a panel set, from column 16 m + 4 g on.
-  const auto own_values = [&](const unsigned char* panels, int m) __attribute__((always_inline)) {
-    const int at = (m * 16 + lane.g * 4) * sizeof(T);
-    const Run<T, 4> v = *reinterpret_cast<const Run<T, 4>*>(
-        panels + at / 128 * C::kPanel + own * 128 + (((at % 128 >> 4) ^ swizzle(own)) << 4) + at % 16);
-    return f32x4{static_cast<float>(v.v[0]), static_cast<float>(v.v[1]), static_cast<float>(v.v[2]),
-                 static_cast<float>(v.v[3])};
+  // Four neighbouring values of this lane's row, in the wave's tile m.
+  const auto own_values = [&](unsigned panels, int m) __attribute__((always_inline)) {
+    if constexpr (kFlip) return half == 0 ? mine.four(panels, m) : mine.four(panels, m + kKeyTiles);
+    return mine.four(panels, m);
   };
   const auto over_groups = [](float v) __attribute__((always_inline)) {
     v += __shfl_xor(v, 16);
     v += __shfl_xor(v, 32);
     return v;
   };
+  // Whether tile m holds partners of this wave's tokens.
+  const auto has = [](int m) __attribute__((always_inline)) {
+    return HALF == 0 ? m / kPer <= SIDE : m / kPer >= SIDE;
+  };
   float norm = 1.f;
 
 #pragma unroll 1
   for (int group = 0; group < groups; ++group) {
     const int h = kh * groups + group;
+    // The compiler is not to keep what follows from a lane's place from one head to the next: registers spilled.
+    int own = own_token, first = lane.g;
+    if constexpr (GROUPED) asm volatile("" : "+v"(own), "+v"(first));
     const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
     const Record<T>* record = reinterpret_cast<const Record<T>*>(a.records) + at;
     f32x4 dq[kKeyTiles], dk[kKeyTiles], back[kKeyTiles];  // dO S^T, Y S^T, U D^T
 #pragma unroll
     for (int m = 0; m < kKeyTiles; ++m) dq[m] = dk[m] = back[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // dP and Y U^T: of rows (registers columns j) and of columns (registers rows i).
-    f32x4 row_p[kTiles], row_a[kTiles], column_p[kTiles], column_a[kTiles];
+    f32x4 pair_p[kTiles], pair_a[kTiles];  // dP and Y U^T
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) row_p[m] = row_a[m] = column_p[m] = column_a[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < kTiles; ++m) pair_p[m] = pair_a[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     float dbeta = 0.f, product = 0.f;
     const T* value = at_token<T>(a.value, a.value_strides, b, t0 + own, h);
 #pragma unroll 1
@@ -1184,50 +1298,54 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           load_panels<T>(buffer_at(panels[i]), lds_address(wide[i]), kPanels, 0, DK * sizeof(T), v_rows,
-                         DK * sizeof(T), wave, kTiles);
+                         DK * sizeof(T), wave, kWaves);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          load_panels<T>(buffer_at(panels[2 + i]), lds_address(narrow[i]), 1, 0, 128, v_rows, 128, wave, kTiles);
+          load_panels<T>(buffer_at(panels[2 + i]), lds_address(narrow[i]), 1, 0, 128, v_rows, 128, wave, kWaves);
         load_panels<T>(buffer_at(at_token<T>(a.grad_output, a.grad_strides, b, t0, h)), lds_address(narrow[2]), 1,
                        static_cast<unsigned>(v0 * sizeof(T)),
                        static_cast<unsigned>(a.grad_strides.token * sizeof(T)), rows,
-                       static_cast<unsigned>(value_size * sizeof(T)), wave, kTiles);
+                       static_cast<unsigned>(value_size * sizeof(T)), wave, kWaves);
       }
       wait_loads();
       __syncthreads();
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const frag g = read_row<T>(narrow[2], own, kt, lane);
-        const frag u = read_column<T, true>(narrow[0], wave, kt, lane);
-        const frag y = read_column<T, true>(narrow[1], wave, kt, lane);
+        const frag g = mine.row(narrow_at + 2 * C::kPanel, kt);
+        const frag u = mine.column(narrow_at, kt);
+        const frag y = mine.column(narrow_at + C::kPanel, kt);
 #pragma unroll
         for (int m = 0; m < kKeyTiles; ++m) {
-          const frag s = read_column<T, true>(wide[0], m, kt, lane);
+          const frag s = read.ordered_column(states, m, kt);
           dq[m] = Fragment<T>::mma(s, g, dq[m]);
           dk[m] = Fragment<T>::mma(s, y, dk[m]);
-          back[m] = Fragment<T>::mma(read_column<T, true>(wide[1], m, kt, lane), u, back[m]);
+          back[m] = Fragment<T>::mma(read.ordered_column(grads, m, kt), u, back[m]);
         }
+        if (half == 0) {
 #pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-          if (m / kPer <= wave / kPer) {
-            const frag other = read_column<T>(narrow[0], m, kt, lane);
-            row_p[m] = Fragment<T>::mma(other, g, row_p[m]);
-            row_a[m] = Fragment<T>::mma(other, y, row_a[m]);
+          for (int m = 0; m < kTiles; ++m) {
+            if (!has(m)) continue;
+            const frag other = read.column(narrow_at, m, kt);
+            pair_p[m] = Fragment<T>::mma(other, g, pair_p[m]);
+            pair_a[m] = Fragment<T>::mma(other, y, pair_a[m]);
           }
-          if (m / kPer >= wave / kPer) {
-            column_p[m] = Fragment<T>::mma(read_row<T>(narrow[2], operand_row<T>(m, lane.l), kt, lane), u, column_p[m]);
-            column_a[m] = Fragment<T>::mma(read_column<T>(narrow[1], m, kt, lane), u, column_a[m]);
-          }
-        }
-        const int v = v0 + kt * C::kStep + lane.g * kVec;
-        if (own < rows && v < value_size) {
-          const frag f = __builtin_bit_cast(frag, load_run<kVec>(value + v));
+          const int v = v0 + kt * C::kStep + lane.g * kVec;
+          if (own < rows && v < value_size) {
+            const frag f = __builtin_bit_cast(frag, load_run<kVec>(value + v));
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) dbeta = fmaf(static_cast<float>(f[i]), static_cast<float>(y[i]), dbeta);
+            for (int i = 0; i < kVec; ++i) dbeta = fmaf(static_cast<float>(f[i]), static_cast<float>(y[i]), dbeta);
+          }
+        } else {
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) {
+            if (!has(m)) continue;
+            pair_p[m] = Fragment<T>::mma(read.operand(narrow_at + 2 * C::kPanel, m, kt), u, pair_p[m]);
+            pair_a[m] = Fragment<T>::mma(read.column(narrow_at + C::kPanel, m, kt), u, pair_a[m]);
+          }
         }
       }
       // The state's product with its gradient.
-      for (int i = threadIdx.x; i < kPanels * C::kPanel / 16; i += kThreads) {
+      for (int i = threadIdx.x; i < kPanels * C::kPanel / 16; i += 64 * kWaves) {
         const frag s = *reinterpret_cast<const frag*>(wide[0] + i * 16);
         const frag d = *reinterpret_cast<const frag*>(wide[1] + i * 16);
 #pragma unroll
@@ -1238,9 +1356,9 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
     {
       const unsigned bytes = static_cast<unsigned>(key_size * sizeof(T));
       load_panels<T>(buffer_at(at_token<T>(a.key, a.key_strides, b, t0, kh)), lds_address(wide[0]), kPanels, 0,
-                     static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kTiles);
+                     static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
       load_panels<T>(buffer_at(at_token<T>(a.query, a.query_strides, b, t0, kh)), lds_address(wide[1]), kPanels, 0,
-                     static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kTiles);
+                     static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
       if (threadIdx.x < kTokens) {
         sum[threadIdx.x] = record->sum[threadIdx.x];
         beta[threadIdx.x] = record->beta[threadIdx.x];
@@ -1254,20 +1372,21 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
     const uint64_t closed = record->closed;
     wait_loads();
     __syncthreads();
-    const unsigned char *keys = wide[0], *queries = wide[1];
+    // Of the wave's keys: `states` and `grads`.
+    const unsigned keys = wide_at, queries = wide_at + kWide;
     const double own_sum = sum[own];
     const float own_beta = beta[own], own_rk = rk[own], own_rq = rq[own];
-    const float c = (closed & (~uint64_t{0} >> (63 - own))) == 0 ? decay_between(own_sum, 0.) : 0.f;
-    const float e_own = open_between(closed, own, kTokens - 1) ? decay_between(sum[kTokens - 1], own_sum) : 0.f;
 
-    float dsum = 0.f;
     dbeta = over_groups(dbeta);
+    float dsum;
     {
       // What comes through the states.
+      const float c = (closed & (~uint64_t{0} >> (63 - own))) == 0 ? decay_between(own_sum, 0.) : 0.f;
+      const float e_own = open_between(closed, own, kTokens - 1) ? decay_between(sum[kTokens - 1], own_sum) : 0.f;
       float q_dot = 0.f, k_dot = 0.f, b_dot = 0.f;
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
-        const f32x4 q = own_values(queries, m), k = own_values(keys, m);
+        const f32x4 q = own_values(grads, m), k = own_values(states, m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           q_dot = fmaf(q[e], dq[m][e], q_dot);
@@ -1282,121 +1401,111 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
       b_dot = over_groups(b_dot) * e_own * own_rk;
       dbeta -= k_dot;
       dsum = q_dot - own_beta * k_dot - b_dot;
-      if (lane.g == 0) kept[own] = b_dot;
+      if (lane.g == 0) kept[half][own] = b_dot;
     }
-    // Pairs: this lane's token as the row.
+    // Pairs.
     f32x4 kk[kTiles], qk[kTiles];
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) kk[m] = qk[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) {
-      const frag q = read_row<T>(queries, own, ks, lane), k = read_row<T>(keys, own, ks, lane);
+      const frag k = mine.row(keys, ks), q = mine.row(queries, ks);
 #pragma unroll
       for (int m = 0; m < kTiles; ++m) {
-        if (m / kPer > wave / kPer) continue;
-        const frag other = read_row<T>(keys, operand_row<T>(m, lane.l), ks, lane);
-        qk[m] = Fragment<T>::mma(other, q, qk[m]);
+        if (!has(m)) continue;
+        const frag other = read.operand(keys, m, ks);
         kk[m] = Fragment<T>::mma(other, k, kk[m]);
+        if (half == 0)
+          qk[m] = Fragment<T>::mma(other, q, qk[m]);
+        else
+          qk[m] = Fragment<T>::mma(read.operand(queries, m, ks), k, qk[m]);
       }
     }
     float pairs = 0.f, steps = 0.f;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
-      if (m / kPer > wave / kPer) continue;
+      if (!has(m)) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = first_row<T>(m, lane.g) + e;
-        const bool open = j <= own && open_between(closed, j < own ? j : own, own);
-        const float ratio = open ? decay_between(own_sum, sum[j]) * rk[j] : 0.f;
-        const float p = open ? ratio * row_p[m][e] : 0.f;
-        const float n = open && j < own ? -ratio * row_a[m][e] : 0.f;
-        pairs = fmaf(p * own_rq, qk[m][e], pairs);
-        steps = fmaf(n * own_rk, kk[m][e], steps);
-        row_p[m][e] = p;
-        row_a[m][e] = own_beta * n;
-      }
-    }
-    steps = over_groups(steps);
-    dbeta += steps;
-    dsum += over_groups(pairs) + own_beta * steps;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      if (kt > wave / kPer) continue;
-      frag p[1], n[1];
-      split<T>(&row_p[kt * kPer], p);
-      split<T>(&row_a[kt * kPer], n);
-#pragma unroll
-      for (int m = 0; m < kKeyTiles; ++m) {
-        const frag k = read_column<T, true>(keys, m, kt, lane);
-        dq[m] = Fragment<T>::mma(k, p[0], dq[m]);
-        dk[m] = Fragment<T>::mma(k, n[0], dk[m]);
-      }
-    }
-    // And as the column.
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) kk[m] = qk[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) {
-      const frag k = read_row<T>(keys, own, ks, lane);
-#pragma unroll
-      for (int m = 0; m < kTiles; ++m) {
-        if (m / kPer < wave / kPer) continue;
-        qk[m] = Fragment<T>::mma(read_row<T>(queries, operand_row<T>(m, lane.l), ks, lane), k, qk[m]);
-        kk[m] = Fragment<T>::mma(read_row<T>(keys, operand_row<T>(m, lane.l), ks, lane), k, kk[m]);
-      }
-    }
-    pairs = 0.f;
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      if (m / kPer < wave / kPer) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = first_row<T>(m, lane.g) + e;
-        const bool open = i >= own && open_between(closed, own, i > own ? i : own);
-        const float ratio = open ? decay_between(sum[i], own_sum) : 0.f;
-        const float p = open ? ratio * rq[i] * column_p[m][e] : 0.f;
-        const float n = open && i > own ? -beta[i] * rk[i] * ratio * column_a[m][e] : 0.f;
+        const int other = first_row<T>(m, first) + e;
+        const int i = half == 0 ? own : other, j = half == 0 ? other : own;
+        const bool open = i >= j && open_between(closed, j < i ? j : i, i);
+        const float ratio = open ? half == 0 ? decay_between(own_sum, sum[other]) : decay_between(sum[other], own_sum) : 0.f;
+        // The other token's factors; this one's are taken out of the sums.
+        const float p = open ? ratio * (half == 0 ? rk[other] : rq[other]) * pair_p[m][e] : 0.f;
+        const float n = open && i > j ? -ratio * rk[other] * pair_a[m][e] : 0.f;
+        const float weighed = half == 0 ? n : n * beta[other];
         pairs = fmaf(p, qk[m][e], pairs);
-        pairs = fmaf(n, kk[m][e], pairs);
-        column_p[m][e] = p;
-        column_a[m][e] = n;
+        steps = fmaf(weighed, kk[m][e], steps);
+        pair_p[m][e] = p;
+        pair_a[m][e] = half == 0 ? own_beta * n : weighed;
       }
     }
-    dsum -= over_groups(pairs) * own_rk;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      if (kt < wave / kPer) continue;
-      frag p[1], n[1];
-      split<T>(&column_p[kt * kPer], p);
-      split<T>(&column_a[kt * kPer], n);
-#pragma unroll
-      for (int m = 0; m < kKeyTiles; ++m) {
-        dk[m] = Fragment<T>::mma(read_column<T, true>(queries, m, kt, lane), p[0], dk[m]);
-        dk[m] = Fragment<T>::mma(read_column<T, true>(keys, m, kt, lane), n[0], dk[m]);
-      }
+    pairs = over_groups(pairs);
+    steps = over_groups(steps);
+    if (half == 0) {
+      dbeta += steps * own_rk;
+      dsum += pairs * own_rq + own_beta * own_rk * steps;
+    } else {
+      dsum -= (pairs + steps) * own_rk;
     }
     if (lane.g == 0) {
-      slope[own] = dsum;
-      if (in_range) store_gate(a.grad_beta, token * a.heads + h, own < rows ? dbeta : 0.f);
+      slope[half][own] = dsum;
+      step[half][own] = dbeta;
+    }
+    // The pairs as fragments, for both waves of these tokens: three of each kind.
+    frag* shared = reinterpret_cast<frag*>(&narrow[0][0]) + block * 6 * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      if (!has(kt * kPer)) continue;
+      frag f[1];
+      split<T>(&pair_p[kt * kPer], f);
+      shared[(kt + half) * 128] = f[0];
+      split<T>(&pair_a[kt * kPer], f);
+      shared[(kt + half) * 128 + 64] = f[0];
     }
     __syncthreads();
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const bool as_row = kt <= SIDE, as_column = kt >= SIDE;
+      const frag row_p = shared[kt * 128], row_a = shared[kt * 128 + 64];
+      const frag column_p = shared[(kt + 1) * 128], column_a = shared[(kt + 1) * 128 + 64];
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) {
+        const frag k = read.ordered_column(states, m, kt);
+        if (as_row) {
+          dq[m] = Fragment<T>::mma(k, row_p, dq[m]);
+          dk[m] = Fragment<T>::mma(k, row_a, dk[m]);
+        }
+        if (as_column) {
+          dk[m] = Fragment<T>::mma(k, column_a, dk[m]);
+          dk[m] = Fragment<T>::mma(read.ordered_column(grads, m, kt), column_p, dk[m]);
+        }
+      }
+    }
     if (wave == 0) {
       // A token's decay: the gradients of the sums from it on, the last of which has the states' too.
       const int t = threadIdx.x & 63;
-      float v = t < kTokens ? slope[t] : 0.f, k = t < kTokens ? kept[t] : 0.f;
+      float v = 0.f, k = 0.f;
+      if (t < kTokens) {
+        v = slope[0][t] + slope[1][t];
+        k = kept[0][t] + kept[1][t];
+      }
       k = lanes_sum<64>(k);
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < kTiles; ++w) s += inner[w];
+      for (int w = 0; w < kWaves; ++w) s += inner[w];
       if (t == kTokens - 1) v += k + record->whole * s;
 #pragma unroll
-      for (int step = 1; step < kTokens; step *= 2) {
-        const float after = __shfl_down(v, step);
-        if (t + step < kTokens) v += after;
+      for (int by = 1; by < kTokens; by *= 2) {
+        const float after = __shfl_down(v, by);
+        if (t + by < kTokens) v += after;
       }
-      if (t < kTokens && t0 + t < a.tokens)
-        store_gate(a.grad_decay, (static_cast<int64_t>(b) * a.tokens + t0 + t) * a.heads + h,
-                   t < rows && (closed >> t & 1) == 0 ? v : 0.f);
+      if (t < kTokens && t0 + t < a.tokens) {
+        const int64_t to = (static_cast<int64_t>(b) * a.tokens + t0 + t) * a.heads + h;
+        store_gate(a.grad_decay, to, t < rows && (closed >> t & 1) == 0 ? v : 0.f);
+        store_gate(a.grad_beta, to, t < rows ? step[0][t] + step[1][t] : 0.f);
+      }
     }
     if constexpr (GROUPED) {
 #pragma unroll
@@ -1413,26 +1522,53 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, GROUPED ? 1 : 2) void delta_
     if (a.normalize) {
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
-        const f32x4 q = own_values(queries, m), k = own_values(keys, m);
+        const f32x4 q = own_values(grads, m), k = own_values(states, m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           q_dot = fmaf(q[e], dqs[m][e], q_dot);
           k_dot = fmaf(k[e], dks[m][e], k_dot);
         }
       }
-      q_dot = over_groups(q_dot) * norm * norm;
-      k_dot = over_groups(k_dot) * own_rk * own_rk;
+      q_dot = over_groups(q_dot);
+      k_dot = over_groups(k_dot);
+      __syncthreads();  // the decays' sums are read
+      if (lane.g == 0) {
+        slope[half][own] = q_dot;
+        step[half][own] = k_dot;
+      }
+      __syncthreads();
+      q_dot = (slope[0][own] + slope[1][own]) * norm * norm;
+      k_dot = (step[0][own] + step[1][own]) * own_rk * own_rk;
     }
     if (in_range) {
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
-        const int d = m * 16 + lane.g * 4;
+        const int d = first_key + m * 16;
         if (d >= key_size) continue;
-        const f32x4 q = own_values(queries, m), k = own_values(keys, m);
+        const f32x4 q = own_values(grads, m), k = own_values(states, m);
         store_four(dq_out + d, own_rq * (dqs[m] - q_dot * q), key_size - d);
         store_four(dk_out + d, own_rk * (dks[m] - k_dot * k), key_size - d);
       }
     }
+  }
+}
+
+template <typename T, int DK, bool GROUPED>
+__global__ __launch_bounds__(Chunk<T>::kTokens * 8, 2) void delta_gradients(DeltaArgs a) {
+  __shared__ __align__(1024) GradientsLds<T, DK> lds;
+  constexpr int kTiles = Chunk<T>::kTiles;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool second = wave % kTiles >= kTiles / 2;
+  if (wave < kTiles) {
+    if (second)
+      gradients_of<T, DK, GROUPED, 0, 1>(a, lds);
+    else
+      gradients_of<T, DK, GROUPED, 0, 0>(a, lds);
+  } else {
+    if (second)
+      gradients_of<T, DK, GROUPED, 1, 1>(a, lds);
+    else
+      gradients_of<T, DK, GROUPED, 1, 0>(a, lds);
   }
 }
 
@@ -1631,7 +1767,7 @@ hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(64 * W), kBytes, stream, a);
   err = hipGetLastError();
   if (err != hipSuccess || a.chunks == 0) return err;
-  const dim3 grid(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)), block(Chunk<T>::kTokens * 4);
+  const dim3 grid(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)), block(Chunk<T>::kTokens * 8);
   if (a.heads == a.key_heads)
     hipLaunchKernelGGL((delta_gradients<T, DK, false>), grid, block, 0, stream, a);
   else
