@@ -427,7 +427,7 @@ __device__ __forceinline__ float decay_between(double later, double earlier) {
 // the float matrix instructions, transposed so that a result is the next product's operand and a lane's
 // four values neighbours in a row.
 template <typename T, int DK>
-__global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs a) {
+__global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
   constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kPanels = DK / kTokens;
@@ -508,6 +508,8 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs
   const int groups = static_cast<int>(a.heads / a.key_heads);
   for (int group = 0; group < groups; ++group) {
     const int h = kh * groups + group;
+    int l = lane.l, g = lane.g;
+    asm volatile("" : "+v"(l), "+v"(g));  // what follows from them is made again for each head
     const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
     // Every wave adds the decays up; the first one keeps them for the rows' use.
     const int token = threadIdx.x & 63;
@@ -560,37 +562,37 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs
       float up[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int i = wave * 16 + lane.g * 4 + e;
+        const int i = wave * 16 + g * 4 + e;
         later[e] = sum[i];
         up[e] = beta[i] * rk[i];
       }
 #pragma unroll
       for (int jb = 0; jb < kTiles; ++jb) {
         if (jb > wave) continue;
-        const int j = jb * 16 + lane.l;
+        const int j = jb * 16 + l;
         const double earlier = sum[j];
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = wave * 16 + lane.g * 4 + e;
+          const int i = wave * 16 + g * 4 + e;
           v[e] = i > j && open_between(closed, j, i) ? up[e] * rk[j] * decay_between(later[e], earlier) * kk[jb][e]
                                                      : 0.f;
         }
-        *reinterpret_cast<f32x4*>(&lds.solve.rest[j][wave * 16 + lane.g * 4]) = v;
+        *reinterpret_cast<f32x4*>(&lds.solve.rest[j][wave * 16 + g * 4]) = v;
       }
     }
     {
       // P: lane's row i, four columns; blocks past the diagonal as far as a fragment reaches.
-      const int i = wave * 16 + lane.l;
+      const int i = wave * 16 + l;
       const double later = sum[i];
-      T* p = panels + C::kTerms * kTokens * kTokens + i * kTokens + lane.g * 4;
+      T* p = panels + C::kTerms * kTokens * kTokens + i * kTokens + g * 4;
 #pragma unroll
       for (int jb = 0; jb < kTiles; ++jb) {
         if (jb / C::kPer > wave / C::kPer) continue;
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int j = jb * 16 + lane.g * 4 + e;
+          const int j = jb * 16 + g * 4 + e;
           v[e] = i >= j && open_between(closed, j, i) ? rq[i] * rk[j] * decay_between(later, sum[j]) * qk[jb][e]
                                                       : 0.f;
         }
@@ -607,17 +609,17 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs
       // Column l of the inverse of this wave's diagonal block, x = e_l - (A - its diagonal) x.
       float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = i == lane.l ? 1.f : 0.f;
+      for (int i = 0; i < 16; ++i) x[i] = i == l ? 1.f : 0.f;
 #pragma unroll
       for (int k = 0; k < 15; ++k) {
         const float* column = &lds.solve.rest[wave * 16 + k][wave * 16];
 #pragma unroll
         for (int i = k + 1; i < 16; ++i) x[i] = fmaf(-column[i], x[k], x[i]);
       }
-      if (lane.g == 0) {
+      if (g == 0) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<f32x4*>(&lds.solve.block[wave][lane.l][i]) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+          *reinterpret_cast<f32x4*>(&lds.solve.block[wave][l][i]) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
       }
     }
     __syncthreads();
@@ -629,20 +631,20 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4) void delta_prepare(DeltaArgs
           t[j] = f32x4{0.f, 0.f, 0.f, 0.f};
         } else if (j == wave) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) t[j][e] = lds.solve.block[wave][lane.g * 4 + e][lane.l];
+          for (int e = 0; e < 4; ++e) t[j][e] = lds.solve.block[wave][g * 4 + e][l];
         } else {
           f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = j + 1; k < kTiles; ++k) {
             if (k > wave) continue;
-            const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.solve.rest[j * 16 + lane.l][k * 16 + lane.g * 4]);
+            const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.solve.rest[j * 16 + l][k * 16 + g * 4]);
             acc = Fragment<float>::mma(f, t[k], acc);
           }
-          const f32x4 d = *reinterpret_cast<const f32x4*>(&lds.solve.block[j][lane.l][lane.g * 4]);
+          const f32x4 d = *reinterpret_cast<const f32x4*>(&lds.solve.block[j][l][g * 4]);
           t[j] = Fragment<float>::mma(-d, acc, f32x4{0.f, 0.f, 0.f, 0.f});
         }
       }
-      T* p = panels + (wave * 16 + lane.l) * kTokens + lane.g * 4;
+      T* p = panels + (wave * 16 + l) * kTokens + g * 4;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         if (j / C::kPer > wave / C::kPer) continue;
