@@ -121,6 +121,20 @@ struct Reader {
     }
   }
 
+  // The same addresses `by` bytes on, as they are: were the sum known, the compiler would add each read's constant
+  // to `by` and the lane's part to that, two instructions a read.
+  __device__ __forceinline__ Reader moved(unsigned by) const {
+    Reader r = *this;
+    const auto move = [by](unsigned& at) __attribute__((always_inline)) {
+      at += by;
+      asm("" : "+v"(at));
+    };
+    for (unsigned& at : r.rows) move(at);
+    for (unsigned& at : r.operands) move(at);
+    for (unsigned& at : r.columns) move(at);
+    return r;
+  }
+
   // Fragment of step ks (two a panel) of row 16 n + l.
   __device__ __forceinline__ frag row(unsigned panels, int n, int ks) const {
     return lds_read<frag>(panels + rows[ks % 2 * 2 + n % 2] + ks / 2 * kPanel + n * 2048);
@@ -661,18 +675,18 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
 
 // ---- the walk over the chunks ------------------------------------------------------------------------
 
-// LDS of a chunk: K, Q, T, P (each in its terms), V or dO, the factors.
+// LDS of a chunk: V or dO, the factors, K, Q, T and P (each in its terms). What is read by a constant beside a
+// lane's address lies within 64 KB of it.
 template <typename T, int DK, int W>
 struct Stage {
   using C = Chunk<T>;
-  static constexpr int kKeys = DK / C::kTokens * C::kPanel;
-  static constexpr int kQuery = kKeys;
-  static constexpr int kSolve = 2 * kKeys;
-  static constexpr int kPairs = kSolve + C::kTerms * C::kPanel;
-  static constexpr int kValues = kPairs + C::kTerms * C::kPanel;
   static constexpr int kValuePanels = W * 16 / C::kTokens;
-  static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
-  static constexpr int kBytes = kFactors + 2048;
+  static constexpr int kFactors = kValuePanels * C::kPanel;
+  static constexpr int kKeys = kFactors + 2048;
+  static constexpr int kQuery = kKeys + DK / C::kTokens * C::kPanel;
+  static constexpr int kSolve = kQuery + DK / C::kTokens * C::kPanel;
+  static constexpr int kPairs = kSolve + C::kTerms * C::kPanel;
+  static constexpr int kBytes = kPairs + C::kTerms * C::kPanel;
   static_assert(W * 16 % C::kTokens == 0, "whole panels of values");
 };
 
@@ -703,7 +717,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
-  const Reader<T> read;
+  const Reader<T> places;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups of a head's columns are a whole number of heads apart: where that is a multiple of eight
   // they run on one XCD and share its L2.
@@ -747,8 +761,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     const unsigned dst = lds_at + (c & 1) * S::kBytes;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
-    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst, wave, rows);
-    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, wave, rows);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
+    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst, wave, rows);
     query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
     pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
     if (wave < 2) {  // the factors, and after them `whole`
@@ -762,21 +776,31 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const int64_t out_token = a.heads * value_size;
   const int store_at = column + lane.g * 4, store_count = value_size - store_at;
   // A chunk's results are stored while the next one is worked on: the wait for loads is for stores too.
+  const bool whole_rows = column + 16 <= value_size;
+  unsigned out_place[kTiles];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
+  const unsigned state_place = mine * DK + lane.g * (16 / sizeof(T));
+  const unsigned update_place = mine * kTokens + lane.g * (16 / sizeof(T));
   f32x4 held_output[kTiles];
   frag held_update[2];
   int held = -1;
   const auto store_held = [&]() __attribute__((always_inline)) {
     if (held < 0) return;
+    T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
+    if (whole_rows && (held + 1) * kTokens <= a.tokens) {
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const int64_t t = static_cast<int64_t>(held) * kTokens + n * 16 + lane.l;
-      if (t < a.tokens && store_count > 0) store_four(out + t * out_token + store_at, held_output[n], store_count);
+      for (int n = 0; n < kTiles; ++n) store_four(to + out_place[n], held_output[n], 4);
+    } else {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+        if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens && store_count > 0)
+          store_four(to + out_place[n], held_output[n], store_count);
     }
     if constexpr (KEEP) {
-      T* keep = static_cast<T*>(a.updates) + ((first_chunk + held) * a.value_pad + mine) * kTokens +
-                lane.g * (16 / sizeof(T));
+      T* keep = static_cast<T*>(a.updates) + (first_chunk + held) * a.value_pad * kTokens;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + kt * C::kStep) = held_update[kt];
+      for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
     }
   };
   if (chunks > 0) load(0);
@@ -788,6 +812,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     if (!active) continue;
     store_held();
     const unsigned at = lds_at + (c & 1) * S::kBytes;
+    const Reader<T> read = places.moved(at), pairs_read = places.moved(at + S::kPairs);
     const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
     const float whole = factors[256];
 
@@ -795,9 +820,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
     if constexpr (KEEP) {
-      T* keep = static_cast<T*>(a.states) + ((first_chunk + c) * a.value_pad + mine) * DK + lane.g * (16 / sizeof(T));
+      T* keep = static_cast<T*>(a.states) + (first_chunk + c) * a.value_pad * DK;
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + ks * C::kStep) = s[ks][0];
+      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
     }
 
     // The chunk's fragments in the order of their products, read kAhead of them before: K, Q, T, K^T, P.
@@ -806,26 +831,27 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     frag kf[kRows], qf[kRows], tf[kTerms * kBlocks], pf[kTerms * kBlocks], cf[kColumns];
     const auto fetch = [&](int i) __attribute__((always_inline)) {
       if (i < kRows) {
-        kf[i] = read.operand(at, i % kTiles, i / kTiles);
+        kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
       } else if ((i -= kRows) < kRows) {
-        qf[i] = read.row(at + S::kQuery, i % kTiles, i / kTiles);
+        qf[i] = read.row(S::kQuery, i % kTiles, i / kTiles);
       } else if ((i -= kRows) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
-        tf[i] = read.operand(at + S::kSolve + i / kBlocks * C::kPanel, b.tile, b.step);
+        tf[i] = read.operand(S::kSolve + i / kBlocks * C::kPanel, b.tile, b.step);
       } else if ((i -= kTerms * kBlocks) < kColumns) {
-        cf[i] = read.column(at, i / 8 * 4 + i % 4, i / 4 % 2);
+        cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
       } else if ((i -= kColumns) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
-        pf[i] = read.row(at + S::kPairs + i / kBlocks * C::kPanel, b.tile, b.step);
+        pf[i] = pairs_read.row(i / kBlocks * C::kPanel, b.tile, b.step);
       }
     };
     constexpr int kFirstQ = kRows, kFirstT = 2 * kRows, kFirstC = kFirstT + kTerms * kBlocks,
                   kFirstP = kFirstC + kColumns;
     f32x4 v[kTiles];
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) v[m] = own.values(at + S::kValues, m);
+    for (int m = 0; m < kTiles; ++m) v[m] = own.values(at, m);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch(i);
+    keep_order();
 
     // R = beta V - (beta c rk) K S.
     Sum<T> sums[kTiles];
@@ -958,7 +984,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 // in the forward walk's form: a wave has 16 columns of D in registers. D and Y of every chunk are kept for
 // delta_gradients.
 template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_backward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
   using S = Stage<T, DK, W>;
@@ -966,7 +992,7 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
   constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
-  const Reader<T> read;
+  const Reader<T> places;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t heads = a.batch * a.heads;
   const int64_t bh = blockIdx.x % heads;
@@ -1009,8 +1035,8 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
     const unsigned dst = lds_at + (c & 1) * S::kBytes;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
-    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst, wave, rows);
-    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, wave, rows);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
+    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst, wave, rows);
     query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
     pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
     if (wave < 2) {  // the factors, and after them `whole`
@@ -1023,6 +1049,34 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
   T* out = static_cast<T*>(a.grad_value) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
   const int64_t out_token = a.heads * value_size;
   const int store_at = column + lane.g * 4, store_count = value_size - store_at;
+  const unsigned state_place = mine * DK + lane.g * (16 / sizeof(T));
+  const unsigned update_place = mine * kTokens + lane.g * (16 / sizeof(T));
+  const bool whole_rows = column + 16 <= value_size;
+  unsigned out_place[kTiles];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
+  // As in the forward a chunk's results are stored while the next one is worked on.
+  Four<T> held_value[kTiles];
+  frag held_update[2];
+  int held = -1;
+  const auto store_held = [&]() __attribute__((always_inline)) {
+    if (held < 0) return;
+    T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      if (whole_rows && (held + 1) * kTokens <= a.tokens) {
+        store_run<4>(to + out_place[n], __builtin_bit_cast(Run<T, 4>, held_value[n]));
+      } else if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < store_count) to[out_place[n] + e] = held_value[n][e];
+        end_of_part();
+      }
+    }
+    T* keep = static_cast<T*>(a.grad_updates) + (first_chunk + held) * a.value_pad * kTokens;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
+  };
   if (chunks > 0) load(chunks - 1);
 #pragma unroll 1
   for (int c = chunks - 1; c >= 0; --c) {
@@ -1030,132 +1084,179 @@ __global__ __launch_bounds__(64 * W) void delta_backward(DeltaArgs a) {
     __syncthreads();
     if (c > 0) load(c - 1);
     if (!active) continue;
+    store_held();
     const unsigned at = lds_at + (c & 1) * S::kBytes;
+    const Reader<T> read = places.moved(at), pairs_read = places.moved(at + S::kPairs);
     const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
     const float whole = factors[256];
-    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
 
     frag s[kSteps][kTerms];
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
     {
-      T* keep = static_cast<T*>(a.grad_states) + ((first_chunk + c) * a.value_pad + mine) * DK +
-                lane.g * (16 / sizeof(T));
+      T* keep = static_cast<T*>(a.grad_states) + (first_chunk + c) * a.value_pad * DK;
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + ks * C::kStep) = s[ks][0];
+      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
     }
+    // Fragments in the order of their products: K, Q^T, P^T, T^T, K^T.
+    constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
+    frag kf[kRows], qf[kColumns], pf[kTerms * kBlocks], tf[kTerms * kBlocks], cf[kColumns];
+    const auto fetch = [&](int i) __attribute__((always_inline)) {
+      if (i < kRows) {
+        kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
+      } else if ((i -= kRows) < kColumns) {
+        qf[i] = read.column(S::kQuery, i / 8 * 4 + i % 4, i / 4 % 2);
+      } else if ((i -= kColumns) < kTerms * kBlocks) {
+        const Triangle<T> b(i % kBlocks);
+        pf[i] = pairs_read.column(i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
+      } else if ((i -= kTerms * kBlocks) < kTerms * kBlocks) {
+        const Triangle<T> b(i % kBlocks);
+        tf[i] = read.column(S::kSolve + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
+      } else if ((i -= kTerms * kBlocks) < kColumns) {
+        cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
+      }
+    };
+    constexpr int kAheadBack = 6;  // of transposing reads, two instructions each
+    constexpr int kFirstQ = kRows, kFirstP = kFirstQ + kColumns, kFirstT = kFirstP + kTerms * kBlocks,
+                  kFirstC = kFirstT + kTerms * kBlocks;
     frag g[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) g[kt] = own.column(at + S::kValues, kt);
+    for (int kt = 0; kt < 2; ++kt) g[kt] = own.column(at, kt);
+#pragma unroll
+    for (int i = 0; i < kAheadBack; ++i) fetch(i);
+    keep_order();
 
-    f32x4 u[kTiles];
+    // dU = diag(e rk) K D + P^T dO.
+    Sum<T> sums[kTiles];
+#pragma unroll
+    for (int i = 0; i < kRows; i += kTiles) {
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) fetch(i + m + kAheadBack);
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) sums[m].add(kf[i + m], s[i / kTiles][term], term > 0);
+      keep_order();
+    }
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
-      Sum<T> sum;
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-        const frag k = read.operand(at, m, ks);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) sum.add(k, s[ks][term], term > 0);
-      }
       const f32x4 factor = *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
-      sum.whole *= factor;
-      sum.rest *= factor;
-#pragma unroll
-      for (int kt = m / kPer; kt < 2; ++kt)
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-          sum.add(read.column(at + S::kPairs + term * C::kPanel, m, kt), g[kt], term > 0);
-      u[m] = sum.value();
+      sums[m].whole *= factor;
+      sums[m].rest *= factor;
     }
-    frag uf[2][kTerms];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
-    f32x4 y[kTiles];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      Sum<T> sum;
-#pragma unroll
-      for (int kt = m / kPer; kt < 2; ++kt)
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          const frag t = read.column(at + S::kSolve + term * C::kPanel, m, kt);
-#pragma unroll
-          for (int other = 0; other < kTerms - term; ++other) sum.add(t, uf[kt][other], term + other > 0);
-        }
-      y[m] = sum.value();
-    }
-    {
-      T* keep = static_cast<T*>(a.grad_updates) + ((first_chunk + c) * a.value_pad + mine) * kTokens +
-                lane.g * (16 / sizeof(T));
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        frag hi[1];
-        split<T>(&y[kt * kPer], hi);
-        *reinterpret_cast<frag*>(keep + kt * C::kStep) = hi[0];
-      }
-    }
-    // dV, through this wave's part of LDS: lanes tokens, four columns each.
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      const int row = first_row<T>(m, lane.g);
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) turn[(row + e) * kTurnPitch + lane.l] = static_cast<T>(beta[e] * y[m][e]);
-    }
-    wait_own_lds();
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const int64_t t = t0 + n * 16 + lane.l;
-      const Run<T, 4> v = load_run<4>(turn + (n * 16 + lane.l) * kTurnPitch + lane.g * 4);
-      if (t < a.tokens && store_count > 0) {
-        T* p = out + t * out_token + store_at;
-        if (store_count >= 4) {
-          store_run<4>(p, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (e < store_count) p[e] = v.v[e];
-          end_of_part();
-        }
-      }
-    }
-    wait_own_lds();
-    // D.
-    frag gf[2][kTerms], yf[2][kTerms];
+    // D = c D + Q^T (c rq dO), until Y is there.
+    frag gf[2][kTerms], yf[2][kTerms], uf[2][kTerms];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       f32x4 v[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int row = first_row<T>(kt * kPer + i, lane.g);
-        const f32x4 f = *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + row);
-        const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
+        const f32x4 factor =
+            *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + first_row<T>(kt * kPer + i, lane.g));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[i][e] = f[e] * static_cast<float>(g[kt][i * 4 + e]);
-          y[kt * kPer + i][e] *= -take[e];
-        }
+        for (int e = 0; e < 4; ++e) v[i][e] = factor[e] * static_cast<float>(g[kt][i * 4 + e]);
       }
       split<T>(v, gf[kt]);
-      split<T>(&y[kt * kPer], yf[kt]);
     }
 #pragma unroll
-    for (int m = 0; m < kStateTiles; ++m) {
-      Sum<T> sum(state[m] * whole);
+    for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
+      Sum<T> part[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) part[m].whole = state[m0 + m] * whole;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const frag q = read.column(at + S::kQuery, m, kt);
-        const frag k = read.column(at, m, kt);
 #pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          sum.add(q, gf[kt][term], term > 0);
-          sum.add(k, yf[kt][term], term > 0);
-        }
+        for (int m = 0; m < 4; ++m) fetch(kFirstQ + m0 * 2 + kt * 4 + m + kAheadBack);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) part[m].add(qf[m0 * 2 + kt * 4 + m], gf[kt][term], term > 0);
+        keep_order();
       }
-      state[m] = sum.value();
+#pragma unroll
+      for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
     }
+#pragma unroll
+    for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const Triangle<T> b(i);
+        fetch(kFirstP + term * kBlocks + i + kAheadBack);
+        sums[kTiles - 1 - b.tile].add(pf[term * kBlocks + i], g[1 - b.step], term > 0);
+      }
+      keep_order();
+    }
+    f32x4 y[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      y[m] = sums[m].value();
+      sums[m] = Sum<T>();
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], uf[kt]);
+    // Y = T^T dU.
+#pragma unroll
+    for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+      for (int other = 0; other < kTerms - term; ++other)
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const Triangle<T> b(i);
+          if (other == 0) fetch(kFirstT + term * kBlocks + i + kAheadBack);
+          sums[kTiles - 1 - b.tile].add(tf[term * kBlocks + i], uf[1 - b.step][other], term + other > 0);
+        }
+      keep_order();
+    }
+    f32x4 dv[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) y[m] = sums[m].value();
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      frag hi[1];
+      split<T>(&y[kt * kPer], hi);
+      held_update[kt] = hi[0];
+    }
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      const int row = first_row<T>(m, lane.g);
+      dv[m] = y[m] * *reinterpret_cast<const f32x4*>(factors + kTokens + row);
+      y[m] *= -*reinterpret_cast<const f32x4*>(factors + row);
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], yf[kt]);
+    // D = D - K^T (beta c rk Y).
+#pragma unroll
+    for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
+      Sum<T> part[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) part[m].whole = state[m0 + m];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) fetch(kFirstC + m0 * 2 + kt * 4 + m + kAheadBack);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) part[m].add(cf[m0 * 2 + kt * 4 + m], yf[kt][term], term > 0);
+        keep_order();
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
+    }
+    // dV, through this wave's part of LDS: lanes tokens, four columns each.
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        turn[(first_row<T>(m, lane.g) + e) * kTurnPitch + lane.l] = static_cast<T>(dv[m][e]);
+    wait_own_lds();
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+      held_value[n] = *reinterpret_cast<const Four<T>*>(turn + (n * 16 + lane.l) * kTurnPitch + lane.g * 4);
+    wait_own_lds();
+    held = c;
   }
+  store_held();
   if (!active) return;
   if (a.grad_first != nullptr) {
 #pragma unroll

@@ -291,6 +291,8 @@ int check_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* p) {
       !mul_ok(total, (p->value_size + 127) * 128, &total))
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes overflow int64");
   // A row's place in a chunk is a 32-bit byte offset.
+  if (!mul_ok(p->heads, p->value_size, &extent) || extent >= int64_t{1} << 23)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule needs fewer than 2^23 values a token");
   if (p->query_token >= kMaxTokenStride || p->key_token >= kMaxTokenStride ||
       p->value_token >= kMaxTokenStride || p->grad_token >= kMaxTokenStride)
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule needs token strides below 2^21 elements");
