@@ -132,6 +132,7 @@ struct Reader {
     for (unsigned& at : r.rows) move(at);
     for (unsigned& at : r.operands) move(at);
     for (unsigned& at : r.columns) move(at);
+    for (unsigned& at : r.ordered) move(at);
     return r;
   }
 
@@ -214,6 +215,12 @@ struct Own {
         columns[x] = tile / 2 * kPanel + g * 512 + (((tile % 2 * 4 + (l >> 2)) ^ swizzle(row)) << 4) + (l & 3) * 4;
       }
     }
+  }
+  __device__ __forceinline__ Own moved(unsigned by) const {
+    Own r = *this;
+    for (unsigned& at : r.rows) at += by;
+    for (unsigned& at : r.columns) at += by;
+    return r;
   }
   __device__ __forceinline__ frag row(unsigned panels, int ks) const {
     return lds_read<frag>(panels + rows[ks % 2] + ks / 2 * kPanel);
@@ -353,11 +360,15 @@ struct PanelLoads {
       offset[j] = at < bytes ? static_cast<unsigned>(r) * stride + at : kNowhere;
     }
   }
-  // Panels that lie in memory one after another as they are.
+  // Lower triangles that lie in memory one after another, without the quarter that no fragment reaches.
   __device__ __forceinline__ explicit PanelLoads(int wave) {
 #pragma unroll
-    for (int j = 0; j < kMine; ++j)
-      offset[j] = (j * W + wave) * 1024 + (threadIdx.x & 63) / 8 * 128 + (((threadIdx.x % 8) ^ swizzle(row(j, wave))) << 4);
+    for (int j = 0; j < kMine; ++j) {
+      const int r = row(j, wave), piece = (threadIdx.x % 8) ^ swizzle(r);
+      offset[j] = r < Chunk<T>::kTokens / 2 && piece >= 4
+                      ? kNowhere
+                      : (j * W + wave) * 1024 + (threadIdx.x & 63) / 8 * 128 + (piece << 4);
+    }
   }
   __device__ __forceinline__ void load(u32x4 buffer, unsigned dst, int wave, int rows) const {
     if (rows == Chunk<T>::kTokens) {
@@ -1288,11 +1299,14 @@ template <typename T, int DK>
 struct GradientsLds {
   using C = Chunk<T>;
   static constexpr int kWide = DK / C::kTokens * C::kPanel;
-  unsigned char wide[2][kWide];         // states and their gradients, then keys and queries
-  unsigned char narrow[3][C::kPanel];   // U and Y transposed, dO; then the pairs as fragments
-  double sum[C::kTokens];
-  float beta[C::kTokens], rk[C::kTokens], rq[C::kTokens], inner[2 * C::kTiles];
-  float slope[2][C::kTokens], kept[2][C::kTokens], step[2][C::kTokens];
+  static constexpr int kRecord = (sizeof(Record<T>) + 1023) / 1024 * 1024;
+  struct Block {
+    unsigned char wide[2][kWide];        // states and their gradients
+    unsigned char narrow[3][C::kPanel];  // U and Y transposed, dO; then the pairs as fragments
+    unsigned char record[kRecord];
+  } blocks[2];
+  unsigned char keys[kWide], queries[kWide];
+  float slope[2][C::kTokens], kept[2][C::kTokens], step[2][C::kTokens], inner[2 * C::kTiles];
 };
 
 // What a wave does that makes the pairs with its tokens as rows (HALF 0) or columns (1), of the first (SIDE 0) or
@@ -1304,7 +1318,10 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kPer = C::kPer, kWaves = 2 * kTiles;
   constexpr int kPanels = DK / kTokens, kSteps = DK / C::kStep, kKeyTiles = DK / 32;  // of a wave
   constexpr int kVec = 16 / sizeof(T);
-  auto& [wide, narrow, sum, beta, rk, rq, inner, slope, kept, step] = lds;
+  auto& slope = lds.slope;
+  auto& kept = lds.kept;
+  auto& step = lds.step;
+  auto& inner = lds.inner;
   const Lane lane;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int half = HALF;
@@ -1313,9 +1330,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   constexpr bool kFlip = DK / 2 * sizeof(T) < 128;
   const Reader<T> read(kFlip ? half * 64 : 0);
   const Own<T> mine(block);
-  const unsigned wide_at = lds_address(wide[0]), narrow_at = lds_address(narrow[0]);
-  constexpr unsigned kWide = kPanels * C::kPanel;
-  const unsigned states = wide_at + (kFlip ? 0 : half * (kWide / 2)), grads = states + kWide;
+  constexpr unsigned kWide = kPanels * C::kPanel, kNarrow = 2 * kWide, kHalf = kFlip ? 0 : half * (kWide / 2);
   const int chunk = static_cast<int>(blockIdx.x % a.chunks);
   const int64_t row = blockIdx.x / a.chunks;
   const int kh = static_cast<int>(row % a.key_heads), b = static_cast<int>(row / a.key_heads);
@@ -1371,6 +1386,42 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     return HALF == 0 ? m / kPer <= SIDE : m / kPer >= SIDE;
   };
   float norm = 1.f;
+  // Blocks of values, of one head after another: the next one's operands load while one is worked on.
+  const int blocks_a_head = static_cast<int>((a.value_pad + kTokens - 1) / kTokens);
+  const auto load = [&](int i) __attribute__((always_inline)) {
+    const int h = kh * groups + i / blocks_a_head, v0 = i % blocks_a_head * kTokens;
+    const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
+    auto& to = lds.blocks[i & 1];
+    const int left = static_cast<int>(a.value_pad) - v0, v_rows = left < kTokens ? left : kTokens;
+    const int64_t v_at = at * a.value_pad + v0;
+    const T* panels[] = {static_cast<const T*>(a.states) + v_at * DK, static_cast<const T*>(a.grad_states) + v_at * DK,
+                         static_cast<const T*>(a.updates) + v_at * kTokens,
+                         static_cast<const T*>(a.grad_updates) + v_at * kTokens};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      load_panels<T>(buffer_at(panels[k]), lds_address(to.wide[k]), kPanels, 0, DK * sizeof(T), v_rows,
+                     DK * sizeof(T), wave, kWaves);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      load_panels<T>(buffer_at(panels[2 + k]), lds_address(to.narrow[k]), 1, 0, 128, v_rows, 128, wave, kWaves);
+    load_panels<T>(buffer_at(at_token<T>(a.grad_output, a.grad_strides, b, t0, h)), lds_address(to.narrow[2]), 1,
+                   static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)), rows,
+                   static_cast<unsigned>(value_size * sizeof(T)), wave, kWaves);
+    if (wave < GradientsLds<T, DK>::kRecord / 1024) {
+      const unsigned at_byte = wave * 1024 + (threadIdx.x & 63) * 16;
+      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + at), lds_address(to.record) + wave * 1024,
+                 at_byte < sizeof(Record<T>) ? at_byte : kNowhere);
+    }
+  };
+  load(0);
+  {
+    const unsigned bytes = static_cast<unsigned>(key_size * sizeof(T));
+    load_panels<T>(buffer_at(at_token<T>(a.key, a.key_strides, b, t0, kh)), lds_address(lds.keys), kPanels, 0,
+                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
+    load_panels<T>(buffer_at(at_token<T>(a.query, a.query_strides, b, t0, kh)), lds_address(lds.queries), kPanels, 0,
+                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
+  }
+  int index = 0;
 
 #pragma unroll 1
   for (int group = 0; group < groups; ++group) {
@@ -1378,8 +1429,6 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     // The compiler is not to keep what follows from a lane's place from one head to the next: registers spilled.
     int own = own_token, first = lane.g;
     if constexpr (GROUPED) asm volatile("" : "+v"(own), "+v"(first));
-    const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
-    const Record<T>* record = reinterpret_cast<const Record<T>*>(a.records) + at;
     f32x4 dq[kKeyTiles], dk[kKeyTiles], back[kKeyTiles];  // dO S^T, Y S^T, U D^T
 #pragma unroll
     for (int m = 0; m < kKeyTiles; ++m) dq[m] = dk[m] = back[m] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1388,47 +1437,32 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     for (int m = 0; m < kTiles; ++m) pair_p[m] = pair_a[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     float dbeta = 0.f, product = 0.f;
     const T* value = at_token<T>(a.value, a.value_strides, b, t0 + own, h);
+    unsigned here = 0;
 #pragma unroll 1
-    for (int v0 = 0; v0 < a.value_pad; v0 += kTokens) {
-      __syncthreads();
-      {
-        const int left = static_cast<int>(a.value_pad) - v0, v_rows = left < kTokens ? left : kTokens;
-        const int64_t v_at = at * a.value_pad + v0;
-        const T* panels[] = {static_cast<const T*>(a.states) + v_at * DK,
-                             static_cast<const T*>(a.grad_states) + v_at * DK,
-                             static_cast<const T*>(a.updates) + v_at * kTokens,
-                             static_cast<const T*>(a.grad_updates) + v_at * kTokens};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          load_panels<T>(buffer_at(panels[i]), lds_address(wide[i]), kPanels, 0, DK * sizeof(T), v_rows,
-                         DK * sizeof(T), wave, kWaves);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          load_panels<T>(buffer_at(panels[2 + i]), lds_address(narrow[i]), 1, 0, 128, v_rows, 128, wave, kWaves);
-        load_panels<T>(buffer_at(at_token<T>(a.grad_output, a.grad_strides, b, t0, h)), lds_address(narrow[2]), 1,
-                       static_cast<unsigned>(v0 * sizeof(T)),
-                       static_cast<unsigned>(a.grad_strides.token * sizeof(T)), rows,
-                       static_cast<unsigned>(value_size * sizeof(T)), wave, kWaves);
-      }
+    for (int v0 = 0; v0 < a.value_pad; v0 += kTokens, ++index) {
       wait_loads();
       __syncthreads();
+      if (index + 1 < groups * blocks_a_head) load(index + 1);
+      here = lds_address(&lds.blocks[index & 1]);
+      const Reader<T> there = read.moved(here);
+      const Own<T> own_there = mine.moved(here);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const frag g = mine.row(narrow_at + 2 * C::kPanel, kt);
-        const frag u = mine.column(narrow_at, kt);
-        const frag y = mine.column(narrow_at + C::kPanel, kt);
+        const frag g = own_there.row(kNarrow + 2 * C::kPanel, kt);
+        const frag u = own_there.column(kNarrow, kt);
+        const frag y = own_there.column(kNarrow + C::kPanel, kt);
 #pragma unroll
         for (int m = 0; m < kKeyTiles; ++m) {
-          const frag s = read.ordered_column(states, m, kt);
+          const frag s = there.ordered_column(kHalf, m, kt);
           dq[m] = Fragment<T>::mma(s, g, dq[m]);
           dk[m] = Fragment<T>::mma(s, y, dk[m]);
-          back[m] = Fragment<T>::mma(read.ordered_column(grads, m, kt), u, back[m]);
+          back[m] = Fragment<T>::mma(there.ordered_column(kWide + kHalf, m, kt), u, back[m]);
         }
         if (half == 0) {
 #pragma unroll
           for (int m = 0; m < kTiles; ++m) {
             if (!has(m)) continue;
-            const frag other = read.column(narrow_at, m, kt);
+            const frag other = there.column(kNarrow, m, kt);
             pair_p[m] = Fragment<T>::mma(other, g, pair_p[m]);
             pair_a[m] = Fragment<T>::mma(other, y, pair_a[m]);
           }
@@ -1442,41 +1476,28 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
 #pragma unroll
           for (int m = 0; m < kTiles; ++m) {
             if (!has(m)) continue;
-            pair_p[m] = Fragment<T>::mma(read.operand(narrow_at + 2 * C::kPanel, m, kt), u, pair_p[m]);
-            pair_a[m] = Fragment<T>::mma(read.column(narrow_at + C::kPanel, m, kt), u, pair_a[m]);
+            pair_p[m] = Fragment<T>::mma(there.operand(kNarrow + 2 * C::kPanel, m, kt), u, pair_p[m]);
+            pair_a[m] = Fragment<T>::mma(there.column(kNarrow + C::kPanel, m, kt), u, pair_a[m]);
           }
         }
       }
       // The state's product with its gradient.
       for (int i = threadIdx.x; i < kPanels * C::kPanel / 16; i += 64 * kWaves) {
-        const frag s = *reinterpret_cast<const frag*>(wide[0] + i * 16);
-        const frag d = *reinterpret_cast<const frag*>(wide[1] + i * 16);
+        const frag s = lds_read<frag>(here + i * 16);
+        const frag d = lds_read<frag>(here + kWide + i * 16);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) product = fmaf(static_cast<float>(s[e]), static_cast<float>(d[e]), product);
       }
     }
-    __syncthreads();
-    {
-      const unsigned bytes = static_cast<unsigned>(key_size * sizeof(T));
-      load_panels<T>(buffer_at(at_token<T>(a.key, a.key_strides, b, t0, kh)), lds_address(wide[0]), kPanels, 0,
-                     static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
-      load_panels<T>(buffer_at(at_token<T>(a.query, a.query_strides, b, t0, kh)), lds_address(wide[1]), kPanels, 0,
-                     static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
-      if (threadIdx.x < kTokens) {
-        sum[threadIdx.x] = record->sum[threadIdx.x];
-        beta[threadIdx.x] = record->beta[threadIdx.x];
-        rk[threadIdx.x] = record->rk[threadIdx.x];
-        rq[threadIdx.x] = record->rq[threadIdx.x];
-      }
-      product = lanes_sum<64>(product);
-      if ((threadIdx.x & 63) == 0) inner[wave] = product;
-    }
-    norm = record->norm[own];
-    const uint64_t closed = record->closed;
-    wait_loads();
-    __syncthreads();
-    // Of the wave's keys: `states` and `grads`.
-    const unsigned keys = wide_at, queries = wide_at + kWide;
+    product = lanes_sum<64>(product);
+    if ((threadIdx.x & 63) == 0) inner[wave] = product;
+    const auto* facts = reinterpret_cast<const Record<T>*>(lds.blocks[(index - 1) & 1].record);
+    const double* sum = facts->sum;
+    const float *beta = facts->beta, *rk = facts->rk, *rq = facts->rq;
+    norm = facts->norm[own];
+    const uint64_t closed = facts->closed;
+    const unsigned keys = lds_address(lds.keys), queries = lds_address(lds.queries);
+    const unsigned states = keys + kHalf, grads = queries + kHalf;  // of the wave's keys
     const double own_sum = sum[own];
     const float own_beta = beta[own], own_rk = rk[own], own_rq = rq[own];
 
@@ -1557,7 +1578,8 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       step[half][own] = dbeta;
     }
     // The pairs as fragments, for both waves of these tokens: three of each kind.
-    frag* shared = reinterpret_cast<frag*>(&narrow[0][0]) + block * 6 * 64 + (threadIdx.x & 63);
+    __syncthreads();  // all have read U, Y and dO
+    frag* shared = reinterpret_cast<frag*>(lds.blocks[(index - 1) & 1].narrow[0]) + block * 6 * 64 + (threadIdx.x & 63);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       if (!has(kt * kPer)) continue;
@@ -1598,7 +1620,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) s += inner[w];
-      if (t == kTokens - 1) v += k + record->whole * s;
+      if (t == kTokens - 1) v += k + facts->whole * s;
 #pragma unroll
       for (int by = 1; by < kTokens; by *= 2) {
         const float after = __shfl_down(v, by);
@@ -1658,7 +1680,8 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
 
 template <typename T, int DK, bool GROUPED>
 __global__ __launch_bounds__(Chunk<T>::kTokens * 8, 2) void delta_gradients(DeltaArgs a) {
-  __shared__ __align__(1024) GradientsLds<T, DK> lds;
+  extern __shared__ __align__(1024) unsigned char shared[];
+  auto& lds = *reinterpret_cast<GradientsLds<T, DK>*>(shared);
   constexpr int kTiles = Chunk<T>::kTiles;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool second = wave % kTiles >= kTiles / 2;
@@ -1681,7 +1704,7 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 8, 2) void delta_gradients(Delt
 // thread four of them at DK / 16 keys. One pass over the state gives S^T k and S^T q together, since
 // o = a S^T q + (k.q) u; a token costs one barrier. Bound by reading and writing the state.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_step(DeltaArgs a) {
+__global__ __launch_bounds__(256, 4) void delta_step(DeltaArgs a) {
   constexpr int kRows = DK / 16, kQuads = kDeltaStepColumns / 4;
   __shared__ float sums[2][4][kQuads][12];
   const int quad = threadIdx.x % kQuads, part = threadIdx.x / kQuads, wave = threadIdx.x >> 6;
@@ -1858,6 +1881,18 @@ hipError_t launch_forward(const DeltaArgs& a, const DeltaPlan& p, hipStream_t st
   return a.states != nullptr ? launch_walk<T, DK, 4, true>(a, stream) : launch_walk<T, DK, 4, false>(a, stream);
 }
 
+template <typename T, int DK, bool GROUPED>
+hipError_t launch_gradients(const DeltaArgs& a, hipStream_t stream) {
+  constexpr int kBytes = sizeof(GradientsLds<T, DK>);
+  const auto kernel = delta_gradients<T, DK, GROUPED>;
+  static std::atomic<uint64_t> asked{0};
+  const hipError_t err = ask_lds(kernel, kBytes, asked);
+  if (err != hipSuccess) return err;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)),
+                     dim3(Chunk<T>::kTokens * 8), kBytes, stream, a);
+  return hipGetLastError();
+}
+
 template <typename T, int DK>
 hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
   constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
@@ -1870,12 +1905,7 @@ hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(64 * W), kBytes, stream, a);
   err = hipGetLastError();
   if (err != hipSuccess || a.chunks == 0) return err;
-  const dim3 grid(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)), block(Chunk<T>::kTokens * 8);
-  if (a.heads == a.key_heads)
-    hipLaunchKernelGGL((delta_gradients<T, DK, false>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((delta_gradients<T, DK, true>), grid, block, 0, stream, a);
-  return hipGetLastError();
+  return a.heads == a.key_heads ? launch_gradients<T, DK, false>(a, stream) : launch_gradients<T, DK, true>(a, stream);
 }
 
 template <typename T>
