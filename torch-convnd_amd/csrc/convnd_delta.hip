@@ -600,7 +600,7 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = wave * 16 + g * 4 + e;
-          v[e] = i > j && open_between(closed, j, i) ? up[e] * rk[j] * decay_between(later[e], earlier) * kk[jb][e]
+          v[e] = i > j && (closed == 0 || open_between(closed, j, i)) ? up[e] * rk[j] * decay_between(later[e], earlier) * kk[jb][e]
                                                      : 0.f;
         }
         *reinterpret_cast<f32x4*>(&lds.solve.rest[j][wave * 16 + g * 4]) = v;
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = jb * 16 + g * 4 + e;
-          v[e] = i >= j && open_between(closed, j, i) ? rq[i] * rk[j] * decay_between(later, sum[j]) * qk[jb][e]
+          v[e] = i >= j && (closed == 0 || open_between(closed, j, i)) ? rq[i] * rk[j] * decay_between(later, sum[j]) * qk[jb][e]
                                                       : 0.f;
         }
 #pragma unroll
@@ -1385,6 +1385,10 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   const auto has = [](int m) __attribute__((always_inline)) {
     return HALF == 0 ? m / kPer <= SIDE : m / kPer >= SIDE;
   };
+  // Tiles of the chunk's tokens that hold partners of this wave's, and the fragments of them that a step reads.
+  constexpr int kFirstOther = HALF == 0 ? 0 : SIDE * kPer;
+  constexpr int kPartners = HALF == 0 ? (SIDE + 1) * kPer : (2 - SIDE) * kPer, kOthers = kPartners * (HALF + 1);
+  constexpr int kAheadGrad = 6;
   float norm = 1.f;
   // Blocks of values, of one head after another: the next one's operands load while one is worked on.
   const int blocks_a_head = static_cast<int>((a.value_pad + kTokens - 1) / kTokens);
@@ -1446,38 +1450,59 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       here = lds_address(&lds.blocks[index & 1]);
       const Reader<T> there = read.moved(here);
       const Own<T> own_there = mine.moved(here);
+      // Fragments in the order of their products, read kAheadGrad before them.
+      constexpr int kStep = 3 + 2 * kKeyTiles + kOthers;
+      frag of[2 * kStep];
+      const auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i >= 2 * kStep) return;
+        const int kt = i / kStep, k = i % kStep, n = k - 3 - 2 * kKeyTiles;
+        of[i] = k == 0   ? own_there.row(kNarrow + 2 * C::kPanel, kt)
+                : k == 1 ? own_there.column(kNarrow, kt)
+                : k == 2 ? own_there.column(kNarrow + C::kPanel, kt)
+                : n < 0  ? there.ordered_column((k - 3) % 2 * kWide + kHalf, (k - 3) / 2, kt)
+                : HALF == 0  ? there.column(kNarrow, kFirstOther + n, kt)
+                : n % 2 == 0 ? there.operand(kNarrow + 2 * C::kPanel, kFirstOther + n / 2, kt)
+                             : there.column(kNarrow + C::kPanel, kFirstOther + n / 2, kt);
+      };
+#pragma unroll
+      for (int i = 0; i < kAheadGrad; ++i) fetch(i);
+      keep_order();
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const frag g = own_there.row(kNarrow + 2 * C::kPanel, kt);
-        const frag u = own_there.column(kNarrow, kt);
-        const frag y = own_there.column(kNarrow + C::kPanel, kt);
+        fetch(kt * kStep + kAheadGrad);
+        fetch(kt * kStep + kAheadGrad + 1);
+        fetch(kt * kStep + kAheadGrad + 2);
+        const frag g = of[kt * kStep], u = of[kt * kStep + 1], y = of[kt * kStep + 2];
 #pragma unroll
         for (int m = 0; m < kKeyTiles; ++m) {
-          const frag s = there.ordered_column(kHalf, m, kt);
-          dq[m] = Fragment<T>::mma(s, g, dq[m]);
-          dk[m] = Fragment<T>::mma(s, y, dk[m]);
-          back[m] = Fragment<T>::mma(there.ordered_column(kWide + kHalf, m, kt), u, back[m]);
+          const int i = kt * kStep + 3 + 2 * m;
+          fetch(i + kAheadGrad);
+          fetch(i + kAheadGrad + 1);
+          dq[m] = Fragment<T>::mma(of[i], g, dq[m]);
+          dk[m] = Fragment<T>::mma(of[i], y, dk[m]);
+          back[m] = Fragment<T>::mma(of[i + 1], u, back[m]);
+          keep_order();
         }
-        if (half == 0) {
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) {
-            if (!has(m)) continue;
-            const frag other = there.column(kNarrow, m, kt);
-            pair_p[m] = Fragment<T>::mma(other, g, pair_p[m]);
-            pair_a[m] = Fragment<T>::mma(other, y, pair_a[m]);
+        for (int n = 0; n < kPartners; ++n) {
+          const int m = kFirstOther + n, i = kt * kStep + 3 + 2 * kKeyTiles + n * (HALF + 1);
+          fetch(i + kAheadGrad);
+          if constexpr (HALF == 0) {
+            pair_p[m] = Fragment<T>::mma(of[i], g, pair_p[m]);
+            pair_a[m] = Fragment<T>::mma(of[i], y, pair_a[m]);
+          } else {
+            fetch(i + kAheadGrad + 1);
+            pair_p[m] = Fragment<T>::mma(of[i], u, pair_p[m]);
+            pair_a[m] = Fragment<T>::mma(of[i + 1], u, pair_a[m]);
           }
+          keep_order();
+        }
+        if constexpr (HALF == 0) {
           const int v = v0 + kt * C::kStep + lane.g * kVec;
           if (own < rows && v < value_size) {
             const frag f = __builtin_bit_cast(frag, load_run<kVec>(value + v));
 #pragma unroll
             for (int i = 0; i < kVec; ++i) dbeta = fmaf(static_cast<float>(f[i]), static_cast<float>(y[i]), dbeta);
-          }
-        } else {
-#pragma unroll
-          for (int m = 0; m < kTiles; ++m) {
-            if (!has(m)) continue;
-            pair_p[m] = Fragment<T>::mma(there.operand(kNarrow + 2 * C::kPanel, m, kt), u, pair_p[m]);
-            pair_a[m] = Fragment<T>::mma(there.column(kNarrow + C::kPanel, m, kt), u, pair_a[m]);
           }
         }
       }
@@ -1531,18 +1556,50 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     f32x4 kk[kTiles], qk[kTiles];
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) kk[m] = qk[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    {
+      constexpr int kStep = 2 + kOthers;
+      frag of[kSteps * kStep];
+      const auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i >= kSteps * kStep) return;
+        const int ks = i / kStep, k = i % kStep, n = k - 2;
+        of[i] = k == 0       ? mine.row(keys, ks)
+                : k == 1     ? mine.row(queries, ks)
+                : HALF == 0  ? read.operand(keys, kFirstOther + n, ks)
+                : n % 2 == 0 ? read.operand(keys, kFirstOther + n / 2, ks)
+                             : read.operand(queries, kFirstOther + n / 2, ks);
+      };
 #pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) {
-      const frag k = mine.row(keys, ks), q = mine.row(queries, ks);
+      for (int i = 0; i < kAheadGrad; ++i) fetch(i);
+      keep_order();
 #pragma unroll
-      for (int m = 0; m < kTiles; ++m) {
-        if (!has(m)) continue;
-        const frag other = read.operand(keys, m, ks);
-        kk[m] = Fragment<T>::mma(other, k, kk[m]);
-        if (half == 0)
-          qk[m] = Fragment<T>::mma(other, q, qk[m]);
-        else
-          qk[m] = Fragment<T>::mma(read.operand(queries, m, ks), k, qk[m]);
+      for (int ks = 0; ks < kSteps; ++ks) {
+        fetch(ks * kStep + kAheadGrad);
+        fetch(ks * kStep + kAheadGrad + 1);
+        const frag k = of[ks * kStep], q = of[ks * kStep + 1];
+#pragma unroll
+        for (int n = 0; n < kPartners; ++n) {
+          const int m = kFirstOther + n, i = ks * kStep + 2 + n * (HALF + 1);
+          fetch(i + kAheadGrad);
+          kk[m] = Fragment<T>::mma(of[i], k, kk[m]);
+          if constexpr (HALF == 0) {
+            qk[m] = Fragment<T>::mma(of[i], q, qk[m]);
+          } else {
+            fetch(i + kAheadGrad + 1);
+            qk[m] = Fragment<T>::mma(of[i + 1], k, qk[m]);
+          }
+          keep_order();
+        }
+      }
+    }
+    // Which pairs no closed gate parts: a bit each.
+    unsigned open_bits = ~0u;
+    if (closed != 0) {
+      open_bits = 0;
+#pragma unroll
+      for (int n = 0; n < 4 * kTiles; ++n) {
+        const int other = first_row<T>(n / 4, first) + n % 4;
+        const int i = half == 0 ? own : other, j = half == 0 ? other : own;
+        if (j <= i && open_between(closed, j, i)) open_bits |= 1u << n;
       }
     }
     float pairs = 0.f, steps = 0.f;
@@ -1553,7 +1610,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       for (int e = 0; e < 4; ++e) {
         const int other = first_row<T>(m, first) + e;
         const int i = half == 0 ? own : other, j = half == 0 ? other : own;
-        const bool open = i >= j && open_between(closed, j < i ? j : i, i);
+        const bool open = i >= j && (open_bits >> (m * 4 + e) & 1) != 0;
         const float ratio = open ? half == 0 ? decay_between(own_sum, sum[other]) : decay_between(sum[other], own_sum) : 0.f;
         // The other token's factors; this one's are taken out of the sums.
         const float p = open ? ratio * (half == 0 ? rk[other] : rq[other]) * pair_p[m][e] : 0.f;
@@ -1590,21 +1647,43 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       shared[(kt + half) * 128 + 64] = f[0];
     }
     __syncthreads();
+    {
+      // k for rows and columns, q for columns of the first (SIDE 0) or the second fragment of tokens and on.
+      frag of[4 * kKeyTiles];
+      const auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i >= 4 * kKeyTiles) return;
+        const int kt = i / (2 * kKeyTiles), m = i % (2 * kKeyTiles) / 2;
+        if (i % 2 == 0)
+          of[i] = read.ordered_column(states, m, kt);
+        else if (kt >= SIDE)
+          of[i] = read.ordered_column(grads, m, kt);
+      };
+      frag weights[2][4];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const bool as_row = kt <= SIDE, as_column = kt >= SIDE;
-      const frag row_p = shared[kt * 128], row_a = shared[kt * 128 + 64];
-      const frag column_p = shared[(kt + 1) * 128], column_a = shared[(kt + 1) * 128 + 64];
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int m = 0; m < kKeyTiles; ++m) {
-        const frag k = read.ordered_column(states, m, kt);
-        if (as_row) {
-          dq[m] = Fragment<T>::mma(k, row_p, dq[m]);
-          dk[m] = Fragment<T>::mma(k, row_a, dk[m]);
-        }
-        if (as_column) {
-          dk[m] = Fragment<T>::mma(k, column_a, dk[m]);
-          dk[m] = Fragment<T>::mma(read.ordered_column(grads, m, kt), column_p, dk[m]);
+        for (int w = 0; w < 4; ++w)
+          if (w < 2 ? kt <= SIDE : kt >= SIDE) weights[kt][w] = shared[(kt + w / 2) * 128 + w % 2 * 64];
+#pragma unroll
+      for (int i = 0; i < kAheadGrad; ++i) fetch(i);
+      keep_order();
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const bool as_row = kt <= SIDE, as_column = kt >= SIDE;
+#pragma unroll
+        for (int m = 0; m < kKeyTiles; ++m) {
+          const int i = (kt * kKeyTiles + m) * 2;
+          fetch(i + kAheadGrad);
+          fetch(i + kAheadGrad + 1);
+          if (as_row) {
+            dq[m] = Fragment<T>::mma(of[i], weights[kt][0], dq[m]);
+            dk[m] = Fragment<T>::mma(of[i], weights[kt][1], dk[m]);
+          }
+          if (as_column) {
+            dk[m] = Fragment<T>::mma(of[i], weights[kt][3], dk[m]);
+            dk[m] = Fragment<T>::mma(of[i + 1], weights[kt][2], dk[m]);
+          }
+          keep_order();
         }
       }
     }
