@@ -469,9 +469,10 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
   __shared__ double sum[kTokens];
   const Lane lane;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunk = static_cast<int>(blockIdx.x % a.chunks);
-  const int64_t row = blockIdx.x / a.chunks;
-  const int kh = static_cast<int>(row % a.key_heads), b = static_cast<int>(row / a.key_heads);
+  const unsigned row = blockIdx.x / static_cast<unsigned>(a.chunks);
+  const int chunk = static_cast<int>(blockIdx.x - row * static_cast<unsigned>(a.chunks));
+  const int b = static_cast<int>(row / static_cast<unsigned>(a.key_heads));
+  const int kh = static_cast<int>(row) - b * static_cast<int>(a.key_heads);
   const int length = length_of(a, b), t0 = chunk * kTokens;
   if (t0 >= length) return;
   const int rows = length - t0 < kTokens ? length - t0 : kTokens;
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
       qk[j] = Fragment<T>::mma(k, own_q, qk[j]);  // registers columns, lanes rows of this wave
     }
   }
-  const int groups = static_cast<int>(a.heads / a.key_heads);
+  const int groups = a.groups;
   for (int group = 0; group < groups; ++group) {
     const int h = kh * groups + group;
     int l = lane.l, g = lane.g;
@@ -732,11 +733,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups of a head's columns are a whole number of heads apart: where that is a multiple of eight
   // they run on one XCD and share its L2.
-  const int64_t heads = a.batch * a.heads;
-  const int64_t bh = blockIdx.x % heads;
-  const int b = static_cast<int>(bh / a.heads), h = static_cast<int>(bh % a.heads);
-  const int kh = h / static_cast<int>(a.heads / a.key_heads);
-  const int v0 = static_cast<int>(blockIdx.x / heads) * W * 16;
+  const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
+  const int64_t bh = blockIdx.x - tile * heads;
+  const int b = static_cast<int>(static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads));
+  const int h = static_cast<int>(bh) - b * static_cast<int>(a.heads);
+  const int kh = h / a.groups;
+  const int v0 = static_cast<int>(tile) * W * 16;
   const int column = v0 + wave * 16;  // of the wave
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
   const bool active = column < value_size;
@@ -1005,11 +1007,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const Lane lane;
   const Reader<T> places;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t heads = a.batch * a.heads;
-  const int64_t bh = blockIdx.x % heads;
-  const int b = static_cast<int>(bh / a.heads), h = static_cast<int>(bh % a.heads);
-  const int kh = h / static_cast<int>(a.heads / a.key_heads);
-  const int v0 = static_cast<int>(blockIdx.x / heads) * W * 16;
+  const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
+  const int64_t bh = blockIdx.x - tile * heads;
+  const int b = static_cast<int>(static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads));
+  const int h = static_cast<int>(bh) - b * static_cast<int>(a.heads);
+  const int kh = h / a.groups;
+  const int v0 = static_cast<int>(tile) * W * 16;
   const int column = v0 + wave * 16;
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
   const bool active = column < value_size;
@@ -1331,46 +1334,52 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   const Reader<T> read(kFlip ? half * 64 : 0);
   const Own<T> mine(block);
   constexpr unsigned kWide = kPanels * C::kPanel, kNarrow = 2 * kWide, kHalf = kFlip ? 0 : half * (kWide / 2);
-  const int chunk = static_cast<int>(blockIdx.x % a.chunks);
-  const int64_t row = blockIdx.x / a.chunks;
-  const int kh = static_cast<int>(row % a.key_heads), b = static_cast<int>(row / a.key_heads);
-  const int length = length_of(a, b), t0 = chunk * kTokens;
-  const int groups = GROUPED ? static_cast<int>(a.heads / a.key_heads) : 1;
+  const int groups = GROUPED ? a.groups : 1;
   const int own_token = block * 16 + lane.l;  // this lane's in the chunk
-  const int64_t token = static_cast<int64_t>(b) * a.tokens + t0 + own_token;
-  const bool in_range = t0 + own_token < a.tokens;
   const int key_size = static_cast<int>(a.key_size), value_size = static_cast<int>(a.value_size);
   const int first_key = half * (DK / 2) + lane.g * 4;  // of the lane's four in the wave's first tile
-  T* dq_out = static_cast<T*>(a.grad_query) + (token * a.key_heads + kh) * key_size;
-  T* dk_out = static_cast<T*>(a.grad_key) + (token * a.key_heads + kh) * key_size;
   const auto store_gate = [&](void* p, int64_t at, float v) __attribute__((always_inline)) {
     if (a.float_gates)
       static_cast<float*>(p)[at] = v;
     else
       static_cast<T*>(p)[at] = static_cast<T>(v);
   };
-  if (t0 >= length) {
-    if (!in_range) return;
-#pragma unroll
-    for (int m = 0; m < kKeyTiles; ++m) {
-      const int d = first_key + m * 16;
-      if (d >= key_size) continue;
-      store_four(dq_out + d, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
-      store_four(dk_out + d, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
-    }
-    if (lane.g == 0 && half == 0)
-      for (int group = 0; group < groups; ++group) {
-        store_gate(a.grad_decay, token * a.heads + kh * groups + group, 0.f);
-        store_gate(a.grad_beta, token * a.heads + kh * groups + group, 0.f);
+  // A key head's chunk. One past its sequence's length has only zeros to be written.
+  struct Item {
+    unsigned id;
+    int chunk, kh, b, t0, rows;
+  };
+  const unsigned key_heads = static_cast<unsigned>(a.key_heads), chunks = static_cast<unsigned>(a.chunks);
+  const unsigned items = static_cast<unsigned>(a.batch) * key_heads * chunks;
+  const auto item_from = [&](unsigned id) __attribute__((always_inline)) {
+    Item it{id, 0, 0, 0, 0, 0};
+    for (; it.id < items; it.id += gridDim.x) {
+      const unsigned row = it.id / chunks, sequence = row / key_heads;
+      it.chunk = static_cast<int>(it.id - row * chunks);
+      it.kh = static_cast<int>(row - sequence * key_heads);
+      it.b = static_cast<int>(sequence);
+      it.t0 = it.chunk * kTokens;
+      const int left = length_of(a, it.b) - it.t0;
+      it.rows = left < kTokens ? left : kTokens;
+      if (left > 0) break;
+      if (it.t0 + own_token >= a.tokens) continue;
+      const int64_t token = static_cast<int64_t>(it.b) * a.tokens + it.t0 + own_token;
+#pragma unroll 1
+      for (int m = 0; m < kKeyTiles; ++m) {
+        const int d = first_key + m * 16;
+        if (d >= key_size) continue;
+        const int64_t to = (token * a.key_heads + it.kh) * key_size + d;
+        store_four(static_cast<T*>(a.grad_query) + to, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
+        store_four(static_cast<T*>(a.grad_key) + to, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
       }
-    return;
-  }
-  const int rows = length - t0 < kTokens ? length - t0 : kTokens;
-  f32x4 dq_all[GROUPED ? kKeyTiles : 1], dk_all[GROUPED ? kKeyTiles : 1];
-  if constexpr (GROUPED) {
-#pragma unroll
-    for (int m = 0; m < kKeyTiles; ++m) dq_all[m] = dk_all[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+      if (lane.g == 0 && half == 0)
+        for (int group = 0; group < groups; ++group) {
+          store_gate(a.grad_decay, token * a.heads + it.kh * groups + group, 0.f);
+          store_gate(a.grad_beta, token * a.heads + it.kh * groups + group, 0.f);
+        }
+    }
+    return it;
+  };
   // Four neighbouring values of this lane's row, in the wave's tile m.
   const auto own_values = [&](unsigned panels, int m) __attribute__((always_inline)) {
     if constexpr (kFlip) return half == 0 ? mine.four(panels, m) : mine.four(panels, m + kKeyTiles);
@@ -1389,50 +1398,72 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   constexpr int kFirstOther = HALF == 0 ? 0 : SIDE * kPer;
   constexpr int kPartners = HALF == 0 ? (SIDE + 1) * kPer : (2 - SIDE) * kPer, kOthers = kPartners * (HALF + 1);
   constexpr int kAheadGrad = 6;
-  float norm = 1.f;
-  // Blocks of values, of one head after another: the next one's operands load while one is worked on.
-  const int blocks_a_head = static_cast<int>((a.value_pad + kTokens - 1) / kTokens);
-  const auto load = [&](int i) __attribute__((always_inline)) {
-    const int h = kh * groups + i / blocks_a_head, v0 = i % blocks_a_head * kTokens;
-    const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.chunks + chunk;
-    auto& to = lds.blocks[i & 1];
+  // Blocks of values, of one head after another and one item after another: the next one's operands load while
+  // one is worked on.
+  // Every wave loads 8 rows of each panel.
+  static_assert(kWaves == kTokens / 8, "a load a wave");
+  const int load_row = wave * 8 + (threadIdx.x & 63) / 8;
+  const unsigned load_piece = ((threadIdx.x % 8) ^ swizzle(load_row)) << 4;
+  const auto load_set = [&](const void* from, unsigned dst, int count, unsigned column, unsigned stride, int rows,
+                            unsigned bytes) __attribute__((always_inline)) {
+    const u32x4 buffer = buffer_at(from);
+    const unsigned at = load_row < rows ? load_row * stride : kNowhere;
+#pragma unroll
+    for (int p = 0; p < count; ++p) {
+      const unsigned in_row = column + p * 128 + load_piece;
+      load_lds16(buffer, dst + p * C::kPanel + wave * 1024, in_row < bytes ? at + in_row : kNowhere);
+    }
+  };
+  const auto load = [&](const Item& it, int group, int v0, int into) __attribute__((always_inline)) {
+    const int h = it.kh * groups + group;
+    const int64_t at = (static_cast<int64_t>(it.b) * a.heads + h) * chunks + it.chunk;
+    auto& to = lds.blocks[into & 1];
     const int left = static_cast<int>(a.value_pad) - v0, v_rows = left < kTokens ? left : kTokens;
     const int64_t v_at = at * a.value_pad + v0;
-    const T* panels[] = {static_cast<const T*>(a.states) + v_at * DK, static_cast<const T*>(a.grad_states) + v_at * DK,
-                         static_cast<const T*>(a.updates) + v_at * kTokens,
-                         static_cast<const T*>(a.grad_updates) + v_at * kTokens};
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      load_panels<T>(buffer_at(panels[k]), lds_address(to.wide[k]), kPanels, 0, DK * sizeof(T), v_rows,
-                     DK * sizeof(T), wave, kWaves);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      load_panels<T>(buffer_at(panels[2 + k]), lds_address(to.narrow[k]), 1, 0, 128, v_rows, 128, wave, kWaves);
-    load_panels<T>(buffer_at(at_token<T>(a.grad_output, a.grad_strides, b, t0, h)), lds_address(to.narrow[2]), 1,
-                   static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)), rows,
-                   static_cast<unsigned>(value_size * sizeof(T)), wave, kWaves);
+    load_set(static_cast<const T*>(a.states) + v_at * DK, lds_address(to.wide[0]), kPanels, 0, DK * sizeof(T), v_rows,
+             DK * sizeof(T));
+    load_set(static_cast<const T*>(a.grad_states) + v_at * DK, lds_address(to.wide[1]), kPanels, 0, DK * sizeof(T),
+             v_rows, DK * sizeof(T));
+    load_set(static_cast<const T*>(a.updates) + v_at * kTokens, lds_address(to.narrow[0]), 1, 0, 128, v_rows, 128);
+    load_set(static_cast<const T*>(a.grad_updates) + v_at * kTokens, lds_address(to.narrow[1]), 1, 0, 128, v_rows, 128);
+    load_set(at_token<T>(a.grad_output, a.grad_strides, it.b, it.t0, h), lds_address(to.narrow[2]), 1,
+             static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)), it.rows,
+             static_cast<unsigned>(value_size * sizeof(T)));
     if (wave < GradientsLds<T, DK>::kRecord / 1024) {
       const unsigned at_byte = wave * 1024 + (threadIdx.x & 63) * 16;
       load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + at), lds_address(to.record) + wave * 1024,
                  at_byte < sizeof(Record<T>) ? at_byte : kNowhere);
     }
   };
-  load(0);
-  {
+  const auto load_keys = [&](const Item& it) __attribute__((always_inline)) {
     const unsigned bytes = static_cast<unsigned>(key_size * sizeof(T));
-    load_panels<T>(buffer_at(at_token<T>(a.key, a.key_strides, b, t0, kh)), lds_address(lds.keys), kPanels, 0,
-                   static_cast<unsigned>(a.key_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
-    load_panels<T>(buffer_at(at_token<T>(a.query, a.query_strides, b, t0, kh)), lds_address(lds.queries), kPanels, 0,
-                   static_cast<unsigned>(a.query_strides.token * sizeof(T)), rows, bytes, wave, kWaves);
-  }
-  int index = 0;
-
+    load_set(at_token<T>(a.key, a.key_strides, it.b, it.t0, it.kh), lds_address(lds.keys), kPanels, 0,
+             static_cast<unsigned>(a.key_strides.token * sizeof(T)), it.rows, bytes);
+    load_set(at_token<T>(a.query, a.query_strides, it.b, it.t0, it.kh), lds_address(lds.queries), kPanels, 0,
+             static_cast<unsigned>(a.query_strides.token * sizeof(T)), it.rows, bytes);
+  };
+  int index = 0;  // of the block, over all items
+  Item it = item_from(blockIdx.x);
+  if (it.id < items) load(it, 0, 0, 0);
+#pragma unroll 1
+  while (it.id < items) {
+    const Item next = item_from(it.id + gridDim.x);
+    const int t0 = it.t0, kh = it.kh, b = it.b, rows = it.rows;
+    const int64_t token = static_cast<int64_t>(b) * a.tokens + t0 + own_token;
+    const bool in_range = t0 + own_token < a.tokens;
+    T* dq_out = static_cast<T*>(a.grad_query) + (token * a.key_heads + kh) * key_size;
+    T* dk_out = static_cast<T*>(a.grad_key) + (token * a.key_heads + kh) * key_size;
+    f32x4 dq_all[GROUPED ? kKeyTiles : 1], dk_all[GROUPED ? kKeyTiles : 1];
+    if constexpr (GROUPED) {
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) dq_all[m] = dk_all[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll 1
   for (int group = 0; group < groups; ++group) {
     const int h = kh * groups + group;
-    // The compiler is not to keep what follows from a lane's place from one head to the next: registers spilled.
+    // The compiler is not to keep what follows from a lane's place from one chunk to the next: registers spilled.
     int own = own_token, first = lane.g;
-    if constexpr (GROUPED) asm volatile("" : "+v"(own), "+v"(first));
+    asm volatile("" : "+v"(own), "+v"(first));
     f32x4 dq[kKeyTiles], dk[kKeyTiles], back[kKeyTiles];  // dO S^T, Y S^T, U D^T
 #pragma unroll
     for (int m = 0; m < kKeyTiles; ++m) dq[m] = dk[m] = back[m] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1446,7 +1477,13 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     for (int v0 = 0; v0 < a.value_pad; v0 += kTokens, ++index) {
       wait_loads();
       __syncthreads();
-      if (index + 1 < groups * blocks_a_head) load(index + 1);
+      if (group == 0 && v0 == 0) load_keys(it);
+      if (v0 + kTokens < a.value_pad)
+        load(it, group, v0 + kTokens, index + 1);
+      else if (group + 1 < groups)
+        load(it, group + 1, 0, index + 1);
+      else if (next.id < items)
+        load(next, 0, 0, index + 1);
       here = lds_address(&lds.blocks[index & 1]);
       const Reader<T> there = read.moved(here);
       const Own<T> own_there = mine.moved(here);
@@ -1514,12 +1551,16 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         for (int e = 0; e < kVec; ++e) product = fmaf(static_cast<float>(s[e]), static_cast<float>(d[e]), product);
       }
     }
+    if (group == 0 && a.value_pad <= kTokens) {  // the keys are under way still
+      wait_loads();
+      __syncthreads();
+    }
     product = lanes_sum<64>(product);
     if ((threadIdx.x & 63) == 0) inner[wave] = product;
     const auto* facts = reinterpret_cast<const Record<T>*>(lds.blocks[(index - 1) & 1].record);
     const double* sum = facts->sum;
     const float *beta = facts->beta, *rk = facts->rk, *rq = facts->rq;
-    norm = facts->norm[own];
+    const float norm = facts->norm[own];
     const uint64_t closed = facts->closed;
     const unsigned keys = lds_address(lds.keys), queries = lds_address(lds.queries);
     const unsigned states = keys + kHalf, grads = queries + kHalf;  // of the wave's keys
@@ -1755,6 +1796,8 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       }
     }
   }
+    it = next;
+  }
 }
 
 template <typename T, int DK, bool GROUPED>
@@ -1787,12 +1830,13 @@ __global__ __launch_bounds__(256, 4) void delta_step(DeltaArgs a) {
   constexpr int kRows = DK / 16, kQuads = kDeltaStepColumns / 4;
   __shared__ float sums[2][4][kQuads][12];
   const int quad = threadIdx.x % kQuads, part = threadIdx.x / kQuads, wave = threadIdx.x >> 6;
-  const int64_t heads = a.batch * a.heads;
-  const int64_t bh = blockIdx.x % heads;
-  const int b = static_cast<int>(bh / a.heads), h = static_cast<int>(bh % a.heads);
-  const int kh = h / static_cast<int>(a.heads / a.key_heads);
+  const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
+  const int64_t bh = blockIdx.x - tile * heads;
+  const int b = static_cast<int>(static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads));
+  const int h = static_cast<int>(bh) - b * static_cast<int>(a.heads);
+  const int kh = h / a.groups;
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
-  const int v0 = static_cast<int>(blockIdx.x / heads) * kDeltaStepColumns + quad * 4;
+  const int v0 = static_cast<int>(tile) * kDeltaStepColumns + quad * 4;
   const int count = value_size - v0;  // columns of this thread, of four
   const int length = length_of(a, b);
   f32x4 state[kRows];
@@ -1967,7 +2011,9 @@ hipError_t launch_gradients(const DeltaArgs& a, hipStream_t stream) {
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.key_heads * a.chunks)),
+  // As many workgroups as run side by side, each with one chunk after another.
+  const int64_t items = a.batch * a.key_heads * a.chunks;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(items, 256 * (163840 / kBytes)))),
                      dim3(Chunk<T>::kTokens * 8), kBytes, stream, a);
   return hipGetLastError();
 }

@@ -697,6 +697,7 @@ struct DeltaArgs {
   int64_t value_pad;          // value_size in whole 16
   DeltaStrides query_strides, key_strides, value_strides, decay_strides, beta_strides, grad_strides;
   float scale;
+  int groups;                 // value heads a key head
   int normalize;
   int float_gates;            // decay and beta are float, else of the element type
   int wide_lengths;           // lengths are int64

@@ -310,6 +310,7 @@ DeltaArgs to_args(convnd_hip_dtype dtype, const convnd_hip_delta_problem& p) {
   const int64_t chunk = delta_chunk(size_of(dtype));
   a.chunks = (p.tokens + chunk - 1) / chunk;
   a.value_pad = (p.value_size + 15) / 16 * 16;
+  a.groups = static_cast<int>(p.heads / p.key_heads);
   a.query_strides = {p.query_batch, p.query_token, p.query_head};
   a.key_strides = {p.key_batch, p.key_token, p.key_head};
   a.value_strides = {p.value_batch, p.value_token, p.value_head};
