@@ -81,6 +81,22 @@ def test_many_chunks(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(
+    ("batch", "heads", "key_size", "value_size"), [(1, 1, 64, 64), (3, 2, 40, 20), (2, 4, 128, 100), (1, 3, 100, 130)]
+)
+def test_segments(batch, heads, key_size, value_size, dtype):
+    """Few heads and many tokens: segments of the tokens side by side, some of them past a sequence's end."""
+    data = make_delta(batch, 1030, 1, heads, key_size, value_size, dtype)
+    data[3][:, 700] = -float("inf")
+    lengths = torch.tensor([1030, 300, 0][:batch])
+    got = check(data, lengths)
+    got = check(data, state=False)
+    again = check(data, state=False)
+    for a, b in zip(got, again):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
 @pytest.mark.parametrize("tokens", [1, 7, 64, 150])
 def test_lengths(tokens, kind, dtype):

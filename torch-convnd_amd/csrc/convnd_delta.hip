@@ -702,6 +702,27 @@ struct Stage {
   static_assert(W * 16 % C::kTokens == 0, "whole panels of values");
 };
 
+// Where a workgroup of a walk is: `columns` values of a head (or columns of the unit matrix) and a segment of its
+// chunks. Workgroups of a head are a whole number of heads apart: where that is a multiple of eight they run on
+// one XCD and share its L2.
+struct WalkPlace {
+  int64_t bh;
+  int b, h, kh, v0, segment;
+  bool unit;
+  __device__ __forceinline__ WalkPlace(const DeltaArgs& a, int columns, int units) {
+    const unsigned heads = static_cast<unsigned>(a.batch * a.heads), group = blockIdx.x / heads;
+    bh = blockIdx.x - group * heads;
+    b = static_cast<int>(static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads));
+    h = static_cast<int>(bh) - b * static_cast<int>(a.heads);
+    kh = h / a.groups;
+    const int tiles = (static_cast<int>(a.value_size) + columns - 1) / columns, all = tiles + units / columns;
+    segment = static_cast<int>(group) / all;
+    const int tile = static_cast<int>(group) - segment * all;
+    unit = tile >= tiles;
+    v0 = (unit ? tile - tiles : tile) * columns;
+  }
+};
+
 // Block i of a lower triangle of tiles by steps of a fragment, its first steps before its second ones.
 template <typename T>
 struct Triangle {
@@ -720,7 +741,7 @@ constexpr int kAhead = 10;  // of the 15 that may be under way
 // operand straight from the results before (operand_row puts them in order) and the shared panels as the
 // other, from LDS, so waves meet only where panels change hands, once a chunk. The next chunk's panels
 // load meanwhile.
-template <typename T, int DK, int W, bool KEEP>
+template <typename T, int DK, int W, bool KEEP, bool TRANSIT>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_forward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
@@ -731,21 +752,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const Lane lane;
   const Reader<T> places;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups of a head's columns are a whole number of heads apart: where that is a multiple of eight
-  // they run on one XCD and share its L2.
-  const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
-  const int64_t bh = blockIdx.x - tile * heads;
-  const int b = static_cast<int>(static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads));
-  const int h = static_cast<int>(bh) - b * static_cast<int>(a.heads);
-  const int kh = h / a.groups;
-  const int v0 = static_cast<int>(tile) * W * 16;
-  const int column = v0 + wave * 16;  // of the wave
+  const WalkPlace w(a, W * 16, TRANSIT ? DK : 0);
+  const int64_t bh = w.bh;
+  const int b = w.b, h = w.h, kh = w.kh;
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
-  const bool active = column < value_size;
+  const int v0 = w.v0, column = v0 + wave * 16;  // of the workgroup and the wave
+  const bool active = TRANSIT && w.unit ? true : column < value_size;
   const int mine = column + lane.l;
   const int length = length_of(a, b);
-  const int chunks = (length + kTokens - 1) / kTokens;
-  const int64_t first_chunk = bh * a.chunks;
+  const int all_chunks = (length + kTokens - 1) / kTokens;
+  const int begin = w.segment * a.segment_chunks;
+  const int end = all_chunks < begin + a.segment_chunks ? all_chunks : begin + a.segment_chunks;
+  const int64_t first_chunk = bh * a.chunks, segment_at = bh * a.segments + w.segment;
 
   f32x4 state[kStateTiles];
 #pragma unroll
@@ -753,9 +771,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = first_row<T>(m, lane.g) + e;
-      state[m][e] = a.first != nullptr && d < key_size && mine < value_size
-                        ? a.first[(bh * key_size + d) * value_size + mine]
-                        : 0.f;
+      if constexpr (TRANSIT)
+        state[m][e] = w.unit && d == mine ? 1.f : 0.f;
+      else if (a.segments > 1)
+        state[m][e] = active ? a.starts[(segment_at * DK + d) * a.value_pad + mine] : 0.f;
+      else
+        state[m][e] = a.first != nullptr && d < key_size && mine < value_size
+                          ? a.first[(bh * key_size + d) * value_size + mine]
+                          : 0.f;
     }
 
   const Own<T> own(wave);
@@ -768,15 +791,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
   const PanelLoads<T, S::kValuePanels, W> value_loads(
       static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
-      static_cast<unsigned>(value_size * sizeof(T)), wave);
-  const PanelLoads<T, 2 * kTerms, W> pair_loads(wave);
+      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
+  const PanelLoads<T, (TRANSIT ? 1 : 2) * kTerms, W> pair_loads(wave);
   auto load = [&](int c) __attribute__((always_inline)) {
     const unsigned dst = lds_at + (c & 1) * S::kBytes;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
     key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
     value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst, wave, rows);
-    query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
+    if constexpr (!TRANSIT) query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
     pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
     if (wave < 2) {  // the factors, and after them `whole`
       const unsigned at = wave * 16 * kTokens + (threadIdx.x & 63) * 16;
@@ -816,14 +839,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
       for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
     }
   };
-  if (chunks > 0) load(0);
+  if (begin < end) load(begin);
 #pragma unroll 1
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = begin; c < end; ++c) {
     wait_loads();
     __syncthreads();
-    if (c + 1 < chunks) load(c + 1);
+    if (c + 1 < end) load(c + 1);
     if (!active) continue;
-    store_held();
+    if constexpr (!TRANSIT) store_held();
     const unsigned at = lds_at + (c & 1) * S::kBytes;
     const Reader<T> read = places.moved(at), pairs_read = places.moved(at + S::kPairs);
     const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
@@ -841,23 +864,24 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     // The chunk's fragments in the order of their products, read kAhead of them before: K, Q, T, K^T, P.
     // Neighbouring products are of different sums, since one waits for the last of its own sum.
     constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
+    constexpr int kQueries = TRANSIT ? 0 : kRows;
     frag kf[kRows], qf[kRows], tf[kTerms * kBlocks], pf[kTerms * kBlocks], cf[kColumns];
     const auto fetch = [&](int i) __attribute__((always_inline)) {
       if (i < kRows) {
         kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
-      } else if ((i -= kRows) < kRows) {
+      } else if ((i -= kRows) < kQueries) {
         qf[i] = read.row(S::kQuery, i % kTiles, i / kTiles);
-      } else if ((i -= kRows) < kTerms * kBlocks) {
+      } else if ((i -= kQueries) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
         tf[i] = read.operand(S::kSolve + i / kBlocks * C::kPanel, b.tile, b.step);
       } else if ((i -= kTerms * kBlocks) < kColumns) {
         cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
-      } else if ((i -= kColumns) < kTerms * kBlocks) {
+      } else if (!TRANSIT && (i -= kColumns) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
         pf[i] = pairs_read.row(i / kBlocks * C::kPanel, b.tile, b.step);
       }
     };
-    constexpr int kFirstQ = kRows, kFirstT = 2 * kRows, kFirstC = kFirstT + kTerms * kBlocks,
+    constexpr int kFirstQ = kRows, kFirstT = kRows + kQueries, kFirstC = kFirstT + kTerms * kBlocks,
                   kFirstP = kFirstC + kColumns;
     f32x4 v[kTiles];
 #pragma unroll
@@ -893,7 +917,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     Sum<T> o[kTiles];
     frag rf[2][kTerms], uf[2][kTerms], df[2][kTerms];
 #pragma unroll
-    for (int i = 0; i < kRows; i += kTiles) {
+    for (int i = 0; i < kQueries; i += kTiles) {
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) fetch(kFirstQ + i + n + kAhead);
 #pragma unroll
@@ -927,8 +951,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     f32x4 u[kTiles];
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) u[m] = sums[m].value();
+    if constexpr (!TRANSIT) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
+      for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
+    }
     // S = c S + K^T (e rk U).
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
@@ -952,6 +978,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
       for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
     }
+    if constexpr (TRANSIT) continue;
     // O = c rq Q S + P U.
 #pragma unroll
     for (int term = 0; term < kTerms; ++term) {
@@ -973,18 +1000,115 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     }
     held = c;
   }
-  store_held();
+  if constexpr (!TRANSIT) store_held();
   if (!active) return;
+  if (TRANSIT || a.segments == 1) {
 #pragma unroll
-  for (int m = 0; m < kStateTiles; ++m)
+    for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = first_row<T>(m, lane.g) + e;
+        if constexpr (TRANSIT) {
+          if (w.unit)
+            a.transits[(segment_at * DK + d) * DK + mine] = state[m][e];
+          else
+            a.partials[(segment_at * DK + d) * a.value_pad + mine] = state[m][e];
+        } else if (d < key_size && mine < value_size) {
+          a.last[(bh * key_size + d) * value_size + mine] = state[m][e];
+        }
+      }
+  }
+  if constexpr (TRANSIT) return;
+  // Tokens past the last chunk give zeros.
+  const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
+                           ? a.tokens
+                           : int64_t{begin + a.segment_chunks} * kTokens;
+  for (int64_t t = int64_t{end > begin ? end : begin} * kTokens + lane.l; t < stop; t += 16)
+    if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
+}
+
+// ---- segments of the chunks --------------------------------------------------------------------------------
+
+// With few heads a walk over all chunks would leave most of the chip idle. What a segment of them makes of the
+// state before it is linear, S' = M S + N: the walk without outputs gives N from a state of zeros and M's columns
+// from those of the unit matrix (and no values), all segments side by side. Here they are put together, one after
+// another in float32 for every state before a segment (REVERSE: from the last one, gradients), from which the
+// walks of all segments then run side by side. A workgroup has 16 columns; a wave a quarter of the rows.
+template <int DK, bool REVERSE>
+__global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
+  constexpr int kTiles = DK / 16, kMine = kTiles / 4;
+  __shared__ f32x4 shared[2][kTiles][64];
+  const int l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, at = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
+  const int64_t bh = blockIdx.x - tile * heads;
+  const int mine = static_cast<int>(tile) * 16 + l;
+  const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
+  const float* from = REVERSE ? a.grad_last : a.first;
+  float* to = REVERSE ? a.grad_first : a.last;
+  f32x4 state[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int d = first_row<T>(m, lane.g) + e;
-      if (d < key_size && mine < value_size) a.last[(bh * key_size + d) * value_size + mine] = state[m][e];
+      const int d = (wave * kMine + i) * 16 + g * 4 + e;
+      state[i][e] = from != nullptr && d < key_size && mine < value_size
+                        ? from[(bh * key_size + d) * value_size + mine]
+                        : 0.f;
     }
-  // Tokens past the last chunk give zeros.
-  for (int64_t t = static_cast<int64_t>(chunks) * kTokens + lane.l; t < a.tokens; t += 16)
-    if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
+  // A segment's rows of M and its N, a segment ahead.
+  f32x4 rows[kMine][kTiles], next[kMine];
+  const auto load = [&](int s) __attribute__((always_inline)) {
+    const int64_t segment = bh * a.segments + s;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int first = (wave * kMine + i) * 16;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        rows[i][t] = *reinterpret_cast<const f32x4*>(a.transits + (segment * DK + first + l) * DK + t * 16 + g * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        next[i][e] = a.partials[(segment * DK + first + g * 4 + e) * a.value_pad + mine];
+    }
+  };
+  load(REVERSE ? a.segments - 1 : 0);
+#pragma unroll 1
+  for (int i = 0; i < a.segments; ++i) {
+    const int s = REVERSE ? a.segments - 1 - i : i;
+    const int64_t segment = bh * a.segments + s;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      shared[i & 1][wave * kMine + k][at] = state[k];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        a.starts[(segment * DK + (wave * kMine + k) * 16 + g * 4 + e) * a.value_pad + mine] = state[k][e];
+    }
+    __syncthreads();
+    // A result's registers at a lane are an operand's of the same tile: rows 4 g to 4 g + 3 of a column.
+    f32x4 part[kMine][2];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      part[k][0] = next[k];
+      part[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      const f32x4 column = shared[i & 1][t][at];
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) part[k][t & 1] = Fragment<float>::mma(rows[k][t], column, part[k][t & 1]);
+    }
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) state[k] = part[k][0] + part[k][1];
+    if (i + 1 < a.segments) load(REVERSE ? s - 1 : s + 1);
+  }
+  if (to == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = (wave * kMine + i) * 16 + g * 4 + e;
+      if (d < key_size && mine < value_size) to[(bh * key_size + d) * value_size + mine] = state[i][e];
+    }
 }
 
 // ---- the walk back ----------------------------------------------------------------------------------------
@@ -996,7 +1120,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 //
 // in the forward walk's form: a wave has 16 columns of D in registers. D and Y of every chunk are kept for
 // delta_gradients.
-template <typename T, int DK, int W>
+template <typename T, int DK, int W, bool TRANSIT>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_backward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
@@ -1007,20 +1131,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const Lane lane;
   const Reader<T> places;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
-  const int64_t bh = blockIdx.x - tile * heads;
-  const int b = static_cast<int>(static_cast<unsigned>(bh) / static_cast<unsigned>(a.heads));
-  const int h = static_cast<int>(bh) - b * static_cast<int>(a.heads);
-  const int kh = h / a.groups;
-  const int v0 = static_cast<int>(tile) * W * 16;
-  const int column = v0 + wave * 16;
+  const WalkPlace w(a, W * 16, TRANSIT ? DK : 0);
+  const int64_t bh = w.bh;
+  const int b = w.b, h = w.h, kh = w.kh;
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
-  const bool active = column < value_size;
+  const int v0 = w.v0, column = v0 + wave * 16;  // of the workgroup and the wave
+  const bool active = TRANSIT && w.unit ? true : column < value_size;
   const int mine = column + lane.l;
   const int length = length_of(a, b);
-  const int chunks = (length + kTokens - 1) / kTokens;
-  const int64_t first_chunk = bh * a.chunks;
-  T* turn = reinterpret_cast<T*>(lds + 2 * S::kBytes) + wave * kTokens * kTurnPitch;
+  const int all_chunks = (length + kTokens - 1) / kTokens;
+  const int begin = w.segment * a.segment_chunks;
+  const int end = all_chunks < begin + a.segment_chunks ? all_chunks : begin + a.segment_chunks;
+  const int64_t first_chunk = bh * a.chunks, segment_at = bh * a.segments + w.segment;
 
   f32x4 state[kStateTiles];
 #pragma unroll
@@ -1028,10 +1150,17 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = first_row<T>(m, lane.g) + e;
-      state[m][e] = a.grad_last != nullptr && d < key_size && mine < value_size
-                        ? a.grad_last[(bh * key_size + d) * value_size + mine]
-                        : 0.f;
+      if constexpr (TRANSIT)
+        state[m][e] = w.unit && d == mine ? 1.f : 0.f;
+      else if (a.segments > 1)
+        state[m][e] = active ? a.starts[(segment_at * DK + d) * a.value_pad + mine] : 0.f;
+      else
+        state[m][e] = a.grad_last != nullptr && d < key_size && mine < value_size
+                          ? a.grad_last[(bh * key_size + d) * value_size + mine]
+                          : 0.f;
     }
+
+  T* turn = reinterpret_cast<T*>(lds + 2 * S::kBytes) + wave * kTokens * kTurnPitch;
 
   const Own<T> own(wave);
   const unsigned lds_at = lds_address(lds);
@@ -1043,7 +1172,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
   const PanelLoads<T, S::kValuePanels, W> value_loads(
       static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
-      static_cast<unsigned>(value_size * sizeof(T)), wave);
+      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
   const PanelLoads<T, 2 * kTerms, W> pair_loads(wave);
   auto load = [&](int c) __attribute__((always_inline)) {
     const unsigned dst = lds_at + (c & 1) * S::kBytes;
@@ -1091,14 +1220,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
   };
-  if (chunks > 0) load(chunks - 1);
+  if (begin < end) load(end - 1);
 #pragma unroll 1
-  for (int c = chunks - 1; c >= 0; --c) {
+  for (int c = end - 1; c >= begin; --c) {
     wait_loads();
     __syncthreads();
-    if (c > 0) load(c - 1);
+    if (c > begin) load(c - 1);
     if (!active) continue;
-    store_held();
+    if constexpr (!TRANSIT) store_held();
     const unsigned at = lds_at + (c & 1) * S::kBytes;
     const Reader<T> read = places.moved(at), pairs_read = places.moved(at + S::kPairs);
     const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
@@ -1107,7 +1236,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     frag s[kSteps][kTerms];
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
-    {
+    if constexpr (!TRANSIT) {
       T* keep = static_cast<T*>(a.grad_states) + (first_chunk + c) * a.value_pad * DK;
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
@@ -1257,6 +1386,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
       for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
     }
+    if constexpr (TRANSIT) continue;
     // dV, through this wave's part of LDS: lanes tokens, four columns each.
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
@@ -1270,18 +1400,29 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     wait_own_lds();
     held = c;
   }
-  store_held();
+  if constexpr (!TRANSIT) store_held();
   if (!active) return;
-  if (a.grad_first != nullptr) {
+  if (TRANSIT || (a.segments == 1 && a.grad_first != nullptr)) {
 #pragma unroll
     for (int m = 0; m < kStateTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = first_row<T>(m, lane.g) + e;
-        if (d < key_size && mine < value_size) a.grad_first[(bh * key_size + d) * value_size + mine] = state[m][e];
+        if constexpr (TRANSIT) {
+          if (w.unit)
+            a.transits[(segment_at * DK + d) * DK + mine] = state[m][e];
+          else
+            a.partials[(segment_at * DK + d) * a.value_pad + mine] = state[m][e];
+        } else if (d < key_size && mine < value_size) {
+          a.grad_first[(bh * key_size + d) * value_size + mine] = state[m][e];
+        }
       }
   }
-  for (int64_t t = static_cast<int64_t>(chunks) * kTokens + lane.l; t < a.tokens; t += 16)
+  if constexpr (TRANSIT) return;
+  const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
+                           ? a.tokens
+                           : int64_t{begin + a.segment_chunks} * kTokens;
+  for (int64_t t = int64_t{end > begin ? end : begin} * kTokens + lane.l; t < stop; t += 16)
     if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
 }
 
@@ -1977,31 +2118,57 @@ hipError_t launch_prepare(const DeltaArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int DK, int W, bool KEEP>
+int64_t value_tiles(const DeltaArgs& a, int columns) { return (a.value_size + columns - 1) / columns; }
+
+// One walk; TRANSIT: of its segments, with the columns of the unit matrix.
+template <typename T, int DK, bool KEEP, bool TRANSIT>
 hipError_t launch_walk(const DeltaArgs& a, hipStream_t stream) {
-  constexpr int kBytes = 2 * Stage<T, DK, W>::kBytes;
-  const auto kernel = delta_forward<T, DK, W, KEEP>;
+  constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes;
+  const auto kernel = delta_forward<T, DK, W, KEEP, TRANSIT>;
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
   if (err != hipSuccess) return err;
-  const int64_t tiles = (a.value_size + W * 16 - 1) / (W * 16);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(64 * W), kBytes, stream, a);
+  const int64_t tiles = value_tiles(a, W * 16) + (TRANSIT ? DK / (W * 16) : 0);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(64 * W), kBytes,
+                     stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, int DK, bool TRANSIT>
+hipError_t launch_walk_back(const DeltaArgs& a, hipStream_t stream) {
+  constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
+  const auto kernel = delta_backward<T, DK, W, TRANSIT>;
+  static std::atomic<uint64_t> asked{0};
+  const hipError_t err = ask_lds(kernel, kBytes, asked);
+  if (err != hipSuccess) return err;
+  const int64_t tiles = value_tiles(a, W * 16) + (TRANSIT ? DK / (W * 16) : 0);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(64 * W), kBytes,
+                     stream, a);
+  return hipGetLastError();
+}
+
+template <int DK, bool REVERSE>
+hipError_t launch_join(const DeltaArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((delta_join<DK, REVERSE>), dim3(static_cast<unsigned>(a.batch * a.heads * value_tiles(a, 16))),
+                     dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
 template <typename T, int DK>
 hipError_t launch_forward(const DeltaArgs& a, const DeltaPlan& p, hipStream_t stream) {
   if (p.step) {
-    const int64_t tiles = (a.value_size + kDeltaStepColumns - 1) / kDeltaStepColumns;
-    hipLaunchKernelGGL((delta_step<T, DK>), dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(256), 0,
+    hipLaunchKernelGGL((delta_step<T, DK>),
+                       dim3(static_cast<unsigned>(a.batch * a.heads * value_tiles(a, kDeltaStepColumns))), dim3(256), 0,
                        stream, a);
     return hipGetLastError();
   }
-  if (a.chunks > 0) {
-    const hipError_t err = launch_prepare<T, DK>(a, stream);
-    if (err != hipSuccess) return err;
+  hipError_t err = a.chunks > 0 ? launch_prepare<T, DK>(a, stream) : hipSuccess;
+  if (err == hipSuccess && a.segments > 1) {
+    err = launch_walk<T, DK, false, true>(a, stream);
+    if (err == hipSuccess) err = launch_join<DK, false>(a, stream);
   }
-  return a.states != nullptr ? launch_walk<T, DK, 4, true>(a, stream) : launch_walk<T, DK, 4, false>(a, stream);
+  if (err != hipSuccess) return err;
+  return a.states != nullptr ? launch_walk<T, DK, true, false>(a, stream) : launch_walk<T, DK, false, false>(a, stream);
 }
 
 template <typename T, int DK, bool GROUPED>
@@ -2020,15 +2187,12 @@ hipError_t launch_gradients(const DeltaArgs& a, hipStream_t stream) {
 
 template <typename T, int DK>
 hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
-  constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
-  const auto kernel = delta_backward<T, DK, W>;
-  static std::atomic<uint64_t> asked{0};
-  hipError_t err = ask_lds(kernel, kBytes, asked);
-  if (err == hipSuccess && a.chunks > 0) err = launch_prepare<T, DK>(a, stream);
-  if (err != hipSuccess) return err;
-  const int64_t tiles = (a.value_size + W * 16 - 1) / (W * 16);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles)), dim3(64 * W), kBytes, stream, a);
-  err = hipGetLastError();
+  hipError_t err = a.chunks > 0 ? launch_prepare<T, DK>(a, stream) : hipSuccess;
+  if (err == hipSuccess && a.segments > 1) {
+    err = launch_walk_back<T, DK, true>(a, stream);
+    if (err == hipSuccess) err = launch_join<DK, true>(a, stream);
+  }
+  if (err == hipSuccess) err = launch_walk_back<T, DK, false>(a, stream);
   if (err != hipSuccess || a.chunks == 0) return err;
   return a.heads == a.key_heads ? launch_gradients<T, DK, false>(a, stream) : launch_gradients<T, DK, true>(a, stream);
 }

@@ -692,8 +692,12 @@ struct DeltaArgs {
   void* grad_decay;
   void* grad_beta;
   float* grad_first;          // or null
+  float* transits;            // [batch, heads, segments, padded key size, padded key size], of several segments
+  float* partials;            // [batch, heads, segments, padded key size, value_pad]
+  float* starts;              // as partials: before each segment (backward: after)
   int64_t batch, tokens, key_heads, heads, key_size, value_size;
   int64_t chunks;             // of `tokens`
+  int segments, segment_chunks;
   int64_t value_pad;          // value_size in whole 16
   DeltaStrides query_strides, key_strides, value_strides, decay_strides, beta_strides, grad_strides;
   float scale;
@@ -704,6 +708,8 @@ struct DeltaArgs {
 };
 struct DeltaPlan {
   bool step;                  // token by token, without workspace
+  int segments;               // of the chunks, walked side by side
+  int segment_chunks;
   int64_t workgroups;         // of the largest launch, and the threads of each
   int threads;
 };

@@ -351,13 +351,27 @@ int fill_rows(convnd_hip_dtype dtype, const DeltaRows& r, hipStream_t stream) {
   return hip_check(launch_delta_copy(dtype, r.copy, stream), "delta rule operand copy");
 }
 
+int64_t delta_key_pad(const DeltaArgs& a) { return a.key_size <= 64 ? 64 : 128; }
+
+// Segments of the chunks where walks over all of them would leave three quarters of the compute units idle: as
+// many as fill them, of eight chunks at least. A segment is walked twice, once with the unit matrix's columns
+// beside its own.
 DeltaPlan plan_delta(const DeltaArgs& a, bool saving) {
   DeltaPlan p{};
   p.step = !saving && a.tokens <= kDeltaStepTokens;
   const int64_t columns = kDeltaStepColumns;  // of a walk's four waves too
-  p.workgroups = a.batch * a.heads * ((a.value_size + columns - 1) / columns);
+  const int64_t walks = a.batch * a.heads * ((a.value_size + columns - 1) / columns);
+  p.workgroups = walks;
   p.threads = 256;
-  if (!p.step) p.workgroups = std::max(p.workgroups, a.batch * a.key_heads * a.chunks);
+  p.segments = 1;
+  p.segment_chunks = static_cast<int>(a.chunks);
+  if (p.step) return p;
+  if (walks > 0 && walks <= 64 && a.chunks >= 16) {
+    const int64_t most = std::min<int64_t>(256 / walks, a.chunks / 8);
+    p.segment_chunks = static_cast<int>((a.chunks + most - 1) / most);
+    p.segments = static_cast<int>((a.chunks + p.segment_chunks - 1) / p.segment_chunks);
+  }
+  p.workgroups = std::max(p.workgroups, a.batch * a.key_heads * a.chunks);
   return p;
 }
 
@@ -378,6 +392,14 @@ DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, const void
     const int64_t records = a->batch * a->heads * a->chunks;
     a->panels = static_cast<char*>(ws->take(records * delta_panel_bytes(size)));
     a->records = static_cast<char*>(ws->take(records * delta_record_bytes(size)));
+    a->segments = p.segments;
+    a->segment_chunks = p.segment_chunks;
+    if (p.segments > 1) {
+      const int64_t rows = a->batch * a->heads * p.segments * delta_key_pad(*a) * int64_t{sizeof(float)};
+      a->transits = static_cast<float*>(ws->take(rows * delta_key_pad(*a)));
+      a->partials = static_cast<float*>(ws->take(rows * a->value_pad));
+      a->starts = static_cast<float*>(ws->take(rows * a->value_pad));
+    }
   }
   a->query = l.query.data;
   a->key = l.key.data;
@@ -390,7 +412,7 @@ DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, const void
 
 // Elements of the saved states and of the saved updates.
 int64_t saved_states(const DeltaArgs& a) {
-  return a.batch * a.heads * a.chunks * a.value_pad * (a.key_size <= 64 ? 64 : 128);
+  return a.batch * a.heads * a.chunks * a.value_pad * delta_key_pad(a);
 }
 int64_t saved_updates(const DeltaArgs& a, int size) {
   return a.batch * a.heads * a.chunks * a.value_pad * delta_chunk(size);
