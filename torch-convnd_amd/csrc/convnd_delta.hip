@@ -687,19 +687,21 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
 
 // ---- the walk over the chunks ------------------------------------------------------------------------
 
-// LDS of a chunk: V or dO, the factors, K, Q, T and P (each in its terms). What is read by a constant beside a
+// LDS of a chunk: K, Q, T and P (each in its terms), V or dO, the factors. What is read by a constant beside a
 // lane's address lies within 64 KB of it.
 template <typename T, int DK, int W>
 struct Stage {
   using C = Chunk<T>;
-  static constexpr int kValuePanels = W * 16 / C::kTokens;
-  static constexpr int kFactors = kValuePanels * C::kPanel;
-  static constexpr int kKeys = kFactors + 2048;
+  static constexpr int kKeys = 0;
   static constexpr int kQuery = kKeys + DK / C::kTokens * C::kPanel;
   static constexpr int kSolve = kQuery + DK / C::kTokens * C::kPanel;
   static constexpr int kPairs = kSolve + C::kTerms * C::kPanel;
-  static constexpr int kBytes = kPairs + C::kTerms * C::kPanel;
+  static constexpr int kValues = kPairs + C::kTerms * C::kPanel;
+  static constexpr int kValuePanels = W * 16 / C::kTokens;
+  static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
+  static constexpr int kBytes = kFactors + 2048;
   static_assert(W * 16 % C::kTokens == 0, "whole panels of values");
+  static_assert(kValues <= 65536, "constants of reads");
 };
 
 // Where a workgroup of a walk is: `columns` values of a head (or columns of the unit matrix) and a segment of its
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
     key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
-    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst, wave, rows);
+    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, wave, rows);
     if constexpr (!TRANSIT) query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
     pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
     if (wave < 2) {  // the factors, and after them `whole`
@@ -818,7 +820,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
   const unsigned state_place = mine * DK + lane.g * (16 / sizeof(T));
   const unsigned update_place = mine * kTokens + lane.g * (16 / sizeof(T));
-  f32x4 held_output[kTiles];
+  Four<T> held_output[kTiles];
   frag held_update[2];
   int held = -1;
   const auto store_held = [&]() __attribute__((always_inline)) {
@@ -826,12 +828,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
     if (whole_rows && (held + 1) * kTokens <= a.tokens) {
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) store_four(to + out_place[n], held_output[n], 4);
+      for (int n = 0; n < kTiles; ++n) *reinterpret_cast<Run<T, 4>*>(to + out_place[n]) = __builtin_bit_cast(Run<T, 4>, held_output[n]);
     } else {
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
-        if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens && store_count > 0)
-          store_four(to + out_place[n], held_output[n], store_count);
+        if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < store_count) to[out_place[n] + e] = held_output[n][e];
+          end_of_part();
+        }
     }
     if constexpr (KEEP) {
       T* keep = static_cast<T*>(a.updates) + (first_chunk + held) * a.value_pad * kTokens;
@@ -848,7 +854,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     if (!active) continue;
     if constexpr (!TRANSIT) store_held();
     const unsigned at = lds_at + (c & 1) * S::kBytes;
-    const Reader<T> read = places.moved(at), pairs_read = places.moved(at + S::kPairs);
+    const Reader<T> read = places.moved(at);
     const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
     const float whole = factors[256];
 
@@ -878,14 +884,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
         cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
       } else if (!TRANSIT && (i -= kColumns) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
-        pf[i] = pairs_read.row(i / kBlocks * C::kPanel, b.tile, b.step);
+        pf[i] = read.row(S::kPairs + i / kBlocks * C::kPanel, b.tile, b.step);
       }
     };
     constexpr int kFirstQ = kRows, kFirstT = kRows + kQueries, kFirstC = kFirstT + kTerms * kBlocks,
                   kFirstP = kFirstC + kColumns;
-    f32x4 v[kTiles];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) v[m] = own.values(at, m);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch(i);
     keep_order();
@@ -906,11 +909,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
       const f32x4 acc = sums[m].value();
+      const f32x4 v = own.values(at + S::kValues, m);
       const int row = first_row<T>(m, lane.g);
       const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
       const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[m][e], -take[e] * acc[e]);
+      for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[e], -take[e] * acc[e]);
       sums[m] = Sum<T>();
     }
     // Q S: O's lanes are tokens and its registers columns.
@@ -993,7 +997,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
       keep_order();
     }
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) held_output[n] = o[n].value();
+    for (int n = 0; n < kTiles; ++n) held_output[n] = nearest<T>(o[n].value());
     if constexpr (KEEP) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) held_update[kt] = uf[kt][0];
@@ -1179,7 +1183,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
     key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
-    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst, wave, rows);
+    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, wave, rows);
     query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
     pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
     if (wave < 2) {  // the factors, and after them `whole`
@@ -1229,7 +1233,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     if (!active) continue;
     if constexpr (!TRANSIT) store_held();
     const unsigned at = lds_at + (c & 1) * S::kBytes;
-    const Reader<T> read = places.moved(at), pairs_read = places.moved(at + S::kPairs);
+    const Reader<T> read = places.moved(at);
     const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
     const float whole = factors[256];
 
@@ -1251,7 +1255,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
         qf[i] = read.column(S::kQuery, i / 8 * 4 + i % 4, i / 4 % 2);
       } else if ((i -= kColumns) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
-        pf[i] = pairs_read.column(i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
+        pf[i] = read.column(S::kPairs + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
       } else if ((i -= kTerms * kBlocks) < kTerms * kBlocks) {
         const Triangle<T> b(i % kBlocks);
         tf[i] = read.column(S::kSolve + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
@@ -1264,7 +1268,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
                   kFirstC = kFirstT + kTerms * kBlocks;
     frag g[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) g[kt] = own.column(at, kt);
+    for (int kt = 0; kt < 2; ++kt) g[kt] = own.column(at + S::kValues, kt);
 #pragma unroll
     for (int i = 0; i < kAheadBack; ++i) fetch(i);
     keep_order();
