@@ -1,10 +1,10 @@
 """A byte-level language model of convolution and recurrence blocks: trains on a text, then writes.
 
-    python examples/byte_model.py [--text FILE] [--steps 200] [--channels 256] [--blocks 4]
+    python examples/byte_model.py [--text FILE] [--steps 200] [--channels 256] [--blocks 4] [--heads 0]
 
 Training runs whole sequences through the blocks (layer norm, causal depthwise convolution, gated
-recurrence and linear layers of ``torch_convnd``); writing keeps each block's state and feeds one byte
-at a time. On a ROCm GPU all of it runs on the gfx950 kernels in bfloat16, elsewhere on PyTorch's
+recurrence and linear layers of ``torch_convnd``; with heads the gated delta rule and gated linear layers);
+writing keeps each block's state and feeds one byte at a time. On a ROCm GPU all of it runs on the gfx950 kernels in bfloat16, elsewhere on PyTorch's
 operations in float32.
 """
 
@@ -22,11 +22,16 @@ import torch_convnd  # noqa: E402
 
 
 class ByteModel(nn.Module):
-    def __init__(self, channels, blocks, device=None, dtype=None, backend="auto"):
+    def __init__(self, channels, blocks, device=None, dtype=None, backend="auto", heads=0):
         super().__init__()
         factory = {"device": device, "dtype": dtype, "backend": backend}
         self.embed = nn.Embedding(256, channels, device=device, dtype=dtype)
-        self.blocks = nn.ModuleList(torch_convnd.GatedConvBlock(channels, **factory) for _ in range(blocks))
+        self.blocks = nn.ModuleList(
+            torch_convnd.GatedDeltaBlock(channels, heads, **factory)
+            if heads
+            else torch_convnd.GatedConvBlock(channels, **factory)
+            for _ in range(blocks)
+        )
         self.norm = torch_convnd.LayerNorm(channels, **factory)
         self.head = torch_convnd.LinearAct(channels, 256, **factory)
 
@@ -84,6 +89,7 @@ def main(argv=None):
     parser.add_argument("--steps", type=int, default=200)
     parser.add_argument("--channels", type=int, default=256)
     parser.add_argument("--blocks", type=int, default=4)
+    parser.add_argument("--heads", type=int, default=0, help="heads of the delta rule (0: the gated recurrence)")
     parser.add_argument("--batch", type=int, default=16)
     parser.add_argument("--length", type=int, default=256)
     parser.add_argument("--write", type=int, default=200, help="bytes to write after training")
@@ -94,7 +100,7 @@ def main(argv=None):
     text = torch.tensor(list(Path(options.text).read_bytes()))
     # "native": the convolution of one axis too runs on the gfx950 kernels ("auto" sends it to PyTorch's).
     backend = "native" if on_gpu else "auto"
-    model = ByteModel(options.channels, options.blocks, device, dtype, backend)
+    model = ByteModel(options.channels, options.blocks, device, dtype, backend, options.heads)
     losses = train(model, text, options.steps, options.batch, min(options.length, len(text) - 2), device)
     if options.write:
         print(write(model, b"def ", options.write, device).decode("utf-8", "replace"))

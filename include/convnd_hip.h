@@ -476,6 +476,11 @@ int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_pro
                               void* grad_value, void* grad_decay, void* grad_beta, float* grad_first,
                               void* workspace, size_t workspace_size, void* stream);
 
+/* JSON description of a delta rule's launch plan (kernel, chunk's tokens, segments of the chunks that are walked
+ * side by side and the chunks of each), as above; `saving` 0 or 1 (a backward: 1). */
+int convnd_hip_delta_plan_describe(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
+                                   int saving, char* buffer, size_t length);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1058,4 +1058,16 @@ int convnd_hip_recurrence_plan_describe(convnd_hip_dtype dtype,
       .write(buffer, length);
 }
 
+int convnd_hip_delta_plan_describe(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
+                                   int saving, char* buffer, size_t length) {
+  const int st = check_delta(dtype, problem);
+  if (st != CONVND_HIP_SUCCESS) return st;
+  const DeltaPlan p = plan_delta(to_args(dtype, *problem), saving != 0);
+  return Description(p.step ? "step" : "chunks")
+      .add("chunk", p.step ? 1 : delta_chunk(size_of(dtype)))
+      .add("segments", p.segments)
+      .add("segment_chunks", p.segment_chunks)
+      .write(buffer, length);
+}
+
 }  // extern "C"

@@ -25,7 +25,7 @@ from .modules import (
 )
 from .partial import PartialConvOutput, partial_conv_nd
 from .sequence import gated_delta_rule, gated_linear, gated_recurrence, layer_norm, linear_act
-from .sequence_modules import GatedConvBlock, LayerNorm, LinearAct
+from .sequence_modules import GatedConvBlock, GatedDeltaBlock, GatedLinear, LayerNorm, LinearAct
 
 ensure_native_definitions()
 ensure_compatible_operator()
@@ -37,6 +37,8 @@ __all__ = [
     "Conv4d",
     "ConvNd",
     "GatedConvBlock",
+    "GatedDeltaBlock",
+    "GatedLinear",
     "LayerNorm",
     "LinearAct",
     "PartialConv1d",

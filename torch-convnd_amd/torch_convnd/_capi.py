@@ -56,6 +56,7 @@ EXPORTED_SYMBOLS = (
     "convnd_hip_delta",
     "convnd_hip_delta_backward_workspace_size",
     "convnd_hip_delta_backward",
+    "convnd_hip_delta_plan_describe",
 )
 
 CHANNELS_FIRST, CHANNELS_LAST, CHANNELS_LAST_INPUT = 0, 1, 2
@@ -126,6 +127,19 @@ class DeltaProblem(ctypes.Structure):
         ("gate_dtype", ctypes.c_int),
         ("wide_lengths", ctypes.c_int),
     ]
+
+    @classmethod
+    def make(cls, batch, tokens, key_heads, heads, key_size, value_size, gate_dtype):
+        """Of contiguous tensors; scale 1."""
+        p = cls(batch=batch, tokens=tokens, key_heads=key_heads, heads=heads, key_size=key_size,
+                value_size=value_size, gate_dtype=gate_dtype, scale=1.0)
+        for name, count, size in (("query", key_heads, key_size), ("key", key_heads, key_size),
+                                  ("value", heads, value_size), ("grad", heads, value_size),
+                                  ("decay", heads, 1), ("beta", heads, 1)):
+            setattr(p, f"{name}_batch", tokens * count * size)
+            setattr(p, f"{name}_token", count * size)
+            setattr(p, f"{name}_head", size)
+        return p
 
 
 def bind(library: ctypes.CDLL) -> ctypes.CDLL:
@@ -231,6 +245,8 @@ def bind(library: ctypes.CDLL) -> ctypes.CDLL:
     library.convnd_hip_delta.argtypes = [ctypes.c_int, D, *[vp] * 11, sz, vp]
     library.convnd_hip_delta_backward_workspace_size.restype = sz
     library.convnd_hip_delta_backward_workspace_size.argtypes = [ctypes.c_int, D, vp, vp, vp, vp]
+    library.convnd_hip_delta_plan_describe.restype = ctypes.c_int
+    library.convnd_hip_delta_plan_describe.argtypes = [ctypes.c_int, D, ctypes.c_int, ctypes.c_char_p, sz]
     library.convnd_hip_delta_backward.restype = ctypes.c_int
     library.convnd_hip_delta_backward.argtypes = [ctypes.c_int, D, *[vp] * 16, sz, vp]
     library.convnd_hip_linear_plan_describe.restype = ctypes.c_int
@@ -306,3 +322,10 @@ def recurrence_plan(library, batch, tokens, channels, dtype, backward=False):
     )
     describe = library.convnd_hip_recurrence_plan_describe
     return _described(library, describe, dtype_code(dtype), ctypes.byref(p), int(backward))
+
+
+def delta_plan(library, batch, tokens, key_heads, heads, key_size, value_size, dtype, saving=False):
+    """Launch plan of a gated delta rule as a dict."""
+    p = DeltaProblem.make(batch, tokens, key_heads, heads, key_size, value_size, FLOAT32)
+    describe = library.convnd_hip_delta_plan_describe
+    return _described(library, describe, dtype_code(dtype), ctypes.byref(p), int(saving))

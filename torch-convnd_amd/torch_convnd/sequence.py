@@ -395,4 +395,6 @@ def _portable_delta(query, key, value, decay, beta, initial_state, lengths, scal
         state = state + k[:, t, :, :, None] * update[:, :, None, :]
         outputs.append((q[:, t, :, :, None] * state).sum(dim=2))
     output = torch.stack(outputs, dim=1) if outputs else v
+    if lengths is not None:
+        output = torch.where(live[..., None, None], output, 0)
     return output.to(value.dtype), state
