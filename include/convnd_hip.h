@@ -439,7 +439,8 @@ typedef struct convnd_hip_delta_problem {
 } convnd_hip_delta_problem;
 
 /* Elements (of the element type) that the forward saves for the backward: for each chunk of 64 tokens (32
- * of float32) the state before it and what its tokens add. */
+ * of float32) the state before it, what its tokens add, and their pairs and factors. At `saved` aligned to 16
+ * bytes. */
 int64_t convnd_hip_delta_saved(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem);
 
 /* Device scratch bytes of convnd_hip_delta; of the pointers only the alignment is looked at (rows that

@@ -115,7 +115,7 @@ def test_fake_kernels():
         v, gate = q.new_empty(3, 70, 4, 20), q.new_empty(3, 70, 4, dtype=torch.float32)
         o, last, saved = ops.gated_delta_rule(q, q, v, gate, gate, None, None, 1.0, True, True)
         assert o.shape == v.shape and last.shape == (3, 4, 16, 20) and last.dtype == torch.float32
-        assert saved.shape == (3 * 4 * 2 * 32 * 128,) and saved.dtype == torch.bfloat16
+        assert saved.shape == (3 * 4 * 2 * (32 * 128 + (4 * 64 * 128 + 36 * 64 + 32) // 2),) and saved.dtype == torch.bfloat16
         assert ops.gated_delta_rule(q, q, v, gate, gate, None, None, 1.0, True, False)[2].numel() == 0
         grads = ops.gated_delta_rule_backward(o, last, q, q, v, gate, gate, None, saved, 1.0, True, True)
         for got, t in zip(grads, (q, q, v, gate, gate, last)):
@@ -184,6 +184,8 @@ def test_c_abi_checks(lib):
     expect(lib, delta(last=None), bad, "must not be null")
     expect(lib, delta(backward=True), bad, "must not be null")  # saved
     expect(lib, delta(workspace=ctypes.c_void_p(20)), bad, "aligned to 16 bytes")
+    expect(lib, delta(saved=ctypes.c_void_p(20)), bad, "saved must be aligned")
+    expect(lib, delta(saved=ctypes.c_void_p(20), backward=True), bad, "saved must be aligned")
     p = ctypes.byref(_capi.DeltaProblem.make(2, 100, 2, 4, 64, 64, f32))
     size = lib.convnd_hip_delta_workspace_size(bf16, p, ONE, ONE, ONE, 0)
     assert size > 0
@@ -191,7 +193,7 @@ def test_c_abi_checks(lib):
     # Rows that do not start on 4 bytes are copied.
     assert lib.convnd_hip_delta_workspace_size(bf16, p, ctypes.c_void_p(18), ONE, ONE, 0) > size
     back = lib.convnd_hip_delta_backward_workspace_size(bf16, p, ONE, ONE, ONE, ONE)
-    assert back > size
+    assert back > lib.convnd_hip_delta_workspace_size(bf16, p, ONE, ONE, ONE, 1)
     expect(lib, delta(backward=True, saved=ONE, size=back - 1), small, str(back))
     p = ctypes.byref(_capi.DeltaProblem.make(2, 3, 2, 4, 64, 64, f32))
     assert lib.convnd_hip_delta_workspace_size(bf16, p, ONE, ONE, ONE, 0) == 0

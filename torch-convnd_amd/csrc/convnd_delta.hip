@@ -2191,8 +2191,8 @@ hipError_t launch_gradients(const DeltaArgs& a, hipStream_t stream) {
 
 template <typename T, int DK>
 hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
-  hipError_t err = a.chunks > 0 ? launch_prepare<T, DK>(a, stream) : hipSuccess;
-  if (err == hipSuccess && a.segments > 1) {
+  hipError_t err = hipSuccess;
+  if (a.segments > 1) {
     err = launch_walk_back<T, DK, true>(a, stream);
     if (err == hipSuccess) err = launch_join<DK, true>(a, stream);
   }

@@ -680,8 +680,8 @@ struct DeltaArgs {
   const void* lengths;        // [batch] int32 or int64, or null: all `tokens`
   void* output;               // [batch, tokens, heads, value_size]
   float* last;                // [batch, heads, key_size, value_size]
-  char* panels;               // [batch, heads, chunks] of delta_panel_bytes: T and P
-  char* records;              // [batch, heads, chunks] of delta_record_bytes
+  char* panels;               // [batch, heads, chunks] of delta_panel_bytes: T and P; a forward that
+  char* records;              // keeps states keeps these and the records of delta_record_bytes too
   void* states;               // [batch, heads, chunks, value_pad, padded key size]: before each chunk; or null
   void* updates;              // [batch, heads, chunks, value_pad, chunk]: U transposed
   void* grad_states;          // as states: the gradient of the state after each chunk

@@ -379,8 +379,8 @@ DeltaPlan plan_delta(const DeltaArgs& a, bool saving) {
 struct DeltaLayout {
   DeltaRows query, key, value, grad;
 };
-DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, const void* query, const void* key,
-                          const void* value, Parts* ws) {
+DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, bool saving, const void* query,
+                          const void* key, const void* value, Parts* ws) {
   DeltaLayout l{};
   l.query = {query, a->query_strides, {}, false};
   l.key = {key, a->key_strides, {}, false};
@@ -389,9 +389,11 @@ DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, const void
     l.query = delta_rows(query, a->query_strides, *a, a->key_heads, a->key_size, size, ws);
     l.key = delta_rows(key, a->key_strides, *a, a->key_heads, a->key_size, size, ws);
     l.value = delta_rows(value, a->value_strides, *a, a->heads, a->value_size, size, ws);
-    const int64_t records = a->batch * a->heads * a->chunks;
-    a->panels = static_cast<char*>(ws->take(records * delta_panel_bytes(size)));
-    a->records = static_cast<char*>(ws->take(records * delta_record_bytes(size)));
+    if (!saving) {
+      const int64_t records = a->batch * a->heads * a->chunks;
+      a->panels = static_cast<char*>(ws->take(records * delta_panel_bytes(size)));
+      a->records = static_cast<char*>(ws->take(records * delta_record_bytes(size)));
+    }
     a->segments = p.segments;
     a->segment_chunks = p.segment_chunks;
     if (p.segments > 1) {
@@ -410,22 +412,33 @@ DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, const void
   return l;
 }
 
-// Elements of the saved states and of the saved updates.
-int64_t saved_states(const DeltaArgs& a) {
-  return a.batch * a.heads * a.chunks * a.value_pad * delta_key_pad(a);
+// What a forward keeps: states, updates, and the chunks' panels and records. In bytes, whole 16 each.
+int64_t saved_states(const DeltaArgs& a, int size) {
+  return a.batch * a.heads * a.chunks * a.value_pad * delta_key_pad(a) * size;
 }
 int64_t saved_updates(const DeltaArgs& a, int size) {
-  return a.batch * a.heads * a.chunks * a.value_pad * delta_chunk(size);
+  return a.batch * a.heads * a.chunks * a.value_pad * delta_chunk(size) * size;
+}
+int64_t saved_bytes(const DeltaArgs& a, int size) {
+  return saved_states(a, size) + saved_updates(a, size) +
+         a.batch * a.heads * a.chunks * (delta_panel_bytes(size) + delta_record_bytes(size));
+}
+void place_saved(DeltaArgs* a, int size, void* saved) {
+  char* at = static_cast<char*>(saved);
+  a->states = at;
+  a->updates = at += saved_states(*a, size);
+  a->panels = at += saved_updates(*a, size);
+  a->records = at + a->batch * a->heads * a->chunks * delta_panel_bytes(size);
 }
 
 DeltaLayout lay_out_delta_backward(DeltaArgs* a, int size, const void* grad_output, const void* query,
                                    const void* key, const void* value, Parts* ws) {
-  DeltaLayout l = lay_out_delta(a, size, plan_delta(*a, true), query, key, value, ws);
+  DeltaLayout l = lay_out_delta(a, size, plan_delta(*a, true), true, query, key, value, ws);
   l.grad = delta_rows(grad_output, a->grad_strides, *a, a->heads, a->value_size, size, ws);
   a->grad_output = l.grad.data;
   a->grad_strides = l.grad.strides;
-  a->grad_states = ws->take(saved_states(*a) * size);
-  a->grad_updates = ws->take(saved_updates(*a, size) * size);
+  a->grad_states = ws->take(saved_states(*a, size));
+  a->grad_updates = ws->take(saved_updates(*a, size));
   return l;
 }
 
@@ -795,7 +808,7 @@ int convnd_hip_linear_backward(convnd_hip_dtype dtype, const convnd_hip_linear_p
 int64_t convnd_hip_delta_saved(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem) {
   if (check_delta(dtype, problem) != CONVND_HIP_SUCCESS) return 0;
   const DeltaArgs a = to_args(dtype, *problem);
-  return saved_states(a) + saved_updates(a, size_of(dtype));
+  return saved_bytes(a, size_of(dtype)) / size_of(dtype);
 }
 
 size_t convnd_hip_delta_workspace_size(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
@@ -803,7 +816,7 @@ size_t convnd_hip_delta_workspace_size(convnd_hip_dtype dtype, const convnd_hip_
   if (check_delta(dtype, problem) != CONVND_HIP_SUCCESS || problem->batch == 0) return 0;
   DeltaArgs a = to_args(dtype, *problem);
   Parts ws{nullptr};
-  lay_out_delta(&a, size_of(dtype), plan_delta(a, saving != 0), query, key, value, &ws);
+  lay_out_delta(&a, size_of(dtype), plan_delta(a, saving != 0), saving != 0, query, key, value, &ws);
   return ws.used;
 }
 
@@ -818,11 +831,13 @@ int convnd_hip_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* pro
                                                   decay == nullptr || beta == nullptr || output == nullptr)))
     return fail(CONVND_HIP_INVALID_ARGUMENT,
                 "query, key, value, decay, beta, output and last must not be null");
+  if (reinterpret_cast<uintptr_t>(saved) % 16 != 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "saved must be aligned to 16 bytes");
   DeltaArgs a = to_args(dtype, *problem);
   const int size = size_of(dtype);
   const DeltaPlan p = plan_delta(a, saved != nullptr);
   Parts ws{static_cast<char*>(workspace)};
-  const DeltaLayout l = lay_out_delta(&a, size, p, query, key, value, &ws);
+  const DeltaLayout l = lay_out_delta(&a, size, p, saved != nullptr, query, key, value, &ws);
   if (!launch_fits(p.workgroups, p.threads))
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes are too large: more than 2^32 threads");
   st = check_parts(ws, workspace_size, "gated_delta_rule");
@@ -833,10 +848,7 @@ int convnd_hip_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* pro
   a.lengths = lengths;
   a.output = output;
   a.last = last;
-  if (saved != nullptr) {
-    a.states = saved;
-    a.updates = static_cast<char*>(saved) + saved_states(a) * size;
-  }
+  if (saved != nullptr) place_saved(&a, size, saved);
   const auto on = static_cast<hipStream_t>(stream);
   for (const DeltaRows* r : {&l.query, &l.key, &l.value}) {
     st = fill_rows(dtype, *r, on);
@@ -871,6 +883,8 @@ int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_pro
        grad_value == nullptr || grad_decay == nullptr || grad_beta == nullptr))
     return fail(CONVND_HIP_INVALID_ARGUMENT,
                 "grad_output, query, key, value, decay, beta, saved and their gradients must not be null");
+  if (reinterpret_cast<uintptr_t>(saved) % 16 != 0)
+    return fail(CONVND_HIP_INVALID_ARGUMENT, "saved must be aligned to 16 bytes");
   DeltaArgs a = to_args(dtype, *problem);
   const int size = size_of(dtype);
   Parts ws{static_cast<char*>(workspace)};
@@ -884,8 +898,7 @@ int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_pro
   a.beta = beta;
   a.lengths = lengths;
   a.grad_last = grad_last;
-  a.states = const_cast<void*>(saved);
-  a.updates = const_cast<char*>(static_cast<const char*>(saved)) + saved_states(a) * size;
+  place_saved(&a, size, const_cast<void*>(saved));
   a.grad_query = grad_query;
   a.grad_key = grad_key;
   a.grad_value = grad_value;

@@ -260,12 +260,15 @@ RECURRENCE_TILE = 64
 
 
 def delta_saved(query, value):
-    """Elements that gated_delta_rule saves: a state and its tokens' updates a chunk
+    """Elements that gated_delta_rule saves: a state, its tokens' updates, their pairs and factors a chunk
     (convnd_hip_delta_saved)."""
     batch, tokens, _, key_size = query.shape
-    chunk = 128 // query.element_size()
-    rows = batch * value.shape[2] * ((tokens + chunk - 1) // chunk) * ((value.shape[3] + 15) // 16 * 16)
-    return rows * ((64 if key_size <= 64 else 128) + chunk)
+    size = query.element_size()
+    chunk = 128 // size
+    columns = (value.shape[3] + 15) // 16 * 16
+    pairs = 2 * chunk * (256 if size == 2 else 128)  # bytes, in one or two terms; the factors follow
+    each = columns * ((64 if key_size <= 64 else 128) + chunk) + (pairs + 36 * chunk + 32) // size
+    return batch * value.shape[2] * ((tokens + chunk - 1) // chunk) * each
 
 
 def _fake_delta(query, key, value, decay, beta, initial_state, lengths, scale, normalize, keep):
