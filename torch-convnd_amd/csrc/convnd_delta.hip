@@ -697,10 +697,10 @@ struct Stage {
   static constexpr int kSolve = kQuery + DK / C::kTokens * C::kPanel;
   static constexpr int kPairs = kSolve + C::kTerms * C::kPanel;
   static constexpr int kValues = kPairs + C::kTerms * C::kPanel;
-  static constexpr int kValuePanels = W * 16 / C::kTokens;
+  static constexpr int kValuePanels = (W * 16 + C::kTokens - 1) / C::kTokens;
   static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
   static constexpr int kBytes = kFactors + 2048;
-  static_assert(W * 16 % C::kTokens == 0, "whole panels of values");
+  static_assert(W * 16 % C::kTokens == 0 || C::kTokens % (W * 16) == 0, "whole panels of values, or parts of one");
   static_assert(kValues <= 65536, "constants of reads");
 };
 
@@ -783,7 +783,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
                           : 0.f;
     }
 
-  const Own<T> own(wave);
+  // Panels of values start at whole ones; the wave's columns lie within.
+  const int from_panel = v0 % (S::kValuePanels * kTokens);
+  const Own<T> own(from_panel / 16 + wave);
   const unsigned lds_at = lds_address(lds);
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
@@ -792,7 +794,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
   const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
   const PanelLoads<T, S::kValuePanels, W> value_loads(
-      static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
+      static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
       TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
   const PanelLoads<T, (TRANSIT ? 1 : 2) * kTerms, W> pair_loads(wave);
   auto load = [&](int c) __attribute__((always_inline)) {
@@ -1166,7 +1168,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 
   T* turn = reinterpret_cast<T*>(lds + 2 * S::kBytes) + wave * kTokens * kTurnPitch;
 
-  const Own<T> own(wave);
+  // Panels of values start at whole ones; the wave's columns lie within.
+  const int from_panel = v0 % (S::kValuePanels * kTokens);
+  const Own<T> own(from_panel / 16 + wave);
   const unsigned lds_at = lds_address(lds);
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
@@ -1175,7 +1179,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
   const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
   const PanelLoads<T, S::kValuePanels, W> value_loads(
-      static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
+      static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
       TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
   const PanelLoads<T, 2 * kTerms, W> pair_loads(wave);
   auto load = [&](int c) __attribute__((always_inline)) {
@@ -2124,10 +2128,12 @@ hipError_t launch_prepare(const DeltaArgs& a, hipStream_t stream) {
 
 int64_t value_tiles(const DeltaArgs& a, int columns) { return (a.value_size + columns - 1) / columns; }
 
+bool narrow_walk(const DeltaArgs& a) { return a.segments == 1 && a.batch * a.heads * value_tiles(a, 64) <= 128; }
+
 // One walk; TRANSIT: of its segments, with the columns of the unit matrix.
-template <typename T, int DK, bool KEEP, bool TRANSIT>
+template <typename T, int DK, bool KEEP, bool TRANSIT, int W>
 hipError_t launch_walk(const DeltaArgs& a, hipStream_t stream) {
-  constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes;
+  constexpr int kBytes = 2 * Stage<T, DK, W>::kBytes;
   const auto kernel = delta_forward<T, DK, W, KEEP, TRANSIT>;
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
@@ -2138,9 +2144,9 @@ hipError_t launch_walk(const DeltaArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int DK, bool TRANSIT>
+template <typename T, int DK, bool TRANSIT, int W>
 hipError_t launch_walk_back(const DeltaArgs& a, hipStream_t stream) {
-  constexpr int W = 4, kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
+  constexpr int kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
   const auto kernel = delta_backward<T, DK, W, TRANSIT>;
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
@@ -2168,11 +2174,13 @@ hipError_t launch_forward(const DeltaArgs& a, const DeltaPlan& p, hipStream_t st
   }
   hipError_t err = a.chunks > 0 ? launch_prepare<T, DK>(a, stream) : hipSuccess;
   if (err == hipSuccess && a.segments > 1) {
-    err = launch_walk<T, DK, false, true>(a, stream);
+    err = launch_walk<T, DK, false, true, 4>(a, stream);
     if (err == hipSuccess) err = launch_join<DK, false>(a, stream);
   }
   if (err != hipSuccess) return err;
-  return a.states != nullptr ? launch_walk<T, DK, true, false>(a, stream) : launch_walk<T, DK, false, false>(a, stream);
+  if (narrow_walk(a))
+    return a.states != nullptr ? launch_walk<T, DK, true, false, 2>(a, stream) : launch_walk<T, DK, false, false, 2>(a, stream);
+  return a.states != nullptr ? launch_walk<T, DK, true, false, 4>(a, stream) : launch_walk<T, DK, false, false, 4>(a, stream);
 }
 
 template <typename T, int DK, bool GROUPED>
@@ -2193,10 +2201,10 @@ template <typename T, int DK>
 hipError_t launch_backward(const DeltaArgs& a, hipStream_t stream) {
   hipError_t err = hipSuccess;
   if (a.segments > 1) {
-    err = launch_walk_back<T, DK, true>(a, stream);
+    err = launch_walk_back<T, DK, true, 4>(a, stream);
     if (err == hipSuccess) err = launch_join<DK, true>(a, stream);
   }
-  if (err == hipSuccess) err = launch_walk_back<T, DK, false>(a, stream);
+  if (err == hipSuccess) err = narrow_walk(a) ? launch_walk_back<T, DK, false, 2>(a, stream) : launch_walk_back<T, DK, false, 4>(a, stream);
   if (err != hipSuccess || a.chunks == 0) return err;
   return a.heads == a.key_heads ? launch_gradients<T, DK, false>(a, stream) : launch_gradients<T, DK, true>(a, stream);
 }
