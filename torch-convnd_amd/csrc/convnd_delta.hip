@@ -95,8 +95,8 @@ struct Reader {
   unsigned rows[4], operands[kHalf ? 4 : 1], columns[4], ordered[kHalf ? 8 : 1];
 
   // `flip` goes into the places of ordered columns (64: two tiles further in a panel).
-  __device__ __forceinline__ explicit Reader(unsigned flip = 0) {
-    const unsigned l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  __device__ __forceinline__ explicit Reader(unsigned flip = 0, unsigned thread = threadIdx.x) {
+    const unsigned l = thread & 15, g = (thread >> 4) & 3;
     const auto bit = [](unsigned v, int i) { return v >> i & 1; };
 #pragma unroll
     for (unsigned x = 0; x < 4; ++x)  // halves of a panel's rows, odd tiles
@@ -195,8 +195,8 @@ struct Own {
   static constexpr int kPanel = Chunk<T>::kPanel;
   unsigned rows[2], columns[kHalf ? 2 : 4], place;
 
-  __device__ __forceinline__ explicit Own(int tile) {
-    const int l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, r = tile * 16 + l;
+  __device__ __forceinline__ explicit Own(int tile, int thread = threadIdx.x) {
+    const int l = thread & 15, g = (thread >> 4) & 3, r = tile * 16 + l;
 #pragma unroll
     for (int x = 0; x < 2; ++x) rows[x] = r * 128 + (((x * 4 + g) ^ swizzle(r)) << 4);
     // Of the first four values of a lane's (tile 0 of 16, four a lane group).
@@ -220,6 +220,7 @@ struct Own {
     Own r = *this;
     for (unsigned& at : r.rows) at += by;
     for (unsigned& at : r.columns) at += by;
+    r.place += by;
     return r;
   }
   __device__ __forceinline__ frag row(unsigned panels, int ks) const {
@@ -1458,8 +1459,15 @@ struct GradientsLds {
     unsigned char record[kRecord];
   } blocks[2];
   unsigned char keys[kWide], queries[kWide];
+  unsigned char values[C::kPanel];  // of the block at work
   float slope[2][C::kTokens], kept[2][C::kTokens], step[2][C::kTokens], inner[2 * C::kTiles];
 };
+
+// Waits for loads with COUNT or more after them.
+template <int COUNT>
+__device__ __forceinline__ void wait_older_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory");
+}
 
 // What a wave does that makes the pairs with its tokens as rows (HALF 0) or columns (1), of the first (SIDE 0) or
 // the second fragment of the chunk's tokens: all of it is known to the compiler but the tokens.
@@ -1474,19 +1482,22 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   auto& kept = lds.kept;
   auto& step = lds.step;
   auto& inner = lds.inner;
-  const Lane lane;
+  // This thread, as a value that the compiler takes for another one each time: what follows from a lane's place is
+  // made where it is used. Kept from one chunk to the next (or one phase), it took registers that then spilled,
+  // and a wait for a reload is one for the next block's loads too.
+  const auto again = []() __attribute__((always_inline)) {
+    int thread = threadIdx.x & 63;
+    asm volatile("" : "+v"(thread));
+    return thread;
+  };
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int half = HALF;
   const int block = wave % kTiles;
   // The wave's keys: from a panel of its half on, or (64 keys of 16 bits) from the middle of the only one.
   constexpr bool kFlip = DK / 2 * sizeof(T) < 128;
-  const Reader<T> read(kFlip ? half * 64 : 0);
-  const Own<T> mine(block);
   constexpr unsigned kWide = kPanels * C::kPanel, kNarrow = 2 * kWide, kHalf = kFlip ? 0 : half * (kWide / 2);
   const int groups = GROUPED ? a.groups : 1;
-  const int own_token = block * 16 + lane.l;  // this lane's in the chunk
   const int key_size = static_cast<int>(a.key_size), value_size = static_cast<int>(a.value_size);
-  const int first_key = half * (DK / 2) + lane.g * 4;  // of the lane's four in the wave's first tile
   const auto store_gate = [&](void* p, int64_t at, float v) __attribute__((always_inline)) {
     if (a.float_gates)
       static_cast<float*>(p)[at] = v;
@@ -1502,6 +1513,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   const unsigned items = static_cast<unsigned>(a.batch) * key_heads * chunks;
   const auto item_from = [&](unsigned id) __attribute__((always_inline)) {
     Item it{id, 0, 0, 0, 0, 0};
+    const int thread = again(), own_token = block * 16 + (thread & 15), first_key = half * (DK / 2) + (thread >> 4) * 4;
     for (; it.id < items; it.id += gridDim.x) {
       const unsigned row = it.id / chunks, sequence = row / key_heads;
       it.chunk = static_cast<int>(it.id - row * chunks);
@@ -1521,7 +1533,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         store_four(static_cast<T*>(a.grad_query) + to, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
         store_four(static_cast<T*>(a.grad_key) + to, f32x4{0.f, 0.f, 0.f, 0.f}, key_size - d);
       }
-      if (lane.g == 0 && half == 0)
+      if (thread < 16 && half == 0)
         for (int group = 0; group < groups; ++group) {
           store_gate(a.grad_decay, token * a.heads + it.kh * groups + group, 0.f);
           store_gate(a.grad_beta, token * a.heads + it.kh * groups + group, 0.f);
@@ -1530,7 +1542,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     return it;
   };
   // Four neighbouring values of this lane's row, in the wave's tile m.
-  const auto own_values = [&](unsigned panels, int m) __attribute__((always_inline)) {
+  const auto own_values = [&](const Own<T>& mine, unsigned panels, int m) __attribute__((always_inline)) {
     if constexpr (kFlip) return half == 0 ? mine.four(panels, m) : mine.four(panels, m + kKeyTiles);
     return mine.four(panels, m);
   };
@@ -1551,10 +1563,10 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
   // one is worked on.
   // Every wave loads 8 rows of each panel.
   static_assert(kWaves == kTokens / 8, "a load a wave");
-  const int load_row = wave * 8 + (threadIdx.x & 63) / 8;
-  const unsigned load_piece = ((threadIdx.x % 8) ^ swizzle(load_row)) << 4;
-  const auto load_set = [&](const void* from, unsigned dst, int count, unsigned column, unsigned stride, int rows,
-                            unsigned bytes) __attribute__((always_inline)) {
+  const auto load_set = [&](int thread, const void* from, unsigned dst, int count, unsigned column, unsigned stride,
+                            int rows, unsigned bytes) __attribute__((always_inline)) {
+    const int load_row = wave * 8 + thread / 8;
+    const unsigned load_piece = ((thread % 8) ^ swizzle(load_row)) << 4;
     const u32x4 buffer = buffer_at(from);
     const unsigned at = load_row < rows ? load_row * stride : kNowhere;
 #pragma unroll
@@ -1563,45 +1575,45 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       load_lds16(buffer, dst + p * C::kPanel + wave * 1024, in_row < bytes ? at + in_row : kNowhere);
     }
   };
-  const auto load = [&](const Item& it, int group, int v0, int into) __attribute__((always_inline)) {
-    const int h = it.kh * groups + group;
+  // As many loads whether there is a block or not (zeros, then), since waits count them.
+  constexpr int kLoads = 2 * kPanels + 3;
+  const auto load = [&](const Item& it, int group, int v0, int into, bool live) __attribute__((always_inline)) {
+    const int h = it.kh * groups + group, thread = again();
     const int64_t at = (static_cast<int64_t>(it.b) * a.heads + h) * chunks + it.chunk;
     auto& to = lds.blocks[into & 1];
-    const int left = static_cast<int>(a.value_pad) - v0, v_rows = left < kTokens ? left : kTokens;
+    const int left = static_cast<int>(a.value_pad) - v0, v_rows = !live ? 0 : left < kTokens ? left : kTokens;
     const int64_t v_at = at * a.value_pad + v0;
-    load_set(static_cast<const T*>(a.states) + v_at * DK, lds_address(to.wide[0]), kPanels, 0, DK * sizeof(T), v_rows,
+    load_set(thread, static_cast<const T*>(a.states) + v_at * DK, lds_address(to.wide[0]), kPanels, 0, DK * sizeof(T), v_rows,
              DK * sizeof(T));
-    load_set(static_cast<const T*>(a.grad_states) + v_at * DK, lds_address(to.wide[1]), kPanels, 0, DK * sizeof(T),
+    load_set(thread, static_cast<const T*>(a.grad_states) + v_at * DK, lds_address(to.wide[1]), kPanels, 0, DK * sizeof(T),
              v_rows, DK * sizeof(T));
-    load_set(static_cast<const T*>(a.updates) + v_at * kTokens, lds_address(to.narrow[0]), 1, 0, 128, v_rows, 128);
-    load_set(static_cast<const T*>(a.grad_updates) + v_at * kTokens, lds_address(to.narrow[1]), 1, 0, 128, v_rows, 128);
-    load_set(at_token<T>(a.grad_output, a.grad_strides, it.b, it.t0, h), lds_address(to.narrow[2]), 1,
-             static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)), it.rows,
+    load_set(thread, static_cast<const T*>(a.updates) + v_at * kTokens, lds_address(to.narrow[0]), 1, 0, 128, v_rows, 128);
+    load_set(thread, static_cast<const T*>(a.grad_updates) + v_at * kTokens, lds_address(to.narrow[1]), 1, 0, 128, v_rows, 128);
+    load_set(thread, at_token<T>(a.grad_output, a.grad_strides, it.b, it.t0, h), lds_address(to.narrow[2]), 1,
+             static_cast<unsigned>(v0 * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)), live ? it.rows : 0,
              static_cast<unsigned>(value_size * sizeof(T)));
     if (wave < GradientsLds<T, DK>::kRecord / 1024) {
-      const unsigned at_byte = wave * 1024 + (threadIdx.x & 63) * 16;
+      const unsigned at_byte = wave * 1024 + thread * 16;
       load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + at), lds_address(to.record) + wave * 1024,
-                 at_byte < sizeof(Record<T>) ? at_byte : kNowhere);
+                 live && at_byte < sizeof(Record<T>) ? at_byte : kNowhere);
     }
   };
   const auto load_keys = [&](const Item& it) __attribute__((always_inline)) {
     const unsigned bytes = static_cast<unsigned>(key_size * sizeof(T));
-    load_set(at_token<T>(a.key, a.key_strides, it.b, it.t0, it.kh), lds_address(lds.keys), kPanels, 0,
+    const int thread = again();
+    load_set(thread, at_token<T>(a.key, a.key_strides, it.b, it.t0, it.kh), lds_address(lds.keys), kPanels, 0,
              static_cast<unsigned>(a.key_strides.token * sizeof(T)), it.rows, bytes);
-    load_set(at_token<T>(a.query, a.query_strides, it.b, it.t0, it.kh), lds_address(lds.queries), kPanels, 0,
+    load_set(thread, at_token<T>(a.query, a.query_strides, it.b, it.t0, it.kh), lds_address(lds.queries), kPanels, 0,
              static_cast<unsigned>(a.query_strides.token * sizeof(T)), it.rows, bytes);
   };
   int index = 0;  // of the block, over all items
   Item it = item_from(blockIdx.x);
-  if (it.id < items) load(it, 0, 0, 0);
+  if (it.id < items) load(it, 0, 0, 0, true);
+  wait_loads();
 #pragma unroll 1
   while (it.id < items) {
     const Item next = item_from(it.id + gridDim.x);
     const int t0 = it.t0, kh = it.kh, b = it.b, rows = it.rows;
-    const int64_t token = static_cast<int64_t>(b) * a.tokens + t0 + own_token;
-    const bool in_range = t0 + own_token < a.tokens;
-    T* dq_out = static_cast<T*>(a.grad_query) + (token * a.key_heads + kh) * key_size;
-    T* dk_out = static_cast<T*>(a.grad_key) + (token * a.key_heads + kh) * key_size;
     f32x4 dq_all[GROUPED ? kKeyTiles : 1], dk_all[GROUPED ? kKeyTiles : 1];
     if constexpr (GROUPED) {
 #pragma unroll
@@ -1610,9 +1622,6 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
 #pragma unroll 1
   for (int group = 0; group < groups; ++group) {
     const int h = kh * groups + group;
-    // The compiler is not to keep what follows from a lane's place from one chunk to the next: registers spilled.
-    int own = own_token, first = lane.g;
-    asm volatile("" : "+v"(own), "+v"(first));
     f32x4 dq[kKeyTiles], dk[kKeyTiles], back[kKeyTiles];  // dO S^T, Y S^T, U D^T
 #pragma unroll
     for (int m = 0; m < kKeyTiles; ++m) dq[m] = dk[m] = back[m] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1620,35 +1629,51 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) pair_p[m] = pair_a[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     float dbeta = 0.f, product = 0.f;
-    const T* value = at_token<T>(a.value, a.value_strides, b, t0 + own, h);
     unsigned here = 0;
+    const int at_blocks = again();
+    Reader<T> read(kFlip ? half * 64 : 0, at_blocks);
+    Own<T> mine(block, at_blocks);
 #pragma unroll 1
     for (int v0 = 0; v0 < a.value_pad; v0 += kTokens, ++index) {
-      wait_loads();
+      // What a first block needs was waited for before the results before it were stored.
+      if (v0 > 0) wait_loads();
       __syncthreads();
+      if constexpr (HALF == 0) {  // the wave's own rows of the values
+        const u32x4 buffer = buffer_at(at_token<T>(a.value, a.value_strides, b, t0, h));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int thread = again(), row = block * 16 + i * 8 + thread / 8;
+          const unsigned in_row = static_cast<unsigned>(v0 * sizeof(T)) + (((thread % 8) ^ swizzle(row)) << 4);
+          load_lds16(buffer, lds_address(lds.values) + (block * 2 + i) * 1024,
+                     row < rows && in_row < static_cast<unsigned>(value_size * sizeof(T))
+                         ? row * static_cast<unsigned>(a.value_strides.token * sizeof(T)) + in_row
+                         : kNowhere);
+        }
+      }
       if (group == 0 && v0 == 0) load_keys(it);
       if (v0 + kTokens < a.value_pad)
-        load(it, group, v0 + kTokens, index + 1);
+        load(it, group, v0 + kTokens, index + 1, true);
       else if (group + 1 < groups)
-        load(it, group + 1, 0, index + 1);
-      else if (next.id < items)
-        load(next, 0, 0, index + 1);
-      here = lds_address(&lds.blocks[index & 1]);
-      const Reader<T> there = read.moved(here);
-      const Own<T> own_there = mine.moved(here);
+        load(it, group + 1, 0, index + 1, true);
+      else
+        load(next, 0, 0, index + 1, next.id < items);
+      const unsigned to = lds_address(&lds.blocks[index & 1]);
+      read = read.moved(to - here);
+      mine = mine.moved(to - here);
+      here = to;
       // Fragments in the order of their products, read kAheadGrad before them.
       constexpr int kStep = 3 + 2 * kKeyTiles + kOthers;
       frag of[2 * kStep];
       const auto fetch = [&](int i) __attribute__((always_inline)) {
         if (i >= 2 * kStep) return;
         const int kt = i / kStep, k = i % kStep, n = k - 3 - 2 * kKeyTiles;
-        of[i] = k == 0   ? own_there.row(kNarrow + 2 * C::kPanel, kt)
-                : k == 1 ? own_there.column(kNarrow, kt)
-                : k == 2 ? own_there.column(kNarrow + C::kPanel, kt)
-                : n < 0  ? there.ordered_column((k - 3) % 2 * kWide + kHalf, (k - 3) / 2, kt)
-                : HALF == 0  ? there.column(kNarrow, kFirstOther + n, kt)
-                : n % 2 == 0 ? there.operand(kNarrow + 2 * C::kPanel, kFirstOther + n / 2, kt)
-                             : there.column(kNarrow + C::kPanel, kFirstOther + n / 2, kt);
+        of[i] = k == 0   ? mine.row(kNarrow + 2 * C::kPanel, kt)
+                : k == 1 ? mine.column(kNarrow, kt)
+                : k == 2 ? mine.column(kNarrow + C::kPanel, kt)
+                : n < 0  ? read.ordered_column((k - 3) % 2 * kWide + kHalf, (k - 3) / 2, kt)
+                : HALF == 0  ? read.column(kNarrow, kFirstOther + n, kt)
+                : n % 2 == 0 ? read.operand(kNarrow + 2 * C::kPanel, kFirstOther + n / 2, kt)
+                             : read.column(kNarrow + C::kPanel, kFirstOther + n / 2, kt);
       };
 #pragma unroll
       for (int i = 0; i < kAheadGrad; ++i) fetch(i);
@@ -1684,12 +1709,10 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
           keep_order();
         }
         if constexpr (HALF == 0) {
-          const int v = v0 + kt * C::kStep + lane.g * kVec;
-          if (own < rows && v < value_size) {
-            const frag f = __builtin_bit_cast(frag, load_run<kVec>(value + v));
+          if (kt == 0) wait_older_loads<kLoads>();
+          const frag f = lds_read<frag>(lds_address(lds.values) - here + mine.rows[kt]);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) dbeta = fmaf(static_cast<float>(f[i]), static_cast<float>(y[i]), dbeta);
-          }
+          for (int i = 0; i < kVec; ++i) dbeta = fmaf(static_cast<float>(f[i]), static_cast<float>(y[i]), dbeta);
         }
       }
       // The state's product with its gradient.
@@ -1701,7 +1724,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       }
     }
     if (group == 0 && a.value_pad <= kTokens) {  // the keys are under way still
-      wait_loads();
+      wait_older_loads<kLoads>();
       __syncthreads();
     }
     product = lanes_sum<64>(product);
@@ -1709,12 +1732,14 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     const auto* facts = reinterpret_cast<const Record<T>*>(lds.blocks[(index - 1) & 1].record);
     const double* sum = facts->sum;
     const float *beta = facts->beta, *rk = facts->rk, *rq = facts->rq;
-    const float norm = facts->norm[own];
     const uint64_t closed = facts->closed;
-    const unsigned keys = lds_address(lds.keys), queries = lds_address(lds.queries);
-    const unsigned states = keys + kHalf, grads = queries + kHalf;  // of the wave's keys
+    const int thread = again(), own = block * 16 + (thread & 15), first = thread >> 4;
+    const Reader<T> key_read = Reader<T>(kFlip ? half * 64 : 0, thread).moved(lds_address(lds.keys));
+    const Own<T> key_mine = Own<T>(block, thread).moved(lds_address(lds.keys));
+    constexpr unsigned keys = 0, queries = kWide;
+    constexpr unsigned states = keys + kHalf, grads = queries + kHalf;  // of the wave's keys
     const double own_sum = sum[own];
-    const float own_beta = beta[own], own_rk = rk[own], own_rq = rq[own];
+    const float own_beta = beta[own], own_rk = rk[own], own_rq = rq[own], norm = facts->norm[own];
 
     dbeta = over_groups(dbeta);
     float dsum;
@@ -1725,7 +1750,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       float q_dot = 0.f, k_dot = 0.f, b_dot = 0.f;
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
-        const f32x4 q = own_values(grads, m), k = own_values(states, m);
+        const f32x4 q = own_values(key_mine, grads, m), k = own_values(key_mine, states, m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           q_dot = fmaf(q[e], dq[m][e], q_dot);
@@ -1740,7 +1765,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       b_dot = over_groups(b_dot) * e_own * own_rk;
       dbeta -= k_dot;
       dsum = q_dot - own_beta * k_dot - b_dot;
-      if (lane.g == 0) kept[half][own] = b_dot;
+      if (first == 0) kept[half][own] = b_dot;
     }
     // Pairs.
     f32x4 kk[kTiles], qk[kTiles];
@@ -1752,11 +1777,11 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       const auto fetch = [&](int i) __attribute__((always_inline)) {
         if (i >= kSteps * kStep) return;
         const int ks = i / kStep, k = i % kStep, n = k - 2;
-        of[i] = k == 0       ? mine.row(keys, ks)
-                : k == 1     ? mine.row(queries, ks)
-                : HALF == 0  ? read.operand(keys, kFirstOther + n, ks)
-                : n % 2 == 0 ? read.operand(keys, kFirstOther + n / 2, ks)
-                             : read.operand(queries, kFirstOther + n / 2, ks);
+        of[i] = k == 0       ? key_mine.row(keys, ks)
+                : k == 1     ? key_mine.row(queries, ks)
+                : HALF == 0  ? key_read.operand(keys, kFirstOther + n, ks)
+                : n % 2 == 0 ? key_read.operand(keys, kFirstOther + n / 2, ks)
+                             : key_read.operand(queries, kFirstOther + n / 2, ks);
       };
 #pragma unroll
       for (int i = 0; i < kAheadGrad; ++i) fetch(i);
@@ -1820,13 +1845,13 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     } else {
       dsum -= (pairs + steps) * own_rk;
     }
-    if (lane.g == 0) {
+    if (first == 0) {
       slope[half][own] = dsum;
       step[half][own] = dbeta;
     }
     // The pairs as fragments, for both waves of these tokens: three of each kind.
     __syncthreads();  // all have read U, Y and dO
-    frag* shared = reinterpret_cast<frag*>(lds.blocks[(index - 1) & 1].narrow[0]) + block * 6 * 64 + (threadIdx.x & 63);
+    frag* shared = reinterpret_cast<frag*>(lds.blocks[(index - 1) & 1].narrow[0]) + block * 6 * 64 + thread;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       if (!has(kt * kPer)) continue;
@@ -1844,9 +1869,9 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         if (i >= 4 * kKeyTiles) return;
         const int kt = i / (2 * kKeyTiles), m = i % (2 * kKeyTiles) / 2;
         if (i % 2 == 0)
-          of[i] = read.ordered_column(states, m, kt);
+          of[i] = key_read.ordered_column(states, m, kt);
         else if (kt >= SIDE)
-          of[i] = read.ordered_column(grads, m, kt);
+          of[i] = key_read.ordered_column(grads, m, kt);
       };
       frag weights[2][4];
 #pragma unroll
@@ -1877,9 +1902,11 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         }
       }
     }
+    // The next block is there, long since: waited for here, so that no wait is for the stores that follow.
+    wait_loads();
     if (wave == 0) {
       // A token's decay: the gradients of the sums from it on, the last of which has the states' too.
-      const int t = threadIdx.x & 63;
+      const int t = thread;
       float v = 0.f, k = 0.f;
       if (t < kTokens) {
         v = slope[0][t] + slope[1][t];
@@ -1916,7 +1943,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     if (a.normalize) {
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
-        const f32x4 q = own_values(grads, m), k = own_values(states, m);
+        const f32x4 q = own_values(key_mine, grads, m), k = own_values(key_mine, states, m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           q_dot = fmaf(q[e], dqs[m][e], q_dot);
@@ -1926,7 +1953,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       q_dot = over_groups(q_dot);
       k_dot = over_groups(k_dot);
       __syncthreads();  // the decays' sums are read
-      if (lane.g == 0) {
+      if (first == 0) {
         slope[half][own] = q_dot;
         step[half][own] = k_dot;
       }
@@ -1934,12 +1961,16 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       q_dot = (slope[0][own] + slope[1][own]) * norm * norm;
       k_dot = (step[0][own] + step[1][own]) * own_rk * own_rk;
     }
-    if (in_range) {
+    if (t0 + own < a.tokens) {
+      const int64_t row = (static_cast<int64_t>(b) * a.tokens + t0 + own) * a.key_heads + kh;
+      T* dq_out = static_cast<T*>(a.grad_query) + row * key_size;
+      T* dk_out = static_cast<T*>(a.grad_key) + row * key_size;
+      const int first_key = half * (DK / 2) + first * 4;
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
         const int d = first_key + m * 16;
         if (d >= key_size) continue;
-        const f32x4 q = own_values(grads, m), k = own_values(states, m);
+        const f32x4 q = own_values(key_mine, grads, m), k = own_values(key_mine, states, m);
         store_four(dq_out + d, own_rq * (dqs[m] - q_dot * q), key_size - d);
         store_four(dk_out + d, own_rk * (dks[m] - k_dot * k), key_size - d);
       }
