@@ -598,12 +598,20 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
         if (jb > wave) continue;
         const int j = jb * 16 + l;
         const double earlier = sum[j];
+        const float own_rk = rk[j];
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = wave * 16 + g * 4 + e;
-          v[e] = i > j && (closed == 0 || open_between(closed, j, i)) ? up[e] * rk[j] * decay_between(later[e], earlier) * kk[jb][e]
-                                                     : 0.f;
+          const float pair = up[e] * own_rk * decay_between(later[e], earlier) * kk[jb][e];
+          v[e] = i > j ? pair : 0.f;
+        }
+        if (closed != 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = wave * 16 + g * 4 + e;
+            if (i > j && !open_between(closed, j, i)) v[e] = 0.f;
+          }
         }
         *reinterpret_cast<f32x4*>(&lds.solve.rest[j][wave * 16 + g * 4]) = v;
       }
@@ -612,6 +620,7 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
       // P: lane's row i, four columns; blocks past the diagonal as far as a fragment reaches.
       const int i = wave * 16 + l;
       const double later = sum[i];
+      const float own_rq = rq[i];
       T* p = panels + C::kTerms * kTokens * kTokens + i * kTokens + g * 4;
 #pragma unroll
       for (int jb = 0; jb < kTiles; ++jb) {
@@ -620,8 +629,15 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = jb * 16 + g * 4 + e;
-          v[e] = i >= j && (closed == 0 || open_between(closed, j, i)) ? rq[i] * rk[j] * decay_between(later, sum[j]) * qk[jb][e]
-                                                      : 0.f;
+          const float pair = own_rq * rk[j] * decay_between(later, sum[j]) * qk[jb][e];
+          v[e] = i >= j ? pair : 0.f;
+        }
+        if (closed != 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = jb * 16 + g * 4 + e;
+            if (i >= j && !open_between(closed, j, i)) v[e] = 0.f;
+          }
         }
 #pragma unroll
         for (int term = 0; term < C::kTerms; ++term) {
@@ -1448,6 +1464,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 // adds up its value heads. Two waves share 16 tokens, which are their lanes throughout: each makes half of the
 // keys' gradients, and one makes the pairs with its token as the row i (registers j), the other those with it
 // as the column j (registers i), so that either is the operand of the next products, which they exchange.
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 template <typename T, int DK>
 struct GradientsLds {
   using C = Chunk<T>;
@@ -1651,12 +1668,11 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         }
       }
       if (group == 0 && v0 == 0) load_keys(it);
-      if (v0 + kTokens < a.value_pad)
-        load(it, group, v0 + kTokens, index + 1, true);
-      else if (group + 1 < groups)
-        load(it, group + 1, 0, index + 1, true);
-      else
-        load(next, 0, 0, index + 1, next.id < items);
+      {
+        const bool more = v0 + kTokens < a.value_pad, stays = more || group + 1 < groups;
+        load(stays ? it : next, more ? group : stays ? group + 1 : 0, more ? v0 + kTokens : 0, index + 1,
+             stays || next.id < items);
+      }
       const unsigned to = lds_address(&lds.blocks[index & 1]);
       read = read.moved(to - here);
       mine = mine.moved(to - here);
@@ -1817,24 +1833,32 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         if (j <= i && open_between(closed, j, i)) open_bits |= 1u << n;
       }
     }
+    // Without branches: all is read and made, then chosen.
     float pairs = 0.f, steps = 0.f;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
       if (!has(m)) continue;
+      const int at = first_row<T>(m, first);
+      const f32x4 other_rk = *reinterpret_cast<const f32x4*>(rk + at);
+      const f32x4 other_rq = HALF == 0 ? other_rk : *reinterpret_cast<const f32x4*>(rq + at);
+      const f32x4 other_beta = HALF == 0 ? other_rk : *reinterpret_cast<const f32x4*>(beta + at);
+      const f64x2 other_sum[2] = {*reinterpret_cast<const f64x2*>(sum + at), *reinterpret_cast<const f64x2*>(sum + at + 2)};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int other = first_row<T>(m, first) + e;
-        const int i = half == 0 ? own : other, j = half == 0 ? other : own;
-        const bool open = i >= j && (open_bits >> (m * 4 + e) & 1) != 0;
-        const float ratio = open ? half == 0 ? decay_between(own_sum, sum[other]) : decay_between(sum[other], own_sum) : 0.f;
+        const int other = at + e;
+        const bool below = HALF == 0 ? own > other : other > own, open = (open_bits >> (m * 4 + e) & 1) != 0;
+        const double to = other_sum[e / 2][e % 2];
+        const float ratio = HALF == 0 ? decay_between(own_sum, to) : decay_between(to, own_sum);
         // The other token's factors; this one's are taken out of the sums.
-        const float p = open ? ratio * (half == 0 ? rk[other] : rq[other]) * pair_p[m][e] : 0.f;
-        const float n = open && i > j ? -ratio * rk[other] * pair_a[m][e] : 0.f;
-        const float weighed = half == 0 ? n : n * beta[other];
+        float p = ratio * (HALF == 0 ? other_rk[e] : other_rq[e]) * pair_p[m][e];
+        float n = -ratio * other_rk[e] * pair_a[m][e];
+        p = open & (below | (own == other)) ? p : 0.f;
+        n = open & below ? n : 0.f;
+        const float weighed = HALF == 0 ? n : n * other_beta[e];
         pairs = fmaf(p, qk[m][e], pairs);
         steps = fmaf(weighed, kk[m][e], steps);
         pair_p[m][e] = p;
-        pair_a[m][e] = half == 0 ? own_beta * n : weighed;
+        pair_a[m][e] = HALF == 0 ? own_beta * n : weighed;
       }
     }
     pairs = over_groups(pairs);
@@ -1904,7 +1928,9 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     }
     // The next block is there, long since: waited for here, so that no wait is for the stores that follow.
     wait_loads();
-    if (wave == 0) {
+    // (By one wave, which the others need not wait for.)
+    const auto store_gates = [&]() __attribute__((always_inline)) {
+      if (wave != 0) return;
       // A token's decay: the gradients of the sums from it on, the last of which has the states' too.
       const int t = thread;
       float v = 0.f, k = 0.f;
@@ -1927,7 +1953,7 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         store_gate(a.grad_decay, to, t < rows && (closed >> t & 1) == 0 ? v : 0.f);
         store_gate(a.grad_beta, to, t < rows ? step[0][t] + step[1][t] : 0.f);
       }
-    }
+    };
     if constexpr (GROUPED) {
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
@@ -1935,7 +1961,10 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         dk_all[m] += dk[m];
       }
     }
-    if (GROUPED && group + 1 < groups) continue;
+    if (GROUPED && group + 1 < groups) {
+      store_gates();
+      continue;
+    }
     // q = q' / rq and k = k' / rk, with their lengths.
     const f32x4* dqs = GROUPED ? dq_all : dq;
     const f32x4* dks = GROUPED ? dk_all : dk;
@@ -1952,29 +1981,32 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
       }
       q_dot = over_groups(q_dot);
       k_dot = over_groups(k_dot);
-      __syncthreads();  // the decays' sums are read
+      float* dots = reinterpret_cast<float*>(lds.values);  // [2][2][kTokens]
       if (first == 0) {
-        slope[half][own] = q_dot;
-        step[half][own] = k_dot;
+        dots[half * kTokens + own] = q_dot;
+        dots[(2 + half) * kTokens + own] = k_dot;
       }
       __syncthreads();
-      q_dot = (slope[0][own] + slope[1][own]) * norm * norm;
-      k_dot = (step[0][own] + step[1][own]) * own_rk * own_rk;
+      q_dot = (dots[own] + dots[kTokens + own]) * norm * norm;
+      k_dot = (dots[2 * kTokens + own] + dots[3 * kTokens + own]) * own_rk * own_rk;
     }
     if (t0 + own < a.tokens) {
       const int64_t row = (static_cast<int64_t>(b) * a.tokens + t0 + own) * a.key_heads + kh;
       T* dq_out = static_cast<T*>(a.grad_query) + row * key_size;
       T* dk_out = static_cast<T*>(a.grad_key) + row * key_size;
       const int first_key = half * (DK / 2) + first * 4;
+      const bool whole = key_size % 4 == 0;
 #pragma unroll
       for (int m = 0; m < kKeyTiles; ++m) {
         const int d = first_key + m * 16;
-        if (d >= key_size) continue;
         const f32x4 q = own_values(key_mine, grads, m), k = own_values(key_mine, states, m);
-        store_four(dq_out + d, own_rq * (dqs[m] - q_dot * q), key_size - d);
-        store_four(dk_out + d, own_rk * (dks[m] - k_dot * k), key_size - d);
+        const f32x4 to_q = own_rq * (dqs[m] - q_dot * q), to_k = own_rk * (dks[m] - k_dot * k);
+        if (d >= key_size) continue;
+        store_four(dq_out + d, to_q, whole ? 4 : key_size - d);
+        store_four(dk_out + d, to_k, whole ? 4 : key_size - d);
       }
     }
+    store_gates();
   }
     it = next;
   }
