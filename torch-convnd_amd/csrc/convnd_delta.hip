@@ -80,6 +80,10 @@ template <typename V>
 __device__ __forceinline__ V lds_read(unsigned at) {
   return *reinterpret_cast<__attribute__((address_space(3))) const V*>(static_cast<uintptr_t>(at));
 }
+template <typename V>
+__device__ __forceinline__ void lds_write(unsigned at, const V& v) {
+  *reinterpret_cast<__attribute__((address_space(3))) V*>(static_cast<uintptr_t>(at)) = v;
+}
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
 }
@@ -347,8 +351,8 @@ __device__ __forceinline__ void load_panels(u32x4 buffer, unsigned dst, int coun
 // The same with the lane's places made once, for a walk over chunks: COUNT panels by W waves.
 template <typename T, int COUNT, int W>
 struct PanelLoads {
-  static constexpr int kLoads = Chunk<T>::kTokens / 8, kMine = COUNT * kLoads / W;
-  static_assert(COUNT * kLoads % W == 0, "as many loads a wave");
+  static constexpr int kLoads = Chunk<T>::kTokens / 8, kAll = COUNT * kLoads, kMine = (kAll + W - 1) / W;
+  static_assert(kAll % W == 0 || kAll < W, "as many loads a wave, or one of some");
   unsigned offset[kMine];
   __device__ __forceinline__ static int row(int j, int wave) {
     return (j * W + wave) % kLoads * 8 + static_cast<int>(threadIdx.x & 63) / 8;
@@ -372,6 +376,7 @@ struct PanelLoads {
     }
   }
   __device__ __forceinline__ void load(u32x4 buffer, unsigned dst, int wave, int rows) const {
+    if (kAll < W && wave >= kAll) return;
     if (rows == Chunk<T>::kTokens) {
 #pragma unroll
       for (int j = 0; j < kMine; ++j) load_lds16(buffer, dst + (j * W + wave) * 1024, offset[j]);
@@ -382,6 +387,12 @@ struct PanelLoads {
     }
   }
 };
+
+// Waits for loads with COUNT or more after them.
+template <int COUNT>
+__device__ __forceinline__ void wait_older_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory");
+}
 
 // A wave's own exchange through LDS: what its lanes wrote is there for the others.
 __device__ __forceinline__ void wait_own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -755,27 +766,60 @@ struct Triangle {
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x40); }
 constexpr int kAhead = 10;  // of the 15 that may be under way
 
-// A wave keeps 16 columns of S in registers, as results [key, column] of the products that update it, and
-// walks through all of them by itself: K S, T R, P U and K^T U take its columns' values as one
-// operand straight from the results before (operand_row puts them in order) and the shared panels as the
-// other, from LDS, so waves meet only where panels change hands, once a chunk. The next chunk's panels
-// load meanwhile.
+// LDS of the walks forward: Q (and, where both do not fit twice, T and P) once, the other panels of a chunk twice,
+// and what a wave of states hands to its wave of outputs.
+template <typename T, int DK, int W, bool OUTPUTS>
+struct Walk {
+  using C = Chunk<T>;
+  static constexpr bool kTwice = W == 2 || !OUTPUTS;  // T and P
+  static constexpr int kKeyBytes = DK / C::kTokens * C::kPanel, kPairBytes = C::kTerms * C::kPanel;
+  static constexpr int kValuePanels = (W * 16 + C::kTokens - 1) / C::kTokens;
+  // Once.
+  static constexpr int kQuery = 0;
+  static constexpr int kSolveOnce = kQuery + (OUTPUTS ? kKeyBytes : 0);
+  static constexpr int kPairsOnce = kSolveOnce + (kTwice ? 0 : kPairBytes);
+  static constexpr int kStages = kPairsOnce + (kTwice ? 0 : kPairBytes);
+  // In a stage.
+  static constexpr int kKeys = 0;
+  static constexpr int kSolve = kKeys + kKeyBytes;
+  static constexpr int kPairs = kSolve + (kTwice ? kPairBytes : 0);
+  static constexpr int kValues = kPairs + (kTwice && OUTPUTS ? kPairBytes : 0);
+  static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
+  static constexpr int kStage = kFactors + 2048;
+  // Handed on, for each wave: fragments of S and of U.
+  static constexpr int kState = kStages + 2 * kStage;
+  static constexpr int kStateBytes = DK / C::kStep * C::kTerms * 1024, kUpdateBytes = 2 * C::kTerms * 1024;
+  static constexpr int kUpdate = kState + W * kStateBytes;
+  static constexpr int kBytes = OUTPUTS ? kUpdate + W * kUpdateBytes : kState;
+  static_assert(W * 16 % C::kTokens == 0 || C::kTokens % (W * 16) == 0, "whole panels of values, or parts of one");
+  static_assert(kFactors <= 65536 && kStages <= 65536 && kBytes <= 163840, "constants of reads, and LDS");
+};
+
+// Two waves share 16 columns. One keeps S in registers, as results [key, column] of the products that update it,
+// and walks through all of them by itself: K S, T R and K^T U take its columns' values as one operand straight
+// from the results before (operand_row puts them in order) and the shared panels as the other, from LDS. The
+// other wave makes the outputs: while the first is at K S and T R it multiplies the S before the chunk, which it
+// is handed through LDS, with Q, and while the first updates S, P with U; it also stores outputs and what is kept
+// for a backward. Waves meet twice a chunk; panels load a chunk or half of one ahead. A walk is bound by the chain
+// from S to the next S (about 2 us a chunk; with the outputs in the same wave 3.9).
 template <typename T, int DK, int W, bool KEEP, bool TRANSIT>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_forward(DeltaArgs a) {
+__global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_waves_per_eu(
+    W == 4 && !TRANSIT ? 2 : 1, W == 4 && !TRANSIT ? 2 : 1))) void delta_forward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
-  using S = Stage<T, DK, W>;
+  using S = Walk<T, DK, W, !TRANSIT>;
   constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kTerms = C::kTerms, kPer = C::kPer;
-  constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
+  constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16, kWaves = TRANSIT ? W : 2 * W;
+  constexpr bool kTwice = S::kTwice;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
-  const Reader<T> places;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int thread = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
   const WalkPlace w(a, W * 16, TRANSIT ? DK : 0);
   const int64_t bh = w.bh;
   const int b = w.b, h = w.h, kh = w.kh;
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
-  const int v0 = w.v0, column = v0 + wave * 16;  // of the workgroup and the wave
+  const int v0 = w.v0, column = v0 + part * 16;  // of the workgroup and the wave
   const bool active = TRANSIT && w.unit ? true : column < value_size;
   const int mine = column + lane.l;
   const int length = length_of(a, b);
@@ -783,271 +827,358 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const int begin = w.segment * a.segment_chunks;
   const int end = all_chunks < begin + a.segment_chunks ? all_chunks : begin + a.segment_chunks;
   const int64_t first_chunk = bh * a.chunks, segment_at = bh * a.segments + w.segment;
-
-  f32x4 state[kStateTiles];
-#pragma unroll
-  for (int m = 0; m < kStateTiles; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = first_row<T>(m, lane.g) + e;
-      if constexpr (TRANSIT)
-        state[m][e] = w.unit && d == mine ? 1.f : 0.f;
-      else if (a.segments > 1)
-        state[m][e] = active ? a.starts[(segment_at * DK + d) * a.value_pad + mine] : 0.f;
-      else
-        state[m][e] = a.first != nullptr && d < key_size && mine < value_size
-                          ? a.first[(bh * key_size + d) * value_size + mine]
-                          : 0.f;
-    }
+  const unsigned lds_at = lds_address(lds);
 
   // Panels of values start at whole ones; the wave's columns lie within.
   const int from_panel = v0 % (S::kValuePanels * kTokens);
-  const Own<T> own(from_panel / 16 + wave);
-  const unsigned lds_at = lds_address(lds);
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
   const T* v_at = at_token<T>(a.value, a.value_strides, b, 0, h);
   const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
-  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
-  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
-  const PanelLoads<T, S::kValuePanels, W> value_loads(
+  const PanelLoads<T, DK / kTokens, kWaves> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, DK / kTokens, kWaves> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, S::kValuePanels, kWaves> value_loads(
       static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
       TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
-  const PanelLoads<T, (TRANSIT ? 1 : 2) * kTerms, W> pair_loads(wave);
-  auto load = [&](int c) __attribute__((always_inline)) {
-    const unsigned dst = lds_at + (c & 1) * S::kBytes;
+  const PanelLoads<T, kTerms, kWaves> pair_loads(wave);
+  const auto rows_of = [&](int c) __attribute__((always_inline)) {
+    const int64_t left = c < end ? length - static_cast<int64_t>(c) * kTokens : 0;
+    return left < kTokens ? static_cast<int>(left) : kTokens;
+  };
+  const auto load_solve = [&](int c, unsigned dst) __attribute__((always_inline)) {
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes)), dst, wave, c < end ? kTokens : 0);
+  };
+  const auto load_pairs = [&](int c, unsigned dst) __attribute__((always_inline)) {
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes) + S::kPairBytes), dst, wave,
+                    c < end ? kTokens : 0);
+  };
+  const auto load_query = [&](int c) __attribute__((always_inline)) {
+    query_loads.load(buffer_at(q_at + static_cast<int64_t>(c) * kTokens * a.query_strides.token), lds_at + S::kQuery, wave,
+                     rows_of(c));
+  };
+  // As many loads whether there is a chunk or not, since waits count them (but the factors').
+  constexpr int kStageLoads = (DK / kTokens + S::kValuePanels) * (kTokens / 8) / kWaves;
+  const auto load_stage = [&](int c) __attribute__((always_inline)) {
+    const unsigned dst = lds_at + S::kStages + (c & 1) * S::kStage;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
-    const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
+    const int rows = rows_of(c);
     key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
     value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, wave, rows);
-    if constexpr (!TRANSIT) query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
-    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
+    if constexpr (kTwice) {
+      load_solve(c, dst + S::kSolve);
+      if constexpr (!TRANSIT) load_pairs(c, dst + S::kPairs);
+    }
     if (wave < 2) {  // the factors, and after them `whole`
-      const unsigned at = wave * 16 * kTokens + (threadIdx.x & 63) * 16;
+      const unsigned at = wave * 16 * kTokens + thread * 16;
       load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
-                 dst + S::kFactors + wave * 1024, at < (wave == 0 ? 16 : 17) * kTokens ? at : kNowhere);
+                 dst + S::kFactors + wave * 1024, c < end && at < (wave == 0 ? 16 : 17) * kTokens ? at : kNowhere);
     }
   };
-
-  T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
-  const int64_t out_token = a.heads * value_size;
-  const int store_at = column + lane.g * 4, store_count = value_size - store_at;
-  // A chunk's results are stored while the next one is worked on: the wait for loads is for stores too.
-  const bool whole_rows = column + 16 <= value_size;
-  unsigned out_place[kTiles];
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
-  const unsigned state_place = mine * DK + lane.g * (16 / sizeof(T));
-  const unsigned update_place = mine * kTokens + lane.g * (16 / sizeof(T));
-  Four<T> held_output[kTiles];
-  frag held_update[2];
-  int held = -1;
-  const auto store_held = [&]() __attribute__((always_inline)) {
-    if (held < 0) return;
-    T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
-    if (whole_rows && (held + 1) * kTokens <= a.tokens) {
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) *reinterpret_cast<Run<T, 4>*>(to + out_place[n]) = __builtin_bit_cast(Run<T, 4>, held_output[n]);
-    } else {
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-        if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < store_count) to[out_place[n] + e] = held_output[n][e];
-          end_of_part();
-        }
-    }
-    if constexpr (KEEP) {
-      T* keep = static_cast<T*>(a.updates) + (first_chunk + held) * a.value_pad * kTokens;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
-    }
-  };
-  if (begin < end) load(begin);
-#pragma unroll 1
-  for (int c = begin; c < end; ++c) {
+  // What was loaded for this chunk is there, and the buffers of the one before are free.
+  const auto meet_at_start = [&](int c) __attribute__((always_inline)) {
     wait_loads();
     __syncthreads();
-    if (c + 1 < end) load(c + 1);
-    if (!active) continue;
-    if constexpr (!TRANSIT) store_held();
-    const unsigned at = lds_at + (c & 1) * S::kBytes;
-    const Reader<T> read = places.moved(at);
-    const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
-    const float whole = factors[256];
-
-    frag s[kSteps][kTerms];
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
-    if constexpr (KEEP) {
-      T* keep = static_cast<T*>(a.states) + (first_chunk + c) * a.value_pad * DK;
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
-    }
-
-    // The chunk's fragments in the order of their products, read kAhead of them before: K, Q, T, K^T, P.
-    // Neighbouring products are of different sums, since one waits for the last of its own sum.
-    constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
-    constexpr int kQueries = TRANSIT ? 0 : kRows;
-    frag kf[kRows], qf[kRows], tf[kTerms * kBlocks], pf[kTerms * kBlocks], cf[kColumns];
-    const auto fetch = [&](int i) __attribute__((always_inline)) {
-      if (i < kRows) {
-        kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
-      } else if ((i -= kRows) < kQueries) {
-        qf[i] = read.row(S::kQuery, i % kTiles, i / kTiles);
-      } else if ((i -= kQueries) < kTerms * kBlocks) {
-        const Triangle<T> b(i % kBlocks);
-        tf[i] = read.operand(S::kSolve + i / kBlocks * C::kPanel, b.tile, b.step);
-      } else if ((i -= kTerms * kBlocks) < kColumns) {
-        cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
-      } else if (!TRANSIT && (i -= kColumns) < kTerms * kBlocks) {
-        const Triangle<T> b(i % kBlocks);
-        pf[i] = read.row(S::kPairs + i / kBlocks * C::kPanel, b.tile, b.step);
-      }
-    };
-    constexpr int kFirstQ = kRows, kFirstT = kRows + kQueries, kFirstC = kFirstT + kTerms * kBlocks,
-                  kFirstP = kFirstC + kColumns;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(i);
-    keep_order();
-
-    // R = beta V - (beta c rk) K S.
-    Sum<T> sums[kTiles];
-#pragma unroll
-    for (int i = 0; i < kRows; i += kTiles) {
-#pragma unroll
-      for (int m = 0; m < kTiles; ++m) fetch(i + m + kAhead);
-#pragma unroll
-      for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) sums[m].add(kf[i + m], s[i / kTiles][term], term > 0);
-      keep_order();
-    }
-    f32x4 r[kTiles];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      const f32x4 acc = sums[m].value();
-      const f32x4 v = own.values(at + S::kValues, m);
-      const int row = first_row<T>(m, lane.g);
-      const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[e], -take[e] * acc[e]);
-      sums[m] = Sum<T>();
-    }
-    // Q S: O's lanes are tokens and its registers columns.
-    Sum<T> o[kTiles];
-    frag rf[2][kTerms], uf[2][kTerms], df[2][kTerms];
-#pragma unroll
-    for (int i = 0; i < kQueries; i += kTiles) {
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) fetch(kFirstQ + i + n + kAhead);
-#pragma unroll
-      for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) o[n].add(s[i / kTiles][term], qf[i + n], term > 0);
-      keep_order();
-    }
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const float factor = factors[3 * kTokens + n * 16 + lane.l];
-      o[n].whole *= factor;
-      o[n].rest *= factor;
-    }
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) split<T>(&r[kt * kPer], rf[kt]);
-    // U = T R.
-#pragma unroll
-    for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-      for (int i = 0; i < kBlocks; ++i) fetch(kFirstT + term * kBlocks + i + kAhead);
-#pragma unroll
-      for (int other = 0; other < kTerms - term; ++other)
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-          const Triangle<T> b(i);
-          sums[b.tile].add(tf[term * kBlocks + i], rf[b.step][other], term + other > 0);
-        }
-      keep_order();
-    }
-    f32x4 u[kTiles];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) u[m] = sums[m].value();
-    if constexpr (!TRANSIT) {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], uf[kt]);
-    }
-    // S = c S + K^T (e rk U).
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], df[kt]);
-#pragma unroll
-    for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
-      Sum<T> part[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) part[m].whole = state[m0 + m] * whole;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int m = 0; m < 4; ++m) fetch(kFirstC + m0 * 2 + kt * 4 + m + kAhead);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-          for (int m = 0; m < 4; ++m) part[m].add(cf[m0 * 2 + kt * 4 + m], df[kt][term], term > 0);
-        keep_order();
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
-    }
-    if constexpr (TRANSIT) continue;
-    // O = c rq Q S + P U.
-#pragma unroll
-    for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-      for (int other = 0; other < kTerms - term; ++other)
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-          const Triangle<T> b(i);
-          if (other == 0) fetch(kFirstP + term * kBlocks + i + kAhead);
-          o[b.tile].add(uf[b.step][other], pf[term * kBlocks + i], term + other > 0);
-        }
-      keep_order();
-    }
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) held_output[n] = nearest<T>(o[n].value());
-    if constexpr (KEEP) {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) held_update[kt] = uf[kt][0];
-    }
-    held = c;
+    if constexpr (!kTwice) load_pairs(c, lds_at + S::kPairsOnce);
+    load_stage(c + 1);
+  };
+  // U is there, and Q and T are done with.
+  const auto meet_at_update = [&](int c) __attribute__((always_inline)) {
+    if constexpr (TRANSIT) return;
+    if constexpr (!kTwice) wait_older_loads<kStageLoads>();
+    __syncthreads();
+    load_query(c + 1);
+    if constexpr (!kTwice) load_solve(c + 1, lds_at + S::kSolveOnce);
+  };
+  if (begin < end) {
+    load_stage(begin);
+    if constexpr (!TRANSIT) load_query(begin);
+    if constexpr (!kTwice) load_solve(begin, lds_at + S::kSolveOnce);
   }
-  if constexpr (!TRANSIT) store_held();
-  if (!active) return;
-  if (TRANSIT || a.segments == 1) {
+  constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
+  const unsigned state_at = lds_at + S::kState + part * S::kStateBytes + thread * 16;
+  const unsigned update_at = lds_at + S::kUpdate + part * S::kUpdateBytes + thread * 16;
+
+  if (TRANSIT || wave < W) {
+    const Reader<T> places;
+    const Own<T> own(from_panel / 16 + part);
+    f32x4 state[kStateTiles];
 #pragma unroll
     for (int m = 0; m < kStateTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = first_row<T>(m, lane.g) + e;
-        if constexpr (TRANSIT) {
-          if (w.unit)
-            a.transits[(segment_at * DK + d) * DK + mine] = state[m][e];
-          else
-            a.partials[(segment_at * DK + d) * a.value_pad + mine] = state[m][e];
-        } else if (d < key_size && mine < value_size) {
-          a.last[(bh * key_size + d) * value_size + mine] = state[m][e];
+        if constexpr (TRANSIT)
+          state[m][e] = w.unit && d == mine ? 1.f : 0.f;
+        else if (a.segments > 1)
+          state[m][e] = active ? a.starts[(segment_at * DK + d) * a.value_pad + mine] : 0.f;
+        else
+          state[m][e] = a.first != nullptr && d < key_size && mine < value_size
+                            ? a.first[(bh * key_size + d) * value_size + mine]
+                            : 0.f;
+      }
+    frag s[kSteps][kTerms];
+    const auto hand_state = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        split<T>(&state[ks * kPer], s[ks]);
+        if constexpr (!TRANSIT) {
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) lds_write(state_at + (ks * kTerms + term) * 1024, s[ks][term]);
         }
       }
+    };
+    hand_state();
+#pragma unroll 1
+    for (int c = begin; c < end; ++c) {
+      meet_at_start(c);
+      if (!active) {
+        meet_at_update(c);
+        continue;
+      }
+      const unsigned at = lds_at + S::kStages + (c & 1) * S::kStage;
+      const Reader<T> read = places.moved(at);
+      const Reader<T> solve_read = kTwice ? read : places.moved(lds_at);
+      constexpr unsigned kSolve = kTwice ? S::kSolve : S::kSolveOnce;
+      const float* factors = reinterpret_cast<const float*>(lds + S::kStages + (c & 1) * S::kStage + S::kFactors);
+      const float whole = factors[256];
+      // The chunk's fragments in the order of their products, read kAhead of them before: K, T, K^T.
+      // Neighbouring products are of different sums, since one waits for the last of its own sum.
+      frag kf[kRows], tf[kTerms * kBlocks], cf[kColumns];
+      const auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i < kRows) {
+          kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
+        } else if ((i -= kRows) < kTerms * kBlocks) {
+          const Triangle<T> b(i % kBlocks);
+          tf[i] = solve_read.operand(kSolve + i / kBlocks * C::kPanel, b.tile, b.step);
+        } else if ((i -= kTerms * kBlocks) < kColumns) {
+          cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
+        }
+      };
+      constexpr int kFirstT = kRows, kFirstC = kFirstT + kTerms * kBlocks;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch(i);
+      keep_order();
+
+      // R = beta V - (beta c rk) K S.
+      Sum<T> sums[kTiles];
+#pragma unroll
+      for (int i = 0; i < kRows; i += kTiles) {
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) fetch(i + m + kAhead);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) sums[m].add(kf[i + m], s[i / kTiles][term], term > 0);
+        keep_order();
+      }
+      f32x4 r[kTiles];
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) {
+        const f32x4 acc = sums[m].value();
+        const f32x4 v = own.values(at + S::kValues, m);
+        const int row = first_row<T>(m, lane.g);
+        const f32x4 take = *reinterpret_cast<const f32x4*>(factors + row);
+        const f32x4 beta = *reinterpret_cast<const f32x4*>(factors + kTokens + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[m][e] = fmaf(beta[e], v[e], -take[e] * acc[e]);
+        sums[m] = Sum<T>();
+      }
+      frag rf[2][kTerms], uf[2][kTerms], df[2][kTerms];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) split<T>(&r[kt * kPer], rf[kt]);
+      // U = T R.
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) fetch(kFirstT + term * kBlocks + i + kAhead);
+#pragma unroll
+        for (int other = 0; other < kTerms - term; ++other)
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i) {
+            const Triangle<T> b(i);
+            sums[b.tile].add(tf[term * kBlocks + i], rf[b.step][other], term + other > 0);
+          }
+        keep_order();
+      }
+      f32x4 u[kTiles];
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) u[m] = sums[m].value();
+      if constexpr (!TRANSIT) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          split<T>(&u[kt * kPer], uf[kt]);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) lds_write(update_at + (kt * kTerms + term) * 1024, uf[kt][term]);
+        }
+      }
+      meet_at_update(c);
+      // S = c S + K^T (e rk U).
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], df[kt]);
+#pragma unroll
+      for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
+        Sum<T> sum[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) sum[m].whole = state[m0 + m] * whole;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) fetch(kFirstC + m0 * 2 + kt * 4 + m + kAhead);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) sum[m].add(cf[m0 * 2 + kt * 4 + m], df[kt][term], term > 0);
+          keep_order();
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) state[m0 + m] = sum[m].value();
+      }
+      hand_state();
+    }
+    wait_loads();  // none into LDS that is another workgroup's by then
+    if (!active) return;
+    if (TRANSIT || a.segments == 1) {
+#pragma unroll
+      for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = first_row<T>(m, lane.g) + e;
+          if constexpr (TRANSIT) {
+            if (w.unit)
+              a.transits[(segment_at * DK + d) * DK + mine] = state[m][e];
+            else
+              a.partials[(segment_at * DK + d) * a.value_pad + mine] = state[m][e];
+          } else if (d < key_size && mine < value_size) {
+            a.last[(bh * key_size + d) * value_size + mine] = state[m][e];
+          }
+        }
+    }
+    return;
   }
-  if constexpr (TRANSIT) return;
-  // Tokens past the last chunk give zeros.
-  const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
-                           ? a.tokens
-                           : int64_t{begin + a.segment_chunks} * kTokens;
-  for (int64_t t = int64_t{end > begin ? end : begin} * kTokens + lane.l; t < stop; t += 16)
-    if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
+
+  if constexpr (!TRANSIT) {
+    const Reader<T> places;
+    const Reader<T> fixed = places.moved(lds_at);
+    T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
+    const int64_t out_token = a.heads * value_size;
+    const int store_at = column + lane.g * 4, store_count = value_size - store_at;
+    // A chunk's results are stored while the next one is worked on: the wait for loads is for stores too.
+    const bool whole_rows = column + 16 <= value_size;
+    unsigned out_place[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
+    const unsigned state_place = mine * DK + lane.g * (16 / sizeof(T));
+    const unsigned update_place = mine * kTokens + lane.g * (16 / sizeof(T));
+    Four<T> held_output[kTiles];
+    frag held_update[2];
+    int held = -1;
+    const auto store_held = [&]() __attribute__((always_inline)) {
+      if (held < 0) return;
+      T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
+      if (whole_rows && (held + 1) * kTokens <= a.tokens) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) *reinterpret_cast<Run<T, 4>*>(to + out_place[n]) = __builtin_bit_cast(Run<T, 4>, held_output[n]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+          if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < store_count) to[out_place[n] + e] = held_output[n][e];
+            end_of_part();
+          }
+      }
+      if constexpr (KEEP) {
+        T* keep = static_cast<T*>(a.updates) + (first_chunk + held) * a.value_pad * kTokens;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
+      }
+    };
+#pragma unroll 1
+    for (int c = begin; c < end; ++c) {
+      meet_at_start(c);
+      if (!active) {
+        meet_at_update(c);
+        continue;
+      }
+      frag s[kSteps][kTerms], qf[kRows];
+      const auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i < kRows) qf[i] = fixed.row(S::kQuery, i % kTiles, i / kTiles);
+      };
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) s[ks][term] = lds_read<frag>(state_at + (ks * kTerms + term) * 1024);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) fetch(i);
+      keep_order();
+      store_held();
+      if constexpr (KEEP) {
+        T* keep = static_cast<T*>(a.states) + (first_chunk + c) * a.value_pad * DK;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
+      }
+      // O = c rq Q S + P U: its lanes are tokens and its registers columns.
+      const float* factors = reinterpret_cast<const float*>(lds + S::kStages + (c & 1) * S::kStage + S::kFactors);
+      Sum<T> o[kTiles];
+#pragma unroll
+      for (int i = 0; i < kRows; i += kTiles) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) fetch(i + n + kTiles);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) o[n].add(s[i / kTiles][term], qf[i + n], term > 0);
+        keep_order();
+      }
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const float factor = factors[3 * kTokens + n * 16 + lane.l];
+        o[n].whole *= factor;
+        o[n].rest *= factor;
+      }
+      meet_at_update(c);
+      const Reader<T> read = kTwice ? places.moved(lds_at + S::kStages + (c & 1) * S::kStage) : fixed;
+      constexpr unsigned kPairs = kTwice ? S::kPairs : S::kPairsOnce;
+      frag uf[2][kTerms], pf[kTerms * kBlocks];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) uf[kt][term] = lds_read<frag>(update_at + (kt * kTerms + term) * 1024);
+#pragma unroll
+      for (int i = 0; i < kTerms * kBlocks; ++i) {
+        const Triangle<T> b(i % kBlocks);
+        pf[i] = read.row(kPairs + i / kBlocks * C::kPanel, b.tile, b.step);
+      }
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+        for (int other = 0; other < kTerms - term; ++other)
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i) {
+            const Triangle<T> b(i);
+            o[b.tile].add(uf[b.step][other], pf[term * kBlocks + i], term + other > 0);
+          }
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) held_output[n] = nearest<T>(o[n].value());
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) held_update[kt] = uf[kt][0];
+      }
+      held = c;
+    }
+    wait_loads();
+    store_held();
+    if (!active) return;
+    // Tokens past the last chunk give zeros.
+    const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
+                             ? a.tokens
+                             : int64_t{begin + a.segment_chunks} * kTokens;
+    for (int64_t t = int64_t{end > begin ? end : begin} * kTokens + lane.l; t < stop; t += 16)
+      if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
+  }
 }
 
 // ---- segments of the chunks --------------------------------------------------------------------------------
@@ -1479,12 +1610,6 @@ struct GradientsLds {
   unsigned char values[C::kPanel];  // of the block at work
   float slope[2][C::kTokens], kept[2][C::kTokens], step[2][C::kTokens], inner[2 * C::kTiles];
 };
-
-// Waits for loads with COUNT or more after them.
-template <int COUNT>
-__device__ __forceinline__ void wait_older_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory");
-}
 
 // What a wave does that makes the pairs with its tokens as rows (HALF 0) or columns (1), of the first (SIDE 0) or
 // the second fragment of the chunk's tokens: all of it is known to the compiler but the tokens.
@@ -2196,13 +2321,13 @@ bool narrow_walk(const DeltaArgs& a) { return a.segments == 1 && a.batch * a.hea
 // One walk; TRANSIT: of its segments, with the columns of the unit matrix.
 template <typename T, int DK, bool KEEP, bool TRANSIT, int W>
 hipError_t launch_walk(const DeltaArgs& a, hipStream_t stream) {
-  constexpr int kBytes = 2 * Stage<T, DK, W>::kBytes;
+  constexpr int kBytes = Walk<T, DK, W, !TRANSIT>::kBytes;
   const auto kernel = delta_forward<T, DK, W, KEEP, TRANSIT>;
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
   if (err != hipSuccess) return err;
   const int64_t tiles = value_tiles(a, W * 16) + (TRANSIT ? DK / (W * 16) : 0);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(64 * W), kBytes,
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(64 * W * (TRANSIT ? 1 : 2)), kBytes,
                      stream, a);
   return hipGetLastError();
 }

@@ -366,6 +366,7 @@ DeltaPlan plan_delta(const DeltaArgs& a, bool saving) {
   p.segments = 1;
   p.segment_chunks = static_cast<int>(a.chunks);
   if (p.step) return p;
+  p.threads = 512;
   if (walks > 0 && walks <= 64 && a.chunks >= 16) {
     const int64_t most = std::min<int64_t>(256 / walks, a.chunks / 8);
     p.segment_chunks = static_cast<int>((a.chunks + most - 1) / most);
