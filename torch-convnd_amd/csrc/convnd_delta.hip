@@ -809,7 +809,7 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
   using frag = typename C::frag;
   using S = Walk<T, DK, W, !TRANSIT>;
   constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kTerms = C::kTerms, kPer = C::kPer;
-  constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16, kWaves = TRANSIT ? W : 2 * W;
+  constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
   constexpr bool kTwice = S::kTwice;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
@@ -835,61 +835,47 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
   const T* v_at = at_token<T>(a.value, a.value_strides, b, 0, h);
   const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
-  const PanelLoads<T, DK / kTokens, kWaves> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
-  const PanelLoads<T, DK / kTokens, kWaves> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
-  const PanelLoads<T, S::kValuePanels, kWaves> value_loads(
+  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, part);
+  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, part);
+  const PanelLoads<T, S::kValuePanels, W> value_loads(
       static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.value_strides.token * sizeof(T)),
-      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
-  const PanelLoads<T, kTerms, kWaves> pair_loads(wave);
+      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), part);
+  const PanelLoads<T, kTerms, W> pair_loads(part);
   const auto rows_of = [&](int c) __attribute__((always_inline)) {
     const int64_t left = c < end ? length - static_cast<int64_t>(c) * kTokens : 0;
     return left < kTokens ? static_cast<int>(left) : kTokens;
   };
   const auto load_solve = [&](int c, unsigned dst) __attribute__((always_inline)) {
-    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes)), dst, wave, c < end ? kTokens : 0);
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes)), dst, part, c < end ? kTokens : 0);
   };
   const auto load_pairs = [&](int c, unsigned dst) __attribute__((always_inline)) {
-    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes) + S::kPairBytes), dst, wave,
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes) + S::kPairBytes), dst, part,
                     c < end ? kTokens : 0);
   };
   const auto load_query = [&](int c) __attribute__((always_inline)) {
-    query_loads.load(buffer_at(q_at + static_cast<int64_t>(c) * kTokens * a.query_strides.token), lds_at + S::kQuery, wave,
+    query_loads.load(buffer_at(q_at + static_cast<int64_t>(c) * kTokens * a.query_strides.token), lds_at + S::kQuery, part,
                      rows_of(c));
   };
   // As many loads whether there is a chunk or not, since waits count them (but the factors').
-  constexpr int kStageLoads = (DK / kTokens + S::kValuePanels) * (kTokens / 8) / kWaves;
+  constexpr int kStageLoads = (DK / kTokens + S::kValuePanels) * (kTokens / 8) / W;
   const auto load_stage = [&](int c) __attribute__((always_inline)) {
     const unsigned dst = lds_at + S::kStages + (c & 1) * S::kStage;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
     const int rows = rows_of(c);
-    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
-    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, wave, rows);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, part, rows);
+    value_loads.load(buffer_at(v_at + t0 * a.value_strides.token), dst + S::kValues, part, rows);
     if constexpr (kTwice) {
       load_solve(c, dst + S::kSolve);
       if constexpr (!TRANSIT) load_pairs(c, dst + S::kPairs);
     }
-    if (wave < 2) {  // the factors, and after them `whole`
-      const unsigned at = wave * 16 * kTokens + thread * 16;
+    if (part < 2) {  // the factors, and after them `whole`
+      const unsigned at = part * 16 * kTokens + thread * 16;
       load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
-                 dst + S::kFactors + wave * 1024, c < end && at < (wave == 0 ? 16 : 17) * kTokens ? at : kNowhere);
+                 dst + S::kFactors + part * 1024, c < end && at < (part == 0 ? 16 : 17) * kTokens ? at : kNowhere);
     }
   };
-  // What was loaded for this chunk is there, and the buffers of the one before are free.
-  const auto meet_at_start = [&](int c) __attribute__((always_inline)) {
-    wait_loads();
-    __syncthreads();
-    if constexpr (!kTwice) load_pairs(c, lds_at + S::kPairsOnce);
-    load_stage(c + 1);
-  };
-  // U is there, and Q and T are done with.
-  const auto meet_at_update = [&](int c) __attribute__((always_inline)) {
-    if constexpr (TRANSIT) return;
-    if constexpr (!kTwice) wait_older_loads<kStageLoads>();
-    __syncthreads();
-    load_query(c + 1);
-    if constexpr (!kTwice) load_solve(c + 1, lds_at + S::kSolveOnce);
-  };
-  if (begin < end) {
+  // The waves of outputs load (without them, the waves of states).
+  if ((TRANSIT || wave >= W) && begin < end) {
     load_stage(begin);
     if constexpr (!TRANSIT) load_query(begin);
     if constexpr (!kTwice) load_solve(begin, lds_at + S::kSolveOnce);
@@ -930,9 +916,11 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
     hand_state();
 #pragma unroll 1
     for (int c = begin; c < end; ++c) {
-      meet_at_start(c);
+      if constexpr (TRANSIT) wait_loads();
+      __syncthreads();  // the chunk is there, and the one before done with
+      if constexpr (TRANSIT) load_stage(c + 1);
       if (!active) {
-        meet_at_update(c);
+        if constexpr (!TRANSIT) __syncthreads();
         continue;
       }
       const unsigned at = lds_at + S::kStages + (c & 1) * S::kStage;
@@ -1011,7 +999,7 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
           for (int term = 0; term < kTerms; ++term) lds_write(update_at + (kt * kTerms + term) * 1024, uf[kt][term]);
         }
       }
-      meet_at_update(c);
+      if constexpr (!TRANSIT) __syncthreads();  // U is handed on
       // S = c S + K^T (e rk U).
 #pragma unroll
       for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
@@ -1037,7 +1025,7 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
       }
       hand_state();
     }
-    wait_loads();  // none into LDS that is another workgroup's by then
+    if constexpr (TRANSIT) wait_loads();  // none into LDS that is another workgroup's by then
     if (!active) return;
     if (TRANSIT || a.segments == 1) {
 #pragma unroll
@@ -1064,45 +1052,28 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
     T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
     const int64_t out_token = a.heads * value_size;
     const int store_at = column + lane.g * 4, store_count = value_size - store_at;
-    // A chunk's results are stored while the next one is worked on: the wait for loads is for stores too.
     const bool whole_rows = column + 16 <= value_size;
     unsigned out_place[kTiles];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
     const unsigned state_place = mine * DK + lane.g * (16 / sizeof(T));
     const unsigned update_place = mine * kTokens + lane.g * (16 / sizeof(T));
-    Four<T> held_output[kTiles];
-    frag held_update[2];
-    int held = -1;
-    const auto store_held = [&]() __attribute__((always_inline)) {
-      if (held < 0) return;
-      T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
-      if (whole_rows && (held + 1) * kTokens <= a.tokens) {
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) *reinterpret_cast<Run<T, 4>*>(to + out_place[n]) = __builtin_bit_cast(Run<T, 4>, held_output[n]);
-      } else {
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-          if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (e < store_count) to[out_place[n] + e] = held_output[n][e];
-            end_of_part();
-          }
-      }
-      if constexpr (KEEP) {
-        T* keep = static_cast<T*>(a.updates) + (first_chunk + held) * a.value_pad * kTokens;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
-      }
-    };
+    // The wait for what was loaded is not for the stores after it, of which there are at least so many.
+    constexpr int kKept = KEEP ? 2 + kSteps : 0;
+    bool all_stored = false;
 #pragma unroll 1
     for (int c = begin; c < end; ++c) {
-      meet_at_start(c);
-      if (!active) {
-        meet_at_update(c);
-        continue;
-      }
+      if (c == begin)
+        wait_loads();
+      else if (all_stored)
+        wait_older_loads<kTiles + kKept>();
+      else if (active)
+        wait_older_loads<kKept>();
+      else
+        wait_loads();
+      __syncthreads();
+      if constexpr (!kTwice) load_pairs(c, lds_at + S::kPairsOnce);
+      load_stage(c + 1);
       frag s[kSteps][kTerms], qf[kRows];
       const auto fetch = [&](int i) __attribute__((always_inline)) {
         if (i < kRows) qf[i] = fixed.row(S::kQuery, i % kTiles, i / kTiles);
@@ -1114,12 +1085,6 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) fetch(i);
       keep_order();
-      store_held();
-      if constexpr (KEEP) {
-        T* keep = static_cast<T*>(a.states) + (first_chunk + c) * a.value_pad * DK;
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
-      }
       // O = c rq Q S + P U: its lanes are tokens and its registers columns.
       const float* factors = reinterpret_cast<const float*>(lds + S::kStages + (c & 1) * S::kStage + S::kFactors);
       Sum<T> o[kTiles];
@@ -1139,7 +1104,12 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
         o[n].whole *= factor;
         o[n].rest *= factor;
       }
-      meet_at_update(c);
+      if constexpr (!kTwice) wait_older_loads<kStageLoads>();  // P
+      __syncthreads();
+      load_query(c + 1);
+      if constexpr (!kTwice) load_solve(c + 1, lds_at + S::kSolveOnce);
+      if (!active) continue;
+      asm volatile("" ::: "memory");  // the stores stay behind the loads
       const Reader<T> read = kTwice ? places.moved(lds_at + S::kStages + (c & 1) * S::kStage) : fixed;
       constexpr unsigned kPairs = kTwice ? S::kPairs : S::kPairsOnce;
       frag uf[2][kTerms], pf[kTerms * kBlocks];
@@ -1161,16 +1131,33 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
             const Triangle<T> b(i);
             o[b.tile].add(uf[b.step][other], pf[term * kBlocks + i], term + other > 0);
           }
+      T* to = out + static_cast<int64_t>(c) * kTokens * out_token;
+      all_stored = whole_rows && (c + 1) * kTokens <= a.tokens;
+      if (all_stored) {
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) held_output[n] = nearest<T>(o[n].value());
-      if constexpr (KEEP) {
+        for (int n = 0; n < kTiles; ++n) *reinterpret_cast<Run<T, 4>*>(to + out_place[n]) = __builtin_bit_cast(Run<T, 4>, nearest<T>(o[n].value()));
+      } else {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) held_update[kt] = uf[kt][0];
+        for (int n = 0; n < kTiles; ++n) {
+          const Four<T> v = nearest<T>(o[n].value());
+          if (static_cast<int64_t>(c) * kTokens + n * 16 + lane.l < a.tokens) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < store_count) to[out_place[n] + e] = v[e];
+            end_of_part();
+          }
+        }
       }
-      held = c;
+      if constexpr (KEEP) {
+        T* updates = static_cast<T*>(a.updates) + (first_chunk + c) * a.value_pad * kTokens;
+        T* states = static_cast<T*>(a.states) + (first_chunk + c) * a.value_pad * DK;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(updates + (update_place + kt * C::kStep)) = uf[kt][0];
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(states + (state_place + ks * C::kStep)) = s[ks][0];
+      }
     }
-    wait_loads();
-    store_held();
+    wait_loads();  // none into LDS that is another workgroup's by then
     if (!active) return;
     // Tokens past the last chunk give zeros.
     const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
