@@ -715,23 +715,6 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 4, 4) void delta_prepare(DeltaA
 
 // ---- the walk over the chunks ------------------------------------------------------------------------
 
-// LDS of a chunk: K, Q, T and P (each in its terms), V or dO, the factors. What is read by a constant beside a
-// lane's address lies within 64 KB of it.
-template <typename T, int DK, int W>
-struct Stage {
-  using C = Chunk<T>;
-  static constexpr int kKeys = 0;
-  static constexpr int kQuery = kKeys + DK / C::kTokens * C::kPanel;
-  static constexpr int kSolve = kQuery + DK / C::kTokens * C::kPanel;
-  static constexpr int kPairs = kSolve + C::kTerms * C::kPanel;
-  static constexpr int kValues = kPairs + C::kTerms * C::kPanel;
-  static constexpr int kValuePanels = (W * 16 + C::kTokens - 1) / C::kTokens;
-  static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
-  static constexpr int kBytes = kFactors + 2048;
-  static_assert(W * 16 % C::kTokens == 0 || C::kTokens % (W * 16) == 0, "whole panels of values, or parts of one");
-  static_assert(kValues <= 65536, "constants of reads");
-};
-
 // Where a workgroup of a walk is: `columns` values of a head (or columns of the unit matrix) and a segment of its
 // chunks. Workgroups of a head are a whole number of heads apart: where that is a multiple of eight they run on
 // one XCD and share its L2.
@@ -803,8 +786,7 @@ struct Walk {
 // for a backward. Waves meet twice a chunk; panels load a chunk or half of one ahead. A walk is bound by the chain
 // from S to the next S (about 2 us a chunk; with the outputs in the same wave 3.9).
 template <typename T, int DK, int W, bool KEEP, bool TRANSIT>
-__global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_waves_per_eu(
-    W == 4 && !TRANSIT ? 2 : 1, W == 4 && !TRANSIT ? 2 : 1))) void delta_forward(DeltaArgs a) {
+__global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, W / 2))) void delta_forward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
   using S = Walk<T, DK, W, !TRANSIT>;
@@ -874,8 +856,7 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
                  dst + S::kFactors + part * 1024, c < end && at < (part == 0 ? 16 : 17) * kTokens ? at : kNowhere);
     }
   };
-  // The waves of outputs load (without them, the waves of states).
-  if ((TRANSIT || wave >= W) && begin < end) {
+  if (wave >= W && begin < end) {  // the waves of outputs load
     load_stage(begin);
     if constexpr (!TRANSIT) load_query(begin);
     if constexpr (!kTwice) load_solve(begin, lds_at + S::kSolveOnce);
@@ -884,7 +865,7 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
   const unsigned state_at = lds_at + S::kState + part * S::kStateBytes + thread * 16;
   const unsigned update_at = lds_at + S::kUpdate + part * S::kUpdateBytes + thread * 16;
 
-  if (TRANSIT || wave < W) {
+  if (wave < W) {
     const Reader<T> places;
     const Own<T> own(from_panel / 16 + part);
     f32x4 state[kStateTiles];
@@ -916,9 +897,7 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
     hand_state();
 #pragma unroll 1
     for (int c = begin; c < end; ++c) {
-      if constexpr (TRANSIT) wait_loads();
       __syncthreads();  // the chunk is there, and the one before done with
-      if constexpr (TRANSIT) load_stage(c + 1);
       if (!active) {
         if constexpr (!TRANSIT) __syncthreads();
         continue;
@@ -1025,7 +1004,6 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
       }
       hand_state();
     }
-    if constexpr (TRANSIT) wait_loads();  // none into LDS that is another workgroup's by then
     if (!active) return;
     if (TRANSIT || a.segments == 1) {
 #pragma unroll
@@ -1046,7 +1024,15 @@ __global__ __launch_bounds__(64 * W * (TRANSIT ? 1 : 2)) __attribute__((amdgpu_w
     return;
   }
 
-  if constexpr (!TRANSIT) {
+  if constexpr (TRANSIT) {
+#pragma unroll 1
+    for (int c = begin; c < end; ++c) {
+      wait_loads();
+      __syncthreads();
+      load_stage(c + 1);
+    }
+    wait_loads();  // none into LDS that is another workgroup's by then
+  } else {
     const Reader<T> places;
     const Reader<T> fixed = places.moved(lds_at);
     T* out = static_cast<T*>(a.output) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
@@ -1259,24 +1245,55 @@ __global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
 //   dU = P^T dO + diag(e rk) K D,  dV = diag(beta) Y
 //   D' = c_C D + Q^T diag(c rq) dO - K^T diag(beta c rk) Y
 //
-// in the forward walk's form: a wave has 16 columns of D in registers. D and Y of every chunk are kept for
-// delta_gradients.
+// in the forward walk's form: of two waves with 16 columns one has D in registers, and walks from D to the next D,
+// and the other makes P^T dO and Q^T dO, which do not need it, loads and stores. D and Y of every chunk are kept
+// for delta_gradients.
+template <typename T, int DK, int W>
+struct WalkBack {
+  using C = Chunk<T>;
+  static constexpr bool kTwice = W == 2;  // T and P
+  static constexpr int kKeyBytes = DK / C::kTokens * C::kPanel, kPairBytes = C::kTerms * C::kPanel;
+  static constexpr int kValuePanels = (W * 16 + C::kTokens - 1) / C::kTokens;
+  // Once.
+  static constexpr int kQuery = 0;
+  static constexpr int kSolveOnce = kQuery + kKeyBytes;
+  static constexpr int kPairsOnce = kSolveOnce + (kTwice ? 0 : kPairBytes);
+  static constexpr int kStages = kPairsOnce + (kTwice ? 0 : kPairBytes);
+  // In a stage.
+  static constexpr int kKeys = 0;
+  static constexpr int kSolve = kKeys + kKeyBytes;
+  static constexpr int kPairs = kSolve + (kTwice ? kPairBytes : 0);
+  static constexpr int kValues = kPairs + (kTwice ? kPairBytes : 0);
+  static constexpr int kFactors = kValues + kValuePanels * C::kPanel;
+  static constexpr int kStage = kFactors + 2048;
+  // Handed on, for each pair of waves: what the chunk adds to D (then D itself), and P^T dO (then dV and Y).
+  static constexpr int kAdded = kStages + 2 * kStage, kAddedBytes = DK / 16 * 1024;
+  static constexpr int kToUpdate = kAdded + W * kAddedBytes;
+  static constexpr int kTurnBytes = C::kTokens * kTurnPitch * int(sizeof(T)), kToUpdateBytes = kTurnBytes + 2048;
+  static constexpr int kBytes = kToUpdate + W * kToUpdateBytes;
+  static_assert(C::kTiles * 1024 <= kToUpdateBytes && DK / C::kStep * 1024 <= kAddedBytes, "in one's place");
+  static_assert(kFactors <= 65536 && kStages <= 65536 && kBytes <= 163840, "constants of reads, and LDS");
+};
+
 template <typename T, int DK, int W, bool TRANSIT>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) void delta_backward(DeltaArgs a) {
+__global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, W / 2))) void delta_backward(DeltaArgs a) {
   using C = Chunk<T>;
   using frag = typename C::frag;
-  using S = Stage<T, DK, W>;
+  using S = WalkBack<T, DK, W>;
   constexpr int kTokens = C::kTokens, kTiles = C::kTiles, kTerms = C::kTerms, kPer = C::kPer;
   constexpr int kSteps = DK / C::kStep, kStateTiles = DK / 16;
+  constexpr bool kTwice = S::kTwice;
+  constexpr int kAheadBack = 6;  // of transposing reads, two instructions each
+  constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
   extern __shared__ __align__(1024) unsigned char lds[];
   const Lane lane;
-  const Reader<T> places;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int thread = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
   const WalkPlace w(a, W * 16, TRANSIT ? DK : 0);
   const int64_t bh = w.bh;
   const int b = w.b, h = w.h, kh = w.kh;
   const int value_size = static_cast<int>(a.value_size), key_size = static_cast<int>(a.key_size);
-  const int v0 = w.v0, column = v0 + wave * 16;  // of the workgroup and the wave
+  const int v0 = w.v0, column = v0 + part * 16;  // of the workgroup and the wave
   const bool active = TRANSIT && w.unit ? true : column < value_size;
   const int mine = column + lane.l;
   const int length = length_of(a, b);
@@ -1284,54 +1301,223 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   const int begin = w.segment * a.segment_chunks;
   const int end = all_chunks < begin + a.segment_chunks ? all_chunks : begin + a.segment_chunks;
   const int64_t first_chunk = bh * a.chunks, segment_at = bh * a.segments + w.segment;
-
-  f32x4 state[kStateTiles];
-#pragma unroll
-  for (int m = 0; m < kStateTiles; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = first_row<T>(m, lane.g) + e;
-      if constexpr (TRANSIT)
-        state[m][e] = w.unit && d == mine ? 1.f : 0.f;
-      else if (a.segments > 1)
-        state[m][e] = active ? a.starts[(segment_at * DK + d) * a.value_pad + mine] : 0.f;
-      else
-        state[m][e] = a.grad_last != nullptr && d < key_size && mine < value_size
-                          ? a.grad_last[(bh * key_size + d) * value_size + mine]
-                          : 0.f;
-    }
-
-  T* turn = reinterpret_cast<T*>(lds + 2 * S::kBytes) + wave * kTokens * kTurnPitch;
-
+  const unsigned lds_at = lds_address(lds);
   // Panels of values start at whole ones; the wave's columns lie within.
   const int from_panel = v0 % (S::kValuePanels * kTokens);
-  const Own<T> own(from_panel / 16 + wave);
-  const unsigned lds_at = lds_address(lds);
+  const unsigned added_at = lds_at + S::kAdded + part * S::kAddedBytes + thread * 16;
+  const unsigned to_update = lds_at + S::kToUpdate + part * S::kToUpdateBytes;
+  const unsigned update_at = to_update + S::kTurnBytes + thread * 16;
+
+  if (wave < W) {
+    const Reader<T> places;
+    f32x4 state[kStateTiles];
+#pragma unroll
+    for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = first_row<T>(m, lane.g) + e;
+        if constexpr (TRANSIT)
+          state[m][e] = w.unit && d == mine ? 1.f : 0.f;
+        else if (a.segments > 1)
+          state[m][e] = active ? a.starts[(segment_at * DK + d) * a.value_pad + mine] : 0.f;
+        else
+          state[m][e] = a.grad_last != nullptr && d < key_size && mine < value_size
+                            ? a.grad_last[(bh * key_size + d) * value_size + mine]
+                            : 0.f;
+      }
+    frag s[kSteps][kTerms];
+    const auto hand_state = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        split<T>(&state[ks * kPer], s[ks]);
+        if constexpr (!TRANSIT) lds_write(added_at + ks * 1024, s[ks][0]);
+      }
+    };
+    hand_state();
+#pragma unroll 1
+    for (int c = end - 1; c >= begin; --c) {
+      __syncthreads();  // the chunk is there, and the one before done with
+      if (!active) {
+        __syncthreads();
+        continue;
+      }
+      const unsigned at = lds_at + S::kStages + (c & 1) * S::kStage;
+      const Reader<T> read = places.moved(at);
+      const Reader<T> solve_read = kTwice ? read : places.moved(lds_at);
+      constexpr unsigned kSolve = kTwice ? S::kSolve : S::kSolveOnce;
+      const float* factors = reinterpret_cast<const float*>(lds + S::kStages + (c & 1) * S::kStage + S::kFactors);
+      const float whole = factors[256];
+      // dU = diag(e rk) K D + P^T dO, whose second part is handed.
+      frag kf[kRows];
+      const auto fetch_key = [&](int i) __attribute__((always_inline)) {
+        if (i < kRows) kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch_key(i);
+      keep_order();
+      Sum<T> sums[kTiles];
+#pragma unroll
+      for (int i = 0; i < kRows; i += kTiles) {
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) fetch_key(i + m + kAhead);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int m = 0; m < kTiles; ++m) sums[m].add(kf[i + m], s[i / kTiles][term], term > 0);
+        keep_order();
+      }
+      f32x4 y[kTiles];
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) {
+        y[m] = sums[m].value() * *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
+        sums[m] = Sum<T>();
+      }
+      __syncthreads();  // what the other wave made, and T
+      // Fragments in the order of their products: T^T, K^T.
+      frag tf[kTerms * kBlocks], cf[kColumns], yf[2][kTerms], uf[2][kTerms];
+      const auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i < kTerms * kBlocks) {
+          const Triangle<T> b(i % kBlocks);
+          tf[i] = solve_read.column(kSolve + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
+        } else if ((i -= kTerms * kBlocks) < kColumns) {
+          cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
+        }
+      };
+      constexpr int kFirstC = kTerms * kBlocks;
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) y[m] += lds_read<f32x4>(to_update + m * 1024 + thread * 16);
+#pragma unroll
+      for (int i = 0; i < kAheadBack; ++i) fetch(i);
+      keep_order();
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], uf[kt]);
+      // Y = T^T dU.
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+        for (int other = 0; other < kTerms - term; ++other)
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i) {
+            const Triangle<T> b(i);
+            if (other == 0) fetch(term * kBlocks + i + kAheadBack);
+            sums[kTiles - 1 - b.tile].add(tf[term * kBlocks + i], uf[1 - b.step][other], term + other > 0);
+          }
+        keep_order();
+      }
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) y[m] = sums[m].value();
+      // dV and Y for the other wave to store: dV as [token][column].
+      if constexpr (!TRANSIT) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          frag hi[1];
+          split<T>(&y[kt * kPer], hi);
+          lds_write(update_at + kt * 1024, hi[0]);
+        }
+#pragma unroll
+        for (int m = 0; m < kTiles; ++m) {
+          const int row = first_row<T>(m, lane.g);
+          const f32x4 dv = y[m] * *reinterpret_cast<const f32x4*>(factors + kTokens + row);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            lds_write(to_update + static_cast<unsigned>(((row + e) * kTurnPitch + lane.l) * sizeof(T)), static_cast<T>(dv[e]));
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) y[m] *= -*reinterpret_cast<const f32x4*>(factors + first_row<T>(m, lane.g));
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], yf[kt]);
+      // D = c D + Q^T (c rq dO), which is handed, - K^T (beta c rk Y).
+#pragma unroll
+      for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
+        Sum<T> sum[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) sum[m].whole = state[m0 + m] * whole + lds_read<f32x4>(added_at + (m0 + m) * 1024);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) fetch(kFirstC + m0 * 2 + kt * 4 + m + kAheadBack);
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) sum[m].add(cf[m0 * 2 + kt * 4 + m], yf[kt][term], term > 0);
+          keep_order();
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) state[m0 + m] = sum[m].value();
+      }
+      hand_state();
+    }
+    __syncthreads();  // the last dV and Y are handed on
+    if (!active) return;
+    if (TRANSIT || (a.segments == 1 && a.grad_first != nullptr)) {
+#pragma unroll
+      for (int m = 0; m < kStateTiles; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = first_row<T>(m, lane.g) + e;
+          if constexpr (TRANSIT) {
+            if (w.unit)
+              a.transits[(segment_at * DK + d) * DK + mine] = state[m][e];
+            else
+              a.partials[(segment_at * DK + d) * a.value_pad + mine] = state[m][e];
+          } else if (d < key_size && mine < value_size) {
+            a.grad_first[(bh * key_size + d) * value_size + mine] = state[m][e];
+          }
+        }
+    }
+    return;
+  }
+
+  // The other waves: loads, what does not need D, and stores.
   const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
   const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
   const T* g_at = at_token<T>(a.grad_output, a.grad_strides, b, 0, h);
   const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
-  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, wave);
-  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, wave);
+  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, part);
+  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, part);
   const PanelLoads<T, S::kValuePanels, W> value_loads(
       static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
-      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), wave);
-  const PanelLoads<T, 2 * kTerms, W> pair_loads(wave);
-  auto load = [&](int c) __attribute__((always_inline)) {
-    const unsigned dst = lds_at + (c & 1) * S::kBytes;
+      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), part);
+  const PanelLoads<T, kTerms, W> pair_loads(part);
+  // As many loads whether there is a chunk or not, since waits count them (but the factors').
+  const auto rows_of = [&](int c) __attribute__((always_inline)) {
+    const int64_t left = c >= begin ? length - static_cast<int64_t>(c) * kTokens : 0;
+    return left < kTokens ? static_cast<int>(left) : kTokens;
+  };
+  const auto load_pair = [&](int c, int which, unsigned dst) __attribute__((always_inline)) {
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes) + which * S::kPairBytes), dst, part,
+                    c >= begin ? kTokens : 0);
+  };
+  constexpr int kStageLoads = (DK / kTokens + S::kValuePanels) * (kTokens / 8) / W;
+  const auto load_stage = [&](int c) __attribute__((always_inline)) {
+    const unsigned dst = lds_at + S::kStages + (c & 1) * S::kStage;
     const int64_t t0 = static_cast<int64_t>(c) * kTokens;
-    const int rows = length - t0 < kTokens ? static_cast<int>(length - t0) : kTokens;
-    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, wave, rows);
-    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, wave, rows);
-    query_loads.load(buffer_at(q_at + t0 * a.query_strides.token), dst + S::kQuery, wave, rows);
-    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * kTerms * C::kPanel)), dst + S::kSolve, wave, kTokens);
-    if (wave < 2) {  // the factors, and after them `whole`
-      const unsigned at = wave * 16 * kTokens + (threadIdx.x & 63) * 16;
+    const int rows = rows_of(c);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, part, rows);
+    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, part, rows);
+    if constexpr (kTwice) {
+      load_pair(c, 0, dst + S::kSolve);
+      load_pair(c, 1, dst + S::kPairs);
+    }
+    if (part < 2) {  // the factors, and after them `whole`
+      const unsigned at = part * 16 * kTokens + thread * 16;
       load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
-                 dst + S::kFactors + wave * 1024, at < (wave == 0 ? 16 : 17) * kTokens ? at : kNowhere);
+                 dst + S::kFactors + part * 1024, c >= begin && at < (part == 0 ? 16 : 17) * kTokens ? at : kNowhere);
     }
   };
-
+  const auto load_once = [&](int c) __attribute__((always_inline)) {
+    query_loads.load(buffer_at(q_at + static_cast<int64_t>(c) * kTokens * a.query_strides.token), lds_at + S::kQuery, part,
+                     rows_of(c));
+    if constexpr (!kTwice) load_pair(c, 1, lds_at + S::kPairsOnce);
+  };
+  if (begin < end) {
+    load_stage(end - 1);
+    load_once(end - 1);
+  }
+  const Reader<T> places;
+  const Own<T> own(from_panel / 16 + part);
+  const Reader<T> fixed = places.moved(lds_at);
   T* out = static_cast<T*>(a.grad_value) + (static_cast<int64_t>(b) * a.tokens * a.heads + h) * value_size;
   const int64_t out_token = a.heads * value_size;
   const int store_at = column + lane.g * 4, store_count = value_size - store_at;
@@ -1341,104 +1527,97 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
   unsigned out_place[kTiles];
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) out_place[n] = (n * 16 + lane.l) * static_cast<unsigned>(out_token) + store_at;
-  // As in the forward a chunk's results are stored while the next one is worked on.
   Four<T> held_value[kTiles];
   frag held_update[2];
-  int held = -1;
-  const auto store_held = [&]() __attribute__((always_inline)) {
-    if (held < 0) return;
-    T* to = out + static_cast<int64_t>(held) * kTokens * out_token;
+  const auto take_held = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      if (whole_rows && (held + 1) * kTokens <= a.tokens) {
-        store_run<4>(to + out_place[n], __builtin_bit_cast(Run<T, 4>, held_value[n]));
-      } else if (static_cast<int64_t>(held) * kTokens + n * 16 + lane.l < a.tokens) {
+    for (int n = 0; n < kTiles; ++n)
+      held_value[n] = lds_read<Four<T>>(to_update + static_cast<unsigned>(((n * 16 + lane.l) * kTurnPitch + lane.g * 4) * sizeof(T)));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < store_count) to[out_place[n] + e] = held_value[n][e];
-        end_of_part();
-      }
+    for (int kt = 0; kt < 2; ++kt) held_update[kt] = lds_read<frag>(update_at + kt * 1024);
+  };
+  // Of chunk c; true if every store was made.
+  const auto store_held = [&](int c) __attribute__((always_inline)) {
+    T* to = out + static_cast<int64_t>(c) * kTokens * out_token;
+    const bool all = whole_rows && (c + 1) * kTokens <= a.tokens;
+    if (all) {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) *reinterpret_cast<Run<T, 4>*>(to + out_place[n]) = __builtin_bit_cast(Run<T, 4>, held_value[n]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+        if (static_cast<int64_t>(c) * kTokens + n * 16 + lane.l < a.tokens) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < store_count) to[out_place[n] + e] = held_value[n][e];
+          end_of_part();
+        }
     }
-    T* keep = static_cast<T*>(a.grad_updates) + (first_chunk + held) * a.value_pad * kTokens;
+    T* keep = static_cast<T*>(a.grad_updates) + (first_chunk + c) * a.value_pad * kTokens;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) *reinterpret_cast<frag*>(keep + (update_place + kt * C::kStep)) = held_update[kt];
+    return all;
   };
-  if (begin < end) load(end - 1);
+  bool all_stored = false;
 #pragma unroll 1
   for (int c = end - 1; c >= begin; --c) {
-    wait_loads();
+    // The wait for what was loaded is not for the stores after it, of which there are at least so many.
+    if (TRANSIT || c == end - 1 || !active)
+      wait_loads();
+    else if (all_stored)
+      wait_older_loads<kTiles + 2 + kSteps>();
+    else
+      wait_older_loads<kSteps>();
     __syncthreads();
-    if (c > begin) load(c - 1);
-    if (!active) continue;
-    if constexpr (!TRANSIT) store_held();
-    const unsigned at = lds_at + (c & 1) * S::kBytes;
-    const Reader<T> read = places.moved(at);
-    const float* factors = reinterpret_cast<const float*>(lds + (c & 1) * S::kBytes + S::kFactors);
-    const float whole = factors[256];
-
-    frag s[kSteps][kTerms];
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) split<T>(&state[ks * kPer], s[ks]);
+    if constexpr (!kTwice) load_pair(c, 0, lds_at + S::kSolveOnce);
+    load_stage(c - 1);
+    const unsigned at = lds_at + S::kStages + (c & 1) * S::kStage;
+    const Reader<T> pair_read = kTwice ? places.moved(at) : fixed;
+    constexpr unsigned kPairs = kTwice ? S::kPairs : S::kPairsOnce;
+    const float* factors = reinterpret_cast<const float*>(lds + S::kStages + (c & 1) * S::kStage + S::kFactors);
+    frag d[kSteps];
     if constexpr (!TRANSIT) {
-      T* keep = static_cast<T*>(a.grad_states) + (first_chunk + c) * a.value_pad * DK;
+      take_held();
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(keep + (state_place + ks * C::kStep)) = s[ks][0];
+      for (int ks = 0; ks < kSteps; ++ks) d[ks] = lds_read<frag>(added_at + ks * 1024);
     }
-    // Fragments in the order of their products: K, Q^T, P^T, T^T, K^T.
-    constexpr int kRows = kTiles * kSteps, kBlocks = Triangle<T>::kBlocks, kColumns = 2 * kStateTiles;
-    frag kf[kRows], qf[kColumns], pf[kTerms * kBlocks], tf[kTerms * kBlocks], cf[kColumns];
-    const auto fetch = [&](int i) __attribute__((always_inline)) {
-      if (i < kRows) {
-        kf[i] = read.operand(S::kKeys, i % kTiles, i / kTiles);
-      } else if ((i -= kRows) < kColumns) {
-        qf[i] = read.column(S::kQuery, i / 8 * 4 + i % 4, i / 4 % 2);
-      } else if ((i -= kColumns) < kTerms * kBlocks) {
-        const Triangle<T> b(i % kBlocks);
-        pf[i] = read.column(S::kPairs + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
-      } else if ((i -= kTerms * kBlocks) < kTerms * kBlocks) {
-        const Triangle<T> b(i % kBlocks);
-        tf[i] = read.column(S::kSolve + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
-      } else if ((i -= kTerms * kBlocks) < kColumns) {
-        cf[i] = read.column(S::kKeys, i / 8 * 4 + i % 4, i / 4 % 2);
-      }
-    };
-    constexpr int kAheadBack = 6;  // of transposing reads, two instructions each
-    constexpr int kFirstQ = kRows, kFirstP = kFirstQ + kColumns, kFirstT = kFirstP + kTerms * kBlocks,
-                  kFirstC = kFirstT + kTerms * kBlocks;
-    frag g[2];
+    frag g[2], pf[kTerms * kBlocks], qf[kColumns];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) g[kt] = own.column(at + S::kValues, kt);
+    const auto fetch = [&](int i) __attribute__((always_inline)) {
+      if (i < kTerms * kBlocks) {
+        const Triangle<T> b(i % kBlocks);
+        pf[i] = pair_read.column(kPairs + i / kBlocks * C::kPanel, kTiles - 1 - b.tile, 1 - b.step);
+      } else if ((i -= kTerms * kBlocks) < kColumns) {
+        qf[i] = fixed.column(S::kQuery, i / 8 * 4 + i % 4, i / 4 % 2);
+      }
+    };
+    constexpr int kFirstQ = kTerms * kBlocks;
 #pragma unroll
     for (int i = 0; i < kAheadBack; ++i) fetch(i);
     keep_order();
-
-    // dU = diag(e rk) K D + P^T dO.
+    // P^T dO.
     Sum<T> sums[kTiles];
 #pragma unroll
-    for (int i = 0; i < kRows; i += kTiles) {
+    for (int term = 0; term < kTerms; ++term) {
 #pragma unroll
-      for (int m = 0; m < kTiles; ++m) fetch(i + m + kAheadBack);
-#pragma unroll
-      for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) sums[m].add(kf[i + m], s[i / kTiles][term], term > 0);
+      for (int i = 0; i < kBlocks; ++i) {
+        const Triangle<T> b(i);
+        fetch(term * kBlocks + i + kAheadBack);
+        sums[kTiles - 1 - b.tile].add(pf[term * kBlocks + i], g[1 - b.step], term > 0);
+      }
       keep_order();
     }
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      const f32x4 factor = *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
-      sums[m].whole *= factor;
-      sums[m].rest *= factor;
-    }
-    // D = c D + Q^T (c rq dO), until Y is there.
-    frag gf[2][kTerms], yf[2][kTerms], uf[2][kTerms];
+    for (int m = 0; m < kTiles; ++m) lds_write(to_update + m * 1024 + thread * 16, sums[m].value());
+    // Q^T (c rq dO).
+    frag gf[2][kTerms];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       f32x4 v[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const f32x4 factor =
-            *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + first_row<T>(kt * kPer + i, lane.g));
+        const f32x4 factor = *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + first_row<T>(kt * kPer + i, lane.g));
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[i][e] = factor[e] * static_cast<float>(g[kt][i * 4 + e]);
       }
@@ -1446,9 +1625,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
     }
 #pragma unroll
     for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
-      Sum<T> part[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) part[m].whole = state[m0 + m] * whole;
+      Sum<T> sum[4];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
@@ -1456,117 +1633,38 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1))) 
 #pragma unroll
         for (int term = 0; term < kTerms; ++term)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) part[m].add(qf[m0 * 2 + kt * 4 + m], gf[kt][term], term > 0);
+          for (int m = 0; m < 4; ++m) sum[m].add(qf[m0 * 2 + kt * 4 + m], gf[kt][term], term > 0);
         keep_order();
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
+      for (int m = 0; m < 4; ++m) lds_write(added_at + (m0 + m) * 1024, sum[m].value());
     }
+    if constexpr (!kTwice) wait_older_loads<kStageLoads>();  // T
+    __syncthreads();
+    load_once(c - 1);
+    asm volatile("" ::: "memory");  // the stores stay behind the loads
+    if constexpr (!TRANSIT) {
+      if (!active) continue;
+      if (c < end - 1) all_stored = store_held(c + 1);
+      T* states = static_cast<T*>(a.grad_states) + (first_chunk + c) * a.value_pad * DK;
 #pragma unroll
-    for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
-        const Triangle<T> b(i);
-        fetch(kFirstP + term * kBlocks + i + kAheadBack);
-        sums[kTiles - 1 - b.tile].add(pf[term * kBlocks + i], g[1 - b.step], term > 0);
-      }
-      keep_order();
+      for (int ks = 0; ks < kSteps; ++ks) *reinterpret_cast<frag*>(states + (state_place + ks * C::kStep)) = d[ks];
     }
-    f32x4 y[kTiles];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      y[m] = sums[m].value();
-      sums[m] = Sum<T>();
-    }
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], uf[kt]);
-    // Y = T^T dU.
-#pragma unroll
-    for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-      for (int other = 0; other < kTerms - term; ++other)
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-          const Triangle<T> b(i);
-          if (other == 0) fetch(kFirstT + term * kBlocks + i + kAheadBack);
-          sums[kTiles - 1 - b.tile].add(tf[term * kBlocks + i], uf[1 - b.step][other], term + other > 0);
-        }
-      keep_order();
-    }
-    f32x4 dv[kTiles];
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) y[m] = sums[m].value();
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      frag hi[1];
-      split<T>(&y[kt * kPer], hi);
-      held_update[kt] = hi[0];
-    }
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      const int row = first_row<T>(m, lane.g);
-      dv[m] = y[m] * *reinterpret_cast<const f32x4*>(factors + kTokens + row);
-      y[m] *= -*reinterpret_cast<const f32x4*>(factors + row);
-    }
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], yf[kt]);
-    // D = D - K^T (beta c rk Y).
-#pragma unroll
-    for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
-      Sum<T> part[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) part[m].whole = state[m0 + m];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int m = 0; m < 4; ++m) fetch(kFirstC + m0 * 2 + kt * 4 + m + kAheadBack);
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-          for (int m = 0; m < 4; ++m) part[m].add(cf[m0 * 2 + kt * 4 + m], yf[kt][term], term > 0);
-        keep_order();
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) state[m0 + m] = part[m].value();
-    }
-    if constexpr (TRANSIT) continue;
-    // dV, through this wave's part of LDS: lanes tokens, four columns each.
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        turn[(first_row<T>(m, lane.g) + e) * kTurnPitch + lane.l] = static_cast<T>(dv[m][e]);
-    wait_own_lds();
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-      held_value[n] = *reinterpret_cast<const Four<T>*>(turn + (n * 16 + lane.l) * kTurnPitch + lane.g * 4);
-    wait_own_lds();
-    held = c;
   }
-  if constexpr (!TRANSIT) store_held();
-  if (!active) return;
-  if (TRANSIT || (a.segments == 1 && a.grad_first != nullptr)) {
-#pragma unroll
-    for (int m = 0; m < kStateTiles; ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = first_row<T>(m, lane.g) + e;
-        if constexpr (TRANSIT) {
-          if (w.unit)
-            a.transits[(segment_at * DK + d) * DK + mine] = state[m][e];
-          else
-            a.partials[(segment_at * DK + d) * a.value_pad + mine] = state[m][e];
-        } else if (d < key_size && mine < value_size) {
-          a.grad_first[(bh * key_size + d) * value_size + mine] = state[m][e];
-        }
-      }
+  wait_loads();  // none into LDS that is another workgroup's by then
+  __syncthreads();
+  if constexpr (!TRANSIT) {
+    if (!active) return;
+    if (begin < end) {
+      take_held();
+      store_held(begin);
+    }
+    const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
+                             ? a.tokens
+                             : int64_t{begin + a.segment_chunks} * kTokens;
+    for (int64_t t = int64_t{end > begin ? end : begin} * kTokens + lane.l; t < stop; t += 16)
+      if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
   }
-  if constexpr (TRANSIT) return;
-  const int64_t stop = a.tokens < int64_t{begin + a.segment_chunks} * kTokens
-                           ? a.tokens
-                           : int64_t{begin + a.segment_chunks} * kTokens;
-  for (int64_t t = int64_t{end > begin ? end : begin} * kTokens + lane.l; t < stop; t += 16)
-    if (store_count > 0) store_four(out + t * out_token + store_at, f32x4{0.f, 0.f, 0.f, 0.f}, store_count);
 }
 
 // ---- gradients within every chunk --------------------------------------------------------------------------
@@ -2314,20 +2412,20 @@ hipError_t launch_walk(const DeltaArgs& a, hipStream_t stream) {
   const hipError_t err = ask_lds(kernel, kBytes, asked);
   if (err != hipSuccess) return err;
   const int64_t tiles = value_tiles(a, W * 16) + (TRANSIT ? DK / (W * 16) : 0);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(64 * W * (TRANSIT ? 1 : 2)), kBytes,
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(128 * W), kBytes,
                      stream, a);
   return hipGetLastError();
 }
 
 template <typename T, int DK, bool TRANSIT, int W>
 hipError_t launch_walk_back(const DeltaArgs& a, hipStream_t stream) {
-  constexpr int kBytes = 2 * Stage<T, DK, W>::kBytes + W * Chunk<T>::kTokens * kTurnPitch * int(sizeof(T));
+  constexpr int kBytes = WalkBack<T, DK, W>::kBytes;
   const auto kernel = delta_backward<T, DK, W, TRANSIT>;
   static std::atomic<uint64_t> asked{0};
   const hipError_t err = ask_lds(kernel, kBytes, asked);
   if (err != hipSuccess) return err;
   const int64_t tiles = value_tiles(a, W * 16) + (TRANSIT ? DK / (W * 16) : 0);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(64 * W), kBytes,
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.batch * a.heads * tiles * a.segments)), dim3(128 * W), kBytes,
                      stream, a);
   return hipGetLastError();
 }
