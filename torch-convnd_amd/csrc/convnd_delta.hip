@@ -1308,7 +1308,45 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
   const unsigned to_update = lds_at + S::kToUpdate + part * S::kToUpdateBytes;
   const unsigned update_at = to_update + S::kTurnBytes + thread * 16;
 
+  const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
+  const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
+  const T* g_at = at_token<T>(a.grad_output, a.grad_strides, b, 0, h);
+  const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
+  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, part);
+  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, part);
+  const PanelLoads<T, S::kValuePanels, W> value_loads(
+      static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
+      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), part);
+  const PanelLoads<T, kTerms, W> pair_loads(part);
+  // As many loads whether there is a chunk or not, since waits count them (but the factors').
+  const auto rows_of = [&](int c) __attribute__((always_inline)) {
+    const int64_t left = c >= begin ? length - static_cast<int64_t>(c) * kTokens : 0;
+    return left < kTokens ? static_cast<int>(left) : kTokens;
+  };
+  const auto load_pair = [&](int c, int which, unsigned dst) __attribute__((always_inline)) {
+    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes) + which * S::kPairBytes), dst, part,
+                    c >= begin ? kTokens : 0);
+  };
+  constexpr int kStageLoads = (DK / kTokens + S::kValuePanels) * (kTokens / 8) / W;
+  const auto load_stage = [&](int c) __attribute__((always_inline)) {
+    const unsigned dst = lds_at + S::kStages + (c & 1) * S::kStage;
+    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
+    const int rows = rows_of(c);
+    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, part, rows);
+    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, part, rows);
+    if constexpr (kTwice) {
+      load_pair(c, 0, dst + S::kSolve);
+      load_pair(c, 1, dst + S::kPairs);
+    }
+    if (part < 2) {  // the factors, and after them `whole`
+      const unsigned at = part * 16 * kTokens + thread * 16;
+      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
+                 dst + S::kFactors + part * 1024, c >= begin && at < (part == 0 ? 16 : 17) * kTokens ? at : kNowhere);
+    }
+  };
+
   if (wave < W) {
+    if (begin < end) load_stage(end - 1);
     const Reader<T> places;
     f32x4 state[kStateTiles];
 #pragma unroll
@@ -1336,8 +1374,12 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
     hand_state();
 #pragma unroll 1
     for (int c = end - 1; c >= begin; --c) {
+      wait_loads();
       __syncthreads();  // the chunk is there, and the one before done with
+      if constexpr (!kTwice) load_pair(c, 0, lds_at + S::kSolveOnce);
+      load_stage(c - 1);
       if (!active) {
+        if constexpr (!kTwice) wait_older_loads<kStageLoads>();
         __syncthreads();
         continue;
       }
@@ -1372,7 +1414,8 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
         y[m] = sums[m].value() * *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
         sums[m] = Sum<T>();
       }
-      __syncthreads();  // what the other wave made, and T
+      if constexpr (!kTwice) wait_older_loads<kStageLoads>();  // T
+      __syncthreads();  // what the other wave made
       // Fragments in the order of their products: T^T, K^T.
       frag tf[kTerms * kBlocks], cf[kColumns], yf[2][kTerms], uf[2][kTerms];
       const auto fetch = [&](int i) __attribute__((always_inline)) {
@@ -1448,6 +1491,7 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
       }
       hand_state();
     }
+    wait_loads();  // none into LDS that is another workgroup's by then
     __syncthreads();  // the last dV and Y are handed on
     if (!active) return;
     if (TRANSIT || (a.segments == 1 && a.grad_first != nullptr)) {
@@ -1469,52 +1513,13 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
     return;
   }
 
-  // The other waves: loads, what does not need D, and stores.
-  const T* k_at = at_token<T>(a.key, a.key_strides, b, 0, kh);
-  const T* q_at = at_token<T>(a.query, a.query_strides, b, 0, kh);
-  const T* g_at = at_token<T>(a.grad_output, a.grad_strides, b, 0, h);
-  const unsigned key_bytes = static_cast<unsigned>(key_size * sizeof(T));
-  const PanelLoads<T, DK / kTokens, W> key_loads(0, static_cast<unsigned>(a.key_strides.token * sizeof(T)), key_bytes, part);
-  const PanelLoads<T, DK / kTokens, W> query_loads(0, static_cast<unsigned>(a.query_strides.token * sizeof(T)), key_bytes, part);
-  const PanelLoads<T, S::kValuePanels, W> value_loads(
-      static_cast<unsigned>((v0 - from_panel) * sizeof(T)), static_cast<unsigned>(a.grad_strides.token * sizeof(T)),
-      TRANSIT && w.unit ? 0u : static_cast<unsigned>(value_size * sizeof(T)), part);
-  const PanelLoads<T, kTerms, W> pair_loads(part);
-  // As many loads whether there is a chunk or not, since waits count them (but the factors').
-  const auto rows_of = [&](int c) __attribute__((always_inline)) {
-    const int64_t left = c >= begin ? length - static_cast<int64_t>(c) * kTokens : 0;
-    return left < kTokens ? static_cast<int>(left) : kTokens;
-  };
-  const auto load_pair = [&](int c, int which, unsigned dst) __attribute__((always_inline)) {
-    pair_loads.load(buffer_at(a.panels + (first_chunk + c) * (2 * S::kPairBytes) + which * S::kPairBytes), dst, part,
-                    c >= begin ? kTokens : 0);
-  };
-  constexpr int kStageLoads = (DK / kTokens + S::kValuePanels) * (kTokens / 8) / W;
-  const auto load_stage = [&](int c) __attribute__((always_inline)) {
-    const unsigned dst = lds_at + S::kStages + (c & 1) * S::kStage;
-    const int64_t t0 = static_cast<int64_t>(c) * kTokens;
-    const int rows = rows_of(c);
-    key_loads.load(buffer_at(k_at + t0 * a.key_strides.token), dst + S::kKeys, part, rows);
-    value_loads.load(buffer_at(g_at + t0 * a.grad_strides.token), dst + S::kValues, part, rows);
-    if constexpr (kTwice) {
-      load_pair(c, 0, dst + S::kSolve);
-      load_pair(c, 1, dst + S::kPairs);
-    }
-    if (part < 2) {  // the factors, and after them `whole`
-      const unsigned at = part * 16 * kTokens + thread * 16;
-      load_lds16(buffer_at(reinterpret_cast<const Record<T>*>(a.records) + first_chunk + c),
-                 dst + S::kFactors + part * 1024, c >= begin && at < (part == 0 ? 16 : 17) * kTokens ? at : kNowhere);
-    }
-  };
+  // The other waves: what does not need D, with its loads, and the stores.
   const auto load_once = [&](int c) __attribute__((always_inline)) {
     query_loads.load(buffer_at(q_at + static_cast<int64_t>(c) * kTokens * a.query_strides.token), lds_at + S::kQuery, part,
                      rows_of(c));
     if constexpr (!kTwice) load_pair(c, 1, lds_at + S::kPairsOnce);
   };
-  if (begin < end) {
-    load_stage(end - 1);
-    load_once(end - 1);
-  }
+  if (begin < end) load_once(end - 1);
   const Reader<T> places;
   const Own<T> own(from_panel / 16 + part);
   const Reader<T> fixed = places.moved(lds_at);
@@ -1569,8 +1574,6 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
     else
       wait_older_loads<kSteps>();
     __syncthreads();
-    if constexpr (!kTwice) load_pair(c, 0, lds_at + S::kSolveOnce);
-    load_stage(c - 1);
     const unsigned at = lds_at + S::kStages + (c & 1) * S::kStage;
     const Reader<T> pair_read = kTwice ? places.moved(at) : fixed;
     constexpr unsigned kPairs = kTwice ? S::kPairs : S::kPairsOnce;
@@ -1639,7 +1642,6 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
 #pragma unroll
       for (int m = 0; m < 4; ++m) lds_write(added_at + (m0 + m) * 1024, sum[m].value());
     }
-    if constexpr (!kTwice) wait_older_loads<kStageLoads>();  // T
     __syncthreads();
     load_once(c - 1);
     asm volatile("" ::: "memory");  // the stores stay behind the loads
