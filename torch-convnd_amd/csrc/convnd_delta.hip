@@ -10,8 +10,10 @@
 //   O = diag(c) Q S + P U,  P_ij = G_ij q_i.k_j (i >= j),  S' = c_C S + K^T diag(e) U
 //
 // T and P do not need the state: delta_prepare makes them for all chunks side by side, then
-// delta_forward walks each head's chunks with S in registers. Of a step's few tokens delta_step
-// computes the definition itself.
+// delta_forward walks each head's chunks with S in registers; delta_backward walks back with S's gradient,
+// and delta_gradients makes the rest of all chunks side by side. Of a step's few tokens delta_step
+// computes the definition itself. Of 8 sequences of 2048 tokens and 8 heads of 128 x 128 in bfloat16:
+// prepare 34 us, forward 92, backward 113, gradients 115 (token by token in torch 16 ms).
 //
 // Products run on the matrix cores: in 16 bits on chunks of 64 tokens, in float of 32 (128 bytes a row
 // of T either way, the row of every panel in LDS). Decays' sums are kept in 64 bits and differences of
@@ -22,7 +24,10 @@
 // What is not an input is split into two 16-bit terms before a product (S, U, T, P and what they are
 // made of), which doubles matrix instructions but not LDS reads of the shared operand, by which the
 // walk is bound: the state stays within 1e-5 of the 64-bit one over thousands of tokens (one term:
-// 3e-3) and outputs within their own rounding (1.65e-3 in bfloat16; one term 3.6e-3).
+// 3e-3) and outputs within their own rounding (1.65e-3 in bfloat16; one term 3.6e-3). What is kept for a
+// backward, S and U (and D and Y for the gradients), is one term: a gradient of q, k or a gate that takes two
+// of them is 2.5e-3 to 3.3e-3 off in bfloat16, where its own rounding is 1.65e-3; with the second terms the
+// backward would move a half more.
 
 #include <algorithm>
 #include <atomic>
@@ -458,7 +463,9 @@ __device__ __forceinline__ float decay_between(double later, double earlier) {
   return __builtin_amdgcn_exp2f(static_cast<float>(later - earlier) * 1.44269504088896341f);
 }
 
-// A workgroup takes a chunk of a key head and its value heads one after another; wave w makes rows 16 w
+// Bound by memory and the latency of its short steps, four workgroups a compute unit: 34 us for 2048 chunks of
+// 128-wide heads, 64 KB each (4 TB/s). A workgroup takes a chunk of a key head and its value heads one after
+// another; wave w makes rows 16 w
 // to 16 w + 15. k.k and q.k are in registers for all heads. T: each wave inverts its 16 x 16 block of I
 // + A by substitution, then makes its row of blocks from the right, T_ij = -(sum_k T_ik A_kj) T_jj, on
 // the float matrix instructions, transposed so that a result is the next product's operand and a lane's
@@ -745,7 +752,7 @@ struct Triangle {
       : tile(i < kTiles ? i : i - kTiles + kPer), step(i < kTiles ? 0 : 1) {}
 };
 // Reads of LDS and matrix instructions stay in the order written; arithmetic and stores may move. Left to
-// itself the compiler reads each fragment right before its product (a chunk 8 us, where this takes XX).
+// itself the compiler reads each fragment right before its product (a chunk took 8 us, and with this 4).
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x40); }
 constexpr int kAhead = 10;  // of the 15 that may be under way
 
@@ -782,9 +789,11 @@ struct Walk {
 // and walks through all of them by itself: K S, T R and K^T U take its columns' values as one operand straight
 // from the results before (operand_row puts them in order) and the shared panels as the other, from LDS. The
 // other wave makes the outputs: while the first is at K S and T R it multiplies the S before the chunk, which it
-// is handed through LDS, with Q, and while the first updates S, P with U; it also stores outputs and what is kept
-// for a backward. Waves meet twice a chunk; panels load a chunk or half of one ahead. A walk is bound by the chain
-// from S to the next S (about 2 us a chunk; with the outputs in the same wave 3.9).
+// is handed through LDS, with Q, and while the first updates S, P with U; it also loads, and stores outputs and what
+// is kept for a backward behind the next chunk's loads. Waves meet twice a chunk; panels load a chunk or half of one
+// ahead. With few heads (W = 2) it is bound by the chain from S to the next S: 2.9 us a chunk of 64 tokens, where
+// all in one wave took 3.9. With all compute units at work (W = 4) memory is near: 263 us for 4096 tokens of 256
+// heads that keep S and U, 1.2 GB (4.6 TB/s); all in one wave 338.
 template <typename T, int DK, int W, bool KEEP, bool TRANSIT>
 __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, W / 2))) void delta_forward(DeltaArgs a) {
   using C = Chunk<T>;
@@ -1160,7 +1169,9 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
 // state before it is linear, S' = M S + N: the walk without outputs gives N from a state of zeros and M's columns
 // from those of the unit matrix (and no values), all segments side by side. Here they are put together, one after
 // another in float32 for every state before a segment (REVERSE: from the last one, gradients), from which the
-// walks of all segments then run side by side. A workgroup has 16 columns; a wave a quarter of the rows.
+// walks of all segments then run side by side. A workgroup has 16 columns; a wave a quarter of the rows. 16
+// segments of 8 heads take 49 us, bound by the one's wait for the one before (32768 tokens in all: 0.34 ms, and
+// in a single segment 1.9).
 template <int DK, bool REVERSE>
 __global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
   constexpr int kTiles = DK / 16, kMine = kTiles / 4;
@@ -1246,8 +1257,8 @@ __global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
 //   D' = c_C D + Q^T diag(c rq) dO - K^T diag(beta c rk) Y
 //
 // in the forward walk's form: of two waves with 16 columns one has D in registers, and walks from D to the next D,
-// and the other makes P^T dO and Q^T dO, which do not need it, loads and stores. D and Y of every chunk are kept
-// for delta_gradients.
+// and the other makes P^T dO and Q^T dO, which do not need it, and stores. D and Y of every chunk are kept
+// for delta_gradients. 3.5 us a chunk with few heads (all in one wave 4.4), 271 us where the forward takes 263 (350).
 template <typename T, int DK, int W>
 struct WalkBack {
   using C = Chunk<T>;
@@ -1682,6 +1693,8 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
 // adds up its value heads. Two waves share 16 tokens, which are their lanes throughout: each makes half of the
 // keys' gradients, and one makes the pairs with its token as the row i (registers j), the other those with it
 // as the column j (registers i), so that either is the operand of the next products, which they exchange.
+// 190 KB are read and written for a chunk of 128 x 128 in bfloat16; 2048 of them take 115 us (3.4 TB/s), the rest
+// of the time goes to the steps between barriers that the one workgroup of a compute unit has nothing beside.
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 template <typename T, int DK>
 struct GradientsLds {
@@ -2248,7 +2261,8 @@ __global__ __launch_bounds__(Chunk<T>::kTokens * 8, 2) void delta_gradients(Delt
 
 // The definition, token by token: a workgroup keeps kDeltaStepColumns columns of a head's state, a
 // thread four of them at DK / 16 keys. One pass over the state gives S^T k and S^T q together, since
-// o = a S^T q + (k.q) u; a token costs one barrier. Bound by reading and writing the state.
+// o = a S^T q + (k.q) u; a token costs one barrier. Bound by reading and writing the state: one token of 32
+// sequences with 8 heads of 128 x 128, 34 MB, in 12.6 us (2.7 TB/s, its launch included).
 template <typename T, int DK>
 __global__ __launch_bounds__(256, 4) void delta_step(DeltaArgs a) {
   constexpr int kRows = DK / 16, kQuads = kDeltaStepColumns / 4;
@@ -2403,6 +2417,8 @@ hipError_t launch_prepare(const DeltaArgs& a, hipStream_t stream) {
 
 int64_t value_tiles(const DeltaArgs& a, int columns) { return (a.value_size + columns - 1) / columns; }
 
+// Walks of 32 columns where those of 64 would leave half of the compute units idle (2048 tokens of 64 heads of
+// 128 x 128, forward and backward in one wave each: 124 and 142 us for 143 and 151).
 bool narrow_walk(const DeltaArgs& a) { return a.segments == 1 && a.batch * a.heads * value_tiles(a, 64) <= 128; }
 
 // One walk; TRANSIT: of its segments, with the columns of the unit matrix.
