@@ -238,6 +238,8 @@ def test_plans(lib):
     assert plan(8, 2048, 8, 8, 128, 128)["segments"] == 1
     long = plan(1, 32768, 8, 8, 128, 128)
     assert long["segments"] == 16 and long["segment_chunks"] == 32
+    assert plan(1, 2047, 8, 8, 128, 128)["segments"] == 4 and plan(1, 1984, 8, 8, 128, 128)["segments"] == 1
+    assert plan(1, 4095, 32, 32, 128, 128)["segments"] == 4 and plan(1, 4032, 32, 32, 128, 128)["segments"] == 1
     for tokens in (1000, 1024, 5000, 65536):
         got = plan(1, tokens, 1, 1, 64, 64)
         chunks = (tokens + 63) // 64

@@ -82,6 +82,37 @@ for a, b in zip((*outputs, *got), (*eager, *torch.autograd.grad(eager, leaves, (
 print("compiled")
 """
 
+# Kernels with more LDS than they get unasked, whose first launch is under capture.
+CAPTURED = HEAD + """
+torch_convnd.load_native()
+torch.manual_seed(0)
+q, k, v, dy = (torch.randn(2, 130, 3, 128, device="cuda").bfloat16() for _ in range(4))
+decay, beta = -torch.rand(2, 130, 3, device="cuda"), torch.rand(2, 130, 3, device="cuda")
+x, w = torch.randn(300, 64, device="cuda").bfloat16(), torch.randn(96, 64, device="cuda").bfloat16()
+g = torch.randn(300, 48, device="cuda").bfloat16()
+
+def call():
+    o, last, saved = ops.gated_delta_rule(q, k, v, decay, beta, None, None, 0.1, True, True)
+    grads = ops.gated_delta_rule_backward(dy, None, q, k, v, decay, beta, None, saved, 0.1, True, False)
+    y, kept = ops.gated_linear(x, w, None, "silu", True)
+    more = ops.gated_linear_backward(g, x, w, kept, "silu", [True, True, True])
+    return o, last, *grads[:5], y, *more
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.no_grad():
+    with torch.cuda.graph(graph):
+        captured = call()
+    for seed in (1, 2, 3):
+        for t in (q, k, v, dy, x, g):
+            t.copy_(torch.randn(t.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, call()):
+            assert torch.equal(a, b)
+print("captured")
+"""
+
 
 def test_derivatives_are_traced_before_loading():
     run(TRACED, "traced")
@@ -90,3 +121,8 @@ def test_derivatives_are_traced_before_loading():
 @pytest.mark.gpu
 def test_compiled_as_first_use():
     run(COMPILED, "compiled")
+
+
+@pytest.mark.gpu
+def test_captured_as_first_use():
+    run(CAPTURED, "captured")

@@ -96,6 +96,15 @@ def test_segments(batch, heads, key_size, value_size, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize(("batch", "heads", "key_size", "value_size"), [(1, 1, 128, 130), (3, 2, 40, 20)])
+def test_segments_of_many_tokens(batch, heads, key_size, value_size, dtype):
+    data = make_delta(batch, 2100, 1, heads, key_size, value_size, dtype)
+    data[3][:, 900] = -float("inf")
+    check(data, torch.tensor([2100, 700, 0][:batch]))
+    check(data, state=False, normalize=True)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
 @pytest.mark.parametrize("tokens", [1, 7, 64, 150])

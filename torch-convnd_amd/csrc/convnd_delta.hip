@@ -399,8 +399,6 @@ __device__ __forceinline__ void wait_older_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory");
 }
 
-// A wave's own exchange through LDS: what its lanes wrote is there for the others.
-__device__ __forceinline__ void wait_own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 constexpr int kTurnPitch = 20;  // elements of a row of 16 columns
 
 // Tokens of sequence b that count.
@@ -2077,8 +2075,8 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
         // The other token's factors; this one's are taken out of the sums.
         float p = ratio * (HALF == 0 ? other_rk[e] : other_rq[e]) * pair_p[m][e];
         float n = -ratio * other_rk[e] * pair_a[m][e];
-        p = open & (below | (own == other)) ? p : 0.f;
-        n = open & below ? n : 0.f;
+        p = (open & (below | (own == other))) ? p : 0.f;
+        n = (open & below) ? n : 0.f;
         const float weighed = HALF == 0 ? n : n * other_beta[e];
         pairs = fmaf(p, qk[m][e], pairs);
         steps = fmaf(weighed, kk[m][e], steps);

@@ -355,7 +355,10 @@ int64_t delta_key_pad(const DeltaArgs& a) { return a.key_size <= 64 ? 64 : 128; 
 
 // Segments of the chunks where walks over all of them would leave three quarters of the compute units idle: as
 // many as fill them, of eight chunks at least. A segment is walked twice, once with the unit matrix's columns
-// beside its own.
+// beside its own, and segments are joined one after another, so it takes 32 chunks, and as many as there are walks,
+// to gain: forward and backward of 128 x 128 take 71 and 97 us where one walk takes 76 and 115 (16 walks of 32
+// chunks), 147 and 296 for 154 and 302 (64 of 64), but 128 and 248 for 125 and 242 (64 of 50), 66 and 92 for 60 and
+// 92 (16 of 24).
 DeltaPlan plan_delta(const DeltaArgs& a, bool saving) {
   DeltaPlan p{};
   p.step = !saving && a.tokens <= kDeltaStepTokens;
@@ -367,7 +370,7 @@ DeltaPlan plan_delta(const DeltaArgs& a, bool saving) {
   p.segment_chunks = static_cast<int>(a.chunks);
   if (p.step) return p;
   p.threads = 512;
-  if (walks > 0 && walks <= 64 && a.chunks >= 16) {
+  if (walks > 0 && walks <= 64 && a.chunks >= std::max<int64_t>(32, walks)) {
     const int64_t most = std::min<int64_t>(256 / walks, a.chunks / 8);
     p.segment_chunks = static_cast<int>((a.chunks + most - 1) / most);
     p.segments = static_cast<int>((a.chunks + p.segment_chunks - 1) / p.segment_chunks);
