@@ -1171,8 +1171,8 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
 // segments of 8 heads take 49 us, bound by the one's wait for the one before (32768 tokens in all: 0.34 ms, and
 // in a single segment 1.9).
 template <int DK, bool REVERSE>
-__global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
-  constexpr int kTiles = DK / 16, kMine = kTiles / 4;
+__global__ __launch_bounds__(DK * 4) void delta_join(DeltaArgs a) {
+  constexpr int kTiles = DK / 16, kMine = 1;  // of a wave
   __shared__ f32x4 shared[2][kTiles][64];
   const int l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, at = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -2449,7 +2449,7 @@ hipError_t launch_walk_back(const DeltaArgs& a, hipStream_t stream) {
 template <int DK, bool REVERSE>
 hipError_t launch_join(const DeltaArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((delta_join<DK, REVERSE>), dim3(static_cast<unsigned>(a.batch * a.heads * value_tiles(a, 16))),
-                     dim3(256), 0, stream, a);
+                     dim3(DK * 4), 0, stream, a);
   return hipGetLastError();
 }
 
