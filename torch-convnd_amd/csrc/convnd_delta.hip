@@ -1167,9 +1167,9 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
 // state before it is linear, S' = M S + N: the walk without outputs gives N from a state of zeros and M's columns
 // from those of the unit matrix (and no values), all segments side by side. Here they are put together, one after
 // another in float32 for every state before a segment (REVERSE: from the last one, gradients), from which the
-// walks of all segments then run side by side. A workgroup has 16 columns; a wave a quarter of the rows. 16
-// segments of 8 heads take 49 us, bound by the one's wait for the one before (32768 tokens in all: 0.34 ms, and
-// in a single segment 1.9).
+// walks of all segments then run side by side. A workgroup has 16 columns, a wave 16 rows. 16
+// segments of 8 heads take 39 us, bound by the one's wait for the one before; loads two segments ahead were no
+// faster (45 us). 32768 tokens in all take 0.3 ms, and in a single segment 1.9.
 template <int DK, bool REVERSE>
 __global__ __launch_bounds__(DK * 4) void delta_join(DeltaArgs a) {
   constexpr int kTiles = DK / 16, kMine = 1;  // of a wave
