@@ -329,6 +329,46 @@ __device__ __forceinline__ void split(const f32x4* tiles, typename Chunk<T>::fra
   }
 }
 
+// A power of two that brings values within float16's range before they are split, and its inverse, which goes to
+// the sums of their products; one beside other types, which have float's range. Factors of rows make it needed: a key
+// near zero has 1 / |k| of up to 1000 (of its unit length), so that what its token brings leaves the range where the
+// product with the key is small. With the largest value from 2^14 on, what is 2^-27 of it keeps 11 bits.
+template <typename T>
+struct Power {
+  float up = 1.f, down = 1.f;
+  __device__ __forceinline__ explicit Power(float largest) {
+    if constexpr (std::is_same_v<T, _Float16>) {
+      // Bounded, so that neither leaves float's range beside sums of other values (2^40 of these are none to them).
+      const int exponent = std::max(__builtin_amdgcn_frexp_expf(largest), -40);
+      up = __builtin_bit_cast(float, (127 + 15 - exponent) << 23);
+      down = __builtin_bit_cast(float, (127 - 15 + exponent) << 23);
+    }
+  }
+};
+// The largest size of N result tiles' values (0 beside other types than float16) in this lane's column: over the
+// lanes 16 and 32 apart.
+template <typename T, int N>
+__device__ __forceinline__ float largest_size(const f32x4* tiles, float most = 0.f) {
+  if constexpr (std::is_same_v<T, _Float16>) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(tiles[i][e]));
+  }
+  return most;
+}
+template <typename T>
+__device__ __forceinline__ float over_lane_groups(float most) {
+  if constexpr (std::is_same_v<T, _Float16>) {
+    unsigned v = __builtin_bit_cast(unsigned, most);  // as float: none is negative or NaN
+    const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = std::max<unsigned>(rows[0], rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    most = __builtin_bit_cast(float, std::max<unsigned>(halves[0], halves[1]));
+  }
+  return most;
+}
+
 __device__ __forceinline__ u32x4 buffer_at(const void* p) {
   const uint64_t at = reinterpret_cast<uint64_t>(p);
   u32x4 r;
@@ -989,13 +1029,17 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
       // S = c S + K^T (e rk U).
 #pragma unroll
       for (int m = 0; m < kTiles; ++m) u[m] *= *reinterpret_cast<const f32x4*>(factors + 2 * kTokens + first_row<T>(m, lane.g));
+      const Power<T> power(over_lane_groups<T>(largest_size<T, kTiles>(u)));
+      const float faded = whole * power.up;
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) u[m] *= power.up;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) split<T>(&u[kt * kPer], df[kt]);
 #pragma unroll
       for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
         Sum<T> sum[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) sum[m].whole = state[m0 + m] * whole;
+        for (int m = 0; m < 4; ++m) sum[m].whole = state[m0 + m] * faded;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
@@ -1007,7 +1051,7 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
           keep_order();
         }
 #pragma unroll
-        for (int m = 0; m < 4; ++m) state[m0 + m] = sum[m].value();
+        for (int m = 0; m < 4; ++m) state[m0 + m] = sum[m].value() * power.down;
       }
       hand_state();
     }
@@ -1477,6 +1521,9 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
       }
 #pragma unroll
       for (int m = 0; m < kTiles; ++m) y[m] *= -*reinterpret_cast<const f32x4*>(factors + first_row<T>(m, lane.g));
+      const Power<T> power(over_lane_groups<T>(largest_size<T, kTiles>(y)));
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) y[m] *= power.up;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) split<T>(&y[kt * kPer], yf[kt]);
       // D = c D + Q^T (c rq dO), which is handed, - K^T (beta c rk Y).
@@ -1484,7 +1531,7 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
       for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
         Sum<T> sum[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) sum[m].whole = state[m0 + m] * whole + lds_read<f32x4>(added_at + (m0 + m) * 1024);
+        for (int m = 0; m < 4; ++m) sum[m].whole = (state[m0 + m] * whole + lds_read<f32x4>(added_at + (m0 + m) * 1024)) * power.up;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
@@ -1496,7 +1543,7 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
           keep_order();
         }
 #pragma unroll
-        for (int m = 0; m < 4; ++m) state[m0 + m] = sum[m].value();
+        for (int m = 0; m < 4; ++m) state[m0 + m] = sum[m].value() * power.down;
       }
       hand_state();
     }
@@ -1624,17 +1671,18 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
     for (int m = 0; m < kTiles; ++m) lds_write(to_update + m * 1024 + thread * 16, sums[m].value());
     // Q^T (c rq dO).
     frag gf[2][kTerms];
+    f32x4 v[kTiles];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      f32x4 v[kPer];
+    for (int i = 0; i < kTiles; ++i) {
+      const f32x4 factor = *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + first_row<T>(i, lane.g));
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const f32x4 factor = *reinterpret_cast<const f32x4*>(factors + 3 * kTokens + first_row<T>(kt * kPer + i, lane.g));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = factor[e] * static_cast<float>(g[kt][i * 4 + e]);
-      }
-      split<T>(v, gf[kt]);
+      for (int e = 0; e < 4; ++e) v[i][e] = factor[e] * static_cast<float>(g[i / kPer][i % kPer * 4 + e]);
     }
+    const Power<T> power(over_lane_groups<T>(largest_size<T, kTiles>(v)));
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) v[i] *= power.up;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) split<T>(&v[kt * kPer], gf[kt]);
 #pragma unroll
     for (int m0 = 0; m0 < kStateTiles; m0 += 4) {
       Sum<T> sum[4];
@@ -1649,7 +1697,7 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
         keep_order();
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m) lds_write(added_at + (m0 + m) * 1024, sum[m].value());
+      for (int m = 0; m < 4; ++m) lds_write(added_at + (m0 + m) * 1024, sum[m].value() * power.down);
     }
     __syncthreads();
     load_once(c - 1);
@@ -2092,12 +2140,31 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
     } else {
       dsum -= (pairs + steps) * own_rk;
     }
+    // Of float16, the largest of the pairs with a token, over both waves: behind the record, whose place is larger.
+    float* pair_sizes = reinterpret_cast<float*>(lds.blocks[(index - 1) & 1].record + sizeof(Record<T>));
+    static_assert(!std::is_same_v<T, _Float16> || GradientsLds<T, DK>::kRecord - sizeof(Record<T>) >= 8 * kTokens);
+    const float most = over_lane_groups<T>(largest_size<T, kTiles>(pair_a, largest_size<T, kTiles>(pair_p)));
     if (first == 0) {
       slope[half][own] = dsum;
       step[half][own] = dbeta;
+      if constexpr (std::is_same_v<T, _Float16>) pair_sizes[half * kTokens + own] = most;
     }
     // The pairs as fragments, for both waves of these tokens: three of each kind.
     __syncthreads();  // all have read U, Y and dO
+    float both = 0.f;
+    if constexpr (std::is_same_v<T, _Float16>) both = fmaxf(pair_sizes[own], pair_sizes[kTokens + own]);
+    const Power<T> power(both);
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      if (!has(m)) continue;
+      pair_p[m] *= power.up;
+      pair_a[m] *= power.up;
+    }
+#pragma unroll
+    for (int m = 0; m < kKeyTiles; ++m) {
+      dq[m] *= power.up;
+      dk[m] *= power.up;
+    }
     frag* shared = reinterpret_cast<frag*>(lds.blocks[(index - 1) & 1].narrow[0]) + block * 6 * 64 + thread;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -2148,6 +2215,11 @@ __device__ __forceinline__ void gradients_of(const DeltaArgs& a, GradientsLds<T,
           keep_order();
         }
       }
+    }
+#pragma unroll
+    for (int m = 0; m < kKeyTiles; ++m) {
+      dq[m] *= power.down;
+      dk[m] *= power.down;
     }
     // The next block is there, long since: waited for here, so that no wait is for the stores that follow.
     wait_loads();
