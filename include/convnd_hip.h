@@ -453,8 +453,8 @@ size_t convnd_hip_delta_workspace_size(convnd_hip_dtype dtype, const convnd_hip_
  * `tokens`: tokens at and past a sequence's length (taken as 0 below 0 and as `tokens` above) change no
  * state and give zeros, whatever the inputs hold there. saved: for the backward, or null. A few tokens
  * without `saved` run token by token in float32; else tokens of a chunk are taken together, and a NaN
- * reaches the outputs of its whole chunk. Beside float16 states, and what tokens add to them, have to be
- * within its range. */
+ * reaches the outputs of its whole chunk, an infinity as a NaN. Beside float16 states, and what tokens add to
+ * them, have to be within its range. */
 int convnd_hip_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem, const void* query,
                      const void* key, const void* value, const void* decay, const void* beta,
                      const float* first, const void* lengths, void* output, float* last, void* saved,
@@ -469,7 +469,9 @@ size_t convnd_hip_delta_backward_workspace_size(convnd_hip_dtype dtype,
  * grad_last [batch, heads, key_size, value_size] float32 (null for zeros), all contiguous: grad_query and
  * grad_key [batch, tokens, key_heads, key_size] (sums over the value heads that share them), grad_value,
  * grad_decay and grad_beta [batch, tokens, heads] of `gate_dtype`, and grad_first float32 or null. Zeros past a
- * sequence's length, and for a closed gate's decay. */
+ * sequence's length, and for a closed gate's decay. Beside float16 the states and their gradients are kept in units
+ * of a head's largest value (and first state) and largest cotangent: with all bits from 2^-16 of it, up to 2^13
+ * times it. */
 int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
                               const void* grad_output, const float* grad_last, const void* query,
                               const void* key, const void* value, const void* decay, const void* beta,

@@ -695,6 +695,8 @@ struct DeltaArgs {
   float* transits;            // [batch, heads, segments, padded key size, padded key size], of several segments
   float* partials;            // [batch, heads, segments, padded key size, value_pad]
   float* starts;              // as partials: before each segment (backward: after)
+  float* largest;             // [batch, heads, parts]: of the values (backward: gradients), where what is kept is
+  float* units;               // in units of them (float16), else null; [batch, heads]: the gradients' units
   int64_t batch, tokens, key_heads, heads, key_size, value_size;
   int64_t chunks;             // of `tokens`
   int segments, segment_chunks;
@@ -702,6 +704,7 @@ struct DeltaArgs {
   DeltaStrides query_strides, key_strides, value_strides, decay_strides, beta_strides, grad_strides;
   float scale;
   int groups;                 // value heads a key head
+  int parts;                  // of a head in `largest`, up to 64
   int normalize;
   int float_gates;            // decay and beta are float, else of the element type
   int wide_lengths;           // lengths are int64

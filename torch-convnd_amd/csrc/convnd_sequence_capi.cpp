@@ -311,6 +311,10 @@ DeltaArgs to_args(convnd_hip_dtype dtype, const convnd_hip_delta_problem& p) {
   a.chunks = (p.tokens + chunk - 1) / chunk;
   a.value_pad = (p.value_size + 15) / 16 * 16;
   a.groups = static_cast<int>(p.heads / p.key_heads);
+  // Eight workgroups a compute unit, of a chunk at least.
+  if (dtype == CONVND_HIP_FLOAT16)
+    a.parts = static_cast<int>(
+        std::clamp<int64_t>(2048 / std::max<int64_t>(p.batch * p.heads, 1), 1, std::clamp<int64_t>(a.chunks, 1, 64)));
   a.query_strides = {p.query_batch, p.query_token, p.query_head};
   a.key_strides = {p.key_batch, p.key_token, p.key_head};
   a.value_strides = {p.value_batch, p.value_token, p.value_head};
@@ -398,6 +402,8 @@ DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, bool savin
       a->panels = static_cast<char*>(ws->take(records * delta_panel_bytes(size)));
       a->records = static_cast<char*>(ws->take(records * delta_record_bytes(size)));
     }
+    if (saving && a->parts > 0)
+      a->largest = static_cast<float*>(ws->take(a->batch * a->heads * a->parts * int64_t{sizeof(float)}));
     a->segments = p.segments;
     a->segment_chunks = p.segment_chunks;
     if (p.segments > 1) {
@@ -443,6 +449,7 @@ DeltaLayout lay_out_delta_backward(DeltaArgs* a, int size, const void* grad_outp
   a->grad_strides = l.grad.strides;
   a->grad_states = ws->take(saved_states(*a, size));
   a->grad_updates = ws->take(saved_updates(*a, size));
+  if (a->parts > 0) a->units = static_cast<float*>(ws->take(a->batch * a->heads * int64_t{sizeof(float)}));
   return l;
 }
 

@@ -308,8 +308,9 @@ def gated_delta_rule(
     ``gated_recurrence``. A decay of -inf (below -104, where its exp in float32 is zero) forgets all before
     it: where a packed document starts. The gfx950 kernels take key sizes up to 128. They read slices of
     wider rows in place, keep states in float32 and products within the last bits of the result's dtype, and
-    take more than a few tokens in chunks: there a NaN reaches its whole chunk of 64 tokens, and beside
-    float16 what is added to states has to be within its range.
+    take more than a few tokens in chunks: there a NaN reaches its whole chunk of 64 tokens, an infinity as a
+    NaN, and beside float16 states, and what is added to them, have to be within its range. Their backward keeps
+    states' gradients beside float16 in units of a head's largest cotangent, up to 2^13 times it.
     """
     if is_autocast_enabled(query.device.type):
         dtype = autocast_dtype(query.device.type)
