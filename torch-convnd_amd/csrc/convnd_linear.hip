@@ -516,8 +516,13 @@ __device__ __forceinline__ void finish_gated(const LinearArgs& a, float (&g)[8],
   float d[8];
   if (a.slope != nullptr) {
     activate_all<T, true>(g, d, a.activation);
+    if (a.activation == CONVND_HIP_ACT_RELU) {  // chosen, not multiplied: u may be infinite
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d[e] *= u[e];
+      for (int e = 0; e < 8; ++e) d[e] = d[e] != 0.f ? u[e] : 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] *= u[e];
+    }
     keep_factors<T>(a, d, m * 2 * a.n + n, count);
     keep_factors<T>(a, g, m * 2 * a.n + a.n + n, count);
   } else {
