@@ -444,7 +444,8 @@ typedef struct convnd_hip_delta_problem {
 int64_t convnd_hip_delta_saved(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem);
 
 /* Device scratch bytes of convnd_hip_delta; of the pointers only the alignment is looked at (rows that
- * do not start on 4 bytes or are no whole 16 bytes long are copied). saving: whether `saved` is given. */
+ * do not start on 4 bytes or are no whole 16 bytes long are copied, in whole 16 bytes, at most 2^25 bytes of a
+ * token). saving: whether `saved` is given. */
 size_t convnd_hip_delta_workspace_size(convnd_hip_dtype dtype, const convnd_hip_delta_problem* problem,
                                        const void* query, const void* key, const void* value, int saving);
 

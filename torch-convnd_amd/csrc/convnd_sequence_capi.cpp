@@ -422,6 +422,16 @@ DeltaLayout lay_out_delta(DeltaArgs* a, int size, const DeltaPlan& p, bool savin
   return l;
 }
 
+// A copied row's place in a chunk is a 32-bit byte offset as well: strides of zero let rows be many where their
+// tokens are near.
+int check_copies(const DeltaLayout& l, int size) {
+  for (const DeltaRows* r : {&l.query, &l.key, &l.value, &l.grad})
+    if (r->copied && r->copy.heads > (int64_t{1} << 25) / (r->copy.pitch * size))
+      return fail(CONVND_HIP_INVALID_ARGUMENT,
+                  "gated_delta_rule rows that are no whole 16 bytes, or do not start on 4, need at most 2^25 bytes a token");
+  return CONVND_HIP_SUCCESS;
+}
+
 // What a forward keeps: states, updates, and the chunks' panels and records. In bytes, whole 16 each.
 int64_t saved_states(const DeltaArgs& a, int size) {
   return a.batch * a.heads * a.chunks * a.value_pad * delta_key_pad(a) * size;
@@ -851,7 +861,8 @@ int convnd_hip_delta(convnd_hip_dtype dtype, const convnd_hip_delta_problem* pro
   const DeltaLayout l = lay_out_delta(&a, size, p, saved != nullptr, query, key, value, &ws);
   if (!launch_fits(p.workgroups, p.threads))
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes are too large: more than 2^32 threads");
-  st = check_parts(ws, workspace_size, "gated_delta_rule");
+  st = check_copies(l, size);
+  if (st == CONVND_HIP_SUCCESS) st = check_parts(ws, workspace_size, "gated_delta_rule");
   if (st != CONVND_HIP_SUCCESS) return st;
   a.decay = decay;
   a.beta = beta;
@@ -903,7 +914,8 @@ int convnd_hip_delta_backward(convnd_hip_dtype dtype, const convnd_hip_delta_pro
   const DeltaPlan p = plan_delta(a, true);
   if (!launch_fits(p.workgroups, p.threads))
     return fail(CONVND_HIP_INVALID_ARGUMENT, "gated_delta_rule sizes are too large: more than 2^32 threads");
-  st = check_parts(ws, workspace_size, "gated_delta_rule backward");
+  st = check_copies(l, size);
+  if (st == CONVND_HIP_SUCCESS) st = check_parts(ws, workspace_size, "gated_delta_rule backward");
   if (st != CONVND_HIP_SUCCESS) return st;
   a.decay = decay;
   a.beta = beta;
