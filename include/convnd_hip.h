@@ -422,7 +422,8 @@ int convnd_hip_recurrence_plan_describe(convnd_hip_dtype dtype,
  * key_heads, key_size], value [batch, tokens, heads, value_size], each by its strides with a contiguous
  * last axis; heads is a multiple of key_heads, and value heads h key_group .. h key_group + key_group - 1
  * share key head h. decay and beta [batch, tokens, heads] are of `gate_dtype`, the element type or float32.
- * A decay below -104, -inf among them, closes the gate (a = 0, as its exp in float32). */
+ * A decay below -104, -inf among them, closes the gate (a = 0, as its exp in float32; 0 times a state that is not
+ * finite is NaN). */
 typedef struct convnd_hip_delta_problem {
   int64_t batch, tokens, key_heads, heads;
   int64_t key_size, value_size; /* 1 to 128; 1 to 65535 */

@@ -28,11 +28,10 @@
 // backward, S and U (and D and Y for the gradients), is one term: a gradient of q, k or a gate that takes two
 // of them is 2.5e-3 to 3.3e-3 off in bfloat16, where its own rounding is 1.65e-3; with the second terms the
 // backward would move a half more. Of float16 that term is in units of the head's largest value or cotangent, and
-// the backward's walk in those of the latter throughout (training 8 x 2048 tokens of 8 heads of 128 x 128: 24 us of
-// 395 to find them, 4 to 7 in the walk).
+// the backward's walk in those of the latter throughout (training 8 x 2048 tokens of 8 heads of 128 x 128: 23 us of
+// 405 to find them, 4 in the walk).
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "convnd_internal.h"
@@ -872,7 +871,7 @@ struct Walk {
 // is handed through LDS, with Q, and while the first updates S, P with U; it also loads, and stores outputs and what
 // is kept for a backward behind the next chunk's loads. Waves meet twice a chunk; panels load a chunk or half of one
 // ahead. With few heads (W = 2) it is bound by the chain from S to the next S: 2.9 us a chunk of 64 tokens, where
-// all in one wave took 3.9. With all compute units at work (W = 4) memory is near: 263 us for 4096 tokens of 256
+// all in one wave took 3.9. With all compute units at work (W = 4) memory is near: 263 us for 4096 tokens of 128
 // heads that keep S and U, 1.2 GB (4.6 TB/s); all in one wave 338.
 template <typename T, int DK, int W, bool KEEP, bool TRANSIT>
 __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, W / 2))) void delta_forward(DeltaArgs a) {
@@ -1255,14 +1254,14 @@ __global__ __launch_bounds__(128 * W) __attribute__((amdgpu_waves_per_eu(W / 2, 
 // from those of the unit matrix (and no values), all segments side by side. Here they are put together, one after
 // another in float32 for every state before a segment (REVERSE: from the last one, gradients), from which the
 // walks of all segments then run side by side. A workgroup has 16 columns, a wave 16 rows. 16
-// segments of 8 heads take 39 us, bound by the one's wait for the one before; loads two segments ahead were no
-// faster (45 us). 32768 tokens in all take 0.3 ms, and in a single segment 1.9.
+// segments of 8 heads take 39 us, bound by the one's wait for the one before (with 32 rows a wave 45, and with loads
+// two segments ahead of that 45 to 49). 32768 tokens in all take 0.3 ms, and in a single segment 1.9.
 template <int DK, bool REVERSE>
 __global__ __launch_bounds__(DK * 4) void delta_join(DeltaArgs a) {
-  constexpr int kTiles = DK / 16, kMine = 1;  // of a wave
+  constexpr int kTiles = DK / 16;
   __shared__ f32x4 shared[2][kTiles][64];
   const int l = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, at = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = wave * 16;
   const unsigned heads = static_cast<unsigned>(a.batch * a.heads), tile = blockIdx.x / heads;
   const int64_t bh = blockIdx.x - tile * heads;
   const int mine = static_cast<int>(tile) * 16 + l;
@@ -1270,69 +1269,45 @@ __global__ __launch_bounds__(DK * 4) void delta_join(DeltaArgs a) {
   const float* from = REVERSE ? a.grad_last : a.first;
   float* to = REVERSE ? a.grad_first : a.last;
   const float unit = REVERSE && a.largest != nullptr ? unit_of(a, bh) : 1.f;  // of gradients
-  f32x4 state[kMine];
+  f32x4 state;
 #pragma unroll
-  for (int i = 0; i < kMine; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = (wave * kMine + i) * 16 + g * 4 + e;
-      state[i][e] = from != nullptr && d < key_size && mine < value_size
-                        ? from[(bh * key_size + d) * value_size + mine] * unit
-                        : 0.f;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const int d = first + g * 4 + e;
+    state[e] = from != nullptr && d < key_size && mine < value_size ? from[(bh * key_size + d) * value_size + mine] * unit
+                                                                    : 0.f;
+  }
   // A segment's rows of M and its N, a segment ahead.
-  f32x4 rows[kMine][kTiles], next[kMine];
+  f32x4 rows[kTiles], next;
   const auto load = [&](int s) __attribute__((always_inline)) {
     const int64_t segment = bh * a.segments + s;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int first = (wave * kMine + i) * 16;
+    for (int t = 0; t < kTiles; ++t)
+      rows[t] = *reinterpret_cast<const f32x4*>(a.transits + (segment * DK + first + l) * DK + t * 16 + g * 4);
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-        rows[i][t] = *reinterpret_cast<const f32x4*>(a.transits + (segment * DK + first + l) * DK + t * 16 + g * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        next[i][e] = a.partials[(segment * DK + first + g * 4 + e) * a.value_pad + mine];
-    }
+    for (int e = 0; e < 4; ++e) next[e] = a.partials[(segment * DK + first + g * 4 + e) * a.value_pad + mine];
   };
   load(REVERSE ? a.segments - 1 : 0);
 #pragma unroll 1
   for (int i = 0; i < a.segments; ++i) {
     const int s = REVERSE ? a.segments - 1 - i : i;
     const int64_t segment = bh * a.segments + s;
+    shared[i & 1][wave][at] = state;
 #pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      shared[i & 1][wave * kMine + k][at] = state[k];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        a.starts[(segment * DK + (wave * kMine + k) * 16 + g * 4 + e) * a.value_pad + mine] = state[k][e];
-    }
+    for (int e = 0; e < 4; ++e) a.starts[(segment * DK + first + g * 4 + e) * a.value_pad + mine] = state[e];
     __syncthreads();
     // A result's registers at a lane are an operand's of the same tile: rows 4 g to 4 g + 3 of a column.
-    f32x4 part[kMine][2];
+    f32x4 part[2] = {next, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      part[k][0] = next[k];
-      part[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const f32x4 column = shared[i & 1][t][at];
-#pragma unroll
-      for (int k = 0; k < kMine; ++k) part[k][t & 1] = Fragment<float>::mma(rows[k][t], column, part[k][t & 1]);
-    }
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) state[k] = part[k][0] + part[k][1];
+    for (int t = 0; t < kTiles; ++t) part[t & 1] = Fragment<float>::mma(rows[t], shared[i & 1][t][at], part[t & 1]);
+    state = part[0] + part[1];
     if (i + 1 < a.segments) load(REVERSE ? s - 1 : s + 1);
   }
   if (to == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < kMine; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = (wave * kMine + i) * 16 + g * 4 + e;
-      if (d < key_size && mine < value_size) to[(bh * key_size + d) * value_size + mine] = state[i][e] / unit;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const int d = first + g * 4 + e;
+    if (d < key_size && mine < value_size) to[(bh * key_size + d) * value_size + mine] = state[e] / unit;
+  }
 }
 
 // ---- the walk back ----------------------------------------------------------------------------------------
@@ -2573,21 +2548,6 @@ __global__ __launch_bounds__(256) void delta_copy(DeltaCopy c) {
   }
 }
 
-// More than 64 KB of LDS has to be asked for, once per device and kernel (`asked` is the kernel's).
-template <typename Kernel>
-hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
-  if (bytes <= 65536) return hipSuccess;
-  int device = 0;
-  hipError_t err = hipGetDevice(&device);
-  if (err != hipSuccess) return err;
-  const uint64_t bit = uint64_t{1} << (device & 63);
-  if ((asked.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
-  err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
-  return err;
-}
-
 template <typename T, bool GRADIENT>
 hipError_t launch_largest(const DeltaArgs& a, hipStream_t stream) {
   if (a.largest == nullptr) return hipSuccess;
@@ -2605,8 +2565,10 @@ hipError_t launch_prepare(const DeltaArgs& a, hipStream_t stream) {
 
 int64_t value_tiles(const DeltaArgs& a, int columns) { return (a.value_size + columns - 1) / columns; }
 
-// Walks of 32 columns where those of 64 would leave half of the compute units idle (2048 tokens of 64 heads of
-// 128 x 128, forward and backward in one wave each: 124 and 142 us for 143 and 151).
+// Walks of 32 columns where those of 64 would leave half of the compute units idle: 2048 tokens of 48 and 64 heads
+// of 128 x 128 (96 and 128 walks of 64 columns) take 83 and 89 us forward and 106 and 108 back where 64 columns take
+// 109 and 112, 113 and 120. From 129 on two of 32 would share a compute unit's time: 72 heads 160 and 195 us for 122
+// and 122.
 bool narrow_walk(const DeltaArgs& a) { return a.segments == 1 && a.batch * a.heads * value_tiles(a, 64) <= 128; }
 
 // One walk; TRANSIT: of its segments, with the columns of the unit matrix.

@@ -26,7 +26,6 @@
 // are first copied to the workspace with padding.
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "convnd_internal.h"
@@ -1170,21 +1169,6 @@ __global__ __launch_bounds__(256) void gated_grad(LinearGradArgs a) {
       a.partial[blockIdx.y * both + half * a.columns + column] = s;
     }
   }
-}
-
-// More than 64 KB of LDS has to be asked for, once per device and kernel (`asked` is the kernel's).
-template <typename Kernel>
-hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
-  if (bytes <= 65536) return hipSuccess;
-  int device = 0;
-  hipError_t err = hipGetDevice(&device);
-  if (err != hipSuccess) return err;
-  const uint64_t bit = uint64_t{1} << (device & 63);
-  if ((asked.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
-  err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
-  return err;
 }
 
 template <int MB, int NB, int WM, int WN>

@@ -1,10 +1,11 @@
 // Shared by the sequence kernels (layer norm, linear, gated recurrence, delta rule): vector accesses of
-// any alignment, reductions over the lanes of a wave, fragments of the matrix instructions and loads
-// from memory straight into LDS.
+// any alignment, reductions over the lanes of a wave, fragments of the matrix instructions, loads
+// from memory straight into LDS, and LDS of more than 64 KB.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "convnd_types.h"
@@ -90,5 +91,20 @@ __device__ __forceinline__ void load_lds4(u32x4 rows, unsigned dst, unsigned off
                : "m0");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// More than 64 KB of LDS has to be asked for, once per device and kernel (`asked` is the kernel's).
+template <typename Kernel>
+inline hipError_t ask_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+  if (bytes <= 65536) return hipSuccess;
+  int device = 0;
+  hipError_t err = hipGetDevice(&device);
+  if (err != hipSuccess) return err;
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if ((asked.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
+  err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return err;
+}
 
 }  // namespace convnd

@@ -306,7 +306,7 @@ def gated_delta_rule(
     ``initial_state`` and ``last_state`` are float32 [batch, heads, key_size, value_size] (zeros if None), so
     that a prompt's last state starts the next call, of one token when decoding. ``lengths`` as for
     ``gated_recurrence``. A decay of -inf (below -104, where its exp in float32 is zero) forgets all before
-    it: where a packed document starts. The gfx950 kernels take key sizes up to 128. They read slices of
+    it (that is finite): where a packed document starts. The gfx950 kernels take key sizes up to 128. They read slices of
     wider rows in place, keep states in float32 and products within the last bits of the result's dtype, and
     take more than a few tokens in chunks: there a NaN reaches its whole chunk of 64 tokens, an infinity as a
     NaN, and beside float16 states, and what is added to them, have to be within its range. Their backward keeps
