@@ -122,3 +122,12 @@ def test_a_replayed_graph_finds_its_own_units():
         torch.cuda.synchronize()
         for a, b in zip(captured, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize(("batch", "tokens"), [(0, 5), (2, 0)])
+def test_empty(batch, tokens):
+    *inputs, first, dy, dlast = (t.cuda() for t in make_delta(batch, tokens, 1, 2, 16, 16, torch.float16))
+    got = train(inputs, first, dy, dlast)
+    assert torch.equal(got[1], first) and torch.equal(got[7], dlast)
+    for grad, t in zip(got[2:7], inputs):
+        assert grad.shape == t.shape

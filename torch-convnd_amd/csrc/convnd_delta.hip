@@ -330,26 +330,28 @@ __device__ __forceinline__ void split(const f32x4* tiles, typename Chunk<T>::fra
   }
 }
 
+// Types whose range is less than that of their sums: their operands are scaled.
+template <typename T>
+constexpr bool kUnits = std::is_same_v<T, _Float16>;
+
 // A power of two that brings values within float16's range before they are split, and its inverse, which goes to
 // the sums of their products; one beside other types, which have float's range. Factors of rows make it needed: a key
 // near zero has 1 / |k| of up to 1000 (of its unit length), so that what its token brings leaves the range where the
 // product with the key is small. With the largest value from 2^14 on, what is 2^-27 of it keeps 11 bits.
 template <typename T>
-constexpr bool kUnits = std::is_same_v<T, _Float16>;
-template <typename T>
 struct Power {
   float up = 1.f, down = 1.f;
   __device__ __forceinline__ explicit Power(float largest) {
     if constexpr (kUnits<T>) {
-      // Bounded, so that neither leaves float's range beside sums of other values (2^40 of these are none to them).
+      // Bounded, so that states that are multiplied by it too, as they join the sums, stay within float's range.
       const int exponent = std::max(__builtin_amdgcn_frexp_expf(largest), -40);
       up = __builtin_bit_cast(float, (127 + 15 - exponent) << 23);
       down = __builtin_bit_cast(float, (127 - 15 + exponent) << 23);
     }
   }
 };
-// The largest size of N result tiles' values (0 beside other types than float16) in this lane's column: over the
-// lanes 16 and 32 apart.
+// The largest size of N result tiles' values in this lane, and that over a column's lanes, 16 and 32 apart (not looked
+// for beside other types).
 template <typename T, int N>
 __device__ __forceinline__ float largest_size(const f32x4* tiles, float most = 0.f) {
   if constexpr (kUnits<T>) {
